@@ -218,7 +218,7 @@ def _run_own(s):
     if kind == "step":
         step = paged.page_step(s["lens"], s["new"], s["tables"], s["free"], s["head"], page_size=s["page"], n_rows=s["rows"])
         return {"lens": step.lens, "head": step.head, "starts": step.starts, "slots": step.slots, "positions": step.positions,
-                "requests": step.requests, "counts": step.counts, "tables": s["tables"], "free": s["free"]}
+                "visible": step.visible, "requests": step.requests, "counts": step.counts, "tables": s["tables"], "free": s["free"]}
     if kind == "attend":
         if s["case"]["cache"] == "rows":
             return paged.sdpa_decode_paged(s["q"], s["keys"], s["values"], s["tables"], s["lens"], s["scale"])
@@ -272,7 +272,8 @@ def _step(s):
     counts = torch.stack([starts[-1], (add - (length - lens) * ~ended).sum(), got.sum(), back.sum()])
     head = base + got.sum()
     return {"lens": length.int(), "head": head.int(), "starts": starts.int(), "slots": torch.where(fits, place, -1).int(),
-            "positions": torch.where(live, position, 0).int(), "requests": torch.where(live, request, -1).int(),
+            "positions": torch.where(live, position, 0).int(),
+            "visible": torch.where(fits, position + 1, 0).int(), "requests": torch.where(live, request, -1).int(),
             "counts": counts.int(), "tables": s["tables"], "free": s["free"]}
 
 
@@ -384,7 +385,7 @@ def work(case):
         rows = sum(max(k, 0) for k in new) + case["spare"]
         taken = sum(_pages(n + k, case["page"]) - _pages(n, case["page"]) for n, k in zip(lens, new) if k > 0)
         back = sum(_pages(n, case["page"]) for n, k in zip(lens, new) if k < 0)
-        return {"bytes": 16 * len(lens) + 12 * rows + 8 * (taken + back), "flops": 0}
+        return {"bytes": 16 * len(lens) + 16 * rows + 8 * (taken + back), "flops": 0}
     size, H, G = SIZE[case["dtype"]], case["heads"], case["kv_heads"]
     row = DIM + DIM // GROUP * 2 * size if case.get("cache") == "q8" else DIM * 2
     if case["kind"] == "attend":
