@@ -337,6 +337,80 @@ int mspr_sdpa_fa_prefill_q8(const void* queries, const void* pk_wq, const void* 
                             int q_len, int64_t past_len, int64_t past_rows, float scale, int group_size,
                             int bits, void* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------ Qwen/Ornith layers over a paged cache
+ *
+ * Extension: the reference serves one sequence a cache (mlx_lm's caches, runtime/qwen/full_attention.py:315). Here the rows of
+ * many requests lie in pages of one pool, [n_pages][n_kv_heads][page_size][256] a side, and a table per request names its
+ * pages. page_size is a power of two from 16 on; slot = page * page_size + row in the page; head_dim 256. */
+
+/* Tables of one step. batch <= 2048 requests of lens rows get new_lens rows each (request by request in one ragged batch of
+ * n_rows), a negative new_lens ends the request and gives its pages back. free_pages: int32 [n_pages], a stack with room for
+ * every page of the pool whose entries from *head on are free. Pages given back go on the stack first (in the order of the
+ * requests), then every request takes those that its new rows begin, as far as there are any.
+ * tables int32 [batch][table_width] and free_pages are updated in place; lens_out int32 [batch] (0 of an ended request),
+ * head_out int32 [1], starts int32 [batch + 1] (first row of every request and the end), per row of n_rows: slots (-1: no page
+ * was left, the table is full, or the row belongs to no request), positions, visible (the rows of its request up to itself, 0
+ * without a slot) and requests (-1 behind the last), counts int32 [4]: rows asked for, of them without a slot, pages taken,
+ * pages given back. A row without a slot is not in lens_out. Rows
+ * asked for behind n_rows are not part of the step. A call on the same lens and head again writes the same. */
+int mspr_page_step(const int32_t* lens, const int32_t* new_lens, int32_t* tables, int32_t* free_pages, const int32_t* head,
+                   int batch, int table_width, int n_pages, int page_size, int n_rows, int32_t* lens_out, int32_t* head_out,
+                   int32_t* starts, int32_t* slots, int32_t* positions, int32_t* visible, int32_t* requests, int32_t* counts,
+                   void* stream);
+
+/* RMS norm of every query and key head (weights of dtype [256]) and rotary position of its first rotary_dim channels (halves
+ * i and i + rotary_dim/2 rotate together, angle = position * inv_freq[i], float32 [rotary_dim/2]) in one pass, rounded once.
+ * The sequence q_norm / k_norm / rope of runtime/qwen/full_attention.py:278-315 (modules of the model there).
+ * q: [n_tokens][n_q_heads][256] of dtype (f32|f16|bf16) at the strides given (elements; rows 16-byte aligned), k likewise with
+ * n_kv_heads; positions: int32 [axes][n_tokens], axes 1 or 3 (time, height, width: frequency i takes axis i % 3 while
+ * i < 3 * height_freqs or 3 * width_freqs, else time); rotary_dim: a multiple of 16 up to 256.
+ * q_out, k_out: dense [n_tokens][heads][256] of dtype. */
+int mspr_qk_norm_rope(const void* q, const void* k, const void* q_weight, const void* k_weight, int dtype, int n_tokens,
+                      int n_q_heads, int n_kv_heads, int head_dim, int64_t q_token_stride, int64_t q_head_stride,
+                      int64_t k_token_stride, int64_t k_head_stride, const int32_t* positions, int axes, int height_freqs,
+                      int width_freqs, const float* inv_freq, int rotary_dim, float eps, void* q_out, void* k_out,
+                      void* stream);
+
+/* The same with the append: keys and values go to their slots (int32 [n_tokens]; rows whose slot is negative or not in the
+ * pool are left out) in pages of 16-bit rows (page_dtype: that of the rows, either 16-bit type for float32 rows) or of affine
+ * 8-bit rows (codes uint32 [..][64], scales and biases [..][4] of dtype; the bytes that mspr_affine_q8_quantize makes of the
+ * rows as mspr_qk_norm_rope rounds them). Two rows of one call must not share a slot. strides: HOST array of six element
+ * strides (token and head of q, k and v). */
+int mspr_qk_norm_rope_append(const void* q, const void* k, const void* v, const void* q_weight, const void* k_weight, int dtype,
+                             int n_tokens, int n_q_heads, int n_kv_heads, int head_dim, const int64_t* strides,
+                             const int32_t* positions, int axes, int height_freqs, int width_freqs, const float* inv_freq,
+                             int rotary_dim, float eps, const int32_t* slots, int n_pages, int page_size, int page_dtype,
+                             void* k_pages, void* v_pages, void* q_out, void* stream);
+int mspr_qk_norm_rope_append_q8(const void* q, const void* k, const void* v, const void* q_weight, const void* k_weight,
+                                int dtype, int n_tokens, int n_q_heads, int n_kv_heads, int head_dim, const int64_t* strides,
+                                const int32_t* positions, int axes, int height_freqs, int width_freqs, const float* inv_freq,
+                                int rotary_dim, float eps, const int32_t* slots, int n_pages, int page_size, void* k_wq,
+                                void* k_scales, void* k_biases, void* v_wq, void* v_scales, void* v_biases, void* q_out,
+                                void* stream);
+
+/* Scratch bytes of the two decode entry points below. */
+size_t mspr_sdpa_decode_paged_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int page_size, int table_width);
+
+/* One new token a request over its pages: out[b] = softmax(q[b] . K^T * scale) V over the first lens[b] rows (at most
+ * table_width * page_size) that the query's table names, 0 where there are none. The table is tables[requests[b]] of n_tables
+ * (none for a request that is not among them), or tables[b] where requests is NULL and n_tables = batch; several queries may
+ * name one request (new rows of a chunk, each with the rows that it sees). Lengths, requests and tables are read on the
+ * device, so that a captured call follows them. Entries behind a request's rows may hold anything, as may the rows behind them in a page;
+ * rows of a page that is not in the pool are left out.
+ * queries, out: [batch][n_q_heads][256] of dtype (f16|bf16), pages of the same; n_q_heads / n_kv_heads <= 16. */
+int mspr_sdpa_decode_paged(const void* queries, const void* k_pages, const void* v_pages, int dtype, const int32_t* tables,
+                           const int32_t* lens, const int32_t* requests, int batch, int n_q_heads, int n_kv_heads,
+                           int head_dim, int n_pages, int page_size, int n_tables, int table_width, float scale, void* out,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same over pages of affine 8-bit rows (scales and biases of sb_dtype); queries and out of q_dtype (f32|f16|bf16). */
+int mspr_sdpa_decode_paged_q8(const void* queries, int q_dtype, const void* k_wq, const void* k_scales, const void* k_biases,
+                              const void* v_wq, const void* v_scales, const void* v_biases, int sb_dtype,
+                              const int32_t* tables, const int32_t* lens, const int32_t* requests, int batch,
+                              int n_q_heads, int n_kv_heads, int head_dim, int n_pages, int page_size, int n_tables,
+                              int table_width, float scale, int group_size, int bits, void* out, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ measurement */
 
 /* Per-kernel GPU timing for benchmarks. Bit k of kernel_mask brackets every later launch of kernel

@@ -130,6 +130,28 @@ SIGNATURES = {
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
                 c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_int64, c_float, c_int, c_int, c_void_p, c_void_p,
                 c_size_t, c_void_p]),
+    "mspr_page_step": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
+                c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "mspr_qk_norm_rope": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64,
+                c_int64, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_float, c_void_p, c_void_p, c_void_p]),
+    "mspr_qk_norm_rope_append": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
+                c_int, c_int, c_int, c_void_p, c_int, c_float, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                c_void_p]),
+    "mspr_qk_norm_rope_append_q8": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
+                c_int, c_int, c_int, c_void_p, c_int, c_float, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "mspr_sdpa_decode_paged_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "mspr_sdpa_decode_paged": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
+                c_int, c_int, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mspr_sdpa_decode_paged_q8": (
+        c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p,
+                c_size_t, c_void_p]),
     "mspr_profile_enable": (c_int, [c_int]),
     "mspr_profile_collect": (c_int, [c_int, c_void_p, c_int]),
 }
@@ -172,6 +194,14 @@ def prefill_attention_workspace(q_dtype, batch: int, n_heads: int, n_tokens: int
 def q8_decode_workspace(batch: int, n_kv_heads: int, n_keys: int, device) -> torch.Tensor:
     """Scratch tensor for the Q8 decode entry points (per-range partials)."""
     nbytes = int(lib().mspr_sdpa_decode_q8_workspace_bytes(int(batch), int(n_kv_heads), int(n_keys)))
+    return torch.empty((max(nbytes, 16) + 3) // 4, dtype=torch.float32, device=device)
+
+
+def paged_decode_workspace(batch: int, n_q_heads: int, n_kv_heads: int, page_size: int, table_width: int,
+                           device) -> torch.Tensor:
+    """Scratch tensor for the paged decode entry points (per-range partials, the plan of the ranges)."""
+    nbytes = int(lib().mspr_sdpa_decode_paged_workspace_bytes(int(batch), int(n_q_heads), int(n_kv_heads), int(page_size),
+                                                              int(table_width)))
     return torch.empty((max(nbytes, 16) + 3) // 4, dtype=torch.float32, device=device)
 
 

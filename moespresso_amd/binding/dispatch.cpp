@@ -638,6 +638,264 @@ PyObject* sdpa_fa_prefill_q8(PyObject* const* a, Py_ssize_t nargs) {
   return failed(rc, "sdpa_fa_prefill_q8") ? nullptr : wrap(out);
 }
 
+// ---------------------------------------------------------------------------------------------- paged cache
+
+bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
+
+bool page_size_ok(int64_t n) { return n >= 16 && n <= INT32_MAX && (n & (n - 1)) == 0; }
+
+// (lens, new_lens int32 [B], tables int32 [B, P], free_pages int32 [n], head int32 [1], page_size, n_rows) -> the eight parts of a step
+PyObject* page_step(PyObject* const* a, Py_ssize_t nargs) {
+  MSPR_NARGS(7)
+  const Tensor *lens = dense(a[0], 1, at::kInt), *add = dense(a[1], 1, at::kInt), *tables = dense(a[2], 2, at::kInt),
+               *pages = dense(a[3], 1, at::kInt), *head = dense(a[4], 1, at::kInt);
+  int page_size, n_rows;
+  if (!lens || !add || !tables || !pages || !head || !whole32(a[5], &page_size) || !whole32(a[6], &n_rows) ||
+      !here({lens, add, tables, pages, head}))
+    return none();
+  const int64_t B = lens->size(0), P = tables->size(1), N = pages->size(0);
+  if (B < 1 || B > 2048 || add->size(0) != B || tables->size(0) != B || P < 1 || P > INT32_MAX || N < 1 || N > INT32_MAX ||
+      head->size(0) != 1 || n_rows < 0 || !page_size_ok(page_size))
+    return none();
+  Tensor out[8];
+  const int64_t sizes[8] = {B, 1, B + 1, n_rows, n_rows, n_rows, n_rows, 4};
+  for (int i = 0; i < 8; i++) out[i] = empty({sizes[i]}, at::kInt, *lens);
+  int32_t* o[8];
+  for (int i = 0; i < 8; i++) o[i] = (int32_t*)out[i].data_ptr();
+  const int rc = launch([&](void* st) {
+    return mspr_page_step((const int32_t*)lens->const_data_ptr(), (const int32_t*)add->const_data_ptr(),
+                          (int32_t*)tables->data_ptr(), (int32_t*)pages->data_ptr(), (const int32_t*)head->const_data_ptr(),
+                          (int)B, (int)P, (int)N, page_size, n_rows, o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7], st);
+  });
+  if (failed(rc, "page_step")) return nullptr;
+  return wrap_tuple(out[0], out[1], out[2], out[3], out[4], out[5], out[6], out[7]);
+}
+
+// Rows [T, heads, 256] at any token and head stride that keeps them 16-byte aligned.
+const Tensor* head_rows(PyObject* o) {
+  if (!THPVariable_Check(o)) return nullptr;
+  const Tensor& t = THPVariable_Unpack(o);
+  if (!t.defined() || !t.is_cuda() || t.dim() != 3 || t.size(2) != 256 || t.stride(2) != 1 || type_code(t.scalar_type()) == kNoType)
+    return nullptr;
+  const int64_t unit = 16 / t.element_size();
+  return t.stride(0) % unit == 0 && t.stride(1) % unit == 0 && t.size(0) >= 1 && t.size(0) <= (1 << 24) && t.size(1) >= 1 &&
+                 t.size(1) <= 1024 && aligned16(t)
+             ? &t
+             : nullptr;
+}
+
+// What the two forms of norm and rope share: q, k, q_weight, k_weight, positions, inv_freq, eps, sections.
+struct Rope {
+  const Tensor *q, *k, *qw, *kw, *pos, *inv;
+  float eps;
+  int axes = 1, height = 0, width = 0, code;
+};
+
+bool rope_operands(PyObject* const* qk, PyObject* const* rest, PyObject* eps, PyObject* sections, Rope* r) {
+  r->q = head_rows(qk[0]);
+  r->k = head_rows(qk[1]);
+  r->qw = dense(rest[0], 1);
+  r->kw = dense(rest[1], 1);
+  r->inv = dense(rest[3], 1, at::kFloat);
+  r->pos = dense(rest[2], sections == Py_None ? 1 : 2, at::kInt);
+  if (!r->q || !r->k || !r->qw || !r->kw || !r->inv || !r->pos || !real(eps, &r->eps)) return false;
+  const at::ScalarType type = r->q->scalar_type();
+  const int64_t T = r->q->size(0), half = r->inv->size(0);
+  r->code = type_code(type);
+  if (r->k->scalar_type() != type || r->k->size(0) != T || r->qw->scalar_type() != type || r->kw->scalar_type() != type ||
+      r->qw->size(0) != 256 || r->kw->size(0) != 256 || !aligned16(*r->qw) || !aligned16(*r->kw) || half < 8 || half > 128 ||
+      half % 8 != 0)
+    return false;
+  if (sections == Py_None) {
+    if (r->pos->size(0) != T) return false;
+  } else {
+    int time;
+    if (!PyTuple_CheckExact(sections) || PyTuple_GET_SIZE(sections) != 3 || !whole32(PyTuple_GET_ITEM(sections, 0), &time) ||
+        !whole32(PyTuple_GET_ITEM(sections, 1), &r->height) || !whole32(PyTuple_GET_ITEM(sections, 2), &r->width))
+      return false;
+    if (time < 0 || r->height < 0 || r->width < 0 || (int64_t)time + r->height + r->width != half ||
+        3 * (int64_t)r->height > half + 1 || 3 * (int64_t)r->width > half || r->pos->size(0) != 3 || r->pos->size(1) != T)
+      return false;
+    r->axes = 3;
+  }
+  return here({r->q, r->k, r->qw, r->kw, r->pos, r->inv});
+}
+
+// (q, k, q_weight, k_weight, positions, inv_freq, eps, sections) -> (q, k) dense
+PyObject* qk_norm_rope(PyObject* const* a, Py_ssize_t nargs) {
+  MSPR_NARGS(8)
+  Rope r;
+  if (!rope_operands(a, a + 2, a[6], a[7], &r)) return none();
+  Tensor q = empty(r.q->sizes(), r.q->scalar_type(), *r.q), k = empty(r.k->sizes(), r.k->scalar_type(), *r.k);
+  const int rc = launch([&](void* st) {
+    return mspr_qk_norm_rope(r.q->const_data_ptr(), r.k->const_data_ptr(), r.qw->const_data_ptr(), r.kw->const_data_ptr(), r.code,
+                             (int)r.q->size(0), (int)r.q->size(1), (int)r.k->size(1), 256, r.q->stride(0), r.q->stride(1),
+                             r.k->stride(0), r.k->stride(1), (const int32_t*)r.pos->const_data_ptr(), r.axes, r.height, r.width,
+                             (const float*)r.inv->const_data_ptr(), 2 * (int)r.inv->size(0), r.eps, q.data_ptr(), k.data_ptr(), st);
+  });
+  return failed(rc, "qk_norm_rope") ? nullptr : wrap_tuple(q, k);
+}
+
+// A layer's pages: two 16-bit tensors, or two triplets.
+struct Pages {
+  const Tensor* t[6];
+  int n = 0, code;  // type of the rows, or of the scales
+  int64_t pages, heads, page;
+};
+
+bool page_rows(const Tensor* t, int64_t width) { return t && t->size(3) == width && aligned16(*t); }
+
+bool page_triplet(PyObject* wq, PyObject* scales, PyObject* biases, const Tensor** t) {
+  t[0] = dense(wq, 4);
+  t[1] = dense(scales, 4);
+  t[2] = dense(biases, 4);
+  return page_rows(t[0], 64) && page_rows(t[1], 4) && page_rows(t[2], 4) &&
+         (t[0]->scalar_type() == at::kUInt32 || t[0]->scalar_type() == at::kInt) && t[1]->sizes() == t[2]->sizes() &&
+         t[1]->scalar_type() == t[2]->scalar_type() && type_code(t[1]->scalar_type()) != kNoType &&
+         t[0]->sizes().slice(0, 3) == t[1]->sizes().slice(0, 3);
+}
+
+bool page_shape(Pages* p) {
+  const Tensor &k = *p->t[0], &v = *p->t[p->n / 2];
+  p->pages = k.size(0);
+  p->heads = k.size(1);
+  p->page = k.size(2);
+  return k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type() && p->pages >= 1 && p->pages <= INT32_MAX &&
+         p->heads >= 1 && p->heads <= 1024 && page_size_ok(p->page);
+}
+
+bool page_tensors(PyObject* keys, PyObject* values, Pages* p) {
+  p->t[0] = dense(keys, 4);
+  p->t[1] = dense(values, 4);
+  p->n = 2;
+  if (!page_rows(p->t[0], 256) || !page_rows(p->t[1], 256)) return false;
+  p->code = type_code(p->t[0]->scalar_type());
+  return (p->code == MSPR_F16 || p->code == MSPR_BF16) && page_shape(p);
+}
+
+bool page_triplets(PyObject* const* six, Pages* p) {
+  p->n = 6;
+  if (!page_triplet(six[0], six[1], six[2], p->t) || !page_triplet(six[3], six[4], six[5], p->t + 3)) return false;
+  p->code = type_code(p->t[1]->scalar_type());
+  return p->t[4]->scalar_type() == p->t[1]->scalar_type() && page_shape(p);
+}
+
+bool together(const Pages& p, const Tensor& with) {
+  for (int i = 0; i < p.n; i++)
+    if (p.t[i]->get_device() != with.get_device()) return false;
+  return true;
+}
+
+// (q, k, v, q_weight, k_weight, positions, inv_freq, slots, keys, values, eps, sections) -> q dense
+PyObject* qk_norm_rope_append(PyObject* const* a, Py_ssize_t nargs) {
+  MSPR_NARGS(12)
+  Rope r;
+  Pages p;
+  if (!rope_operands(a, a + 3, a[10], a[11], &r)) return none();
+  const Tensor *v = head_rows(a[2]), *slots = dense(a[7], 1, at::kInt);
+  if (!v || !slots) return none();
+  if (THPVariable_Check(a[8])) {
+    if (!page_tensors(a[8], a[9], &p) || (r.code != MSPR_F32 && p.code != r.code)) return none();
+  } else {
+    if (!PyTuple_CheckExact(a[8]) || !PyTuple_CheckExact(a[9]) || PyTuple_GET_SIZE(a[8]) != 3 || PyTuple_GET_SIZE(a[9]) != 3)
+      return none();
+    PyObject* six[6];
+    for (int i = 0; i < 3; i++) {
+      six[i] = PyTuple_GET_ITEM(a[8], i);
+      six[3 + i] = PyTuple_GET_ITEM(a[9], i);
+    }
+    if (!page_triplets(six, &p) || p.code != r.code) return none();
+  }
+  const int64_t T = r.q->size(0);
+  if (v->scalar_type() != r.q->scalar_type() || v->size(0) != T || v->size(1) != p.heads || r.k->size(1) != p.heads ||
+      slots->size(0) != T || !here({r.q, v, slots}) || !together(p, *r.q))
+    return none();
+  Tensor q = empty(r.q->sizes(), r.q->scalar_type(), *r.q);
+  const int64_t strides[6] = {r.q->stride(0), r.q->stride(1), r.k->stride(0), r.k->stride(1), v->stride(0), v->stride(1)};
+  void* o[6];
+  for (int i = 0; i < p.n; i++) o[i] = p.t[i]->data_ptr();
+  const auto* pos = (const int32_t*)r.pos->const_data_ptr();
+  const auto* inv = (const float*)r.inv->const_data_ptr();
+  const auto* at = (const int32_t*)slots->const_data_ptr();
+  const int rc = launch([&](void* st) {
+    if (p.n == 2)
+      return mspr_qk_norm_rope_append(r.q->const_data_ptr(), r.k->const_data_ptr(), v->const_data_ptr(), r.qw->const_data_ptr(),
+                                      r.kw->const_data_ptr(), r.code, (int)T, (int)r.q->size(1), (int)p.heads, 256, strides, pos,
+                                      r.axes, r.height, r.width, inv, 2 * (int)r.inv->size(0), r.eps, at, (int)p.pages,
+                                      (int)p.page, p.code, o[0], o[1], q.data_ptr(), st);
+    return mspr_qk_norm_rope_append_q8(r.q->const_data_ptr(), r.k->const_data_ptr(), v->const_data_ptr(), r.qw->const_data_ptr(),
+                                       r.kw->const_data_ptr(), r.code, (int)T, (int)r.q->size(1), (int)p.heads, 256, strides,
+                                       pos, r.axes, r.height, r.width, inv, 2 * (int)r.inv->size(0), r.eps, at, (int)p.pages,
+                                       (int)p.page, o[0], o[1], o[2], o[3], o[4], o[5], q.data_ptr(), st);
+  });
+  return failed(rc, "qk_norm_rope_append") ? nullptr : wrap(q);
+}
+
+// What the two forms of paged decode share: queries, tables, lens, requests, scale, workspace.
+struct Decode {
+  const Tensor *q, *tables, *lens, *requests = nullptr;
+  float scale;
+  int64_t R, Hq, B, P;
+};
+
+bool decode_operands(PyObject* queries, PyObject* const* rest, const Pages& p, Decode* d, Tensor* ws) {
+  d->q = dense(queries, 3);
+  d->tables = dense(rest[0], 2, at::kInt);
+  d->lens = dense(rest[1], 1, at::kInt);
+  if (!d->q || !d->tables || !d->lens || !real(rest[3], &d->scale)) return false;
+  if (rest[2] != Py_None && !(d->requests = dense(rest[2], 1, at::kInt))) return false;
+  d->R = d->q->size(0);
+  d->Hq = d->q->size(1);
+  d->B = d->tables->size(0);
+  d->P = d->tables->size(1);
+  if (d->q->size(2) != 256 || d->R < 1 || d->R > 65535 || d->Hq < 1 || d->Hq % p.heads != 0 || d->Hq / p.heads > 16 || d->B < 1 ||
+      d->B > INT32_MAX || d->P < 1 || d->P > INT32_MAX || d->lens->size(0) != d->R || !aligned16(*d->q) ||
+      (d->requests ? d->requests->size(0) != d->R : d->B != d->R))
+    return false;
+  if (!here({d->q, d->tables, d->lens}) || (d->requests && !here({d->q, d->requests})) || !together(p, *d->q)) return false;
+  return take_workspace(rest[4], mspr_sdpa_decode_paged_workspace_bytes((int)d->R, (int)d->Hq, (int)p.heads, (int)p.page, (int)d->P),
+                        *d->q, ws);
+}
+
+// (queries [R, Hq, 256], keys, values, tables, lens, requests or None, scale, workspace) -> like queries
+PyObject* sdpa_decode_paged(PyObject* const* a, Py_ssize_t nargs) {
+  MSPR_NARGS(8)
+  Pages p;
+  Decode d;
+  Tensor ws;
+  if (!page_tensors(a[1], a[2], &p) || !decode_operands(a[0], a + 3, p, &d, &ws) || type_code(d.q->scalar_type()) != p.code)
+    return none();
+  Tensor out = empty(d.q->sizes(), d.q->scalar_type(), *d.q);
+  const int rc = launch([&](void* st) {
+    return mspr_sdpa_decode_paged(d.q->const_data_ptr(), p.t[0]->const_data_ptr(), p.t[1]->const_data_ptr(), p.code,
+                                  (const int32_t*)d.tables->const_data_ptr(), (const int32_t*)d.lens->const_data_ptr(),
+                                  (const int32_t*)at_or_null(d.requests), (int)d.R, (int)d.Hq, (int)p.heads, 256, (int)p.pages,
+                                  (int)p.page, (int)d.B, (int)d.P, d.scale, out.data_ptr(), ws.data_ptr(), ws.nbytes(), st);
+  });
+  return failed(rc, "sdpa_decode_paged") ? nullptr : wrap(out);
+}
+
+// (queries [R, Hq, 256], six page parts, tables, lens, requests or None, scale, workspace) -> like queries
+PyObject* sdpa_decode_paged_q8(PyObject* const* a, Py_ssize_t nargs) {
+  MSPR_NARGS(12)
+  Pages p;
+  Decode d;
+  Tensor ws;
+  if (!page_triplets(a + 1, &p) || !decode_operands(a[0], a + 7, p, &d, &ws)) return none();
+  const int code = type_code(d.q->scalar_type());
+  if (code == kNoType) return none();
+  Tensor out = empty(d.q->sizes(), d.q->scalar_type(), *d.q);
+  const int rc = launch([&](void* st) {
+    return mspr_sdpa_decode_paged_q8(d.q->const_data_ptr(), code, p.t[0]->const_data_ptr(), p.t[1]->const_data_ptr(),
+                                     p.t[2]->const_data_ptr(), p.t[3]->const_data_ptr(), p.t[4]->const_data_ptr(),
+                                     p.t[5]->const_data_ptr(), p.code, (const int32_t*)d.tables->const_data_ptr(),
+                                     (const int32_t*)d.lens->const_data_ptr(), (const int32_t*)at_or_null(d.requests), (int)d.R,
+                                     (int)d.Hq, (int)p.heads, 256, (int)p.pages, (int)p.page, (int)d.B, (int)d.P, d.scale, 64, 8,
+                                     out.data_ptr(), ws.data_ptr(), ws.nbytes(), st);
+  });
+  return failed(rc, "sdpa_decode_paged_q8") ? nullptr : wrap(out);
+}
+
 PyMethodDef kMethods[] = {
 #define MSPR_METHOD(name) {#name, (PyCFunction)(void (*)(void))guarded<name>, METH_FASTCALL, nullptr}
     {"indexer_qat_rows", (PyCFunction)(void (*)(void))guarded<qat_rows<false>>, METH_FASTCALL, nullptr},
@@ -658,6 +916,11 @@ PyMethodDef kMethods[] = {
     MSPR_METHOD(sdpa_decode_q8),
     MSPR_METHOD(sdpa_decode_q8_0),
     MSPR_METHOD(sdpa_fa_prefill_q8),
+    MSPR_METHOD(page_step),
+    MSPR_METHOD(qk_norm_rope),
+    MSPR_METHOD(qk_norm_rope_append),
+    MSPR_METHOD(sdpa_decode_paged),
+    MSPR_METHOD(sdpa_decode_paged_q8),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_dispatch", "Native call path of the operators.", -1, kMethods,

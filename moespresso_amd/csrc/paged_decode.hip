@@ -1,0 +1,781 @@
+// Attention of one new token per request over a paged KV cache.
+//
+//   out[b, h] = sum_k softmax_k(q[b, h] . K[k] * scale) V[k]   over the lens[b] rows that the query's table names, 0 where
+//                                                              there are none
+//
+// Pages [n_pages][KV heads][page_size][256] of 16-bit rows, or affine 8-bit rows in groups of 64 (value = code * scale + bias).
+// Head dim 256, up to 16 query heads per KV head.
+//
+// Bound by HBM: every key and value row is read once (1024 bytes of 16-bit rows a key and KV head, 544 of 8-bit ones with
+// 16-bit scales) and met by 16 FLOP a byte. A workgroup owns (request, KV head, key range); each of its four waves walks
+// 32-key tiles of the range with an online softmax of its own, the waves meet in LDS, ranges in a second kernel.
+//
+// Which ranges there are follows from the lengths, which only the device knows: every workgroup adds up the requests' tiles
+// and deals them out, `per` tiles a range, so that a batch of any lengths makes about kRanges ranges. A request of one range
+// needs no second kernel.
+//
+// Per tile and wave: K rows come from HBM into registers as the A operand of S^T = K.Q^T (keys x heads, so that a head's
+// statistics lie in one lane column); V rows pass through LDS, whose transpose read yields the A operand of O^T = V^T.P^T.
+// Products are exact: 16-bit rows are multiplied as they are and the scale is applied to the sums; 8-bit codes are multiplied
+// as the whole numbers they are, each group's sum takes its scale and bias afterwards, in float32 (K), or its scale goes
+// into the weights first and its bias into a sum of its own (V). Weights, and queries whose type has more digits than an
+// operand, go in as two or three terms of it, so that nothing is rounded below float32's order but their last term.
+#include "common.h"
+#include "q8_codes.h"
+
+namespace {
+
+constexpr int kD = 256;
+constexpr int kTileKeys = 32;
+constexpr int kWaves = 4;
+constexpr int kVPitch = kD * 2 + 16;  // bytes per key row of the V tile
+constexpr int kVTileBytes = kTileKeys * kVPitch;
+constexpr int kRanges = 256;    // ranges a full batch is cut into: one workgroup a compute unit
+constexpr int kMinTiles = kWaves;  // a range gives every wave a tile
+
+constexpr int kAffine = 3;  // page format beside MSPR_F16 and MSPR_BF16
+
+struct PagedArgs {
+  const void* q;  // [B, Hq, D]
+  const void *k, *v;
+  const void *k_scales, *k_biases, *v_scales, *v_biases;
+  const int32_t* tables;    // [n_tables, width]
+  const int32_t* lens;      // [B]
+  const int32_t* requests;  // [B], the table of a query; null: its own place
+  int batch, n_kv, rep, n_tables, width, n_pages, page_shift;
+  uint32_t kv_inverse;
+  float scale_log2;
+  float* ws_o;   // [range][rep][256]
+  float* ws_ml;  // [range][16][2]
+  int32_t* plan; // [B][2]: first range of a request, ranges a KV head
+  void* out;     // [B, Hq, D]
+};
+
+__device__ __forceinline__ int wave_sum(int v) {
+#pragma unroll
+  for (int m = 1; m < MSPR_WAVE; m <<= 1) v += __shfl_xor(v, m, MSPR_WAVE);
+  return v;
+}
+
+__device__ __forceinline__ int tiles_of(int len, int cap) {
+  len = len < 0 ? 0 : len > cap ? cap : len;
+  return (len + kTileKeys - 1) / kTileKeys;
+}
+
+struct Range {
+  int b, kvh, first, count, tiles, per, index;  // `first`: the request's first range
+  bool live;
+};
+
+// The range of workgroup `wg`: requests in order, a request's ranges in order, its KV heads side by side.
+__device__ __forceinline__ Range find_range(const PagedArgs& a, int wg, int cap) {
+  const int lane = threadIdx.x & 63;
+  int total = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += MSPR_WAVE) total += b0 + lane < a.batch ? tiles_of(a.lens[b0 + lane], cap) : 0;
+  total = wave_sum(total);
+  Range r;
+  const int share = (int)(((int64_t)total * a.n_kv + kRanges - 1) / kRanges);
+  r.per = share < kMinTiles ? kMinTiles : share;
+  r.live = false;
+  int before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += MSPR_WAVE) {
+    const int tiles = b0 + lane < a.batch ? tiles_of(a.lens[b0 + lane], cap) : 0;
+    int n = b0 + lane < a.batch ? (tiles + r.per - 1) / r.per : 0;
+    if (b0 + lane < a.batch && n == 0) n = 1;
+    int s = n * a.n_kv;
+#pragma unroll
+    for (int m = 1; m < MSPR_WAVE; m <<= 1) {
+      const int o = __shfl_up(s, m, MSPR_WAVE);
+      if (lane >= m) s += o;
+    }
+    const uint64_t beyond = __ballot(before + s > wg);
+    if (beyond) {
+      const int at = __builtin_ctzll(beyond);
+      r.b = b0 + at;
+      r.count = __builtin_amdgcn_readlane(n, at);
+      r.tiles = __builtin_amdgcn_readlane(tiles, at);
+      r.first = before + __builtin_amdgcn_readlane(s, at) - r.count * a.n_kv;
+      const int in = wg - r.first;
+      r.index = mspr_div(in, a.n_kv, a.kv_inverse);
+      r.kvh = in - r.index * a.n_kv;
+      r.live = true;
+      return r;
+    }
+    before += __builtin_amdgcn_readlane(s, 63);
+  }
+  return r;
+}
+
+template <int FMT>
+__device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
+  if constexpr (FMT == MSPR_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// Eight float32 values as terms of eight 16-bit operands each: x ~ t[0] + t[1] (+ t[2]), every term the rounded rest.
+template <int FMT, int TERMS>
+__device__ __forceinline__ void split_terms(const float* x, u32x4_t* t) {
+  float rest[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) rest[i] = x[i];
+#pragma unroll
+  for (int k = 0; k < TERMS; k++) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if constexpr (FMT == MSPR_BF16) {
+        const bf16x2_t h = {(__bf16)rest[2 * j], (__bf16)rest[2 * j + 1]};
+        t[k][j] = __builtin_bit_cast(uint32_t, h);
+        rest[2 * j] -= (float)h.x;
+        rest[2 * j + 1] -= (float)h.y;
+      } else {
+        const h2_t h = {(_Float16)rest[2 * j], (_Float16)rest[2 * j + 1]};
+        t[k][j] = h2_bits(h);
+        rest[2 * j] -= (float)h.x;
+        rest[2 * j + 1] -= (float)h.y;
+      }
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void widen8(u32x4_t w, float* x) {
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    if constexpr (DT == MSPR_F16) {
+      x[2 * j] = f16_bits_to_f32((uint16_t)(w[j] & 0xFFFFu));
+      x[2 * j + 1] = f16_bits_to_f32((uint16_t)(w[j] >> 16));
+    } else {
+      x[2 * j] = __uint_as_float(w[j] << 16);
+      x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+    }
+  }
+}
+
+// Sixteen codes to bfloat16, exactly (whole numbers up to 256 are): the upper halves of their float32 values.
+__device__ __forceinline__ void codes_to_bf16(u32x4_t c, u32x4_t& lo, u32x4_t& hi) {
+  uint32_t o[8];
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    const float b0 = (float)(c[w] & 0xFFu), b1 = (float)((c[w] >> 8) & 0xFFu), b2 = (float)((c[w] >> 16) & 0xFFu),
+                b3 = (float)(c[w] >> 24);
+    o[2 * w] = __builtin_amdgcn_perm(__float_as_uint(b1), __float_as_uint(b0), 0x07060302u);
+    o[2 * w + 1] = __builtin_amdgcn_perm(__float_as_uint(b3), __float_as_uint(b2), 0x07060302u);
+  }
+  lo = u32x4_t{o[0], o[1], o[2], o[3]};
+  hi = u32x4_t{o[4], o[5], o[6], o[7]};
+}
+
+// Sixteen neighbouring scales or biases, as the rows hold them.
+template <int SDT>
+struct Sixteen {
+  u32x4_t w[SDT == MSPR_F32 ? 4 : 2];
+  __device__ __forceinline__ void load(const void* p, int64_t i) {
+    const u32x4_t* s = reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint8_t*>(p) + i * (SDT == MSPR_F32 ? 4 : 2));
+#pragma unroll
+    for (int j = 0; j < (SDT == MSPR_F32 ? 4 : 2); j++) w[j] = s[j];
+  }
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (SDT == MSPR_F32) return __uint_as_float(w[i >> 2][i & 3]);
+    const uint32_t word = w[i >> 3][(i >> 1) & 3];
+    if constexpr (SDT == MSPR_F16) return f16_bits_to_f32((uint16_t)(i & 1 ? word >> 16 : word & 0xFFFFu));
+    return __uint_as_float(i & 1 ? word & 0xFFFF0000u : word << 16);
+  }
+};
+
+// Output of one head's four channels, divided by its sum of weights.
+template <int ODT>
+__device__ __forceinline__ void store_out(void* out, int64_t i, f32x4_t o, float l) {
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if constexpr (ODT == MSPR_F32) {
+    *reinterpret_cast<f32x4_t*>(reinterpret_cast<float*>(out) + i) = o * inv;
+  } else {
+    uint16_t h[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) h[j] = ODT == MSPR_BF16 ? f32_to_bf16_bits(o[j] * inv) : f32_to_f16_bits(o[j] * inv);
+    *reinterpret_cast<u32x2_t*>(reinterpret_cast<uint16_t*>(out) + i) =
+        u32x2_t{(uint32_t)h[0] | ((uint32_t)h[1] << 16), (uint32_t)h[2] | ((uint32_t)h[3] << 16)};
+  }
+}
+
+// QDT: type of queries and output; FMT: page format; SDT: type of scales and biases (8-bit pages)
+template <int QDT, int FMT, int SDT>
+__global__ __launch_bounds__(64 * kWaves, 1) void paged_decode_kernel(PagedArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  constexpr bool kCodes = FMT == kAffine;
+  constexpr int kVType = kCodes ? MSPR_BF16 : FMT;                 // operands of the second product
+  constexpr int kPTerms = QDT == MSPR_F32 ? 3 : 2;                 // terms of a weight
+  constexpr int kQTerms = kCodes && QDT == MSPR_F32 ? 2 : 1;       // terms of a query element
+  // float16 weights are taken 2^7 times as large: up to 2^15 with the lazy maximum, and the smallest that is not lost is 2^-31
+  // of the largest (at 2^-24, the many small weights of a long context would all be rounded the same way)
+  constexpr float kUp = kVType == MSPR_F16 ? 7.0f : 0.0f;
+  constexpr int kRowBytes = kCodes ? kD : kD * 2;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15;  // MFMA column: query head of the group; row (key) of the K operand
+  const int g = lane >> 4;
+  unsigned char* vt = lds + wave * kVTileBytes;
+
+  const int cap = a.width << a.page_shift;
+  const Range r = find_range(a, blockIdx.x, cap);
+  if (!r.live) return;
+  int len = a.lens[r.b];
+  len = len < 0 ? 0 : len > cap ? cap : len;
+  const int tile0 = r.index * r.per;
+  const int tile1 = min(tile0 + r.per, r.tiles);
+  const int page_mask = (1 << a.page_shift) - 1;
+  int request = a.requests ? a.requests[r.b] : r.b;
+  if (request < 0 || request >= a.n_tables) len = request = 0;
+  const int32_t* table = a.tables + (int64_t)request * a.width;
+  if (r.index == 0 && r.kvh == 0 && threadIdx.x == 0) {
+    a.plan[2 * r.b] = r.first;
+    a.plan[2 * r.b + 1] = r.count;
+  }
+
+  f32x4_t oacc[16];
+#pragma unroll
+  for (int mt = 0; mt < 16; mt++) oacc[mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float m_run = -__builtin_inff(), l_run = 0.0f;
+  float bsum[4] = {0.f, 0.f, 0.f, 0.f};  // weighted biases of the four groups
+
+  // Pages of this wave's tiles, two half tiles of 16 keys each (a page holds 16 rows or more): lane i of `ids` has the page
+  // of half tile i of 32 tiles, the next 32 tiles' are on their way while these are used.
+  const int n_mine = len > 0 && tile1 - tile0 > wave ? (tile1 - tile0 - wave + kWaves - 1) / kWaves : 0;
+  auto load_ids = [&](int block) {
+    const int it = 32 * block + (lane >> 1);
+    const int key = (tile0 + wave + kWaves * it) * kTileKeys + 16 * (lane & 1);
+    const int e = it < n_mine && key < len ? key >> a.page_shift : -1;
+    return e >= 0 ? table[e] : -1;
+  };
+
+  // A half tile: its page's rows, and how many of them count (none of a page that is not in the pool).
+  struct Half {
+    int64_t row;  // first row in the pages
+    int rows;
+  };
+  auto half_at = [&](int ids, int it, int u) {
+    const int key = (tile0 + wave + kWaves * it) * kTileKeys + 16 * u;
+    const int p = __builtin_amdgcn_readlane(ids, 2 * (it & 31) + u);
+    const bool good = p >= 0 && p < a.n_pages;
+    Half h;
+    h.row = ((((int64_t)(good ? p : 0) * a.n_kv + r.kvh) << a.page_shift) + (key & page_mask));
+    h.rows = !good ? 0 : len - key >= 16 ? 16 : len - key < 0 ? 0 : len - key;
+    return h;
+  };
+
+  constexpr int kKLoads = kCodes ? 4 : 8;   // 16-byte pieces a lane and half tile
+  constexpr int kVLoads = kCodes ? 4 : 8;
+  u32x4_t kr[2][kKLoads], vr[2][kVLoads];
+  Sixteen<SDT> ks[2], kb[2], vs[2], vb[2];
+  auto load_k = [&](const Half* h) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const uint8_t* p = reinterpret_cast<const uint8_t*>(a.k) + h[u].row * kRowBytes + n * kRowBytes + 16 * g;
+#pragma unroll
+      for (int j = 0; j < kKLoads; j++) kr[u][j] = *reinterpret_cast<const u32x4_t*>(p + 64 * j);
+      if constexpr (kCodes) {
+        ks[u].load(a.k_scales, (h[u].row + 4 * g) * 4);
+        kb[u].load(a.k_biases, (h[u].row + 4 * g) * 4);
+      }
+    }
+  };
+  auto load_v = [&](const Half* h) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const uint8_t* p = reinterpret_cast<const uint8_t*>(a.v) + h[u].row * kRowBytes + 16 * lane;
+#pragma unroll
+      for (int j = 0; j < kVLoads; j++) vr[u][j] = *reinterpret_cast<const u32x4_t*>(p + 1024 * j);
+      if constexpr (kCodes) {
+        vs[u].load(a.v_scales, (h[u].row + 4 * g) * 4);
+        vb[u].load(a.v_biases, (h[u].row + 4 * g) * 4);
+      }
+    }
+  };
+
+  Half cur[2], nxt[2];
+  int ids = 0, ids_next = 0;
+  if (n_mine) {
+    ids = load_ids(0);
+    cur[0] = half_at(ids, 0, 0);
+    cur[1] = half_at(ids, 0, 1);
+    load_k(cur);
+    load_v(cur);
+    ids_next = load_ids(1);
+  }
+  __builtin_amdgcn_sched_barrier(0);  // the first tile is on its way before the query is fetched
+
+  // ---- Q^T operand: lane (n = head, g) holds the eight channels that the K operand has in its place
+  u32x4_t qf[8][kQTerms];
+  float q_unit = a.scale_log2;        // what a product's unit stands for, in powers of two
+  float qsum[4] = {0.f, 0.f, 0.f, 0.f};  // sums of the query over the four groups
+  {
+    const bool mine = n < a.rep;
+    const int64_t q0 = (((int64_t)r.b * a.n_kv + r.kvh) * a.rep + (mine ? n : 0)) * kD;
+    if constexpr (!kCodes) {
+      const u32x4_t* p = reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint16_t*>(a.q) + q0 + 8 * g);
+#pragma unroll
+      for (int s = 0; s < 8; s++) qf[s][0] = mine ? p[4 * s] : u32x4_t{0u, 0u, 0u, 0u};
+    } else {
+      float x[8][8];  // step s: channels 64 (s / 2) + 16 g + 8 (s % 2) on
+      float top = 0.0f;
+#pragma unroll
+      for (int s = 0; s < 8; s++) {
+        const int64_t c = q0 + 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+        if constexpr (QDT == MSPR_F32) {
+          const f32x4_t* p = reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(a.q) + c);
+          const f32x4_t lo = p[0], hi = p[1];
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            x[s][j] = lo[j];
+            x[s][4 + j] = hi[j];
+          }
+        } else {
+          widen8<QDT>(*reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint16_t*>(a.q) + c), x[s]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          x[s][j] = mine ? x[s][j] : 0.0f;
+          top = fmaxf(top, fabsf(x[s][j]));
+        }
+      }
+      // The operand is float16: a power of two brings the head's largest element to [1, 2), so that what falls below
+      // float16's range is 2^-25 of it; float16 queries go in as they are.
+      int e = 0;
+      if constexpr (QDT != MSPR_F16) {
+        top = half_wave_max(row_pair_max(top));
+        if (top > 0.0f && top < __builtin_inff()) e = __builtin_amdgcn_frexp_expf(top) - 1;
+      }
+#pragma unroll
+      for (int s = 0; s < 8; s++) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          x[s][j] = __builtin_amdgcn_ldexpf(x[s][j], -e);
+          qsum[s >> 1] += x[s][j];
+        }
+        split_terms<MSPR_F16, kQTerms>(x[s], qf[s]);
+      }
+      q_unit = __builtin_amdgcn_ldexpf(q_unit, e);
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        qsum[j] += __shfl_xor(qsum[j], 16, MSPR_WAVE);
+        qsum[j] += __shfl_xor(qsum[j], 32, MSPR_WAVE);
+      }
+    }
+  }
+
+  const int tr_off = (4 * g + ((lane & 15) >> 2)) * kVPitch + 4 * (lane & 3) * 2;
+  for (int it = 0; it < n_mine; it++) {
+    // the next tile (a wave at its last reads that again, so that what is outstanding does not depend on the tile)
+    const int it_next = it + 1 < n_mine ? it + 1 : it;
+    if ((it_next & 31) == 0 && it_next != it) {
+      ids = ids_next;
+      ids_next = load_ids(it_next / 32 + 1);
+    }
+    nxt[0] = half_at(ids, it_next, 0);
+    nxt[1] = half_at(ids, it_next, 1);
+
+    // ---- S^T = K . Q^T
+    float s[8];  // key 16 u + 4 g + i at 4 u + i
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      if constexpr (!kCodes) {
+        f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 8; j++) acc = mfma<FMT>(kr[u][j], qf[j][0], acc);
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[4 * u + i] = acc[i] * q_unit;
+      } else {
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            u32x4_t c;
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+              h2_t lo, hi;
+              codes4_to_h<kFmtAffine>(kr[u][j][2 * h + w], lo, hi);
+              c[2 * w] = h2_bits(lo);
+              c[2 * w + 1] = h2_bits(hi);
+            }
+#pragma unroll
+            for (int t = 0; t < kQTerms; t++) acc = mfma<MSPR_F16>(c, qf[2 * j + h][t], acc);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; i++) sum[i] += acc[i] * ks[u].at(4 * i + j) + qsum[j] * kb[u].at(4 * i + j);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[4 * u + i] = sum[i] * q_unit;
+      }
+    }
+    load_k(nxt);
+    __builtin_amdgcn_sched_barrier(0);
+
+    // ---- online softmax (powers of two), the reference maximum moves only past 2^8
+    float tmax = -__builtin_inff();
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if (4 * g + i >= cur[u].rows) s[4 * u + i] = -__builtin_inff();
+        tmax = fmaxf(tmax, s[4 * u + i]);
+      }
+    tmax = half_wave_max(row_pair_max(tmax));
+    const bool grow = tmax > m_run + 8.0f;
+    if (__any(grow)) {
+      const float m_new = grow ? tmax : m_run;
+      const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+      l_run *= alpha;
+      m_run = m_new;
+#pragma unroll
+      for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] * alpha;
+#pragma unroll
+      for (int j = 0; j < 4; j++) bsum[j] *= alpha;
+    }
+    const float m_safe = (m_run == -__builtin_inff() ? 0.0f : m_run) - kUp;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      s[i] = __builtin_amdgcn_exp2f(s[i] - m_safe);
+      l_run += s[i];
+    }
+
+    // ---- V rows to LDS. Rows that do not count may hold anything: they are zeros there (0 * NaN is none).
+    if (cur[0].rows < 16 || cur[1].rows < 16) {
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+#pragma unroll
+        for (int j = 0; j < kVLoads; j++) {
+          const int row = kCodes ? 4 * j + (lane >> 4) : 2 * j + (lane >> 5);
+          if (row >= cur[u].rows) vr[u][j] = u32x4_t{0u, 0u, 0u, 0u};
+        }
+        if constexpr (kCodes) {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (4 * g + i >= cur[u].rows) {
+              // (four scales of a row are one or two words)
+              if constexpr (SDT == MSPR_F32) {
+                vs[u].w[i] = vb[u].w[i] = u32x4_t{0u, 0u, 0u, 0u};
+              } else {
+                vs[u].w[i >> 1][2 * (i & 1)] = vs[u].w[i >> 1][2 * (i & 1) + 1] = 0u;
+                vb[u].w[i >> 1][2 * (i & 1)] = vb[u].w[i >> 1][2 * (i & 1) + 1] = 0u;
+              }
+            }
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int j = 0; j < kVLoads; j++) {
+        if constexpr (!kCodes) {
+          *reinterpret_cast<u32x4_t*>(vt + (16 * u + 2 * j + (lane >> 5)) * kVPitch + 16 * (lane & 31)) = vr[u][j];
+        } else {
+          u32x4_t lo, hi;
+          codes_to_bf16(vr[u][j], lo, hi);
+          unsigned char* d = vt + (16 * u + 4 * j + (lane >> 4)) * kVPitch + 32 * (lane & 15);
+          *reinterpret_cast<u32x4_t*>(d) = lo;
+          *reinterpret_cast<u32x4_t*>(d + 16) = hi;
+        }
+      }
+    constexpr int kGroups = kCodes ? 4 : 1;  // weights of their own
+    u32x4_t pf[kGroups][kPTerms];
+#pragma unroll
+    for (int j = 0; j < kGroups; j++) {
+      if constexpr (kCodes) {
+        float w[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          w[i] = s[i] * vs[i >> 2].at(4 * (i & 3) + j);
+          bsum[j] += s[i] * vb[i >> 2].at(4 * (i & 3) + j);
+        }
+        split_terms<kVType, kPTerms>(w, pf[j]);
+      } else {
+        split_terms<kVType, kPTerms>(s, pf[j]);
+      }
+    }
+    load_v(nxt);
+    cur[0] = nxt[0];
+    cur[1] = nxt[1];
+    __builtin_amdgcn_sched_barrier(0);
+
+    // ---- O^T += V^T . P^T (the tile was written by this wave only: LDS operations of one wave complete in order, the wave
+    //      barrier keeps the compiler from moving the reads up)
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int mt = 0; mt < 16; mt++) {
+      const unsigned char* base = vt + tr_off + mt * 32;
+      const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, base)));
+      const u32x2_t hi =
+          __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, base + 16 * kVPitch)));
+#pragma unroll
+      for (int t = 0; t < kPTerms; t++)
+        oacc[mt] = mfma<kVType>(u32x4_t{lo.x, lo.y, hi.x, hi.y}, pf[kCodes ? mt >> 2 : 0][t], oacc[mt]);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+
+  // ---- merge the waves through LDS (the V tiles are free now)
+  l_run += __shfl_xor(l_run, 16, MSPR_WAVE);
+  l_run += __shfl_xor(l_run, 32, MSPR_WAVE);
+  if constexpr (kCodes) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      bsum[j] += __shfl_xor(bsum[j], 16, MSPR_WAVE);
+      bsum[j] += __shfl_xor(bsum[j], 32, MSPR_WAVE);
+    }
+#pragma unroll
+    for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] + bsum[mt >> 2];
+  }
+  __syncthreads();
+  float* xo = reinterpret_cast<float*>(lds);   // [waves][16 mt][64 lanes][4]
+  float* xml = xo + kWaves * 16 * 64 * 4;      // [waves][16 heads][2]
+#pragma unroll
+  for (int mt = 0; mt < 16; mt++) *reinterpret_cast<f32x4_t*>(xo + ((wave * 16 + mt) * 64 + lane) * 4) = oacc[mt];
+  if (g == 0) {
+    xml[(wave * 16 + n) * 2] = m_run;
+    xml[(wave * 16 + n) * 2 + 1] = l_run;
+  }
+  __syncthreads();
+  float mw[kWaves], m_all = -__builtin_inff();
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) {
+    mw[w] = xml[(w * 16 + n) * 2];
+    m_all = fmaxf(m_all, mw[w]);
+  }
+  const float m_safe = m_all == -__builtin_inff() ? 0.0f : m_all;
+  float l_all = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) {
+    mw[w] = __builtin_amdgcn_exp2f(mw[w] - m_safe);
+    l_all += xml[(w * 16 + n) * 2 + 1] * mw[w];
+  }
+  const bool whole = r.count == 1;  // this range is the whole request
+  const int64_t head = ((int64_t)r.b * a.n_kv + r.kvh) * a.rep + n;
+  float* po = a.ws_o + ((int64_t)blockIdx.x * a.rep + n) * kD;
+#pragma unroll
+  for (int k = 0; k < 16 / kWaves; k++) {
+    const int mt = wave * (16 / kWaves) + k;
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) acc += *reinterpret_cast<const f32x4_t*>(xo + ((w * 16 + mt) * 64 + lane) * 4) * mw[w];
+    if (n < a.rep) {
+      if (whole) store_out<QDT>(a.out, head * kD + 16 * mt + 4 * g, acc, l_all);
+      else *reinterpret_cast<f32x4_t*>(po + 16 * mt + 4 * g) = acc;
+    }
+  }
+  if (!whole && wave == 0 && g == 0) {
+    a.ws_ml[((int64_t)blockIdx.x * 16 + n) * 2] = m_all;
+    a.ws_ml[((int64_t)blockIdx.x * 16 + n) * 2 + 1] = l_all;
+  }
+}
+
+// Joins the ranges of one (request, KV head, query head): 64 lanes cover the channels four at a time, wave w takes ranges w,
+// w + 4, ..., sixteen of them fetched at once.
+constexpr int kMergeWaves = 4;
+template <int ODT>
+__global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(PagedArgs a) {
+  __shared__ float xm[kMergeWaves], xl[kMergeWaves];
+  __shared__ __attribute__((aligned(16))) float xo[kMergeWaves][kD];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kvh = blockIdx.x, hn = blockIdx.y, b = blockIdx.z;
+  const int first = a.plan[2 * b], count = a.plan[2 * b + 1];
+  if (count <= 1) return;
+  constexpr int kAtOnce = 16;
+  float m_run = -__builtin_inff(), l = 0.0f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = wave; s0 < count; s0 += kMergeWaves * kAtOnce) {
+    const int mine = s0 + kMergeWaves * (lane % kAtOnce);
+    f32x2_t stat = {-__builtin_inff(), 0.0f};
+    if (mine < count)
+      stat = *reinterpret_cast<const f32x2_t*>(a.ws_ml + (((int64_t)first + mine * a.n_kv + kvh) * 16 + hn) * 2);
+    f32x4_t ov[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; j++) {
+      const int sp = s0 + kMergeWaves * j;
+      if (sp < count)
+        ov[j] = *reinterpret_cast<const f32x4_t*>(a.ws_o + (((int64_t)first + sp * a.n_kv + kvh) * a.rep + hn) * kD + 4 * lane);
+    }
+    float m_new = stat.x;
+    m_new = fmaxf(m_new, lane_xor<1>(m_new));
+    m_new = fmaxf(m_new, lane_xor<2>(m_new));
+    m_new = fmaxf(m_new, lane_xor<4>(m_new));
+    m_new = fmaxf(m_run, fmaxf(m_new, lane_xor<8>(m_new)));
+    const float m_safe = m_new == -__builtin_inff() ? 0.0f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(m_run - m_safe);
+    const float w = __builtin_amdgcn_exp2f(stat.x - m_safe);
+    float lw = stat.y * w;
+    lw += lane_xor<1>(lw);
+    lw += lane_xor<2>(lw);
+    lw += lane_xor<4>(lw);
+    l = l * alpha + (lw + lane_xor<8>(lw));
+    o = o * alpha;
+#pragma unroll
+    for (int j = 0; j < kAtOnce; j++)
+      if (s0 + kMergeWaves * j < count) o += ov[j] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), j));
+    m_run = m_new;
+  }
+  if (lane == 0) {
+    xm[wave] = m_run;
+    xl[wave] = l;
+  }
+  *reinterpret_cast<f32x4_t*>(&xo[wave][4 * lane]) = o;
+  __syncthreads();
+  if (wave != 0) return;
+  float m_all = -__builtin_inff();
+#pragma unroll
+  for (int w = 0; w < kMergeWaves; w++) m_all = fmaxf(m_all, xm[w]);
+  const float m_safe = m_all == -__builtin_inff() ? 0.0f : m_all;
+  float l_all = 0.0f;
+  f32x4_t o_all = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < kMergeWaves; w++) {
+    const float wt = __builtin_amdgcn_exp2f(xm[w] - m_safe);
+    l_all += xl[w] * wt;
+    o_all += *reinterpret_cast<const f32x4_t*>(&xo[w][4 * lane]) * wt;
+  }
+  store_out<ODT>(a.out, (((int64_t)b * a.n_kv + kvh) * a.rep + hn) * kD + 4 * lane, o_all, l_all);
+}
+
+// Workgroups that any lengths may need: `per` tiles a range make kRanges of them and one more a request and KV head at most,
+// and no request has more than its table's tiles give.
+int64_t paged_ranges(int batch, int n_kv, int64_t cap) {
+  const int64_t tiles = (cap + kTileKeys - 1) / kTileKeys;
+  const int64_t rows = (int64_t)batch * n_kv;
+  const int64_t by_table = rows * ((tiles + kMinTiles - 1) / kMinTiles);
+  const int64_t by_share = rows + kRanges;
+  return by_table < by_share ? by_table : by_share;
+}
+
+// Scratch: partial outputs and statistics of every range, the plan.
+size_t paged_scratch(int batch, int n_kv, int rep, int64_t cap) {
+  return (size_t)paged_ranges(batch, n_kv, cap) * ((size_t)rep * kD + 32) * sizeof(float) + (size_t)batch * 2 * sizeof(int32_t) + 64;
+}
+
+template <int QDT, int FMT, int SDT>
+int paged_launch(const PagedArgs& a, hipStream_t st) {
+  constexpr int kMergeLds = (kWaves * 16 * 64 * 4 + kWaves * 16 * 2) * 4;
+  constexpr int kLds = kWaves * kVTileBytes > kMergeLds ? kWaves * kVTileBytes : kMergeLds;
+  static bool attr_set[64] = {};  // by device
+  int device = 0;
+  if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64 || !attr_set[device]) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_decode_kernel<QDT, FMT, SDT>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    if (e != hipSuccess) {
+      mspr_set_error("sdpa_decode_paged: cannot reserve %d bytes of LDS: %s", kLds, hipGetErrorString(e));
+      return MSPR_ERR_LAUNCH;
+    }
+    if (device >= 0 && device < 64) attr_set[device] = true;
+  }
+  const int64_t cap = (int64_t)a.width << a.page_shift;
+  paged_decode_kernel<QDT, FMT, SDT><<<dim3((unsigned)paged_ranges(a.batch, a.n_kv, cap)), dim3(64 * kWaves), kLds, st>>>(a);
+  MSPR_CHECK_LAUNCH("sdpa_decode_paged (ranges)");
+  if (cap > kMinTiles * kTileKeys) {  // (else no request can have two)
+    paged_merge_kernel<QDT><<<dim3((unsigned)a.n_kv, (unsigned)a.rep, (unsigned)a.batch), dim3(64 * kMergeWaves), 0, st>>>(a);
+    MSPR_CHECK_LAUNCH("sdpa_decode_paged (merge)");
+  }
+  return MSPR_OK;
+}
+
+int paged_fill(const char* what, PagedArgs& a, const void* q, const void* k, const void* v, const int32_t* tables,
+               const int32_t* lens, const int32_t* requests, int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_pages,
+               int page_size, int n_tables, int table_width, float scale, void* out, void* workspace, size_t workspace_bytes) {
+  MSPR_REQUIRE(q && k && v && tables && lens && out, "%s: null pointer", what);
+  MSPR_REQUIRE(head_dim == kD, "%s: head_dim must be 256", what);
+  MSPR_REQUIRE(batch >= 1 && batch <= 65535, "%s: 1 to 65535 queries", what);
+  MSPR_REQUIRE(n_tables >= 1 && (requests || n_tables == batch), "%s: a table for every query, or the requests they belong to", what);
+  MSPR_REQUIRE(n_kv_heads >= 1 && n_kv_heads <= 1024 && n_q_heads >= n_kv_heads && n_q_heads % n_kv_heads == 0,
+               "%s: bad head counts", what);
+  MSPR_REQUIRE(n_q_heads / n_kv_heads <= 16, "%s: at most 16 query heads per KV head", what);
+  MSPR_REQUIRE(page_size >= 16 && (page_size & (page_size - 1)) == 0, "%s: page_size must be a power of two from 16 on", what);
+  MSPR_REQUIRE(n_pages >= 1 && (int64_t)n_pages * page_size <= 0x7FFFFFFF, "%s: the pool must hold fewer than 2^31 tokens", what);
+  MSPR_REQUIRE(table_width >= 1 && (int64_t)table_width * page_size <= 0x40000000,
+               "%s: a request's table must hold 1 page or more and at most 2^30 tokens", what);
+  MSPR_REQUIRE((int64_t)batch * (((int64_t)table_width * page_size + kTileKeys - 1) / kTileKeys) <= 0x3FFFFFFF,
+               "%s: the tables hold too many tokens together", what);
+  MSPR_REQUIRE(mspr_aligned(q, 16) && mspr_aligned(k, 16) && mspr_aligned(v, 16) && mspr_aligned(out, 16),
+               "%s: pointers must be 16-byte aligned", what);
+  const int rep = n_q_heads / n_kv_heads;
+  const int64_t cap = (int64_t)table_width * page_size;
+  const size_t need = paged_scratch(batch, n_kv_heads, rep, cap);
+  MSPR_REQUIRE(workspace && workspace_bytes >= need && mspr_aligned(workspace, 16),
+               "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", what, need, workspace_bytes);
+  const int64_t ranges = paged_ranges(batch, n_kv_heads, cap);
+  a = PagedArgs{};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.tables = tables;
+  a.lens = lens;
+  a.requests = requests;
+  a.n_tables = n_tables;
+  a.batch = batch;
+  a.n_kv = n_kv_heads;
+  a.rep = rep;
+  a.width = table_width;
+  a.n_pages = n_pages;
+  a.page_shift = __builtin_ctz(page_size);
+  a.kv_inverse = mspr_inverse(n_kv_heads);
+  a.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  a.ws_o = reinterpret_cast<float*>(workspace);
+  a.ws_ml = a.ws_o + ranges * rep * kD;
+  a.plan = reinterpret_cast<int32_t*>(a.ws_ml + ranges * 32);
+  a.out = out;
+  return MSPR_OK;
+}
+
+template <int QDT>
+int paged_q8_launch(const PagedArgs& a, int sb_dtype, hipStream_t st) {
+  if (sb_dtype == MSPR_F32) return paged_launch<QDT, kAffine, MSPR_F32>(a, st);
+  if (sb_dtype == MSPR_F16) return paged_launch<QDT, kAffine, MSPR_F16>(a, st);
+  return paged_launch<QDT, kAffine, MSPR_BF16>(a, st);
+}
+
+}  // namespace
+
+extern "C" size_t mspr_sdpa_decode_paged_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int page_size, int table_width) {
+  if (batch < 1 || n_kv_heads < 1 || n_q_heads < n_kv_heads || page_size < 1 || table_width < 1) return 0;
+  return paged_scratch(batch, n_kv_heads, n_q_heads / n_kv_heads, (int64_t)page_size * table_width);
+}
+
+extern "C" int mspr_sdpa_decode_paged(const void* queries, const void* k_pages, const void* v_pages, int dtype,
+                                      const int32_t* tables, const int32_t* lens, const int32_t* requests, int batch,
+                                      int n_q_heads, int n_kv_heads, int head_dim, int n_pages, int page_size, int n_tables,
+                                      int table_width, float scale, void* out, void* workspace, size_t workspace_bytes,
+                                      void* stream) {
+  MSPR_REQUIRE(dtype == MSPR_F16 || dtype == MSPR_BF16, "sdpa_decode_paged: dtype must be f16 or bf16");
+  PagedArgs a;
+  if (int rc = paged_fill("sdpa_decode_paged", a, queries, k_pages, v_pages, tables, lens, requests, batch, n_q_heads, n_kv_heads,
+                          head_dim, n_pages, page_size, n_tables, table_width, scale, out, workspace, workspace_bytes))
+    return rc;
+  if (dtype == MSPR_F16) return paged_launch<MSPR_F16, MSPR_F16, MSPR_F16>(a, (hipStream_t)stream);
+  return paged_launch<MSPR_BF16, MSPR_BF16, MSPR_BF16>(a, (hipStream_t)stream);
+}
+
+extern "C" int mspr_sdpa_decode_paged_q8(const void* queries, int q_dtype, const void* k_wq, const void* k_scales,
+                                         const void* k_biases, const void* v_wq, const void* v_scales, const void* v_biases,
+                                         int sb_dtype, const int32_t* tables, const int32_t* lens, const int32_t* requests,
+                                         int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_pages, int page_size,
+                                         int n_tables, int table_width, float scale, int group_size, int bits, void* out,
+                                         void* workspace, size_t workspace_bytes, void* stream) {
+  MSPR_REQUIRE(group_size == 64 && bits == 8, "sdpa_decode_paged_q8: only group_size=64, bits=8 is supported");
+  MSPR_REQUIRE(q_dtype >= MSPR_F32 && q_dtype <= MSPR_BF16, "sdpa_decode_paged_q8: queries must be f32, f16 or bf16");
+  MSPR_REQUIRE(sb_dtype >= MSPR_F32 && sb_dtype <= MSPR_BF16, "sdpa_decode_paged_q8: scales must be f32, f16 or bf16");
+  MSPR_REQUIRE(k_scales && k_biases && v_scales && v_biases, "sdpa_decode_paged_q8: null pointer");
+  MSPR_REQUIRE(mspr_aligned(k_scales, 16) && mspr_aligned(k_biases, 16) && mspr_aligned(v_scales, 16) && mspr_aligned(v_biases, 16),
+               "sdpa_decode_paged_q8: pointers must be 16-byte aligned");
+  PagedArgs a;
+  if (int rc = paged_fill("sdpa_decode_paged_q8", a, queries, k_wq, v_wq, tables, lens, requests, batch, n_q_heads, n_kv_heads,
+                          head_dim, n_pages, page_size, n_tables, table_width, scale, out, workspace, workspace_bytes))
+    return rc;
+  a.k_scales = k_scales;
+  a.k_biases = k_biases;
+  a.v_scales = v_scales;
+  a.v_biases = v_biases;
+  hipStream_t st = (hipStream_t)stream;
+  if (q_dtype == MSPR_F32) return paged_q8_launch<MSPR_F32>(a, sb_dtype, st);
+  if (q_dtype == MSPR_F16) return paged_q8_launch<MSPR_F16>(a, sb_dtype, st);
+  return paged_q8_launch<MSPR_BF16>(a, sb_dtype, st);
+}

@@ -17,6 +17,7 @@
 // O^T = V^T.P^T comes out of it through the LDS transpose read.
 #include "common.h"
 #include "profile.h"
+#include "q8_codes.h"
 
 namespace {
 
@@ -25,10 +26,6 @@ constexpr int kTileKeys = 32;
 constexpr int kQ8Waves = 4;  // waves per workgroup of the split kernel (8 measured 7-25 % slower at batch 8 / 1)
 constexpr int kVPitch = kD * 2 + 16;           // bytes per key row of the float16 V tile
 constexpr int kVTileBytes = kTileKeys * kVPitch;
-constexpr int kFmtQ8_0 = 0;
-constexpr int kFmtAffine = 1;
-
-typedef __attribute__((ext_vector_type(2))) _Float16 h2_t;
 
 struct Q8Args {
   const void* q;        // [B, Hq, D]
@@ -53,23 +50,6 @@ struct Q8Args {
 __device__ __forceinline__ f32x4_t mfma16(u32x4_t a, u32x4_t b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0,
                                                 0);
-}
-
-__device__ __forceinline__ uint32_t h2_bits(h2_t v) { return __builtin_bit_cast(uint32_t, v); }
-__device__ __forceinline__ h2_t bits_h2(uint32_t v) { return __builtin_bit_cast(h2_t, v); }
-
-// Four codes of one 32-bit word to four float16 values (two packed registers), exact integers:
-// byte b becomes the float16 with bits 0x6400 | b = 1024 + b, then the offset is taken off.
-template <int FMT>
-__device__ __forceinline__ void codes4_to_h(uint32_t w, h2_t& lo, h2_t& hi) {
-  if constexpr (FMT == kFmtQ8_0) {
-    w ^= 0x80808080u;  // int8 -> offset binary
-    lo = bits_h2(__builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - h2_t{(_Float16)1152.0f, (_Float16)1152.0f};
-    hi = bits_h2(__builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - h2_t{(_Float16)1152.0f, (_Float16)1152.0f};
-  } else {
-    lo = bits_h2(__builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - h2_t{(_Float16)1024.0f, (_Float16)1024.0f};
-    hi = bits_h2(__builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - h2_t{(_Float16)1024.0f, (_Float16)1024.0f};
-  }
 }
 
 // What the split kernel needs behind its first loads.
