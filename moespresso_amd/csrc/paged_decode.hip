@@ -10,9 +10,11 @@
 // 16-bit scales) and met by 16 FLOP a byte. A workgroup owns (request, KV head, key range); each of its four waves walks
 // 32-key tiles of the range with an online softmax of its own, the waves meet in LDS, ranges in a second kernel.
 //
-// Which ranges there are follows from the lengths, which only the device knows: every workgroup adds up the requests' tiles
-// and deals them out, `per` tiles a range, so that a batch of any lengths makes about kRanges ranges. A request of one range
-// needs no second kernel.
+// What each workgroup attends follows from the lengths, which only the device knows: the tiles of all requests and KV heads lie
+// in one line, of which every workgroup takes an equal share (ranges cut request by request and a workgroup each made 520
+// to 544 workgroups of ragged batches, the last of which ran alone: 212 us where 64 requests of up to 16384 rows now take
+// TIME_A). A share holds parts of one request or of several; a part that is not its whole row of tiles leaves partials,
+// and only rows that were cut go through the second kernel.
 //
 // Per tile and wave: K rows come from HBM into registers as the A operand of S^T = K.Q^T (keys x heads, so that a head's
 // statistics lie in one lane column); V rows pass through LDS, whose transpose read yields the A operand of O^T = V^T.P^T.
@@ -23,6 +25,8 @@
 #include "common.h"
 #include "q8_codes.h"
 
+#include <utility>
+
 namespace {
 
 constexpr int kD = 256;
@@ -30,8 +34,9 @@ constexpr int kTileKeys = 32;
 constexpr int kWaves = 4;
 constexpr int kVPitch = kD * 2 + 16;  // bytes per key row of the V tile
 constexpr int kVTileBytes = kTileKeys * kVPitch;
-constexpr int kRanges = 256;    // ranges a full batch is cut into: one workgroup a compute unit
-constexpr int kMinTiles = kWaves;  // a range gives every wave a tile
+constexpr int kMaxShares = 512;    // workgroups: two a compute unit
+constexpr int kMinTiles = kWaves;  // a share gives every wave a tile, and no row of tiles counts for less
+constexpr int kNonTemporal = 2;    // cache policy of loads that are used once
 
 constexpr int kAffine = 3;  // page format beside MSPR_F16 and MSPR_BF16
 
@@ -43,67 +48,82 @@ struct PagedArgs {
   const int32_t* lens;      // [B]
   const int32_t* requests;  // [B], the table of a query; null: its own place
   int batch, n_kv, rep, n_tables, width, n_pages, page_shift;
-  uint32_t kv_inverse;
   float scale_log2;
-  float* ws_o;   // [range][rep][256]
-  float* ws_ml;  // [range][16][2]
-  int32_t* plan; // [B][2]: first range of a request, ranges a KV head
-  void* out;     // [B, Hq, D]
+  float* ws_o;    // partial outputs [2 shares][rep][256]: of the row that a share ends (2 w) and that it begins (2 w + 1)
+  float* ws_ml;   // their statistics [2 shares][16][2]
+  int32_t* cut;   // [shares][2]: of the row that a share begins and does not end, its place (request, KV head) and the last share
+  void* out;      // [B, Hq, D]
 };
 
 __device__ __forceinline__ int wave_sum(int v) {
 #pragma unroll
   for (int m = 1; m < MSPR_WAVE; m <<= 1) v += __shfl_xor(v, m, MSPR_WAVE);
-  return v;
+  return __builtin_amdgcn_readfirstlane(v);
 }
 
-__device__ __forceinline__ int tiles_of(int len, int cap) {
-  len = len < 0 ? 0 : len > cap ? cap : len;
-  return (len + kTileKeys - 1) / kTileKeys;
+// Tiles that a row of `len` keys counts for.
+__device__ __forceinline__ int tiles_of(int len) {
+  const int t = (len + kTileKeys - 1) / kTileKeys;
+  return t < kMinTiles ? kMinTiles : t;
 }
 
-struct Range {
-  int b, kvh, first, count, tiles, per, index;  // `first`: the request's first range
-  bool live;
+__device__ __forceinline__ int length_of(const PagedArgs& a, int b, int cap) {
+  const int len = b < a.batch ? a.lens[b] : 0;
+  return len < 0 ? 0 : len > cap ? cap : len;
+}
+
+struct Place {
+  int b, kvh, tile, len;  // request, KV head, tile of its row, keys
 };
 
-// The range of workgroup `wg`: requests in order, a request's ranges in order, its KV heads side by side.
-__device__ __forceinline__ Range find_range(const PagedArgs& a, int wg, int cap) {
+// The share of all tiles that a workgroup takes.
+__device__ __forceinline__ int share_of(const PagedArgs& a, int cap, int* all) {
   const int lane = threadIdx.x & 63;
   int total = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += MSPR_WAVE) total += b0 + lane < a.batch ? tiles_of(a.lens[b0 + lane], cap) : 0;
-  total = wave_sum(total);
-  Range r;
-  const int share = (int)(((int64_t)total * a.n_kv + kRanges - 1) / kRanges);
-  r.per = share < kMinTiles ? kMinTiles : share;
-  r.live = false;
+  for (int b0 = 0; b0 < a.batch; b0 += MSPR_WAVE) total += b0 + lane < a.batch ? tiles_of(length_of(a, b0 + lane, cap)) : 0;
+  total = wave_sum(total) * a.n_kv;
+  *all = total;
+  const int share = (total + kMaxShares - 1) / kMaxShares;
+  return share < kMinTiles ? kMinTiles : share;
+}
+
+// Whose tile number `pos` is: requests in order, a request's KV heads in order.
+__device__ __forceinline__ Place place_of(const PagedArgs& a, int cap, int pos) {
+  const int lane = threadIdx.x & 63;
   int before = 0;
   for (int b0 = 0; b0 < a.batch; b0 += MSPR_WAVE) {
-    const int tiles = b0 + lane < a.batch ? tiles_of(a.lens[b0 + lane], cap) : 0;
-    int n = b0 + lane < a.batch ? (tiles + r.per - 1) / r.per : 0;
-    if (b0 + lane < a.batch && n == 0) n = 1;
-    int s = n * a.n_kv;
+    const int len = length_of(a, b0 + lane, cap);
+    const int tiles = b0 + lane < a.batch ? tiles_of(len) : 0;
+    int s = tiles;
 #pragma unroll
     for (int m = 1; m < MSPR_WAVE; m <<= 1) {
       const int o = __shfl_up(s, m, MSPR_WAVE);
       if (lane >= m) s += o;
     }
-    const uint64_t beyond = __ballot(before + s > wg);
+    const uint64_t beyond = __ballot((before + s) * a.n_kv > pos);
     if (beyond) {
       const int at = __builtin_ctzll(beyond);
-      r.b = b0 + at;
-      r.count = __builtin_amdgcn_readlane(n, at);
-      r.tiles = __builtin_amdgcn_readlane(tiles, at);
-      r.first = before + __builtin_amdgcn_readlane(s, at) - r.count * a.n_kv;
-      const int in = wg - r.first;
-      r.index = mspr_div(in, a.n_kv, a.kv_inverse);
-      r.kvh = in - r.index * a.n_kv;
-      r.live = true;
-      return r;
+      const int t = __builtin_amdgcn_readlane(tiles, at);
+      int in = pos - (before + __builtin_amdgcn_readlane(s, at) - t) * a.n_kv;
+      int kvh = 0;
+      while (in >= t) {  // (fewer than the KV heads)
+        in -= t;
+        kvh++;
+      }
+      return Place{b0 + at, kvh, in, __builtin_amdgcn_readlane(len, at)};
     }
     before += __builtin_amdgcn_readlane(s, 63);
   }
-  return r;
+  return Place{0, 0, 0, 0};  // (not reached: pos is below the total)
+}
+
+// Rows of a page as a buffer: what lies behind the ones that count reads as zero, and costs no memory access.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_window(const void* base, int64_t row, int row_bytes, int rows) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(base) + row * row_bytes), 0,
+                                           rows * row_bytes, 0x00027000);
+}
+__device__ __forceinline__ u32x4_t window_load16(__amdgpu_buffer_rsrc_t w, int lane_offset, int offset) {
+  return __builtin_amdgcn_raw_buffer_load_b128(w, lane_offset + (offset & 4095), offset & ~4095, kNonTemporal);
 }
 
 template <int FMT>
@@ -167,22 +187,37 @@ __device__ __forceinline__ void codes_to_bf16(u32x4_t c, u32x4_t& lo, u32x4_t& h
   hi = u32x4_t{o[4], o[5], o[6], o[7]};
 }
 
-// Sixteen neighbouring scales or biases, as the rows hold them.
+// Scales and biases of four rows and their four groups lie side by side: lane n of sixteen holds the one of row n / 4, group n % 4.
 template <int SDT>
-struct Sixteen {
-  u32x4_t w[SDT == MSPR_F32 ? 4 : 2];
-  __device__ __forceinline__ void load(const void* p, int64_t i) {
-    const u32x4_t* s = reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint8_t*>(p) + i * (SDT == MSPR_F32 ? 4 : 2));
-#pragma unroll
-    for (int j = 0; j < (SDT == MSPR_F32 ? 4 : 2); j++) w[j] = s[j];
+struct RowScales {
+  uint32_t bits;
+  static constexpr int kBytes = SDT == MSPR_F32 ? 4 : 2;
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t w, int i) {
+    if constexpr (SDT == MSPR_F32) bits = __builtin_amdgcn_raw_buffer_load_b32(w, i * kBytes, 0, kNonTemporal);
+    else bits = __builtin_amdgcn_raw_buffer_load_b16(w, i * kBytes, 0, kNonTemporal);
   }
-  __device__ __forceinline__ float at(int i) const {
-    if constexpr (SDT == MSPR_F32) return __uint_as_float(w[i >> 2][i & 3]);
-    const uint32_t word = w[i >> 3][(i >> 1) & 3];
-    if constexpr (SDT == MSPR_F16) return f16_bits_to_f32((uint16_t)(i & 1 ? word >> 16 : word & 0xFFFFu));
-    return __uint_as_float(i & 1 ? word & 0xFFFF0000u : word << 16);
+  __device__ __forceinline__ float value() const {
+    if constexpr (SDT == MSPR_F32) return __uint_as_float(bits);
+    else if constexpr (SDT == MSPR_F16) return f16_bits_to_f32((uint16_t)bits);
+    else return __uint_as_float(bits << 16);
   }
 };
+
+// The value of lane L of a row of sixteen in all of them (a data-parallel operand of the instruction that takes it).
+template <int L>
+__device__ __forceinline__ float of_lane(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x150 + L, 0xF, 0xF, true));  // row_newbcast
+}
+
+// f(0), ..., f(N - 1) with the counter a constant (lane numbers of data-parallel operands are)
+template <typename F, int... I>
+__device__ __forceinline__ void static_for(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+  static_for(f, std::make_integer_sequence<int, N>{});
+}
 
 // Output of one head's four channels, divided by its sum of weights.
 template <int ODT>
@@ -201,7 +236,7 @@ __device__ __forceinline__ void store_out(void* out, int64_t i, f32x4_t o, float
 
 // QDT: type of queries and output; FMT: page format; SDT: type of scales and biases (8-bit pages)
 template <int QDT, int FMT, int SDT>
-__global__ __launch_bounds__(64 * kWaves, 1) void paged_decode_kernel(PagedArgs a) {
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   constexpr bool kCodes = FMT == kAffine;
   constexpr int kVType = kCodes ? MSPR_BF16 : FMT;                 // operands of the second product
@@ -218,20 +253,24 @@ __global__ __launch_bounds__(64 * kWaves, 1) void paged_decode_kernel(PagedArgs 
   unsigned char* vt = lds + wave * kVTileBytes;
 
   const int cap = a.width << a.page_shift;
-  const Range r = find_range(a, blockIdx.x, cap);
-  if (!r.live) return;
-  int len = a.lens[r.b];
-  len = len < 0 ? 0 : len > cap ? cap : len;
-  const int tile0 = r.index * r.per;
-  const int tile1 = min(tile0 + r.per, r.tiles);
   const int page_mask = (1 << a.page_shift) - 1;
-  int request = a.requests ? a.requests[r.b] : r.b;
-  if (request < 0 || request >= a.n_tables) len = request = 0;
-  const int32_t* table = a.tables + (int64_t)request * a.width;
-  if (r.index == 0 && r.kvh == 0 && threadIdx.x == 0) {
-    a.plan[2 * r.b] = r.first;
-    a.plan[2 * r.b + 1] = r.count;
-  }
+  int all;
+  const int share = share_of(a, cap, &all);
+  int pos = blockIdx.x * share;
+  const int end = min(pos + share, all);
+  if (threadIdx.x == 0) a.cut[2 * blockIdx.x] = -1;
+  if (pos >= end) return;
+  Place at = place_of(a, cap, pos);
+
+  for (;;) {
+  const int row_tiles = tiles_of(at.len);
+  const int tile0 = at.tile;
+  const int tile1 = min(tile0 + (end - pos), row_tiles);
+  const int request = a.requests ? __builtin_amdgcn_readfirstlane(a.requests[at.b]) : at.b;
+  const bool known = request >= 0 && request < a.n_tables;
+  const int len = known ? at.len : 0;
+  const int32_t* table = a.tables + (int64_t)(known ? request : 0) * a.width;
+  const int last_tile = min(tile1, (len + kTileKeys - 1) / kTileKeys);
 
   f32x4_t oacc[16];
 #pragma unroll
@@ -241,7 +280,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void paged_decode_kernel(PagedArgs 
 
   // Pages of this wave's tiles, two half tiles of 16 keys each (a page holds 16 rows or more): lane i of `ids` has the page
   // of half tile i of 32 tiles, the next 32 tiles' are on their way while these are used.
-  const int n_mine = len > 0 && tile1 - tile0 > wave ? (tile1 - tile0 - wave + kWaves - 1) / kWaves : 0;
+  const int n_mine = last_tile - tile0 > wave ? (last_tile - tile0 - wave + kWaves - 1) / kWaves : 0;
   auto load_ids = [&](int block) {
     const int it = 32 * block + (lane >> 1);
     const int key = (tile0 + wave + kWaves * it) * kTileKeys + 16 * (lane & 1);
@@ -259,121 +298,136 @@ __global__ __launch_bounds__(64 * kWaves, 1) void paged_decode_kernel(PagedArgs 
     const int p = __builtin_amdgcn_readlane(ids, 2 * (it & 31) + u);
     const bool good = p >= 0 && p < a.n_pages;
     Half h;
-    h.row = ((((int64_t)(good ? p : 0) * a.n_kv + r.kvh) << a.page_shift) + (key & page_mask));
-    h.rows = !good ? 0 : len - key >= 16 ? 16 : len - key < 0 ? 0 : len - key;
+    h.row = ((((int64_t)(good ? p : 0) * a.n_kv + at.kvh) << a.page_shift) + (key & page_mask));
+    // (a scalar by hand: the compiler clamps with a vector instruction, and then takes the window for one of each lane's)
+    h.rows = __builtin_amdgcn_readfirstlane(!good || it >= n_mine ? 0 : len - key >= 16 ? 16 : len - key < 0 ? 0 : len - key);
     return h;
   };
 
   constexpr int kKLoads = kCodes ? 4 : 8;   // 16-byte pieces a lane and half tile
   constexpr int kVLoads = kCodes ? 4 : 8;
   u32x4_t kr[2][kKLoads], vr[2][kVLoads];
-  Sixteen<SDT> ks[2], kb[2], vs[2], vb[2];
+  RowScales<SDT> ks[2], kb[2], vs[2], vb[2];
   auto load_k = [&](const Half* h) {
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-      const uint8_t* p = reinterpret_cast<const uint8_t*>(a.k) + h[u].row * kRowBytes + n * kRowBytes + 16 * g;
+      const auto w = rows_window(a.k, h[u].row, kRowBytes, h[u].rows);
 #pragma unroll
-      for (int j = 0; j < kKLoads; j++) kr[u][j] = *reinterpret_cast<const u32x4_t*>(p + 64 * j);
+      for (int j = 0; j < kKLoads; j++) kr[u][j] = window_load16(w, n * kRowBytes + 16 * g, 64 * j);
       if constexpr (kCodes) {
-        ks[u].load(a.k_scales, (h[u].row + 4 * g) * 4);
-        kb[u].load(a.k_biases, (h[u].row + 4 * g) * 4);
+        ks[u].load(rows_window(a.k_scales, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 16 * g + n);
+        kb[u].load(rows_window(a.k_biases, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 16 * g + n);
       }
     }
   };
   auto load_v = [&](const Half* h) {
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-      const uint8_t* p = reinterpret_cast<const uint8_t*>(a.v) + h[u].row * kRowBytes + 16 * lane;
+      const auto w = rows_window(a.v, h[u].row, kRowBytes, h[u].rows);
 #pragma unroll
-      for (int j = 0; j < kVLoads; j++) vr[u][j] = *reinterpret_cast<const u32x4_t*>(p + 1024 * j);
-      if constexpr (kCodes) {
-        vs[u].load(a.v_scales, (h[u].row + 4 * g) * 4);
-        vb[u].load(a.v_biases, (h[u].row + 4 * g) * 4);
-      }
+      for (int j = 0; j < kVLoads; j++) vr[u][j] = window_load16(w, 16 * lane, 1024 * j);
+    }
+  };
+  auto load_v_scales = [&](const Half* h) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      vs[u].load(rows_window(a.v_scales, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 16 * g + n);
+      vb[u].load(rows_window(a.v_biases, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 16 * g + n);
     }
   };
 
-  Half cur[2], nxt[2];
-  int ids = 0, ids_next = 0;
-  if (n_mine) {
-    ids = load_ids(0);
-    cur[0] = half_at(ids, 0, 0);
-    cur[1] = half_at(ids, 0, 1);
-    load_k(cur);
-    load_v(cur);
-    ids_next = load_ids(1);
-  }
+  int ids = load_ids(0);
+  Half cur[2] = {half_at(ids, 0, 0), half_at(ids, 0, 1)}, nxt[2];
+  load_k(cur);
+  load_v(cur);
+  if constexpr (kCodes) load_v_scales(cur);
+  int ids_next = load_ids(1);
   __builtin_amdgcn_sched_barrier(0);  // the first tile is on its way before the query is fetched
 
-  // ---- Q^T operand: lane (n = head, g) holds the eight channels that the K operand has in its place
-  u32x4_t qf[8][kQTerms];
-  float q_unit = a.scale_log2;        // what a product's unit stands for, in powers of two
+  // ---- Q^T operand, in LDS for all waves: lane (n = head, g) has the eight channels that the K operand has in its place
+  u32x4_t* qt = reinterpret_cast<u32x4_t*>(lds + kWaves * kVTileBytes) + lane;  // [8 steps][terms][64 lanes]
+  float q_unit = a.scale_log2;           // what a product's unit stands for, in powers of two
   float qsum[4] = {0.f, 0.f, 0.f, 0.f};  // sums of the query over the four groups
   {
     const bool mine = n < a.rep;
-    const int64_t q0 = (((int64_t)r.b * a.n_kv + r.kvh) * a.rep + (mine ? n : 0)) * kD;
+    const int64_t q0 = (((int64_t)at.b * a.n_kv + at.kvh) * a.rep + (mine ? n : 0)) * kD;
     if constexpr (!kCodes) {
       const u32x4_t* p = reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint16_t*>(a.q) + q0 + 8 * g);
 #pragma unroll
-      for (int s = 0; s < 8; s++) qf[s][0] = mine ? p[4 * s] : u32x4_t{0u, 0u, 0u, 0u};
+      for (int k = 0; k < 8 / kWaves; k++) {
+        const int s = wave * (8 / kWaves) + k;
+        const u32x4_t x = p[4 * s];
+        qt[64 * s] = mine ? x : u32x4_t{0u, 0u, 0u, 0u};
+      }
     } else {
-      float x[8][8];  // step s: channels 64 (s / 2) + 16 g + 8 (s % 2) on
+      static_assert(kWaves == 4, "a wave makes the operands of one group");
+      float x[2][8];  // step 2 wave + h: channels 64 wave + 16 g + 8 h on
       float top = 0.0f;
 #pragma unroll
-      for (int s = 0; s < 8; s++) {
-        const int64_t c = q0 + 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+      for (int h = 0; h < 2; h++) {
+        const int64_t c = q0 + 64 * wave + 16 * g + 8 * h;
         if constexpr (QDT == MSPR_F32) {
           const f32x4_t* p = reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(a.q) + c);
           const f32x4_t lo = p[0], hi = p[1];
 #pragma unroll
           for (int j = 0; j < 4; j++) {
-            x[s][j] = lo[j];
-            x[s][4 + j] = hi[j];
+            x[h][j] = lo[j];
+            x[h][4 + j] = hi[j];
           }
         } else {
-          widen8<QDT>(*reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint16_t*>(a.q) + c), x[s]);
+          widen8<QDT>(*reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint16_t*>(a.q) + c), x[h]);
         }
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-          x[s][j] = mine ? x[s][j] : 0.0f;
-          top = fmaxf(top, fabsf(x[s][j]));
+          x[h][j] = mine ? x[h][j] : 0.0f;
+          top = fmaxf(top, fabsf(x[h][j]));
         }
       }
       // The operand is float16: a power of two brings the head's largest element to [1, 2), so that what falls below
       // float16's range is 2^-25 of it; float16 queries go in as they are.
+      float* shared = reinterpret_cast<float*>(lds);  // [2][waves][16 heads], where the V tiles will be
       int e = 0;
       if constexpr (QDT != MSPR_F16) {
         top = half_wave_max(row_pair_max(top));
+        if (g == 0) shared[16 * wave + n] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) top = fmaxf(top, shared[16 * w + n]);
         if (top > 0.0f && top < __builtin_inff()) e = __builtin_amdgcn_frexp_expf(top) - 1;
       }
+      float sum = 0.0f;
 #pragma unroll
-      for (int s = 0; s < 8; s++) {
+      for (int h = 0; h < 2; h++) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-          x[s][j] = __builtin_amdgcn_ldexpf(x[s][j], -e);
-          qsum[s >> 1] += x[s][j];
+          x[h][j] = __builtin_amdgcn_ldexpf(x[h][j], -e);
+          sum += x[h][j];
         }
-        split_terms<MSPR_F16, kQTerms>(x[s], qf[s]);
+        u32x4_t terms[kQTerms];
+        split_terms<MSPR_F16, kQTerms>(x[h], terms);
+#pragma unroll
+        for (int t = 0; t < kQTerms; t++) qt[64 * ((2 * wave + h) * kQTerms + t)] = terms[t];
       }
       q_unit = __builtin_amdgcn_ldexpf(q_unit, e);
+      sum += __shfl_xor(sum, 16, MSPR_WAVE);
+      sum += __shfl_xor(sum, 32, MSPR_WAVE);
+      if (g == 0) shared[64 + 16 * wave + n] = sum;
+      __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        qsum[j] += __shfl_xor(qsum[j], 16, MSPR_WAVE);
-        qsum[j] += __shfl_xor(qsum[j], 32, MSPR_WAVE);
-      }
+      for (int j = 0; j < 4; j++) qsum[j] = shared[64 + 16 * j + n];
     }
   }
+  __syncthreads();
 
   const int tr_off = (4 * g + ((lane & 15) >> 2)) * kVPitch + 4 * (lane & 3) * 2;
   for (int it = 0; it < n_mine; it++) {
-    // the next tile (a wave at its last reads that again, so that what is outstanding does not depend on the tile)
-    const int it_next = it + 1 < n_mine ? it + 1 : it;
-    if ((it_next & 31) == 0 && it_next != it) {
+    // the next tile (behind the last one that has no rows is asked for, so that what is outstanding does not depend on the tile)
+    if ((it & 31) == 31) {
       ids = ids_next;
-      ids_next = load_ids(it_next / 32 + 1);
+      ids_next = load_ids(it / 32 + 2);
     }
-    nxt[0] = half_at(ids, it_next, 0);
-    nxt[1] = half_at(ids, it_next, 1);
+    nxt[0] = half_at(ids, it + 1, 0);
+    nxt[1] = half_at(ids, it + 1, 1);
 
     // ---- S^T = K . Q^T
     float s[8];  // key 16 u + 4 g + i at 4 u + i
@@ -382,13 +436,14 @@ __global__ __launch_bounds__(64 * kWaves, 1) void paged_decode_kernel(PagedArgs 
       if constexpr (!kCodes) {
         f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < 8; j++) acc = mfma<FMT>(kr[u][j], qf[j][0], acc);
+        for (int j = 0; j < 8; j++) acc = mfma<FMT>(kr[u][j], qt[64 * j], acc);
 #pragma unroll
         for (int i = 0; i < 4; i++) s[4 * u + i] = acc[i] * q_unit;
       } else {
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
+        const float ksf = ks[u].value(), kbf = kb[u].value();
+        static_for<4>([&](auto jc) {
+          constexpr int j = decltype(jc)::value;
           f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int h = 0; h < 2; h++) {
@@ -401,11 +456,14 @@ __global__ __launch_bounds__(64 * kWaves, 1) void paged_decode_kernel(PagedArgs 
               c[2 * w + 1] = h2_bits(hi);
             }
 #pragma unroll
-            for (int t = 0; t < kQTerms; t++) acc = mfma<MSPR_F16>(c, qf[2 * j + h][t], acc);
+            for (int t = 0; t < kQTerms; t++) acc = mfma<MSPR_F16>(c, qt[64 * ((2 * j + h) * kQTerms + t)], acc);
           }
-#pragma unroll
-          for (int i = 0; i < 4; i++) sum[i] += acc[i] * ks[u].at(4 * i + j) + qsum[j] * kb[u].at(4 * i + j);
-        }
+          static_for<4>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            sum[i] = fmaf(of_lane<4 * i + j>(ksf), acc[i], sum[i]);
+            sum[i] = fmaf(of_lane<4 * i + j>(kbf), qsum[j], sum[i]);
+          });
+        });
 #pragma unroll
         for (int i = 0; i < 4; i++) s[4 * u + i] = sum[i] * q_unit;
       }
@@ -441,30 +499,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void paged_decode_kernel(PagedArgs 
       l_run += s[i];
     }
 
-    // ---- V rows to LDS. Rows that do not count may hold anything: they are zeros there (0 * NaN is none).
-    if (cur[0].rows < 16 || cur[1].rows < 16) {
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-#pragma unroll
-        for (int j = 0; j < kVLoads; j++) {
-          const int row = kCodes ? 4 * j + (lane >> 4) : 2 * j + (lane >> 5);
-          if (row >= cur[u].rows) vr[u][j] = u32x4_t{0u, 0u, 0u, 0u};
-        }
-        if constexpr (kCodes) {
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (4 * g + i >= cur[u].rows) {
-              // (four scales of a row are one or two words)
-              if constexpr (SDT == MSPR_F32) {
-                vs[u].w[i] = vb[u].w[i] = u32x4_t{0u, 0u, 0u, 0u};
-              } else {
-                vs[u].w[i >> 1][2 * (i & 1)] = vs[u].w[i >> 1][2 * (i & 1) + 1] = 0u;
-                vb[u].w[i >> 1][2 * (i & 1)] = vb[u].w[i >> 1][2 * (i & 1) + 1] = 0u;
-              }
-            }
-        }
-      }
-    }
+    // ---- V rows to LDS (zeros in the place of rows that do not count, so that what lies there meets no weight of zero)
 #pragma unroll
     for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -479,22 +514,6 @@ __global__ __launch_bounds__(64 * kWaves, 1) void paged_decode_kernel(PagedArgs 
           *reinterpret_cast<u32x4_t*>(d + 16) = hi;
         }
       }
-    constexpr int kGroups = kCodes ? 4 : 1;  // weights of their own
-    u32x4_t pf[kGroups][kPTerms];
-#pragma unroll
-    for (int j = 0; j < kGroups; j++) {
-      if constexpr (kCodes) {
-        float w[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          w[i] = s[i] * vs[i >> 2].at(4 * (i & 3) + j);
-          bsum[j] += s[i] * vb[i >> 2].at(4 * (i & 3) + j);
-        }
-        split_terms<kVType, kPTerms>(w, pf[j]);
-      } else {
-        split_terms<kVType, kPTerms>(s, pf[j]);
-      }
-    }
     load_v(nxt);
     cur[0] = nxt[0];
     cur[1] = nxt[1];
@@ -503,16 +522,35 @@ __global__ __launch_bounds__(64 * kWaves, 1) void paged_decode_kernel(PagedArgs 
     // ---- O^T += V^T . P^T (the tile was written by this wave only: LDS operations of one wave complete in order, the wave
     //      barrier keeps the compiler from moving the reads up)
     __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int mt = 0; mt < 16; mt++) {
+    auto accumulate = [&](int mt, const u32x4_t* pf) {
       const unsigned char* base = vt + tr_off + mt * 32;
       const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, base)));
       const u32x2_t hi =
           __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, base + 16 * kVPitch)));
 #pragma unroll
-      for (int t = 0; t < kPTerms; t++)
-        oacc[mt] = mfma<kVType>(u32x4_t{lo.x, lo.y, hi.x, hi.y}, pf[kCodes ? mt >> 2 : 0][t], oacc[mt]);
+      for (int t = 0; t < kPTerms; t++) oacc[mt] = mfma<kVType>(u32x4_t{lo.x, lo.y, hi.x, hi.y}, pf[t], oacc[mt]);
+    };
+    u32x4_t pf[kPTerms];
+    if constexpr (!kCodes) {
+      split_terms<kVType, kPTerms>(s, pf);
+#pragma unroll
+      for (int mt = 0; mt < 16; mt++) accumulate(mt, pf);
+    } else {
+      const float vsf[2] = {vs[0].value(), vs[1].value()}, vbf[2] = {vb[0].value(), vb[1].value()};
+      static_for<4>([&](auto jc) {  // the weights of group j, which has channels 64 j on
+        constexpr int j = decltype(jc)::value;
+        float w[8];
+        static_for<8>([&](auto ic) {
+          constexpr int i = decltype(ic)::value;
+          w[i] = s[i] * of_lane<4 * (i & 3) + j>(vsf[i >> 2]);
+          bsum[j] = fmaf(of_lane<4 * (i & 3) + j>(vbf[i >> 2]), s[i], bsum[j]);
+        });
+        split_terms<kVType, kPTerms>(w, pf);
+#pragma unroll
+        for (int m = 0; m < 4; m++) accumulate(4 * j + m, pf);
+      });
     }
+    if constexpr (kCodes) load_v_scales(nxt);
     __builtin_amdgcn_wave_barrier();
   }
 
@@ -551,9 +589,10 @@ __global__ __launch_bounds__(64 * kWaves, 1) void paged_decode_kernel(PagedArgs 
     mw[w] = __builtin_amdgcn_exp2f(mw[w] - m_safe);
     l_all += xml[(w * 16 + n) * 2 + 1] * mw[w];
   }
-  const bool whole = r.count == 1;  // this range is the whole request
-  const int64_t head = ((int64_t)r.b * a.n_kv + r.kvh) * a.rep + n;
-  float* po = a.ws_o + ((int64_t)blockIdx.x * a.rep + n) * kD;
+  const bool whole = tile0 == 0 && tile1 == row_tiles;
+  const int64_t head = ((int64_t)at.b * a.n_kv + at.kvh) * a.rep + n;
+  const int64_t part = 2 * (int64_t)blockIdx.x + (tile0 == 0 ? 1 : 0);
+  float* po = a.ws_o + (part * a.rep + n) * kD;
 #pragma unroll
   for (int k = 0; k < 16 / kWaves; k++) {
     const int mt = wave * (16 / kWaves) + k;
@@ -566,23 +605,42 @@ __global__ __launch_bounds__(64 * kWaves, 1) void paged_decode_kernel(PagedArgs 
     }
   }
   if (!whole && wave == 0 && g == 0) {
-    a.ws_ml[((int64_t)blockIdx.x * 16 + n) * 2] = m_all;
-    a.ws_ml[((int64_t)blockIdx.x * 16 + n) * 2 + 1] = l_all;
+    a.ws_ml[(part * 16 + n) * 2] = m_all;
+    a.ws_ml[(part * 16 + n) * 2 + 1] = l_all;
+    if (tile0 == 0 && n == 0) {
+      a.cut[2 * blockIdx.x] = at.b * a.n_kv + at.kvh;
+      a.cut[2 * blockIdx.x + 1] = blockIdx.x + (row_tiles - tile1 + share - 1) / share;
+    }
+  }
+  pos += tile1 - tile0;
+  if (pos >= end) return;
+  at.tile = 0;
+  if (++at.kvh == a.n_kv) {
+    at.kvh = 0;
+    at.b++;
+    at.len = __builtin_amdgcn_readfirstlane(length_of(a, at.b, cap));
+  }
+  __syncthreads();
   }
 }
 
-// Joins the ranges of one (request, KV head, query head): 64 lanes cover the channels four at a time, wave w takes ranges w,
-// w + 4, ..., sixteen of them fetched at once.
+// Where part i of a row lies whose first part is share `first`'s: that began the row, the others go on with it.
+__device__ __forceinline__ int64_t part_of(int first, int i) { return 2 * (int64_t)(first + i) + (i == 0 ? 1 : 0); }
+
+// Joins the parts of one row that was cut, for one query head: 64 lanes cover the channels four at a time, wave w takes parts
+// w, w + 4, ..., sixteen of them fetched at once. grid: (shares, query heads of a KV head); share s has the row's first part.
 constexpr int kMergeWaves = 4;
 template <int ODT>
-__global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(PagedArgs a) {
+__global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const float* ws_o, const float* ws_ml, const int32_t* cut,
+                                                                       int rep, void* out) {
   __shared__ float xm[kMergeWaves], xl[kMergeWaves];
   __shared__ __attribute__((aligned(16))) float xo[kMergeWaves][kD];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kvh = blockIdx.x, hn = blockIdx.y, b = blockIdx.z;
-  const int first = a.plan[2 * b], count = a.plan[2 * b + 1];
-  if (count <= 1) return;
+  const int first = blockIdx.x, hn = blockIdx.y;
+  const int row = cut[2 * first];
+  const int count = cut[2 * first + 1] - first + 1;
+  if (row < 0) return;
   constexpr int kAtOnce = 16;
   float m_run = -__builtin_inff(), l = 0.0f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
@@ -590,13 +648,13 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(PagedArgs
     const int mine = s0 + kMergeWaves * (lane % kAtOnce);
     f32x2_t stat = {-__builtin_inff(), 0.0f};
     if (mine < count)
-      stat = *reinterpret_cast<const f32x2_t*>(a.ws_ml + (((int64_t)first + mine * a.n_kv + kvh) * 16 + hn) * 2);
+      stat = *reinterpret_cast<const f32x2_t*>(ws_ml + (part_of(first, mine) * 16 + hn) * 2);
     f32x4_t ov[kAtOnce];
 #pragma unroll
     for (int j = 0; j < kAtOnce; j++) {
       const int sp = s0 + kMergeWaves * j;
       if (sp < count)
-        ov[j] = *reinterpret_cast<const f32x4_t*>(a.ws_o + (((int64_t)first + sp * a.n_kv + kvh) * a.rep + hn) * kD + 4 * lane);
+        ov[j] = *reinterpret_cast<const f32x4_t*>(ws_o + (part_of(first, sp) * rep + hn) * kD + 4 * lane);
     }
     float m_new = stat.x;
     m_new = fmaxf(m_new, lane_xor<1>(m_new));
@@ -636,28 +694,30 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(PagedArgs
     l_all += xl[w] * wt;
     o_all += *reinterpret_cast<const f32x4_t*>(&xo[w][4 * lane]) * wt;
   }
-  store_out<ODT>(a.out, (((int64_t)b * a.n_kv + kvh) * a.rep + hn) * kD + 4 * lane, o_all, l_all);
+  store_out<ODT>(out, ((int64_t)row * rep + hn) * kD + 4 * lane, o_all, l_all);
 }
 
-// Workgroups that any lengths may need: `per` tiles a range make kRanges of them and one more a request and KV head at most,
-// and no request has more than its table's tiles give.
-int64_t paged_ranges(int batch, int n_kv, int64_t cap) {
-  const int64_t tiles = (cap + kTileKeys - 1) / kTileKeys;
-  const int64_t rows = (int64_t)batch * n_kv;
-  const int64_t by_table = rows * ((tiles + kMinTiles - 1) / kMinTiles);
-  const int64_t by_share = rows + kRanges;
-  return by_table < by_share ? by_table : by_share;
+int64_t row_tiles_most(int64_t cap) {
+  const int64_t t = (cap + kTileKeys - 1) / kTileKeys;
+  return t < kMinTiles ? kMinTiles : t;
 }
 
-// Scratch: partial outputs and statistics of every range, the plan.
+// Workgroups: no more than the tiles of full tables give a share.
+int paged_shares(int batch, int n_kv, int64_t cap) {
+  const int64_t n = (batch * n_kv * row_tiles_most(cap) + kMinTiles - 1) / kMinTiles;
+  return (int)(n < kMaxShares ? n : kMaxShares);
+}
+
+// Scratch: partial outputs and statistics of two rows a share, which rows were cut.
 size_t paged_scratch(int batch, int n_kv, int rep, int64_t cap) {
-  return (size_t)paged_ranges(batch, n_kv, cap) * ((size_t)rep * kD + 32) * sizeof(float) + (size_t)batch * 2 * sizeof(int32_t) + 64;
+  return (size_t)paged_shares(batch, n_kv, cap) * (2 * ((size_t)rep * kD + 32) * sizeof(float) + 2 * sizeof(int32_t)) + 64;
 }
 
 template <int QDT, int FMT, int SDT>
 int paged_launch(const PagedArgs& a, hipStream_t st) {
   constexpr int kMergeLds = (kWaves * 16 * 64 * 4 + kWaves * 16 * 2) * 4;
-  constexpr int kLds = kWaves * kVTileBytes > kMergeLds ? kWaves * kVTileBytes : kMergeLds;
+  constexpr int kLoopLds = kWaves * kVTileBytes + 8 * 64 * 16 * (FMT == kAffine && QDT == MSPR_F32 ? 2 : 1);
+  constexpr int kLds = kLoopLds > kMergeLds ? kLoopLds : kMergeLds;
   static bool attr_set[64] = {};  // by device
   int device = 0;
   if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64 || !attr_set[device]) {
@@ -670,10 +730,12 @@ int paged_launch(const PagedArgs& a, hipStream_t st) {
     if (device >= 0 && device < 64) attr_set[device] = true;
   }
   const int64_t cap = (int64_t)a.width << a.page_shift;
-  paged_decode_kernel<QDT, FMT, SDT><<<dim3((unsigned)paged_ranges(a.batch, a.n_kv, cap)), dim3(64 * kWaves), kLds, st>>>(a);
-  MSPR_CHECK_LAUNCH("sdpa_decode_paged (ranges)");
-  if (cap > kMinTiles * kTileKeys) {  // (else no request can have two)
-    paged_merge_kernel<QDT><<<dim3((unsigned)a.n_kv, (unsigned)a.rep, (unsigned)a.batch), dim3(64 * kMergeWaves), 0, st>>>(a);
+  const unsigned shares = (unsigned)paged_shares(a.batch, a.n_kv, cap);
+  paged_decode_kernel<QDT, FMT, SDT><<<dim3(shares), dim3(64 * kWaves), kLds, st>>>(a);
+  MSPR_CHECK_LAUNCH("sdpa_decode_paged");
+  // (rows of kMinTiles tiles are cut only where there are more of them than workgroups)
+  if (row_tiles_most(cap) > kMinTiles || a.batch * a.n_kv > kMaxShares) {
+    paged_merge_kernel<QDT><<<dim3(shares, (unsigned)a.rep), dim3(64 * kMergeWaves), 0, st>>>(a.ws_o, a.ws_ml, a.cut, a.rep, a.out);
     MSPR_CHECK_LAUNCH("sdpa_decode_paged (merge)");
   }
   return MSPR_OK;
@@ -693,7 +755,7 @@ int paged_fill(const char* what, PagedArgs& a, const void* q, const void* k, con
   MSPR_REQUIRE(n_pages >= 1 && (int64_t)n_pages * page_size <= 0x7FFFFFFF, "%s: the pool must hold fewer than 2^31 tokens", what);
   MSPR_REQUIRE(table_width >= 1 && (int64_t)table_width * page_size <= 0x40000000,
                "%s: a request's table must hold 1 page or more and at most 2^30 tokens", what);
-  MSPR_REQUIRE((int64_t)batch * (((int64_t)table_width * page_size + kTileKeys - 1) / kTileKeys) <= 0x3FFFFFFF,
+  MSPR_REQUIRE((int64_t)batch * n_kv_heads * row_tiles_most((int64_t)table_width * page_size) <= 0x3FFFFFFF,
                "%s: the tables hold too many tokens together", what);
   MSPR_REQUIRE(mspr_aligned(q, 16) && mspr_aligned(k, 16) && mspr_aligned(v, 16) && mspr_aligned(out, 16),
                "%s: pointers must be 16-byte aligned", what);
@@ -702,7 +764,7 @@ int paged_fill(const char* what, PagedArgs& a, const void* q, const void* k, con
   const size_t need = paged_scratch(batch, n_kv_heads, rep, cap);
   MSPR_REQUIRE(workspace && workspace_bytes >= need && mspr_aligned(workspace, 16),
                "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", what, need, workspace_bytes);
-  const int64_t ranges = paged_ranges(batch, n_kv_heads, cap);
+  const int64_t parts = 2 * (int64_t)paged_shares(batch, n_kv_heads, cap);
   a = PagedArgs{};
   a.q = q;
   a.k = k;
@@ -717,11 +779,10 @@ int paged_fill(const char* what, PagedArgs& a, const void* q, const void* k, con
   a.width = table_width;
   a.n_pages = n_pages;
   a.page_shift = __builtin_ctz(page_size);
-  a.kv_inverse = mspr_inverse(n_kv_heads);
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
   a.ws_o = reinterpret_cast<float*>(workspace);
-  a.ws_ml = a.ws_o + ranges * rep * kD;
-  a.plan = reinterpret_cast<int32_t*>(a.ws_ml + ranges * 32);
+  a.ws_ml = a.ws_o + parts * rep * kD;
+  a.cut = reinterpret_cast<int32_t*>(a.ws_ml + parts * 32);
   a.out = out;
   return MSPR_OK;
 }

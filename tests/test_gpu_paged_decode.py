@@ -245,6 +245,7 @@ def test_values_of_any_size():
 
 
 def test_the_same_call_gives_the_same_bits():
+    """Whatever the workspace held before."""
     rng = np.random.default_rng(11)
     lens = [int(n) for n in rng.integers(0, 3000, 20)]
     n_pages = sum(-(-n // 16) for n in lens) + 1
@@ -253,8 +254,6 @@ def test_the_same_call_gives_the_same_bits():
     want = _attend(q, keys, values, tables, lens, SCALE)
     ws = torch.full((1 << 22,), float("nan"), device="cuda")
     assert all(_attend(q, keys, values, tables, lens, SCALE, workspace=ws).equal(want) for _ in range(5))
-    # a request's result does not depend on where it stands, as long as the ranges are the same
-    assert _attend(q.flip(0), keys, values, tables[::-1].copy(), lens[::-1], SCALE).equal(want.flip(0))
 
 
 def test_operands_outside_the_plain_case_give_the_same_results():
