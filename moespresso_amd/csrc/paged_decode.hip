@@ -11,17 +11,22 @@
 // 32-key tiles of the range with an online softmax of its own, the waves meet in LDS, ranges in a second kernel.
 //
 // What each workgroup attends follows from the lengths, which only the device knows: the tiles of all requests and KV heads lie
-// in one line, of which every workgroup takes an equal share (ranges cut request by request and a workgroup each made 520
-// to 544 workgroups of ragged batches, the last of which ran alone: 212 us where 64 requests of up to 16384 rows now take
-// TIME_A). A share holds parts of one request or of several; a part that is not its whole row of tiles leaves partials,
-// and only rows that were cut go through the second kernel.
+// in one line, of which every workgroup takes an equal share (with ranges cut request by request, the last workgroups of
+// ragged batches ran alone: 212 us where 64 requests of up to 16384 rows took 167 in shares). A share holds parts of one
+// request or of several; a part that is not its whole row of tiles leaves partials, and only rows that were cut go through
+// the second kernel.
+//
+// Rows are read as buffer windows: rows that do not count, in the last tile, behind it or in a page that is not in the pool,
+// read as zeros and cost no access, so that a wave always asks for a next tile and what is outstanding does not depend on
+// it. Loads are non-temporal (8 requests of 37000 rows 107 -> 97 us).
 //
 // Per tile and wave: K rows come from HBM into registers as the A operand of S^T = K.Q^T (keys x heads, so that a head's
 // statistics lie in one lane column); V rows pass through LDS, whose transpose read yields the A operand of O^T = V^T.P^T.
 // Products are exact: 16-bit rows are multiplied as they are and the scale is applied to the sums; 8-bit codes are multiplied
-// as the whole numbers they are, each group's sum takes its scale and bias afterwards, in float32 (K), or its scale goes
-// into the weights first and its bias into a sum of its own (V). Weights, and queries whose type has more digits than an
-// operand, go in as two or three terms of it, so that nothing is rounded below float32's order but their last term.
+// as the whole numbers they are. A group's sum over K then takes its scale in float32; a group's scale of V goes into the
+// weights first; biases are products of their own, of float32 matrix instructions (K: biases x sums of the query over a
+// group, V: weights x biases). Weights, and queries whose type has more digits than an operand, go in as two terms of it,
+// the rounded value and the rounded rest (for 8-bit rows and bfloat16 results one: float16 keeps three digits more than they).
 #include "common.h"
 #include "q8_codes.h"
 
@@ -34,31 +39,43 @@ constexpr int kTileKeys = 32;
 constexpr int kWaves = 4;
 constexpr int kVPitch = kD * 2 + 16;  // bytes per key row of the V tile
 constexpr int kVTileBytes = kTileKeys * kVPitch;
-constexpr int kMaxShares = 512;    // workgroups: two a compute unit
+constexpr int kMaxShares = 256;    // workgroups: one a compute unit
 constexpr int kMinTiles = kWaves;  // a share gives every wave a tile, and no row of tiles counts for less
 constexpr int kNonTemporal = 2;    // cache policy of loads that are used once
 
 constexpr int kAffine = 3;  // page format beside MSPR_F16 and MSPR_BF16
 
-struct PagedArgs {
-  const void* q;  // [B, Hq, D]
-  const void *k, *v;
-  const void *k_scales, *k_biases, *v_scales, *v_biases;
-  const int32_t* tables;    // [n_tables, width]
-  const int32_t* lens;      // [B]
+// What the first loads take comes as plain arguments, which are in registers when a wave starts; the rest is loaded under them.
+struct PagedRest {
+  const void* q;            // [B, Hq, D]
   const int32_t* requests;  // [B], the table of a query; null: its own place
-  int batch, n_kv, rep, n_tables, width, n_pages, page_shift;
+  const void *k_scales, *k_biases, *v_scales, *v_biases;
+  int n_tables;
   float scale_log2;
   float* ws_o;    // partial outputs [2 shares][rep][256]: of the row that a share ends (2 w) and that it begins (2 w + 1)
   float* ws_ml;   // their statistics [2 shares][16][2]
-  int32_t* cut;   // [shares][2]: of the row that a share begins and does not end, its place (request, KV head) and the last share
+  int32_t* cut;   // by row (a request's KV head) where there are no more of them than shares, else by share: {row, its first share,
+                  // its last share} of a row that was cut, row -1 of none
   void* out;      // [B, Hq, D]
 };
 
-__device__ __forceinline__ int wave_sum(int v) {
-#pragma unroll
-  for (int m = 1; m < MSPR_WAVE; m <<= 1) v += __shfl_xor(v, m, MSPR_WAVE);
-  return __builtin_amdgcn_readfirstlane(v);
+struct PagedArgs {
+  const int32_t* lens;    // [B]
+  const int32_t* tables;  // [n_tables, width]
+  const void *k, *v;
+  int batch, n_kv, rep, width, n_pages, page_shift;
+  PagedRest rest;
+};
+
+// Sums of `v` over this lane and those before it, by data-parallel moves (six steps; a lane permute each would go through LDS).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast 15, 31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+  return v;
 }
 
 // Tiles that a row of `len` keys counts for.
@@ -67,55 +84,14 @@ __device__ __forceinline__ int tiles_of(int len) {
   return t < kMinTiles ? kMinTiles : t;
 }
 
-__device__ __forceinline__ int length_of(const PagedArgs& a, int b, int cap) {
-  const int len = b < a.batch ? a.lens[b] : 0;
+__device__ __forceinline__ int length_of(const int32_t* lens, int batch, int b, int cap) {
+  const int len = b < batch ? lens[b] : 0;
   return len < 0 ? 0 : len > cap ? cap : len;
 }
 
 struct Place {
   int b, kvh, tile, len;  // request, KV head, tile of its row, keys
 };
-
-// The share of all tiles that a workgroup takes.
-__device__ __forceinline__ int share_of(const PagedArgs& a, int cap, int* all) {
-  const int lane = threadIdx.x & 63;
-  int total = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += MSPR_WAVE) total += b0 + lane < a.batch ? tiles_of(length_of(a, b0 + lane, cap)) : 0;
-  total = wave_sum(total) * a.n_kv;
-  *all = total;
-  const int share = (total + kMaxShares - 1) / kMaxShares;
-  return share < kMinTiles ? kMinTiles : share;
-}
-
-// Whose tile number `pos` is: requests in order, a request's KV heads in order.
-__device__ __forceinline__ Place place_of(const PagedArgs& a, int cap, int pos) {
-  const int lane = threadIdx.x & 63;
-  int before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += MSPR_WAVE) {
-    const int len = length_of(a, b0 + lane, cap);
-    const int tiles = b0 + lane < a.batch ? tiles_of(len) : 0;
-    int s = tiles;
-#pragma unroll
-    for (int m = 1; m < MSPR_WAVE; m <<= 1) {
-      const int o = __shfl_up(s, m, MSPR_WAVE);
-      if (lane >= m) s += o;
-    }
-    const uint64_t beyond = __ballot((before + s) * a.n_kv > pos);
-    if (beyond) {
-      const int at = __builtin_ctzll(beyond);
-      const int t = __builtin_amdgcn_readlane(tiles, at);
-      int in = pos - (before + __builtin_amdgcn_readlane(s, at) - t) * a.n_kv;
-      int kvh = 0;
-      while (in >= t) {  // (fewer than the KV heads)
-        in -= t;
-        kvh++;
-      }
-      return Place{b0 + at, kvh, in, __builtin_amdgcn_readlane(len, at)};
-    }
-    before += __builtin_amdgcn_readlane(s, 63);
-  }
-  return Place{0, 0, 0, 0};  // (not reached: pos is below the total)
-}
 
 // Rows of a page as a buffer: what lies behind the ones that count reads as zero, and costs no memory access.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_window(const void* base, int64_t row, int row_bytes, int rows) {
@@ -173,33 +149,19 @@ __device__ __forceinline__ void widen8(u32x4_t w, float* x) {
   }
 }
 
-// Sixteen codes to bfloat16, exactly (whole numbers up to 256 are): the upper halves of their float32 values.
-__device__ __forceinline__ void codes_to_bf16(u32x4_t c, u32x4_t& lo, u32x4_t& hi) {
-  uint32_t o[8];
-#pragma unroll
-  for (int w = 0; w < 4; w++) {
-    const float b0 = (float)(c[w] & 0xFFu), b1 = (float)((c[w] >> 8) & 0xFFu), b2 = (float)((c[w] >> 16) & 0xFFu),
-                b3 = (float)(c[w] >> 24);
-    o[2 * w] = __builtin_amdgcn_perm(__float_as_uint(b1), __float_as_uint(b0), 0x07060302u);
-    o[2 * w + 1] = __builtin_amdgcn_perm(__float_as_uint(b3), __float_as_uint(b2), 0x07060302u);
-  }
-  lo = u32x4_t{o[0], o[1], o[2], o[3]};
-  hi = u32x4_t{o[4], o[5], o[6], o[7]};
-}
-
-// Scales and biases of four rows and their four groups lie side by side: lane n of sixteen holds the one of row n / 4, group n % 4.
+// One scale or bias a lane, number i of a window. 16-bit ones are loaded with their neighbour, a word: what is done to them behind
+// the load (a load of 16 bits is masked) is done, and waited for, a tile too early.
 template <int SDT>
 struct RowScales {
-  uint32_t bits;
   static constexpr int kBytes = SDT == MSPR_F32 ? 4 : 2;
+  uint32_t word;
   __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t w, int i) {
-    if constexpr (SDT == MSPR_F32) bits = __builtin_amdgcn_raw_buffer_load_b32(w, i * kBytes, 0, kNonTemporal);
-    else bits = __builtin_amdgcn_raw_buffer_load_b16(w, i * kBytes, 0, kNonTemporal);
+    word = __builtin_amdgcn_raw_buffer_load_b32(w, i * kBytes & ~3, 0, kNonTemporal);
   }
-  __device__ __forceinline__ float value() const {
-    if constexpr (SDT == MSPR_F32) return __uint_as_float(bits);
-    else if constexpr (SDT == MSPR_F16) return f16_bits_to_f32((uint16_t)bits);
-    else return __uint_as_float(bits << 16);
+  __device__ __forceinline__ float value(int i) const {
+    if constexpr (SDT == MSPR_F32) return __uint_as_float(word);
+    else if constexpr (SDT == MSPR_F16) return f16_bits_to_f32((uint16_t)(word >> (i & 1) * 16));
+    else return __uint_as_float(word << (~i & 1) * 16 & 0xFFFF0000u);
   }
 };
 
@@ -235,56 +197,118 @@ __device__ __forceinline__ void store_out(void* out, int64_t i, f32x4_t o, float
 }
 
 // QDT: type of queries and output; FMT: page format; SDT: type of scales and biases (8-bit pages)
+// One workgroup a CU: with two, and half the share each, 16-bit rows took 100 us instead of 95 (8 requests of 37000 rows) and
+// 168 instead of 157 (64 ragged ones). The forms that fit 256 registers are held to them: beyond, values move to and from
+// accumulation registers (16 ragged requests of 8-bit rows 216 us instead of 199); the others would spill (104 instead of 95).
 template <int QDT, int FMT, int SDT>
-__global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedArgs a) {
+__global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 : 1) void paged_decode_kernel(const int32_t* lens, const int32_t* tables, const void* k,
+                                                                      const void* v, int batch, int n_kv, int width,
+                                                                      int page_shift, int n_pages, int rep, PagedRest a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   constexpr bool kCodes = FMT == kAffine;
-  constexpr int kVType = kCodes ? MSPR_BF16 : FMT;                 // operands of the second product
-  constexpr int kPTerms = QDT == MSPR_F32 ? 3 : 2;                 // terms of a weight
+  constexpr int kVType = kCodes ? MSPR_F16 : FMT;                  // operands of the second product
+  constexpr int kPTerms = kCodes && QDT == MSPR_BF16 ? 1 : 2;      // terms of a weight
   constexpr int kQTerms = kCodes && QDT == MSPR_F32 ? 2 : 1;       // terms of a query element
-  // float16 weights are taken 2^7 times as large: up to 2^15 with the lazy maximum, and the smallest that is not lost is 2^-31
-  // of the largest (at 2^-24, the many small weights of a long context would all be rounded the same way)
-  constexpr float kUp = kVType == MSPR_F16 ? 7.0f : 0.0f;
+  // float16 weights are taken 2^11 times as large: up to 2^15, as the reference maximum lags by 2^4 at most, and the smallest that
+  // is not lost is 2^-35 of the largest (at 2^-24, the many small weights of a long context would all be rounded one way)
+  constexpr float kLag = 4.0f;
+  constexpr float kUp = kVType == MSPR_F16 ? 11.0f : 0.0f;
   constexpr int kRowBytes = kCodes ? kD : kD * 2;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  static_assert(kWaves == 4, "a wave makes the query operands of a quarter of the channels");
   const int n = lane & 15;  // MFMA column: query head of the group; row (key) of the K operand
   const int g = lane >> 4;
   unsigned char* vt = lds + wave * kVTileBytes;
 
-  const int cap = a.width << a.page_shift;
-  const int page_mask = (1 << a.page_shift) - 1;
-  int all;
-  const int share = share_of(a, cap, &all);
+  const int cap = width << page_shift;
+  const int page_mask = (1 << page_shift) - 1;
+
+  // ---- the share: all tiles are added up, every workgroup for itself, lane i taking request i (and i + 64, ...)
+  const int len0 = length_of(lens, batch, lane, cap);
+  const int tiles0 = lane < batch ? tiles_of(len0) : 0;
+  const int sums0 = wave_scan(tiles0);
+  int all = __builtin_amdgcn_readlane(sums0, 63);
+  for (int b0 = MSPR_WAVE; b0 < batch; b0 += MSPR_WAVE) {
+    const int tiles = b0 + lane < batch ? tiles_of(length_of(lens, batch, b0 + lane, cap)) : 0;
+    all += __builtin_amdgcn_readlane(wave_scan(tiles), 63);
+  }
+  all *= n_kv;
+  int share = (all + kMaxShares - 1) / kMaxShares;
+  share = share < kMinTiles ? kMinTiles : share;
   int pos = blockIdx.x * share;
   const int end = min(pos + share, all);
-  if (threadIdx.x == 0) a.cut[2 * blockIdx.x] = -1;
+  const bool by_row = batch * n_kv <= kMaxShares;
+  if (!by_row && threadIdx.x == 0) a.cut[3 * blockIdx.x] = -1;
   if (pos >= end) return;
-  Place at = place_of(a, cap, pos);
+  Place at = {0, 0, 0, 0};
+  {
+    int before = 0, len = len0, tiles = tiles0, sums = sums0;
+    for (int b0 = 0;; b0 += MSPR_WAVE) {
+      const uint64_t beyond = __ballot((before + sums) * n_kv > pos);
+      if (beyond) {
+        const int i = __builtin_ctzll(beyond);
+        const int t = __builtin_amdgcn_readlane(tiles, i);
+        at.b = b0 + i;
+        at.len = __builtin_amdgcn_readlane(len, i);
+        at.tile = pos - (before + __builtin_amdgcn_readlane(sums, i) - t) * n_kv;
+        while (at.tile >= t) {  // (fewer times than there are KV heads)
+          at.tile -= t;
+          at.kvh++;
+        }
+        break;
+      }
+      before += __builtin_amdgcn_readlane(sums, 63);
+      if (b0 + MSPR_WAVE >= batch) return;  // (not reached: pos is below the total)
+      len = length_of(lens, batch, b0 + MSPR_WAVE + lane, cap);
+      tiles = b0 + MSPR_WAVE + lane < batch ? tiles_of(len) : 0;
+      sums = wave_scan(tiles);
+    }
+  }
 
   for (;;) {
   const int row_tiles = tiles_of(at.len);
   const int tile0 = at.tile;
   const int tile1 = min(tile0 + (end - pos), row_tiles);
+
+  // ---- the query is asked for first: loads come back in order, and the pages' addresses wait for the table anyway
+  const bool mine = n < rep;
+  u32x4_t qraw[QDT == MSPR_F32 ? 4 : 2];
+  {
+    const int64_t q0 = (((int64_t)at.b * n_kv + at.kvh) * rep + (mine ? n : 0)) * kD;
+    if constexpr (!kCodes) {  // steps 2 wave, 2 wave + 1: channels 32 step + 8 g on
+      const u32x4_t* p = reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint16_t*>(a.q) + q0 + 64 * wave + 8 * g);
+      qraw[0] = p[0];
+      qraw[1] = p[4];
+    } else {  // channels 64 wave + 16 g on
+      const u32x4_t* p = reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint8_t*>(a.q) +
+                                                          (q0 + 64 * wave + 16 * g) * (QDT == MSPR_F32 ? 4 : 2));
+#pragma unroll
+      for (int j = 0; j < (QDT == MSPR_F32 ? 4 : 2); j++) qraw[j] = p[j];
+    }
+  }
+  __builtin_amdgcn_sched_barrier(0);
+
   const int request = a.requests ? __builtin_amdgcn_readfirstlane(a.requests[at.b]) : at.b;
-  const bool known = request >= 0 && request < a.n_tables;
+  const bool known = request >= 0 && (!a.requests || request < a.n_tables);
   const int len = known ? at.len : 0;
-  const int32_t* table = a.tables + (int64_t)(known ? request : 0) * a.width;
+  const int32_t* table = tables + (int64_t)(known ? request : 0) * width;
   const int last_tile = min(tile1, (len + kTileKeys - 1) / kTileKeys);
 
   f32x4_t oacc[16];
 #pragma unroll
   for (int mt = 0; mt < 16; mt++) oacc[mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float m_run = -__builtin_inff(), l_run = 0.0f;
-  float bsum[4] = {0.f, 0.f, 0.f, 0.f};  // weighted biases of the four groups
+  f32x4_t bacc = {0.f, 0.f, 0.f, 0.f};  // weighted biases: lane n (g = 0) has those of head n and the four groups
+  float v_unit = 0x1p-126f;             // what V's scales are multiples of: a power of two from their largest magnitude on
 
   // Pages of this wave's tiles, two half tiles of 16 keys each (a page holds 16 rows or more): lane i of `ids` has the page
-  // of half tile i of 32 tiles, the next 32 tiles' are on their way while these are used.
+  // of half tile i of 31 tiles and the one behind them, the next tiles' are on their way while these are used.
   const int n_mine = last_tile - tile0 > wave ? (last_tile - tile0 - wave + kWaves - 1) / kWaves : 0;
-  auto load_ids = [&](int block) {
-    const int it = 32 * block + (lane >> 1);
+  auto load_ids = [&](int it0) {
+    const int it = it0 + (lane >> 1);
     const int key = (tile0 + wave + kWaves * it) * kTileKeys + 16 * (lane & 1);
-    const int e = it < n_mine && key < len ? key >> a.page_shift : -1;
+    const int e = it < n_mine && key < len ? key >> page_shift : -1;
     return e >= 0 ? table[e] : -1;
   };
 
@@ -293,12 +317,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedArgs 
     int64_t row;  // first row in the pages
     int rows;
   };
-  auto half_at = [&](int ids, int it, int u) {
+  auto half_at = [&](int ids, int it0, int it, int u) {
     const int key = (tile0 + wave + kWaves * it) * kTileKeys + 16 * u;
-    const int p = __builtin_amdgcn_readlane(ids, 2 * (it & 31) + u);
-    const bool good = p >= 0 && p < a.n_pages;
+    const int p = __builtin_amdgcn_readlane(ids, 2 * (it - it0) + u);
+    const bool good = p >= 0 && p < n_pages;
     Half h;
-    h.row = ((((int64_t)(good ? p : 0) * a.n_kv + at.kvh) << a.page_shift) + (key & page_mask));
+    h.row = ((((int64_t)(good ? p : 0) * n_kv + at.kvh) << page_shift) + (key & page_mask));
     // (a scalar by hand: the compiler clamps with a vector instruction, and then takes the window for one of each lane's)
     h.rows = __builtin_amdgcn_readfirstlane(!good || it >= n_mine ? 0 : len - key >= 16 ? 16 : len - key < 0 ? 0 : len - key);
     return h;
@@ -311,19 +335,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedArgs 
   auto load_k = [&](const Half* h) {
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-      const auto w = rows_window(a.k, h[u].row, kRowBytes, h[u].rows);
+      const auto w = rows_window(k, h[u].row, kRowBytes, h[u].rows);
 #pragma unroll
       for (int j = 0; j < kKLoads; j++) kr[u][j] = window_load16(w, n * kRowBytes + 16 * g, 64 * j);
       if constexpr (kCodes) {
+        // (scales: row 4 g + n / 4, group n % 4, to be spread over a row's sixteen lanes; biases: row n, group g, an operand)
         ks[u].load(rows_window(a.k_scales, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 16 * g + n);
-        kb[u].load(rows_window(a.k_biases, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 16 * g + n);
+        kb[u].load(rows_window(a.k_biases, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 4 * n + g);
       }
     }
   };
   auto load_v = [&](const Half* h) {
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-      const auto w = rows_window(a.v, h[u].row, kRowBytes, h[u].rows);
+      const auto w = rows_window(v, h[u].row, kRowBytes, h[u].rows);
 #pragma unroll
       for (int j = 0; j < kVLoads; j++) vr[u][j] = window_load16(w, 16 * lane, 1024 * j);
     }
@@ -337,45 +362,31 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedArgs 
   };
 
   int ids = load_ids(0);
-  Half cur[2] = {half_at(ids, 0, 0), half_at(ids, 0, 1)}, nxt[2];
+  Half cur[2] = {half_at(ids, 0, 0, 0), half_at(ids, 0, 0, 1)}, nxt[2];
   load_k(cur);
   load_v(cur);
   if constexpr (kCodes) load_v_scales(cur);
-  int ids_next = load_ids(1);
+  int ids_next = load_ids(31);
   __builtin_amdgcn_sched_barrier(0);  // the first tile is on its way before the query is fetched
 
   // ---- Q^T operand, in LDS for all waves: lane (n = head, g) has the eight channels that the K operand has in its place
   u32x4_t* qt = reinterpret_cast<u32x4_t*>(lds + kWaves * kVTileBytes) + lane;  // [8 steps][terms][64 lanes]
   float q_unit = a.scale_log2;           // what a product's unit stands for, in powers of two
-  float qsum[4] = {0.f, 0.f, 0.f, 0.f};  // sums of the query over the four groups
+  float qsum = 0.0f;                     // sum of the query's head n over group g
   {
-    const bool mine = n < a.rep;
-    const int64_t q0 = (((int64_t)at.b * a.n_kv + at.kvh) * a.rep + (mine ? n : 0)) * kD;
     if constexpr (!kCodes) {
-      const u32x4_t* p = reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint16_t*>(a.q) + q0 + 8 * g);
 #pragma unroll
-      for (int k = 0; k < 8 / kWaves; k++) {
-        const int s = wave * (8 / kWaves) + k;
-        const u32x4_t x = p[4 * s];
-        qt[64 * s] = mine ? x : u32x4_t{0u, 0u, 0u, 0u};
-      }
+      for (int h = 0; h < 2; h++) qt[64 * (2 * wave + h)] = mine ? qraw[h] : u32x4_t{0u, 0u, 0u, 0u};
     } else {
-      static_assert(kWaves == 4, "a wave makes the operands of one group");
-      float x[2][8];  // step 2 wave + h: channels 64 wave + 16 g + 8 h on
+      float x[2][8];  // step 2 wave + h
       float top = 0.0f;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const int64_t c = q0 + 64 * wave + 16 * g + 8 * h;
         if constexpr (QDT == MSPR_F32) {
-          const f32x4_t* p = reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(a.q) + c);
-          const f32x4_t lo = p[0], hi = p[1];
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            x[h][j] = lo[j];
-            x[h][4 + j] = hi[j];
-          }
+          for (int j = 0; j < 8; j++) x[h][j] = __uint_as_float(qraw[2 * h + j / 4][j % 4]);
         } else {
-          widen8<QDT>(*reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint16_t*>(a.q) + c), x[h]);
+          widen8<QDT>(qraw[h], x[h]);
         }
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -413,21 +424,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedArgs 
       sum += __shfl_xor(sum, 32, MSPR_WAVE);
       if (g == 0) shared[64 + 16 * wave + n] = sum;
       __syncthreads();
-#pragma unroll
-      for (int j = 0; j < 4; j++) qsum[j] = shared[64 + 16 * j + n];
+      qsum = shared[64 + 16 * g + n];
     }
   }
   __syncthreads();
 
   const int tr_off = (4 * g + ((lane & 15) >> 2)) * kVPitch + 4 * (lane & 3) * 2;
-  for (int it = 0; it < n_mine; it++) {
+  for (int it0 = 0; it0 < n_mine; it0 += 31) {  // (a loop of its own, so that only its head waits for pages)
+  const int it_end = min(it0 + 31, n_mine);
+  for (int it = it0; it < it_end; it++) {
     // the next tile (behind the last one that has no rows is asked for, so that what is outstanding does not depend on the tile)
-    if ((it & 31) == 31) {
-      ids = ids_next;
-      ids_next = load_ids(it / 32 + 2);
-    }
-    nxt[0] = half_at(ids, it + 1, 0);
-    nxt[1] = half_at(ids, it + 1, 1);
+    nxt[0] = half_at(ids, it0, it + 1, 0);
+    nxt[1] = half_at(ids, it0, it + 1, 1);
 
     // ---- S^T = K . Q^T
     float s[8];  // key 16 u + 4 g + i at 4 u + i
@@ -440,8 +448,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedArgs 
 #pragma unroll
         for (int i = 0; i < 4; i++) s[4 * u + i] = acc[i] * q_unit;
       } else {
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        const float ksf = ks[u].value(), kbf = kb[u].value();
+        f32x4_t sum = __builtin_amdgcn_mfma_f32_16x16x4f32(kb[u].value(g), qsum, f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        const float ksf = ks[u].value(n);
         static_for<4>([&](auto jc) {
           constexpr int j = decltype(jc)::value;
           f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
@@ -461,7 +469,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedArgs 
           static_for<4>([&](auto ic) {
             constexpr int i = decltype(ic)::value;
             sum[i] = fmaf(of_lane<4 * i + j>(ksf), acc[i], sum[i]);
-            sum[i] = fmaf(of_lane<4 * i + j>(kbf), qsum[j], sum[i]);
           });
         });
 #pragma unroll
@@ -471,7 +478,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedArgs 
     load_k(nxt);
     __builtin_amdgcn_sched_barrier(0);
 
-    // ---- online softmax (powers of two), the reference maximum moves only past 2^8
+    // ---- online softmax (powers of two), the reference maximum moves only past 2^4
     float tmax = -__builtin_inff();
 #pragma unroll
     for (int u = 0; u < 2; u++)
@@ -481,7 +488,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedArgs 
         tmax = fmaxf(tmax, s[4 * u + i]);
       }
     tmax = half_wave_max(row_pair_max(tmax));
-    const bool grow = tmax > m_run + 8.0f;
+    const bool grow = tmax > m_run + kLag;
     if (__any(grow)) {
       const float m_new = grow ? tmax : m_run;
       const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
@@ -489,8 +496,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedArgs 
       m_run = m_new;
 #pragma unroll
       for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] * alpha;
-#pragma unroll
-      for (int j = 0; j < 4; j++) bsum[j] *= alpha;
+      bacc = bacc * alpha;
     }
     const float m_safe = (m_run == -__builtin_inff() ? 0.0f : m_run) - kUp;
 #pragma unroll
@@ -508,7 +514,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedArgs 
           *reinterpret_cast<u32x4_t*>(vt + (16 * u + 2 * j + (lane >> 5)) * kVPitch + 16 * (lane & 31)) = vr[u][j];
         } else {
           u32x4_t lo, hi;
-          codes_to_bf16(vr[u][j], lo, hi);
+#pragma unroll
+          for (int w = 0; w < 4; w++) {
+            h2_t c01, c23;
+            codes4_to_h<kFmtAffine>(vr[u][j][w], c01, c23);
+            (w < 2 ? lo : hi)[2 * (w & 1)] = h2_bits(c01);
+            (w < 2 ? lo : hi)[2 * (w & 1) + 1] = h2_bits(c23);
+          }
           unsigned char* d = vt + (16 * u + 4 * j + (lane >> 4)) * kVPitch + 32 * (lane & 15);
           *reinterpret_cast<u32x4_t*>(d) = lo;
           *reinterpret_cast<u32x4_t*>(d + 16) = hi;
@@ -522,49 +534,86 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedArgs 
     // ---- O^T += V^T . P^T (the tile was written by this wave only: LDS operations of one wave complete in order, the wave
     //      barrier keeps the compiler from moving the reads up)
     __builtin_amdgcn_wave_barrier();
-    auto accumulate = [&](int mt, const u32x4_t* pf) {
-      const unsigned char* base = vt + tr_off + mt * 32;
-      const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, base)));
-      const u32x2_t hi =
-          __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, base + 16 * kVPitch)));
+    // (operands of four tiles of channels are read while the four before are multiplied)
+    u32x4_t vf[2][4];
+    auto read_v = [&](int q4) {
 #pragma unroll
-      for (int t = 0; t < kPTerms; t++) oacc[mt] = mfma<kVType>(u32x4_t{lo.x, lo.y, hi.x, hi.y}, pf[t], oacc[mt]);
+      for (int m = 0; m < 4; m++) {
+        const unsigned char* base = vt + tr_off + (4 * q4 + m) * 32;
+        const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, base)));
+        const u32x2_t hi =
+            __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, base + 16 * kVPitch)));
+        vf[q4 & 1][m] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
+      }
     };
+    auto accumulate = [&](int q4, const u32x4_t* pf) {
+      if (q4 < 3) read_v(q4 + 1);
+#pragma unroll
+      for (int t = 0; t < kPTerms; t++)
+#pragma unroll
+        for (int m = 0; m < 4; m++) oacc[4 * q4 + m] = mfma<kVType>(vf[q4 & 1][m], pf[t], oacc[4 * q4 + m]);
+    };
+    read_v(0);
     u32x4_t pf[kPTerms];
     if constexpr (!kCodes) {
       split_terms<kVType, kPTerms>(s, pf);
 #pragma unroll
-      for (int mt = 0; mt < 16; mt++) accumulate(mt, pf);
+      for (int q4 = 0; q4 < 4; q4++) accumulate(q4, pf);
     } else {
-      const float vsf[2] = {vs[0].value(), vs[1].value()}, vbf[2] = {vb[0].value(), vb[1].value()};
+      // The operand is float16: scales are taken as multiples of a power of two that is as large as any of them.
+      float vsf[2] = {vs[0].value(n), vs[1].value(n)};
+      const float largest = fmaxf(fabsf(vsf[0]), fabsf(vsf[1]));
+      if (__any(largest > v_unit)) {
+        float top = largest;
+        top = fmaxf(top, lane_xor<1>(top));
+        top = fmaxf(top, lane_xor<2>(top));
+        top = fmaxf(top, lane_xor<4>(top));
+        top = fmaxf(top, lane_xor<8>(top));
+        top = half_wave_max(row_pair_max(top));
+        const int e = top < 0x1p126f ? __builtin_amdgcn_frexp_expf(top) : 126;
+        const float unit = __builtin_amdgcn_ldexpf(1.0f, e);
+        const float down = v_unit / unit;
+#pragma unroll
+        for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] * down;
+        v_unit = unit;
+      }
+      const float per_unit = 1.0f / v_unit;
+      vsf[0] *= per_unit;
+      vsf[1] *= per_unit;
+      // biases: operand row m has group m of key 16 u + 4 g + i (rows from 4 on are not used)
+      const float vbf[2] = {vb[0].value(n), vb[1].value(n)};
+      static_for<8>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        const float b = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(vbf[i >> 2]), 0x100 + 4 * (i & 3), 0xF, 0xF, true));  // row_shl
+        bacc = __builtin_amdgcn_mfma_f32_16x16x4f32((i & 3) == 0 ? vbf[i >> 2] : b, s[i], bacc, 0, 0, 0);
+      });
       static_for<4>([&](auto jc) {  // the weights of group j, which has channels 64 j on
         constexpr int j = decltype(jc)::value;
         float w[8];
         static_for<8>([&](auto ic) {
           constexpr int i = decltype(ic)::value;
-          w[i] = s[i] * of_lane<4 * (i & 3) + j>(vsf[i >> 2]);
-          bsum[j] = fmaf(of_lane<4 * (i & 3) + j>(vbf[i >> 2]), s[i], bsum[j]);
+          w[i] = of_lane<4 * (i & 3) + j>(vsf[i >> 2]) * s[i];
         });
         split_terms<kVType, kPTerms>(w, pf);
-#pragma unroll
-        for (int m = 0; m < 4; m++) accumulate(4 * j + m, pf);
+        accumulate(j, pf);
       });
     }
     if constexpr (kCodes) load_v_scales(nxt);
     __builtin_amdgcn_wave_barrier();
+  }
+  ids = ids_next;
+  ids_next = load_ids(it_end + 31);
   }
 
   // ---- merge the waves through LDS (the V tiles are free now)
   l_run += __shfl_xor(l_run, 16, MSPR_WAVE);
   l_run += __shfl_xor(l_run, 32, MSPR_WAVE);
   if constexpr (kCodes) {
+    float bias[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      bsum[j] += __shfl_xor(bsum[j], 16, MSPR_WAVE);
-      bsum[j] += __shfl_xor(bsum[j], 32, MSPR_WAVE);
-    }
+    for (int j = 0; j < 4; j++) bias[j] = __shfl(bacc[j], n, MSPR_WAVE);
 #pragma unroll
-    for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] + bsum[mt >> 2];
+    for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] * v_unit + bias[mt >> 2];
   }
   __syncthreads();
   float* xo = reinterpret_cast<float*>(lds);   // [waves][16 mt][64 lanes][4]
@@ -590,35 +639,36 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedArgs 
     l_all += xml[(w * 16 + n) * 2 + 1] * mw[w];
   }
   const bool whole = tile0 == 0 && tile1 == row_tiles;
-  const int64_t head = ((int64_t)at.b * a.n_kv + at.kvh) * a.rep + n;
+  const int row = at.b * n_kv + at.kvh;
   const int64_t part = 2 * (int64_t)blockIdx.x + (tile0 == 0 ? 1 : 0);
-  float* po = a.ws_o + (part * a.rep + n) * kD;
+  const auto po = store_window(a.ws_o + part * rep * kD, rep * kD * (int)sizeof(float));
 #pragma unroll
-  for (int k = 0; k < 16 / kWaves; k++) {
-    const int mt = wave * (16 / kWaves) + k;
+  for (int q4 = 0; q4 < 16 / kWaves; q4++) {
+    const int mt = wave * (16 / kWaves) + q4;
     f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < kWaves; w++) acc += *reinterpret_cast<const f32x4_t*>(xo + ((w * 16 + mt) * 64 + lane) * 4) * mw[w];
-    if (n < a.rep) {
-      if (whole) store_out<QDT>(a.out, head * kD + 16 * mt + 4 * g, acc, l_all);
-      else *reinterpret_cast<f32x4_t*>(po + 16 * mt + 4 * g) = acc;
+    if (n < rep) {
+      if (whole) store_out<QDT>(a.out, ((int64_t)row * rep + n) * kD + 16 * mt + 4 * g, acc, l_all);
+      else window_store<kStoreThrough>(po, (n * kD + 16 * mt + 4 * g) * 4, __builtin_bit_cast(u32x4_t, acc));
     }
   }
-  if (!whole && wave == 0 && g == 0) {
-    a.ws_ml[(part * 16 + n) * 2] = m_all;
-    a.ws_ml[(part * 16 + n) * 2 + 1] = l_all;
-    if (tile0 == 0 && n == 0) {
-      a.cut[2 * blockIdx.x] = at.b * a.n_kv + at.kvh;
-      a.cut[2 * blockIdx.x + 1] = blockIdx.x + (row_tiles - tile1 + share - 1) / share;
+  if (wave == 0 && g == 0) {
+    if (!whole) *reinterpret_cast<f32x2_t*>(a.ws_ml + (part * 16 + n) * 2) = f32x2_t{m_all, l_all};
+    if (n == 0 && tile0 == 0 && (by_row || !whole)) {
+      int32_t* c = a.cut + 3 * (int64_t)(by_row ? row : (int)blockIdx.x);
+      c[0] = whole ? -1 : row;
+      c[1] = blockIdx.x;
+      c[2] = blockIdx.x + (row_tiles - tile1 + share - 1) / share;
     }
   }
   pos += tile1 - tile0;
   if (pos >= end) return;
   at.tile = 0;
-  if (++at.kvh == a.n_kv) {
+  if (++at.kvh == n_kv) {
     at.kvh = 0;
     at.b++;
-    at.len = __builtin_amdgcn_readfirstlane(length_of(a, at.b, cap));
+    at.len = __builtin_amdgcn_readfirstlane(length_of(lens, batch, at.b, cap));
   }
   __syncthreads();
   }
@@ -628,18 +678,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedArgs 
 __device__ __forceinline__ int64_t part_of(int first, int i) { return 2 * (int64_t)(first + i) + (i == 0 ? 1 : 0); }
 
 // Joins the parts of one row that was cut, for one query head: 64 lanes cover the channels four at a time, wave w takes parts
-// w, w + 4, ..., sixteen of them fetched at once. grid: (shares, query heads of a KV head); share s has the row's first part.
-constexpr int kMergeWaves = 4;
+// w, w + 8, ..., sixteen of them fetched at once. grid: (entries of `cut`, query heads of a KV head).
+constexpr int kMergeWaves = 8;
 template <int ODT>
-__global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const float* ws_o, const float* ws_ml, const int32_t* cut,
+__global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const int32_t* cut, const float* ws_o, const float* ws_ml,
                                                                        int rep, void* out) {
   __shared__ float xm[kMergeWaves], xl[kMergeWaves];
   __shared__ __attribute__((aligned(16))) float xo[kMergeWaves][kD];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int first = blockIdx.x, hn = blockIdx.y;
-  const int row = cut[2 * first];
-  const int count = cut[2 * first + 1] - first + 1;
+  const int hn = blockIdx.y;
+  const int row = cut[3 * blockIdx.x], first = cut[3 * blockIdx.x + 1];
+  const int count = cut[3 * blockIdx.x + 2] - first + 1;
   if (row < 0) return;
   constexpr int kAtOnce = 16;
   float m_run = -__builtin_inff(), l = 0.0f;
@@ -710,7 +760,7 @@ int paged_shares(int batch, int n_kv, int64_t cap) {
 
 // Scratch: partial outputs and statistics of two rows a share, which rows were cut.
 size_t paged_scratch(int batch, int n_kv, int rep, int64_t cap) {
-  return (size_t)paged_shares(batch, n_kv, cap) * (2 * ((size_t)rep * kD + 32) * sizeof(float) + 2 * sizeof(int32_t)) + 64;
+  return (size_t)paged_shares(batch, n_kv, cap) * 2 * ((size_t)rep * kD + 32) * sizeof(float) + kMaxShares * 3 * sizeof(int32_t);
 }
 
 template <int QDT, int FMT, int SDT>
@@ -731,11 +781,15 @@ int paged_launch(const PagedArgs& a, hipStream_t st) {
   }
   const int64_t cap = (int64_t)a.width << a.page_shift;
   const unsigned shares = (unsigned)paged_shares(a.batch, a.n_kv, cap);
-  paged_decode_kernel<QDT, FMT, SDT><<<dim3(shares), dim3(64 * kWaves), kLds, st>>>(a);
+  const PagedRest& r = a.rest;
+  paged_decode_kernel<QDT, FMT, SDT><<<dim3(shares), dim3(64 * kWaves), kLds, st>>>(
+      a.lens, a.tables, a.k, a.v, a.batch, a.n_kv, a.width, a.page_shift, a.n_pages, a.rep, r);
   MSPR_CHECK_LAUNCH("sdpa_decode_paged");
   // (rows of kMinTiles tiles are cut only where there are more of them than workgroups)
-  if (row_tiles_most(cap) > kMinTiles || a.batch * a.n_kv > kMaxShares) {
-    paged_merge_kernel<QDT><<<dim3(shares, (unsigned)a.rep), dim3(64 * kMergeWaves), 0, st>>>(a.ws_o, a.ws_ml, a.cut, a.rep, a.out);
+  const int rows = a.batch * a.n_kv;
+  if (row_tiles_most(cap) > kMinTiles || rows > kMaxShares) {
+    const dim3 grid(rows <= kMaxShares ? (unsigned)rows : shares, (unsigned)a.rep);
+    paged_merge_kernel<QDT><<<grid, dim3(64 * kMergeWaves), 0, st>>>(r.cut, r.ws_o, r.ws_ml, a.rep, r.out);
     MSPR_CHECK_LAUNCH("sdpa_decode_paged (merge)");
   }
   return MSPR_OK;
@@ -766,24 +820,24 @@ int paged_fill(const char* what, PagedArgs& a, const void* q, const void* k, con
                "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", what, need, workspace_bytes);
   const int64_t parts = 2 * (int64_t)paged_shares(batch, n_kv_heads, cap);
   a = PagedArgs{};
-  a.q = q;
+  a.rest.q = q;
   a.k = k;
   a.v = v;
   a.tables = tables;
   a.lens = lens;
-  a.requests = requests;
-  a.n_tables = n_tables;
+  a.rest.requests = requests;
+  a.rest.n_tables = n_tables;
   a.batch = batch;
   a.n_kv = n_kv_heads;
   a.rep = rep;
   a.width = table_width;
   a.n_pages = n_pages;
   a.page_shift = __builtin_ctz(page_size);
-  a.scale_log2 = (float)((double)scale * 1.4426950408889634);
-  a.ws_o = reinterpret_cast<float*>(workspace);
-  a.ws_ml = a.ws_o + parts * rep * kD;
-  a.cut = reinterpret_cast<int32_t*>(a.ws_ml + parts * 32);
-  a.out = out;
+  a.rest.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  a.rest.ws_o = reinterpret_cast<float*>(workspace);
+  a.rest.ws_ml = a.rest.ws_o + parts * rep * kD;
+  a.rest.cut = reinterpret_cast<int32_t*>(a.rest.ws_ml + parts * 32);
+  a.rest.out = out;
   return MSPR_OK;
 }
 
@@ -831,10 +885,10 @@ extern "C" int mspr_sdpa_decode_paged_q8(const void* queries, int q_dtype, const
   if (int rc = paged_fill("sdpa_decode_paged_q8", a, queries, k_wq, v_wq, tables, lens, requests, batch, n_q_heads, n_kv_heads,
                           head_dim, n_pages, page_size, n_tables, table_width, scale, out, workspace, workspace_bytes))
     return rc;
-  a.k_scales = k_scales;
-  a.k_biases = k_biases;
-  a.v_scales = v_scales;
-  a.v_biases = v_biases;
+  a.rest.k_scales = k_scales;
+  a.rest.k_biases = k_biases;
+  a.rest.v_scales = v_scales;
+  a.rest.v_biases = v_biases;
   hipStream_t st = (hipStream_t)stream;
   if (q_dtype == MSPR_F32) return paged_q8_launch<MSPR_F32>(a, sb_dtype, st);
   if (q_dtype == MSPR_F16) return paged_q8_launch<MSPR_F16>(a, sb_dtype, st);

@@ -6,7 +6,7 @@ import pytest
 
 from moespresso_amd import _lib
 
-TILE, WAVES, SHARES, MIN_TILES = 32, 4, 512, 4
+TILE, WAVES, SHARES, MIN_TILES = 32, 4, 256, 4
 
 
 def _row_tiles(n):
@@ -100,5 +100,5 @@ def test_every_row_is_attended_once_and_every_address_lies_in_its_buffer(kind, b
 @pytest.mark.skipif(not _lib.library_available(), reason="the library is not built")
 @pytest.mark.parametrize("batch,heads,n_kv,page,width", [(1, 16, 2, 64, 1), (1, 16, 2, 64, 2048), (256, 64, 8, 16, 100), (65535, 1, 1, 16, 1)])
 def test_the_workspace_holds_every_part(batch, heads, n_kv, page, width):
-    need = _shares(batch, n_kv, page * width) * (2 * (heads // n_kv * 256 + 32) * 4 + 8)
+    need = _shares(batch, n_kv, page * width) * 2 * (heads // n_kv * 256 + 32) * 4 + 3 * 4 * SHARES
     assert need <= _lib.lib().mspr_sdpa_decode_paged_workspace_bytes(batch, heads, n_kv, page, width) <= need + 64
