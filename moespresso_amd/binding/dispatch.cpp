@@ -644,6 +644,14 @@ bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_dat
 
 bool page_size_ok(int64_t n) { return n >= 16 && n <= INT32_MAX && (n & (n - 1)) == 0; }
 
+// `n` elements of a tensor from `offset` on, as a tensor of their own.
+Tensor part(const Tensor& of, int64_t offset, int64_t n) {
+  auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(of.storage()), of.key_set(), of.dtype());
+  impl->set_sizes_contiguous({n});
+  impl->set_storage_offset(offset);
+  return Tensor(std::move(impl));
+}
+
 // (lens, new_lens int32 [B], tables int32 [B, P], free_pages int32 [n], head int32 [1], page_size, n_rows) -> the eight parts of a step
 PyObject* page_step(PyObject* const* a, Py_ssize_t nargs) {
   MSPR_NARGS(7)
@@ -657,9 +665,17 @@ PyObject* page_step(PyObject* const* a, Py_ssize_t nargs) {
   if (B < 1 || B > 2048 || add->size(0) != B || tables->size(0) != B || P < 1 || P > INT32_MAX || N < 1 || N > INT32_MAX ||
       head->size(0) != 1 || n_rows < 0 || !page_size_ok(page_size))
     return none();
+  // eight tensors in one allocation (allocated one by one they were half of the call: 9.2 us a step of 16 requests)
   Tensor out[8];
   const int64_t sizes[8] = {B, 1, B + 1, n_rows, n_rows, n_rows, n_rows, 4};
-  for (int i = 0; i < 8; i++) out[i] = empty({sizes[i]}, at::kInt, *lens);
+  int64_t total = 0;
+  for (const int64_t n : sizes) total += (n + 3) / 4 * 4;
+  const Tensor all = empty({total}, at::kInt, *lens);
+  total = 0;
+  for (int i = 0; i < 8; i++) {
+    out[i] = part(all, total, sizes[i]);
+    total += (sizes[i] + 3) / 4 * 4;
+  }
   int32_t* o[8];
   for (int i = 0; i < 8; i++) o[i] = (int32_t*)out[i].data_ptr();
   const int rc = launch([&](void* st) {

@@ -6,13 +6,15 @@
 // back; each page that moves and each row then finds its request by bisection of a sum.
 //
 // Bound by latency: a step of 16 requests reads 128 bytes and writes 500. One launch; every workgroup makes the sums anew
-// (2048 requests are two a thread) rather than wait for another's, and writes its share of the rows. What one workgroup
+// (2048 requests are eight a thread) rather than wait for another's, and writes its share of the rows. What one workgroup
 // writes no other reads: pages given back go below `head` and pages taken from there are read where they come from, the table
 // of the ended request; new table entries lie behind those that rows of the last started page read.
 #include "common.h"
 
 namespace {
 
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / MSPR_WAVE;
 constexpr int kMaxRequests = 2048;  // (five sums of them in 40 KB of LDS)
 
 struct StepArgs {
@@ -32,34 +34,46 @@ struct StepArgs {
   int32_t* counts;
 };
 
-// a + b of values from 0 on, at most 2^31 - 1: asked-for rows may add up to more
-__device__ __forceinline__ int sat_add(int a, int b) {
-  const uint32_t s = (uint32_t)a + (uint32_t)b;
-  return s > 0x7FFFFFFFu ? 0x7FFFFFFF : (int)s;
+// a + b of values from 0 on, at most 2^32 - 1: asked-for rows may add up to more
+__device__ __forceinline__ uint32_t sat_add(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t scan_step(uint32_t v) {
+  return sat_add(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false));
 }
 
-// Sums of `v` over the threads before this one, and of all of them in `total`.
-template <int THREADS>
-__device__ __forceinline__ int block_scan(int v, int* wave_sums, int& total) {
-  const int lane = threadIdx.x & 63;
+// Sums over this lane and those before it, by data-parallel moves.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v = scan_step<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v = scan_step<0x112, 0xF>(v);
+  v = scan_step<0x114, 0xF>(v);
+  v = scan_step<0x118, 0xF>(v);
+  v = scan_step<0x142, 0xA>(v);  // row_bcast 15, 31
+  return scan_step<0x143, 0xC>(v);
+}
+
+// Sums of N values over the threads before this one (in place), and over all of them in `total`, at most 2^31 - 1.
+template <int N>
+__device__ __forceinline__ void block_scan(uint32_t* v, uint32_t (*wave_sums)[N], int* total) {
   const int wave = threadIdx.x >> 6;
-  int s = v;
+  uint32_t s[N];
 #pragma unroll
-  for (int m = 1; m < MSPR_WAVE; m <<= 1) {
-    const int o = __shfl_up(s, m, MSPR_WAVE);
-    if (lane >= m) s = sat_add(s, o);
+  for (int k = 0; k < N; k++) {
+    s[k] = wave_scan(v[k]);
+    if ((threadIdx.x & 63) == 63) wave_sums[wave][k] = s[k];
   }
-  if (lane == 63) wave_sums[wave] = s;
   __syncthreads();
-  int before = 0;
-  total = 0;
 #pragma unroll
-  for (int w = 0; w < THREADS / MSPR_WAVE; w++) {
-    if (w == wave) before = total;
-    total = sat_add(total, wave_sums[w]);
+  for (int k = 0; k < N; k++) {
+    uint32_t all = 0, before = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+      if (w == wave) before = all;
+      all = sat_add(all, wave_sums[w][k]);
+    }
+    v[k] = sat_add(before, s[k] - v[k]);  // (a sum that is cut off counts for nothing: rows end at n_rows, far below)
+    total[k] = all > 0x7FFFFFFFu ? 0x7FFFFFFF : (int)all;
   }
-  const int up = __shfl_up(s, 1, MSPR_WAVE);
-  return sat_add(before, lane == 0 ? 0 : up);
 }
 
 // The last index in [0, n) whose sum is at most x (sums ascend, sums[0] = 0).
@@ -73,11 +87,11 @@ __device__ __forceinline__ int last_at_most(const int* sums, int n, int x) {
   return lo;
 }
 
-// grid: workgroups that share rows and returned pages; LDS: five arrays of `batch` integers
-template <int THREADS, int ITEMS>
-__global__ __launch_bounds__(THREADS) void page_step_kernel(StepArgs a) {
+// grid: workgroups that share rows and returned pages; LDS: five arrays of `batch` integers. ITEMS requests a thread.
+template <int ITEMS>
+__global__ __launch_bounds__(kThreads) void page_step_kernel(StepArgs a) {
   extern __shared__ int lds[];
-  __shared__ int wave_sums[3][THREADS / MSPR_WAVE];
+  __shared__ uint32_t wave_sums[3][kWaves][2];
   const int tid = threadIdx.x;
   const int B = a.batch;
   int* s_start = lds;           // first row
@@ -89,7 +103,6 @@ __global__ __launch_bounds__(THREADS) void page_step_kernel(StepArgs a) {
   const int cap = a.width << a.page_shift;
 
   int old_[ITEMS], add_[ITEMS];
-  int rows = 0;
 #pragma unroll
   for (int i = 0; i < ITEMS; i++) {
     const int b = tid * ITEMS + i;
@@ -98,31 +111,34 @@ __global__ __launch_bounds__(THREADS) void page_step_kernel(StepArgs a) {
   }
   int head = *a.head;
   head = head < 0 ? 0 : head > a.n_pages ? a.n_pages : head;
+  uint32_t rows[1] = {0};
 #pragma unroll
   for (int i = 0; i < ITEMS; i++) {
     old_[i] = old_[i] < 0 ? 0 : old_[i] > cap ? cap : old_[i];
-    rows = sat_add(rows, add_[i] > 0 ? add_[i] : 0);
+    rows[0] = sat_add(rows[0], add_[i] > 0 ? add_[i] : 0);
   }
-  int all_rows, all_need, all_back;
-  int start = block_scan<THREADS>(rows, wave_sums[0], all_rows);
+  int all_rows;
+  block_scan<1>(rows, reinterpret_cast<uint32_t(*)[1]>(wave_sums[0]), &all_rows);
   // rows behind n_rows are not part of the step: what a request may add ends there, and at its table's end
-  int start_[ITEMS], goal_[ITEMS], need = 0, back = 0;
+  int start_[ITEMS], goal_[ITEMS];
+  uint32_t pages[2] = {0, 0};  // needed, given back
 #pragma unroll
   for (int i = 0; i < ITEMS; i++) {
     const int asked = add_[i] > 0 ? add_[i] : 0;
-    start_[i] = start < a.n_rows ? start : a.n_rows;
-    const int room = a.n_rows - start_[i];
-    goal_[i] = old_[i] + min(min(asked, room), cap - old_[i]);
-    start = sat_add(start, asked);
+    start_[i] = rows[0] < (uint32_t)a.n_rows ? (int)rows[0] : a.n_rows;
+    goal_[i] = old_[i] + min(min(asked, a.n_rows - start_[i]), cap - old_[i]);
+    rows[0] = sat_add(rows[0], asked);
     const int held = (old_[i] + page - 1) >> a.page_shift;
-    if (add_[i] < 0) back += held;
-    else need += ((goal_[i] + page - 1) >> a.page_shift) - held;
+    if (add_[i] < 0) pages[1] += held;
+    else pages[0] += ((goal_[i] + page - 1) >> a.page_shift) - held;
   }
-  int first = block_scan<THREADS>(need, wave_sums[1], all_need);
-  int given = block_scan<THREADS>(back, wave_sums[2], all_back);
+  int all_pages[2];
+  block_scan<2>(pages, wave_sums[1], all_pages);
+  const int all_need = all_pages[0], all_back = all_pages[1];
+  int first = (int)pages[0], given = (int)pages[1];
   const int base = head - all_back;  // the stack's new top, before pages are taken (below 0 only if pages were lent twice)
   const int avail = a.n_pages - base;
-  int placed = 0;
+  uint32_t placed[1] = {0};
 #pragma unroll
   for (int i = 0; i < ITEMS; i++) {
     const int b = tid * ITEMS + i;
@@ -140,7 +156,7 @@ __global__ __launch_bounds__(THREADS) void page_step_kernel(StepArgs a) {
       if (blockIdx.x == 0) {
         a.lens_out[b] = len;
         a.starts[b] = start_[i];
-        if (!ended) placed += len - old_[i];
+        if (!ended) placed[0] += len - old_[i];
       }
     }
     first += want;
@@ -149,7 +165,7 @@ __global__ __launch_bounds__(THREADS) void page_step_kernel(StepArgs a) {
   __syncthreads();
   if (blockIdx.x == 0) {
     int all_placed;
-    block_scan<THREADS>(placed, wave_sums[0], all_placed);
+    block_scan<1>(placed, reinterpret_cast<uint32_t(*)[1]>(wave_sums[2]), &all_placed);
     if (tid == 0) {
       const int taken = max(0, min(all_need, avail));
       const int top = base + taken;
@@ -162,13 +178,13 @@ __global__ __launch_bounds__(THREADS) void page_step_kernel(StepArgs a) {
     }
   }
 
-  const int stride = gridDim.x * THREADS;
-  for (int k = blockIdx.x * THREADS + tid; k < all_back; k += stride) {
+  const int stride = gridDim.x * kThreads;
+  for (int k = blockIdx.x * kThreads + tid; k < all_back; k += stride) {
     const int b = last_at_most(s_back, B, k);
     const int at = base + k;
     if (at >= 0) a.free_pages[at] = a.tables[(int64_t)b * a.width + (k - s_back[b])];
   }
-  for (int t = blockIdx.x * THREADS + tid; t < a.n_rows; t += stride) {
+  for (int t = blockIdx.x * kThreads + tid; t < a.n_rows; t += stride) {
     int slot = -1, position = 0, request = -1;
     if (t < all_rows) {
       const int b = last_at_most(s_start, B, t);
@@ -201,13 +217,15 @@ __global__ __launch_bounds__(THREADS) void page_step_kernel(StepArgs a) {
   }
 }
 
-template <int THREADS, int ITEMS>
+template <int ITEMS>
 int step_launch(const StepArgs& a, hipStream_t st) {
-  // one row a thread, and no more workgroups than a row each of 64 keeps busy: each makes the sums
-  int grid = (a.n_rows + THREADS - 1) / THREADS;
-  grid = grid < 1 ? 1 : grid > 64 ? 64 : grid;
+  // A row a thread; pages given back, of which the host knows no number, get a workgroup per sixteen requests. Each workgroup
+  // makes the sums, so there are no more of them than half the compute units.
+  const int for_rows = (a.n_rows + kThreads - 1) / kThreads, for_pages = (a.batch + 15) / 16;
+  const int most = for_rows > for_pages ? for_rows : for_pages;
+  const int grid = most < 1 ? 1 : most > 128 ? 128 : most;
   const int bytes = 5 * a.batch * (int)sizeof(int);
-  page_step_kernel<THREADS, ITEMS><<<dim3(grid), dim3(THREADS), bytes, st>>>(a);
+  page_step_kernel<ITEMS><<<dim3(grid), dim3(kThreads), bytes, st>>>(a);
   MSPR_CHECK_LAUNCH("page_step");
   return MSPR_OK;
 }
@@ -232,7 +250,8 @@ extern "C" int mspr_page_step(const int32_t* lens, const int32_t* new_lens, int3
   const StepArgs a{lens, new_lens, tables, free_pages, head, batch, table_width, n_pages, __builtin_ctz(page_size), n_rows,
                    lens_out, head_out, starts, slots, positions, visible, requests, counts};
   hipStream_t st = (hipStream_t)stream;
-  if (batch <= 256) return step_launch<256, 1>(a, st);
-  if (batch <= 1024) return step_launch<1024, 1>(a, st);
-  return step_launch<1024, 2>(a, st);
+  if (batch <= 256) return step_launch<1>(a, st);
+  if (batch <= 512) return step_launch<2>(a, st);
+  if (batch <= 1024) return step_launch<4>(a, st);
+  return step_launch<8>(a, st);
 }

@@ -67,7 +67,7 @@ def page_step(lens, new_lens, tables, free_pages, head, *, page_size: int, n_row
     """
     done = _lib.dispatch.page_step(lens, new_lens, tables, free_pages, head, page_size, n_rows)
     if done is not None:
-        return PageStep(*done)
+        return tuple.__new__(PageStep, done)
     page_size, n_rows = int(page_size), int(n_rows)
     _check_page_size(page_size)
     if lens.ndim != 1 or tables.ndim != 2 or free_pages.ndim != 1:
