@@ -7,9 +7,12 @@
 // frequencies left (axis 1: 3 i' + 1 < 3 n_1, axis 2: 3 i' + 2 < 3 n_2), else axis 0. The angle is the exact product, reduced to
 // a turn in 64 bits: a float32 product is off by 2^-24 of it, 0.007 radians at position 120000, which no later step makes good.
 //
-// Bound by HBM: every element is read and written once. Half a wave owns a head's row (a lane eight neighbouring channels,
-// so that a 16-bit row is one 16-byte load a lane), the sum of squares is five lane exchanges, the partner of a channel
-// eight more. The cosines and sines of a workgroup's tokens are made once, a thread each, and shared through LDS.
+// Bound by HBM: every element is read and written once. A lane owns 16 bytes of a head's row, so that a load or store of a wave
+// is whole rows (with 32 bytes of a float32 row a lane, every line was asked for twice), the sum of squares is five or six lane
+// exchanges, the partner of a channel one more. A wave takes neighbouring heads of one kind, so that whose row it is and where
+// it lies is scalar arithmetic, and asks for its next rows before it works on these. Loads are non-temporal, as nothing reads
+// the projections' output again (16384 tokens of bfloat16 rows, appended: 56 us, 6.0 TB/s, instead of 67). The cosines and sines of a workgroup's tokens are made once, a thread each, under the first rows'
+// loads, and shared through LDS.
 #include "affine_q8.h"
 #include "common.h"
 
@@ -17,8 +20,13 @@ namespace {
 
 constexpr int kD = 256;
 constexpr int kThreads = 256;
-constexpr int kRowLanes = 32;
-constexpr int kRowsAtOnce = kThreads / kRowLanes;
+// a lane's channels of a row, the lanes of a row, the rows of a wave
+template <int DT>
+constexpr int kChannels = DT == MSPR_F32 ? 4 : 8;
+template <int DT>
+constexpr int kRowLanes = kD / kChannels<DT>;
+template <int DT>
+constexpr int kRows = MSPR_WAVE / kRowLanes<DT>;
 constexpr int kMaxTokens = 8;  // tokens a workgroup
 constexpr int kMaxHalf = kD / 2;
 
@@ -35,8 +43,7 @@ struct RopeArgs {
   const float* inv_freq;
   const int32_t* slots;
   int n_tokens, n_q, n_kv, half, axes, sec1, sec2;
-  int tokens_per_wg, rows_per_wg;
-  uint32_t rows_inverse;  // of the rows of a token that a workgroup takes
+  int tokens_per_wg, groups_per_wg;
   float eps;
   int page_shift, n_pages;
   void *q_out, *k_out;      // dense [n_tokens][heads][256]; k_out: pages in the paged forms
@@ -44,21 +51,20 @@ struct RopeArgs {
   void *k_scales, *k_biases, *v_scales, *v_biases;
 };
 
+// A lane's channels as they lie in memory.
 template <int DT>
-__device__ __forceinline__ void load8(const void* p, int64_t i, float* x) {
-  if constexpr (DT == MSPR_F32) {
-    const f32x4_t* s = reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(p) + i);
-    const f32x4_t a = s[0], b = s[1];
+struct Raw {
+  u32x4_t w;
+  __device__ __forceinline__ void load(const void* p, int64_t i) {
+    w = __builtin_nontemporal_load(
+        reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint8_t*>(p) + i * (DT == MSPR_F32 ? 4 : 2)));
+  }
+  __device__ __forceinline__ void widen(float* x) const {
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      x[j] = a[j];
-      x[4 + j] = b[j];
-    }
-  } else {
-    const u32x4_t w = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint16_t*>(p) + i);
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      if constexpr (DT == MSPR_F16) {
+      if constexpr (DT == MSPR_F32) {
+        x[j] = __uint_as_float(w[j]);
+      } else if constexpr (DT == MSPR_F16) {
         x[2 * j] = f16_bits_to_f32((uint16_t)(w[j] & 0xFFFFu));
         x[2 * j + 1] = f16_bits_to_f32((uint16_t)(w[j] >> 16));
       } else {
@@ -67,31 +73,39 @@ __device__ __forceinline__ void load8(const void* p, int64_t i, float* x) {
       }
     }
   }
-}
+};
 
 template <int DT>
 __device__ __forceinline__ uint16_t bits16(float v) {
   if constexpr (DT == MSPR_F16) return f32_to_f16_bits(v);
-  else return f32_to_bf16_bits(v);
+  else return __builtin_bit_cast(uint16_t, (__bf16)v);
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pair16(float a, float b) {
+  if constexpr (DT == MSPR_BF16) return __builtin_bit_cast(uint32_t, bf16x2_t{(__bf16)a, (__bf16)b});  // one instruction
+  else return (uint32_t)bits16<DT>(a) | ((uint32_t)bits16<DT>(b) << 16);
 }
 
 template <int DT>
 __device__ __forceinline__ float rounded(float v) {
   if constexpr (DT == MSPR_F32) return v;
   else if constexpr (DT == MSPR_F16) return f16_bits_to_f32(f32_to_f16_bits(v));
-  else return bf16_bits_to_f32(f32_to_bf16_bits(v));
+  else return (float)(__bf16)v;
 }
 
-template <int DT>
-__device__ __forceinline__ void store8(void* p, int64_t i, const float* x) {
+// N channels of type DT.
+template <int DT, int N>
+__device__ __forceinline__ void store_row(void* p, int64_t i, const float* x) {
   if constexpr (DT == MSPR_F32) {
-    f32x4_t* d = reinterpret_cast<f32x4_t*>(reinterpret_cast<float*>(p) + i);
-    d[0] = f32x4_t{x[0], x[1], x[2], x[3]};
-    d[1] = f32x4_t{x[4], x[5], x[6], x[7]};
+    static_assert(N == 4, "16 bytes");
+    *reinterpret_cast<f32x4_t*>(reinterpret_cast<float*>(p) + i) = f32x4_t{x[0], x[1], x[2], x[3]};
+  } else if constexpr (N == 4) {
+    *reinterpret_cast<u32x2_t*>(reinterpret_cast<uint16_t*>(p) + i) = u32x2_t{pair16<DT>(x[0], x[1]), pair16<DT>(x[2], x[3])};
   } else {
     u32x4_t w;
 #pragma unroll
-    for (int j = 0; j < 4; j++) w[j] = (uint32_t)bits16<DT>(x[2 * j]) | ((uint32_t)bits16<DT>(x[2 * j + 1]) << 16);
+    for (int j = 0; j < 4; j++) w[j] = pair16<DT>(x[2 * j], x[2 * j + 1]);
     *reinterpret_cast<u32x4_t*>(reinterpret_cast<uint16_t*>(p) + i) = w;
   }
 }
@@ -102,18 +116,19 @@ __device__ __forceinline__ void store1(void* p, int64_t i, float v) {
   else reinterpret_cast<uint16_t*>(p)[i] = bits16<DT>(v);
 }
 
-// A row to its page: 16-bit channels, or codes with a scale and bias of the row's type per 64 channels (eight lanes).
+// A row to its page: 16-bit channels, or codes with a scale and bias of the row's type per 64 channels.
 template <int DT, int KEEP, int PT>
 __device__ __forceinline__ void keep_row(void* out, void* scales, void* biases, int64_t row, int lane, const float* y) {
+  constexpr int N = kChannels<DT>;
   if constexpr (KEEP == kPages) {
-    store8<PT>(out, row * kD + 8 * lane, y);
+    store_row<PT, N>(out, row * kD + N * lane, y);
   } else {
-    float x[8];
+    float x[N];
 #pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = rounded<DT>(y[j]);  // (codes of the row as a dense tensor of its type would hold it)
+    for (int j = 0; j < N; j++) x[j] = rounded<DT>(y[j]);  // (codes of the row as a dense tensor of its type would hold it)
     float mn = x[0], mx = x[0];
 #pragma unroll
-    for (int j = 1; j < 8; j++) {
+    for (int j = 1; j < N; j++) {
       mn = fminf(mn, x[j]);
       mx = fmaxf(mx, x[j]);
     }
@@ -123,33 +138,76 @@ __device__ __forceinline__ void keep_row(void* out, void* scales, void* biases, 
     mx = fmaxf(mx, lane_xor<2>(mx));
     mn = fminf(mn, lane_xor<4>(mn));
     mx = fmaxf(mx, lane_xor<4>(mx));
+    if constexpr (N == 4) {
+      mn = fminf(mn, lane_xor<8>(mn));
+      mx = fmaxf(mx, lane_xor<8>(mx));
+    }
     float scale, bias;
     affine_q8_scale(mn, mx, scale, bias);
-    u32x2_t w = {0u, 0u};
+    uint32_t w[N / 4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      w.x |= affine_q8_code(x[j], scale, bias) << (8 * j);
-      w.y |= affine_q8_code(x[4 + j], scale, bias) << (8 * j);
+    for (int k = 0; k < N / 4; k++) {
+      w[k] = 0;
+#pragma unroll
+      for (int j = 0; j < 4; j++) w[k] |= affine_q8_code(x[4 * k + j], scale, bias) << (8 * j);
     }
-    reinterpret_cast<u32x2_t*>(out)[row * (kD / 8) + lane] = w;
-    if ((lane & 7) == 0) {
-      store1<DT>(scales, row * (kD / 64) + (lane >> 3), scale);
-      store1<DT>(biases, row * (kD / 64) + (lane >> 3), bias);
+    uint32_t* codes = reinterpret_cast<uint32_t*>(out) + row * (kD / 4) + lane * (N / 4);
+    if constexpr (N == 8) *reinterpret_cast<u32x2_t*>(codes) = u32x2_t{w[0], w[1]};
+    else *codes = w[0];
+    if (lane % (64 / N) == 0) {
+      store1<DT>(scales, row * (kD / 64) + lane / (64 / N), scale);
+      store1<DT>(biases, row * (kD / 64) + lane / (64 / N), bias);
     }
   }
 }
 
-// grid: (tokens / tokens_per_wg, rows of a token / rows_per_wg); a token's rows are its query heads, its key heads and, where
-// they are kept, its value heads
+// grid: (tokens / tokens_per_wg, groups of a token / groups_per_wg); a token's groups are a wave's rows each of its query heads,
+// its key heads and, where they are kept, its value heads (a kind whose heads are not a multiple of them ends with part of one)
 template <int DT, int KEEP, int PT>
 __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(RopeArgs a) {
-  __shared__ f32x2_t turn[kMaxTokens * kMaxHalf];  // cosine and sine
+  constexpr int N = kChannels<DT>, R = kRows<DT>;
+  __shared__ __attribute__((aligned(16))) f32x2_t turn[kMaxTokens * 2 * kMaxHalf];  // [token][lower, upper half][cosine, sine]
   const int tid = threadIdx.x;
-  const int lane = tid & (kRowLanes - 1);
+  const int lane = tid % kRowLanes<DT>;
+  const int mine = tid % MSPR_WAVE / kRowLanes<DT>;  // row of the group
+  const int wave = __builtin_amdgcn_readfirstlane(tid / MSPR_WAVE);
   const int t0 = blockIdx.x * a.tokens_per_wg;
   const int tokens = min(a.tokens_per_wg, a.n_tokens - t0);
-  const int row0 = blockIdx.y * a.rows_per_wg;
-  const int all_rows = a.n_q + (KEEP == kDense ? 1 : 2) * a.n_kv;
+  const int q_groups = (a.n_q + R - 1) / R, kv_groups = (a.n_kv + R - 1) / R;
+  const int group0 = blockIdx.y * a.groups_per_wg;
+  const int groups = min(a.groups_per_wg, q_groups + (KEEP == kDense ? 1 : 2) * kv_groups - group0);
+
+  const int64_t q_lane = mine * a.q_head + N * lane, k_lane = mine * a.k_head + N * lane, v_lane = mine * a.v_head + N * lane;
+  // A wave's items are those of number wave, wave + 4, ... in the order token by token.
+  struct Item {
+    int t, group;
+  };
+  auto next = [&](Item& i, int by) {
+    i.group += by;
+    while (i.group >= groups) {
+      i.group -= groups;
+      i.t++;
+    }
+  };
+  auto load = [&](const Item& i, Raw<DT>& raw) {
+    const int64_t token = t0 + i.t;
+    const int group = group0 + i.group;
+    if (group < q_groups) {
+      if (R * group + mine < a.n_q) raw.load(a.q, token * a.q_token + R * group * a.q_head + q_lane);
+    } else if (group < q_groups + kv_groups) {
+      const int head = R * (group - q_groups);
+      if (head + mine < a.n_kv) raw.load(a.k, token * a.k_token + head * a.k_head + k_lane);
+    } else if constexpr (KEEP != kDense) {
+      const int head = R * (group - q_groups - kv_groups);
+      if (head + mine < a.n_kv) raw.load(a.v, token * a.v_token + head * a.v_head + v_lane);
+    }
+  };
+  Item item = {0, 0};
+  next(item, wave);
+  Raw<DT> raw, qw, kw;
+  if (item.t < tokens) load(item, raw);
+  qw.load(a.q_weight, N * lane);
+  kw.load(a.k_weight, N * lane);
 
   for (int i = tid; i < tokens * a.half; i += kThreads) {
     const int t = i / a.half;
@@ -161,77 +219,95 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(RopeArgs a) {
     turns -= rint(turns);
     float s, c;
     sincospif(2.0f * (float)turns, &s, &c);
-    turn[i] = f32x2_t{c, s};
+    turn[2 * t * a.half + f] = f32x2_t{c, -s};
+    turn[(2 * t + 1) * a.half + f] = f32x2_t{c, s};
   }
   __syncthreads();
 
-  const int span = a.half / 8;  // lanes of half the rotary width
+  const int span = a.half / N;  // lanes of half the rotary width
   const bool low = lane < span, rotary = lane < 2 * span;
   const int partner = low ? lane + span : lane - span;
-  for (int item = tid / kRowLanes; item < tokens * a.rows_per_wg; item += kRowsAtOnce) {
-    const int t = mspr_div(item, a.rows_per_wg, a.rows_inverse);
-    const int row = row0 + item - t * a.rows_per_wg;
-    if (row >= all_rows) continue;
-    const int64_t token = t0 + t;
-    const bool is_q = row < a.n_q;
-    const bool is_v = KEEP != kDense && row >= a.n_q + a.n_kv;
-    const int head = is_q ? row : is_v ? row - a.n_q - a.n_kv : row - a.n_q;
+  auto process = [&](const Item& here, const Raw<DT>& raw) {
+    const int64_t token = t0 + here.t;
+    const int group = group0 + here.group;
+    const bool is_q = group < q_groups;
+    const bool is_v = KEEP != kDense && group >= q_groups + kv_groups;
+    const int head = R * (is_q ? group : is_v ? group - q_groups - kv_groups : group - q_groups) + mine;
     int64_t at = 0;  // row in the pages
     if constexpr (KEEP != kDense) {
       if (!is_q) {
         const int slot = a.slots[token];
         const int page = slot >> a.page_shift;
-        if (slot < 0 || page >= a.n_pages) continue;
+        if (slot < 0 || page >= a.n_pages) return;
         at = (((int64_t)page * a.n_kv + head) << a.page_shift) + (slot & ((1 << a.page_shift) - 1));
       }
     }
-    float x[8];
-    if (is_v) {
-      load8<DT>(a.v, token * a.v_token + head * a.v_head + 8 * lane, x);
-      if constexpr (KEEP != kDense) keep_row<DT, KEEP, PT>(a.v_out, a.v_scales, a.v_biases, at, lane, x);
-      continue;
-    }
-    load8<DT>(is_q ? a.q : a.k, is_q ? token * a.q_token + head * a.q_head + 8 * lane : token * a.k_token + head * a.k_head + 8 * lane, x);
-    float w[8];
-    load8<DT>(is_q ? a.q_weight : a.k_weight, 8 * lane, w);
-    float ss = 0.0f;
+    if (head >= (is_q ? a.n_q : a.n_kv)) return;
+    float x[N];
+    raw.widen(x);
+    if (!is_v) {
+      float w[N];
+      if (is_q) qw.widen(w);
+      else kw.widen(w);
+      float ss = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) ss += x[j] * x[j];
-    ss += lane_xor<1>(ss);
-    ss += lane_xor<2>(ss);
-    ss += lane_xor<4>(ss);
-    ss += lane_xor<8>(ss);
-    ss += lane_xor<16>(ss);
-    const float r = 1.0f / sqrtf(ss * (1.0f / kD) + a.eps);
+      for (int j = 0; j < N; j++) ss += x[j] * x[j];
+      ss += lane_xor<1>(ss);
+      ss += lane_xor<2>(ss);
+      ss += lane_xor<4>(ss);
+      ss += lane_xor<8>(ss);
+      ss += lane_xor<16>(ss);
+      if constexpr (N == 4) ss = half_wave_sum(ss);
+      const float r = __builtin_amdgcn_rsqf(ss * (1.0f / kD) + a.eps);  // (off by a unit of its last place at most)
 #pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = x[j] * r * w[j];
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const float other = __shfl(x[j], partner, kRowLanes);
+      for (int j = 0; j < N; j++) x[j] = x[j] * r * w[j];
       if (rotary) {
-        const f32x2_t cs = turn[t * a.half + 8 * (low ? lane : partner) + j];
-        x[j] = x[j] * cs.x + (low ? -other : other) * cs.y;
+        const f32x4_t* cs = reinterpret_cast<const f32x4_t*>(turn + (2 * here.t + (low ? 0 : 1)) * a.half + N * (low ? lane : partner));
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+          const f32x4_t c = cs[j / 2];
+          const float o0 = __shfl(x[j], partner, kRowLanes<DT>), o1 = __shfl(x[j + 1], partner, kRowLanes<DT>);
+          x[j] = x[j] * c.x + o0 * c.y;
+          x[j + 1] = x[j + 1] * c.z + o1 * c.w;
+        }
       }
     }
     if (is_q) {
-      store8<DT>(a.q_out, (token * a.n_q + head) * kD + 8 * lane, x);
+      store_row<DT, N>(a.q_out, (token * a.n_q + head) * kD + N * lane, x);
     } else if constexpr (KEEP == kDense) {
-      store8<DT>(a.k_out, (token * a.n_kv + head) * kD + 8 * lane, x);
+      store_row<DT, N>(a.k_out, (token * a.n_kv + head) * kD + N * lane, x);
     } else {
-      keep_row<DT, KEEP, PT>(a.k_out, a.k_scales, a.k_biases, at, lane, x);
+      keep_row<DT, KEEP, PT>(is_v ? a.v_out : a.k_out, is_v ? a.v_scales : a.k_scales, is_v ? a.v_biases : a.k_biases, at, lane, x);
     }
+  };
+  // (two sets of registers in turn: a copy from one to the other would wait for its load)
+  while (item.t < tokens) {
+    Item here = item;
+    Raw<DT> other;
+    next(item, kThreads / MSPR_WAVE);
+    if (item.t < tokens) load(item, other);
+    process(here, raw);
+    if (item.t >= tokens) break;
+    here = item;
+    next(item, kThreads / MSPR_WAVE);
+    if (item.t < tokens) load(item, raw);
+    process(here, other);
   }
 }
 
 template <int DT, int KEEP, int PT>
 int rope_launch(RopeArgs a, hipStream_t st) {
-  const int rows = a.n_q + (KEEP == kDense ? 1 : 2) * a.n_kv;
-  // eight tokens a workgroup share the angles' cost; few tokens are spread a pass of rows a workgroup, for latency
-  a.tokens_per_wg = a.n_tokens >= 2048 ? kMaxTokens : 1;
-  a.rows_per_wg = a.n_tokens >= 256 ? rows : kRowsAtOnce;
-  a.rows_inverse = mspr_inverse(a.rows_per_wg);
+  constexpr int R = kRows<DT>;
+  const int groups = (a.n_q + R - 1) / R + (KEEP == kDense ? 1 : 2) * ((a.n_kv + R - 1) / R);
+  // Few rows: a group a wave, for latency, while the chip holds all of them at once. Many: a token's groups together, and up to
+  // eight tokens, which share the angles' cost, where eight workgroups a compute unit are left (3844 tokens of float32 rows, in
+  // workgroups of seven tokens each: 50 us, of one: 27; 16384 tokens of bfloat16 rows: 56 either way).
+  const bool few = (int64_t)a.n_tokens * groups <= 8192;
+  const int share = a.n_tokens / 2048;
+  a.tokens_per_wg = few || share < 1 ? 1 : share > kMaxTokens ? kMaxTokens : share;
+  a.groups_per_wg = few ? kThreads / MSPR_WAVE : groups;
   const dim3 grid((unsigned)((a.n_tokens + a.tokens_per_wg - 1) / a.tokens_per_wg),
-                  (unsigned)((rows + a.rows_per_wg - 1) / a.rows_per_wg));
+                  (unsigned)((groups + a.groups_per_wg - 1) / a.groups_per_wg));
   qk_norm_rope_kernel<DT, KEEP, PT><<<grid, dim3(kThreads), 0, st>>>(a);
   MSPR_CHECK_LAUNCH("qk_norm_rope");
   return MSPR_OK;
