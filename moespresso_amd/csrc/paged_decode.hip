@@ -26,7 +26,8 @@
 // as the whole numbers they are. A group's sum over K then takes its scale in float32; a group's scale of V goes into the
 // weights first; biases are products of their own, of float32 matrix instructions (K: biases x sums of the query over a
 // group, V: weights x biases). Weights, and queries whose type has more digits than an operand, go in as two terms of it,
-// the rounded value and the rounded rest (for 8-bit rows and bfloat16 results one: float16 keeps three digits more than they).
+// the rounded value and the rounded rest (8-bit rows: one for bfloat16 results, which float16 has three digits more than,
+// three for float32 results).
 #include "common.h"
 #include "q8_codes.h"
 
@@ -149,6 +150,20 @@ __device__ __forceinline__ void widen8(u32x4_t w, float* x) {
   }
 }
 
+// Sixteen codes to bfloat16, exactly (whole numbers up to 256 are): the upper halves of their float32 values.
+__device__ __forceinline__ void codes_to_bf16(u32x4_t c, u32x4_t& lo, u32x4_t& hi) {
+  uint32_t o[8];
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    const float b0 = (float)(c[w] & 0xFFu), b1 = (float)((c[w] >> 8) & 0xFFu), b2 = (float)((c[w] >> 16) & 0xFFu),
+                b3 = (float)(c[w] >> 24);
+    o[2 * w] = __builtin_amdgcn_perm(__float_as_uint(b1), __float_as_uint(b0), 0x07060302u);
+    o[2 * w + 1] = __builtin_amdgcn_perm(__float_as_uint(b3), __float_as_uint(b2), 0x07060302u);
+  }
+  lo = u32x4_t{o[0], o[1], o[2], o[3]};
+  hi = u32x4_t{o[4], o[5], o[6], o[7]};
+}
+
 // One scale or bias a lane, number i of a window. 16-bit ones are loaded with their neighbour, a word: what is done to them behind
 // the load (a load of 16 bits is masked) is done, and waited for, a tile too early.
 template <int SDT>
@@ -206,8 +221,11 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
                                                                       int page_shift, int n_pages, int rep, PagedRest a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   constexpr bool kCodes = FMT == kAffine;
-  constexpr int kVType = kCodes ? MSPR_F16 : FMT;                  // operands of the second product
-  constexpr int kPTerms = kCodes && QDT == MSPR_BF16 ? 1 : 2;      // terms of a weight
+  // Operands of the second product: of 8-bit rows float16, in which the codes cost fewest instructions and a term of a weight has
+  // eleven digits; float32 results want weights without a floor (the rest of a float16 term ends at 2^-25: 1.2e-5 of a result
+  // over 37000 keys), so theirs are three terms of bfloat16 (1.4e-6).
+  constexpr int kVType = !kCodes ? FMT : QDT == MSPR_F32 ? MSPR_BF16 : MSPR_F16;
+  constexpr int kPTerms = kCodes && QDT == MSPR_BF16 ? 1 : QDT == MSPR_F32 ? 3 : 2;  // terms of a weight
   constexpr int kQTerms = kCodes && QDT == MSPR_F32 ? 2 : 1;       // terms of a query element
   // float16 weights are taken 2^11 times as large: up to 2^15, as the reference maximum lags by 2^4 at most, and the smallest that
   // is not lost is 2^-35 of the largest (at 2^-24, the many small weights of a long context would all be rounded one way)
@@ -514,8 +532,9 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
           *reinterpret_cast<u32x4_t*>(vt + (16 * u + 2 * j + (lane >> 5)) * kVPitch + 16 * (lane & 31)) = vr[u][j];
         } else {
           u32x4_t lo, hi;
+          if constexpr (kVType == MSPR_BF16) codes_to_bf16(vr[u][j], lo, hi);
 #pragma unroll
-          for (int w = 0; w < 4; w++) {
+          for (int w = 0; w < 4 && kVType == MSPR_F16; w++) {
             h2_t c01, c23;
             codes4_to_h<kFmtAffine>(vr[u][j][w], c01, c23);
             (w < 2 ? lo : hi)[2 * (w & 1)] = h2_bits(c01);

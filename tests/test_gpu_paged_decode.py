@@ -4,7 +4,7 @@ Tolerance, from the arithmetic. A score is a float32 sum of 256 exact products a
 260 * 2^-24 * A, A = scale * sum |q| |k| at its largest over the keys (natural units; the same relative to the exponent's
 argument for its rounding). An error d of every score moves the result by at most 2 d of sum p |v|. A weight is two terms
 of a 16-bit type, each off by half a step of it (bfloat16 pages 2^-8 of 2^-8 of the weight, float16 operands 2^-11 of 2^-11), or
-one float16 term (8-bit pages, bfloat16 result: 2^-11); float16 operands are taken 2^11 times as large and end at 2^-25, so
+one float16 term (8-bit pages, bfloat16 result: 2^-11), or three bfloat16 terms (float32 result: 2^-24); float16 operands are taken 2^11 times as large and end at 2^-25, so
 that n weights lose at most n * 2^-36 of the largest value together (8-bit pages: of 255 times twice the largest scale). Sums
 over n keys run over n / 8 float32 additions at most, counted for both the weights' and the values' sums; the result is
 rounded once more, to eps / 2 of its type.
@@ -64,7 +64,7 @@ def _reference(q, keys, values, tables, lens, scale, requests=None):
     out, bound = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda")
     n_pages, G, page = (keys if torch.is_tensor(keys) else keys[0]).shape[:3]
     rep = q.shape[1] // G
-    terms = 2.0 ** (-16 if torch.is_tensor(keys) and q.dtype == BF16 else -11 if q.dtype == BF16 else -22)
+    terms = 2.0 ** (-16 if torch.is_tensor(keys) and q.dtype == BF16 else -11 if q.dtype == BF16 else -24 if q.dtype == F32 else -22)
     for r in range(q.shape[0]):
         b = r if requests is None else int(requests[r])
         n = min(max(int(lens[r]), 0), tables.shape[1] * page) if 0 <= b < len(tables) else 0
@@ -92,7 +92,7 @@ def _reference(q, keys, values, tables, lens, scale, requests=None):
                 c = (c.view(torch.uint8).double() * s.double().repeat_interleave(64, -1)).abs() + z.double().repeat_interleave(64, -1).abs()
                 most = (x.abs() @ c.reshape(-1, 256)[keep].t()).amax(-1, keepdim=True) * abs(scale)
             bound[r, g * rep:(g + 1) * rep] = size * (2 * 260 * 2.0 ** -24 * most + terms + 2 * (k.shape[0] / 8 + 8) * 2.0 ** -24)
-            if not (torch.is_tensor(keys) and q.dtype == BF16):
+            if q.dtype == F16 or q.dtype == BF16 and not torch.is_tensor(keys):
                 bound[r, g * rep:(g + 1) * rep] += k.shape[0] * 2.0 ** -36 * largest
     return out, bound
 
