@@ -41,7 +41,7 @@ constexpr int kWaves = 4;
 constexpr int kVPitch = kD * 2 + 16;  // bytes per key row of the V tile
 constexpr int kVTileBytes = kTileKeys * kVPitch;
 constexpr int kMaxShares = 256;    // workgroups: one a compute unit
-constexpr int kMinTiles = kWaves;  // a share gives every wave a tile, and no row of tiles counts for less
+constexpr int kMinTiles = 2;      // a share, and what a row counts for at least (four, a tile a wave: 1 request of 8191 rows 10.2 us, not 8.2)
 constexpr int kNonTemporal = 2;    // cache policy of loads that are used once
 
 constexpr int kAffine = 3;  // page format beside MSPR_F16 and MSPR_BF16

@@ -410,11 +410,14 @@ class PagedKVCache:
                                    sections=sections)
 
     def attend(self, queries, tables, lens, scale, *, requests=None, workspace=None):
-        """One query a request over these pages."""
+        """One query a request over these pages (float32 queries over 16-bit rows are rounded to the rows' type)."""
         if self.quantized:
             return sdpa_decode_paged_q8(queries, *self.keys, *self.values, tables, lens, scale, requests=requests,
                                         workspace=workspace)
-        return sdpa_decode_paged(queries, self.keys, self.values, tables, lens, scale, requests=requests, workspace=workspace)
+        if queries.dtype != torch.float32:
+            return sdpa_decode_paged(queries, self.keys, self.values, tables, lens, scale, requests=requests, workspace=workspace)
+        return sdpa_decode_paged(queries.to(self.keys.dtype), self.keys, self.values, tables, lens, scale, requests=requests,
+                                 workspace=workspace).float()
 
 
 class PagedAttention(torch.nn.Module):

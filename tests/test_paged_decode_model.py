@@ -6,7 +6,7 @@ import pytest
 
 from moespresso_amd import _lib
 
-TILE, WAVES, SHARES, MIN_TILES = 32, 4, 256, 4
+TILE, WAVES, SHARES, MIN_TILES = 32, 4, 256, 2
 
 
 def _row_tiles(n):
