@@ -71,7 +71,7 @@ __device__ __forceinline__ void block_scan(uint32_t* v, uint32_t (*wave_sums)[N]
       if (w == wave) before = all;
       all = sat_add(all, wave_sums[w][k]);
     }
-    v[k] = sat_add(before, s[k] - v[k]);  // (a sum that is cut off counts for nothing: rows end at n_rows, far below)
+    v[k] = sat_add(before, s[k] - v[k]);
     total[k] = all > 0x7FFFFFFFu ? 0x7FFFFFFF : (int)all;
   }
 }
@@ -117,6 +117,7 @@ __global__ __launch_bounds__(kThreads) void page_step_kernel(StepArgs a) {
     old_[i] = old_[i] < 0 ? 0 : old_[i] > cap ? cap : old_[i];
     rows[0] = sat_add(rows[0], add_[i] > 0 ? add_[i] : 0);
   }
+  rows[0] = min(rows[0], 0x7FFFFFFFu);  // (so that a sum that is cut off stays far above n_rows without this thread's)
   int all_rows;
   block_scan<1>(rows, reinterpret_cast<uint32_t(*)[1]>(wave_sums[0]), &all_rows);
   // rows behind n_rows are not part of the step: what a request may add ends there, and at its table's end

@@ -242,14 +242,30 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
   const int cap = width << page_shift;
   const int page_mask = (1 << page_shift) - 1;
 
-  // ---- the share: all tiles are added up, every workgroup for itself, lane i taking request i (and i + 64, ...)
-  const int len0 = length_of(lens, batch, lane, cap);
-  const int tiles0 = lane < batch ? tiles_of(len0) : 0;
-  const int sums0 = wave_scan(tiles0);
-  int all = __builtin_amdgcn_readlane(sums0, 63);
-  for (int b0 = MSPR_WAVE; b0 < batch; b0 += MSPR_WAVE) {
-    const int tiles = b0 + lane < batch ? tiles_of(length_of(lens, batch, b0 + lane, cap)) : 0;
-    all += __builtin_amdgcn_readlane(wave_scan(tiles), 63);
+  // ---- the share: every workgroup adds up all tiles for itself, a chunk of 64 queries a wave at a time
+  const int chunks = (batch + MSPR_WAVE - 1) / MSPR_WAVE;
+  int* chunk_sums = reinterpret_cast<int*>(lds);  // [chunks], where the V tiles will be
+  auto tiles_at = [&](int i, int& len) {
+    len = length_of(lens, batch, i, cap);
+    return i < batch ? tiles_of(len) : 0;
+  };
+  Place at = {0, 0, 0, 0};
+  int all = 0, chunk = 0, before = 0, len0, tiles0 = tiles_at(lane, len0);
+  int sums0 = wave_scan(tiles0);
+  int chunk_sum = 0, in_lanes = 0, per_lane = 1;  // (more than one chunk: lane i has the sum of `per_lane` of them, and those before)
+  if (chunks == 1) {
+    all = __builtin_amdgcn_readlane(sums0, 63);
+  } else {
+    for (int c = wave; c < chunks; c += kWaves) {
+      int len;
+      const int sum = wave_scan(tiles_at(c * MSPR_WAVE + lane, len));
+      if (lane == 63) chunk_sums[c] = sum;
+    }
+    __syncthreads();
+    per_lane = (chunks + MSPR_WAVE - 1) / MSPR_WAVE;
+    for (int c = lane * per_lane; c < min((lane + 1) * per_lane, chunks); c++) chunk_sum += chunk_sums[c];
+    in_lanes = wave_scan(chunk_sum);
+    all = __builtin_amdgcn_readlane(in_lanes, 63);
   }
   all *= n_kv;
   int share = (all + kMaxShares - 1) / kMaxShares;
@@ -259,437 +275,445 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
   const bool by_row = batch * n_kv <= kMaxShares;
   if (!by_row && threadIdx.x == 0) a.cut[3 * blockIdx.x] = -1;
   if (pos >= end) return;
-  Place at = {0, 0, 0, 0};
-  {
-    int before = 0, len = len0, tiles = tiles0, sums = sums0;
-    for (int b0 = 0;; b0 += MSPR_WAVE) {
-      const uint64_t beyond = __ballot((before + sums) * n_kv > pos);
-      if (beyond) {
-        const int i = __builtin_ctzll(beyond);
-        const int t = __builtin_amdgcn_readlane(tiles, i);
-        at.b = b0 + i;
-        at.len = __builtin_amdgcn_readlane(len, i);
-        at.tile = pos - (before + __builtin_amdgcn_readlane(sums, i) - t) * n_kv;
-        while (at.tile >= t) {  // (fewer times than there are KV heads)
-          at.tile -= t;
-          at.kvh++;
-        }
-        break;
-      }
-      before += __builtin_amdgcn_readlane(sums, 63);
-      if (b0 + MSPR_WAVE >= batch) return;  // (not reached: pos is below the total)
-      len = length_of(lens, batch, b0 + MSPR_WAVE + lane, cap);
-      tiles = b0 + MSPR_WAVE + lane < batch ? tiles_of(len) : 0;
-      sums = wave_scan(tiles);
+  // (Whose tile `pos` is: it is below the total, so that there is one. Lengths that another stream changes meanwhile may say
+  // otherwise: every loop ends and every index stays in its range all the same.)
+  auto first_beyond = [&](int sum) {
+    const uint64_t beyond = __ballot(sum * n_kv > pos);
+    return beyond ? __builtin_ctzll(beyond) : MSPR_WAVE - 1;
+  };
+  if (chunks > 1) {
+    const int i = first_beyond(in_lanes);
+    before = __builtin_amdgcn_readlane(in_lanes, i) - __builtin_amdgcn_readlane(chunk_sum, i);
+    for (chunk = min(i * per_lane, chunks - 1); chunk < chunks - 1; chunk++) {
+      const int sum = __builtin_amdgcn_readfirstlane(chunk_sums[chunk]);
+      if ((before + sum) * n_kv > pos) break;
+      before += sum;
     }
+    __syncthreads();  // (the sums' place is used again)
+    tiles0 = tiles_at(chunk * MSPR_WAVE + lane, len0);
+    sums0 = wave_scan(tiles0);
+  }
+  {
+    const int i = first_beyond(before + sums0);
+    const int t = __builtin_amdgcn_readlane(tiles0, i);
+    at.b = chunk * MSPR_WAVE + i;
+    at.len = __builtin_amdgcn_readlane(len0, i);
+    at.tile = pos - (before + __builtin_amdgcn_readlane(sums0, i) - t) * n_kv;
+    while (at.tile >= t && at.kvh < n_kv - 1) {
+      at.tile -= t;
+      at.kvh++;
+    }
+    if (at.b >= batch) return;
   }
 
   for (;;) {
-  const int row_tiles = tiles_of(at.len);
-  const int tile0 = at.tile;
-  const int tile1 = min(tile0 + (end - pos), row_tiles);
+    const int row_tiles = tiles_of(at.len);
+    const int tile0 = at.tile;
+    const int tile1 = min(tile0 + (end - pos), row_tiles);
 
-  // ---- the query is asked for first: loads come back in order, and the pages' addresses wait for the table anyway
-  const bool mine = n < rep;
-  u32x4_t qraw[QDT == MSPR_F32 ? 4 : 2];
-  {
-    const int64_t q0 = (((int64_t)at.b * n_kv + at.kvh) * rep + (mine ? n : 0)) * kD;
-    if constexpr (!kCodes) {  // steps 2 wave, 2 wave + 1: channels 32 step + 8 g on
-      const u32x4_t* p = reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint16_t*>(a.q) + q0 + 64 * wave + 8 * g);
-      qraw[0] = p[0];
-      qraw[1] = p[4];
-    } else {  // channels 64 wave + 16 g on
-      const u32x4_t* p = reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint8_t*>(a.q) +
-                                                          (q0 + 64 * wave + 16 * g) * (QDT == MSPR_F32 ? 4 : 2));
+    // ---- the query is asked for first: loads come back in order, and the pages' addresses wait for the table anyway
+    const bool mine = n < rep;
+    u32x4_t qraw[QDT == MSPR_F32 ? 4 : 2];
+    {
+      const int64_t q0 = (((int64_t)at.b * n_kv + at.kvh) * rep + (mine ? n : 0)) * kD;
+      if constexpr (!kCodes) {  // steps 2 wave, 2 wave + 1: channels 32 step + 8 g on
+        const u32x4_t* p = reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint16_t*>(a.q) + q0 + 64 * wave + 8 * g);
+        qraw[0] = p[0];
+        qraw[1] = p[4];
+      } else {  // channels 64 wave + 16 g on
+        const u32x4_t* p = reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint8_t*>(a.q) +
+                                                            (q0 + 64 * wave + 16 * g) * (QDT == MSPR_F32 ? 4 : 2));
 #pragma unroll
-      for (int j = 0; j < (QDT == MSPR_F32 ? 4 : 2); j++) qraw[j] = p[j];
-    }
-  }
-  __builtin_amdgcn_sched_barrier(0);
-
-  const int request = a.requests ? __builtin_amdgcn_readfirstlane(a.requests[at.b]) : at.b;
-  const bool known = request >= 0 && (!a.requests || request < a.n_tables);
-  const int len = known ? at.len : 0;
-  const int32_t* table = tables + (int64_t)(known ? request : 0) * width;
-  const int last_tile = min(tile1, (len + kTileKeys - 1) / kTileKeys);
-
-  f32x4_t oacc[16];
-#pragma unroll
-  for (int mt = 0; mt < 16; mt++) oacc[mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float m_run = -__builtin_inff(), l_run = 0.0f;
-  f32x4_t bacc = {0.f, 0.f, 0.f, 0.f};  // weighted biases: lane n (g = 0) has those of head n and the four groups
-  float v_unit = 0x1p-126f;             // what V's scales are multiples of: a power of two from their largest magnitude on
-
-  // Pages of this wave's tiles, two half tiles of 16 keys each (a page holds 16 rows or more): lane i of `ids` has the page
-  // of half tile i of 31 tiles and the one behind them, the next tiles' are on their way while these are used.
-  const int n_mine = last_tile - tile0 > wave ? (last_tile - tile0 - wave + kWaves - 1) / kWaves : 0;
-  auto load_ids = [&](int it0) {
-    const int it = it0 + (lane >> 1);
-    const int key = (tile0 + wave + kWaves * it) * kTileKeys + 16 * (lane & 1);
-    const int e = it < n_mine && key < len ? key >> page_shift : -1;
-    return e >= 0 ? table[e] : -1;
-  };
-
-  // A half tile: its page's rows, and how many of them count (none of a page that is not in the pool).
-  struct Half {
-    int64_t row;  // first row in the pages
-    int rows;
-  };
-  auto half_at = [&](int ids, int it0, int it, int u) {
-    const int key = (tile0 + wave + kWaves * it) * kTileKeys + 16 * u;
-    const int p = __builtin_amdgcn_readlane(ids, 2 * (it - it0) + u);
-    const bool good = p >= 0 && p < n_pages;
-    Half h;
-    h.row = ((((int64_t)(good ? p : 0) * n_kv + at.kvh) << page_shift) + (key & page_mask));
-    // (a scalar by hand: the compiler clamps with a vector instruction, and then takes the window for one of each lane's)
-    h.rows = __builtin_amdgcn_readfirstlane(!good || it >= n_mine ? 0 : len - key >= 16 ? 16 : len - key < 0 ? 0 : len - key);
-    return h;
-  };
-
-  constexpr int kKLoads = kCodes ? 4 : 8;   // 16-byte pieces a lane and half tile
-  constexpr int kVLoads = kCodes ? 4 : 8;
-  u32x4_t kr[2][kKLoads], vr[2][kVLoads];
-  RowScales<SDT> ks[2], kb[2], vs[2], vb[2];
-  auto load_k = [&](const Half* h) {
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-      const auto w = rows_window(k, h[u].row, kRowBytes, h[u].rows);
-#pragma unroll
-      for (int j = 0; j < kKLoads; j++) kr[u][j] = window_load16(w, n * kRowBytes + 16 * g, 64 * j);
-      if constexpr (kCodes) {
-        // (scales: row 4 g + n / 4, group n % 4, to be spread over a row's sixteen lanes; biases: row n, group g, an operand)
-        ks[u].load(rows_window(a.k_scales, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 16 * g + n);
-        kb[u].load(rows_window(a.k_biases, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 4 * n + g);
+        for (int j = 0; j < (QDT == MSPR_F32 ? 4 : 2); j++) qraw[j] = p[j];
       }
     }
-  };
-  auto load_v = [&](const Half* h) {
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-      const auto w = rows_window(v, h[u].row, kRowBytes, h[u].rows);
-#pragma unroll
-      for (int j = 0; j < kVLoads; j++) vr[u][j] = window_load16(w, 16 * lane, 1024 * j);
-    }
-  };
-  auto load_v_scales = [&](const Half* h) {
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-      vs[u].load(rows_window(a.v_scales, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 16 * g + n);
-      vb[u].load(rows_window(a.v_biases, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 16 * g + n);
-    }
-  };
+    __builtin_amdgcn_sched_barrier(0);
 
-  int ids = load_ids(0);
-  Half cur[2] = {half_at(ids, 0, 0, 0), half_at(ids, 0, 0, 1)}, nxt[2];
-  load_k(cur);
-  load_v(cur);
-  if constexpr (kCodes) load_v_scales(cur);
-  int ids_next = load_ids(31);
-  __builtin_amdgcn_sched_barrier(0);  // the first tile is on its way before the query is fetched
+    const int request = a.requests ? __builtin_amdgcn_readfirstlane(a.requests[at.b]) : at.b;
+    const bool known = request >= 0 && (!a.requests || request < a.n_tables);
+    const int len = known ? at.len : 0;
+    const int32_t* table = tables + (int64_t)(known ? request : 0) * width;
+    const int last_tile = min(tile1, (len + kTileKeys - 1) / kTileKeys);
 
-  // ---- Q^T operand, in LDS for all waves: lane (n = head, g) has the eight channels that the K operand has in its place
-  u32x4_t* qt = reinterpret_cast<u32x4_t*>(lds + kWaves * kVTileBytes) + lane;  // [8 steps][terms][64 lanes]
-  float q_unit = a.scale_log2;           // what a product's unit stands for, in powers of two
-  float qsum = 0.0f;                     // sum of the query's head n over group g
-  {
-    if constexpr (!kCodes) {
+    f32x4_t oacc[16];
 #pragma unroll
-      for (int h = 0; h < 2; h++) qt[64 * (2 * wave + h)] = mine ? qraw[h] : u32x4_t{0u, 0u, 0u, 0u};
-    } else {
-      float x[2][8];  // step 2 wave + h
-      float top = 0.0f;
+    for (int mt = 0; mt < 16; mt++) oacc[mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float m_run = -__builtin_inff(), l_run = 0.0f;
+    f32x4_t bacc = {0.f, 0.f, 0.f, 0.f};  // weighted biases: lane n (g = 0) has those of head n and the four groups
+    float v_unit = 0x1p-126f;             // what V's scales are multiples of: a power of two from their largest magnitude on
+
+    // Pages of this wave's tiles, two half tiles of 16 keys each (a page holds 16 rows or more): lane i of `ids` has the page
+    // of half tile i of 31 tiles and the one behind them, the next tiles' are on their way while these are used.
+    const int n_mine = last_tile - tile0 > wave ? (last_tile - tile0 - wave + kWaves - 1) / kWaves : 0;
+    auto load_ids = [&](int it0) {
+      const int it = it0 + (lane >> 1);
+      const int key = (tile0 + wave + kWaves * it) * kTileKeys + 16 * (lane & 1);
+      const int e = it < n_mine && key < len ? key >> page_shift : -1;
+      return e >= 0 ? table[e] : -1;
+    };
+
+    // A half tile: its page's rows, and how many of them count (none of a page that is not in the pool).
+    struct Half {
+      int64_t row;  // first row in the pages
+      int rows;
+    };
+    auto half_at = [&](int ids, int it0, int it, int u) {
+      const int key = (tile0 + wave + kWaves * it) * kTileKeys + 16 * u;
+      const int p = __builtin_amdgcn_readlane(ids, 2 * (it - it0) + u);
+      const bool good = p >= 0 && p < n_pages;
+      Half h;
+      h.row = ((((int64_t)(good ? p : 0) * n_kv + at.kvh) << page_shift) + (key & page_mask));
+      // (a scalar by hand: the compiler clamps with a vector instruction, and then takes the window for one of each lane's)
+      h.rows = __builtin_amdgcn_readfirstlane(!good || it >= n_mine ? 0 : len - key >= 16 ? 16 : len - key < 0 ? 0 : len - key);
+      return h;
+    };
+
+    constexpr int kKLoads = kCodes ? 4 : 8;   // 16-byte pieces a lane and half tile
+    constexpr int kVLoads = kCodes ? 4 : 8;
+    u32x4_t kr[2][kKLoads], vr[2][kVLoads];
+    RowScales<SDT> ks[2], kb[2], vs[2], vb[2];
+    auto load_k = [&](const Half* h) {
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        if constexpr (QDT == MSPR_F32) {
+      for (int u = 0; u < 2; u++) {
+        const auto w = rows_window(k, h[u].row, kRowBytes, h[u].rows);
 #pragma unroll
-          for (int j = 0; j < 8; j++) x[h][j] = __uint_as_float(qraw[2 * h + j / 4][j % 4]);
-        } else {
-          widen8<QDT>(qraw[h], x[h]);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          x[h][j] = mine ? x[h][j] : 0.0f;
-          top = fmaxf(top, fabsf(x[h][j]));
+        for (int j = 0; j < kKLoads; j++) kr[u][j] = window_load16(w, n * kRowBytes + 16 * g, 64 * j);
+        if constexpr (kCodes) {
+          // (scales: row 4 g + n / 4, group n % 4, to be spread over a row's sixteen lanes; biases: row n, group g, an operand)
+          ks[u].load(rows_window(a.k_scales, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 16 * g + n);
+          kb[u].load(rows_window(a.k_biases, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 4 * n + g);
         }
       }
-      // The operand is float16: a power of two brings the head's largest element to [1, 2), so that what falls below
-      // float16's range is 2^-25 of it; float16 queries go in as they are.
-      float* shared = reinterpret_cast<float*>(lds);  // [2][waves][16 heads], where the V tiles will be
-      int e = 0;
-      if constexpr (QDT != MSPR_F16) {
-        top = half_wave_max(row_pair_max(top));
-        if (g == 0) shared[16 * wave + n] = top;
-        __syncthreads();
+    };
+    auto load_v = [&](const Half* h) {
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) top = fmaxf(top, shared[16 * w + n]);
-        if (top > 0.0f && top < __builtin_inff()) e = __builtin_amdgcn_frexp_expf(top) - 1;
+      for (int u = 0; u < 2; u++) {
+        const auto w = rows_window(v, h[u].row, kRowBytes, h[u].rows);
+#pragma unroll
+        for (int j = 0; j < kVLoads; j++) vr[u][j] = window_load16(w, 16 * lane, 1024 * j);
       }
-      float sum = 0.0f;
+    };
+    auto load_v_scales = [&](const Half* h) {
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          x[h][j] = __builtin_amdgcn_ldexpf(x[h][j], -e);
-          sum += x[h][j];
-        }
-        u32x4_t terms[kQTerms];
-        split_terms<MSPR_F16, kQTerms>(x[h], terms);
-#pragma unroll
-        for (int t = 0; t < kQTerms; t++) qt[64 * ((2 * wave + h) * kQTerms + t)] = terms[t];
+      for (int u = 0; u < 2; u++) {
+        vs[u].load(rows_window(a.v_scales, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 16 * g + n);
+        vb[u].load(rows_window(a.v_biases, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 16 * g + n);
       }
-      q_unit = __builtin_amdgcn_ldexpf(q_unit, e);
-      sum += __shfl_xor(sum, 16, MSPR_WAVE);
-      sum += __shfl_xor(sum, 32, MSPR_WAVE);
-      if (g == 0) shared[64 + 16 * wave + n] = sum;
-      __syncthreads();
-      qsum = shared[64 + 16 * g + n];
-    }
-  }
-  __syncthreads();
+    };
 
-  const int tr_off = (4 * g + ((lane & 15) >> 2)) * kVPitch + 4 * (lane & 3) * 2;
-  for (int it0 = 0; it0 < n_mine; it0 += 31) {  // (a loop of its own, so that only its head waits for pages)
-  const int it_end = min(it0 + 31, n_mine);
-  for (int it = it0; it < it_end; it++) {
-    // the next tile (behind the last one that has no rows is asked for, so that what is outstanding does not depend on the tile)
-    nxt[0] = half_at(ids, it0, it + 1, 0);
-    nxt[1] = half_at(ids, it0, it + 1, 1);
+    int ids = load_ids(0);
+    Half cur[2] = {half_at(ids, 0, 0, 0), half_at(ids, 0, 0, 1)}, nxt[2];
+    load_k(cur);
+    load_v(cur);
+    if constexpr (kCodes) load_v_scales(cur);
+    int ids_next = load_ids(31);
+    __builtin_amdgcn_sched_barrier(0);  // the first tile is on its way before the query is fetched
 
-    // ---- S^T = K . Q^T
-    float s[8];  // key 16 u + 4 g + i at 4 u + i
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
+    // ---- Q^T operand, in LDS for all waves: lane (n = head, g) has the eight channels that the K operand has in its place
+    u32x4_t* qt = reinterpret_cast<u32x4_t*>(lds + kWaves * kVTileBytes) + lane;  // [8 steps][terms][64 lanes]
+    float q_unit = a.scale_log2;           // what a product's unit stands for, in powers of two
+    float qsum = 0.0f;                     // sum of the query's head n over group g
+    {
       if constexpr (!kCodes) {
-        f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < 8; j++) acc = mfma<FMT>(kr[u][j], qt[64 * j], acc);
-#pragma unroll
-        for (int i = 0; i < 4; i++) s[4 * u + i] = acc[i] * q_unit;
+        for (int h = 0; h < 2; h++) qt[64 * (2 * wave + h)] = mine ? qraw[h] : u32x4_t{0u, 0u, 0u, 0u};
       } else {
-        f32x4_t sum = __builtin_amdgcn_mfma_f32_16x16x4f32(kb[u].value(g), qsum, f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-        const float ksf = ks[u].value(n);
-        static_for<4>([&](auto jc) {
-          constexpr int j = decltype(jc)::value;
-          f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+        float x[2][8];  // step 2 wave + h
+        float top = 0.0f;
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            u32x4_t c;
+        for (int h = 0; h < 2; h++) {
+          if constexpr (QDT == MSPR_F32) {
 #pragma unroll
-            for (int w = 0; w < 2; w++) {
-              h2_t lo, hi;
-              codes4_to_h<kFmtAffine>(kr[u][j][2 * h + w], lo, hi);
-              c[2 * w] = h2_bits(lo);
-              c[2 * w + 1] = h2_bits(hi);
-            }
-#pragma unroll
-            for (int t = 0; t < kQTerms; t++) acc = mfma<MSPR_F16>(c, qt[64 * ((2 * j + h) * kQTerms + t)], acc);
+            for (int j = 0; j < 8; j++) x[h][j] = __uint_as_float(qraw[2 * h + j / 4][j % 4]);
+          } else {
+            widen8<QDT>(qraw[h], x[h]);
           }
-          static_for<4>([&](auto ic) {
-            constexpr int i = decltype(ic)::value;
-            sum[i] = fmaf(of_lane<4 * i + j>(ksf), acc[i], sum[i]);
-          });
-        });
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[4 * u + i] = sum[i] * q_unit;
-      }
-    }
-    load_k(nxt);
-    __builtin_amdgcn_sched_barrier(0);
-
-    // ---- online softmax (powers of two), the reference maximum moves only past 2^4
-    float tmax = -__builtin_inff();
-#pragma unroll
-    for (int u = 0; u < 2; u++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        if (4 * g + i >= cur[u].rows) s[4 * u + i] = -__builtin_inff();
-        tmax = fmaxf(tmax, s[4 * u + i]);
-      }
-    tmax = half_wave_max(row_pair_max(tmax));
-    const bool grow = tmax > m_run + kLag;
-    if (__any(grow)) {
-      const float m_new = grow ? tmax : m_run;
-      const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
-      l_run *= alpha;
-      m_run = m_new;
-#pragma unroll
-      for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] * alpha;
-      bacc = bacc * alpha;
-    }
-    const float m_safe = (m_run == -__builtin_inff() ? 0.0f : m_run) - kUp;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      s[i] = __builtin_amdgcn_exp2f(s[i] - m_safe);
-      l_run += s[i];
-    }
-
-    // ---- V rows to LDS (zeros in the place of rows that do not count, so that what lies there meets no weight of zero)
-#pragma unroll
-    for (int u = 0; u < 2; u++)
-#pragma unroll
-      for (int j = 0; j < kVLoads; j++) {
-        if constexpr (!kCodes) {
-          *reinterpret_cast<u32x4_t*>(vt + (16 * u + 2 * j + (lane >> 5)) * kVPitch + 16 * (lane & 31)) = vr[u][j];
-        } else {
-          u32x4_t lo, hi;
-          if constexpr (kVType == MSPR_BF16) codes_to_bf16(vr[u][j], lo, hi);
-#pragma unroll
-          for (int w = 0; w < 4 && kVType == MSPR_F16; w++) {
-            h2_t c01, c23;
-            codes4_to_h<kFmtAffine>(vr[u][j][w], c01, c23);
-            (w < 2 ? lo : hi)[2 * (w & 1)] = h2_bits(c01);
-            (w < 2 ? lo : hi)[2 * (w & 1) + 1] = h2_bits(c23);
+          for (int j = 0; j < 8; j++) {
+            x[h][j] = mine ? x[h][j] : 0.0f;
+            top = fmaxf(top, fabsf(x[h][j]));
           }
-          unsigned char* d = vt + (16 * u + 4 * j + (lane >> 4)) * kVPitch + 32 * (lane & 15);
-          *reinterpret_cast<u32x4_t*>(d) = lo;
-          *reinterpret_cast<u32x4_t*>(d + 16) = hi;
         }
+        // The operand is float16: a power of two brings the head's largest element to [1, 2), so that what falls below
+        // float16's range is 2^-25 of it; float16 queries go in as they are.
+        float* shared = reinterpret_cast<float*>(lds);  // [2][waves][16 heads], where the V tiles will be
+        int e = 0;
+        if constexpr (QDT != MSPR_F16) {
+          top = half_wave_max(row_pair_max(top));
+          if (g == 0) shared[16 * wave + n] = top;
+          __syncthreads();
+#pragma unroll
+          for (int w = 0; w < kWaves; w++) top = fmaxf(top, shared[16 * w + n]);
+          if (top > 0.0f && top < __builtin_inff()) e = __builtin_amdgcn_frexp_expf(top) - 1;
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            x[h][j] = __builtin_amdgcn_ldexpf(x[h][j], -e);
+            sum += x[h][j];
+          }
+          u32x4_t terms[kQTerms];
+          split_terms<MSPR_F16, kQTerms>(x[h], terms);
+#pragma unroll
+          for (int t = 0; t < kQTerms; t++) qt[64 * ((2 * wave + h) * kQTerms + t)] = terms[t];
+        }
+        q_unit = __builtin_amdgcn_ldexpf(q_unit, e);
+        sum += __shfl_xor(sum, 16, MSPR_WAVE);
+        sum += __shfl_xor(sum, 32, MSPR_WAVE);
+        if (g == 0) shared[64 + 16 * wave + n] = sum;
+        __syncthreads();
+        qsum = shared[64 + 16 * g + n];
       }
-    load_v(nxt);
-    cur[0] = nxt[0];
-    cur[1] = nxt[1];
-    __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();
 
-    // ---- O^T += V^T . P^T (the tile was written by this wave only: LDS operations of one wave complete in order, the wave
-    //      barrier keeps the compiler from moving the reads up)
-    __builtin_amdgcn_wave_barrier();
-    // (operands of four tiles of channels are read while the four before are multiplied)
-    u32x4_t vf[2][4];
-    auto read_v = [&](int q4) {
-#pragma unroll
-      for (int m = 0; m < 4; m++) {
-        const unsigned char* base = vt + tr_off + (4 * q4 + m) * 32;
-        const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, base)));
-        const u32x2_t hi =
-            __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, base + 16 * kVPitch)));
-        vf[q4 & 1][m] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
-      }
-    };
-    auto accumulate = [&](int q4, const u32x4_t* pf) {
-      if (q4 < 3) read_v(q4 + 1);
-#pragma unroll
-      for (int t = 0; t < kPTerms; t++)
-#pragma unroll
-        for (int m = 0; m < 4; m++) oacc[4 * q4 + m] = mfma<kVType>(vf[q4 & 1][m], pf[t], oacc[4 * q4 + m]);
-    };
-    read_v(0);
-    u32x4_t pf[kPTerms];
-    if constexpr (!kCodes) {
-      split_terms<kVType, kPTerms>(s, pf);
-#pragma unroll
-      for (int q4 = 0; q4 < 4; q4++) accumulate(q4, pf);
-    } else {
-      // The operand is float16: scales are taken as multiples of a power of two that is as large as any of them.
-      float vsf[2] = {vs[0].value(n), vs[1].value(n)};
-      const float largest = fmaxf(fabsf(vsf[0]), fabsf(vsf[1]));
-      if (__any(largest > v_unit)) {
-        float top = largest;
-        top = fmaxf(top, lane_xor<1>(top));
-        top = fmaxf(top, lane_xor<2>(top));
-        top = fmaxf(top, lane_xor<4>(top));
-        top = fmaxf(top, lane_xor<8>(top));
-        top = half_wave_max(row_pair_max(top));
-        const int e = top < 0x1p126f ? __builtin_amdgcn_frexp_expf(top) : 126;
-        const float unit = __builtin_amdgcn_ldexpf(1.0f, e);
-        const float down = v_unit / unit;
-#pragma unroll
-        for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] * down;
-        v_unit = unit;
-      }
-      const float per_unit = 1.0f / v_unit;
-      vsf[0] *= per_unit;
-      vsf[1] *= per_unit;
-      // biases: operand row m has group m of key 16 u + 4 g + i (rows from 4 on are not used)
-      const float vbf[2] = {vb[0].value(n), vb[1].value(n)};
-      static_for<8>([&](auto ic) {
-        constexpr int i = decltype(ic)::value;
-        const float b = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(vbf[i >> 2]), 0x100 + 4 * (i & 3), 0xF, 0xF, true));  // row_shl
-        bacc = __builtin_amdgcn_mfma_f32_16x16x4f32((i & 3) == 0 ? vbf[i >> 2] : b, s[i], bacc, 0, 0, 0);
-      });
-      static_for<4>([&](auto jc) {  // the weights of group j, which has channels 64 j on
-        constexpr int j = decltype(jc)::value;
-        float w[8];
-        static_for<8>([&](auto ic) {
-          constexpr int i = decltype(ic)::value;
-          w[i] = of_lane<4 * (i & 3) + j>(vsf[i >> 2]) * s[i];
-        });
-        split_terms<kVType, kPTerms>(w, pf);
-        accumulate(j, pf);
-      });
-    }
-    if constexpr (kCodes) load_v_scales(nxt);
-    __builtin_amdgcn_wave_barrier();
-  }
-  ids = ids_next;
-  ids_next = load_ids(it_end + 31);
-  }
+    const int tr_off = (4 * g + ((lane & 15) >> 2)) * kVPitch + 4 * (lane & 3) * 2;
+    for (int it0 = 0; it0 < n_mine; it0 += 31) {  // (a loop of its own, so that only its head waits for pages)
+      const int it_end = min(it0 + 31, n_mine);
+      for (int it = it0; it < it_end; it++) {
+        // the next tile (behind the last one that has no rows is asked for, so that what is outstanding does not depend on the tile)
+        nxt[0] = half_at(ids, it0, it + 1, 0);
+        nxt[1] = half_at(ids, it0, it + 1, 1);
 
-  // ---- merge the waves through LDS (the V tiles are free now)
-  l_run += __shfl_xor(l_run, 16, MSPR_WAVE);
-  l_run += __shfl_xor(l_run, 32, MSPR_WAVE);
-  if constexpr (kCodes) {
-    float bias[4];
+        // ---- S^T = K . Q^T
+        float s[8];  // key 16 u + 4 g + i at 4 u + i
 #pragma unroll
-    for (int j = 0; j < 4; j++) bias[j] = __shfl(bacc[j], n, MSPR_WAVE);
+        for (int u = 0; u < 2; u++) {
+          if constexpr (!kCodes) {
+            f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] * v_unit + bias[mt >> 2];
-  }
-  __syncthreads();
-  float* xo = reinterpret_cast<float*>(lds);   // [waves][16 mt][64 lanes][4]
-  float* xml = xo + kWaves * 16 * 64 * 4;      // [waves][16 heads][2]
+            for (int j = 0; j < 8; j++) acc = mfma<FMT>(kr[u][j], qt[64 * j], acc);
 #pragma unroll
-  for (int mt = 0; mt < 16; mt++) *reinterpret_cast<f32x4_t*>(xo + ((wave * 16 + mt) * 64 + lane) * 4) = oacc[mt];
-  if (g == 0) {
-    xml[(wave * 16 + n) * 2] = m_run;
-    xml[(wave * 16 + n) * 2 + 1] = l_run;
-  }
-  __syncthreads();
-  float mw[kWaves], m_all = -__builtin_inff();
+            for (int i = 0; i < 4; i++) s[4 * u + i] = acc[i] * q_unit;
+          } else {
+            f32x4_t sum = __builtin_amdgcn_mfma_f32_16x16x4f32(kb[u].value(g), qsum, f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+            const float ksf = ks[u].value(n);
+            static_for<4>([&](auto jc) {
+              constexpr int j = decltype(jc)::value;
+              f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int w = 0; w < kWaves; w++) {
-    mw[w] = xml[(w * 16 + n) * 2];
-    m_all = fmaxf(m_all, mw[w]);
-  }
-  const float m_safe = m_all == -__builtin_inff() ? 0.0f : m_all;
-  float l_all = 0.0f;
+              for (int h = 0; h < 2; h++) {
+                u32x4_t c;
 #pragma unroll
-  for (int w = 0; w < kWaves; w++) {
-    mw[w] = __builtin_amdgcn_exp2f(mw[w] - m_safe);
-    l_all += xml[(w * 16 + n) * 2 + 1] * mw[w];
-  }
-  const bool whole = tile0 == 0 && tile1 == row_tiles;
-  const int row = at.b * n_kv + at.kvh;
-  const int64_t part = 2 * (int64_t)blockIdx.x + (tile0 == 0 ? 1 : 0);
-  const auto po = store_window(a.ws_o + part * rep * kD, rep * kD * (int)sizeof(float));
+                for (int w = 0; w < 2; w++) {
+                  h2_t lo, hi;
+                  codes4_to_h<kFmtAffine>(kr[u][j][2 * h + w], lo, hi);
+                  c[2 * w] = h2_bits(lo);
+                  c[2 * w + 1] = h2_bits(hi);
+                }
 #pragma unroll
-  for (int q4 = 0; q4 < 16 / kWaves; q4++) {
-    const int mt = wave * (16 / kWaves) + q4;
-    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+                for (int t = 0; t < kQTerms; t++) acc = mfma<MSPR_F16>(c, qt[64 * ((2 * j + h) * kQTerms + t)], acc);
+              }
+              static_for<4>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+                sum[i] = fmaf(of_lane<4 * i + j>(ksf), acc[i], sum[i]);
+              });
+            });
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) acc += *reinterpret_cast<const f32x4_t*>(xo + ((w * 16 + mt) * 64 + lane) * 4) * mw[w];
-    if (n < rep) {
-      if (whole) store_out<QDT>(a.out, ((int64_t)row * rep + n) * kD + 16 * mt + 4 * g, acc, l_all);
-      else window_store<kStoreThrough>(po, (n * kD + 16 * mt + 4 * g) * 4, __builtin_bit_cast(u32x4_t, acc));
+            for (int i = 0; i < 4; i++) s[4 * u + i] = sum[i] * q_unit;
+          }
+        }
+        load_k(nxt);
+        __builtin_amdgcn_sched_barrier(0);
+
+        // ---- online softmax (powers of two), the reference maximum moves only past 2^4
+        float tmax = -__builtin_inff();
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            if (4 * g + i >= cur[u].rows) s[4 * u + i] = -__builtin_inff();
+            tmax = fmaxf(tmax, s[4 * u + i]);
+          }
+        tmax = half_wave_max(row_pair_max(tmax));
+        const bool grow = tmax > m_run + kLag;
+        if (__any(grow)) {
+          const float m_new = grow ? tmax : m_run;
+          const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+          l_run *= alpha;
+          m_run = m_new;
+#pragma unroll
+          for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] * alpha;
+          bacc = bacc * alpha;
+        }
+        const float m_safe = (m_run == -__builtin_inff() ? 0.0f : m_run) - kUp;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          s[i] = __builtin_amdgcn_exp2f(s[i] - m_safe);
+          l_run += s[i];
+        }
+
+        // ---- V rows to LDS (zeros in the place of rows that do not count, so that what lies there meets no weight of zero)
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int j = 0; j < kVLoads; j++) {
+            if constexpr (!kCodes) {
+              *reinterpret_cast<u32x4_t*>(vt + (16 * u + 2 * j + (lane >> 5)) * kVPitch + 16 * (lane & 31)) = vr[u][j];
+            } else {
+              u32x4_t lo, hi;
+              if constexpr (kVType == MSPR_BF16) codes_to_bf16(vr[u][j], lo, hi);
+#pragma unroll
+              for (int w = 0; w < 4 && kVType == MSPR_F16; w++) {
+                h2_t c01, c23;
+                codes4_to_h<kFmtAffine>(vr[u][j][w], c01, c23);
+                (w < 2 ? lo : hi)[2 * (w & 1)] = h2_bits(c01);
+                (w < 2 ? lo : hi)[2 * (w & 1) + 1] = h2_bits(c23);
+              }
+              unsigned char* d = vt + (16 * u + 4 * j + (lane >> 4)) * kVPitch + 32 * (lane & 15);
+              *reinterpret_cast<u32x4_t*>(d) = lo;
+              *reinterpret_cast<u32x4_t*>(d + 16) = hi;
+            }
+          }
+        load_v(nxt);
+        cur[0] = nxt[0];
+        cur[1] = nxt[1];
+        __builtin_amdgcn_sched_barrier(0);
+
+        // ---- O^T += V^T . P^T (the tile was written by this wave only: LDS operations of one wave complete in order, the wave
+        //      barrier keeps the compiler from moving the reads up)
+        __builtin_amdgcn_wave_barrier();
+        // (operands of four tiles of channels are read while the four before are multiplied)
+        u32x4_t vf[2][4];
+        auto read_v = [&](int q4) {
+#pragma unroll
+          for (int m = 0; m < 4; m++) {
+            const unsigned char* base = vt + tr_off + (4 * q4 + m) * 32;
+            const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, base)));
+            const u32x2_t hi =
+                __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, base + 16 * kVPitch)));
+            vf[q4 & 1][m] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
+          }
+        };
+        auto accumulate = [&](int q4, const u32x4_t* pf) {
+          if (q4 < 3) read_v(q4 + 1);
+#pragma unroll
+          for (int t = 0; t < kPTerms; t++)
+#pragma unroll
+            for (int m = 0; m < 4; m++) oacc[4 * q4 + m] = mfma<kVType>(vf[q4 & 1][m], pf[t], oacc[4 * q4 + m]);
+        };
+        read_v(0);
+        u32x4_t pf[kPTerms];
+        if constexpr (!kCodes) {
+          split_terms<kVType, kPTerms>(s, pf);
+#pragma unroll
+          for (int q4 = 0; q4 < 4; q4++) accumulate(q4, pf);
+        } else {
+          // The operand is float16: scales are taken as multiples of a power of two that is as large as any of them.
+          float vsf[2] = {vs[0].value(n), vs[1].value(n)};
+          const float largest = fmaxf(fabsf(vsf[0]), fabsf(vsf[1]));
+          if (__any(largest > v_unit)) {
+            float top = largest;
+            top = fmaxf(top, lane_xor<1>(top));
+            top = fmaxf(top, lane_xor<2>(top));
+            top = fmaxf(top, lane_xor<4>(top));
+            top = fmaxf(top, lane_xor<8>(top));
+            top = half_wave_max(row_pair_max(top));
+            const int e = top < 0x1p126f ? __builtin_amdgcn_frexp_expf(top) : 126;
+            const float unit = __builtin_amdgcn_ldexpf(1.0f, e);
+            const float down = v_unit / unit;
+#pragma unroll
+            for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] * down;
+            v_unit = unit;
+          }
+          const float per_unit = 1.0f / v_unit;
+          vsf[0] *= per_unit;
+          vsf[1] *= per_unit;
+          // biases: operand row m has group m of key 16 u + 4 g + i (rows from 4 on are not used)
+          const float vbf[2] = {vb[0].value(n), vb[1].value(n)};
+          static_for<8>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            float b = vbf[i >> 2];
+            if constexpr ((i & 3) != 0)
+              b = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(b), 0x100 + 4 * (i & 3), 0xF, 0xF, true));  // row_shl
+            bacc = __builtin_amdgcn_mfma_f32_16x16x4f32(b, s[i], bacc, 0, 0, 0);
+          });
+          static_for<4>([&](auto jc) {  // the weights of group j, which has channels 64 j on
+            constexpr int j = decltype(jc)::value;
+            float w[8];
+            static_for<8>([&](auto ic) {
+              constexpr int i = decltype(ic)::value;
+              w[i] = of_lane<4 * (i & 3) + j>(vsf[i >> 2]) * s[i];
+            });
+            split_terms<kVType, kPTerms>(w, pf);
+            accumulate(j, pf);
+          });
+        }
+        if constexpr (kCodes) load_v_scales(nxt);
+        __builtin_amdgcn_wave_barrier();
+      }
+      ids = ids_next;
+      ids_next = load_ids(it_end + 31);
     }
-  }
-  if (wave == 0 && g == 0) {
-    if (!whole) *reinterpret_cast<f32x2_t*>(a.ws_ml + (part * 16 + n) * 2) = f32x2_t{m_all, l_all};
-    if (n == 0 && tile0 == 0 && (by_row || !whole)) {
-      int32_t* c = a.cut + 3 * (int64_t)(by_row ? row : (int)blockIdx.x);
-      c[0] = whole ? -1 : row;
-      c[1] = blockIdx.x;
-      c[2] = blockIdx.x + (row_tiles - tile1 + share - 1) / share;
+
+    // ---- merge the waves through LDS (the V tiles are free now)
+    l_run += __shfl_xor(l_run, 16, MSPR_WAVE);
+    l_run += __shfl_xor(l_run, 32, MSPR_WAVE);
+    if constexpr (kCodes) {
+      float bias[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) bias[j] = __shfl(bacc[j], n, MSPR_WAVE);
+#pragma unroll
+      for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] * v_unit + bias[mt >> 2];
     }
-  }
-  pos += tile1 - tile0;
-  if (pos >= end) return;
-  at.tile = 0;
-  if (++at.kvh == n_kv) {
-    at.kvh = 0;
-    at.b++;
-    at.len = __builtin_amdgcn_readfirstlane(length_of(lens, batch, at.b, cap));
-  }
-  __syncthreads();
+    __syncthreads();
+    float* xo = reinterpret_cast<float*>(lds);   // [waves][16 mt][64 lanes][4]
+    float* xml = xo + kWaves * 16 * 64 * 4;      // [waves][16 heads][2]
+#pragma unroll
+    for (int mt = 0; mt < 16; mt++) *reinterpret_cast<f32x4_t*>(xo + ((wave * 16 + mt) * 64 + lane) * 4) = oacc[mt];
+    if (g == 0) {
+      xml[(wave * 16 + n) * 2] = m_run;
+      xml[(wave * 16 + n) * 2 + 1] = l_run;
+    }
+    __syncthreads();
+    float mw[kWaves], m_all = -__builtin_inff();
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+      mw[w] = xml[(w * 16 + n) * 2];
+      m_all = fmaxf(m_all, mw[w]);
+    }
+    const float m_safe = m_all == -__builtin_inff() ? 0.0f : m_all;
+    float l_all = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+      mw[w] = __builtin_amdgcn_exp2f(mw[w] - m_safe);
+      l_all += xml[(w * 16 + n) * 2 + 1] * mw[w];
+    }
+    const bool whole = tile0 == 0 && tile1 == row_tiles;
+    const int row = at.b * n_kv + at.kvh;
+    const int64_t part = 2 * (int64_t)blockIdx.x + (tile0 == 0 ? 1 : 0);
+    const auto po = store_window(a.ws_o + part * rep * kD, rep * kD * (int)sizeof(float));
+#pragma unroll
+    for (int q4 = 0; q4 < 16 / kWaves; q4++) {
+      const int mt = wave * (16 / kWaves) + q4;
+      f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) acc += *reinterpret_cast<const f32x4_t*>(xo + ((w * 16 + mt) * 64 + lane) * 4) * mw[w];
+      if (n < rep) {
+        if (whole) store_out<QDT>(a.out, ((int64_t)row * rep + n) * kD + 16 * mt + 4 * g, acc, l_all);
+        else window_store<kStoreThrough>(po, (n * kD + 16 * mt + 4 * g) * 4, __builtin_bit_cast(u32x4_t, acc));
+      }
+    }
+    if (wave == 0 && g == 0) {
+      if (!whole) *reinterpret_cast<f32x2_t*>(a.ws_ml + (part * 16 + n) * 2) = f32x2_t{m_all, l_all};
+      if (n == 0 && tile0 == 0 && (by_row || !whole)) {
+        int32_t* c = a.cut + 3 * (int64_t)(by_row ? row : (int)blockIdx.x);
+        c[0] = whole ? -1 : row;
+        c[1] = blockIdx.x;
+        c[2] = min((int)(blockIdx.x + (row_tiles - tile1 + share - 1) / share), (int)gridDim.x - 1);
+      }
+    }
+    pos += tile1 - tile0;
+    if (pos >= end) return;
+    at.tile = 0;
+    if (++at.kvh == n_kv) {
+      at.kvh = 0;
+      if (++at.b >= batch) return;
+      at.len = __builtin_amdgcn_readfirstlane(length_of(lens, batch, at.b, cap));
+    }
+    __syncthreads();
   }
 }
 

@@ -96,6 +96,23 @@ def test_lengths_and_stack_that_are_out_of_range_stay_in_the_buffers():
     assert (edge == 12345).all()
 
 
+@pytest.mark.parametrize("batch", [40, 1025, 2048])
+def test_asked_for_rows_that_add_up_beyond_all_integers(batch):
+    rng = np.random.default_rng(batch)
+    lens = rng.integers(0, 64, batch)
+    tables, free, head = _pool(rng, lens, 16, 8, 30)
+    new = np.full(batch, 2 ** 31 - 1)
+    new[0], new[3], new[9:17] = 5, 0, -1
+    got, want = None, oracle.page_step(lens, new, tables, free, head, 16, 300)
+    t, f = _dev(tables), _dev(free)
+    got = paged.page_step(_dev(lens), _dev(new), t, f, _dev([head]), page_size=16, n_rows=300)
+    for name in NAMES:
+        if name != "counts":
+            np.testing.assert_array_equal(getattr(got, name).cpu().numpy(), np.asarray(want[name]), err_msg=name)
+    assert got.counts.tolist()[0] == 2 ** 31 - 1 and got.counts.tolist()[2:] == want["counts"][2:]
+    np.testing.assert_array_equal(t.cpu().numpy(), want["tables"])
+
+
 def test_a_server_of_many_steps_keeps_every_page_in_one_place():
     rng = np.random.default_rng(11)
     B, page, n_pages = 37, 16, 150

@@ -201,6 +201,25 @@ def test_pages_that_are_not_in_the_pool_are_left_out(dtype, form):
     assert (got[3] == 0).all()
 
 
+@pytest.mark.parametrize("batch,n_kv", [(64, 2), (65, 2), (128, 1), (129, 8), (1000, 2), (4097, 1), (5000, 2)])
+def test_many_queries_of_few_tables(batch, n_kv):
+    """More queries than lanes, and more chunks of them than lanes; lengths from none to some tiles, runs of zeros among them."""
+    rng = np.random.default_rng(batch)
+    keys, values = _cache(rng, (12, n_kv, 16, 256), BF16, "rows")
+    tables = rng.integers(0, 12, (7, 9))
+    lens, requests = rng.integers(0, 145, batch), rng.integers(0, 7, batch)
+    lens[rng.random(batch) < 0.3] = 0
+    lens[batch // 3:batch // 2] = 0
+    q = _rows(rng, (batch, 2 * n_kv, 256), BF16)
+    got = _attend(q, keys, values, tables, lens, SCALE, requests=_i32(requests))
+    some = rng.choice(batch, 40, replace=False)
+    some[:2] = 0, batch - 1
+    want, bound = _reference(q[some], keys, values, tables, lens[some], SCALE, requests[some])
+    bound = bound + torch.finfo(BF16).eps / 2 * want.abs() + torch.finfo(BF16).tiny
+    assert ((got[some].double() - want).abs() <= bound).all()
+    assert (got[torch.from_numpy(lens == 0).cuda()] == 0).all() and not got.isnan().any()
+
+
 def test_lengths_beyond_the_table_and_below_zero():
     rng = np.random.default_rng(4)
     keys, values = _cache(rng, (9, 2, 16, 256), BF16, "rows")
