@@ -245,7 +245,8 @@ extern "C" int mspr_page_step(const int32_t* lens, const int32_t* new_lens, int3
   MSPR_REQUIRE(table_width >= 1 && (int64_t)table_width * page_size <= 0x40000000,
                "page_step: a request's table must hold 1 page or more and at most 2^30 tokens");
   MSPR_REQUIRE((int64_t)batch * table_width <= 0x40000000, "page_step: too many table entries");
-  MSPR_REQUIRE(n_pages >= 1 && (int64_t)n_pages * page_size <= 0x7FFFFFFF, "page_step: the pool must hold fewer than 2^31 tokens");
+  MSPR_REQUIRE(n_pages >= 1 && (int64_t)n_pages * page_size <= 0x7FFFFFFF,
+               "page_step: the pool must hold fewer than 2^31 tokens");
   MSPR_REQUIRE(n_rows >= 0 && n_rows <= 0x3FFFFFFF, "page_step: n_rows out of range");
   MSPR_REQUIRE(lens_out != lens && head_out != head, "page_step: lengths and head are not updated in place");
   const StepArgs a{lens, new_lens, tables, free_pages, head, batch, table_width, n_pages, __builtin_ctz(page_size), n_rows,

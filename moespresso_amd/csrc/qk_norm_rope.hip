@@ -11,8 +11,8 @@
 // is whole rows (with 32 bytes of a float32 row a lane, every line was asked for twice), the sum of squares is five or six lane
 // exchanges, the partner of a channel one more. A wave takes neighbouring heads of one kind, so that whose row it is and where
 // it lies is scalar arithmetic, and asks for its next rows before it works on these. Loads are non-temporal, as nothing reads
-// the projections' output again (16384 tokens of bfloat16 rows, appended: 56 us, 6.0 TB/s, instead of 67). The cosines and sines of a workgroup's tokens are made once, a thread each, under the first rows'
-// loads, and shared through LDS.
+// the projections' output again (16384 tokens of bfloat16 rows, appended: 56 us, 6.0 TB/s, instead of 67). The cosines and
+// sines of a workgroup's tokens are made once, a thread each, under the first rows' loads, and shared through LDS.
 #include "affine_q8.h"
 #include "common.h"
 
@@ -262,7 +262,8 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(RopeArgs a) {
 #pragma unroll
       for (int j = 0; j < N; j++) x[j] = x[j] * r * w[j];
       if (rotary) {
-        const f32x4_t* cs = reinterpret_cast<const f32x4_t*>(turn + (2 * here.t + (low ? 0 : 1)) * a.half + N * (low ? lane : partner));
+        const f32x2_t* of_token = turn + (2 * here.t + (low ? 0 : 1)) * a.half;
+        const f32x4_t* cs = reinterpret_cast<const f32x4_t*>(of_token + N * (low ? lane : partner));
 #pragma unroll
         for (int j = 0; j < N; j += 2) {
           const f32x4_t c = cs[j / 2];
@@ -277,7 +278,8 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(RopeArgs a) {
     } else if constexpr (KEEP == kDense) {
       store_row<DT, N>(a.k_out, (token * a.n_kv + head) * kD + N * lane, x);
     } else {
-      keep_row<DT, KEEP, PT>(is_v ? a.v_out : a.k_out, is_v ? a.v_scales : a.k_scales, is_v ? a.v_biases : a.k_biases, at, lane, x);
+      keep_row<DT, KEEP, PT>(is_v ? a.v_out : a.k_out, is_v ? a.v_scales : a.k_scales, is_v ? a.v_biases : a.k_biases, at, lane,
+                             x);
     }
   };
   // (two sets of registers in turn: a copy from one to the other would wait for its load)
@@ -314,12 +316,14 @@ int rope_launch(RopeArgs a, hipStream_t st) {
 }
 
 int rope_checks(const char* what, const RopeArgs& a, int dtype, int head_dim) {
-  MSPR_REQUIRE(a.q && a.k && a.q_weight && a.k_weight && a.positions && a.inv_freq && a.q_out && a.k_out, "%s: null pointer", what);
+  MSPR_REQUIRE(a.q && a.k && a.q_weight && a.k_weight && a.positions && a.inv_freq && a.q_out && a.k_out, "%s: null pointer",
+               what);
   MSPR_REQUIRE(dtype >= MSPR_F32 && dtype <= MSPR_BF16, "%s: dtype must be f32, f16 or bf16", what);
   MSPR_REQUIRE(head_dim == kD, "%s: head_dim must be 256", what);
   MSPR_REQUIRE(a.n_tokens >= 1 && a.n_tokens <= (1 << 24), "%s: 1 to 2^24 tokens", what);
   MSPR_REQUIRE(a.n_q >= 1 && a.n_kv >= 1 && a.n_q <= 1024 && a.n_kv <= 1024, "%s: 1 to 1024 heads of each kind", what);
-  MSPR_REQUIRE(a.half >= 8 && a.half <= kMaxHalf && a.half % 8 == 0, "%s: the rotary width must be a multiple of 16 up to 256", what);
+  MSPR_REQUIRE(a.half >= 8 && a.half <= kMaxHalf && a.half % 8 == 0, "%s: the rotary width must be a multiple of 16 up to 256",
+               what);
   MSPR_REQUIRE(a.axes == 1 || a.axes == 3, "%s: positions have one axis or three", what);
   MSPR_REQUIRE(a.axes == 1 || (a.sec1 >= 0 && a.sec2 >= 0 && 3 * a.sec1 <= a.half + 1 && 3 * a.sec2 <= a.half),
                "%s: the height and width axes have more frequencies than their turns", what);
@@ -361,7 +365,8 @@ RopeArgs rope_args(const void* q, const void* k, const void* q_weight, const voi
 int append_checks(const char* what, const RopeArgs& a, int page_size) {
   MSPR_REQUIRE(a.v && a.slots && a.v_out, "%s: null pointer", what);
   MSPR_REQUIRE(page_size >= 16 && (page_size & (page_size - 1)) == 0, "%s: page_size must be a power of two from 16 on", what);
-  MSPR_REQUIRE(a.n_pages >= 1 && (int64_t)a.n_pages * page_size <= 0x7FFFFFFF, "%s: the pool must hold fewer than 2^31 tokens", what);
+  MSPR_REQUIRE(a.n_pages >= 1 && (int64_t)a.n_pages * page_size <= 0x7FFFFFFF, "%s: the pool must hold fewer than 2^31 tokens",
+               what);
   return MSPR_OK;
 }
 

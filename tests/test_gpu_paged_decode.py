@@ -4,10 +4,11 @@ Tolerance, from the arithmetic. A score is a float32 sum of 256 exact products a
 260 * 2^-24 * A, A = scale * sum |q| |k| at its largest over the keys (natural units; the same relative to the exponent's
 argument for its rounding). An error d of every score moves the result by at most 2 d of sum p |v|. A weight is two terms
 of a 16-bit type, each off by half a step of it (bfloat16 pages 2^-8 of 2^-8 of the weight, float16 operands 2^-11 of 2^-11), or
-one float16 term (8-bit pages, bfloat16 result: 2^-11), or three bfloat16 terms (float32 result: 2^-24); float16 operands are taken 2^11 times as large and end at 2^-25, so
-that n weights lose at most n * 2^-36 of the largest value together (8-bit pages: of 255 times twice the largest scale). Sums
-over n keys run over n / 8 float32 additions at most, counted for both the weights' and the values' sums; the result is
-rounded once more, to eps / 2 of its type.
+one float16 term (8-bit pages, bfloat16 result: 2^-11), or three bfloat16 terms (float32 result: 2^-24); float16 operands
+are taken 2^11 times as large and end at 2^-25, so that n weights lose at most n * 2^-36 of the largest value together (8-bit
+pages: of 255 times twice the largest scale). Sums over n keys run over n / 8 float32 additions at most where four waves
+share a row of keys, over n / 4 where one has it for itself (64 rows or more: a lane adds eight weights of every 32 keys),
+counted for both the weights' and the values' sums; the result is rounded once more, to eps / 2 of its type.
 """
 
 import numpy as np
@@ -91,7 +92,8 @@ def _reference(q, keys, values, tables, lens, scale, requests=None):
                 c, s, z = (_pick(t, p)[:, g] for t in keys)
                 c = (c.view(torch.uint8).double() * s.double().repeat_interleave(64, -1)).abs() + z.double().repeat_interleave(64, -1).abs()
                 most = (x.abs() @ c.reshape(-1, 256)[keep].t()).amax(-1, keepdim=True) * abs(scale)
-            bound[r, g * rep:(g + 1) * rep] = size * (2 * 260 * 2.0 ** -24 * most + terms + 2 * (k.shape[0] / 8 + 8) * 2.0 ** -24)
+            adds = k.shape[0] / (8 if q.shape[0] * G < 64 else 4) + 8
+            bound[r, g * rep:(g + 1) * rep] = size * (2 * 260 * 2.0 ** -24 * most + terms + 2 * adds * 2.0 ** -24)
             if q.dtype == F16 or q.dtype == BF16 and not torch.is_tensor(keys):
                 bound[r, g * rep:(g + 1) * rep] += k.shape[0] * 2.0 ** -36 * largest
     return out, bound
@@ -167,6 +169,22 @@ def test_long_and_ragged_batches(dtype, form):
         keys, values = _cache(rng, (n_pages, n_kv, page, 256), dtype, form)
         q = _rows(rng, (len(lens), 8 * n_kv, 256), dtype) * 2
         _check(q, keys, values, _tables(rng, lens, page, -(-max(lens) // page), n_pages), lens)
+
+
+@pytest.mark.parametrize("dtype,form", [(BF16, "rows"), (F32, F32), (F16, BF16)])
+@pytest.mark.parametrize("n_kv,page,lens", [
+    (2, 64, [8000] + [1] * 31),                # a row in more than a hundred parts among whole ones
+    (2, 16, [1] * 20 + [5000, 0, 3000] + [40] * 20),
+    (8, 32, [70, 3] * 64 + [3000, 65]),        # more rows than shares, one in more than sixteen parts
+    (1, 16, [129, 0, 64] * 21 + [1]),          # as few rows as are dealt out to single waves
+    (1, 16, [129, 0, 64] * 21),                # one fewer
+])
+def test_long_rows_among_many(n_kv, page, lens, dtype, form):
+    rng = np.random.default_rng(len(lens))
+    n_pages = sum(-(-n // page) for n in lens) + 1
+    keys, values = _cache(rng, (n_pages, n_kv, page, 256), dtype, form)
+    q = _rows(rng, (len(lens), 3 * n_kv, 256), dtype) * 2
+    _check(q, keys, values, _tables(rng, lens, page, -(-max(lens) // page), n_pages), lens)
 
 
 @pytest.mark.parametrize("dtype,form", [(BF16, "rows"), (F16, "rows"), (F32, F32), (F16, F16)])
@@ -278,7 +296,7 @@ def test_the_same_call_gives_the_same_bits():
     keys, values = _cache(rng, (n_pages, 2, 16, 256), BF16, "rows")
     q, tables = _rows(rng, (20, 16, 256), BF16), _tables(rng, lens, 16, 190, n_pages)
     want = _attend(q, keys, values, tables, lens, SCALE)
-    ws = torch.full((1 << 22,), float("nan"), device="cuda")
+    ws = torch.full((1 << 23,), float("nan"), device="cuda")
     assert all(_attend(q, keys, values, tables, lens, SCALE, workspace=ws).equal(want) for _ in range(5))
 
 

@@ -6,7 +6,7 @@ import pytest
 
 from moespresso_amd import _lib
 
-TILE, WAVES, SHARES, MIN_TILES = 32, 4, 256, 2
+TILE, WAVES, GROUPS, MIN_TILES, MANY_ROWS = 32, 4, 256, 2, 64
 
 
 def _row_tiles(n):
@@ -14,14 +14,21 @@ def _row_tiles(n):
     return max(MIN_TILES, -(-n // TILE))
 
 
+def _most(batch, n_kv):
+    """Shares at most, and waves that take a share's tiles in turn: of few rows workgroups have shares, of many waves."""
+    return (GROUPS * WAVES, 1) if batch * n_kv >= MANY_ROWS else (GROUPS, WAVES)
+
+
 def _shares(batch, n_kv, cap):
-    return min(SHARES, -(-batch * n_kv * _row_tiles(cap) // MIN_TILES))
+    most, waves = _most(batch, n_kv)
+    unit = WAVES // waves
+    return min(most, -(-(-(-batch * n_kv * _row_tiles(cap) // MIN_TILES)) // unit) * unit)
 
 
 def _parts(wg, lens, n_kv):
-    """The parts of rows that a workgroup attends: (request, KV head, first tile, end tile, tiles of the row), and its share."""
+    """The parts of rows that share wg holds: (request, KV head, first tile, end tile, tiles of the row), and its share."""
     total = sum(_row_tiles(n) for n in lens) * n_kv
-    share = max(MIN_TILES, -(-total // SHARES))
+    share = max(MIN_TILES, -(-total // _most(len(lens), n_kv)[0]))
     pos, end = wg * share, min((wg + 1) * share, total)
     parts, before = [], 0
     for b, n in enumerate(lens):
@@ -46,7 +53,8 @@ def _lens(rng, batch, cap, kind):
 
 @pytest.mark.parametrize("kind", ["all", "one", "empty", "any"])
 @pytest.mark.parametrize("batch,n_kv,page,width", [(1, 1, 16, 1), (1, 2, 16, 9), (1, 2, 64, 128), (3, 2, 16, 100), (65, 1, 32, 7),
-                                                   (130, 8, 16, 3), (16, 2, 256, 40), (64, 4, 128, 2), (300, 2, 16, 1), (70, 8, 32, 4), (600, 1, 64, 2)])
+                                                   (130, 8, 16, 3), (16, 2, 256, 40), (64, 4, 128, 2),
+                                                   (300, 2, 16, 1), (70, 8, 32, 4), (600, 1, 64, 2)])
 def test_every_row_is_attended_once_and_every_address_lies_in_its_buffer(kind, batch, n_kv, page, width):
     rng = np.random.default_rng(batch * 1000 + width)
     cap = page * width
@@ -59,7 +67,8 @@ def test_every_row_is_attended_once_and_every_address_lies_in_its_buffer(kind, b
         tables[b, :h] = order[used:used + h]
         used += h
     seen = np.zeros((batch, n_kv, cap), dtype=np.int64)
-    slots = {}  # partials by row: the slots that the workgroups write, in the order of the row's tiles
+    most, waves = _most(batch, n_kv)
+    slots = {}  # partials by row: the slots that the shares write, in the order of the row's tiles
     cuts, written = {}, set()
     grid = _shares(batch, n_kv, cap)
     for wg in range(grid):
@@ -74,11 +83,11 @@ def test_every_row_is_attended_once_and_every_address_lies_in_its_buffer(kind, b
                     assert wg not in cuts  # only a share's last part begins a row that it does not end
                     cuts[wg] = (b, kvh), wg + -(-(row_tiles - tile1) // share)
             last = min(tile1, -(-lens[b] // TILE))
-            for wave in range(WAVES):
-                mine = -(-(last - tile0 - wave) // WAVES) if last - tile0 > wave else 0
+            for wave in range(waves):
+                mine = -(-(last - tile0 - wave) // waves) if last - tile0 > wave else 0
                 for it in range(mine):
                     for u in range(2):
-                        key = (tile0 + wave + WAVES * it) * TILE + 16 * u
+                        key = (tile0 + wave + waves * it) * TILE + 16 * u
                         p = tables[b, key // page] if key < lens[b] else -1
                         good = 0 <= p < n_pages
                         row = ((p if good else 0) * n_kv + kvh) * page + key % page
@@ -93,12 +102,13 @@ def test_every_row_is_attended_once_and_every_address_lies_in_its_buffer(kind, b
     assert all(0 <= s < 2 * grid for part in slots.values() for s in part)
     assert len({s for part in slots.values() for s in part}) == sum(len(part) for part in slots.values())
     assert not _parts(grid, lens, n_kv)[0]  # nothing is left over
-    if _row_tiles(cap) == MIN_TILES and batch * n_kv <= SHARES:
+    if _row_tiles(cap) == MIN_TILES and batch * n_kv <= most:
         assert not merged  # the merge is not launched
 
 
 @pytest.mark.skipif(not _lib.library_available(), reason="the library is not built")
-@pytest.mark.parametrize("batch,heads,n_kv,page,width", [(1, 16, 2, 64, 1), (1, 16, 2, 64, 2048), (256, 64, 8, 16, 100), (65535, 1, 1, 16, 1)])
+@pytest.mark.parametrize("batch,heads,n_kv,page,width", [(1, 16, 2, 64, 1), (1, 16, 2, 64, 2048), (256, 64, 8, 16, 100), (65535, 1, 1, 16, 1),
+                                                             (63, 4, 1, 16, 3), (64, 4, 1, 16, 3), (65, 4, 1, 16, 2)])
 def test_the_workspace_holds_every_part(batch, heads, n_kv, page, width):
-    need = _shares(batch, n_kv, page * width) * 2 * (heads // n_kv * 256 + 32) * 4 + 3 * 4 * SHARES
+    need = _shares(batch, n_kv, page * width) * 2 * (heads // n_kv * 256 + 32) * 4 + 3 * 4 * GROUPS * WAVES
     assert need <= _lib.lib().mspr_sdpa_decode_paged_workspace_bytes(batch, heads, n_kv, page, width) <= need + 64
