@@ -27,9 +27,11 @@
 // Products are exact: 16-bit rows are multiplied as they are and the scale is applied to the sums; 8-bit codes are multiplied
 // as the whole numbers they are. A group's sum over K then takes its scale in float32; a group's scale of V goes into the
 // weights first; biases are products of their own, of float32 matrix instructions (K: biases x sums of the query over a
-// group, V: weights x biases). Weights, and queries whose type has more digits than an operand, go in as two terms of it,
-// the rounded value and the rounded rest (8-bit rows: one for bfloat16 results, which float16 has three digits more than,
-// three for float32 results).
+// group, V: weights x biases). Codes of V are taken from 128 on, and 128 scales go into their biases: of rows around zero, the
+// sums over codes and over biases would be many times the result, and what the weights lose in rounding with them (float32
+// results over 37000 keys: 4.9e-6 off instead of 1.6e-6). Weights, and queries whose type has more digits than an operand, go
+// in as two terms of it, the rounded value and the rounded rest (weights of 8-bit rows for a bfloat16 result, which has three
+// digits fewer than float16: one).
 #include "common.h"
 #include "q8_codes.h"
 
@@ -121,8 +123,8 @@ __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
-// Eight float32 values as terms of eight 16-bit operands each: x ~ t[0] + t[1] (+ t[2]), every term the rounded rest.
-template <int FMT, int TERMS>
+// Eight float32 values as terms of eight 16-bit operands each: x ~ t[0] + t[1] 2^-REST_UP, the second the rounded rest.
+template <int FMT, int TERMS, int REST_UP = 0>
 __device__ __forceinline__ void split_terms(const float* x, u32x4_t* t) {
   float rest[8];
 #pragma unroll
@@ -136,11 +138,12 @@ __device__ __forceinline__ void split_terms(const float* x, u32x4_t* t) {
         t[k][j] = __builtin_bit_cast(uint32_t, h);
         rest[2 * j] -= (float)h.x;
         rest[2 * j + 1] -= (float)h.y;
+        static_assert(FMT != MSPR_BF16 || REST_UP == 0, "only float16 rests need it");
       } else {
         const h2_t h = {(_Float16)rest[2 * j], (_Float16)rest[2 * j + 1]};
         t[k][j] = h2_bits(h);
-        rest[2 * j] -= (float)h.x;
-        rest[2 * j + 1] -= (float)h.y;
+        rest[2 * j] = (rest[2 * j] - (float)h.x) * (float)(1 << REST_UP);
+        rest[2 * j + 1] = (rest[2 * j + 1] - (float)h.y) * (float)(1 << REST_UP);
       }
     }
   }
@@ -158,20 +161,6 @@ __device__ __forceinline__ void widen8(u32x4_t w, float* x) {
       x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
     }
   }
-}
-
-// Sixteen codes to bfloat16, exactly (whole numbers up to 256 are): the upper halves of their float32 values.
-__device__ __forceinline__ void codes_to_bf16(u32x4_t c, u32x4_t& lo, u32x4_t& hi) {
-  uint32_t o[8];
-#pragma unroll
-  for (int w = 0; w < 4; w++) {
-    const float b0 = (float)(c[w] & 0xFFu), b1 = (float)((c[w] >> 8) & 0xFFu), b2 = (float)((c[w] >> 16) & 0xFFu),
-                b3 = (float)(c[w] >> 24);
-    o[2 * w] = __builtin_amdgcn_perm(__float_as_uint(b1), __float_as_uint(b0), 0x07060302u);
-    o[2 * w + 1] = __builtin_amdgcn_perm(__float_as_uint(b3), __float_as_uint(b2), 0x07060302u);
-  }
-  lo = u32x4_t{o[0], o[1], o[2], o[3]};
-  hi = u32x4_t{o[4], o[5], o[6], o[7]};
 }
 
 // One scale or bias a lane, number i of a window. 16-bit ones are loaded with their neighbour, a word: what is done to them
@@ -240,10 +229,14 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   constexpr bool kCodes = FMT == kAffine;
   // Operands of the second product: of 8-bit rows float16, in which the codes cost fewest instructions and a term of a weight
-  // has eleven digits; float32 results want weights without a floor (the rest of a float16 term ends at 2^-25: 1.2e-5 of a
-  // result over 37000 keys), so theirs are three terms of bfloat16 (1.4e-6).
-  constexpr int kVType = !kCodes ? FMT : QDT == MSPR_F32 ? MSPR_BF16 : MSPR_F16;
-  constexpr int kPTerms = kCodes && QDT == MSPR_BF16 ? 1 : QDT == MSPR_F32 ? 3 : 2;  // terms of a weight
+  // has eleven digits. A second term beside the first in one sum ends at float16's 2^-25, which is enough for a float16 result.
+  // Of float32 ones it takes a sum of its own, 2^11 times as large: weights then have 22 digits without a floor that shows (the
+  // error over 37000 keys is 1.2e-5 of the result with one sum, 1.6e-6 with two; three terms of bfloat16 in one sum are as
+  // good and take 79 us where two sums take 77, for 66 requests of 1 to 1985 keys).
+  constexpr int kVType = kCodes ? MSPR_F16 : FMT;
+  constexpr int kPTerms = kCodes && QDT == MSPR_BF16 ? 1 : 2;  // terms of a weight
+  constexpr int kSums = QDT == MSPR_F32 ? 2 : 1;
+  constexpr int kRestUp = kSums == 2 ? 11 : 0;
   constexpr int kQTerms = kCodes && QDT == MSPR_F32 ? 2 : 1;                         // terms of a query element
   // float16 weights are taken 2^11 times as large: up to 2^15, as the reference maximum lags by 2^4 at most, and the smallest
   // that is not lost is 2^-35 of the largest (at 2^-24, the many small weights of a long context would all be rounded one way)
@@ -358,9 +351,18 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
     const int32_t* table = tables + (int64_t)(known ? request : 0) * width;
     const int last_tile = min(tile1, (len + kTileKeys - 1) / kTileKeys);
 
-    f32x4_t oacc[16];
+    f32x4_t oacc[16], orest[kSums == 2 ? 16 : 1];
 #pragma unroll
     for (int mt = 0; mt < 16; mt++) oacc[mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int mt = 0; mt < 16 && kSums == 2; mt++) orest[mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    auto rescale = [&](float by) {
+#pragma unroll
+      for (int mt = 0; mt < 16; mt++) {
+        oacc[mt] = oacc[mt] * by;
+        if constexpr (kSums == 2) orest[mt] = orest[mt] * by;
+      }
+    };
     float m_run = -__builtin_inff(), l_run = 0.0f;
     f32x4_t bacc = {0.f, 0.f, 0.f, 0.f};  // weighted biases: lane n (g = 0) has those of head n and the four groups
     float v_unit = 0x1p-126f;             // what V's scales are multiples of: a power of two from their largest magnitude on
@@ -569,12 +571,13 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
         const bool grow = tmax > m_run + kLag;
         if (__any(grow)) {
           const float m_new = grow ? tmax : m_run;
-          const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
-          l_run *= alpha;
+          if (it > 0) {  // (sums of nothing need no new scale)
+            const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+            l_run *= alpha;
+            rescale(alpha);
+            bacc = bacc * alpha;
+          }
           m_run = m_new;
-#pragma unroll
-          for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] * alpha;
-          bacc = bacc * alpha;
         }
         const float m_safe = (m_run == -__builtin_inff() ? 0.0f : m_run) - kUp;
 #pragma unroll
@@ -592,11 +595,10 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
               *reinterpret_cast<u32x4_t*>(vt + (16 * u + 2 * j + (lane >> 5)) * kVPitch + 16 * (lane & 31)) = vr[u][j];
             } else {
               u32x4_t lo, hi;
-              if constexpr (kVType == MSPR_BF16) codes_to_bf16(vr[u][j], lo, hi);
 #pragma unroll
-              for (int w = 0; w < 4 && kVType == MSPR_F16; w++) {
+              for (int w = 0; w < 4; w++) {
                 h2_t c01, c23;
-                codes4_to_h<kFmtAffine>(vr[u][j][w], c01, c23);
+                codes4_to_h<kFmtQ8_0>(vr[u][j][w] ^ 0x80808080u, c01, c23);  // code - 128, a signed byte
                 (w < 2 ? lo : hi)[2 * (w & 1)] = h2_bits(c01);
                 (w < 2 ? lo : hi)[2 * (w & 1) + 1] = h2_bits(c23);
               }
@@ -630,7 +632,10 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
 #pragma unroll
           for (int t = 0; t < kPTerms; t++)
 #pragma unroll
-            for (int m = 0; m < 4; m++) oacc[4 * q4 + m] = mfma<kVType>(vf[q4 & 1][m], pf[t], oacc[4 * q4 + m]);
+            for (int m = 0; m < 4; m++) {
+              f32x4_t& sum = t == 1 && kSums == 2 ? orest[4 * q4 + m] : oacc[4 * q4 + m];
+              sum = mfma<kVType>(vf[q4 & 1][m], pf[t], sum);
+            }
         };
         read_v(0);
         u32x4_t pf[kPTerms];
@@ -651,16 +656,14 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
             top = half_wave_max(row_pair_max(top));
             const int e = top < 0x1p126f ? __builtin_amdgcn_frexp_expf(top) : 126;
             const float unit = __builtin_amdgcn_ldexpf(1.0f, e);
-            const float down = v_unit / unit;
-#pragma unroll
-            for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] * down;
+            if (it > 0) rescale(v_unit / unit);
             v_unit = unit;
           }
           const float per_unit = 1.0f / v_unit;
           vsf[0] *= per_unit;
           vsf[1] *= per_unit;
           // biases: operand row m has group m of key 16 u + 4 g + i (rows from 4 on are not used)
-          const float vbf[2] = {vb[0].value(n), vb[1].value(n)};
+          const float vbf[2] = {fmaf(128.0f, vs[0].value(n), vb[0].value(n)), fmaf(128.0f, vs[1].value(n), vb[1].value(n))};
           static_for<8>([&](auto ic) {
             constexpr int i = decltype(ic)::value;
             float b = vbf[i >> 2];
@@ -675,7 +678,7 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
               constexpr int i = decltype(ic)::value;
               w[i] = of_lane<4 * (i & 3) + j>(vsf[i >> 2]) * s[i];
             });
-            split_terms<kVType, kPTerms>(w, pf);
+            split_terms<kVType, kPTerms, kRestUp>(w, pf);
             accumulate(j, pf);
           });
         }
@@ -694,7 +697,10 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
 #pragma unroll
       for (int j = 0; j < 4; j++) bias[j] = __shfl(bacc[j], n, MSPR_WAVE);
 #pragma unroll
-      for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] * v_unit + bias[mt >> 2];
+      for (int mt = 0; mt < 16; mt++) {
+        if constexpr (kSums == 2) oacc[mt] += orest[mt] * (1.0f / (1 << kRestUp));
+        oacc[mt] = oacc[mt] * v_unit + bias[mt >> 2];
+      }
     }
     const bool whole = tile0 == 0 && tile1 == row_tiles;
     const int row = at.b * n_kv + at.kvh;
@@ -876,26 +882,25 @@ __global__ __launch_bounds__(64 * kWaves) void paged_merge_many_kernel(const int
   __shared__ __attribute__((aligned(16))) float xo[kWaves][kD + 2];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hn = blockIdx.y;
-  Cut c[kWaves], mine = {0, 0, 0};
-#pragma unroll
-  for (int w = 0; w < kWaves; w++) c[w].load(cut, min(blockIdx.x + gridDim.x * w, entries - 1), rows, shares);
-#pragma unroll
-  for (int w = 0; w < kWaves; w++) {
-    if (blockIdx.x + gridDim.x * w >= entries) c[w].count = 0;
-    if (w == wave) mine = c[w];
-  }
-  if (mine.count > 0 && mine.count <= kAtOnce) {
+  __shared__ Cut entry[kWaves];
+  Cut c = {0, 0, 0};
+  const unsigned e = blockIdx.x + gridDim.x * wave;
+  if (e < entries) c.load(cut, e, rows, shares);
+  if ((threadIdx.x & 63) == 0) entry[wave] = c;
+  if (c.count > 0 && c.count <= kAtOnce) {
     Join join;
-    join.add(ws_o, ws_ml, mine.first, 0, 1, mine.count, rep, hn);
-    store_out<ODT>(out, ((int64_t)mine.row * rep + hn) * kD + 4 * (threadIdx.x & 63), join.o, join.l);
+    join.add(ws_o, ws_ml, c.first, 0, 1, c.count, rep, hn);
+    store_out<ODT>(out, ((int64_t)c.row * rep + hn) * kD + 4 * (threadIdx.x & 63), join.o, join.l);
   }
-#pragma unroll
+  __syncthreads();
+#pragma unroll 1
   for (int w = 0; w < kWaves; w++) {
-    if (c[w].count <= kAtOnce) continue;
+    const int count = __builtin_amdgcn_readfirstlane(entry[w].count);
+    if (count <= kAtOnce) continue;
+    const int first = __builtin_amdgcn_readfirstlane(entry[w].first);
     Join join;
-    for (int p0 = wave; p0 < c[w].count; p0 += kAtOnce * kWaves)
-      join.add(ws_o, ws_ml, c[w].first, p0, kWaves, c[w].count, rep, hn);
-    join_waves<ODT, kWaves>(join, xo, out, ((int64_t)c[w].row * rep + hn) * kD);
+    for (int p0 = wave; p0 < count; p0 += kAtOnce * kWaves) join.add(ws_o, ws_ml, first, p0, kWaves, count, rep, hn);
+    join_waves<ODT, kWaves>(join, xo, out, ((int64_t)__builtin_amdgcn_readfirstlane(entry[w].row) * rep + hn) * kD);
     __syncthreads();
   }
 }

@@ -4,11 +4,12 @@ Tolerance, from the arithmetic. A score is a float32 sum of 256 exact products a
 260 * 2^-24 * A, A = scale * sum |q| |k| at its largest over the keys (natural units; the same relative to the exponent's
 argument for its rounding). An error d of every score moves the result by at most 2 d of sum p |v|. A weight is two terms
 of a 16-bit type, each off by half a step of it (bfloat16 pages 2^-8 of 2^-8 of the weight, float16 operands 2^-11 of 2^-11), or
-one float16 term (8-bit pages, bfloat16 result: 2^-11), or three bfloat16 terms (float32 result: 2^-24); float16 operands
-are taken 2^11 times as large and end at 2^-25, so that n weights lose at most n * 2^-36 of the largest value together (8-bit
-pages: of 255 times twice the largest scale). Sums over n keys run over n / 8 float32 additions at most where four waves
-share a row of keys, over n / 4 where one has it for itself (64 rows or more: a lane adds eight weights of every 32 keys),
-counted for both the weights' and the values' sums; the result is rounded once more, to eps / 2 of its type.
+one float16 term (8-bit pages, bfloat16 result: 2^-11); float16 operands are taken 2^11 times as large and end at 2^-25, so
+that n weights lose at most n * 2^-36 of the largest value together (8-bit pages: of 128 times twice the largest scale),
+n * 2^-47 where the second term is 2^11 times as large again (float32 results). Sums over n keys run over n / 8 float32
+additions at most where four waves share a row of keys, over n / 4 where one has it for itself (64 rows or more: a lane adds
+eight weights of every 32 keys), counted for both the weights' and the values' sums; the result is rounded once more, to
+eps / 2 of its type.
 """
 
 import numpy as np
@@ -65,7 +66,7 @@ def _reference(q, keys, values, tables, lens, scale, requests=None):
     out, bound = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda")
     n_pages, G, page = (keys if torch.is_tensor(keys) else keys[0]).shape[:3]
     rep = q.shape[1] // G
-    terms = 2.0 ** (-16 if torch.is_tensor(keys) and q.dtype == BF16 else -11 if q.dtype == BF16 else -24 if q.dtype == F32 else -22)
+    terms = 2.0 ** (-16 if torch.is_tensor(keys) and q.dtype == BF16 else -11 if q.dtype == BF16 else -22)
     for r in range(q.shape[0]):
         b = r if requests is None else int(requests[r])
         n = min(max(int(lens[r]), 0), tables.shape[1] * page) if 0 <= b < len(tables) else 0
@@ -84,18 +85,19 @@ def _reference(q, keys, values, tables, lens, scale, requests=None):
             size = w @ v.abs()
             out[r, g * rep:(g + 1) * rep] = w @ v
             largest = v.abs().max()
-            if not torch.is_tensor(values):  # codes and biases are summed apart: their magnitudes count, not the values'
+            if not torch.is_tensor(values):  # codes (from 128 on) and biases are summed apart: their magnitudes count, not the values'
                 c, s, z = (_pick(t, p)[:, g] for t in values)
-                c = (c.view(torch.uint8).double() * s.double().repeat_interleave(64, -1)).abs() + z.double().repeat_interleave(64, -1).abs()
+                s, z = (t.double().repeat_interleave(64, -1) for t in (s, z))
+                c = ((c.view(torch.uint8).double() - 128) * s).abs() + (z + 128 * s).abs()
                 size = w @ c.reshape(-1, 256)[keep]
-                largest = 255 * 2 * s.double().abs().reshape(-1, 4)[keep].max()
+                largest = 128 * 2 * s.abs().reshape(-1, 256)[keep].max()
                 c, s, z = (_pick(t, p)[:, g] for t in keys)
                 c = (c.view(torch.uint8).double() * s.double().repeat_interleave(64, -1)).abs() + z.double().repeat_interleave(64, -1).abs()
                 most = (x.abs() @ c.reshape(-1, 256)[keep].t()).amax(-1, keepdim=True) * abs(scale)
             adds = k.shape[0] / (8 if q.shape[0] * G < 64 else 4) + 8
             bound[r, g * rep:(g + 1) * rep] = size * (2 * 260 * 2.0 ** -24 * most + terms + 2 * adds * 2.0 ** -24)
-            if q.dtype == F16 or q.dtype == BF16 and not torch.is_tensor(keys):
-                bound[r, g * rep:(g + 1) * rep] += k.shape[0] * 2.0 ** -36 * largest
+            if q.dtype != BF16 or not torch.is_tensor(keys):
+                bound[r, g * rep:(g + 1) * rep] += k.shape[0] * 2.0 ** (-47 if q.dtype == F32 else -36) * largest
     return out, bound
 
 
