@@ -199,7 +199,7 @@ def q8_decode_workspace(batch: int, n_kv_heads: int, n_keys: int, device) -> tor
 
 def paged_decode_workspace(batch: int, n_q_heads: int, n_kv_heads: int, page_size: int, table_width: int,
                            device) -> torch.Tensor:
-    """Scratch tensor for the paged decode entry points (per-range partials, the plan of the ranges)."""
+    """Scratch tensor for the paged decode entry points (partials of the rows that are cut, and which are)."""
     nbytes = int(lib().mspr_sdpa_decode_paged_workspace_bytes(int(batch), int(n_q_heads), int(n_kv_heads), int(page_size),
                                                               int(table_width)))
     return torch.empty((max(nbytes, 16) + 3) // 4, dtype=torch.float32, device=device)

@@ -652,7 +652,8 @@ Tensor part(const Tensor& of, int64_t offset, int64_t n) {
   return Tensor(std::move(impl));
 }
 
-// (lens, new_lens int32 [B], tables int32 [B, P], free_pages int32 [n], head int32 [1], page_size, n_rows) -> the eight parts of a step
+// (lens, new_lens int32 [B], tables int32 [B, P], free_pages int32 [n], head int32 [1], page_size, n_rows) -> the eight parts
+// of a step
 PyObject* page_step(PyObject* const* a, Py_ssize_t nargs) {
   MSPR_NARGS(7)
   const Tensor *lens = dense(a[0], 1, at::kInt), *add = dense(a[1], 1, at::kInt), *tables = dense(a[2], 2, at::kInt),

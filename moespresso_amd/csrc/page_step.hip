@@ -5,10 +5,11 @@
 // page) for every new row. Four running sums over the requests decide everything: rows asked for, pages needed, pages given
 // back; each page that moves and each row then finds its request by bisection of a sum.
 //
-// Bound by latency: a step of 16 requests reads 128 bytes and writes 500. One launch; every workgroup makes the sums anew
-// (2048 requests are eight a thread) rather than wait for another's, and writes its share of the rows. What one workgroup
-// writes no other reads: pages given back go below `head` and pages taken from there are read where they come from, the table
-// of the ended request; new table entries lie behind those that rows of the last started page read.
+// Bound by latency: a step of 16 requests reads 128 bytes and writes 500, in 2.9 us; one of 1000, of which some end, takes 6.7.
+// One launch; every workgroup makes the sums anew (2048 requests are eight a thread) rather than wait for another's, and writes
+// its share of the rows. What one workgroup writes no other reads: pages given back go below `head` and pages taken from there
+// are read where they come from, the table of the ended request; new table entries lie behind those that rows of the last
+// started page read.
 #include "common.h"
 
 namespace {

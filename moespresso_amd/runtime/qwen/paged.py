@@ -333,8 +333,8 @@ def sdpa_decode_paged_q8(queries, k_wq, k_scales, k_biases, v_wq, v_scales, v_bi
     """``sdpa_decode_paged`` over pages of affine 8-bit rows (``kquant``'s layout within a page).
 
     Args:
-        queries: ``[R, Hq, 256]`` float32, float16 or bfloat16. The codes are multiplied as whole numbers and the weights in
-            two (float32 queries: three) terms, so that float32 queries keep float32 results.
+        queries: ``[R, Hq, 256]`` float32, float16 or bfloat16. The codes are multiplied as whole numbers, and weights
+            and float32 queries in two terms each, so that float32 queries keep float32 results.
         k_wq, v_wq: uint32 codes ``[n_pages, Hkv, page_size, 64]``; scales and biases ``[n_pages, Hkv, page_size, 4]``.
         tables, lens, requests, scale: as for ``sdpa_decode_paged``.
     """
@@ -425,12 +425,14 @@ class PagedAttention(torch.nn.Module):
 
     ``inner`` is a block as ``full_attention.FlashPrefillD256Attention`` wraps it; of its modules this takes ``q_proj`` (with
     the output gate in the second half of every head), ``k_proj``, ``v_proj``, ``o_proj``, ``q_norm`` and ``k_norm``
-    (``weight``, ``eps``), ``rope`` (``inv_freq`` and, for three position axes, ``sections``), ``scale``,
+    (``weight`` and one ``eps``), ``rope`` (``inv_freq`` and, for three position axes, ``sections``), ``scale``,
     ``num_attention_heads`` and ``num_key_value_heads``.
     """
 
     def __init__(self, inner, cache: PagedKVCache):
         super().__init__()
+        if inner.q_norm.eps != inner.k_norm.eps:
+            raise ValueError("q_norm and k_norm must share an eps")
         self.inner = inner
         self.cache = cache
 

@@ -242,3 +242,15 @@ def test_operands_on_different_devices_are_refused():
     with FakeTensorMode(), pytest.raises(RuntimeError, match="same HIP device"):
         paged.page_step(_on("cuda:0", 3, dtype=I32), _on("cuda:1", 3, dtype=I32), _on("cuda:0", 3, 5, dtype=I32),
                         _on("cuda:0", 20, dtype=I32), _on("cuda:0", 1, dtype=I32), page_size=16, n_rows=3)
+
+
+def test_norms_of_two_eps_are_refused():
+    class Norm:
+        def __init__(self, eps):
+            self.eps = eps
+
+    class Block:
+        q_norm, k_norm = Norm(1e-6), Norm(1e-5)
+
+    with pytest.raises(ValueError, match="share an eps"):
+        paged.PagedAttention(Block(), None)
