@@ -351,8 +351,8 @@ int mspr_sdpa_fa_prefill_q8(const void* queries, const void* pk_wq, const void* 
  * head_out int32 [1], starts int32 [batch + 1] (first row of every request and the end), per row of n_rows: slots (-1: no page
  * was left, the table is full, or the row belongs to no request), positions, visible (the rows of its request up to itself, 0
  * without a slot) and requests (-1 behind the last), counts int32 [4]: rows asked for, of them without a slot, pages taken,
- * pages given back. A row without a slot is not in lens_out. Rows
- * asked for behind n_rows are not part of the step. A call on the same lens and head again writes the same. */
+ * pages given back. A row without a slot is not in lens_out. Rows asked for behind n_rows are not part of the step. A call on
+ * the same lens and head again writes the same. */
 int mspr_page_step(const int32_t* lens, const int32_t* new_lens, int32_t* tables, int32_t* free_pages, const int32_t* head,
                    int batch, int table_width, int n_pages, int page_size, int n_rows, int32_t* lens_out, int32_t* head_out,
                    int32_t* starts, int32_t* slots, int32_t* positions, int32_t* visible, int32_t* requests, int32_t* counts,
@@ -395,8 +395,8 @@ size_t mspr_sdpa_decode_paged_workspace_bytes(int batch, int n_q_heads, int n_kv
  * table_width * page_size) that the query's table names, 0 where there are none. The table is tables[requests[b]] of n_tables
  * (none for a request that is not among them), or tables[b] where requests is NULL and n_tables = batch; several queries may
  * name one request (new rows of a chunk, each with the rows that it sees). Lengths, requests and tables are read on the
- * device, so that a captured call follows them. Entries behind a request's rows may hold anything, as may the rows behind them in a page;
- * rows of a page that is not in the pool are left out.
+ * device, so that a captured call follows them. Entries behind a request's rows may hold anything, as may the rows behind them
+ * in a page; rows of a page that is not in the pool are left out.
  * queries, out: [batch][n_q_heads][256] of dtype (f16|bf16), pages of the same; n_q_heads / n_kv_heads <= 16. */
 int mspr_sdpa_decode_paged(const void* queries, const void* k_pages, const void* v_pages, int dtype, const int32_t* tables,
                            const int32_t* lens, const int32_t* requests, int batch, int n_q_heads, int n_kv_heads,
