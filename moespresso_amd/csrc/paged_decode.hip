@@ -27,9 +27,9 @@
 // Products are exact: 16-bit rows are multiplied as they are and the scale is applied to the sums; 8-bit codes are multiplied
 // as the whole numbers they are. A group's sum over K then takes its scale in float32; a group's scale of V goes into the
 // weights first; biases are products of their own, of float32 matrix instructions (K: biases x sums of the query over a
-// group, V: weights x biases). Codes of V are taken from 128 on, and 128 scales go into their biases: of rows around zero, the
-// sums over codes and over biases would be many times the result, and what the weights lose in rounding with them (float32
-// results over 37000 keys: 4.9e-6 off instead of 1.6e-6). Weights, and queries whose type has more digits than an operand, go
+// group, V: weights x biases). Codes count from 128 on, and 128 scales go into the biases: of rows around zero, the sums over
+// codes and over biases would be many times the result, and what is lost in them (float32 results over 37000 keys are 0.5e-6
+// off, 0.9e-6 with K's codes from 0 on, 4.9e-6 with V's). Weights, and queries whose type has more digits than an operand, go
 // in as two terms of it, the rounded value and the rounded rest (weights of 8-bit rows for a bfloat16 result, which has three
 // digits fewer than float16: one).
 #include "common.h"
@@ -123,8 +123,8 @@ __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
-// Eight float32 values as terms of eight 16-bit operands each: x ~ t[0] + t[1] 2^-REST_UP, the second the rounded rest.
-template <int FMT, int TERMS, int REST_UP = 0>
+// Eight float32 values as terms of eight 16-bit operands each: x ~ t[0] + t[1], the second the rounded rest.
+template <int FMT, int TERMS>
 __device__ __forceinline__ void split_terms(const float* x, u32x4_t* t) {
   float rest[8];
 #pragma unroll
@@ -138,12 +138,11 @@ __device__ __forceinline__ void split_terms(const float* x, u32x4_t* t) {
         t[k][j] = __builtin_bit_cast(uint32_t, h);
         rest[2 * j] -= (float)h.x;
         rest[2 * j + 1] -= (float)h.y;
-        static_assert(FMT != MSPR_BF16 || REST_UP == 0, "only float16 rests need it");
       } else {
         const h2_t h = {(_Float16)rest[2 * j], (_Float16)rest[2 * j + 1]};
         t[k][j] = h2_bits(h);
-        rest[2 * j] = (rest[2 * j] - (float)h.x) * (float)(1 << REST_UP);
-        rest[2 * j + 1] = (rest[2 * j + 1] - (float)h.y) * (float)(1 << REST_UP);
+        rest[2 * j] -= (float)h.x;
+        rest[2 * j + 1] -= (float)h.y;
       }
     }
   }
@@ -162,6 +161,9 @@ __device__ __forceinline__ void widen8(u32x4_t w, float* x) {
     }
   }
 }
+
+// Four affine codes less 128 (signed bytes, were their upper bits turned) to float16, exactly.
+__device__ __forceinline__ void centred_to_h(uint32_t w, h2_t& lo, h2_t& hi) { codes4_to_h<kFmtQ8_0>(w ^ 0x80808080u, lo, hi); }
 
 // One scale or bias a lane, number i of a window. 16-bit ones are loaded with their neighbour, a word: what is done to them
 // behind the load (a load of 16 bits is masked) is done, and waited for, a tile too early.
@@ -229,14 +231,10 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   constexpr bool kCodes = FMT == kAffine;
   // Operands of the second product: of 8-bit rows float16, in which the codes cost fewest instructions and a term of a weight
-  // has eleven digits. A second term beside the first in one sum ends at float16's 2^-25, which is enough for a float16 result.
-  // Of float32 ones it takes a sum of its own, 2^11 times as large: weights then have 22 digits without a floor that shows (the
-  // error over 37000 keys is 1.2e-5 of the result with one sum, 1.6e-6 with two; three terms of bfloat16 in one sum are as
-  // good and take 79 us where two sums take 77, for 66 requests of 1 to 1985 keys).
+  // has eleven digits (three terms of bfloat16 are as exact; 66 requests of 1 to 1985 keys with float32 queries took 79 us with
+  // them, 73 with these).
   constexpr int kVType = kCodes ? MSPR_F16 : FMT;
   constexpr int kPTerms = kCodes && QDT == MSPR_BF16 ? 1 : 2;  // terms of a weight
-  constexpr int kSums = QDT == MSPR_F32 ? 2 : 1;
-  constexpr int kRestUp = kSums == 2 ? 11 : 0;
   constexpr int kQTerms = kCodes && QDT == MSPR_F32 ? 2 : 1;                         // terms of a query element
   // float16 weights are taken 2^11 times as large: up to 2^15, as the reference maximum lags by 2^4 at most, and the smallest
   // that is not lost is 2^-35 of the largest (at 2^-24, the many small weights of a long context would all be rounded one way)
@@ -351,17 +349,12 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
     const int32_t* table = tables + (int64_t)(known ? request : 0) * width;
     const int last_tile = min(tile1, (len + kTileKeys - 1) / kTileKeys);
 
-    f32x4_t oacc[16], orest[kSums == 2 ? 16 : 1];
+    f32x4_t oacc[16];
 #pragma unroll
     for (int mt = 0; mt < 16; mt++) oacc[mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int mt = 0; mt < 16 && kSums == 2; mt++) orest[mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     auto rescale = [&](float by) {
 #pragma unroll
-      for (int mt = 0; mt < 16; mt++) {
-        oacc[mt] = oacc[mt] * by;
-        if constexpr (kSums == 2) orest[mt] = orest[mt] * by;
-      }
+      for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] * by;
     };
     float m_run = -__builtin_inff(), l_run = 0.0f;
     f32x4_t bacc = {0.f, 0.f, 0.f, 0.f};  // weighted biases: lane n (g = 0) has those of head n and the four groups
@@ -454,8 +447,8 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
 #pragma unroll
         for (int j = 0; j < 8; j++) x[j] = mine ? x[j] : 0.0f;
       };
-      // The operand is float16: a power of two brings the head's largest element to [1, 2), so that what falls below
-      // float16's range is 2^-25 of it; float16 queries go in as they are.
+      // The operand is float16: a power of two brings the head's largest element to [2^14, 2^15), so that what falls below
+      // float16's range is 2^-39 of it; float16 queries go in as they are.
       float* shared = reinterpret_cast<float*>(lds);  // [2][waves][16 heads], where the V tiles will be
       int e = 0;
       if constexpr (QDT != MSPR_F16) {
@@ -474,7 +467,7 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
 #pragma unroll
           for (int w = 0; w < kWaves; w++) top = fmaxf(top, shared[16 * w + n]);
         }
-        if (top > 0.0f && top < __builtin_inff()) e = __builtin_amdgcn_frexp_expf(top) - 1;
+        if (top > 0.0f && top < __builtin_inff()) e = __builtin_amdgcn_frexp_expf(top) - 15;
       }
       float sums[kSteps / 2] = {};  // by group
 #pragma unroll
@@ -484,10 +477,17 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
 #pragma unroll
         for (int j = 0; j < 8; j++) {
           x[j] = __builtin_amdgcn_ldexpf(x[j], -e);
-          sums[i / 2] += x[j];
         }
         u32x4_t terms[kQTerms];
         split_terms<MSPR_F16, kQTerms>(x, terms);
+        // (of the terms, as the products are: what the two have too little is then multiplied with a value, not with its code)
+#pragma unroll
+        for (int t = 0; t < kQTerms; t++) {
+          float y[8];
+          widen8<MSPR_F16>(terms[t], y);
+#pragma unroll
+          for (int j = 0; j < 8; j++) sums[i / 2] += y[j];
+        }
 #pragma unroll
         for (int t = 0; t < kQTerms; t++) qt[64 * ((step0 + i) * kQTerms + t)] = terms[t];
       }
@@ -528,8 +528,9 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
             for (int i = 0; i < 4; i++) s[4 * u + i] = acc[i] * q_unit;
           } else {
             const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
-            f32x4_t sum = __builtin_amdgcn_mfma_f32_16x16x4f32(kb[u].value(g), qsum, zero, 0, 0, 0);
             const float ksf = ks[u].value(n);
+            const float of_bias = __int_as_float(__builtin_amdgcn_ds_bpermute(4 * (4 * n + g), __float_as_int(ksf)));
+            f32x4_t sum = __builtin_amdgcn_mfma_f32_16x16x4f32(fmaf(128.0f, of_bias, kb[u].value(g)), qsum, zero, 0, 0, 0);
             static_for<4>([&](auto jc) {
               constexpr int j = decltype(jc)::value;
               f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
@@ -539,7 +540,7 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
 #pragma unroll
                 for (int w = 0; w < 2; w++) {
                   h2_t lo, hi;
-                  codes4_to_h<kFmtAffine>(kr[u][j][2 * h + w], lo, hi);
+                  centred_to_h(kr[u][j][2 * h + w], lo, hi);
                   c[2 * w] = h2_bits(lo);
                   c[2 * w + 1] = h2_bits(hi);
                 }
@@ -598,7 +599,7 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
 #pragma unroll
               for (int w = 0; w < 4; w++) {
                 h2_t c01, c23;
-                codes4_to_h<kFmtQ8_0>(vr[u][j][w] ^ 0x80808080u, c01, c23);  // code - 128, a signed byte
+                centred_to_h(vr[u][j][w], c01, c23);
                 (w < 2 ? lo : hi)[2 * (w & 1)] = h2_bits(c01);
                 (w < 2 ? lo : hi)[2 * (w & 1) + 1] = h2_bits(c23);
               }
@@ -632,10 +633,7 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
 #pragma unroll
           for (int t = 0; t < kPTerms; t++)
 #pragma unroll
-            for (int m = 0; m < 4; m++) {
-              f32x4_t& sum = t == 1 && kSums == 2 ? orest[4 * q4 + m] : oacc[4 * q4 + m];
-              sum = mfma<kVType>(vf[q4 & 1][m], pf[t], sum);
-            }
+            for (int m = 0; m < 4; m++) oacc[4 * q4 + m] = mfma<kVType>(vf[q4 & 1][m], pf[t], oacc[4 * q4 + m]);
         };
         read_v(0);
         u32x4_t pf[kPTerms];
@@ -677,8 +675,11 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
             static_for<8>([&](auto ic) {
               constexpr int i = decltype(ic)::value;
               w[i] = of_lane<4 * (i & 3) + j>(vsf[i >> 2]) * s[i];
+              // (a rounded product: else the compiler makes a term's operand from that and what it takes off for the rest from
+              // the exact product, and where the two round apart the weight is off by a step of the first term)
+              asm("" : "+v"(w[i]));
             });
-            split_terms<kVType, kPTerms, kRestUp>(w, pf);
+            split_terms<kVType, kPTerms>(w, pf);
             accumulate(j, pf);
           });
         }
@@ -697,10 +698,7 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
 #pragma unroll
       for (int j = 0; j < 4; j++) bias[j] = __shfl(bacc[j], n, MSPR_WAVE);
 #pragma unroll
-      for (int mt = 0; mt < 16; mt++) {
-        if constexpr (kSums == 2) oacc[mt] += orest[mt] * (1.0f / (1 << kRestUp));
-        oacc[mt] = oacc[mt] * v_unit + bias[mt >> 2];
-      }
+      for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] * v_unit + bias[mt >> 2];
     }
     const bool whole = tile0 == 0 && tile1 == row_tiles;
     const int row = at.b * n_kv + at.kvh;

@@ -5,11 +5,10 @@ Tolerance, from the arithmetic. A score is a float32 sum of 256 exact products a
 argument for its rounding). An error d of every score moves the result by at most 2 d of sum p |v|. A weight is two terms
 of a 16-bit type, each off by half a step of it (bfloat16 pages 2^-8 of 2^-8 of the weight, float16 operands 2^-11 of 2^-11), or
 one float16 term (8-bit pages, bfloat16 result: 2^-11); float16 operands are taken 2^11 times as large and end at 2^-25, so
-that n weights lose at most n * 2^-36 of the largest value together (8-bit pages: of 128 times twice the largest scale),
-n * 2^-47 where the second term is 2^11 times as large again (float32 results). Sums over n keys run over n / 8 float32
-additions at most where four waves share a row of keys, over n / 4 where one has it for itself (64 rows or more: a lane adds
-eight weights of every 32 keys), counted for both the weights' and the values' sums; the result is rounded once more, to
-eps / 2 of its type.
+that n weights lose at most n * 2^-36 of the largest value together (8-bit pages: of 128 times twice the largest scale). Sums
+over n keys run over n / 8 float32 additions at most where four waves share a row of keys, over n / 4 where one has it for
+itself (64 rows or more: a lane adds eight weights of every 32 keys), counted for both the weights' and the values' sums; the
+result is rounded once more, to eps / 2 of its type.
 """
 
 import numpy as np
@@ -92,12 +91,13 @@ def _reference(q, keys, values, tables, lens, scale, requests=None):
                 size = w @ c.reshape(-1, 256)[keep]
                 largest = 128 * 2 * s.abs().reshape(-1, 256)[keep].max()
                 c, s, z = (_pick(t, p)[:, g] for t in keys)
-                c = (c.view(torch.uint8).double() * s.double().repeat_interleave(64, -1)).abs() + z.double().repeat_interleave(64, -1).abs()
+                s, z = (t.double().repeat_interleave(64, -1) for t in (s, z))
+                c = ((c.view(torch.uint8).double() - 128) * s).abs() + (z + 128 * s).abs()
                 most = (x.abs() @ c.reshape(-1, 256)[keep].t()).amax(-1, keepdim=True) * abs(scale)
             adds = k.shape[0] / (8 if q.shape[0] * G < 64 else 4) + 8
             bound[r, g * rep:(g + 1) * rep] = size * (2 * 260 * 2.0 ** -24 * most + terms + 2 * adds * 2.0 ** -24)
             if q.dtype != BF16 or not torch.is_tensor(keys):
-                bound[r, g * rep:(g + 1) * rep] += k.shape[0] * 2.0 ** (-47 if q.dtype == F32 else -36) * largest
+                bound[r, g * rep:(g + 1) * rep] += k.shape[0] * 2.0 ** -36 * largest
     return out, bound
 
 
@@ -271,6 +271,18 @@ def test_sharp_and_flat_weights():
         q = torch.zeros(1, 4, 256, dtype=dtype, device="cuda")
         q[0, :, 0] = torch.tensor([0.0, 13.8629, 30.0, 80.0])
         _check(q, keys, values, tables, [n], scale=1.0)
+
+
+@pytest.mark.parametrize("dtype,form", [(F32, F32), (F32, BF16), (F16, F16), (BF16, BF16)])
+@pytest.mark.parametrize("batch", [3, 300])
+def test_every_weight_keeps_its_digits(batch, dtype, form):
+    """Small queries, whose scores are off by next to nothing, over few keys: a weight of which a term is off by a step of its
+    type shows. 300 requests meet 150000 products of a weight and a scale."""
+    rng = np.random.default_rng(batch)
+    lens = [int(n) for n in rng.integers(1, 12, batch)]
+    keys, values = _cache(rng, (batch + 1, 1, 16, 256), dtype, form)
+    q = _rows(rng, (batch, 16, 256), dtype) * 2.0 ** -9
+    _check(q, keys, values, _tables(rng, lens, 16, 1, batch + 1), lens)
 
 
 def test_large_queries_of_8_bit_rows():
