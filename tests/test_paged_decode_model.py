@@ -20,9 +20,17 @@ def _most(batch, n_kv):
 
 
 def _shares(batch, n_kv, cap):
+    return min(_most(batch, n_kv)[0], -(-batch * n_kv * _row_tiles(cap) // MIN_TILES))
+
+
+def _numbers(batch, n_kv, cap, lens):
+    """The share of every wave (of few rows: of every workgroup) that is launched."""
     most, waves = _most(batch, n_kv)
-    unit = WAVES // waves
-    return min(most, -(-(-(-batch * n_kv * _row_tiles(cap) // MIN_TILES)) // unit) * unit)
+    groups = min(GROUPS, _shares(batch, n_kv, cap))
+    if waves == WAVES:
+        return list(range(groups))
+    spread = sum(_row_tiles(n) for n in lens) * n_kv <= MIN_TILES * GROUPS * (WAVES // 2)
+    return [g + groups * w if spread else g * WAVES + w for g in range(groups) for w in range(WAVES)]
 
 
 def _parts(wg, lens, n_kv):
@@ -101,7 +109,10 @@ def test_every_row_is_attended_once_and_every_address_lies_in_its_buffer(kind, b
     assert merged == slots and not written & set(merged) and len(written) + len(merged) == batch * n_kv
     assert all(0 <= s < 2 * grid for part in slots.values() for s in part)
     assert len({s for part in slots.values() for s in part}) == sum(len(part) for part in slots.values())
-    assert not _parts(grid, lens, n_kv)[0]  # nothing is left over
+    # every share with work has one wave, and nothing is left over; waves without work stay in the table of cuts
+    numbers = _numbers(batch, n_kv, cap, lens)
+    assert len(set(numbers)) == len(numbers) and set(range(grid)) <= set(numbers) and max(numbers) < most
+    assert not any(_parts(n, lens, n_kv)[0] for n in set(numbers) - set(range(grid))) and not _parts(grid, lens, n_kv)[0]
     if _row_tiles(cap) == MIN_TILES and batch * n_kv <= most:
         assert not merged  # the merge is not launched
 
