@@ -29,7 +29,7 @@
 // weights first; biases are products of their own, of float32 matrix instructions (K: biases x sums of the query over a
 // group, V: weights x biases). Codes count from 128 on, and 128 scales go into the biases: of rows around zero, the sums over
 // codes and over biases would be many times the result, and what is lost in them (float32 results over 37000 keys are 0.5e-6
-// off, 0.9e-6 with K's codes from 0 on, 4.9e-6 with V's). Weights, and queries whose type has more digits than an operand, go
+// off, 0.9e-6 with K's codes from 0 on, 1.8e-6 with V's). Weights, and queries whose type has more digits than an operand, go
 // in as two terms of it, the rounded value and the rounded rest (weights of 8-bit rows for a bfloat16 result, which has three
 // digits fewer than float16: one).
 #include "common.h"
