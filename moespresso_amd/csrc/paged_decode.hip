@@ -50,6 +50,13 @@ constexpr int kNonTemporal = 2;    // cache policy of loads that are used once
 // Tiles of a share, and what a row counts for, at least. (Four, a tile a wave: a request of 8191 rows 10.2 us, not 8.2.)
 constexpr int kMinTiles = 2;
 
+// What a part of a row costs beside its tiles (query, page numbers, first loads, output: 10000 cycles, a tile 6000), in tiles of a
+// share of four waves, and of one. A row counts for so many more, so that a share with several parts has fewer tiles: without
+// that, those ended last (1712 rows of 0 to 612 8-bit keys 91 us, 78 with it; 528 of 1 to 1985 with float32 queries 74 and 63;
+// 2 of 37000 with float32 queries 23.8 and 20.8; 16 of 0 to 2000 keys 14.8 and 11.3). No more than a share, which costs and
+// tiles then fill about evenly (with half a share, 512 rows of 1 to 300 keys 30 us instead of 27.5).
+constexpr int kGroupCost = 8, kWaveCost = 2;
+
 // Rows of tiles from which on waves take shares of their own. Shares of workgroups and of waves, in us: 2 rows of 8191 keys 12.1
 // and 16.0, 32 ragged ones (8-bit) 186 and 190, 64 of 0 to 3000 keys 32 and 30, 128 ragged ones 161 and 159, 256 of 0 to
 // 8000 keys (8-bit) 118 and 107, 528 of 1 to 1985 keys (float32 queries, 8-bit) 129 and 78, 1712 of 0 to 612 keys (8-bit) 169
@@ -282,6 +289,9 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
     all = __builtin_amdgcn_readlane(in_lanes, 63);
   }
   all *= n_kv;
+  // (none where no row is longer than the smallest share: none is cut then, and the second kernel is not launched)
+  const int cost = cap <= kMinTiles * kTileKeys ? 0 : min(ALONE ? kWaveCost : kGroupCost, (all + kShares - 1) / kShares);
+  all += cost * n_kv * batch;
   int share = (all + kShares - 1) / kShares;
   share = share < kMinTiles ? kMinTiles : share;
   // Number of the share. Up to two a workgroup, waves' shares go round the workgroups, to be on as many compute units as can be
@@ -302,10 +312,12 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
     return beyond ? __builtin_ctzll(beyond) : MSPR_WAVE - 1;
   };
   if (chunks > 1) {
-    const int i = first_beyond(in_lanes);
+    const int i = first_beyond(in_lanes + cost * min((lane + 1) * per_lane * MSPR_WAVE, batch));
     before = __builtin_amdgcn_readlane(in_lanes, i) - __builtin_amdgcn_readlane(chunk_sum, i);
-    for (chunk = min(i * per_lane, chunks - 1); chunk < chunks - 1; chunk++) {
-      const int sum = __builtin_amdgcn_readfirstlane(chunk_sums[chunk]);
+    chunk = min(i * per_lane, chunks - 1);
+    before += cost * chunk * MSPR_WAVE;
+    for (; chunk < chunks - 1; chunk++) {
+      const int sum = __builtin_amdgcn_readfirstlane(chunk_sums[chunk]) + cost * MSPR_WAVE;
       if ((before + sum) * n_kv > pos) break;
       before += sum;
     }
@@ -313,8 +325,9 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
     sums0 = wave_scan(tiles0);
   }
   {
+    sums0 += cost * min(lane + 1, batch - chunk * MSPR_WAVE);
     const int i = first_beyond(before + sums0);
-    const int t = __builtin_amdgcn_readlane(tiles0, i);
+    const int t = __builtin_amdgcn_readlane(tiles0, i) + cost;
     at.b = chunk * MSPR_WAVE + i;
     at.len = __builtin_amdgcn_readlane(len0, i);
     at.tile = pos - (before + __builtin_amdgcn_readlane(sums0, i) - t) * n_kv;
@@ -325,9 +338,23 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
     if (at.b >= batch) return;
   }
 
+  auto go_on = [&](int by) {  // to the next row, if the share reaches it
+    pos += by;
+    if (pos >= end) return false;
+    at.tile = 0;
+    if (++at.kvh < n_kv) return true;
+    at.kvh = 0;
+    if (++at.b >= batch) return false;
+    at.len = __builtin_amdgcn_readfirstlane(length_of(lens, batch, at.b, cap));
+    return true;
+  };
   for (;;) {
     const int row_tiles = tiles_of(at.len);
     const int tile0 = at.tile;
+    if (tile0 >= row_tiles) {  // (a share may begin in a row's cost, which lies behind its tiles)
+      if (!go_on(row_tiles + cost - tile0)) return;
+      continue;
+    }
     const int tile1 = min(tile0 + (end - pos), row_tiles);
 
     // ---- the query is asked for first: loads come back in order, and the pages' addresses wait for the table anyway
@@ -760,14 +787,7 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
         c[2] = min(number + (row_tiles - tile1 + share - 1) / share, (int)gridDim.x * (ALONE ? kWaves : 1) - 1);
       }
     }
-    pos += tile1 - tile0;
-    if (pos >= end) return;
-    at.tile = 0;
-    if (++at.kvh == n_kv) {
-      at.kvh = 0;
-      if (++at.b >= batch) return;
-      at.len = __builtin_amdgcn_readfirstlane(length_of(lens, batch, at.b, cap));
-    }
+    if (!go_on(row_tiles + cost - tile0)) return;
     if constexpr (ALONE) __builtin_amdgcn_wave_barrier();
     else __syncthreads();
   }
@@ -916,10 +936,11 @@ int64_t row_tiles_most(int64_t cap) {
 
 bool paged_alone(int batch, int n_kv) { return (int64_t)batch * n_kv >= kManyRows; }
 
-// Shares: no more than the tiles of full tables give.
+// Shares: no more than the tiles of full tables give, with their rows' costs (at most kMinTiles where there are too few tiles
+// for all shares, as a cost is at most a share).
 int paged_shares(int batch, int n_kv, int64_t cap) {
   const int most = kMaxGroups * (paged_alone(batch, n_kv) ? kWaves : 1);
-  const int64_t n = (batch * n_kv * row_tiles_most(cap) + kMinTiles - 1) / kMinTiles;
+  const int64_t n = (batch * n_kv * (row_tiles_most(cap) + kMinTiles) + kMinTiles - 1) / kMinTiles;
   return (int)(n < most ? n : most);
 }
 

@@ -7,6 +7,7 @@ import pytest
 from moespresso_amd import _lib
 
 TILE, WAVES, GROUPS, MIN_TILES, MANY_ROWS = 32, 4, 256, 2, 64
+GROUP_COST, WAVE_COST = 8, 2
 
 
 def _row_tiles(n):
@@ -20,7 +21,16 @@ def _most(batch, n_kv):
 
 
 def _shares(batch, n_kv, cap):
-    return min(_most(batch, n_kv)[0], -(-batch * n_kv * _row_tiles(cap) // MIN_TILES))
+    return min(_most(batch, n_kv)[0], -(-batch * n_kv * (_row_tiles(cap) + MIN_TILES) // MIN_TILES))
+
+
+def _line(lens, n_kv, cap):
+    """Length of the line of all rows, what a row counts for beside its tiles, and the shares' length."""
+    most, waves = _most(len(lens), n_kv)
+    tiles = sum(_row_tiles(n) for n in lens) * n_kv
+    cost = 0 if cap <= MIN_TILES * TILE else min(GROUP_COST if waves == WAVES else WAVE_COST, -(-tiles // most))
+    total = tiles + cost * n_kv * len(lens)
+    return total, cost, max(MIN_TILES, -(-total // most))
 
 
 def _numbers(batch, n_kv, cap, lens):
@@ -29,14 +39,13 @@ def _numbers(batch, n_kv, cap, lens):
     groups = min(GROUPS, _shares(batch, n_kv, cap))
     if waves == WAVES:
         return list(range(groups))
-    spread = sum(_row_tiles(n) for n in lens) * n_kv <= MIN_TILES * GROUPS * (WAVES // 2)
+    spread = _line(lens, n_kv, cap)[0] <= MIN_TILES * GROUPS * (WAVES // 2)
     return [g + groups * w if spread else g * WAVES + w for g in range(groups) for w in range(WAVES)]
 
 
-def _parts(wg, lens, n_kv):
+def _parts(wg, lens, n_kv, cap):
     """The parts of rows that share wg holds: (request, KV head, first tile, end tile, tiles of the row), and its share."""
-    total = sum(_row_tiles(n) for n in lens) * n_kv
-    share = max(MIN_TILES, -(-total // _most(len(lens), n_kv)[0]))
+    total, cost, share = _line(lens, n_kv, cap)
     pos, end = wg * share, min((wg + 1) * share, total)
     parts, before = [], 0
     for b, n in enumerate(lens):
@@ -45,7 +54,7 @@ def _parts(wg, lens, n_kv):
             lo, hi = max(pos, before), min(end, before + t)
             if lo < hi:
                 parts.append((b, kvh, lo - before, hi - before, t))
-            before += t
+            before += t + cost
     return parts, share
 
 
@@ -80,7 +89,7 @@ def test_every_row_is_attended_once_and_every_address_lies_in_its_buffer(kind, b
     cuts, written = {}, set()
     grid = _shares(batch, n_kv, cap)
     for wg in range(grid):
-        parts, share = _parts(wg, lens, n_kv)
+        parts, share = _parts(wg, lens, n_kv, cap)
         for b, kvh, tile0, tile1, row_tiles in parts:
             assert (b, kvh) not in written
             if tile0 == 0 and tile1 == row_tiles:
@@ -112,9 +121,20 @@ def test_every_row_is_attended_once_and_every_address_lies_in_its_buffer(kind, b
     # every share with work has one wave, and nothing is left over; waves without work stay in the table of cuts
     numbers = _numbers(batch, n_kv, cap, lens)
     assert len(set(numbers)) == len(numbers) and set(range(grid)) <= set(numbers) and max(numbers) < most
-    assert not any(_parts(n, lens, n_kv)[0] for n in set(numbers) - set(range(grid))) and not _parts(grid, lens, n_kv)[0]
+    assert not any(_parts(n, lens, n_kv, cap)[0] for n in set(numbers) - set(range(grid)))
+    assert not _parts(grid, lens, n_kv, cap)[0]
     if _row_tiles(cap) == MIN_TILES and batch * n_kv <= most:
         assert not merged  # the merge is not launched
+
+
+@pytest.mark.parametrize("n_kv", [1, 2, 8])
+def test_no_share_with_work_is_behind_those_that_are_launched(n_kv):
+    rng = np.random.default_rng(n_kv)
+    for batch in (1, 2, 3, 7, 8, 31, 32, 63, 64, 65, 100, 127, 128, 129, 255, 256, 300, 600, 1000):
+        for cap in (16, 32, 48, 64, 80, 96, 112, 128, 160, 256, 272, 512, 1040, 4096, 70000):
+            for kind in ("all", "one", "empty", "any"):
+                total, _, share = _line(_lens(rng, batch, cap, kind), n_kv, cap)
+                assert -(-total // share) <= _shares(batch, n_kv, cap), (batch, cap, kind)
 
 
 @pytest.mark.skipif(not _lib.library_available(), reason="the library is not built")
