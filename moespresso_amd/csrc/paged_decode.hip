@@ -16,7 +16,7 @@
 // that is not its whole row leaves partials, and only rows that were cut go through the second kernel.
 //
 // With few rows the four waves of a workgroup take a share's tiles in turn and meet in LDS. With many, whose parts have few
-// tiles, every wave takes shares of its own: nothing is exchanged, and no wave waits for another.
+// tiles, every wave takes a share of its own: nothing is exchanged, and no wave waits for another.
 //
 // Rows are read as buffer windows: rows that do not count, in the last tile, behind it or in a page that is not in the pool,
 // read as zeros and cost no access, so that a wave always asks for a next tile and what is outstanding does not depend on
@@ -57,11 +57,10 @@ constexpr int kMinTiles = 2;
 // tiles then fill about evenly (with half a share, 512 rows of 1 to 300 keys 30 us instead of 27.5).
 constexpr int kGroupCost = 8, kWaveCost = 2;
 
-// Rows of tiles from which on waves take shares of their own. Shares of workgroups and of waves, in us: 2 rows of 8191 keys 12.1
-// and 16.0, 32 ragged ones (8-bit) 186 and 190, 64 of 0 to 3000 keys 32 and 30, 128 ragged ones 161 and 159, 256 of 0 to
-// 8000 keys (8-bit) 118 and 107, 528 of 1 to 1985 keys (float32 queries, 8-bit) 129 and 78, 1712 of 0 to 612 keys (8-bit) 169
-// and 92.
-constexpr int kManyRows = 64;
+// Rows of tiles from which on waves take shares of their own. Shares of workgroups and of waves, in us: 2 rows of 8191 keys
+// 12.2 and 16.1; of 8-bit rows, 80 of 0 to 300 keys 12.1 and 14.2, of 0 to 4000 27.2 and 32.8; 126 of these 16.9 and 14.9, 36.4
+// and 38.0; 240 of them 19.3 and 16.3, 59.9 and 59.2; 500 of them 30.6 and 22.4, 107.3 and 106.7.
+constexpr int kManyRows = 128;
 
 constexpr int kAffine = 3;  // page format beside MSPR_F16 and MSPR_BF16
 

@@ -7,7 +7,7 @@ of a 16-bit type, each off by half a step of it (bfloat16 pages 2^-8 of 2^-8 of 
 one float16 term (8-bit pages, bfloat16 result: 2^-11); float16 operands are taken 2^11 times as large and end at 2^-25, so
 that n weights lose at most n * 2^-36 of the largest value together (8-bit pages: of 128 times twice the largest scale). Sums
 over n keys run over n / 8 float32 additions at most where four waves share a row of keys, over n / 4 where one has it for
-itself (64 rows or more: a lane adds eight weights of every 32 keys), counted for both the weights' and the values' sums; the
+itself (128 rows or more: a lane adds eight weights of every 32 keys), counted for both the weights' and the values' sums; the
 result is rounded once more, to eps / 2 of its type.
 """
 
@@ -94,7 +94,7 @@ def _reference(q, keys, values, tables, lens, scale, requests=None):
                 s, z = (t.double().repeat_interleave(64, -1) for t in (s, z))
                 c = ((c.view(torch.uint8).double() - 128) * s).abs() + (z + 128 * s).abs()
                 most = (x.abs() @ c.reshape(-1, 256)[keep].t()).amax(-1, keepdim=True) * abs(scale)
-            adds = k.shape[0] / (8 if q.shape[0] * G < 64 else 4) + 8
+            adds = k.shape[0] / (8 if q.shape[0] * G < 128 else 4) + 8
             bound[r, g * rep:(g + 1) * rep] = size * (2 * 260 * 2.0 ** -24 * most + terms + 2 * adds * 2.0 ** -24)
             if q.dtype != BF16 or not torch.is_tensor(keys):
                 bound[r, g * rep:(g + 1) * rep] += k.shape[0] * 2.0 ** -36 * largest
@@ -175,11 +175,11 @@ def test_long_and_ragged_batches(dtype, form):
 
 @pytest.mark.parametrize("dtype,form", [(BF16, "rows"), (F32, F32), (F16, BF16)])
 @pytest.mark.parametrize("n_kv,page,lens", [
-    (2, 64, [8000] + [1] * 31),                # a row in more than a hundred parts among whole ones
+    (4, 64, [8000] + [1] * 31),                # rows in tens of parts among whole ones
     (2, 16, [1] * 20 + [5000, 0, 3000] + [40] * 20),
     (8, 32, [70, 3] * 64 + [3000, 65]),        # more rows than shares, one in more than sixteen parts
-    (1, 16, [129, 0, 64] * 21 + [1]),          # as few rows as are dealt out to single waves
-    (1, 16, [129, 0, 64] * 21),                # one fewer
+    (2, 16, [129, 0, 64] * 21 + [1]),          # as few rows as are dealt out to single waves
+    (1, 16, [129, 0, 64] * 42 + [1]),          # one fewer
 ])
 def test_long_rows_among_many(n_kv, page, lens, dtype, form):
     rng = np.random.default_rng(len(lens))

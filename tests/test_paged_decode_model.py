@@ -6,7 +6,7 @@ import pytest
 
 from moespresso_amd import _lib
 
-TILE, WAVES, GROUPS, MIN_TILES, MANY_ROWS = 32, 4, 256, 2, 64
+TILE, WAVES, GROUPS, MIN_TILES, MANY_ROWS = 32, 4, 256, 2, 128
 GROUP_COST, WAVE_COST = 8, 2
 
 
@@ -70,7 +70,7 @@ def _lens(rng, batch, cap, kind):
 
 @pytest.mark.parametrize("kind", ["all", "one", "empty", "any"])
 @pytest.mark.parametrize("batch,n_kv,page,width", [(1, 1, 16, 1), (1, 2, 16, 9), (1, 2, 64, 128), (3, 2, 16, 100), (65, 1, 32, 7),
-                                                   (130, 8, 16, 3), (16, 2, 256, 40), (64, 4, 128, 2),
+                                                   (130, 8, 16, 3), (16, 2, 256, 40), (64, 4, 128, 2), (127, 1, 16, 9),
                                                    (300, 2, 16, 1), (70, 8, 32, 4), (600, 1, 64, 2)])
 def test_every_row_is_attended_once_and_every_address_lies_in_its_buffer(kind, batch, n_kv, page, width):
     rng = np.random.default_rng(batch * 1000 + width)
@@ -139,7 +139,7 @@ def test_no_share_with_work_is_behind_those_that_are_launched(n_kv):
 
 @pytest.mark.skipif(not _lib.library_available(), reason="the library is not built")
 @pytest.mark.parametrize("batch,heads,n_kv,page,width", [(1, 16, 2, 64, 1), (1, 16, 2, 64, 2048), (256, 64, 8, 16, 100), (65535, 1, 1, 16, 1),
-                                                             (63, 4, 1, 16, 3), (64, 4, 1, 16, 3), (65, 4, 1, 16, 2)])
+                                                             (127, 4, 1, 16, 3), (128, 4, 1, 16, 3), (129, 4, 1, 16, 2)])
 def test_the_workspace_holds_every_part(batch, heads, n_kv, page, width):
     need = _shares(batch, n_kv, page * width) * 2 * (heads // n_kv * 256 + 32) * 4 + 3 * 4 * GROUPS * WAVES
     assert need <= _lib.lib().mspr_sdpa_decode_paged_workspace_bytes(batch, heads, n_kv, page, width) <= need + 64
