@@ -203,6 +203,8 @@ __device__ __forceinline__ void static_for(F&& f) {
   static_for(f, std::make_integer_sequence<int, N>{});
 }
 
+constexpr int kNearInts = kWaves * 2 * MSPR_WAVE;  // what every wave knows of the first chunks' lengths
+
 // LDS of a workgroup: the waves' V tiles (or what they exchange at the end) and the query operands, of all or of each.
 __host__ __device__ constexpr int loop_lds(int qdt, int fmt, bool alone) {
   const int tiles = kWaves * kVTileBytes;
@@ -264,19 +266,23 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
 
   // ---- the share: every wave adds up all tiles for itself, of more than 64 queries the four together, a chunk of 64 at a time
   const int chunks = (batch + MSPR_WAVE - 1) / MSPR_WAVE;
-  int* chunk_sums = reinterpret_cast<int*>(lds + loop_lds(QDT, FMT, ALONE));  // [chunks]
+  int* near = reinterpret_cast<int*>(lds + loop_lds(QDT, FMT, ALONE));  // lengths and sums of the first four: [4][2][64]
+  int* chunk_sums = near + kNearInts;                                   // [chunks]
   auto tiles_at = [&](int i, int& len) {
     len = length_of(lens, batch, i, cap);
     return i < batch ? tiles_of(len) : 0;
   };
   Place at = {0, 0, 0, 0};
-  int all = 0, chunk = 0, before = 0, len0, tiles0 = tiles_at(lane, len0);
+  int chunk = chunks == 1 ? 0 : wave, all = 0, before = 0, len0, tiles0 = tiles_at(chunk * MSPR_WAVE + lane, len0);
   int sums0 = wave_scan(tiles0);
   int chunk_sum = 0, in_lanes = 0, per_lane = 1;  // (of more chunks than one: lane i has the sum of `per_lane`, and those before)
   if (chunks == 1) {
     all = __builtin_amdgcn_readlane(sums0, 63);
   } else {
-    for (int c = wave; c < chunks; c += kWaves) {
+    near[2 * MSPR_WAVE * wave + lane] = len0;
+    near[2 * MSPR_WAVE * wave + MSPR_WAVE + lane] = sums0;
+    if (lane == 63 && wave < chunks) chunk_sums[wave] = sums0;
+    for (int c = wave + kWaves; c < chunks; c += kWaves) {
       int len;
       const int sum = wave_scan(tiles_at(c * MSPR_WAVE + lane, len));
       if (lane == 63) chunk_sums[c] = sum;
@@ -320,8 +326,14 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
       if ((before + sum) * n_kv > pos) break;
       before += sum;
     }
-    tiles0 = tiles_at(chunk * MSPR_WAVE + lane, len0);
-    sums0 = wave_scan(tiles0);
+    if (chunk < kWaves) {
+      len0 = near[2 * MSPR_WAVE * chunk + lane];
+      sums0 = near[2 * MSPR_WAVE * chunk + MSPR_WAVE + lane];
+      tiles0 = tiles_of(len0);
+    } else {
+      tiles0 = tiles_at(chunk * MSPR_WAVE + lane, len0);
+      sums0 = wave_scan(tiles0);
+    }
   }
   {
     sums0 += cost * min(lane + 1, batch - chunk * MSPR_WAVE);
@@ -953,8 +965,8 @@ template <int QDT, int FMT, int SDT, bool ALONE>
 int paged_launch_form(const PagedArgs& a, hipStream_t st) {
   const int64_t cap = (int64_t)a.width << a.page_shift;
   const int chunks = (a.batch + MSPR_WAVE - 1) / MSPR_WAVE;
-  constexpr int kLds = loop_lds(QDT, FMT, ALONE), kMostLds = kLds + 65536 / MSPR_WAVE * (int)sizeof(int);
-  const int lds = kLds + (chunks > 1 ? chunks * (int)sizeof(int) : 0);
+  constexpr int kLds = loop_lds(QDT, FMT, ALONE), kMostLds = kLds + (kNearInts + 65536 / MSPR_WAVE) * (int)sizeof(int);
+  const int lds = kLds + (chunks > 1 ? (kNearInts + chunks) * (int)sizeof(int) : 0);
   static bool attr_set[64] = {};  // by device
   int device = 0;
   if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64 || !attr_set[device]) {
