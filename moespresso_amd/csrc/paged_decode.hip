@@ -47,7 +47,8 @@ constexpr int kVTileBytes = kTileKeys * kVPitch;
 constexpr int kMaxGroups = 256;    // workgroups: one a compute unit
 constexpr int kNonTemporal = 2;    // cache policy of loads that are used once
 
-// Tiles of a share, and what a row counts for, at least. (Four, a tile a wave: a request of 8191 rows 10.2 us, not 8.2.)
+// Tiles of a share, and what a row counts for, at least. (Four, a tile a wave: a request of 8191 rows 10.2 us
+// where two took 8.2, with no cost of rows.)
 constexpr int kMinTiles = 2;
 
 // What a part of a row costs beside its tiles (query, page numbers, first loads, output: 10000 cycles, a tile 6000), in tiles of a
