@@ -30,8 +30,10 @@
 // group, V: weights x biases). Codes count from 128 on, and 128 scales go into the biases: of rows around zero, the sums over
 // codes and over biases would be many times the result, and what is lost in them (float32 results over 37000 keys are 0.5e-6
 // off, 0.9e-6 with K's codes from 0 on, 1.8e-6 with V's). Weights, and queries whose type has more digits than an operand, go
-// in as two terms of it, the rounded value and the rounded rest (weights of 8-bit rows for a bfloat16 result, which has three
-// digits fewer than float16: one).
+// in as two terms of it, the rounded value and the rounded rest. Weights of 8-bit rows do so for a bfloat16 result too, though
+// it has fewer digits than one float16 term: the sums over codes and over biases, which take the weights apart, may be many
+// times the result (a key whose scale is 10^4 of the others' left results 1.8e-2 of the values' sum off; one term took 185 us
+// for 16 ragged requests where two take 192).
 #include "common.h"
 #include "q8_codes.h"
 
@@ -243,8 +245,8 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
   // has eleven digits (three terms of bfloat16 are as exact; 66 requests of 1 to 1985 keys with float32 queries took 79 us with
   // them, 73 with these).
   constexpr int kVType = kCodes ? MSPR_F16 : FMT;
-  constexpr int kPTerms = kCodes && QDT == MSPR_BF16 ? 1 : 2;  // terms of a weight
-  constexpr int kQTerms = kCodes && QDT == MSPR_F32 ? 2 : 1;                         // terms of a query element
+  constexpr int kPTerms = 2;                                   // terms of a weight
+  constexpr int kQTerms = kCodes && QDT == MSPR_F32 ? 2 : 1;  // terms of a query element
   // float16 weights are taken 2^11 times as large: up to 2^15, as the reference maximum lags by 2^4 at most, and the smallest
   // that is not lost is 2^-35 of the largest (at 2^-24, the many small weights of a long context would all be rounded one way)
   constexpr float kLag = 4.0f;
