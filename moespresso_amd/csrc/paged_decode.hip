@@ -404,7 +404,9 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
     };
     float m_run = -__builtin_inff(), l_run = 0.0f;
     f32x4_t bacc = {0.f, 0.f, 0.f, 0.f};  // weighted biases: lane n (g = 0) has those of head n and the four groups
-    float v_unit = 0x1p-126f;             // what V's scales are multiples of: a power of two from their largest magnitude on
+    // what V's scales of group n % 4 are multiples of: a power of two from their largest magnitude on. (A group's own: weights
+    // end at 2^-36 of it, and one for all four cost a group whose scales are 10^-6 of another's all but 2^-12 of its results.)
+    float v_unit = 0x1p-126f;
 
     // Pages of this wave's tiles, two half tiles of 16 keys each (a page holds 16 rows or more): lane i of `ids` has the page
     // of half tile i of 31 tiles and the one behind them, the next tiles' are on their way while these are used.
@@ -688,19 +690,20 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
 #pragma unroll
           for (int q4 = 0; q4 < 4; q4++) accumulate(q4, pf);
         } else {
-          // The operand is float16: scales are taken as multiples of a power of two that is as large as any of them.
+          // The operand is float16: scales are taken as multiples of a power of two that is as large as any of their group.
           float vsf[2] = {vs[0].value(n), vs[1].value(n)};
           const float largest = fmaxf(fabsf(vsf[0]), fabsf(vsf[1]));
           if (__any(largest > v_unit)) {
             float top = largest;
-            top = fmaxf(top, lane_xor<1>(top));
-            top = fmaxf(top, lane_xor<2>(top));
             top = fmaxf(top, lane_xor<4>(top));
             top = fmaxf(top, lane_xor<8>(top));
             top = half_wave_max(row_pair_max(top));
             const int e = top < 0x1p126f ? __builtin_amdgcn_frexp_expf(top) : 126;
-            const float unit = __builtin_amdgcn_ldexpf(1.0f, e);
-            if (it > 0) rescale(v_unit / unit);
+            const float unit = top > v_unit ? __builtin_amdgcn_ldexpf(1.0f, e) : v_unit;
+            if (it > 0) {
+              const float by = v_unit / unit;
+              static_for<16>([&](auto mt) { oacc[mt] = oacc[mt] * of_lane<decltype(mt)::value / 4>(by); });
+            }
             v_unit = unit;
           }
           const float per_unit = 1.0f / v_unit;
@@ -743,8 +746,7 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
       float bias[4];
 #pragma unroll
       for (int j = 0; j < 4; j++) bias[j] = __shfl(bacc[j], n, MSPR_WAVE);
-#pragma unroll
-      for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] * v_unit + bias[mt >> 2];
+      static_for<16>([&](auto mt) { oacc[mt] = oacc[mt] * of_lane<decltype(mt)::value / 4>(v_unit) + bias[mt >> 2]; });
     }
     const bool whole = tile0 == 0 && tile1 == row_tiles;
     const int row = at.b * n_kv + at.kvh;

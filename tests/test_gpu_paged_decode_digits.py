@@ -5,7 +5,7 @@ moves the result by twice that of the values' sum. A weight times a scale is two
 it; taken 2^11 times as large in multiples of a power of two that is less than twice the largest scale, a term ends at 2^-25 of
 that, so that n weights lose n * 2^-36 of twice the largest scale and 128 codes. Codes (from 128 on) and biases are
 summed apart, in float32: over n / 8 additions where four waves share the keys, n / 4 where one has them, of the weights' and of
-the values' sums. The result is rounded once more, to eps / 2 of its type.
+the values' sums. The result is rounded once more, to eps / 2 of its type (beyond float16's largest number it is infinite).
 """
 
 import pytest
@@ -52,7 +52,11 @@ def _check(dtype, n, queries, seed, change):
     adds = n / (8 if queries < 128 else 4) + 8
     bound = (w @ size) * (2 * 260 * 2.0 ** -24 * most + 2.0 ** -22 + 2 * adds * 2.0 ** -24)
     bound += n * 2.0 ** -36 * 2 * 128 * scale.amax(0) + torch.finfo(dtype).eps / 2 * want.abs() + torch.finfo(dtype).tiny
-    err = (got.double() - want).abs()
+    # (a result beyond the type's largest number, by more than it may be off, is infinite; one that may lie on either side is either)
+    top = torch.finfo(dtype).max
+    over = want.abs() - bound > top
+    assert got.double()[over.expand_as(got)].equal((want.sign() * torch.inf).expand_as(got)[over.expand_as(got)])
+    err = torch.where(want.abs() + bound > top, 0.0, (got.double() - want).abs())
     assert (err <= bound).all(), float((err / bound).max())
 
 
@@ -66,3 +70,18 @@ def test_a_key_whose_scales_are_far_above_the_others(n, dtype, queries):
             scales[HOT] *= ratio
 
         _check(dtype, n, queries, 1, change)
+
+
+@pytest.mark.parametrize("queries", [1, 130])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n", [500, 5000, 37000])
+def test_groups_of_channels_of_different_size(n, dtype, queries):
+    """No group loses digits to another's scales, whichever is met first."""
+    for ratio in (1e2, 1e4, 1e6):
+        def change(scales):
+            scales[:, 1] *= ratio
+            scales[:, 3] /= ratio
+            scales[n // 2:, 2] *= ratio
+            scales[:n // 3, 0] *= ratio
+
+        _check(dtype, n, queries, 2, change)
