@@ -94,6 +94,18 @@ __device__ __forceinline__ float rounded(float v) {
   else return (float)(__bf16)v;
 }
 
+// 1 / sqrt(v), off by little more than half a unit of its last place: the instruction's value, a unit off at most, and one step
+// of Newton's method with the rounding of v * y in it. The instruction takes numbers below 2^-126 for zero: they are scaled.
+__device__ __forceinline__ float rsqrt_near(float v) {
+  const bool tiny = v < 0x1p-96f;
+  const float u = tiny ? v * 0x1p64f : v;
+  const float y = __builtin_amdgcn_rsqf(u);
+  const float h = u * y;
+  const float e = fmaf(-y, fmaf(u, y, -h), fmaf(-h, y, 1.0f));  // 1 - u y^2
+  const float z = u > 0.0f && u < __builtin_inff() ? fmaf(0.5f * y, e, y) : y;
+  return tiny ? z * 0x1p32f : z;
+}
+
 // N channels of type DT.
 template <int DT, int N>
 __device__ __forceinline__ void store_row(void* p, int64_t i, const float* x) {
@@ -258,7 +270,7 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(RopeArgs a) {
       ss += lane_xor<8>(ss);
       ss += lane_xor<16>(ss);
       if constexpr (N == 4) ss = half_wave_sum(ss);
-      const float r = __builtin_amdgcn_rsqf(ss * (1.0f / kD) + a.eps);  // (off by a unit of its last place at most)
+      const float r = rsqrt_near(fmaf(ss, 1.0f / kD, a.eps));
 #pragma unroll
       for (int j = 0; j < N; j++) x[j] = x[j] * r * w[j];
       if (rotary) {
