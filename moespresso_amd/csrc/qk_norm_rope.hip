@@ -4,8 +4,8 @@
 //   (y_i, y_{i+r/2}) <- (y_i cos t - y_{i+r/2} sin t, y_{i+r/2} cos t + y_i sin t)   for i < r/2, t = position * inv_freq_i
 //
 // rounded once, to the type of what is written. With three position axes frequency i takes axis i % 3 while that axis has
-// frequencies left (axis 1: 3 i' + 1 < 3 n_1, axis 2: 3 i' + 2 < 3 n_2), else axis 0. The angle is the exact product, reduced to
-// a turn in 64 bits: a float32 product is off by 2^-24 of it, 0.007 radians at position 120000, which no later step makes good.
+// frequencies left (axis 1: 3 i' + 1 < 3 n_1, axis 2: 3 i' + 2 < 3 n_2), else axis 0. The angle is the product in 64 bits, reduced
+// to a turn there: a float32 product is off by 2^-24 of it, 0.007 radians at position 120000, which no later step makes good.
 //
 // Bound by HBM: every element is read and written once. A lane owns 16 bytes of a head's row, so that a load or store of a wave
 // is whole rows (with 32 bytes of a float32 row a lane, every line was asked for twice), the sum of squares is five or six lane
@@ -229,8 +229,13 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(RopeArgs a) {
     const int pos = a.positions[(int64_t)axis * a.n_tokens + t0 + t];
     double turns = (double)pos * (double)a.inv_freq[f] * 0.15915494309189535;  // 1 / (2 pi)
     turns -= rint(turns);
+    const float near = (float)turns;  // (2 pi of what that rounds off, up to 9e-8, is added to the angle to first order)
+    const float rest = (float)(turns - (double)near) * 6.2831853f;
     float s, c;
-    sincospif(2.0f * (float)turns, &s, &c);
+    sincospif(2.0f * near, &s, &c);
+    const float c0 = c;
+    c = fmaf(-s, rest, c);
+    s = fmaf(c0, rest, s);
     turn[2 * t * a.half + f] = f32x2_t{c, -s};
     turn[(2 * t + 1) * a.half + f] = f32x2_t{c, s};
   }
