@@ -441,11 +441,12 @@ class PagedAttention(torch.nn.Module):
         inner = self.inner
         T = int(x.shape[0])
         heads, kv_heads = inner.num_attention_heads, inner.num_key_value_heads
-        q, gate = inner.q_proj(x).reshape(T, heads, -1).chunk(2, dim=-1)
-        k = inner.k_proj(x).reshape(T, kv_heads, -1)
-        v = inner.v_proj(x).reshape(T, kv_heads, -1)
+        # (widths in full: a step in which every request ends has no rows, of which a width could not be told)
+        q, gate = inner.q_proj(x).reshape(T, heads, 2 * _HEAD_DIM).chunk(2, dim=-1)
+        k = inner.k_proj(x).reshape(T, kv_heads, _HEAD_DIM)
+        v = inner.v_proj(x).reshape(T, kv_heads, _HEAD_DIM)
         q = self.cache.append(q, k, v, inner.q_norm.weight, inner.k_norm.weight,
                               step.positions if positions is None else positions, inner.rope.inv_freq, step.slots,
                               eps=inner.q_norm.eps, sections=None if positions is None else inner.rope.sections)
         out = self.cache.attend(q, tables.tables, step.visible, inner.scale, requests=step.requests)
-        return inner.o_proj((out * torch.sigmoid(gate)).reshape(T, -1))
+        return inner.o_proj((out * torch.sigmoid(gate)).reshape(T, heads * _HEAD_DIM))
