@@ -286,6 +286,11 @@ def _check_decode(queries, heads, tables, lens, requests):
     return R, Hq
 
 
+def _queries_a_call(heads: int, page_size: int, width: int) -> int:
+    """How many queries one decode call takes over tables of ``width`` pages: 65535, and 2^30 tiles of 32 keys if full together."""
+    return min(65535, 0x3FFFFFFF // (heads * max(2, -(-width * page_size // 32))))
+
+
 def sdpa_decode_paged(queries, keys, values, tables, lens, scale, *, requests=None, workspace=None):
     """One new query of every request over the request's pages of 16-bit rows.
 
@@ -433,6 +438,11 @@ class PagedAttention(torch.nn.Module):
         super().__init__()
         if inner.q_norm.eps != inner.k_norm.eps:
             raise ValueError("q_norm and k_norm must share an eps")
+        _, kv_heads, _ = _check_pages(cache.keys, cache.values)
+        if inner.num_key_value_heads != kv_heads:
+            raise ValueError("the block and the cache disagree on the number of KV heads")
+        if inner.num_attention_heads % kv_heads != 0 or not 1 <= inner.num_attention_heads // kv_heads <= 16:
+            raise ValueError("query heads must be a multiple (at most 16x) of the KV heads")
         self.inner = inner
         self.cache = cache
 
@@ -441,6 +451,9 @@ class PagedAttention(torch.nn.Module):
         inner = self.inner
         T = int(x.shape[0])
         heads, kv_heads = inner.num_attention_heads, inner.num_key_value_heads
+        most = _queries_a_call(kv_heads, tables.page_size, int(tables.tables.shape[1]))
+        if most < 1:  # (before anything is written)
+            raise ValueError("the tables hold too many tokens together")
         # (widths in full: a step in which every request ends has no rows, of which a width could not be told)
         q, gate = inner.q_proj(x).reshape(T, heads, 2 * _HEAD_DIM).chunk(2, dim=-1)
         k = inner.k_proj(x).reshape(T, kv_heads, _HEAD_DIM)
@@ -448,5 +461,9 @@ class PagedAttention(torch.nn.Module):
         q = self.cache.append(q, k, v, inner.q_norm.weight, inner.k_norm.weight,
                               step.positions if positions is None else positions, inner.rope.inv_freq, step.slots,
                               eps=inner.q_norm.eps, sections=None if positions is None else inner.rope.sections)
-        out = self.cache.attend(q, tables.tables, step.visible, inner.scale, requests=step.requests)
+        if T <= most:
+            out = self.cache.attend(q, tables.tables, step.visible, inner.scale, requests=step.requests)
+        else:
+            out = torch.cat([self.cache.attend(q[i:i + most], tables.tables, step.visible[i:i + most], inner.scale,
+                                               requests=step.requests[i:i + most]) for i in range(0, T, most)])
         return inner.o_proj((out * torch.sigmoid(gate)).reshape(T, heads * _HEAD_DIM))
