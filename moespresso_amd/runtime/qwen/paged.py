@@ -425,6 +425,18 @@ class PagedKVCache:
                                  workspace=workspace).float()
 
 
+class _NoGradient(torch.autograd.Function):
+    """``out`` as it is, in the graph of the tensors it was made from, through which there is no way back."""
+
+    @staticmethod
+    def forward(ctx, out, *made_from):
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("PagedAttention serves and has no backward pass: run it under torch.no_grad(), or detach what goes in")
+
+
 class PagedAttention(torch.nn.Module):
     """One full-attention layer over a paged cache: a step's rows of many requests through the wrapped block's projections.
 
@@ -432,6 +444,9 @@ class PagedAttention(torch.nn.Module):
     the output gate in the second half of every head), ``k_proj``, ``v_proj``, ``o_proj``, ``q_norm`` and ``k_norm``
     (``weight`` and one ``eps``), ``rope`` (``inv_freq`` and, for three position axes, ``sections``), ``scale``,
     ``num_attention_heads`` and ``num_key_value_heads``.
+
+    The layer serves: a backward pass that would have to go through its attention raises (the gate and the projection behind it
+    alone would leave gradients that lack a part).
     """
 
     def __init__(self, inner, cache: PagedKVCache):
@@ -458,6 +473,7 @@ class PagedAttention(torch.nn.Module):
         q, gate = inner.q_proj(x).reshape(T, heads, 2 * _HEAD_DIM).chunk(2, dim=-1)
         k = inner.k_proj(x).reshape(T, kv_heads, _HEAD_DIM)
         v = inner.v_proj(x).reshape(T, kv_heads, _HEAD_DIM)
+        made_from = (q, k, v, inner.q_norm.weight, inner.k_norm.weight)
         q = self.cache.append(q, k, v, inner.q_norm.weight, inner.k_norm.weight,
                               step.positions if positions is None else positions, inner.rope.inv_freq, step.slots,
                               eps=inner.q_norm.eps, sections=None if positions is None else inner.rope.sections)
@@ -466,4 +482,6 @@ class PagedAttention(torch.nn.Module):
         else:
             out = torch.cat([self.cache.attend(q[i:i + most], tables.tables, step.visible[i:i + most], inner.scale,
                                                requests=step.requests[i:i + most]) for i in range(0, T, most)])
+        if torch.is_grad_enabled() and any(t.requires_grad for t in made_from):
+            out = _NoGradient.apply(out, *made_from)
         return inner.o_proj((out * torch.sigmoid(gate)).reshape(T, heads * _HEAD_DIM))
