@@ -16,6 +16,7 @@ A step of a server, every part of it enqueued without waiting for the device:
 
 from __future__ import annotations
 
+import inspect
 from ctypes import c_int64
 from typing import NamedTuple
 
@@ -437,13 +438,58 @@ class _NoGradient(torch.autograd.Function):
         raise RuntimeError("PagedAttention serves and has no backward pass: run it under torch.no_grad(), or detach what goes in")
 
 
+def _called(module, *args, **kwargs):
+    """What the module makes of the arguments, None where it has no forward that takes them."""
+    call = module.forward if isinstance(module, torch.nn.Module) else module
+    if getattr(call, "__func__", call) is torch.nn.Module.forward or not callable(call):
+        return None
+    try:
+        inspect.signature(call).bind(*args, **kwargs)
+    except TypeError:
+        return None
+    with torch.no_grad():
+        return call(*args, **kwargs)
+
+
+def _check_modules(inner):
+    """The operators take weights, eps and frequencies of the norms and the rope, not the modules: refuse modules that make
+    something else of them (a weight counted from 1, another pairing of channels, angles that are scaled)."""
+    for name in ("q_norm", "k_norm"):
+        norm = getattr(inner, name)
+        w = norm.weight
+        if tuple(w.shape) != (_HEAD_DIM,):
+            raise ValueError(f"{name} must have a weight of 256 channels")
+        # (a row of ordinary size, and one whose mean square is about an eps)
+        x = torch.cos(torch.arange(2 * _HEAD_DIM, device=w.device)).reshape(1, 2, 1, _HEAD_DIM).to(w.dtype)
+        x[:, 1] *= 1e-3
+        got = _called(norm, x)
+        y = x.float()
+        want = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + norm.eps) * w.detach().float()
+        if got is not None and bool(((got.float() - want).abs().amax(-1) > 0.05 * want.abs().amax(-1)).any()):
+            raise ValueError(f"{name} is not weight * x / sqrt(mean(x^2) + eps), which is what this layer computes")
+    inv = inner.rope.inv_freq
+    half = int(inv.shape[-1])
+    x = torch.cos(torch.arange(3 * _HEAD_DIM, device=inv.device)).reshape(1, 1, 3, _HEAD_DIM).to(inner.q_norm.weight.dtype)
+    got = _called(inner.rope, x, offset=5)
+    if got is None:
+        return
+    angle = torch.arange(5, 8, device=inv.device)[:, None] * inv.float()
+    a, b, rest = x.float().tensor_split((half, 2 * half), dim=-1)
+    want = torch.cat([a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin(), rest], dim=-1)
+    if got.shape != want.shape or bool((got.float() - want).abs().max() > 0.05):
+        raise ValueError("rope does not rotate channels i and i + rotary_dim / 2 by position * inv_freq[i], which is what this "
+                         "layer computes")
+
+
 class PagedAttention(torch.nn.Module):
     """One full-attention layer over a paged cache: a step's rows of many requests through the wrapped block's projections.
 
     ``inner`` is a block as ``full_attention.FlashPrefillD256Attention`` wraps it; of its modules this takes ``q_proj`` (with
     the output gate in the second half of every head), ``k_proj``, ``v_proj``, ``o_proj``, ``q_norm`` and ``k_norm``
-    (``weight`` and one ``eps``), ``rope`` (``inv_freq`` and, for three position axes, ``sections``), ``scale``,
-    ``num_attention_heads`` and ``num_key_value_heads``.
+    (``weight``, of the type of ``x`` and multiplied as it is, and one ``eps``), ``rope`` (``inv_freq`` and, for three position
+    axes, ``sections``), ``scale``, ``num_attention_heads`` and ``num_key_value_heads``. Norms and rope are not called, but made
+    anew from these: a norm or rope that can be called and gives something else is refused, and so are hooks on them. A block
+    may come without ``eps``, ``inv_freq`` or ``sections`` where only the wrapper uses it; this layer needs them.
 
     The layer serves: a backward pass that would have to go through its attention raises (the gate and the projection behind it
     alone would leave gradients that lack a part).
@@ -458,12 +504,16 @@ class PagedAttention(torch.nn.Module):
             raise ValueError("the block and the cache disagree on the number of KV heads")
         if inner.num_attention_heads % kv_heads != 0 or not 1 <= inner.num_attention_heads // kv_heads <= 16:
             raise ValueError("query heads must be a multiple (at most 16x) of the KV heads")
+        _check_modules(inner)
         self.inner = inner
         self.cache = cache
 
     def forward(self, x, step: PageStep, tables: PageTables, positions=None):
         """``x``: ``[n_rows, hidden]``, the rows of ``step``. ``positions``: int32 ``[3, n_rows]`` where the rope has sections."""
         inner = self.inner
+        for module in (inner.q_norm, inner.k_norm, inner.rope):
+            if getattr(module, "_forward_hooks", None) or getattr(module, "_forward_pre_hooks", None):
+                raise RuntimeError("hooks of q_norm, k_norm and rope would not run: this layer takes their weights and frequencies")
         T = int(x.shape[0])
         heads, kv_heads = inner.num_attention_heads, inner.num_key_value_heads
         most = _queries_a_call(kv_heads, tables.page_size, int(tables.tables.shape[1]))

@@ -62,3 +62,85 @@ def test_a_backward_pass_is_refused(monkeypatch):
     x.requires_grad_(False)
     layer(x, step, tables).sum().backward()
     assert layer.inner.o_proj.weight.grad.abs().sum() > 0
+
+
+class _CalledNorm(_Norm):
+    centre, power = 0.0, 0.5
+
+    def forward(self, x):
+        y = x.float()
+        y = y * (y.square().mean(-1, keepdim=True) + self.eps) ** -self.power
+        return (y * (self.centre + self.weight.float())).to(x.dtype)
+
+
+class _CalledRope(_Rope):
+    pairs, stretch = "halves", 1.0
+
+    def __init__(self, rotary=64):
+        super().__init__()
+        self.inv_freq = (1e7 ** (-torch.arange(0, rotary, 2, dtype=torch.float64) / rotary)).float()
+
+    def forward(self, x, offset=0):
+        half = self.inv_freq.numel()
+        angle = (offset + torch.arange(x.shape[-2]))[:, None] * self.inv_freq * self.stretch
+        y = x.float().clone()
+        i = torch.arange(half)
+        first, second = (i, i + half) if self.pairs == "halves" else (2 * i, 2 * i + 1)
+        a, b = y[..., first].clone(), y[..., second].clone()
+        y[..., first], y[..., second] = a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()
+        return y.to(x.dtype)
+
+
+def _with(**modules):
+    block = _Block()
+    for name, module in modules.items():
+        setattr(block, name, module)
+    return paged.PagedAttention(block, paged.PagedKVCache(4, KV_HEADS, page_size=16, device="cpu", dtype=torch.float16))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rotary", [16, 64, 256])
+def test_modules_that_compute_what_the_operators_do_are_taken(dtype, rotary):
+    _with(q_norm=_CalledNorm().to(dtype), k_norm=_CalledNorm().to(dtype), rope=_CalledRope(rotary))
+
+
+@pytest.mark.parametrize("name", ["q_norm", "k_norm"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_norms_that_compute_something_else_are_refused(name, dtype):
+    """Else the layer would give wrong rows without a word."""
+    from_one = _CalledNorm().to(dtype)
+    from_one.centre = 1.0
+    fresh = _CalledNorm().to(dtype)
+    fresh.centre = 1.0
+    torch.nn.init.zeros_(fresh.weight)
+    other_eps = _CalledNorm().to(dtype)
+    other_eps.forward = lambda x: (x.float() * torch.rsqrt(x.float().square().mean(-1, keepdim=True) + 1e-5) * other_eps.weight).to(x.dtype)
+    no_root = _CalledNorm().to(dtype)
+    no_root.power = 1.0
+    for norm in (from_one, fresh, other_eps, no_root):
+        with pytest.raises(ValueError, match=f"{name} is not weight"):
+            _with(**{name: norm})
+    narrow = _Norm()
+    narrow.weight = torch.nn.Parameter(torch.ones(128))
+    with pytest.raises(ValueError, match="256 channels"):
+        _with(**{name: narrow})
+
+
+def test_ropes_that_compute_something_else_are_refused():
+    turned, stretched = _CalledRope(), _CalledRope()
+    turned.pairs, stretched.stretch = "neighbours", 0.25
+    for rope in (turned, stretched):
+        with pytest.raises(ValueError, match="rope does not rotate"):
+            _with(rope=rope)
+
+
+def test_hooks_that_would_not_run_are_refused(monkeypatch):
+    layer, step, tables = _layer(monkeypatch)
+    x = torch.randn(5, HIDDEN)
+    for module in (layer.inner.q_norm, layer.inner.k_norm, layer.inner.rope):
+        for register in (module.register_forward_hook, module.register_forward_pre_hook):
+            hook = register(lambda *a: None)
+            with pytest.raises(RuntimeError, match="would not run"):
+                layer(x, step, tables)
+            hook.remove()
+    layer(x, step, tables)
