@@ -310,8 +310,9 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
                                                                      : (int)blockIdx.x * kWaves + wave;
   int pos = number * share;
   const int end = min(pos + share, all);
-  const bool by_row = batch * n_kv <= kShares;
-  if (!by_row && lane == 0 && first_tile == 0) a.cut[3 * number] = -1;
+  const bool by_row = !ALONE || batch * n_kv <= kShares;
+  static_assert(kManyRows <= kMaxGroups, "with a share a workgroup there are fewer rows than shares");
+  if (!by_row && lane == 0) a.cut[3 * number] = -1;
   if (pos >= end) return;
   // (Whose tile `pos` is: it is below the total, so that there is one. Lengths that another stream changes meanwhile may say
   // otherwise: every loop ends and every index stays in its range all the same.)
@@ -882,7 +883,7 @@ __device__ __forceinline__ void join_waves(const Join& part, float (*xo)[kD + 2]
   store_out<ODT>(out, at + 4 * lane, o_all, l_all);
 }
 
-// An entry of `cut`: a row and how many parts it has, none of a row that was not cut. (Bounded by the call's rows and shares,
+// An entry of `cut`: a row and how many parts it has, none where no row was cut. (Bounded by the call's rows and shares,
 // whatever is there.)
 struct Cut {
   int row, first, count;
@@ -895,7 +896,7 @@ struct Cut {
 };
 
 // Joins the parts of one row that was cut, for one query head: eight waves take every eighth part.
-// grid: (entries of `cut`, query heads of a KV head)
+// grid: (rows, query heads of a KV head)
 constexpr int kMergeWaves = 8;
 template <int ODT>
 __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const int32_t* cut, const float* ws_o, const float* ws_ml,
@@ -990,15 +991,17 @@ int paged_launch_form(const PagedArgs& a, hipStream_t st) {
       a.lens, a.tables, a.k, a.v, a.batch, a.n_kv, a.width, a.page_shift, a.n_pages, a.rep, r);
   MSPR_CHECK_LAUNCH("sdpa_decode_paged");
   // (rows of kMinTiles tiles are cut only where there are more of them than shares)
-  const int rows = a.batch * a.n_kv, most = ALONE ? kMaxGroups * kWaves : kMaxGroups;
-  if (row_tiles_most(cap) > kMinTiles || rows > most) {
-    const unsigned entries = (unsigned)(rows <= most ? rows : shares);
-    if constexpr (ALONE)
+  const int rows = a.batch * a.n_kv;
+  const bool more = ALONE && rows > kMaxGroups * kWaves;
+  if (row_tiles_most(cap) > kMinTiles || more) {
+    if constexpr (ALONE) {
+      const unsigned entries = (unsigned)(more ? shares : rows);
       paged_merge_many_kernel<QDT><<<dim3((entries + kWaves - 1) / kWaves, (unsigned)a.rep), dim3(64 * kWaves), 0, st>>>(
           r.cut, r.ws_o, r.ws_ml, a.rep, rows, shares, entries, r.out);
-    else
-      paged_merge_kernel<QDT><<<dim3(entries, (unsigned)a.rep), dim3(64 * kMergeWaves), 0, st>>>(r.cut, r.ws_o, r.ws_ml, a.rep,
-                                                                                                 rows, shares, r.out);
+    } else {
+      paged_merge_kernel<QDT><<<dim3((unsigned)rows, (unsigned)a.rep), dim3(64 * kMergeWaves), 0, st>>>(r.cut, r.ws_o, r.ws_ml, a.rep,
+                                                                                                        rows, shares, r.out);
+    }
     MSPR_CHECK_LAUNCH("sdpa_decode_paged (merge)");
   }
   return MSPR_OK;
