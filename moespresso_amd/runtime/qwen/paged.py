@@ -438,17 +438,18 @@ class _NoGradient(torch.autograd.Function):
         raise RuntimeError("PagedAttention serves and has no backward pass: run it under torch.no_grad(), or detach what goes in")
 
 
-def _called(module, *args, **kwargs):
-    """What the module makes of the arguments, None where it has no forward that takes them."""
+def _called(module, x, **kwargs):
+    """What the module makes of ``x``, None where it has no forward that takes it and gives its like."""
     call = module.forward if isinstance(module, torch.nn.Module) else module
     if getattr(call, "__func__", call) is torch.nn.Module.forward or not callable(call):
         return None
     try:
-        inspect.signature(call).bind(*args, **kwargs)
+        inspect.signature(call).bind(x, **kwargs)
     except TypeError:
         return None
     with torch.no_grad():
-        return call(*args, **kwargs)
+        out = call(x, **kwargs)
+    return out if torch.is_tensor(out) and out.shape == x.shape else None
 
 
 def _check_modules(inner):
@@ -476,7 +477,7 @@ def _check_modules(inner):
     angle = torch.arange(5, 8, device=inv.device)[:, None] * inv.float()
     a, b, rest = x.float().tensor_split((half, 2 * half), dim=-1)
     want = torch.cat([a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin(), rest], dim=-1)
-    if got.shape != want.shape or bool((got.float() - want).abs().max() > 0.05):
+    if bool((got.float() - want).abs().max() > 0.05):
         raise ValueError("rope does not rotate channels i and i + rotary_dim / 2 by position * inv_freq[i], which is what this "
                          "layer computes")
 

@@ -144,3 +144,21 @@ def test_hooks_that_would_not_run_are_refused(monkeypatch):
                 layer(x, step, tables)
             hook.remove()
     layer(x, step, tables)
+
+
+def test_modules_that_give_something_of_another_kind_are_not_compared():
+    """A rope that makes cosines and sines, or takes positions: the layer needs its frequencies only."""
+    class Tables(_Rope):
+        def forward(self, x, offset=0):
+            return torch.cos(self.inv_freq), torch.sin(self.inv_freq)
+
+    class Positions(_Rope):
+        def forward(self, x, position_ids):
+            raise AssertionError("not called")
+
+    class Residual(_Norm):
+        def forward(self, x, **kwargs):
+            return x, None
+
+    _with(rope=Tables(), q_norm=Residual())
+    _with(rope=Positions())
