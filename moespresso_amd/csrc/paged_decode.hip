@@ -32,8 +32,8 @@
 // off, 0.9e-6 with K's codes from 0 on, 1.8e-6 with V's). Weights, and queries whose type has more digits than an operand, go
 // in as two terms of it, the rounded value and the rounded rest. Weights of 8-bit rows do so for a bfloat16 result too, though
 // it has fewer digits than one float16 term: the sums over codes and over biases, which take the weights apart, may be many
-// times the result (a key whose scale is 10^4 of the others' left results 1.8e-2 of the values' sum off; one term took 185 us
-// for 16 ragged requests where two take 192).
+// times the result (a key whose scale is 10^4 of the others' left results 1.8e-2 of the values' sum off; one term took 186 us
+// for 16 ragged requests where two take 193).
 #include "common.h"
 #include "q8_codes.h"
 
@@ -234,7 +234,7 @@ __device__ __forceinline__ void store_out(void* out, int64_t i, f32x4_t o, float
 // QDT: type of queries and output; FMT: page format; SDT: type of scales and biases (8-bit pages); ALONE: a share a wave
 // One workgroup a CU: with two, and half the share each, 16-bit rows took 100 us instead of 95 (8 requests of 37000 rows) and
 // 168 instead of 157 (64 ragged ones). The forms that fit 256 registers are held to them: beyond, values move to and from
-// accumulation registers (16 ragged requests of 8-bit rows 216 us instead of 199); the others would spill (104 instead of 95).
+// accumulation registers (16 ragged requests of 8-bit rows 204 us instead of 193); the others would spill (104 instead of 95).
 template <int QDT, int FMT, int SDT, bool ALONE>
 __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 : 1) void paged_decode_kernel(
     const int32_t* lens, const int32_t* tables, const void* k, const void* v, int batch, int n_kv, int width, int page_shift,

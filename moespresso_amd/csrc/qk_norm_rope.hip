@@ -11,8 +11,9 @@
 // is whole rows (with 32 bytes of a float32 row a lane, every line was asked for twice), the sum of squares is five or six lane
 // exchanges, the partner of a channel one more. A wave takes neighbouring heads of one kind, so that whose row it is and where
 // it lies is scalar arithmetic, and asks for its next rows before it works on these. Loads are non-temporal, as nothing reads
-// the projections' output again (16384 tokens of bfloat16 rows, appended: 56 us, 6.0 TB/s, instead of 67). The cosines and
-// sines of a workgroup's tokens are made once, a thread each, under the first rows' loads, and shared through LDS.
+// the projections' output again (16384 tokens of bfloat16 rows, appended: the kernel alone 56 us, 6.0 TB/s, instead of 67; calls
+// behind each other, of which each finds the last one's writes still under way, 71 us, 4.7 TB/s). The cosines and sines of a
+// workgroup's tokens are made once, a thread each, under the first rows' loads, and shared through LDS.
 #include "affine_q8.h"
 #include "common.h"
 
