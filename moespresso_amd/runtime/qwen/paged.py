@@ -500,7 +500,7 @@ class PagedAttention(torch.nn.Module):
         super().__init__()
         if inner.q_norm.eps != inner.k_norm.eps:
             raise ValueError("q_norm and k_norm must share an eps")
-        _, kv_heads, _ = _check_pages(cache.keys, cache.values)
+        self.n_pages, kv_heads, self.page_size = _check_pages(cache.keys, cache.values)
         if inner.num_key_value_heads != kv_heads:
             raise ValueError("the block and the cache disagree on the number of KV heads")
         if inner.num_attention_heads % kv_heads != 0 or not 1 <= inner.num_attention_heads // kv_heads <= 16:
@@ -517,6 +517,8 @@ class PagedAttention(torch.nn.Module):
                 raise RuntimeError("hooks of q_norm, k_norm and rope would not run: this layer takes their weights and frequencies")
         T = int(x.shape[0])
         heads, kv_heads = inner.num_attention_heads, inner.num_key_value_heads
+        if tables.page_size != self.page_size or int(tables.free_pages.shape[0]) > self.n_pages:
+            raise ValueError("the tables name pages of another size, or more of them, than the cache has")
         most = _queries_a_call(kv_heads, tables.page_size, int(tables.tables.shape[1]))
         if most < 1:  # (before anything is written)
             raise ValueError("the tables hold too many tokens together")

@@ -162,3 +162,13 @@ def test_modules_that_give_something_of_another_kind_are_not_compared():
 
     _with(rope=Tables(), q_norm=Residual())
     _with(rope=Positions())
+
+
+def test_tables_of_another_pool_are_refused(monkeypatch):
+    """Slots of another page size are other rows, and pages beyond the pool would be left out without a word."""
+    layer, step, tables = _layer(monkeypatch)
+    x = torch.randn(5, HIDDEN)
+    for n_pages, page_size in ((4, 32), (2, 64), (5, 16)):
+        with pytest.raises(ValueError, match="than the cache has"):
+            layer(x, step, paged.PageTables(2, n_pages, page_size=page_size, max_tokens=64, device="cpu"))
+    layer(x, step, paged.PageTables(2, 3, page_size=16, max_tokens=64, device="cpu"))
