@@ -152,6 +152,14 @@ SIGNATURES = {
         c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
                 c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p,
                 c_size_t, c_void_p]),
+    "mspr_sdpa_decode_paged_shared_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "mspr_sdpa_decode_paged_shared": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mspr_sdpa_decode_paged_shared_q8": (
+        c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                c_float, c_int, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
     "mspr_profile_enable": (c_int, [c_int]),
     "mspr_profile_collect": (c_int, [c_int, c_void_p, c_int]),
 }
@@ -202,6 +210,12 @@ def paged_decode_workspace(batch: int, n_q_heads: int, n_kv_heads: int, page_siz
     """Scratch tensor for the paged decode entry points (partials of the rows that are cut, and which are)."""
     nbytes = int(lib().mspr_sdpa_decode_paged_workspace_bytes(int(batch), int(n_q_heads), int(n_kv_heads), int(page_size),
                                                               int(table_width)))
+    return torch.empty((max(nbytes, 16) + 3) // 4, dtype=torch.float32, device=device)
+
+
+def paged_shared_workspace(batch: int, n_q_heads: int, n_kv_heads: int, n_prefixes: int, device) -> torch.Tensor:
+    """Scratch tensor for the decode entry points over shared prefixes (partials of every piece, and which a query has)."""
+    nbytes = int(lib().mspr_sdpa_decode_paged_shared_workspace_bytes(int(batch), int(n_q_heads), int(n_kv_heads), int(n_prefixes)))
     return torch.empty((max(nbytes, 16) + 3) // 4, dtype=torch.float32, device=device)
 
 

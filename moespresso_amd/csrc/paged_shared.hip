@@ -1,0 +1,1028 @@
+// Attention of new tokens over a paged KV cache in which groups of requests share a prefix.
+//
+//   out[r, h] = sum_k softmax_k(q[r, h] . K[k] * scale) V[k]   over the rows of the prefix that the query's request continues,
+//                                                              then the first lens[r] rows of the request's own table
+//
+// Pages, head dim and arithmetic are those of paged_decode.hip (16-bit rows, or affine 8-bit rows in groups of 64; S^T = K.Q^T
+// and O^T = V^T.P^T by 16x16x32 matrix instructions, an online softmax a wave, weights in two terms). What differs: a wave
+// multiplies a tile of 32 keys, once it is in registers, with up to 32 columns, the query heads of several members of a group.
+//
+// Work is cut into pieces: a block of a prefix's members (as many as fill 32 columns) or a query's own rows, of one KV head, over
+// a range of tiles. Every workgroup plans for itself (lengths and groups are known on the device only): a range's length follows
+// from all tiles there are, so that a piece falls to every compute unit; the number of a piece says what it is. Blocks of one
+// range lie eight workgroups apart, on one XCD, whose L2 then has the rows for the second block. The four waves of a workgroup
+// take the tiles of a piece in turn and meet in LDS; a second kernel joins a query's pieces.
+#include "paged_rows.h"
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kGroups = 256;    // workgroups that run at once: one a compute unit
+constexpr int kColumns = 32;    // of a piece, in blocks of 16
+constexpr int kBlocks = kColumns / 16;
+constexpr int kMinShare = 4;    // tiles of a range, at least: one a wave
+constexpr int kMaxRows = 2048;  // queries, and prefixes, of a call
+
+struct SharedRest {
+  const void* q;                  // [B, Hq, D]
+  const int32_t* prefix_tables;   // [n_prefixes, prefix_width]
+  const int32_t* tables;          // [n_tables, width]
+  const void *k, *v, *k_scales, *k_biases, *v_scales, *v_biases;
+  int n_pages, page_shift, prefix_width, width, prefix_slots, own_slots;
+  float scale_log2;
+  float* ws_pre;      // partial outputs of prefix pieces [prefix_slots][32 columns][256]
+  float* ws_pre_ml;   // their statistics [prefix_slots][32][2]
+  float* ws_own;      // of own pieces [own_slots][rep][256]
+  float* ws_own_ml;   // [own_slots][16][2]
+  int32_t* parts;     // [B * n_kv][8]: of own pieces the first and how many; of prefix pieces the first, ranges, blocks, first column
+  void* out;          // [B, Hq, D]
+};
+
+struct SharedArgs {
+  const int32_t *requests, *groups, *lens, *prefix_lens;
+  int batch, n_prefixes, n_tables, n_kv, rep;
+  int pieces;  // workgroups: no less than the pieces there can be
+  SharedRest rest;
+};
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// Pieces of a prefix: ranges of all KV heads ("bundles" of blocks) by eights, block by block, so that the blocks of a bundle are
+// multiples of eight apart.
+__device__ __forceinline__ int bundle_piece(int bundle, int block, int bundles, int blocks) {
+  const int q = bundle / 8;
+  return 8 * blocks * q + block * min(8, bundles - 8 * q) + bundle % 8;
+}
+
+constexpr int kPlanInts = 3 * kMaxRows + 2 * kMaxRows;  // groups of rows; tiles of prefixes and rows; members of prefixes
+
+__host__ __device__ constexpr int shared_query_bytes(int qdt, int fmt) {
+  return kBlocks * 8 * 64 * 16 * (fmt == kAffine && qdt == MSPR_F32 ? 2 : 1);
+}
+__host__ __device__ constexpr int shared_lds(int qdt, int fmt) { return kWaves * kVTileBytes + shared_query_bytes(qdt, fmt); }
+static_assert(kWaves * kVTileBytes >= kPlanInts * 4, "the plan fits into the V tiles");
+static_assert(kWaves * kVTileBytes >= (kWaves * 16 * 64 * 4 + kWaves * 16 * 2) * 4, "the exchange fits into the V tiles");
+
+// What a workgroup works on.
+struct Piece {
+  int prefix;          // number of the prefix, -1: a query's own rows
+  int row;             // the query (own rows), its first column's (a prefix)
+  int block, blocks;   // of a prefix's members
+  int kvh, range, ranges;
+  int first;           // the first piece of the prefix, or the query's first piece of this KV head among own pieces
+  int slot;            // where partials go
+};
+
+// The tiles of one piece for NB blocks of 16 columns.
+template <int QDT, int FMT, int SDT, int NB>
+__device__ __forceinline__ void attend_piece(const SharedRest& a, const Piece& p, const int32_t* table, int len, int tile0, int tile1,
+                                             int n_kv, int rep, int columns, bool whole, const int* members, unsigned char* lds) {
+  constexpr bool kCodes = FMT == kAffine;
+  constexpr int kVType = kCodes ? MSPR_F16 : FMT;
+  constexpr int kPTerms = 2;                                   // terms of a weight
+  constexpr int kQTerms = kCodes && QDT == MSPR_F32 ? 2 : 1;  // terms of a query element
+  // (float16 weights are taken 2^11 times as large, see paged_decode.hip; the reference maximum lags by 2^4 at most)
+  constexpr float kLag = 4.0f;
+  constexpr float kUp = kVType == MSPR_F16 ? 11.0f : 0.0f;
+  constexpr int kRowBytes = kCodes ? kD : kD * 2;
+  constexpr int kSteps = 8 / kWaves;  // of the query operand, made by a wave
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15;  // MFMA column within its block; row (key) of the K operand
+  const int g = lane >> 4;
+  unsigned char* vt = lds + wave * kVTileBytes;
+  const int page_mask = (1 << a.page_shift) - 1;
+  const int last_tile = min(tile1, ceil_div(len, kTileKeys));
+
+  // ---- the queries are asked for first: loads come back in order, and the pages' addresses wait for the table anyway
+  constexpr int kQWords = QDT == MSPR_F32 ? 2 : 1;  // of sixteen bytes a step
+  bool mine[NB];
+  u32x4_t qraw[NB][kSteps * kQWords];
+#pragma unroll
+  for (int b = 0; b < NB; b++) {
+    const int column = 16 * b + n;
+    mine[b] = column < columns;
+    const int member = mine[b] ? column / rep : 0;
+    const int64_t q0 = (((int64_t)members[member] * n_kv + p.kvh) * rep + (mine[b] ? column - member * rep : 0)) * kD;
+#pragma unroll
+    for (int i = 0; i < kSteps; i++) {
+      const int step = kSteps * wave + i;
+      const int channel = kCodes ? 32 * (step & ~1) + 16 * g + 8 * (i & 1) : 32 * step + 8 * g;
+      constexpr int kQBytes = QDT == MSPR_F32 ? 4 : 2;
+      const u32x4_t* from = reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint8_t*>(a.q) + (q0 + channel) * kQBytes);
+#pragma unroll
+      for (int j = 0; j < kQWords; j++) qraw[b][i * kQWords + j] = from[j];
+    }
+  }
+  __builtin_amdgcn_sched_barrier(0);
+
+  f32x4_t oacc[NB][16];
+#pragma unroll
+  for (int b = 0; b < NB; b++)
+#pragma unroll
+    for (int mt = 0; mt < 16; mt++) oacc[b][mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float m_run[NB], l_run[NB];
+  f32x4_t bacc[NB];  // weighted biases: lane n (g = 0) has those of column n and the four groups
+#pragma unroll
+  for (int b = 0; b < NB; b++) {
+    m_run[b] = -__builtin_inff();
+    l_run[b] = 0.0f;
+    bacc[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  float v_unit = 0x1p-126f;  // what V's scales of group n % 4 are multiples of
+
+  // Pages of this wave's tiles, two half tiles of 16 keys each: lane i of `ids` has the page of half tile i of 31 tiles and the
+  // one behind them.
+  const int n_mine = last_tile - tile0 > wave ? (last_tile - tile0 - wave + kWaves - 1) / kWaves : 0;
+  auto load_ids = [&](int it0) {
+    const int it = it0 + (lane >> 1);
+    const int key = (tile0 + wave + kWaves * it) * kTileKeys + 16 * (lane & 1);
+    const int e = it < n_mine && key < len ? key >> a.page_shift : -1;
+    return e >= 0 ? table[e] : -1;
+  };
+  struct Half {
+    int64_t row;  // first row in the pages
+    int rows;     // how many count
+  };
+  auto half_at = [&](int ids, int it0, int it, int u) {
+    const int key = (tile0 + wave + kWaves * it) * kTileKeys + 16 * u;
+    const int page = __builtin_amdgcn_readlane(ids, 2 * (it - it0) + u);
+    const bool good = page >= 0 && page < a.n_pages;
+    Half h;
+    h.row = ((((int64_t)(good ? page : 0) * n_kv + p.kvh) << a.page_shift) + (key & page_mask));
+    h.rows = __builtin_amdgcn_readfirstlane(!good || it >= n_mine ? 0 : len - key >= 16 ? 16 : len - key < 0 ? 0 : len - key);
+    return h;
+  };
+
+  constexpr int kLoads = kCodes ? 4 : 8;  // 16-byte pieces a lane and half tile
+  u32x4_t kr[2][kLoads], vr[2][kLoads];
+  RowScales<SDT> ks[2], kb[2], vs[2], vb[2];
+  auto load_k = [&](const Half* h) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const auto w = rows_window(a.k, h[u].row, kRowBytes, h[u].rows);
+#pragma unroll
+      for (int j = 0; j < kLoads; j++) kr[u][j] = window_load16(w, n * kRowBytes + 16 * g, 64 * j);
+      if constexpr (kCodes) {
+        ks[u].load(rows_window(a.k_scales, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 16 * g + n);
+        kb[u].load(rows_window(a.k_biases, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 4 * n + g);
+      }
+    }
+  };
+  auto load_v = [&](const Half* h) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const auto w = rows_window(a.v, h[u].row, kRowBytes, h[u].rows);
+#pragma unroll
+      for (int j = 0; j < kLoads; j++) vr[u][j] = window_load16(w, 16 * lane, 1024 * j);
+    }
+  };
+  auto load_v_scales = [&](const Half* h) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      vs[u].load(rows_window(a.v_scales, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 16 * g + n);
+      vb[u].load(rows_window(a.v_biases, h[u].row, 4 * RowScales<SDT>::kBytes, h[u].rows), 16 * g + n);
+    }
+  };
+
+  int ids = load_ids(0);
+  Half cur[2] = {half_at(ids, 0, 0, 0), half_at(ids, 0, 0, 1)}, nxt[2];
+  load_k(cur);
+  load_v(cur);
+  if constexpr (kCodes) load_v_scales(cur);
+  int ids_next = load_ids(31);
+  __builtin_amdgcn_sched_barrier(0);  // the first tile is on its way before the queries are fetched
+
+  // ---- Q^T operands, in LDS for all waves: [blocks][8 steps][terms][64 lanes]
+  u32x4_t* qt = reinterpret_cast<u32x4_t*>(lds + kWaves * kVTileBytes) + lane;
+  float q_unit[NB], qsum[NB];
+#pragma unroll
+  for (int b = 0; b < NB; b++) {
+    q_unit[b] = a.scale_log2;
+    qsum[b] = 0.0f;
+  }
+  if constexpr (!kCodes) {
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int i = 0; i < kSteps; i++)
+        qt[64 * (8 * b + kSteps * wave + i)] = mine[b] ? qraw[b][i] : u32x4_t{0u, 0u, 0u, 0u};
+  } else {
+    auto element = [&](int b, int i, float* x) {
+      if constexpr (QDT == MSPR_F32) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = __uint_as_float(qraw[b][2 * i + j / 4][j % 4]);
+      } else {
+        widen8<QDT>(qraw[b][i], x);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] = mine[b] ? x[j] : 0.0f;
+    };
+    float* shared = reinterpret_cast<float*>(lds);  // [2][blocks][waves][16 columns], where the V tiles will be
+    int e[NB] = {};
+    if constexpr (QDT != MSPR_F16) {  // a power of two brings the column's largest element to [2^14, 2^15)
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kSteps; i++) {
+          float x[8];
+          element(b, i, x);
+#pragma unroll
+          for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[j]));
+        }
+        top = half_wave_max(row_pair_max(top));
+        if (g == 0) shared[64 * b + 16 * wave + n] = top;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        float top = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) top = fmaxf(top, shared[64 * b + 16 * w + n]);
+        if (top > 0.0f && top < __builtin_inff()) e[b] = __builtin_amdgcn_frexp_expf(top) - 15;
+      }
+    }
+    static_assert(kSteps == 2, "a wave makes the operands of one group of 64 channels");
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kSteps; i++) {
+        float x[8];
+        element(b, i, x);
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = __builtin_amdgcn_ldexpf(x[j], -e[b]);
+        u32x4_t terms[kQTerms];
+        split_terms<MSPR_F16, kQTerms>(x, terms);
+#pragma unroll
+        for (int t = 0; t < kQTerms; t++) {  // (of the terms, as the products are)
+          float y[8];
+          widen8<MSPR_F16>(terms[t], y);
+#pragma unroll
+          for (int j = 0; j < 8; j++) sum += y[j];
+          qt[64 * ((8 * b + kSteps * wave + i) * kQTerms + t)] = terms[t];
+        }
+      }
+      q_unit[b] = __builtin_amdgcn_ldexpf(a.scale_log2, e[b]);
+      sum += __shfl_xor(sum, 16, MSPR_WAVE);
+      sum += __shfl_xor(sum, 32, MSPR_WAVE);
+      if (g == 0) shared[64 * kBlocks + 64 * b + 16 * wave + n] = sum;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < NB; b++) qsum[b] = shared[64 * kBlocks + 64 * b + 16 * g + n];
+  }
+  __syncthreads();
+
+  const int tr_off = (4 * g + ((lane & 15) >> 2)) * kVPitch + 4 * (lane & 3) * 2;
+  for (int it0 = 0; it0 < n_mine; it0 += 31) {
+    const int it_end = min(it0 + 31, n_mine);
+    for (int it = it0; it < it_end; it++) {
+      nxt[0] = half_at(ids, it0, it + 1, 0);
+      nxt[1] = half_at(ids, it0, it + 1, 1);
+
+      // ---- S^T = K . Q^T
+      float s[NB][8];  // key 16 u + 4 g + i at 4 u + i
+      if constexpr (!kCodes) {
+        f32x4_t acc[2][NB];
+#pragma unroll
+        for (int b = 0; b < NB; b++) acc[0][b] = acc[1][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+#pragma unroll
+          for (int b = 0; b < NB; b++) {
+            const u32x4_t qf = qt[64 * (8 * b + j)];
+            acc[0][b] = mfma<FMT>(kr[0][j], qf, acc[0][b]);
+            acc[1][b] = mfma<FMT>(kr[1][j], qf, acc[1][b]);
+          }
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int i = 0; i < 8; i++) s[b][i] = acc[i >> 2][b][i & 3] * q_unit[b];
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+          const float ksf = ks[u].value(n);
+          const float of_bias = __int_as_float(__builtin_amdgcn_ds_bpermute(4 * (4 * n + g), __float_as_int(ksf)));
+          const float bias = fmaf(128.0f, of_bias, kb[u].value(g));
+          f32x4_t sum[NB];
+#pragma unroll
+          for (int b = 0; b < NB; b++) sum[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(bias, qsum[b], zero, 0, 0, 0);
+          static_for<4>([&](auto jc) {
+            constexpr int j = decltype(jc)::value;
+            f32x4_t acc[NB];
+#pragma unroll
+            for (int b = 0; b < NB; b++) acc[b] = zero;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              u32x4_t c;
+#pragma unroll
+              for (int w = 0; w < 2; w++) {
+                h2_t lo, hi;
+                centred_to_h(kr[u][j][2 * h + w], lo, hi);
+                c[2 * w] = h2_bits(lo);
+                c[2 * w + 1] = h2_bits(hi);
+              }
+#pragma unroll
+              for (int t = 0; t < kQTerms; t++)
+#pragma unroll
+                for (int b = 0; b < NB; b++) acc[b] = mfma<MSPR_F16>(c, qt[64 * ((8 * b + 2 * j + h) * kQTerms + t)], acc[b]);
+            }
+            static_for<4>([&](auto ic) {
+              constexpr int i = decltype(ic)::value;
+              const float by = of_lane<4 * i + j>(ksf);
+#pragma unroll
+              for (int b = 0; b < NB; b++) sum[b][i] = fmaf(by, acc[b][i], sum[b][i]);
+            });
+          });
+#pragma unroll
+          for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[b][4 * u + i] = sum[b][i] * q_unit[b];
+        }
+      }
+      load_k(nxt);
+      __builtin_amdgcn_sched_barrier(0);
+
+      // ---- online softmax (powers of two), the reference maximum moves only past 2^4
+      float tmax[NB];
+      bool grow = false;
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        tmax[b] = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          if (4 * g + (i & 3) >= cur[i >> 2].rows) s[b][i] = -__builtin_inff();
+          tmax[b] = fmaxf(tmax[b], s[b][i]);
+        }
+        tmax[b] = half_wave_max(row_pair_max(tmax[b]));
+        grow |= tmax[b] > m_run[b] + kLag;
+      }
+      if (__any(grow)) {
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+          const bool up = tmax[b] > m_run[b] + kLag;
+          const float m_new = up ? tmax[b] : m_run[b];
+          if (it > 0) {  // (sums of nothing need no new scale)
+            const float alpha = up ? __builtin_amdgcn_exp2f(m_run[b] - m_new) : 1.0f;
+            l_run[b] *= alpha;
+#pragma unroll
+            for (int mt = 0; mt < 16; mt++) oacc[b][mt] = oacc[b][mt] * alpha;
+            bacc[b] = bacc[b] * alpha;
+          }
+          m_run[b] = m_new;
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        const float m_safe = (m_run[b] == -__builtin_inff() ? 0.0f : m_run[b]) - kUp;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          s[b][i] = __builtin_amdgcn_exp2f(s[b][i] - m_safe);
+          l_run[b] += s[b][i];
+        }
+      }
+
+      // ---- V rows to LDS (zeros in the place of rows that do not count)
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int j = 0; j < kLoads; j++) {
+          if constexpr (!kCodes) {
+            *reinterpret_cast<u32x4_t*>(vt + (16 * u + 2 * j + (lane >> 5)) * kVPitch + 16 * (lane & 31)) = vr[u][j];
+          } else {
+            u32x4_t lo, hi;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+              h2_t c01, c23;
+              centred_to_h(vr[u][j][w], c01, c23);
+              (w < 2 ? lo : hi)[2 * (w & 1)] = h2_bits(c01);
+              (w < 2 ? lo : hi)[2 * (w & 1) + 1] = h2_bits(c23);
+            }
+            unsigned char* d = vt + (16 * u + 4 * j + (lane >> 4)) * kVPitch + 32 * (lane & 15);
+            *reinterpret_cast<u32x4_t*>(d) = lo;
+            *reinterpret_cast<u32x4_t*>(d + 16) = hi;
+          }
+        }
+      load_v(nxt);
+      cur[0] = nxt[0];
+      cur[1] = nxt[1];
+      __builtin_amdgcn_sched_barrier(0);
+
+      // ---- O^T += V^T . P^T (the tile was written by this wave only: LDS operations of one wave complete in order)
+      __builtin_amdgcn_wave_barrier();
+      u32x4_t vf[2][4];
+      auto read_v = [&](int q4) {
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+          const unsigned char* base = vt + tr_off + (4 * q4 + m) * 32;
+          const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, base)));
+          const u32x2_t hi =
+              __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, base + 16 * kVPitch)));
+          vf[q4 & 1][m] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
+        }
+      };
+      u32x4_t pf[NB][kPTerms];
+      auto accumulate = [&](int q4) {
+        if (q4 < 3) read_v(q4 + 1);
+#pragma unroll
+        for (int t = 0; t < kPTerms; t++)
+#pragma unroll
+          for (int m = 0; m < 4; m++)
+#pragma unroll
+            for (int b = 0; b < NB; b++) oacc[b][4 * q4 + m] = mfma<kVType>(vf[q4 & 1][m], pf[b][t], oacc[b][4 * q4 + m]);
+      };
+      read_v(0);
+      if constexpr (!kCodes) {
+#pragma unroll
+        for (int b = 0; b < NB; b++) split_terms<kVType, kPTerms>(s[b], pf[b]);
+#pragma unroll
+        for (int q4 = 0; q4 < 4; q4++) accumulate(q4);
+      } else {
+        float vsf[2] = {vs[0].value(n), vs[1].value(n)};
+        const float largest = fmaxf(fabsf(vsf[0]), fabsf(vsf[1]));
+        if (__any(largest > v_unit)) {
+          float top = largest;
+          top = fmaxf(top, lane_xor<4>(top));
+          top = fmaxf(top, lane_xor<8>(top));
+          top = half_wave_max(row_pair_max(top));
+          const int e = top < 0x1p126f ? __builtin_amdgcn_frexp_expf(top) : 126;
+          const float unit = top > v_unit ? __builtin_amdgcn_ldexpf(1.0f, e) : v_unit;
+          if (it > 0) {
+            const float by = v_unit / unit;
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+              static_for<16>([&](auto mt) { oacc[b][mt] = oacc[b][mt] * of_lane<decltype(mt)::value / 4>(by); });
+          }
+          v_unit = unit;
+        }
+        const float per_unit = 1.0f / v_unit;
+        vsf[0] *= per_unit;
+        vsf[1] *= per_unit;
+        const float vbf[2] = {fmaf(128.0f, vs[0].value(n), vb[0].value(n)), fmaf(128.0f, vs[1].value(n), vb[1].value(n))};
+        static_for<8>([&](auto ic) {
+          constexpr int i = decltype(ic)::value;
+          float bias = vbf[i >> 2];
+          if constexpr ((i & 3) != 0)
+            bias = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(bias), 0x100 + 4 * (i & 3), 0xF, 0xF, true));  // row_shl
+#pragma unroll
+          for (int b = 0; b < NB; b++) bacc[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(bias, s[b][i], bacc[b], 0, 0, 0);
+        });
+        static_for<4>([&](auto jc) {  // the weights of group j, which has channels 64 j on
+          constexpr int j = decltype(jc)::value;
+          float of_key[8];
+          static_for<8>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            of_key[i] = of_lane<4 * (i & 3) + j>(vsf[i >> 2]);
+          });
+#pragma unroll
+          for (int b = 0; b < NB; b++) {
+            float w[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              w[i] = of_key[i] * s[b][i];
+              asm("" : "+v"(w[i]));  // (a rounded product, see paged_decode.hip)
+            }
+            split_terms<kVType, kPTerms>(w, pf[b]);
+          }
+          accumulate(j);
+        });
+      }
+      if constexpr (kCodes) load_v_scales(nxt);
+      __builtin_amdgcn_wave_barrier();
+    }
+    ids = ids_next;
+    ids_next = load_ids(it_end + 31);
+  }
+
+  // ---- the four waves meet in LDS, a block of columns at a time (the V tiles are free now)
+  float* xo = reinterpret_cast<float*>(lds);   // [waves][16 mt][64 lanes][4]
+  float* xml = xo + kWaves * 16 * 64 * 4;      // [waves][16 columns][2]
+  const int width = p.prefix >= 0 ? kColumns : rep;  // columns of a partial
+  const auto po = store_window((p.prefix >= 0 ? a.ws_pre : a.ws_own) + (int64_t)p.slot * width * kD, width * kD * (int)sizeof(float));
+  float* ml = p.prefix >= 0 ? a.ws_pre_ml + (int64_t)p.slot * kColumns * 2 : a.ws_own_ml + (int64_t)p.slot * 16 * 2;
+#pragma unroll
+  for (int b = 0; b < NB; b++) {
+    l_run[b] += __shfl_xor(l_run[b], 16, MSPR_WAVE);
+    l_run[b] += __shfl_xor(l_run[b], 32, MSPR_WAVE);
+    if constexpr (kCodes) {
+      float bias[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) bias[j] = __shfl(bacc[b][j], n, MSPR_WAVE);
+      static_for<16>([&](auto mt) { oacc[b][mt] = oacc[b][mt] * of_lane<decltype(mt)::value / 4>(v_unit) + bias[mt >> 2]; });
+    }
+    __syncthreads();
+#pragma unroll
+    for (int mt = 0; mt < 16; mt++) *reinterpret_cast<f32x4_t*>(xo + ((wave * 16 + mt) * 64 + lane) * 4) = oacc[b][mt];
+    if (g == 0) {
+      xml[(wave * 16 + n) * 2] = m_run[b];
+      xml[(wave * 16 + n) * 2 + 1] = l_run[b];
+    }
+    __syncthreads();
+    float mw[kWaves], m_all = -__builtin_inff(), l_all = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+      mw[w] = xml[(w * 16 + n) * 2];
+      m_all = fmaxf(m_all, mw[w]);
+    }
+    const float m_safe = m_all == -__builtin_inff() ? 0.0f : m_all;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+      mw[w] = __builtin_amdgcn_exp2f(mw[w] - m_safe);
+      l_all += xml[(w * 16 + n) * 2 + 1] * mw[w];
+    }
+    const int column = 16 * b + n;
+#pragma unroll
+    for (int q4 = 0; q4 < 16 / kWaves; q4++) {
+      const int mt = wave * (16 / kWaves) + q4;
+      f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) acc += *reinterpret_cast<const f32x4_t*>(xo + ((w * 16 + mt) * 64 + lane) * 4) * mw[w];
+      if (!mine[b]) continue;
+      if (whole) store_out<QDT>(a.out, (((int64_t)p.row * n_kv + p.kvh) * rep + column) * kD + 16 * mt + 4 * g, acc, l_all);
+      else window_store<kStoreThrough>(po, (column * kD + 16 * mt + 4 * g) * 4, __builtin_bit_cast(u32x4_t, acc));
+    }
+    if (!whole && wave == 0 && g == 0 && mine[b]) *reinterpret_cast<f32x2_t*>(ml + 2 * column) = f32x2_t{m_all, l_all};
+  }
+}
+
+// QDT: type of queries and output; FMT: page format; SDT: type of scales and biases (8-bit pages). A piece a workgroup.
+template <int QDT, int FMT, int SDT>
+__global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(const int32_t* requests, const int32_t* groups, const int32_t* lens,
+                                                                   const int32_t* prefix_lens, int batch, int n_prefixes,
+                                                                   int n_tables, int n_kv, int rep, SharedRest a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  __shared__ int wave_sums[3][kWaves];
+  __shared__ int members[kColumns];
+  __shared__ Piece found;
+  const int t = threadIdx.x;
+  const int lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int number = blockIdx.x;
+
+  // ---- the plan: which query belongs to which prefix, and how many tiles there are
+  int* row_group = reinterpret_cast<int*>(lds);       // [batch]
+  int* tiles = row_group + kMaxRows;                  // [n_prefixes, then batch]
+  int* count = tiles + 2 * kMaxRows;                  // [n_prefixes]
+  const int prefix_cap = a.prefix_width << a.page_shift, cap = a.width << a.page_shift;
+  for (int i = t; i < n_prefixes; i += kThreads) {
+    tiles[i] = ceil_div(length_of(prefix_lens, n_prefixes, i, prefix_cap), kTileKeys);
+    count[i] = 0;
+  }
+  __syncthreads();
+  for (int r = t; r < batch; r += kThreads) {
+    const int request = requests ? requests[r] : r;
+    const bool known = request >= 0 && request < n_tables;
+    int group = known ? groups[request] : -1;
+    if (group < 0 || group >= n_prefixes || tiles[group] == 0) group = -1;
+    row_group[r] = group;
+    tiles[n_prefixes + r] = known ? ceil_div(length_of(lens, batch, r, cap), kTileKeys) : 0;
+    if (group >= 0) atomicAdd(&count[group], 1);
+  }
+  if (t == 0) found.kvh = -1;
+  __syncthreads();
+  const int rows_a_block = kColumns / rep;
+  const int entries = n_prefixes + batch, per = ceil_div(entries, kThreads);
+  const int e0 = min(t * per, entries), e1 = min(e0 + per, entries);
+  int sum = 0, units = 0;
+  for (int e = e0; e < e1; e++) {
+    const int blocks = e < n_prefixes ? ceil_div(count[e], rows_a_block) : 1;
+    sum += blocks * tiles[e];
+    units += blocks;
+  }
+  sum = wave_scan(sum);
+  units = wave_scan(units);
+  if (lane == 63) {
+    wave_sums[0][wave] = sum;
+    wave_sums[1][wave] = units;
+  }
+  __syncthreads();
+  int all = 0, all_units = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) {
+    all += wave_sums[0][w];
+    all_units += wave_sums[1][w];
+  }
+  all = __builtin_amdgcn_readfirstlane(all) * n_kv;
+  all_units = __builtin_amdgcn_readfirstlane(all_units) * n_kv;
+  // A range's tiles: no more pieces than compute units, as a unit has at most one piece that is not full; where there are too
+  // many units for that, half as many again.
+  const int share = max(kMinShare, ceil_div(all, max(kGroups - all_units, kGroups / 2)));
+  int pieces = 0, of_prefixes = 0;
+  for (int e = e0; e < e1; e++) {
+    const int ranges = max(1, ceil_div(tiles[e], share));
+    const int blocks = e < n_prefixes ? ceil_div(count[e], rows_a_block) : 1;
+    pieces += n_kv * blocks * ranges;
+    if (e < n_prefixes) of_prefixes += n_kv * blocks * ranges;
+  }
+  const int upto = wave_scan(pieces);
+  of_prefixes = wave_scan(of_prefixes);
+  __syncthreads();
+  if (lane == 63) {
+    wave_sums[0][wave] = upto;
+    wave_sums[2][wave] = of_prefixes;
+  }
+  __syncthreads();
+  int before = upto - pieces, prefix_pieces = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) {
+    if (w < wave) before += wave_sums[0][w];
+    prefix_pieces += wave_sums[2][w];
+  }
+  if (number >= before && number < before + pieces) {
+    for (int e = e0; e < e1; e++) {
+      const int ranges = max(1, ceil_div(tiles[e], share));
+      const int blocks = e < n_prefixes ? ceil_div(count[e], rows_a_block) : 1;
+      const int own = n_kv * blocks * ranges;
+      if (number < before + own) {
+        Piece p;
+        p.blocks = blocks;
+        p.ranges = ranges;
+        const int i = number - before;
+        int bundle;
+        if (e < n_prefixes) {
+          const int bundles = n_kv * ranges, q = i / (8 * blocks), j = i - 8 * blocks * q, m = min(8, bundles - 8 * q);
+          p.prefix = e;
+          p.row = 0;
+          p.block = j / m;
+          bundle = 8 * q + j % m;
+          p.first = before;
+          p.slot = number;
+        } else {
+          p.prefix = -1;
+          p.row = e - n_prefixes;
+          p.block = 0;
+          bundle = i;
+          p.slot = number - prefix_pieces;
+          p.first = p.slot - i % ranges;
+        }
+        p.kvh = bundle / ranges;
+        p.range = bundle - p.kvh * ranges;
+        found = p;
+        break;
+      }
+      before += own;
+    }
+  }
+  __syncthreads();
+  Piece p;
+  p.kvh = __builtin_amdgcn_readfirstlane(found.kvh);
+  if (p.kvh < 0) return;  // (more workgroups than pieces)
+  p.prefix = __builtin_amdgcn_readfirstlane(found.prefix);
+  p.row = __builtin_amdgcn_readfirstlane(found.row);
+  p.block = __builtin_amdgcn_readfirstlane(found.block);
+  p.blocks = __builtin_amdgcn_readfirstlane(found.blocks);
+  p.range = __builtin_amdgcn_readfirstlane(found.range);
+  p.ranges = __builtin_amdgcn_readfirstlane(found.ranges);
+  p.first = __builtin_amdgcn_readfirstlane(found.first);
+  p.slot = __builtin_amdgcn_readfirstlane(found.slot);
+
+  // ---- the queries of the piece
+  int n_members = 1, n_tiles, len;
+  const int32_t* table;
+  bool whole = false;
+  if (p.prefix >= 0) {
+    const int per_row = ceil_div(batch, kThreads);
+    const int r0 = min(t * per_row, batch), r1 = min(r0 + per_row, batch);
+    int mine = 0;
+    for (int r = r0; r < r1; r++) mine += row_group[r] == p.prefix;
+    const int scanned = wave_scan(mine);
+    if (lane == 63) wave_sums[1][wave] = scanned;
+    __syncthreads();
+    int rank = scanned - mine - p.block * rows_a_block;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++)
+      if (w < wave) rank += wave_sums[1][w];
+    for (int r = r0; r < r1; r++)
+      if (row_group[r] == p.prefix) {
+        if (rank >= 0 && rank < rows_a_block) {
+          members[rank] = r;
+          if (p.range == 0) {
+            int32_t* at = a.parts + 8 * ((int64_t)r * n_kv + p.kvh);
+            at[2] = p.first;
+            at[3] = p.ranges;
+            at[4] = p.blocks;
+            at[5] = p.block * kColumns + rank * rep;
+          }
+        }
+        rank++;
+      }
+    n_members = min(rows_a_block, __builtin_amdgcn_readfirstlane(count[p.prefix]) - p.block * rows_a_block);
+    n_tiles = __builtin_amdgcn_readfirstlane(tiles[p.prefix]);
+    len = __builtin_amdgcn_readfirstlane(length_of(prefix_lens, n_prefixes, p.prefix, prefix_cap));
+    table = a.prefix_tables + (int64_t)p.prefix * a.prefix_width;
+  } else {
+    n_tiles = __builtin_amdgcn_readfirstlane(tiles[n_prefixes + p.row]);
+    const bool alone = __builtin_amdgcn_readfirstlane(row_group[p.row]) < 0;
+    whole = alone && p.ranges == 1;
+    const bool some = !whole && n_tiles > 0;
+    const int request = requests ? __builtin_amdgcn_readfirstlane(requests[p.row]) : p.row;
+    len = __builtin_amdgcn_readfirstlane(length_of(lens, batch, p.row, cap));
+    table = a.tables + (int64_t)(n_tiles > 0 ? request : 0) * a.width;
+    if (n_tiles == 0) len = 0;
+    if (t == 0) {
+      members[0] = p.row;
+      if (p.range == 0) {
+        int32_t* at = a.parts + 8 * ((int64_t)p.row * n_kv + p.kvh);
+        at[0] = p.first;
+        at[1] = some ? p.ranges : 0;
+        if (alone) at[3] = 0;
+      }
+    }
+    if (!whole && !some) return;  // (no rows of its own behind a prefix)
+  }
+  __syncthreads();  // (the plan lies where the V tiles will be)
+  if (p.slot >= (p.prefix >= 0 ? a.prefix_slots : a.own_slots)) return;  // (cannot be, unless lengths change meanwhile)
+  const int tile0 = (int)((int64_t)n_tiles * p.range / p.ranges), tile1 = (int)((int64_t)n_tiles * (p.range + 1) / p.ranges);
+  const int columns = n_members * rep;
+  if (columns <= 16)
+    attend_piece<QDT, FMT, SDT, 1>(a, p, table, len, tile0, tile1, n_kv, rep, columns, whole, members, lds);
+  else
+    attend_piece<QDT, FMT, SDT, 2>(a, p, table, len, tile0, tile1, n_kv, rep, columns, whole, members, lds);
+}
+
+constexpr int kAtOnce = 16;  // pieces that a wave joins at a time
+
+// Joins the pieces of one query head: WAVES of them a head take every WAVES-th, and meet in LDS.
+// grid: heads / (kMergeWaves / WAVES)
+constexpr int kMergeWaves = 8;
+template <int ODT, int WAVES>
+__global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(const int32_t* parts, const float* ws_pre,
+                                                                              const float* ws_pre_ml, const float* ws_own,
+                                                                              const float* ws_own_ml, int rep, int n_kv, int heads,
+                                                                              int prefix_slots, int own_slots, void* out) {
+  __shared__ __attribute__((aligned(16))) float xo[kMergeWaves][kD + 2];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int head = (int)blockIdx.x * (kMergeWaves / WAVES) + wave / WAVES;
+  const int part = wave % WAVES;
+  const bool here = head < heads;
+  const int row = here ? head / rep : 0, hn = here ? head - row * rep : 0;
+  const int32_t* at = parts + 8 * (int64_t)row;
+  const int n_own = here ? at[1] : 0, ranges = here ? at[3] : 0;
+  const int total = n_own + ranges;
+  const int own_first = at[0], pre_first = at[2], blocks = at[4], column = at[5] + hn;
+  const int kvh = row % n_kv;
+  // (bounded by the workspace, whatever is there)
+  auto slot_of = [&](int i, int& col) {
+    if (i < n_own) {
+      col = hn;
+      const int s = own_first + i;
+      return s >= 0 && s < own_slots ? s : 0;
+    }
+    col = column % kColumns;
+    const int s = pre_first + bundle_piece(kvh * ranges + (i - n_own), column / kColumns, n_kv * ranges, blocks);
+    return s >= 0 && s < prefix_slots ? s : 0;
+  };
+  float m = -__builtin_inff(), l = 0.0f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  for (int p0 = part; p0 < total; p0 += kAtOnce * WAVES) {
+    const int mine = p0 + WAVES * (lane % kAtOnce);
+    f32x2_t stat = {-__builtin_inff(), 0.0f};
+    if (mine < total) {
+      int col;
+      const int s = slot_of(mine, col);
+      stat = mine < n_own ? *reinterpret_cast<const f32x2_t*>(ws_own_ml + ((int64_t)s * 16 + col) * 2)
+                          : *reinterpret_cast<const f32x2_t*>(ws_pre_ml + ((int64_t)s * kColumns + col) * 2);
+    }
+    f32x4_t ov[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; j++)  // (wave-uniform: pieces past the end cost no load)
+      if (p0 + WAVES * j < total) {
+        int col;
+        const int s = slot_of(p0 + WAVES * j, col);
+        const float* from = p0 + WAVES * j < n_own ? ws_own + ((int64_t)s * rep + col) * kD : ws_pre + ((int64_t)s * kColumns + col) * kD;
+        ov[j] = *reinterpret_cast<const f32x4_t*>(from + 4 * lane);
+      }
+    float m_new = stat.x;
+    m_new = fmaxf(m_new, lane_xor<1>(m_new));
+    m_new = fmaxf(m_new, lane_xor<2>(m_new));
+    m_new = fmaxf(m_new, lane_xor<4>(m_new));
+    m_new = fmaxf(m, fmaxf(m_new, lane_xor<8>(m_new)));
+    const float m_safe = m_new == -__builtin_inff() ? 0.0f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(m - m_safe);
+    const float w = __builtin_amdgcn_exp2f(stat.x - m_safe);
+    float lw = stat.y * w;
+    lw += lane_xor<1>(lw);
+    lw += lane_xor<2>(lw);
+    lw += lane_xor<4>(lw);
+    l = l * alpha + (lw + lane_xor<8>(lw));
+    o = o * alpha;
+#pragma unroll
+    for (int j = 0; j < kAtOnce; j++)
+      if (p0 + WAVES * j < total) o += ov[j] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), j));
+    m = m_new;
+  }
+  if constexpr (WAVES > 1) {
+    if (lane == 0) {
+      xo[wave][kD] = m;
+      xo[wave][kD + 1] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) xo[wave][4 * lane + i] = o[i];
+    __syncthreads();
+    if (part != 0) return;
+    float m_all = -__builtin_inff();
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) m_all = fmaxf(m_all, xo[wave + w][kD]);
+    const float m_safe = m_all == -__builtin_inff() ? 0.0f : m_all;
+    l = 0.0f;
+    o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+      const float wt = __builtin_amdgcn_exp2f(xo[wave + w][kD] - m_safe);
+      l += xo[wave + w][kD + 1] * wt;
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[i] += xo[wave + w][4 * lane + i] * wt;
+    }
+  }
+  if (total > 0) store_out<ODT>(out, ((int64_t)row * rep + hn) * kD + 4 * lane, o, l);
+}
+
+// Units of a call, at most: blocks of members (every prefix may have one that is not full) and queries, of every KV head.
+int64_t shared_units(int batch, int n_prefixes, int n_kv, int rep) {
+  const int rows_a_block = kColumns / rep;
+  const int used = n_prefixes < batch ? n_prefixes : batch;
+  return (int64_t)n_kv * ((batch + (int64_t)used * (rows_a_block - 1)) / rows_a_block + batch);
+}
+
+// Pieces: a call has at most max(kGroups, kGroups / 2 + units), see `share`.
+int64_t shared_pieces(int batch, int n_prefixes, int n_kv, int rep) {
+  const int64_t n = kGroups / 2 + shared_units(batch, n_prefixes, n_kv, rep);
+  return n > kGroups ? n : kGroups;
+}
+
+struct SharedScratch {
+  int64_t prefix_slots, own_slots;  // every query has a piece of its own, at least
+  size_t pre, pre_ml, own, own_ml, parts;  // bytes
+  size_t total() const { return pre + pre_ml + own + own_ml + parts; }
+};
+SharedScratch shared_scratch(int batch, int n_prefixes, int n_kv, int rep) {
+  SharedScratch s;
+  const int64_t pieces = shared_pieces(batch, n_prefixes, n_kv, rep), own = (int64_t)batch * n_kv;
+  s.prefix_slots = pieces > own ? pieces - own : 0;
+  s.own_slots = kGroups / 2 + own > kGroups ? kGroups / 2 + own : kGroups;
+  s.pre = (size_t)s.prefix_slots * kColumns * kD * sizeof(float);
+  s.pre_ml = (size_t)s.prefix_slots * kColumns * 2 * sizeof(float);
+  s.own = (size_t)s.own_slots * rep * kD * sizeof(float);
+  s.own_ml = (size_t)s.own_slots * 16 * 2 * sizeof(float);
+  s.parts = (size_t)own * 8 * sizeof(int32_t);
+  return s;
+}
+
+template <int QDT, int FMT, int SDT>
+int shared_launch(const SharedArgs& a, hipStream_t st) {
+  constexpr int kLds = shared_lds(QDT, FMT);
+  static bool attr_set[64] = {};  // by device
+  int device = 0;
+  if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64 || !attr_set[device]) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_shared_kernel<QDT, FMT, SDT>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    if (e != hipSuccess) {
+      mspr_set_error("sdpa_decode_paged_shared: cannot reserve %d bytes of LDS: %s", kLds, hipGetErrorString(e));
+      return MSPR_ERR_LAUNCH;
+    }
+    if (device >= 0 && device < 64) attr_set[device] = true;
+  }
+  const SharedRest& r = a.rest;
+  paged_shared_kernel<QDT, FMT, SDT><<<dim3((unsigned)a.pieces), dim3(kThreads), kLds, st>>>(
+      a.requests, a.groups, a.lens, a.prefix_lens, a.batch, a.n_prefixes, a.n_tables, a.n_kv, a.rep, r);
+  MSPR_CHECK_LAUNCH("sdpa_decode_paged_shared");
+  const int heads = a.batch * a.n_kv * a.rep;
+  auto merge = [&](auto waves) {
+    constexpr int kWavesAHead = decltype(waves)::value, kHeads = kMergeWaves / kWavesAHead;
+    paged_shared_merge_kernel<QDT, kWavesAHead><<<dim3((unsigned)((heads + kHeads - 1) / kHeads)), dim3(64 * kMergeWaves), 0, st>>>(
+        r.parts, r.ws_pre, r.ws_pre_ml, r.ws_own, r.ws_own_ml, a.rep, a.n_kv, heads, r.prefix_slots, r.own_slots, r.out);
+  };
+  // (a head has as many pieces as compute units divided by blocks: few where heads are many)
+  if (heads <= 1024) merge(std::integral_constant<int, 8>{});
+  else merge(std::integral_constant<int, 1>{});
+  MSPR_CHECK_LAUNCH("sdpa_decode_paged_shared (merge)");
+  return MSPR_OK;
+}
+
+int shared_fill(const char* what, SharedArgs& a, const void* q, const void* k, const void* v, const int32_t* prefix_tables,
+                const int32_t* prefix_lens, const int32_t* groups, const int32_t* tables, const int32_t* lens,
+                const int32_t* requests, int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_pages, int page_size,
+                int n_prefixes, int prefix_width, int n_tables, int table_width, float scale, void* out, void* workspace,
+                size_t workspace_bytes) {
+  MSPR_REQUIRE(q && k && v && prefix_tables && prefix_lens && groups && tables && lens && out, "%s: null pointer", what);
+  MSPR_REQUIRE(head_dim == kD, "%s: head_dim must be 256", what);
+  MSPR_REQUIRE(batch >= 1 && batch <= kMaxRows, "%s: 1 to %d queries", what, kMaxRows);
+  MSPR_REQUIRE(n_prefixes >= 1 && n_prefixes <= kMaxRows, "%s: 1 to %d prefixes", what, kMaxRows);
+  MSPR_REQUIRE(n_tables >= 1 && (requests || n_tables == batch), "%s: a table for every query, or the requests they belong to",
+               what);
+  MSPR_REQUIRE(n_kv_heads >= 1 && n_kv_heads <= 1024 && n_q_heads >= n_kv_heads && n_q_heads % n_kv_heads == 0,
+               "%s: bad head counts", what);
+  MSPR_REQUIRE(n_q_heads / n_kv_heads <= 16, "%s: at most 16 query heads per KV head", what);
+  MSPR_REQUIRE(page_size >= 16 && (page_size & (page_size - 1)) == 0, "%s: page_size must be a power of two from 16 on", what);
+  MSPR_REQUIRE(n_pages >= 1 && (int64_t)n_pages * page_size <= 0x7FFFFFFF, "%s: the pool must hold fewer than 2^31 tokens", what);
+  MSPR_REQUIRE(table_width >= 1 && (int64_t)table_width * page_size <= 0x40000000 && prefix_width >= 1 &&
+                   (int64_t)prefix_width * page_size <= 0x40000000,
+               "%s: a table must hold 1 page or more and at most 2^30 tokens", what);
+  const int rep = n_q_heads / n_kv_heads;
+  const int64_t most = (int64_t)table_width * page_size > (int64_t)prefix_width * page_size ? (int64_t)table_width * page_size
+                                                                                           : (int64_t)prefix_width * page_size;
+  MSPR_REQUIRE(shared_units(batch, n_prefixes, n_kv_heads, rep) * ((most + kTileKeys - 1) / kTileKeys + 1) <= 0x3FFFFFFF,
+               "%s: the tables hold too many tokens together", what);
+  MSPR_REQUIRE(mspr_aligned(q, 16) && mspr_aligned(k, 16) && mspr_aligned(v, 16) && mspr_aligned(out, 16),
+               "%s: pointers must be 16-byte aligned", what);
+  const SharedScratch s = shared_scratch(batch, n_prefixes, n_kv_heads, rep);
+  MSPR_REQUIRE(workspace && workspace_bytes >= s.total() && mspr_aligned(workspace, 16),
+               "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", what, s.total(), workspace_bytes);
+  a = SharedArgs{};
+  a.requests = requests;
+  a.groups = groups;
+  a.lens = lens;
+  a.prefix_lens = prefix_lens;
+  a.batch = batch;
+  a.n_prefixes = n_prefixes;
+  a.n_tables = n_tables;
+  a.n_kv = n_kv_heads;
+  a.rep = rep;
+  a.pieces = (int)shared_pieces(batch, n_prefixes, n_kv_heads, rep);
+  SharedRest& r = a.rest;
+  r.q = q;
+  r.k = k;
+  r.v = v;
+  r.prefix_tables = prefix_tables;
+  r.tables = tables;
+  r.n_pages = n_pages;
+  r.page_shift = __builtin_ctz(page_size);
+  r.prefix_width = prefix_width;
+  r.width = table_width;
+  r.prefix_slots = (int)s.prefix_slots;
+  r.own_slots = (int)s.own_slots;
+  r.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  uint8_t* at = reinterpret_cast<uint8_t*>(workspace);
+  r.ws_pre = reinterpret_cast<float*>(at);
+  r.ws_pre_ml = reinterpret_cast<float*>(at += s.pre);
+  r.ws_own = reinterpret_cast<float*>(at += s.pre_ml);
+  r.ws_own_ml = reinterpret_cast<float*>(at += s.own);
+  r.parts = reinterpret_cast<int32_t*>(at + s.own_ml);
+  r.out = out;
+  return MSPR_OK;
+}
+
+template <int QDT>
+int shared_q8_launch(const SharedArgs& a, int sb_dtype, hipStream_t st) {
+  if (sb_dtype == MSPR_F32) return shared_launch<QDT, kAffine, MSPR_F32>(a, st);
+  if (sb_dtype == MSPR_F16) return shared_launch<QDT, kAffine, MSPR_F16>(a, st);
+  return shared_launch<QDT, kAffine, MSPR_BF16>(a, st);
+}
+
+}  // namespace
+
+extern "C" size_t mspr_sdpa_decode_paged_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int n_prefixes) {
+  if (batch < 1 || n_kv_heads < 1 || n_q_heads < n_kv_heads || n_q_heads / n_kv_heads > 16 || n_prefixes < 1) return 0;
+  return shared_scratch(batch, n_prefixes, n_kv_heads, n_q_heads / n_kv_heads).total();
+}
+
+extern "C" int mspr_sdpa_decode_paged_shared(const void* queries, const void* k_pages, const void* v_pages, int dtype,
+                                             const int32_t* prefix_tables, const int32_t* prefix_lens, const int32_t* groups,
+                                             const int32_t* tables, const int32_t* lens, const int32_t* requests, int batch,
+                                             int n_q_heads, int n_kv_heads, int head_dim, int n_pages, int page_size,
+                                             int n_prefixes, int prefix_width, int n_tables, int table_width, float scale,
+                                             void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  MSPR_REQUIRE(dtype == MSPR_F16 || dtype == MSPR_BF16, "sdpa_decode_paged_shared: dtype must be f16 or bf16");
+  SharedArgs a;
+  if (int rc = shared_fill("sdpa_decode_paged_shared", a, queries, k_pages, v_pages, prefix_tables, prefix_lens, groups, tables,
+                           lens, requests, batch, n_q_heads, n_kv_heads, head_dim, n_pages, page_size, n_prefixes, prefix_width,
+                           n_tables, table_width, scale, out, workspace, workspace_bytes))
+    return rc;
+  if (dtype == MSPR_F16) return shared_launch<MSPR_F16, MSPR_F16, MSPR_F16>(a, (hipStream_t)stream);
+  return shared_launch<MSPR_BF16, MSPR_BF16, MSPR_BF16>(a, (hipStream_t)stream);
+}
+
+extern "C" int mspr_sdpa_decode_paged_shared_q8(const void* queries, int q_dtype, const void* k_wq, const void* k_scales,
+                                                const void* k_biases, const void* v_wq, const void* v_scales,
+                                                const void* v_biases, int sb_dtype, const int32_t* prefix_tables,
+                                                const int32_t* prefix_lens, const int32_t* groups, const int32_t* tables,
+                                                const int32_t* lens, const int32_t* requests, int batch, int n_q_heads,
+                                                int n_kv_heads, int head_dim, int n_pages, int page_size, int n_prefixes,
+                                                int prefix_width, int n_tables, int table_width, float scale, int group_size,
+                                                int bits, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  MSPR_REQUIRE(group_size == 64 && bits == 8, "sdpa_decode_paged_shared_q8: only group_size=64, bits=8 is supported");
+  MSPR_REQUIRE(q_dtype >= MSPR_F32 && q_dtype <= MSPR_BF16, "sdpa_decode_paged_shared_q8: queries must be f32, f16 or bf16");
+  MSPR_REQUIRE(sb_dtype >= MSPR_F32 && sb_dtype <= MSPR_BF16, "sdpa_decode_paged_shared_q8: scales must be f32, f16 or bf16");
+  MSPR_REQUIRE(k_scales && k_biases && v_scales && v_biases, "sdpa_decode_paged_shared_q8: null pointer");
+  MSPR_REQUIRE(mspr_aligned(k_scales, 16) && mspr_aligned(k_biases, 16) && mspr_aligned(v_scales, 16) &&
+                   mspr_aligned(v_biases, 16),
+               "sdpa_decode_paged_shared_q8: pointers must be 16-byte aligned");
+  SharedArgs a;
+  if (int rc = shared_fill("sdpa_decode_paged_shared_q8", a, queries, k_wq, v_wq, prefix_tables, prefix_lens, groups, tables, lens,
+                           requests, batch, n_q_heads, n_kv_heads, head_dim, n_pages, page_size, n_prefixes, prefix_width,
+                           n_tables, table_width, scale, out, workspace, workspace_bytes))
+    return rc;
+  a.rest.k_scales = k_scales;
+  a.rest.k_biases = k_biases;
+  a.rest.v_scales = v_scales;
+  a.rest.v_biases = v_biases;
+  hipStream_t st = (hipStream_t)stream;
+  if (q_dtype == MSPR_F32) return shared_q8_launch<MSPR_F32>(a, sb_dtype, st);
+  if (q_dtype == MSPR_F16) return shared_q8_launch<MSPR_F16>(a, sb_dtype, st);
+  return shared_q8_launch<MSPR_BF16>(a, sb_dtype, st);
+}

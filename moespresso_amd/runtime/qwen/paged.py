@@ -27,6 +27,7 @@ from moespresso_amd import _lib
 _HEAD_DIM = 256
 _GROUP = 64
 MAX_REQUESTS = 2048  # requests of one page_step
+MAX_SHARED = 2048    # queries, and prefixes, of one call over shared prefixes
 
 
 def _check_page_size(page_size: int):
@@ -367,6 +368,96 @@ def sdpa_decode_paged_q8(queries, k_wq, k_scales, k_biases, v_wq, v_scales, v_bi
         _lib.DTYPE_CODE[k_scales.dtype], _lib.ptr(tables), _lib.ptr(lens), _lib.ptr(requests), R, Hq, heads, _HEAD_DIM,
         n_pages, page_size, int(tables.shape[0]), int(tables.shape[1]), float(scale), 64, 8, _lib.ptr(out),
         _lib.ptr(workspace), workspace.numel() * workspace.element_size()), "sdpa_decode_paged_q8")
+    return out
+
+
+def _check_prefixes(prefix_tables, prefix_lens, groups, tables):
+    """Number of prefixes and the width of their tables."""
+    if prefix_tables.ndim != 2 or int(prefix_tables.shape[0]) < 1 or int(prefix_tables.shape[1]) < 1:
+        raise ValueError("prefix_tables must be [G, P]")
+    n = int(prefix_tables.shape[0])
+    if n > MAX_SHARED:
+        raise ValueError(f"at most {MAX_SHARED} prefixes a call")
+    _check_ints("prefix_tables", prefix_tables, prefix_tables.shape)
+    _check_ints("prefix_lens", prefix_lens, (n,))
+    _check_ints("groups", groups, (int(tables.shape[0]),))
+    return n, int(prefix_tables.shape[1])
+
+
+def sdpa_decode_paged_shared(queries, keys, values, prefix_tables, prefix_lens, groups, tables, lens, scale, *, requests=None,
+                             workspace=None):
+    """``sdpa_decode_paged`` for requests that continue a prefix which others continue too: its rows are read once for a group.
+
+    A query attends the rows of its request's prefix and then those of the request's own table. Positions are the caller's:
+    the first row behind a prefix is at the prefix's length.
+
+    Args:
+        queries: ``[R, Hq, 256]`` float16 or bfloat16, already rotated, at most 2048 of them.
+        keys, values, tables, lens, scale, requests: as for ``sdpa_decode_paged``; ``tables`` and ``lens`` are those of the
+            requests' own rows (a query that sees none of them still sees the prefix).
+        prefix_tables: int32 ``[G, P]``, the pages of every prefix, in the same pool; at most 2048 prefixes.
+        prefix_lens: int32 ``[G]``, the rows of every prefix; the last page may be part-filled.
+        groups: int32 ``[B]``, the prefix that a request continues (none of ``G``: none). A query of no request sees nothing.
+
+    Returns:
+        ``[R, Hq, 256]`` in the dtype of ``queries``.
+    """
+    if not torch.is_tensor(keys) or not torch.is_tensor(values):
+        raise ValueError("keys and values must be 16-bit pages (8-bit ones: sdpa_decode_paged_shared_q8)")
+    n_pages, heads, page_size = _check_pages(keys, values)
+    if queries.dtype != keys.dtype:
+        raise ValueError("pages must have the dtype of queries")
+    R, Hq = _check_decode(queries, heads, tables, lens, requests)
+    G, width = _check_prefixes(prefix_tables, prefix_lens, groups, tables)
+    if R > MAX_SHARED:
+        raise ValueError(f"at most {MAX_SHARED} queries a call")
+    dev = _lib.require_device(queries, keys, values, prefix_tables, prefix_lens, groups, tables, lens, requests)
+    out = torch.empty(tuple(queries.shape), dtype=queries.dtype, device=dev)
+    if R == 0:
+        return out
+    q = _aligned(queries.contiguous())
+    if workspace is None:
+        workspace = _lib.paged_shared_workspace(R, Hq, heads, G, dev)
+    _lib.check(_lib.launch(
+        dev, "mspr_sdpa_decode_paged_shared", _lib.ptr(q), _lib.ptr(keys), _lib.ptr(values), _lib.DTYPE_CODE[q.dtype],
+        _lib.ptr(prefix_tables), _lib.ptr(prefix_lens), _lib.ptr(groups), _lib.ptr(tables), _lib.ptr(lens), _lib.ptr(requests), R,
+        Hq, heads, _HEAD_DIM, n_pages, page_size, G, width, int(tables.shape[0]), int(tables.shape[1]), float(scale),
+        _lib.ptr(out), _lib.ptr(workspace), workspace.numel() * workspace.element_size()), "sdpa_decode_paged_shared")
+    return out
+
+
+def sdpa_decode_paged_shared_q8(queries, k_wq, k_scales, k_biases, v_wq, v_scales, v_biases, prefix_tables, prefix_lens, groups,
+                                tables, lens, scale, *, group_size: int = 64, bits: int = 8, requests=None, workspace=None):
+    """``sdpa_decode_paged_shared`` over pages of affine 8-bit rows.
+
+    Args:
+        queries: ``[R, Hq, 256]`` float32, float16 or bfloat16.
+        k_wq, k_scales, k_biases, v_wq, v_scales, v_biases: as for ``sdpa_decode_paged_q8``.
+        prefix_tables, prefix_lens, groups, tables, lens, scale, requests: as for ``sdpa_decode_paged_shared``.
+    """
+    if group_size != 64 or bits != 8:
+        raise ValueError("sdpa_decode_paged_shared_q8 supports group_size=64, bits=8 only")
+    n_pages, heads, page_size = _check_pages((k_wq, k_scales, k_biases), (v_wq, v_scales, v_biases))
+    if queries.dtype not in _lib.DTYPE_CODE:
+        raise ValueError("queries must be float32, float16 or bfloat16")
+    R, Hq = _check_decode(queries, heads, tables, lens, requests)
+    G, width = _check_prefixes(prefix_tables, prefix_lens, groups, tables)
+    if R > MAX_SHARED:
+        raise ValueError(f"at most {MAX_SHARED} queries a call")
+    parts = (k_wq, k_scales, k_biases, v_wq, v_scales, v_biases)
+    dev = _lib.require_device(queries, *parts, prefix_tables, prefix_lens, groups, tables, lens, requests)
+    out = torch.empty(tuple(queries.shape), dtype=queries.dtype, device=dev)
+    if R == 0:
+        return out
+    q = _aligned(queries.contiguous())
+    if workspace is None:
+        workspace = _lib.paged_shared_workspace(R, Hq, heads, G, dev)
+    _lib.check(_lib.launch(
+        dev, "mspr_sdpa_decode_paged_shared_q8", _lib.ptr(q), _lib.DTYPE_CODE[q.dtype], *(_lib.ptr(t) for t in parts),
+        _lib.DTYPE_CODE[k_scales.dtype], _lib.ptr(prefix_tables), _lib.ptr(prefix_lens), _lib.ptr(groups), _lib.ptr(tables),
+        _lib.ptr(lens), _lib.ptr(requests), R, Hq, heads, _HEAD_DIM, n_pages, page_size, G, width, int(tables.shape[0]),
+        int(tables.shape[1]), float(scale), 64, 8, _lib.ptr(out), _lib.ptr(workspace),
+        workspace.numel() * workspace.element_size()), "sdpa_decode_paged_shared_q8")
     return out
 
 
