@@ -436,6 +436,51 @@ int mspr_sdpa_decode_paged_shared_q8(const void* queries, int q_dtype, const voi
                                      int table_width, float scale, int group_size, int bits, void* out, void* workspace,
                                      size_t workspace_bytes, void* stream);
 
+/* Bounds of the keys of every page that a step wrote to, per page and KV head over the rows that the page holds so far:
+ * with e the smallest exponent (within +-50) for which max |k| <= 127 * 2^e, codes: int8 [n_pages][n_kv_heads][2][256], the lower
+ * bounds floor(min k * 2^-e), then the upper ones ceil(max k * 2^-e); scales: f32 [n_pages][n_kv_heads], 2^e. Updated in place from
+ * the old ones and the new rows (the new rows alone where they begin the page), which gives what all rows would.
+ * slots: int32 [n_rows], those of the step's append (negative or not in the pool: no row); rows of one page one behind the other,
+ * as mspr_page_step gives them. A second call on the same slots changes nothing. k_pages: 16-bit rows of dtype (f16|bf16). */
+int mspr_page_bounds(const int32_t* slots, const void* k_pages, int dtype, int n_rows, int n_kv_heads, int head_dim, int n_pages,
+                     int page_size, int8_t* codes, float* scales, void* stream);
+/* The same of affine 8-bit rows (of code * scale + bias, unrounded). */
+int mspr_page_bounds_q8(const int32_t* slots, const void* k_wq, const void* k_scales, const void* k_biases, int sb_dtype,
+                        int n_rows, int n_kv_heads, int head_dim, int n_pages, int page_size, int8_t* codes, float* scales,
+                        void* stream);
+
+/* The pages that a query may weigh most, per KV head, from such bounds. Of the pages p of query b's request (ceil(lens[b] /
+ * page_size) of them) that are more than `selected`: the first `first`, the last `recent` (1 or more) and, of the others, those of
+ * greatest max_h (bound[h][p] - max_p' bound[h][p']), ties to the lower page; h are the query heads of the KV head, bound[h][p] the
+ * largest product of the head's query, in codes of 8 bits as the bounds', with a key within the bounds of page p (exact). Pages that
+ * are not in the pool come last. out_tables: int32 [batch][n_kv_heads][selected], ascending in position, as pages of a pool of one
+ * head a page (page * n_kv_heads + head; -1 of one that is not in the pool, and behind the last); out_lens: int32
+ * [batch][n_kv_heads], the rows in them (lens[b] where all pages are taken).
+ * queries: [batch][n_q_heads][256] of q_dtype (f32|f16|bf16); batch * n_kv_heads <= 65535, table_width <= 32768, selected <= 4096;
+ * tables, lens and requests as for mspr_sdpa_decode_paged. */
+size_t mspr_select_pages_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int table_width);
+int mspr_select_pages(const void* queries, int q_dtype, const int8_t* codes, const float* scales, const int32_t* tables,
+                      const int32_t* lens, const int32_t* requests, int batch, int n_q_heads, int n_kv_heads, int head_dim,
+                      int n_pages, int page_size, int n_tables, int table_width, int selected, int first, int recent,
+                      int32_t* out_tables, int32_t* out_lens, void* workspace, size_t workspace_bytes, void* stream);
+
+/* mspr_sdpa_decode_paged over the pages that mspr_select_pages selects, per KV head. scale must not be negative. */
+size_t mspr_sdpa_decode_paged_sparse_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int page_size, int table_width,
+                                                     int selected);
+int mspr_sdpa_decode_paged_sparse(const void* queries, const void* k_pages, const void* v_pages, int dtype, const int8_t* codes,
+                                  const float* scales, const int32_t* tables, const int32_t* lens, const int32_t* requests,
+                                  int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_pages, int page_size, int n_tables,
+                                  int table_width, int selected, int first, int recent, float scale, void* out, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+/* The same over pages of affine 8-bit rows (scales and biases of sb_dtype); queries and out of q_dtype (f32|f16|bf16). */
+int mspr_sdpa_decode_paged_sparse_q8(const void* queries, int q_dtype, const void* k_wq, const void* k_scales,
+                                     const void* k_biases, const void* v_wq, const void* v_scales, const void* v_biases,
+                                     int sb_dtype, const int8_t* codes, const float* scales, const int32_t* tables,
+                                     const int32_t* lens, const int32_t* requests, int batch, int n_q_heads, int n_kv_heads,
+                                     int head_dim, int n_pages, int page_size, int n_tables, int table_width, int selected,
+                                     int first, int recent, float scale, int group_size, int bits, void* out, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ measurement */
 
 /* Per-kernel GPU timing for benchmarks. Bit k of kernel_mask brackets every later launch of kernel

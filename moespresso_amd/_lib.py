@@ -160,6 +160,22 @@ SIGNATURES = {
         c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
                 c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                 c_float, c_int, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mspr_page_bounds": (
+        c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "mspr_page_bounds_q8": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "mspr_select_pages_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "mspr_select_pages": (
+        c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
+                c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mspr_sdpa_decode_paged_sparse_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "mspr_sdpa_decode_paged_sparse": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+                c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mspr_sdpa_decode_paged_sparse_q8": (
+        c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                c_float, c_int, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
     "mspr_profile_enable": (c_int, [c_int]),
     "mspr_profile_collect": (c_int, [c_int, c_void_p, c_int]),
 }
@@ -216,6 +232,20 @@ def paged_decode_workspace(batch: int, n_q_heads: int, n_kv_heads: int, page_siz
 def paged_shared_workspace(batch: int, n_q_heads: int, n_kv_heads: int, n_prefixes: int, device) -> torch.Tensor:
     """Scratch tensor for the decode entry points over shared prefixes (partials of every piece, and which a query has)."""
     nbytes = int(lib().mspr_sdpa_decode_paged_shared_workspace_bytes(int(batch), int(n_q_heads), int(n_kv_heads), int(n_prefixes)))
+    return torch.empty((max(nbytes, 16) + 3) // 4, dtype=torch.float32, device=device)
+
+
+def select_pages_workspace(batch: int, n_q_heads: int, n_kv_heads: int, table_width: int, device) -> torch.Tensor:
+    """Scratch tensor for mspr_select_pages (bounds of every page, query head and query, and maxima of sixteen pages)."""
+    nbytes = int(lib().mspr_select_pages_workspace_bytes(int(batch), int(n_q_heads), int(n_kv_heads), int(table_width)))
+    return torch.empty((max(nbytes, 16) + 3) // 4, dtype=torch.float32, device=device)
+
+
+def paged_sparse_workspace(batch: int, n_q_heads: int, n_kv_heads: int, page_size: int, table_width: int, selected: int,
+                           device) -> torch.Tensor:
+    """Scratch tensor for the decode entry points over selected pages (the selection's, its tables, the decode's)."""
+    nbytes = int(lib().mspr_sdpa_decode_paged_sparse_workspace_bytes(int(batch), int(n_q_heads), int(n_kv_heads), int(page_size),
+                                                                     int(table_width), int(selected)))
     return torch.empty((max(nbytes, 16) + 3) // 4, dtype=torch.float32, device=device)
 
 

@@ -1,0 +1,479 @@
+// The pages that a query may weigh most, per KV head, and attention over them.
+//
+//   bound[h, p] = sum_d max(c[h, d] lo[p, d], c[h, d] hi[p, d]) * 2^(e_h + e_p)       c, e_h: the head's query in 8 bits
+//   worth[p]    = max_h (bound[h, p] - max_p' bound[h, p'])
+//
+// over the pages p of the query's request: how far the largest product that a page may hold with a head lies below that head's
+// best, at its best head (softmax weights fall with the exponential of that distance). The first pages and the last ones are taken
+// whatever they are worth, of the others the best, ties to the lower page.
+//
+// A bound is a product of 512: the negative codes with lo, the positive ones with hi, by 16x16x64 integer matrix instructions.
+// Sums are whole numbers below 2^24 and scales powers of two, so that a bound is exact in float32, and the selection does not
+// depend on the order of anything.
+//
+// Two launches: bounds of 16 pages a wave and step, read at the rate of HBM (516 bytes a page and KV head) with their maxima, and the
+// choice, a workgroup a query and KV head, in LDS. The pages of a KV head are then pages of a pool of its own (page * n_kv + head,
+// one head a page), over which paged_decode.hip attends.
+#include "page_bounds.h"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(4))) int i32x4_t;
+
+constexpr int kTile = 16;          // pages of a matrix instruction
+constexpr int kScoreWaves = 4;
+constexpr int kTilesAWave = 2;
+constexpr int kPagesAGroup = kTile * kScoreWaves * kTilesAWave;
+constexpr int kMaxTablePages = 32768;  // their keys fit into LDS
+constexpr int kMaxSelected = 4096;
+
+struct SelectArgs {
+  const void* q;            // [R, n_kv * rep, 256]
+  const int32_t* requests;  // [R] or null
+  const int32_t* lens;      // [R]
+  const int32_t* tables;    // [n_tables, width]
+  const int8_t* codes;      // [n_pages, n_kv, 2, 256]
+  const float* scales;      // [n_pages, n_kv]
+  int rows, n_kv, rep, width, n_tables, n_pages, page_shift, selected, first, recent;
+  float* bounds;            // [R * n_kv][rep][padded]
+  float* most;              // [R * n_kv][padded / 16][rep], maxima of 16 pages
+  int padded;               // width, up to a multiple of 16
+  int32_t* out;             // [R * n_kv][selected]
+  int32_t* out_lens;        // [R * n_kv]
+};
+
+// Rows that query r sees, and its request's table (none: no rows).
+struct Seen {
+  int len, request;
+};
+__device__ __forceinline__ Seen seen_by(const SelectArgs& a, int r) {
+  const int request = a.requests ? a.requests[r] : r;
+  const int cap = a.width << a.page_shift;
+  const int len = a.lens[r];
+  const bool known = request >= 0 && request < a.n_tables;
+  return Seen{!known || len < 0 ? 0 : len > cap ? cap : len, known ? request : 0};
+}
+
+// grid: (groups of pages, queries x KV heads)
+template <int QDT>
+__global__ __launch_bounds__(64 * kScoreWaves) void page_score_kernel(SelectArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = blockIdx.y, r = row / a.n_kv, kvh = row - r * a.n_kv;
+  const Seen seen = seen_by(a, r);
+  const int n = (seen.len + (1 << a.page_shift) - 1) >> a.page_shift;
+  if (n <= a.selected) return;  // (all of them are taken)
+  const int tile0 = ((int)blockIdx.x * kScoreWaves + wave) * kTilesAWave;
+  if (tile0 * kTile >= n) return;
+  const int head = lane & 15, g = lane >> 4;
+  // ---- page numbers, then the bounds of two tiles; the query in the meantime
+  const int32_t* table = a.tables + (int64_t)seen.request * a.width;
+  int page[kTilesAWave];
+  bool good[kTilesAWave];
+#pragma unroll
+  for (int i = 0; i < kTilesAWave; i++) {
+    const int p = (tile0 + i) * kTile + head;
+    page[i] = p < n ? table[p] : -1;
+  }
+  const bool mine = head < a.rep;
+  float x[64];  // channels 64 s + 16 g + j
+  {
+    const int64_t q0 = ((int64_t)row * a.rep + (mine ? head : 0)) * 256;
+    constexpr int kBytes = QDT == MSPR_F32 ? 4 : 2;
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+      const u32x4_t* from = reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint8_t*>(a.q) + (q0 + 64 * s + 16 * g) * kBytes);
+      u32x4_t w[kBytes];
+#pragma unroll
+      for (int j = 0; j < kBytes; j++) w[j] = from[j];
+#pragma unroll
+      for (int j = 0; j < 16; j++) {
+        if constexpr (QDT == MSPR_F32) x[16 * s + j] = __uint_as_float(w[j / 4][j % 4]);
+        else if constexpr (QDT == MSPR_F16) x[16 * s + j] = f16_bits_to_f32((uint16_t)(w[j / 8][j / 2 % 4] >> 16 * (j % 2)));
+        else x[16 * s + j] = bf16_bits_to_f32((uint16_t)(w[j / 8][j / 2 % 4] >> 16 * (j % 2)));
+      }
+    }
+  }
+  i32x4_t tile[kTilesAWave][8];
+  float scale[kTilesAWave];
+#pragma unroll
+  for (int i = 0; i < kTilesAWave; i++) {
+    good[i] = page[i] >= 0 && page[i] < a.n_pages;
+    const int64_t at = (int64_t)(good[i] ? page[i] : 0) * a.n_kv + kvh;
+    const i32x4_t* from = reinterpret_cast<const i32x4_t*>(a.codes + at * kBoundBytes + 16 * g);
+#pragma unroll
+    for (int s = 0; s < 8; s++) tile[i][s] = from[4 * s];
+    scale[i] = a.scales[at];
+  }
+  // ---- the query's codes: operand s < 4 has the negative ones of 64 channels, 4 + s the positive ones
+  float top = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 64; j++) top = fmaxf(top, mine ? fabsf(x[j]) : 0.0f);
+  top = half_wave_max(row_pair_max(top));
+  const int e = bound_exponent(top);
+  i32x4_t neg[4], pos[4];
+#pragma unroll
+  for (int s = 0; s < 4; s++)
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      uint32_t m = 0, p = 0;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int c = mine ? bound_code(rintf(__builtin_amdgcn_ldexpf(x[16 * s + 4 * w + j], -e))) : 0;
+        m |= (uint32_t)((c < 0 ? c : 0) & 0xFF) << 8 * j;
+        p |= (uint32_t)(c > 0 ? c : 0) << 8 * j;
+      }
+      neg[s][w] = (int)m;
+      pos[s][w] = (int)p;
+    }
+  const float unit = __builtin_amdgcn_ldexpf(1.0f, e);
+#pragma unroll
+  for (int i = 0; i < kTilesAWave; i++) {
+    const int p0 = (tile0 + i) * kTile;
+    if (p0 >= n) break;
+    i32x4_t acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(tile[i][s], neg[s], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(tile[i][4 + s], pos[s], acc, 0, 0, 0);
+    }
+    // page 4 g + j of the tile, head `head`
+    f32x4_t b;
+    float best = -__builtin_inff();
+    const float of_page = good[i] ? scale[i] : 0.0f;  // (bounds of a page that is not in the pool: none)
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float s = __shfl(of_page, 4 * g + j, MSPR_WAVE);
+      const bool there = __shfl((int)good[i], 4 * g + j, MSPR_WAVE) != 0;
+      b[j] = there ? (float)acc[j] * unit * s : -__builtin_inff();
+      best = fmaxf(best, b[j]);
+    }
+    best = half_wave_max(row_pair_max(best));
+    if (mine) {
+      *reinterpret_cast<f32x4_t*>(a.bounds + ((int64_t)row * a.rep + head) * a.padded + p0 + 4 * g) = b;
+      if (g == 0) a.most[((int64_t)row * (a.padded / kTile) + tile0 + i) * a.rep + head] = best;
+    }
+  }
+}
+
+constexpr int kChooseThreads = 1024;
+constexpr int kChooseWaves = kChooseThreads / 64;
+constexpr int kBins = 2048;
+
+__device__ __forceinline__ int scan_up(int v) {  // sums over this lane and those before it
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const int o = __shfl_up(v, m, MSPR_WAVE);
+    if ((int)(threadIdx.x & 63) >= m) v += o;
+  }
+  return v;
+}
+
+// One workgroup a query and KV head. LDS: keys of all pages.
+__global__ __launch_bounds__(kChooseThreads) void page_choose_kernel(SelectArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  uint32_t* keys = reinterpret_cast<uint32_t*>(lds);  // [width]
+  __shared__ int bins[kBins];
+  __shared__ float tops[16];
+  __shared__ int sums[kChooseWaves];
+  __shared__ int found[2];
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int row = blockIdx.x, r = row / a.n_kv, kvh = row - r * a.n_kv;
+  const Seen seen = seen_by(a, r);
+  const int page_size = 1 << a.page_shift;
+  const int n = (seen.len + page_size - 1) >> a.page_shift;
+  const int32_t* table = a.tables + (int64_t)seen.request * a.width;
+  int32_t* out = a.out + (int64_t)row * a.selected;
+  auto id_of = [&](int p) {
+    const int page = table[p];
+    return page >= 0 && page < a.n_pages ? page * a.n_kv + kvh : -1;
+  };
+  if (t == 0) a.out_lens[row] = n > a.selected ? seen.len - ((n - a.selected) << a.page_shift) : seen.len;
+  if (n <= a.selected) {
+    for (int i = t; i < a.selected; i += kChooseThreads) out[i] = i < n ? id_of(i) : -1;
+    return;
+  }
+  // ---- every head's best bound
+  for (int h = wave; h < a.rep; h += kChooseWaves) {
+    float best = -__builtin_inff();
+    const float* most = a.most + (int64_t)row * (a.padded / kTile) * a.rep + h;
+    for (int i = lane; i * kTile < n; i += 64) best = fmaxf(best, most[(int64_t)i * a.rep]);
+    for (int m = 32; m > 0; m >>= 1) best = fmaxf(best, __shfl_xor(best, m, MSPR_WAVE));
+    if (lane == 0) tops[h] = best == -__builtin_inff() ? 0.0f : best;
+  }
+  __syncthreads();
+  // ---- keys in the order of worth: 32 bits that grow with it
+  for (int p = t; p < n; p += kChooseThreads) {
+    float worth = -__builtin_inff();
+    for (int h = 0; h < a.rep; h++) worth = fmaxf(worth, a.bounds[((int64_t)row * a.rep + h) * a.padded + p] - tops[h]);
+    keys[p] = p < a.first || p >= n - a.recent ? 0xFFFFFFFFu : score_key(worth);
+  }
+  // ---- the key of rank `selected`, eleven, eleven and ten bits at a time
+  uint32_t prefix = 0, known = 0;
+  int want = a.selected;  // rank of the key among those with this prefix
+#pragma unroll 1
+  for (int pass = 0; pass < 3; pass++) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t mask = pass == 2 ? 1023u : 2047u;
+    for (int i = t; i < kBins; i += kChooseThreads) bins[i] = 0;
+    __syncthreads();
+    for (int p = t; p < n; p += kChooseThreads)
+      if ((keys[p] & known) == prefix) atomicAdd(&bins[keys[p] >> shift & mask], 1);
+    __syncthreads();
+    // from the highest bin down: thread t has bins 2047 - 2 t and the one below
+    const int b0 = bins[kBins - 1 - 2 * t], b1 = bins[kBins - 2 - 2 * t];
+    const int upto = scan_up(b0 + b1);
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    int before = upto - b0 - b1;
+    for (int w = 0; w < wave; w++) before += sums[w];
+    if (before < want && want <= before + b0 + b1) {
+      const bool second = want > before + b0;
+      found[0] = kBins - 1 - 2 * t - (second ? 1 : 0);
+      found[1] = want - before - (second ? b0 : 0);
+    }
+    __syncthreads();
+    prefix |= (uint32_t)found[0] << shift;
+    known |= mask << shift;
+    want = found[1];
+  }
+  // ---- pages above that key, and the first `want` with it, in order: a stretch of pages a thread
+  const int per = (n + kChooseThreads - 1) / kChooseThreads;
+  const int p0 = min(t * per, n), p1 = min(p0 + per, n);
+  int above = 0, ties = 0;
+  for (int p = p0; p < p1; p++) {
+    above += keys[p] > prefix;
+    ties += keys[p] == prefix;
+  }
+  const int upto = scan_up(above), ties_upto = scan_up(ties);
+  __syncthreads();
+  if (lane == 63) {
+    sums[wave] = upto;
+    bins[wave] = ties_upto;
+  }
+  __syncthreads();
+  int at = upto - above, tied = ties_upto - ties;
+  for (int w = 0; w < wave; w++) {
+    at += sums[w];
+    tied += bins[w];
+  }
+  for (int p = p0; p < p1; p++) {
+    const bool tie = keys[p] == prefix;
+    if (keys[p] > prefix || (tie && tied < want)) {
+      const int i = at + min(tied, want);
+      if (i < a.selected) out[i] = id_of(p);
+    }
+    at += keys[p] > prefix;
+    tied += tie;
+  }
+}
+
+struct SelectScratch {
+  int padded;
+  size_t bounds, most;  // bytes
+  size_t total() const { return bounds + most; }
+};
+SelectScratch select_scratch(int64_t rows, int rep, int width) {
+  SelectScratch s;
+  s.padded = (width + kTile - 1) / kTile * kTile;
+  s.bounds = (size_t)rows * rep * s.padded * sizeof(float);
+  s.most = ((size_t)rows * rep * (s.padded / kTile) * sizeof(float) + 15) / 16 * 16;
+  return s;
+}
+
+int select_fill(const char* what, SelectArgs& a, const void* q, int q_dtype, const int8_t* codes, const float* scales,
+                const int32_t* tables, const int32_t* lens, const int32_t* requests, int rows, int n_q_heads, int n_kv_heads,
+                int head_dim, int n_pages, int page_size, int n_tables, int table_width, int selected, int first, int recent,
+                void* workspace, size_t workspace_bytes) {
+  MSPR_REQUIRE(q && codes && scales && tables && lens, "%s: null pointer", what);
+  MSPR_REQUIRE(q_dtype >= MSPR_F32 && q_dtype <= MSPR_BF16, "%s: queries must be f32, f16 or bf16", what);
+  MSPR_REQUIRE(head_dim == 256, "%s: head_dim must be 256", what);
+  MSPR_REQUIRE(n_kv_heads >= 1 && n_kv_heads <= 1024 && n_q_heads >= n_kv_heads && n_q_heads % n_kv_heads == 0,
+               "%s: bad head counts", what);
+  MSPR_REQUIRE(n_q_heads / n_kv_heads <= 16, "%s: at most 16 query heads per KV head", what);
+  MSPR_REQUIRE(rows >= 1 && (int64_t)rows * n_kv_heads <= 65535, "%s: 1 to 65535 queries times KV heads", what);
+  MSPR_REQUIRE(n_tables >= 1 && (requests || n_tables == rows), "%s: a table for every query, or the requests they belong to", what);
+  MSPR_REQUIRE(page_size >= 16 && (page_size & (page_size - 1)) == 0, "%s: page_size must be a power of two from 16 on", what);
+  MSPR_REQUIRE(n_pages >= 1 && (int64_t)n_pages * n_kv_heads * page_size <= 0x7FFFFFFF,
+               "%s: the pool must hold fewer than 2^31 tokens times KV heads", what);
+  MSPR_REQUIRE(table_width >= 1 && table_width <= kMaxTablePages && (int64_t)table_width * page_size <= 0x40000000,
+               "%s: a request's table must hold 1 to %d pages and at most 2^30 tokens", what, kMaxTablePages);
+  MSPR_REQUIRE(first >= 0 && recent >= 1 && selected >= 1 && selected <= kMaxSelected && (int64_t)first + recent <= selected,
+               "%s: first >= 0, recent >= 1, and both together within 1 to %d selected pages", what, kMaxSelected);
+  MSPR_REQUIRE(mspr_aligned(q, 16) && mspr_aligned(codes, 16) && mspr_aligned(scales, 4), "%s: pointers must be 16-byte aligned", what);
+  const int rep = n_q_heads / n_kv_heads;
+  const SelectScratch s = select_scratch((int64_t)rows * n_kv_heads, rep, table_width);
+  MSPR_REQUIRE(workspace && workspace_bytes >= s.total() && mspr_aligned(workspace, 16),
+               "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", what, s.total(), workspace_bytes);
+  a = SelectArgs{};
+  a.q = q;
+  a.requests = requests;
+  a.lens = lens;
+  a.tables = tables;
+  a.codes = codes;
+  a.scales = scales;
+  a.rows = rows;
+  a.n_kv = n_kv_heads;
+  a.rep = rep;
+  a.width = table_width;
+  a.n_tables = n_tables;
+  a.n_pages = n_pages;
+  a.page_shift = __builtin_ctz(page_size);
+  a.selected = selected;
+  a.first = first;
+  a.recent = recent;
+  a.padded = s.padded;
+  a.bounds = reinterpret_cast<float*>(workspace);
+  a.most = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + s.bounds);
+  return MSPR_OK;
+}
+
+int select_launch(const char* what, const SelectArgs& a, int q_dtype, hipStream_t st) {
+  const unsigned rows = (unsigned)(a.rows * a.n_kv);
+  static bool attr_set[64] = {};  // by device
+  constexpr int kMostLds = kMaxTablePages * (int)sizeof(uint32_t);
+  int device = 0;
+  if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64 || !attr_set[device]) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&page_choose_kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, kMostLds);
+    if (e != hipSuccess) {
+      mspr_set_error("%s: cannot reserve %d bytes of LDS: %s", what, kMostLds, hipGetErrorString(e));
+      return MSPR_ERR_LAUNCH;
+    }
+    if (device >= 0 && device < 64) attr_set[device] = true;
+  }
+  if (a.width > a.selected) {
+    const dim3 grid((unsigned)((a.width + kPagesAGroup - 1) / kPagesAGroup), rows);
+    if (q_dtype == MSPR_F32) page_score_kernel<MSPR_F32><<<grid, dim3(64 * kScoreWaves), 0, st>>>(a);
+    else if (q_dtype == MSPR_F16) page_score_kernel<MSPR_F16><<<grid, dim3(64 * kScoreWaves), 0, st>>>(a);
+    else page_score_kernel<MSPR_BF16><<<grid, dim3(64 * kScoreWaves), 0, st>>>(a);
+    MSPR_CHECK_LAUNCH(what);
+  }
+  page_choose_kernel<<<dim3(rows), dim3(kChooseThreads), (size_t)a.width * sizeof(uint32_t), st>>>(a);
+  MSPR_CHECK_LAUNCH(what);
+  return MSPR_OK;
+}
+
+// Scratch of a sparse call: the selection's, then its tables and lengths, then the decode's.
+struct SparseScratch {
+  size_t select, tables, lens, decode;
+  size_t total() const { return select + tables + lens + decode; }
+};
+SparseScratch sparse_scratch(int rows, int n_q_heads, int n_kv_heads, int page_size, int table_width, int selected) {
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  SparseScratch s;
+  s.select = up(select_scratch((int64_t)rows * n_kv_heads, n_q_heads / n_kv_heads, table_width).total());
+  s.tables = up((size_t)rows * n_kv_heads * selected * sizeof(int32_t));
+  s.lens = up((size_t)rows * n_kv_heads * sizeof(int32_t));
+  s.decode = mspr_sdpa_decode_paged_workspace_bytes(rows * n_kv_heads, n_q_heads / n_kv_heads, 1, page_size, selected);
+  return s;
+}
+
+bool sparse_sizes_ok(int rows, int n_q_heads, int n_kv_heads, int page_size, int table_width, int selected) {
+  return rows >= 1 && n_kv_heads >= 1 && n_q_heads >= n_kv_heads && page_size >= 1 && table_width >= 1 && selected >= 1 &&
+         (int64_t)rows * n_kv_heads <= 65535 && n_q_heads / n_kv_heads <= 16 && table_width <= kMaxTablePages &&
+         selected <= kMaxSelected;
+}
+
+// The selection of a sparse call into its workspace; then the decode's operands.
+struct Sparse {
+  int32_t *tables, *lens;
+  void* workspace;
+  size_t bytes;
+};
+int sparse_select(const char* what, const void* q, int q_dtype, const int8_t* codes, const float* scales, const int32_t* tables,
+                  const int32_t* lens, const int32_t* requests, int rows, int n_q_heads, int n_kv_heads, int head_dim, int n_pages,
+                  int page_size, int n_tables, int table_width, int selected, int first, int recent, float scale, void* workspace,
+                  size_t workspace_bytes, Sparse* s, hipStream_t st) {
+  MSPR_REQUIRE(selected >= 1 && (int64_t)selected * page_size <= 0x40000000 &&
+                   (int64_t)rows * n_kv_heads * (((int64_t)selected * page_size + 31) / 32 + 1) <= 0x3FFFFFFF,
+               "%s: the selected pages hold too many tokens together", what);
+  // (a negative scale would turn the order of the bounds round)
+  MSPR_REQUIRE(scale >= 0.0f, "%s: the softmax scale must not be negative", what);
+  SelectArgs a;
+  if (int rc = select_fill(what, a, q, q_dtype, codes, scales, tables, lens, requests, rows, n_q_heads, n_kv_heads, head_dim, n_pages,
+                           page_size, n_tables, table_width, selected, first, recent, workspace, workspace_bytes))
+    return rc;
+  const SparseScratch z = sparse_scratch(rows, n_q_heads, n_kv_heads, page_size, table_width, selected);
+  MSPR_REQUIRE(workspace_bytes >= z.total(), "%s: workspace of %zu bytes needed, %zu given", what, z.total(), workspace_bytes);
+  uint8_t* at = reinterpret_cast<uint8_t*>(workspace) + z.select;
+  s->tables = a.out = reinterpret_cast<int32_t*>(at);
+  s->lens = a.out_lens = reinterpret_cast<int32_t*>(at += z.tables);
+  s->workspace = at + z.lens;
+  s->bytes = z.decode;
+  return select_launch(what, a, q_dtype, st);
+}
+
+}  // namespace
+
+extern "C" size_t mspr_select_pages_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int table_width) {
+  if (!sparse_sizes_ok(batch, n_q_heads, n_kv_heads, 16, table_width, 1)) return 0;
+  return select_scratch((int64_t)batch * n_kv_heads, n_q_heads / n_kv_heads, table_width).total();
+}
+
+extern "C" int mspr_select_pages(const void* queries, int q_dtype, const int8_t* codes, const float* scales, const int32_t* tables,
+                                 const int32_t* lens, const int32_t* requests, int batch, int n_q_heads, int n_kv_heads,
+                                 int head_dim, int n_pages, int page_size, int n_tables, int table_width, int selected, int first,
+                                 int recent, int32_t* out_tables, int32_t* out_lens, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+  MSPR_REQUIRE(out_tables && out_lens, "select_pages: null pointer");
+  SelectArgs a;
+  if (int rc = select_fill("select_pages", a, queries, q_dtype, codes, scales, tables, lens, requests, batch, n_q_heads, n_kv_heads,
+                           head_dim, n_pages, page_size, n_tables, table_width, selected, first, recent, workspace, workspace_bytes))
+    return rc;
+  a.out = out_tables;
+  a.out_lens = out_lens;
+  return select_launch("select_pages", a, q_dtype, (hipStream_t)stream);
+}
+
+extern "C" size_t mspr_sdpa_decode_paged_sparse_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int page_size,
+                                                                int table_width, int selected) {
+  if (!sparse_sizes_ok(batch, n_q_heads, n_kv_heads, page_size, table_width, selected)) return 0;
+  return sparse_scratch(batch, n_q_heads, n_kv_heads, page_size, table_width, selected).total();
+}
+
+extern "C" int mspr_sdpa_decode_paged_sparse(const void* queries, const void* k_pages, const void* v_pages, int dtype,
+                                             const int8_t* codes, const float* scales, const int32_t* tables, const int32_t* lens,
+                                             const int32_t* requests, int batch, int n_q_heads, int n_kv_heads, int head_dim,
+                                             int n_pages, int page_size, int n_tables, int table_width, int selected, int first,
+                                             int recent, float scale, void* out, void* workspace, size_t workspace_bytes,
+                                             void* stream) {
+  const char* what = "sdpa_decode_paged_sparse";
+  MSPR_REQUIRE(dtype == MSPR_F16 || dtype == MSPR_BF16, "%s: dtype must be f16 or bf16", what);
+  MSPR_REQUIRE(k_pages && v_pages && out, "%s: null pointer", what);
+  MSPR_REQUIRE(mspr_aligned(k_pages, 16) && mspr_aligned(v_pages, 16) && mspr_aligned(out, 16), "%s: pointers must be 16-byte aligned", what);
+  Sparse s;
+  if (int rc = sparse_select(what, queries, dtype, codes, scales, tables, lens, requests, batch, n_q_heads, n_kv_heads, head_dim,
+                             n_pages, page_size, n_tables, table_width, selected, first, recent, scale, workspace, workspace_bytes, &s,
+                             (hipStream_t)stream))
+    return rc;
+  return mspr_sdpa_decode_paged(queries, k_pages, v_pages, dtype, s.tables, s.lens, nullptr, batch * n_kv_heads,
+                                n_q_heads / n_kv_heads, 1, head_dim, n_pages * n_kv_heads, page_size, batch * n_kv_heads, selected,
+                                scale, out, s.workspace, s.bytes, stream);
+}
+
+extern "C" int mspr_sdpa_decode_paged_sparse_q8(const void* queries, int q_dtype, const void* k_wq, const void* k_scales,
+                                                const void* k_biases, const void* v_wq, const void* v_scales,
+                                                const void* v_biases, int sb_dtype, const int8_t* codes, const float* scales,
+                                                const int32_t* tables, const int32_t* lens, const int32_t* requests, int batch,
+                                                int n_q_heads, int n_kv_heads, int head_dim, int n_pages, int page_size,
+                                                int n_tables, int table_width, int selected, int first, int recent, float scale,
+                                                int group_size, int bits, void* out, void* workspace, size_t workspace_bytes,
+                                                void* stream) {
+  const char* what = "sdpa_decode_paged_sparse_q8";
+  MSPR_REQUIRE(group_size == 64 && bits == 8, "%s: only group_size=64, bits=8 is supported", what);
+  MSPR_REQUIRE(sb_dtype >= MSPR_F32 && sb_dtype <= MSPR_BF16, "%s: scales must be f32, f16 or bf16", what);
+  for (const void* p : {k_wq, k_scales, k_biases, v_wq, v_scales, v_biases, (const void*)out}) {
+    MSPR_REQUIRE(p, "%s: null pointer", what);
+    MSPR_REQUIRE(mspr_aligned(p, 16), "%s: pointers must be 16-byte aligned", what);
+  }
+  Sparse s;
+  if (int rc = sparse_select(what, queries, q_dtype, codes, scales, tables, lens, requests, batch, n_q_heads, n_kv_heads, head_dim,
+                             n_pages, page_size, n_tables, table_width, selected, first, recent, scale, workspace, workspace_bytes, &s,
+                             (hipStream_t)stream))
+    return rc;
+  return mspr_sdpa_decode_paged_q8(queries, q_dtype, k_wq, k_scales, k_biases, v_wq, v_scales, v_biases, sb_dtype, s.tables, s.lens,
+                                   nullptr, batch * n_kv_heads, n_q_heads / n_kv_heads, 1, head_dim, n_pages * n_kv_heads, page_size,
+                                   batch * n_kv_heads, selected, scale, group_size, bits, out, s.workspace, s.bytes, stream);
+}

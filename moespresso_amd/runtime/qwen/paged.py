@@ -28,6 +28,8 @@ _HEAD_DIM = 256
 _GROUP = 64
 MAX_REQUESTS = 2048  # requests of one page_step
 MAX_SHARED = 2048    # queries, and prefixes, of one call over shared prefixes
+MAX_SELECTED = 4096      # pages that a query may select
+MAX_TABLE_PAGES = 32768  # pages of a request of which some are selected
 
 
 def _check_page_size(page_size: int):
@@ -458,6 +460,179 @@ def sdpa_decode_paged_shared_q8(queries, k_wq, k_scales, k_biases, v_wq, v_scale
         _lib.ptr(lens), _lib.ptr(requests), R, Hq, heads, _HEAD_DIM, n_pages, page_size, G, width, int(tables.shape[0]),
         int(tables.shape[1]), float(scale), 64, 8, _lib.ptr(out), _lib.ptr(workspace),
         workspace.numel() * workspace.element_size()), "sdpa_decode_paged_shared_q8")
+    return out
+
+
+# ---------------------------------------------------------------------------------------------- pages that matter
+
+
+def _check_bounds(codes, scales, heads, n_pages=None):
+    """Number of pages of the bounds of a layer's pages."""
+    if codes.dtype != torch.int8 or codes.ndim != 4 or int(codes.shape[0]) < 1 or tuple(codes.shape[1:]) != (heads, 2, _HEAD_DIM) or \
+            (n_pages is not None and int(codes.shape[0]) != n_pages):
+        raise ValueError("codes must be int8 [n_pages, Hkv, 2, 256]")
+    if scales.dtype != torch.float32 or tuple(scales.shape) != tuple(codes.shape[:2]):
+        raise ValueError("scales must be float32 [n_pages, Hkv]")
+    if not codes.is_contiguous() or not scales.is_contiguous() or codes.storage_offset() % 16 != 0:
+        raise ValueError("codes and scales must be contiguous, codes 16-byte aligned")
+    return int(codes.shape[0])
+
+
+def page_bounds(slots, keys, codes, scales):
+    """Bounds of the keys of every page that a step wrote to, kept up with its append: what ``select_pages`` reads.
+
+    Per page and KV head, over the rows that the page holds so far: ``scale`` is the smallest power of two (from 2^-50 to 2^50)
+    with ``max |k| <= 127 * scale``, ``lower = floor(min k / scale)``, ``upper = ceil(max k / scale)``. They are made of the new rows and
+    of the old bounds where the page held rows before, and are what all of its rows give. (Rows that were taken back and written
+    anew leave their mark until the page is begun again: the bounds are wider then, and bounds still.)
+
+    Args:
+        slots: int32 ``[T]``, as for ``qk_norm_rope_append``, behind which this is called; the rows of a page one behind the
+            other, as ``page_step`` gives them.
+        keys: pages ``[n_pages, Hkv, page_size, 256]`` of 16-bit rows, or ``(codes, scales, biases)`` of 8-bit ones.
+        codes: int8 ``[n_pages, Hkv, 2, 256]``, lower and upper bounds, updated in place; scales: float32 ``[n_pages, Hkv]``. Of a page
+            that was never written to they may hold anything.
+    """
+    n_pages, heads, page_size = _check_pages(keys, keys)
+    _check_bounds(codes, scales, heads, n_pages)
+    if slots.ndim != 1:
+        raise ValueError("slots must be [T]")
+    _check_ints("slots", slots, slots.shape)
+    parts = (keys,) if torch.is_tensor(keys) else tuple(keys)
+    dev = _lib.require_device(slots, *parts, codes, scales)
+    T = int(slots.shape[0])
+    if T == 0:
+        return
+    rest = (T, heads, _HEAD_DIM, n_pages, page_size, _lib.ptr(codes), _lib.ptr(scales))
+    if torch.is_tensor(keys):
+        rc = _lib.launch(dev, "mspr_page_bounds", _lib.ptr(slots), _lib.ptr(keys), _lib.DTYPE_CODE[keys.dtype], *rest)
+    else:
+        rc = _lib.launch(dev, "mspr_page_bounds_q8", _lib.ptr(slots), *(_lib.ptr(t) for t in parts), _lib.DTYPE_CODE[keys[1].dtype], *rest)
+    _lib.check(rc, "page_bounds")
+
+
+def _check_selection(R, heads, tables, n_selected, first, recent):
+    n_selected, first, recent = int(n_selected), int(first), int(recent)
+    if not 1 <= n_selected <= MAX_SELECTED or first < 0 or recent < 1 or first + recent > n_selected:
+        raise ValueError(f"n_selected must be 1 to {MAX_SELECTED}, first 0 or more, recent 1 or more, and both together no more than n_selected")
+    if int(tables.shape[1]) > MAX_TABLE_PAGES:
+        raise ValueError(f"tables must hold at most {MAX_TABLE_PAGES} pages a request")
+    if R * heads > 65535:
+        raise ValueError("at most 65535 queries times KV heads a call")
+    return n_selected, first, recent
+
+
+def select_pages(queries, codes, scales, tables, lens, n_selected, *, page_size: int, first: int = 1, recent: int = 2, requests=None,
+                 workspace=None):
+    """The pages that every query may weigh most, per KV head, from the bounds of its request's pages.
+
+    The bound of a page and query head is the largest product of the head's query (in 8 bits, a power of two a head) with any
+    key within the page's bounds. A page is worth, at the query head where that is most, how far its bound lies above (below) the
+    best bound of that head. Of requests of more than ``n_selected`` pages the first ``first`` and the last ``recent`` pages are taken,
+    and those of greatest worth among the others, ties to the lower page. Bounds are exact whole numbers times a power of two: the
+    same call gives the same pages.
+
+    Args:
+        queries: ``[R, Hq, 256]`` float32, float16 or bfloat16, already rotated, at most 16 query heads per KV head.
+        codes, scales: of ``page_bounds``.
+        tables, lens, requests: as for ``sdpa_decode_paged``; at most 32768 pages a request.
+        page_size: that of the pages.
+        n_selected: pages a query and KV head, at most 4096.
+
+    Returns:
+        ``(tables, lens)``: int32 ``[R, Hkv, n_selected]``, the pages in the order of their positions as pages of a pool of one head
+        a page (``page * Hkv + head``, -1 behind the last), and int32 ``[R, Hkv]``, the rows in them. With a layer's pages viewed as
+        ``[n_pages * Hkv, 1, page_size, 256]`` and queries as ``[R * Hkv, Hq / Hkv, 256]``, they are the tables and lengths of
+        ``sdpa_decode_paged``.
+    """
+    if queries.dtype not in _lib.DTYPE_CODE:
+        raise ValueError("queries must be float32, float16 or bfloat16")
+    page_size = int(page_size)
+    _check_page_size(page_size)
+    if codes.ndim != 4 or int(codes.shape[1]) < 1:
+        raise ValueError("codes must be int8 [n_pages, Hkv, 2, 256]")
+    heads = int(codes.shape[1])
+    n_pages = _check_bounds(codes, scales, heads)
+    R, Hq = _check_decode(queries, heads, tables, lens, requests)
+    n_selected, first, recent = _check_selection(R, heads, tables, n_selected, first, recent)
+    dev = _lib.require_device(queries, codes, scales, tables, lens, requests)
+    out_tables = torch.empty((R, heads, n_selected), dtype=torch.int32, device=dev)
+    out_lens = torch.empty((R, heads), dtype=torch.int32, device=dev)
+    if R == 0:
+        return out_tables, out_lens
+    q = _aligned(queries.contiguous())
+    if workspace is None:
+        workspace = _lib.select_pages_workspace(R, Hq, heads, int(tables.shape[1]), dev)
+    _lib.check(_lib.launch(
+        dev, "mspr_select_pages", _lib.ptr(q), _lib.DTYPE_CODE[q.dtype], _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(tables),
+        _lib.ptr(lens), _lib.ptr(requests), R, Hq, heads, _HEAD_DIM, n_pages, page_size, int(tables.shape[0]), int(tables.shape[1]),
+        n_selected, first, recent, _lib.ptr(out_tables), _lib.ptr(out_lens), _lib.ptr(workspace),
+        workspace.numel() * workspace.element_size()), "select_pages")
+    return out_tables, out_lens
+
+
+def sdpa_decode_paged_sparse(queries, keys, values, codes, scales, tables, lens, scale, n_selected, *, first: int = 1, recent: int = 2,
+                             requests=None, workspace=None):
+    """``sdpa_decode_paged`` over the pages that ``select_pages`` selects for every query and KV head.
+
+    Args:
+        queries, keys, values, tables, lens, scale, requests: as for ``sdpa_decode_paged``; the scale must not be negative.
+        codes, scales, n_selected, first, recent: as for ``select_pages``.
+    """
+    if not torch.is_tensor(keys) or not torch.is_tensor(values):
+        raise ValueError("keys and values must be 16-bit pages (8-bit ones: sdpa_decode_paged_sparse_q8)")
+    n_pages, heads, page_size = _check_pages(keys, values)
+    if queries.dtype != keys.dtype:
+        raise ValueError("pages must have the dtype of queries")
+    R, Hq = _check_decode(queries, heads, tables, lens, requests)
+    _check_bounds(codes, scales, heads, n_pages)
+    n_selected, first, recent = _check_selection(R, heads, tables, n_selected, first, recent)
+    dev = _lib.require_device(queries, keys, values, codes, scales, tables, lens, requests)
+    out = torch.empty(tuple(queries.shape), dtype=queries.dtype, device=dev)
+    if R == 0:
+        return out
+    q = _aligned(queries.contiguous())
+    if workspace is None:
+        workspace = _lib.paged_sparse_workspace(R, Hq, heads, page_size, int(tables.shape[1]), n_selected, dev)
+    _lib.check(_lib.launch(
+        dev, "mspr_sdpa_decode_paged_sparse", _lib.ptr(q), _lib.ptr(keys), _lib.ptr(values), _lib.DTYPE_CODE[q.dtype],
+        _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(tables), _lib.ptr(lens), _lib.ptr(requests), R, Hq, heads, _HEAD_DIM, n_pages,
+        page_size, int(tables.shape[0]), int(tables.shape[1]), n_selected, first, recent, float(scale), _lib.ptr(out),
+        _lib.ptr(workspace), workspace.numel() * workspace.element_size()), "sdpa_decode_paged_sparse")
+    return out
+
+
+def sdpa_decode_paged_sparse_q8(queries, k_wq, k_scales, k_biases, v_wq, v_scales, v_biases, codes, scales, tables, lens, scale,
+                                n_selected, *, first: int = 1, recent: int = 2, group_size: int = 64, bits: int = 8, requests=None,
+                                workspace=None):
+    """``sdpa_decode_paged_sparse`` over pages of affine 8-bit rows.
+
+    Args:
+        queries: ``[R, Hq, 256]`` float32, float16 or bfloat16.
+        k_wq, k_scales, k_biases, v_wq, v_scales, v_biases: as for ``sdpa_decode_paged_q8``.
+        codes, scales, tables, lens, scale, n_selected, first, recent, requests: as for ``sdpa_decode_paged_sparse``.
+    """
+    if group_size != 64 or bits != 8:
+        raise ValueError("sdpa_decode_paged_sparse_q8 supports group_size=64, bits=8 only")
+    n_pages, heads, page_size = _check_pages((k_wq, k_scales, k_biases), (v_wq, v_scales, v_biases))
+    if queries.dtype not in _lib.DTYPE_CODE:
+        raise ValueError("queries must be float32, float16 or bfloat16")
+    R, Hq = _check_decode(queries, heads, tables, lens, requests)
+    _check_bounds(codes, scales, heads, n_pages)
+    n_selected, first, recent = _check_selection(R, heads, tables, n_selected, first, recent)
+    parts = (k_wq, k_scales, k_biases, v_wq, v_scales, v_biases)
+    dev = _lib.require_device(queries, *parts, codes, scales, tables, lens, requests)
+    out = torch.empty(tuple(queries.shape), dtype=queries.dtype, device=dev)
+    if R == 0:
+        return out
+    q = _aligned(queries.contiguous())
+    if workspace is None:
+        workspace = _lib.paged_sparse_workspace(R, Hq, heads, page_size, int(tables.shape[1]), n_selected, dev)
+    _lib.check(_lib.launch(
+        dev, "mspr_sdpa_decode_paged_sparse_q8", _lib.ptr(q), _lib.DTYPE_CODE[q.dtype], *(_lib.ptr(t) for t in parts),
+        _lib.DTYPE_CODE[k_scales.dtype], _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(tables), _lib.ptr(lens), _lib.ptr(requests), R,
+        Hq, heads, _HEAD_DIM, n_pages, page_size, int(tables.shape[0]), int(tables.shape[1]), n_selected, first, recent, float(scale),
+        64, 8, _lib.ptr(out), _lib.ptr(workspace), workspace.numel() * workspace.element_size()), "sdpa_decode_paged_sparse_q8")
     return out
 
 

@@ -102,3 +102,58 @@ def paged_attention(q, keys, values, tables, lens, scale, requests=None):
             w = np.exp(s - s.max(-1, keepdims=True))
             out[r, g * rep:(g + 1) * rep] = w @ v / w.sum(-1, keepdims=True)
     return out
+
+
+LIMIT = 50  # exponents of bounds and query codes lie within +-50
+
+
+def exponent(top):
+    """The smallest e with top <= 127 * 2^e, within the limit."""
+    e = -LIMIT
+    while top > 127 * 2.0 ** e and e < LIMIT:
+        e += 1
+    return e
+
+
+def bounds(rows):
+    """(lower codes, upper codes, exponent) of rows [n, D] of one page and KV head, in float64."""
+    rows = np.asarray(rows, dtype=np.float64)
+    low, high = rows.min(0), rows.max(0)
+    e = exponent(max(-low.min(), high.max()))
+    low, high = (np.clip(f(x / 2.0 ** e), -127, 127).astype(np.int64) for f, x in ((np.floor, low), (np.ceil, high)))
+    return low, high, e
+
+
+def select_pages(q, codes, scales, tables, lens, page_size, selected, first, recent, requests=None):
+    """(tables [R, Hkv, selected], lens [R, Hkv]) as ``mspr_select_pages`` defines them; sums in Python's whole numbers."""
+    q, codes = np.asarray(q, dtype=np.float64), np.asarray(codes, dtype=np.int64)
+    n_pages, G = codes.shape[:2]
+    R, Hq, _ = q.shape
+    rep = Hq // G
+    out, out_lens = np.full((R, G, selected), -1), np.zeros((R, G), dtype=np.int64)
+    for r in range(R):
+        b = r if requests is None else int(requests[r])
+        seen = min(max(int(lens[r]), 0), len(tables[0]) * page_size) if 0 <= b < len(tables) else 0
+        n = -(-seen // page_size)
+        pages = [int(p) if 0 <= p < n_pages else -1 for p in tables[b][:n]] if n else []
+        for g in range(G):
+            chosen = range(n)
+            if n > selected:
+                worth = np.full(n, -np.inf)
+                for h in range(rep):
+                    x = q[r, g * rep + h]
+                    e = exponent(np.abs(x).max())
+                    c = np.clip(np.rint(x / 2.0 ** e), -127, 127)
+                    bound = np.full(n, -np.inf)
+                    for i, p in enumerate(pages):
+                        if p >= 0:
+                            bound[i] = np.maximum(c * codes[p, g, 0], c * codes[p, g, 1]).sum() * 2.0 ** e * float(scales[p, g])
+                    if np.isfinite(bound.max()):
+                        worth = np.maximum(worth, (bound - bound.max()).astype(np.float32))
+                worth[:first] = np.inf
+                worth[n - recent:] = np.inf
+                chosen = sorted(sorted(range(n), key=lambda i: (-worth[i], i))[:selected])
+            ids = [pages[i] * G + g if pages[i] >= 0 else -1 for i in chosen]
+            out[r, g, :len(ids)] = ids
+            out_lens[r, g] = (len(ids) - 1) * page_size + seen - (n - 1) * page_size if n else 0
+    return out, out_lens
