@@ -855,21 +855,25 @@ struct Decode {
   int64_t R, Hq, B, P;
 };
 
-bool decode_operands(PyObject* queries, PyObject* const* rest, const Pages& p, Decode* d, Tensor* ws) {
+bool decode_shapes(PyObject* queries, PyObject* const* rest, int64_t heads, Decode* d) {
   d->q = dense(queries, 3);
   d->tables = dense(rest[0], 2, at::kInt);
   d->lens = dense(rest[1], 1, at::kInt);
-  if (!d->q || !d->tables || !d->lens || !real(rest[3], &d->scale)) return false;
+  if (!d->q || !d->tables || !d->lens) return false;
   if (rest[2] != Py_None && !(d->requests = dense(rest[2], 1, at::kInt))) return false;
   d->R = d->q->size(0);
   d->Hq = d->q->size(1);
   d->B = d->tables->size(0);
   d->P = d->tables->size(1);
-  if (d->q->size(2) != 256 || d->R < 1 || d->R > 65535 || d->Hq < 1 || d->Hq % p.heads != 0 || d->Hq / p.heads > 16 || d->B < 1 ||
+  if (d->q->size(2) != 256 || d->R < 1 || d->R > 65535 || d->Hq < 1 || d->Hq % heads != 0 || d->Hq / heads > 16 || d->B < 1 ||
       d->B > INT32_MAX || d->P < 1 || d->P > INT32_MAX || d->lens->size(0) != d->R || !aligned16(*d->q) ||
       (d->requests ? d->requests->size(0) != d->R : d->B != d->R))
     return false;
-  if (!here({d->q, d->tables, d->lens}) || (d->requests && !here({d->q, d->requests})) || !together(p, *d->q)) return false;
+  return here({d->q, d->tables, d->lens}) && (!d->requests || here({d->q, d->requests}));
+}
+
+bool decode_operands(PyObject* queries, PyObject* const* rest, const Pages& p, Decode* d, Tensor* ws) {
+  if (!real(rest[3], &d->scale) || !decode_shapes(queries, rest, p.heads, d) || !together(p, *d->q)) return false;
   return take_workspace(rest[4], mspr_sdpa_decode_paged_workspace_bytes((int)d->R, (int)d->Hq, (int)p.heads, (int)p.page, (int)d->P),
                         *d->q, ws);
 }
@@ -913,6 +917,199 @@ PyObject* sdpa_decode_paged_q8(PyObject* const* a, Py_ssize_t nargs) {
   return failed(rc, "sdpa_decode_paged_q8") ? nullptr : wrap(out);
 }
 
+// Prefixes of a call: tables, lengths, the prefix of every request; then as Decode.
+struct Shared : Decode {
+  const Tensor *prefix_tables, *prefix_lens, *groups;
+  int64_t G, width;
+};
+
+// (rest: prefix_tables, prefix_lens, groups, tables, lens, requests or None, scale, workspace)
+bool shared_operands(PyObject* queries, PyObject* const* rest, const Pages& p, Shared* d, Tensor* ws) {
+  d->prefix_tables = dense(rest[0], 2, at::kInt);
+  d->prefix_lens = dense(rest[1], 1, at::kInt);
+  d->groups = dense(rest[2], 1, at::kInt);
+  if (!d->prefix_tables || !d->prefix_lens || !d->groups || !real(rest[6], &d->scale) ||
+      !decode_shapes(queries, rest + 3, p.heads, d) || !together(p, *d->q))
+    return false;
+  d->G = d->prefix_tables->size(0);
+  d->width = d->prefix_tables->size(1);
+  if (d->R > 2048 || d->G < 1 || d->G > 2048 || d->width < 1 || d->width > INT32_MAX || d->prefix_lens->size(0) != d->G ||
+      d->groups->size(0) != d->B || !here({d->q, d->prefix_tables, d->prefix_lens, d->groups}))
+    return false;
+  return take_workspace(rest[7], mspr_sdpa_decode_paged_shared_workspace_bytes((int)d->R, (int)d->Hq, (int)p.heads, (int)d->G), *d->q,
+                        ws);
+}
+
+const int32_t* ints(const Tensor* t) { return (const int32_t*)at_or_null(t); }
+
+// (queries [R, Hq, 256], keys, values, eight as above) -> like queries
+PyObject* sdpa_decode_paged_shared(PyObject* const* a, Py_ssize_t nargs) {
+  MSPR_NARGS(11)
+  Pages p;
+  Shared d;
+  Tensor ws;
+  if (!page_tensors(a[1], a[2], &p) || !shared_operands(a[0], a + 3, p, &d, &ws) || type_code(d.q->scalar_type()) != p.code)
+    return none();
+  Tensor out = empty(d.q->sizes(), d.q->scalar_type(), *d.q);
+  const int rc = launch([&](void* st) {
+    return mspr_sdpa_decode_paged_shared(d.q->const_data_ptr(), p.t[0]->const_data_ptr(), p.t[1]->const_data_ptr(), p.code,
+                                         ints(d.prefix_tables), ints(d.prefix_lens), ints(d.groups), ints(d.tables), ints(d.lens),
+                                         ints(d.requests), (int)d.R, (int)d.Hq, (int)p.heads, 256, (int)p.pages, (int)p.page,
+                                         (int)d.G, (int)d.width, (int)d.B, (int)d.P, d.scale, out.data_ptr(), ws.data_ptr(),
+                                         ws.nbytes(), st);
+  });
+  return failed(rc, "sdpa_decode_paged_shared") ? nullptr : wrap(out);
+}
+
+// (queries [R, Hq, 256], six page parts, eight as above) -> like queries
+PyObject* sdpa_decode_paged_shared_q8(PyObject* const* a, Py_ssize_t nargs) {
+  MSPR_NARGS(15)
+  Pages p;
+  Shared d;
+  Tensor ws;
+  if (!page_triplets(a + 1, &p) || !shared_operands(a[0], a + 7, p, &d, &ws)) return none();
+  const int code = type_code(d.q->scalar_type());
+  if (code == kNoType) return none();
+  Tensor out = empty(d.q->sizes(), d.q->scalar_type(), *d.q);
+  const int rc = launch([&](void* st) {
+    return mspr_sdpa_decode_paged_shared_q8(
+        d.q->const_data_ptr(), code, p.t[0]->const_data_ptr(), p.t[1]->const_data_ptr(), p.t[2]->const_data_ptr(),
+        p.t[3]->const_data_ptr(), p.t[4]->const_data_ptr(), p.t[5]->const_data_ptr(), p.code, ints(d.prefix_tables),
+        ints(d.prefix_lens), ints(d.groups), ints(d.tables), ints(d.lens), ints(d.requests), (int)d.R, (int)d.Hq, (int)p.heads, 256,
+        (int)p.pages, (int)p.page, (int)d.G, (int)d.width, (int)d.B, (int)d.P, d.scale, 64, 8, out.data_ptr(), ws.data_ptr(),
+        ws.nbytes(), st);
+  });
+  return failed(rc, "sdpa_decode_paged_shared_q8") ? nullptr : wrap(out);
+}
+
+// Bounds of a layer's pages: codes int8 [n_pages, heads, 2, 256], scales f32 [n_pages, heads].
+bool bound_tensors(PyObject* codes, PyObject* scales, const Tensor** c, const Tensor** s) {
+  *c = dense(codes, 4, at::kChar);
+  *s = dense(scales, 2, at::kFloat);
+  return *c && *s && (*c)->size(0) >= 1 && (*c)->size(0) <= INT32_MAX && (*c)->size(1) >= 1 && (*c)->size(1) <= 1024 &&
+         (*c)->size(2) == 2 && (*c)->size(3) == 256 && (*s)->size(0) == (*c)->size(0) && (*s)->size(1) == (*c)->size(1) &&
+         aligned16(**c);
+}
+
+// (slots int32 [T], keys or (codes, scales, biases), codes, scales) -> True where it was done
+PyObject* page_bounds(PyObject* const* a, Py_ssize_t nargs) {
+  MSPR_NARGS(4)
+  const Tensor *slots = dense(a[0], 1, at::kInt), *c, *s, *t[3];
+  if (!slots || !bound_tensors(a[2], a[3], &c, &s) || !here({slots, c, s})) return none();
+  const bool coded = PyTuple_CheckExact(a[1]) && PyTuple_GET_SIZE(a[1]) == 3;
+  if (coded) {
+    if (!page_triplet(PyTuple_GET_ITEM(a[1], 0), PyTuple_GET_ITEM(a[1], 1), PyTuple_GET_ITEM(a[1], 2), t) ||
+        !here({slots, t[0], t[1], t[2]}))
+      return none();
+  } else {
+    t[0] = dense(a[1], 4);
+    if (!page_rows(t[0], 256) || (t[0]->scalar_type() != at::kHalf && t[0]->scalar_type() != at::kBFloat16) || !here({slots, t[0]}))
+      return none();
+  }
+  const int64_t T = slots->size(0), N = t[0]->size(0), heads = t[0]->size(1), page = t[0]->size(2);
+  if (T < 1 || T > INT32_MAX || c->size(0) != N || c->size(1) != heads || !page_size_ok(page)) return none();
+  auto* to = (int8_t*)c->data_ptr();
+  auto* of = (float*)s->data_ptr();
+  const int code = type_code(t[coded ? 1 : 0]->scalar_type());
+  const int rc = launch([&](void* st) {
+    return coded ? mspr_page_bounds_q8(ints(slots), t[0]->const_data_ptr(), t[1]->const_data_ptr(), t[2]->const_data_ptr(), code,
+                                       (int)T, (int)heads, 256, (int)N, (int)page, to, of, st)
+                 : mspr_page_bounds(ints(slots), t[0]->const_data_ptr(), code, (int)T, (int)heads, 256, (int)N, (int)page, to, of, st);
+  });
+  if (failed(rc, "page_bounds")) return nullptr;
+  Py_RETURN_TRUE;
+}
+
+// What the selection takes beside queries, tables, lens and requests.
+struct Selection {
+  const Tensor *codes, *scales;
+  int selected, first, recent;
+};
+bool selection_operands(PyObject* codes, PyObject* scales, PyObject* const* counts, const Decode& d, Selection* s) {
+  return bound_tensors(codes, scales, &s->codes, &s->scales) && whole32(counts[0], &s->selected) && whole32(counts[1], &s->first) &&
+         whole32(counts[2], &s->recent) && s->selected >= 1 && s->selected <= 4096 && s->first >= 0 && s->recent >= 1 &&
+         (int64_t)s->first + s->recent <= s->selected && d.P <= 32768 && d.R * s->codes->size(1) <= 65535 &&
+         here({d.q, s->codes, s->scales});
+}
+
+// (queries [R, Hq, 256], codes, scales, tables, lens, requests or None, n_selected, first, recent, page_size, workspace)
+// -> (tables, lens)
+PyObject* select_pages(PyObject* const* a, Py_ssize_t nargs) {
+  MSPR_NARGS(11)
+  Decode d;
+  Selection s;
+  int page;
+  if (!bound_tensors(a[1], a[2], &s.codes, &s.scales)) return none();
+  const int64_t heads = s.codes->size(1);
+  if (!decode_shapes(a[0], a + 3, heads, &d) || !selection_operands(a[1], a[2], a + 6, d, &s) || !whole32(a[9], &page) ||
+      !page_size_ok(page))
+    return none();
+  const int code = type_code(d.q->scalar_type());
+  Tensor ws;
+  if (code == kNoType || !take_workspace(a[10], mspr_select_pages_workspace_bytes((int)d.R, (int)d.Hq, (int)heads, (int)d.P), *d.q, &ws))
+    return none();
+  Tensor tables = empty({d.R, heads, s.selected}, at::kInt, *d.q), lens = empty({d.R, heads}, at::kInt, *d.q);
+  const int rc = launch([&](void* st) {
+    return mspr_select_pages(d.q->const_data_ptr(), code, (const int8_t*)s.codes->const_data_ptr(),
+                             (const float*)s.scales->const_data_ptr(), ints(d.tables), ints(d.lens), ints(d.requests), (int)d.R,
+                             (int)d.Hq, (int)heads, 256, (int)s.codes->size(0), page, (int)d.B, (int)d.P, s.selected, s.first,
+                             s.recent, (int32_t*)tables.data_ptr(), (int32_t*)lens.data_ptr(), ws.data_ptr(), ws.nbytes(), st);
+  });
+  return failed(rc, "select_pages") ? nullptr : wrap_tuple(tables, lens);
+}
+
+// (rest: codes, scales, tables, lens, requests or None, scale, n_selected, first, recent, workspace)
+bool sparse_operands(PyObject* queries, PyObject* const* rest, const Pages& p, Decode* d, Selection* s, Tensor* ws) {
+  if (!real(rest[5], &d->scale) || !decode_shapes(queries, rest + 2, p.heads, d) || !together(p, *d->q) ||
+      !selection_operands(rest[0], rest[1], rest + 6, *d, s) || s->codes->size(0) != p.pages || s->codes->size(1) != p.heads)
+    return false;
+  return take_workspace(rest[9], mspr_sdpa_decode_paged_sparse_workspace_bytes((int)d->R, (int)d->Hq, (int)p.heads, (int)p.page,
+                                                                               (int)d->P, s->selected),
+                        *d->q, ws);
+}
+
+// (queries [R, Hq, 256], keys, values, ten as above) -> like queries
+PyObject* sdpa_decode_paged_sparse(PyObject* const* a, Py_ssize_t nargs) {
+  MSPR_NARGS(13)
+  Pages p;
+  Decode d;
+  Selection s;
+  Tensor ws;
+  if (!page_tensors(a[1], a[2], &p) || !sparse_operands(a[0], a + 3, p, &d, &s, &ws) || type_code(d.q->scalar_type()) != p.code)
+    return none();
+  Tensor out = empty(d.q->sizes(), d.q->scalar_type(), *d.q);
+  const int rc = launch([&](void* st) {
+    return mspr_sdpa_decode_paged_sparse(d.q->const_data_ptr(), p.t[0]->const_data_ptr(), p.t[1]->const_data_ptr(), p.code,
+                                         (const int8_t*)s.codes->const_data_ptr(), (const float*)s.scales->const_data_ptr(),
+                                         ints(d.tables), ints(d.lens), ints(d.requests), (int)d.R, (int)d.Hq, (int)p.heads, 256,
+                                         (int)p.pages, (int)p.page, (int)d.B, (int)d.P, s.selected, s.first, s.recent, d.scale,
+                                         out.data_ptr(), ws.data_ptr(), ws.nbytes(), st);
+  });
+  return failed(rc, "sdpa_decode_paged_sparse") ? nullptr : wrap(out);
+}
+
+// (queries [R, Hq, 256], six page parts, ten as above) -> like queries
+PyObject* sdpa_decode_paged_sparse_q8(PyObject* const* a, Py_ssize_t nargs) {
+  MSPR_NARGS(17)
+  Pages p;
+  Decode d;
+  Selection s;
+  Tensor ws;
+  if (!page_triplets(a + 1, &p) || !sparse_operands(a[0], a + 7, p, &d, &s, &ws)) return none();
+  const int code = type_code(d.q->scalar_type());
+  if (code == kNoType) return none();
+  Tensor out = empty(d.q->sizes(), d.q->scalar_type(), *d.q);
+  const int rc = launch([&](void* st) {
+    return mspr_sdpa_decode_paged_sparse_q8(
+        d.q->const_data_ptr(), code, p.t[0]->const_data_ptr(), p.t[1]->const_data_ptr(), p.t[2]->const_data_ptr(),
+        p.t[3]->const_data_ptr(), p.t[4]->const_data_ptr(), p.t[5]->const_data_ptr(), p.code, (const int8_t*)s.codes->const_data_ptr(),
+        (const float*)s.scales->const_data_ptr(), ints(d.tables), ints(d.lens), ints(d.requests), (int)d.R, (int)d.Hq, (int)p.heads,
+        256, (int)p.pages, (int)p.page, (int)d.B, (int)d.P, s.selected, s.first, s.recent, d.scale, 64, 8, out.data_ptr(),
+        ws.data_ptr(), ws.nbytes(), st);
+  });
+  return failed(rc, "sdpa_decode_paged_sparse_q8") ? nullptr : wrap(out);
+}
+
 PyMethodDef kMethods[] = {
 #define MSPR_METHOD(name) {#name, (PyCFunction)(void (*)(void))guarded<name>, METH_FASTCALL, nullptr}
     {"indexer_qat_rows", (PyCFunction)(void (*)(void))guarded<qat_rows<false>>, METH_FASTCALL, nullptr},
@@ -938,6 +1135,12 @@ PyMethodDef kMethods[] = {
     MSPR_METHOD(qk_norm_rope_append),
     MSPR_METHOD(sdpa_decode_paged),
     MSPR_METHOD(sdpa_decode_paged_q8),
+    MSPR_METHOD(sdpa_decode_paged_shared),
+    MSPR_METHOD(sdpa_decode_paged_shared_q8),
+    MSPR_METHOD(page_bounds),
+    MSPR_METHOD(select_pages),
+    MSPR_METHOD(sdpa_decode_paged_sparse),
+    MSPR_METHOD(sdpa_decode_paged_sparse_q8),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_dispatch", "Native call path of the operators.", -1, kMethods,

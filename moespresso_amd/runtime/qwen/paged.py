@@ -404,6 +404,10 @@ def sdpa_decode_paged_shared(queries, keys, values, prefix_tables, prefix_lens, 
     Returns:
         ``[R, Hq, 256]`` in the dtype of ``queries``.
     """
+    out = _lib.dispatch.sdpa_decode_paged_shared(queries, keys, values, prefix_tables, prefix_lens, groups, tables, lens, requests,
+                                                 scale, workspace)
+    if out is not None:
+        return out
     if not torch.is_tensor(keys) or not torch.is_tensor(values):
         raise ValueError("keys and values must be 16-bit pages (8-bit ones: sdpa_decode_paged_shared_q8)")
     n_pages, heads, page_size = _check_pages(keys, values)
@@ -439,6 +443,10 @@ def sdpa_decode_paged_shared_q8(queries, k_wq, k_scales, k_biases, v_wq, v_scale
     """
     if group_size != 64 or bits != 8:
         raise ValueError("sdpa_decode_paged_shared_q8 supports group_size=64, bits=8 only")
+    out = _lib.dispatch.sdpa_decode_paged_shared_q8(queries, k_wq, k_scales, k_biases, v_wq, v_scales, v_biases, prefix_tables,
+                                                    prefix_lens, groups, tables, lens, requests, scale, workspace)
+    if out is not None:
+        return out
     n_pages, heads, page_size = _check_pages((k_wq, k_scales, k_biases), (v_wq, v_scales, v_biases))
     if queries.dtype not in _lib.DTYPE_CODE:
         raise ValueError("queries must be float32, float16 or bfloat16")
@@ -493,6 +501,8 @@ def page_bounds(slots, keys, codes, scales):
         codes: int8 ``[n_pages, Hkv, 2, 256]``, lower and upper bounds, updated in place; scales: float32 ``[n_pages, Hkv]``. Of a page
             that was never written to they may hold anything.
     """
+    if _lib.dispatch.page_bounds(slots, keys, codes, scales) is not None:
+        return
     n_pages, heads, page_size = _check_pages(keys, keys)
     _check_bounds(codes, scales, heads, n_pages)
     if slots.ndim != 1:
@@ -545,6 +555,9 @@ def select_pages(queries, codes, scales, tables, lens, n_selected, *, page_size:
         ``[n_pages * Hkv, 1, page_size, 256]`` and queries as ``[R * Hkv, Hq / Hkv, 256]``, they are the tables and lengths of
         ``sdpa_decode_paged``.
     """
+    done = _lib.dispatch.select_pages(queries, codes, scales, tables, lens, requests, n_selected, first, recent, page_size, workspace)
+    if done is not None:
+        return done
     if queries.dtype not in _lib.DTYPE_CODE:
         raise ValueError("queries must be float32, float16 or bfloat16")
     page_size = int(page_size)
@@ -579,6 +592,10 @@ def sdpa_decode_paged_sparse(queries, keys, values, codes, scales, tables, lens,
         queries, keys, values, tables, lens, scale, requests: as for ``sdpa_decode_paged``; the scale must not be negative.
         codes, scales, n_selected, first, recent: as for ``select_pages``.
     """
+    out = _lib.dispatch.sdpa_decode_paged_sparse(queries, keys, values, codes, scales, tables, lens, requests, scale, n_selected,
+                                                 first, recent, workspace)
+    if out is not None:
+        return out
     if not torch.is_tensor(keys) or not torch.is_tensor(values):
         raise ValueError("keys and values must be 16-bit pages (8-bit ones: sdpa_decode_paged_sparse_q8)")
     n_pages, heads, page_size = _check_pages(keys, values)
@@ -614,6 +631,10 @@ def sdpa_decode_paged_sparse_q8(queries, k_wq, k_scales, k_biases, v_wq, v_scale
     """
     if group_size != 64 or bits != 8:
         raise ValueError("sdpa_decode_paged_sparse_q8 supports group_size=64, bits=8 only")
+    out = _lib.dispatch.sdpa_decode_paged_sparse_q8(queries, k_wq, k_scales, k_biases, v_wq, v_scales, v_biases, codes, scales, tables,
+                                                    lens, requests, scale, n_selected, first, recent, workspace)
+    if out is not None:
+        return out
     n_pages, heads, page_size = _check_pages((k_wq, k_scales, k_biases), (v_wq, v_scales, v_biases))
     if queries.dtype not in _lib.DTYPE_CODE:
         raise ValueError("queries must be float32, float16 or bfloat16")
