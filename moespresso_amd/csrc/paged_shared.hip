@@ -7,11 +7,17 @@
 // and O^T = V^T.P^T by 16x16x32 matrix instructions, an online softmax a wave, weights in two terms). What differs: a wave
 // multiplies a tile of 32 keys, once it is in registers, with up to 32 columns, the query heads of several members of a group.
 //
-// Work is cut into pieces: a block of a prefix's members (as many as fill 32 columns) or a query's own rows, of one KV head, over
-// a range of tiles. Every workgroup plans for itself (lengths and groups are known on the device only): a range's length follows
-// from all tiles there are, so that a piece falls to every compute unit; the number of a piece says what it is. Blocks of one
-// range lie eight workgroups apart, on one XCD, whose L2 then has the rows for the second block. The four waves of a workgroup
-// take the tiles of a piece in turn and meet in LDS; a second kernel joins a query's pieces.
+// Work is cut into pieces: a block of a prefix's members, or a query's own rows, of one KV head, over a range of tiles. Every
+// workgroup plans for itself (lengths and groups are known on the device only): a range's length follows from all tiles there are,
+// so that a piece falls to every compute unit; the number of a piece says what it is. Blocks of one range lie eight workgroups
+// apart, on one XCD, whose L2 then has the rows for the second block. A last kernel joins a query's pieces.
+//
+// Prefixes of 16-bit rows (paged_prefix_kernel): up to 256 columns a block. Tiles of 32 keys come by asynchronous copies into a
+// ring of LDS that eight waves share, 32 columns a wave: read from HBM once, from LDS by every wave (the layout and the order of
+// flash_prefill.hip). Up to 128 columns the waves take two tiles at a time, four each.
+//
+// Own rows (and prefixes of 8-bit rows, in blocks of 32 columns; paged_shared_kernel): a tile is a wave's own, in registers, and the
+// four waves of a workgroup, which take the tiles of a piece in turn, meet in LDS.
 #include "paged_rows.h"
 
 namespace {
@@ -20,6 +26,9 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kGroups = 256;    // workgroups that run at once: one a compute unit
 constexpr int kColumns = 32;    // of a piece, in blocks of 16
+constexpr int kWideWaves = 8;   // of the kernel for prefixes of 16-bit rows
+constexpr int kWideThreads = 64 * kWideWaves;
+constexpr int kWideColumns = 32 * kWideWaves;
 constexpr int kBlocks = kColumns / 16;
 constexpr int kMinShare = 4;    // tiles of a range, at least: one a wave
 constexpr int kMaxRows = 2048;  // queries, and prefixes, of a call
@@ -30,9 +39,10 @@ struct SharedRest {
   const int32_t* tables;          // [n_tables, width]
   const void *k, *v, *k_scales, *k_biases, *v_scales, *v_biases;
   int n_pages, page_shift, prefix_width, width, prefix_slots, own_slots;
+  int block;          // columns of a block of a prefix's members, at most
   float scale_log2;
-  float* ws_pre;      // partial outputs of prefix pieces [prefix_slots][32 columns][256]
-  float* ws_pre_ml;   // their statistics [prefix_slots][32][2]
+  float* ws_pre;      // partial outputs of prefix pieces [prefix_slots][block columns][256]
+  float* ws_pre_ml;   // their statistics [prefix_slots][block][2]
   float* ws_own;      // of own pieces [own_slots][rep][256]
   float* ws_own_ml;   // [own_slots][16][2]
   int32_t* parts;     // [B * n_kv][8]: of own pieces the first and how many; of prefix pieces the first, ranges, blocks, first column
@@ -42,7 +52,7 @@ struct SharedRest {
 struct SharedArgs {
   const int32_t *requests, *groups, *lens, *prefix_lens;
   int batch, n_prefixes, n_tables, n_kv, rep;
-  int pieces;  // workgroups: no less than the pieces there can be
+  int pieces, prefix_pieces;  // workgroups: no less than the pieces there can be (of own rows and prefixes, or each)
   SharedRest rest;
 };
 
@@ -501,9 +511,9 @@ __device__ __forceinline__ void attend_piece(const SharedRest& a, const Piece& p
   // ---- the four waves meet in LDS, a block of columns at a time (the V tiles are free now)
   float* xo = reinterpret_cast<float*>(lds);   // [waves][16 mt][64 lanes][4]
   float* xml = xo + kWaves * 16 * 64 * 4;      // [waves][16 columns][2]
-  const int width = p.prefix >= 0 ? kColumns : rep;  // columns of a partial
+  const int width = p.prefix >= 0 ? a.block : rep;  // columns of a partial
   const auto po = store_window((p.prefix >= 0 ? a.ws_pre : a.ws_own) + (int64_t)p.slot * width * kD, width * kD * (int)sizeof(float));
-  float* ml = p.prefix >= 0 ? a.ws_pre_ml + (int64_t)p.slot * kColumns * 2 : a.ws_own_ml + (int64_t)p.slot * 16 * 2;
+  float* ml = p.prefix >= 0 ? a.ws_pre_ml + (int64_t)p.slot * a.block * 2 : a.ws_own_ml + (int64_t)p.slot * 16 * 2;
 #pragma unroll
   for (int b = 0; b < NB; b++) {
     l_run[b] += __shfl_xor(l_run[b], 16, MSPR_WAVE);
@@ -555,6 +565,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(const int32_t
                                                                    const int32_t* prefix_lens, int batch, int n_prefixes,
                                                                    int n_tables, int n_kv, int rep, SharedRest a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  constexpr bool kPrefixes = FMT == kAffine;  // else another kernel's
   __shared__ int wave_sums[3][kWaves];
   __shared__ int members[kColumns];
   __shared__ Piece found;
@@ -585,11 +596,12 @@ __global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(const int32_t
   if (t == 0) found.kvh = -1;
   __syncthreads();
   const int rows_a_block = kColumns / rep;
+  auto blocks_of = [&](int e) { return e >= n_prefixes ? 1 : kPrefixes ? ceil_div(count[e], rows_a_block) : 0; };
   const int entries = n_prefixes + batch, per = ceil_div(entries, kThreads);
   const int e0 = min(t * per, entries), e1 = min(e0 + per, entries);
   int sum = 0, units = 0;
   for (int e = e0; e < e1; e++) {
-    const int blocks = e < n_prefixes ? ceil_div(count[e], rows_a_block) : 1;
+    const int blocks = blocks_of(e);
     sum += blocks * tiles[e];
     units += blocks;
   }
@@ -614,7 +626,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(const int32_t
   int pieces = 0, of_prefixes = 0;
   for (int e = e0; e < e1; e++) {
     const int ranges = max(1, ceil_div(tiles[e], share));
-    const int blocks = e < n_prefixes ? ceil_div(count[e], rows_a_block) : 1;
+    const int blocks = blocks_of(e);
     pieces += n_kv * blocks * ranges;
     if (e < n_prefixes) of_prefixes += n_kv * blocks * ranges;
   }
@@ -635,7 +647,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(const int32_t
   if (number >= before && number < before + pieces) {
     for (int e = e0; e < e1; e++) {
       const int ranges = max(1, ceil_div(tiles[e], share));
-      const int blocks = e < n_prefixes ? ceil_div(count[e], rows_a_block) : 1;
+      const int blocks = blocks_of(e);
       const int own = n_kv * blocks * ranges;
       if (number < before + own) {
         Piece p;
@@ -684,7 +696,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(const int32_t
   int n_members = 1, n_tiles, len;
   const int32_t* table;
   bool whole = false;
-  if (p.prefix >= 0) {
+  if (kPrefixes && p.prefix >= 0) {
     const int per_row = ceil_div(batch, kThreads);
     const int r0 = min(t * per_row, batch), r1 = min(r0 + per_row, batch);
     int mine = 0;
@@ -705,7 +717,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(const int32_t
             at[2] = p.first;
             at[3] = p.ranges;
             at[4] = p.blocks;
-            at[5] = p.block * kColumns + rank * rep;
+            at[5] = p.block * a.block + rank * rep;
           }
         }
         rank++;
@@ -738,10 +750,449 @@ __global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(const int32_t
   if (p.slot >= (p.prefix >= 0 ? a.prefix_slots : a.own_slots)) return;  // (cannot be, unless lengths change meanwhile)
   const int tile0 = (int)((int64_t)n_tiles * p.range / p.ranges), tile1 = (int)((int64_t)n_tiles * (p.range + 1) / p.ranges);
   const int columns = n_members * rep;
-  if (columns <= 16)
+  if (!kPrefixes || columns <= 16)
     attend_piece<QDT, FMT, SDT, 1>(a, p, table, len, tile0, tile1, n_kv, rep, columns, whole, members, lds);
-  else
+  else if constexpr (kPrefixes)
     attend_piece<QDT, FMT, SDT, 2>(a, p, table, len, tile0, tile1, n_kv, rep, columns, whole, members, lds);
+}
+
+// ---------------------------------------------------------------------------------------------- prefixes of 16-bit rows
+
+constexpr int kRowBytes = kD * 2;
+constexpr int kTileBytes = kTileKeys * kRowBytes;  // 16 KB, K and V each
+constexpr int kStageBytes = 2 * kTileBytes;
+constexpr int kStages = 4;                         // tiles of the ring
+constexpr int kWideLds = kStages * kStageBytes;    // 128 KB
+constexpr int kChunk = 30;                         // tiles whose pages a wave has at hand, with two more behind them
+static_assert(kWideLds >= 3 * kMaxRows * 4, "the plan fits into the ring");
+
+__device__ const uint32_t g_no_rows[kRowBytes / 4] = {};  // what half tiles without rows are copied from
+
+template <int FMT>
+__device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
+  if constexpr (FMT == MSPR_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+template <int N>
+__device__ __forceinline__ void wait_copies_and_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+// Lane i's 16 bytes at base + offset land at lds_base + 16 i. In an asm statement, so that the compiler does not wait for it in
+// front of other LDS reads (s_nop: an instruction has to lie between the scalar write of M0 and the copy).
+__device__ __forceinline__ void copy_16(uint64_t base, uint32_t offset, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %0" ::"s"(base), "v"(offset), "s"(lds_base) : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t lds_address(const unsigned char* p) {
+  return (uint32_t)(uintptr_t)MSPR_LDS_PTR(const unsigned char, p);
+}
+// Sixteen-byte piece p of tile row r lies at place (p & 16) | ((p ^ swizzle(r)) & 15): neither the K operand's reads (lane = row) nor the
+// transposed ones of V meet a bank twice.
+__device__ __forceinline__ int swizzle(int r) { return ((r & 7) << 1) | ((r >> 3) & 1); }
+
+// One piece: `columns` columns (head rows of q in `column_row`) over tiles [tile0, tile1). KS tiles at a time: wave w has columns 32 (w %
+// (8 / KS)) on and every KS-th tile.
+template <int FMT, int KS>
+__device__ __forceinline__ void prefix_piece(const SharedRest& a, const int32_t* table, int len, int tile0, int tile1, int n_kv, int kvh,
+                                             int slot, int columns, const int* column_row, unsigned char* lds, float (*xml)[32][2]) {
+  constexpr float kLag = 4.0f;                              // (as in paged_decode.hip)
+  constexpr float kUp = FMT == MSPR_F16 ? 11.0f : 0.0f;
+  constexpr int kAhead = 2 / KS;                            // steps whose copies are under way behind the present one
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 31, g = lane >> 5;  // column within the wave's; key of the K operand
+  constexpr int kColumnWaves = kWideWaves / KS;
+  const int column0 = 32 * (wave % kColumnWaves), part = wave / kColumnWaves;
+  const int mine = __builtin_amdgcn_readfirstlane(min(max(columns - column0, 0), 32));  // columns of this wave
+  const int page_mask = (1 << a.page_shift) - 1;
+
+  // ---- copies: a thread has row tid / 32 of both half tiles of 16 keys, of K and of V
+  const int c_row = tid >> 5;
+  const int c_piece = (tid & 16) | ((tid ^ swizzle(c_row)) & 15);  // (row 16 + c_row has the same swizzle)
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds)) + wave * 1024;
+  auto load_ids = [&](int t0) {  // lane i: page of half tile i from tile t0 on
+    const int t = t0 + (lane >> 1), key = t * kTileKeys + 16 * (lane & 1);
+    const int e = t < tile1 && key < len ? key >> a.page_shift : -1;
+    return e >= 0 ? table[e] : -1;
+  };
+  // Rows of tile t that count, of its first half and (from bit 8 on) of its second. Rows behind them are copies of the last: they
+  // are masked, and must not be what is no number where that is not.
+  auto issue_tile = [&](int ids, int t0, int t, int stage) {
+    uint32_t rows = 0;
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const int page = __builtin_amdgcn_readlane(ids, 2 * (t - t0) + u);
+      const int key = t * kTileKeys + 16 * u;
+      const bool good = page >= 0 && page < a.n_pages && t < tile1;
+      const int count = !good ? 0 : len - key >= 16 ? 16 : len - key < 0 ? 0 : len - key;
+      const int64_t row = ((((int64_t)(good ? page : 0) * n_kv + kvh) << a.page_shift) + (key & page_mask));
+      const uint64_t none = (uint64_t)(const void*)g_no_rows;
+      const uint64_t kb = count > 0 ? (uint64_t)a.k + row * kRowBytes : none, vb = count > 0 ? (uint64_t)a.v + row * kRowBytes : none;
+      const uint32_t offset = (uint32_t)(min(c_row, max(count, 1) - 1) * kRowBytes + c_piece * 16);
+      const uint32_t to = lds0 + stage * kStageBytes + u * 8192;
+      copy_16(kb, offset, to);
+      copy_16(vb, offset, to + kTileBytes);
+      rows |= (uint32_t)count << 8 * u;
+    }
+    return rows;
+  };
+  uint32_t ahead[kAhead + 1];  // rows of this wave's tile in the steps under way
+  auto issue_step = [&](int ids, int t0, int step) {
+    uint32_t rows = 0;
+#pragma unroll
+    for (int i = 0; i < KS; i++) {
+      const int t = tile0 + step * KS + i;
+      const uint32_t r = issue_tile(ids, t0, t, (step * KS + i) % kStages);
+      if (i == part) rows = r;
+    }
+    return rows;
+  };
+  const int n_steps = __builtin_amdgcn_readfirstlane((tile1 - tile0 + KS - 1) / KS);
+  int ids = load_ids(tile0);
+#pragma unroll
+  for (int i = 0; i < kAhead; i++) ahead[i] = issue_step(ids, tile0, i);
+  int ids_next = load_ids(tile0 + kChunk);
+
+  // ---- Q^T operand: lane (n, g) holds q[column][16 s + 8 g ...] for step s. The wave's rows come in halves of 128 channels, in whole
+  //      runs of 256 bytes, and change lanes in 8 KB of LDS that no tile uses yet (piece p of row r at p ^ (r & 15)).
+  u32x4_t qf[16];
+  {
+    const int xr = lane / 16, xc = lane % 16;
+    u32x4_t raw[2][8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int column = column0 + 4 * i + xr;
+      const int64_t row = column_row[column < columns ? column : 0];
+#pragma unroll
+      for (int h = 0; h < 2; h++) raw[h][i] = reinterpret_cast<const u32x4_t*>(a.q)[row * 32 + h * 16 + xc];
+    }
+    unsigned char* xq = lds + 2 * kStageBytes + (wave << 13);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) *reinterpret_cast<u32x4_t*>(xq + (4 * i + xr) * 256 + 16 * (xc ^ ((4 * i + xr) & 15))) = raw[h][i];
+#pragma unroll
+      for (int s = 0; s < 8; s++) qf[8 * h + s] = *reinterpret_cast<const u32x4_t*>(xq + n * 256 + 16 * ((2 * s + g) ^ (n & 15)));
+    }
+#pragma unroll
+    for (int s = 0; s < 16; s++) asm volatile("" : "+v"(qf[s]));
+  }
+
+  f32x16_t oacc[8];
+#pragma unroll
+  for (int mt = 0; mt < 8; mt++) oacc[mt] = f32x16_t{0};
+  float m_run = -__builtin_inff(), l_run = 0.0f;
+
+  const int k_off = n * kRowBytes + 32 * (n & 7) + 16 * (g ^ ((n >> 3) & 1));
+  const int tr_s = lane & 15;
+  const int tr_row = 4 * g + (tr_s >> 2);                          // + 8 h + 16 half
+  const int tr_piece = 2 * ((lane >> 4) & 1) + ((tr_s & 3) >> 1);  // of the 64 bytes that 32 channels take
+  int v_off[2];
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const int r = tr_row + 8 * h;
+    v_off[h] = kTileBytes + r * kRowBytes + 16 * ((tr_piece ^ swizzle(r)) & 15) + 8 * (tr_s & 1);
+  }
+
+  auto attend_tile = [&](const unsigned char* st, uint32_t rows) {
+    // ---- S^T = K . Q^T: register i is key 8 (i / 4) + 4 g + i % 4
+    f32x16_t s = f32x16_t{0};
+    {
+      constexpr int kReadAhead = 4;
+      const uint32_t kb = lds_address(st) + (uint32_t)k_off;
+      u32x4_t af[16];
+#pragma unroll
+      for (int j = 0; j < 16; j++)
+        af[j] = *MSPR_LDS_PTR(const u32x4_t, (uintptr_t)((kb ^ (uint32_t)((j & 7) << 5)) + (uint32_t)((j >> 3) * 256)));
+#pragma unroll
+      for (int j = 0; j < 16; j++) s = mfma32<FMT>(af[j], qf[j], s);
+      __builtin_amdgcn_sched_group_barrier(0x100, kReadAhead, 0);  // LDS reads
+#pragma unroll
+      for (int j = 0; j < 16 - kReadAhead; j++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix instructions
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, kReadAhead, 0);
+    }
+    // ---- online softmax
+    float tmax = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < 16; i++) s[i] *= a.scale_log2;
+    if (rows != 0x1010u) {
+      const int first = (int)(rows & 0xFFu) - 4 * g, second = (int)(rows >> 8) - 4 * g;
+#pragma unroll
+      for (int i = 0; i < 16; i++)
+        if (8 * ((i & 7) / 4) + i % 4 >= (i < 8 ? first : second)) s[i] = -__builtin_inff();
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i++) tmax = fmaxf(tmax, s[i]);
+    tmax = half_wave_max(tmax);
+    const bool grow = tmax > m_run + kLag;
+    if (__any(grow)) {
+      const float m_new = grow ? tmax : m_run;
+      const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+      l_run *= alpha;
+      m_run = m_new;
+#pragma unroll
+      for (int mt = 0; mt < 8; mt++) oacc[mt] = oacc[mt] * alpha;
+    }
+    const float m_safe = (m_run == -__builtin_inff() ? 0.0f : m_run) - kUp;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      s[i] = __builtin_amdgcn_exp2f(s[i] - m_safe);
+      l_run += s[i];
+    }
+    // ---- O^T += V^T . P^T, half a tile at a time (of whose weights only one half's terms take registers then)
+    const uint32_t vb0 = lds_address(st) + (uint32_t)v_off[0], vb1 = lds_address(st) + (uint32_t)v_off[1];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      constexpr int kReadAhead = 3;
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) p[i] = s[8 * h + i];
+      u32x4_t pf[2];
+      split_terms<FMT, 2>(p, pf);
+      u32x4_t vf[8];
+#pragma unroll
+      for (int mt = 0; mt < 8; mt++) {
+        const uint32_t lo_a = (vb0 ^ (uint32_t)((mt & 3) << 6)) + (uint32_t)((mt >> 2) * 256 + h * 16 * kRowBytes);
+        const uint32_t hi_a = (vb1 ^ (uint32_t)((mt & 3) << 6)) + (uint32_t)((mt >> 2) * 256 + h * 16 * kRowBytes);
+        const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, (uintptr_t)lo_a)));
+        const u32x2_t hi = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, (uintptr_t)hi_a)));
+        vf[mt] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
+      }
+#pragma unroll
+      for (int mt = 0; mt < 8; mt++) {
+        oacc[mt] = mfma32<FMT>(vf[mt], pf[0], oacc[mt]);
+        oacc[mt] = mfma32<FMT>(vf[mt], pf[1], oacc[mt]);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * kReadAhead, 0);
+#pragma unroll
+      for (int i = 0; i < 8 - kReadAhead; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 2 * kReadAhead, 0);
+    }
+  };
+
+  for (int s0 = 0; s0 < n_steps; s0 += kChunk / KS) {
+    const int s_end = min(s0 + kChunk / KS, n_steps), t0 = tile0 + s0 * KS;
+    for (int step = s0; step < s_end; step++) {
+      // This step's tiles have landed once the wave's copies of them have (four a tile, in order) and every wave got here; the
+      // stages of the step before are free then.
+      wait_copies_and_barrier<4 * KS * (kAhead - 1)>();
+      ahead[kAhead] = issue_step(ids, t0, step + kAhead);  // (behind the last, tiles without rows: what is under way is the same)
+      const uint32_t rows = ahead[0];
+#pragma unroll
+      for (int i = 0; i < kAhead; i++) ahead[i] = ahead[i + 1];
+      if (mine > 0 && rows != 0) attend_tile(lds + ((step * KS + part) % kStages) * kStageBytes, rows);
+    }
+    ids = ids_next;
+    ids_next = load_ids(t0 + 2 * kChunk);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the last copies must not outlive the piece)
+
+  // ---- the waves of one block of columns meet in LDS; rows of the partial leave in whole runs, through 16 KB a wave
+  l_run += __shfl_xor(l_run, 32, MSPR_WAVE);
+  __syncthreads();  // every wave has left the tiles
+  int tl = tid;
+  asm volatile("" : "+v"(tl));  // (the offsets below are made here, not carried through the tile loop)
+  const int en = tl & 31, eg = (tl >> 5) & 1;
+  if constexpr (KS == 2) {
+    f32x4_t* xo = reinterpret_cast<f32x4_t*>(lds + (wave % kColumnWaves) * 32768) + (tl & 63);  // [32 quads][64 lanes]
+    if (part == 1 && mine > 0) {
+#pragma unroll
+      for (int mt = 0; mt < 8; mt++)
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+          xo[64 * (4 * mt + c)] = f32x4_t{oacc[mt][4 * c], oacc[mt][4 * c + 1], oacc[mt][4 * c + 2], oacc[mt][4 * c + 3]};
+      if (eg == 0) {
+        xml[wave % kColumnWaves][en][0] = m_run;
+        xml[wave % kColumnWaves][en][1] = l_run;
+      }
+    }
+    __syncthreads();
+    if (part == 1 || mine == 0) return;
+    const float m2 = xml[wave][en][0], l2 = xml[wave][en][1];
+    const float m_all = fmaxf(m_run, m2), m_safe = m_all == -__builtin_inff() ? 0.0f : m_all;
+    const float w1 = __builtin_amdgcn_exp2f(m_run - m_safe), w2 = __builtin_amdgcn_exp2f(m2 - m_safe);
+    m_run = m_all;
+    l_run = l_run * w1 + l2 * w2;
+#pragma unroll
+    for (int mt = 0; mt < 8; mt++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const f32x4_t o = xo[64 * (4 * mt + c)];
+#pragma unroll
+        for (int i = 0; i < 4; i++) oacc[mt][4 * c + i] = oacc[mt][4 * c + i] * w1 + o[i] * w2;
+      }
+  }
+  if (mine == 0) return;
+  int row0 = slot * a.block + column0;  // (a scalar by hand: with the lanes' addresses below, the compiler takes it for one of each lane's)
+  asm volatile("" : "+s"(row0));
+  if (eg == 0 && en < mine) *reinterpret_cast<f32x2_t*>(a.ws_pre_ml + 2 * (int64_t)(row0 + en)) = f32x2_t{m_run, l_run};
+  unsigned char* xo = lds + (wave << (KS == 2 ? 15 : 14));  // (of two parts, where the wave's own exchange was)
+  const auto to = store_window(a.ws_pre + (int64_t)row0 * kD, mine * kD * 4);
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    if constexpr (KS == 2) __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int mt = 0; mt < 4; mt++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const f32x16_t& o = oacc[4 * h + mt];
+        *reinterpret_cast<f32x4_t*>(xo + en * 512 + 16 * ((8 * mt + 2 * c + eg) ^ (en & 15))) =
+            f32x4_t{o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]};
+      }
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const int r = 2 * i + eg;
+      const f32x4_t v = *reinterpret_cast<const f32x4_t*>(xo + r * 512 + 16 * (en ^ (r & 15)));
+      window_store<kStoreThrough>(to, r * kD * 4 + 512 * h + 16 * en, __builtin_bit_cast(u32x4_t, v));
+    }
+  }
+}
+
+// A piece of a prefix a workgroup.
+template <int FMT>
+__global__ __launch_bounds__(kWideThreads, 1) void paged_prefix_kernel(const int32_t* requests, const int32_t* groups,
+                                                                       const int32_t* prefix_lens, int batch, int n_prefixes,
+                                                                       int n_tables, int n_kv, int rep, SharedRest a) {
+  extern __shared__ __attribute__((aligned(256))) unsigned char lds[];  // tile bases: zero low bits under the address XORs
+  __shared__ int wave_sums[2][kWideWaves];
+  __shared__ int column_row[kWideColumns];
+  __shared__ float xml[kWideWaves / 2][32][2];
+  __shared__ Piece found;
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int number = blockIdx.x;
+
+  // ---- the plan: members of every prefix, tiles, the length of a range
+  int* row_group = reinterpret_cast<int*>(lds);  // [batch]
+  int* tiles = row_group + kMaxRows;             // [n_prefixes]
+  int* count = tiles + kMaxRows;                 // [n_prefixes]
+  const int prefix_cap = a.prefix_width << a.page_shift;
+  for (int i = t; i < n_prefixes; i += kWideThreads) {
+    tiles[i] = ceil_div(length_of(prefix_lens, n_prefixes, i, prefix_cap), kTileKeys);
+    count[i] = 0;
+  }
+  if (t == 0) found.kvh = -1;
+  __syncthreads();
+  for (int r = t; r < batch; r += kWideThreads) {
+    const int request = requests ? requests[r] : r;
+    int group = request >= 0 && request < n_tables ? groups[request] : -1;
+    if (group < 0 || group >= n_prefixes || tiles[group] == 0) group = -1;
+    row_group[r] = group;
+    if (group >= 0) atomicAdd(&count[group], 1);
+  }
+  __syncthreads();
+  const int most = a.block / rep;  // members of a block
+  const int per = ceil_div(n_prefixes, kWideThreads);
+  const int e0 = min(t * per, n_prefixes), e1 = min(e0 + per, n_prefixes);
+  auto total = [&](int v, int which) {
+    const int sum = wave_scan(v);
+    if (lane == 63) wave_sums[which][wave] = sum;
+    return sum;
+  };
+  int sum = 0, units = 0;
+  for (int e = e0; e < e1; e++) {
+    const int blocks = ceil_div(count[e], most);
+    sum += blocks * tiles[e];
+    units += blocks;
+  }
+  total(sum, 0);
+  total(units, 1);
+  __syncthreads();
+  int all = 0, all_units = 0;
+#pragma unroll
+  for (int w = 0; w < kWideWaves; w++) {
+    all += wave_sums[0][w];
+    all_units += wave_sums[1][w];
+  }
+  all = __builtin_amdgcn_readfirstlane(all) * n_kv;
+  all_units = __builtin_amdgcn_readfirstlane(all_units) * n_kv;
+  if (all == 0) return;
+  const int share = max(kMinShare, ceil_div(all, max(kGroups - all_units, kGroups / 2)));
+  int pieces = 0;
+  for (int e = e0; e < e1; e++) pieces += n_kv * ceil_div(count[e], most) * ceil_div(tiles[e], share);
+  __syncthreads();
+  int before = total(pieces, 0) - pieces;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWideWaves; w++)
+    if (w < wave) before += wave_sums[0][w];
+  if (number >= before && number < before + pieces) {
+    for (int e = e0; e < e1; e++) {
+      const int blocks = ceil_div(count[e], most), ranges = ceil_div(tiles[e], share);
+      const int own = n_kv * blocks * ranges;
+      if (number < before + own) {
+        const int i = number - before, bundles = n_kv * ranges;
+        const int q = i / (8 * blocks), j = i - 8 * blocks * q, m = min(8, bundles - 8 * q);
+        const int bundle = 8 * q + j % m;
+        Piece p;
+        p.prefix = e;
+        p.row = 0;
+        p.block = j / m;
+        p.blocks = blocks;
+        p.kvh = bundle / ranges;
+        p.range = bundle - p.kvh * ranges;
+        p.ranges = ranges;
+        p.first = before;
+        p.slot = number;
+        found = p;
+        break;
+      }
+      before += own;
+    }
+  }
+  __syncthreads();
+  const int kvh = __builtin_amdgcn_readfirstlane(found.kvh);
+  if (kvh < 0 || number >= a.prefix_slots) return;  // (more workgroups than pieces)
+  const int prefix = __builtin_amdgcn_readfirstlane(found.prefix);
+  const int block = __builtin_amdgcn_readfirstlane(found.block), blocks = __builtin_amdgcn_readfirstlane(found.blocks);
+  const int range = __builtin_amdgcn_readfirstlane(found.range), ranges = __builtin_amdgcn_readfirstlane(found.ranges);
+
+  // ---- its queries: members block by block, as many in each as it takes to have them about equal
+  const int members = __builtin_amdgcn_readfirstlane(count[prefix]);
+  const int a_block = ceil_div(members, blocks);
+  const int n_members = min(a_block, members - block * a_block);
+  const int n_tiles = __builtin_amdgcn_readfirstlane(tiles[prefix]);
+  {
+    const int per_row = ceil_div(batch, kWideThreads);
+    const int r0 = min(t * per_row, batch), r1 = min(r0 + per_row, batch);
+    int mine = 0;
+    for (int r = r0; r < r1; r++) mine += row_group[r] == prefix;
+    int rank = total(mine, 1) - mine - block * a_block;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWideWaves; w++)
+      if (w < wave) rank += wave_sums[1][w];
+    for (int r = r0; r < r1; r++)
+      if (row_group[r] == prefix) {
+        if (rank >= 0 && rank < a_block) {
+          for (int h = 0; h < rep; h++) column_row[rank * rep + h] = (r * n_kv + kvh) * rep + h;
+          if (range == 0) {
+            int32_t* at = a.parts + 8 * ((int64_t)r * n_kv + kvh);
+            at[2] = found.first;
+            at[3] = ranges;
+            at[4] = blocks;
+            at[5] = block * a.block + rank * rep;
+          }
+        }
+        rank++;
+      }
+  }
+  const int len = __builtin_amdgcn_readfirstlane(length_of(prefix_lens, n_prefixes, prefix, prefix_cap));
+  const int32_t* table = a.prefix_tables + (int64_t)prefix * a.prefix_width;
+  __syncthreads();  // (the plan lies where the tiles will be)
+  const int tile0 = __builtin_amdgcn_readfirstlane((int)((int64_t)n_tiles * range / ranges));
+  const int tile1 = __builtin_amdgcn_readfirstlane((int)((int64_t)n_tiles * (range + 1) / ranges));
+  const int columns = __builtin_amdgcn_readfirstlane(n_members * rep);
+  if (columns <= kWideColumns / 2) prefix_piece<FMT, 2>(a, table, len, tile0, tile1, n_kv, kvh, number, columns, column_row, lds, xml);
+  else prefix_piece<FMT, 1>(a, table, len, tile0, tile1, n_kv, kvh, number, columns, column_row, lds, xml);
 }
 
 constexpr int kAtOnce = 16;  // pieces that a wave joins at a time
@@ -752,7 +1203,7 @@ constexpr int kMergeWaves = 8;
 template <int ODT, int WAVES>
 __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(const int32_t* parts, const float* ws_pre,
                                                                               const float* ws_pre_ml, const float* ws_own,
-                                                                              const float* ws_own_ml, int rep, int n_kv, int heads,
+                                                                              const float* ws_own_ml, int rep, int n_kv, int heads, int block,
                                                                               int prefix_slots, int own_slots, void* out) {
   __shared__ __attribute__((aligned(16))) float xo[kMergeWaves][kD + 2];
   const int lane = threadIdx.x & 63;
@@ -773,8 +1224,8 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
       const int s = own_first + i;
       return s >= 0 && s < own_slots ? s : 0;
     }
-    col = column % kColumns;
-    const int s = pre_first + bundle_piece(kvh * ranges + (i - n_own), column / kColumns, n_kv * ranges, blocks);
+    col = column % block;
+    const int s = pre_first + bundle_piece(kvh * ranges + (i - n_own), column / block, n_kv * ranges, blocks);
     return s >= 0 && s < prefix_slots ? s : 0;
   };
   float m = -__builtin_inff(), l = 0.0f;
@@ -786,7 +1237,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
       int col;
       const int s = slot_of(mine, col);
       stat = mine < n_own ? *reinterpret_cast<const f32x2_t*>(ws_own_ml + ((int64_t)s * 16 + col) * 2)
-                          : *reinterpret_cast<const f32x2_t*>(ws_pre_ml + ((int64_t)s * kColumns + col) * 2);
+                          : *reinterpret_cast<const f32x2_t*>(ws_pre_ml + ((int64_t)s * block + col) * 2);
     }
     f32x4_t ov[kAtOnce];
 #pragma unroll
@@ -794,7 +1245,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
       if (p0 + WAVES * j < total) {
         int col;
         const int s = slot_of(p0 + WAVES * j, col);
-        const float* from = p0 + WAVES * j < n_own ? ws_own + ((int64_t)s * rep + col) * kD : ws_pre + ((int64_t)s * kColumns + col) * kD;
+        const float* from = p0 + WAVES * j < n_own ? ws_own + ((int64_t)s * rep + col) * kD : ws_pre + ((int64_t)s * block + col) * kD;
         ov[j] = *reinterpret_cast<const f32x4_t*>(from + 4 * lane);
       }
     float m_new = stat.x;
@@ -842,52 +1293,76 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
   if (total > 0) store_out<ODT>(out, ((int64_t)row * rep + hn) * kD + 4 * lane, o, l);
 }
 
-// Units of a call, at most: blocks of members (every prefix may have one that is not full) and queries, of every KV head.
-int64_t shared_units(int batch, int n_prefixes, int n_kv, int rep) {
-  const int rows_a_block = kColumns / rep;
-  const int used = n_prefixes < batch ? n_prefixes : batch;
-  return (int64_t)n_kv * ((batch + (int64_t)used * (rows_a_block - 1)) / rows_a_block + batch);
+// Columns of a block of members. Of 8-bit rows 32; of 16-bit ones as many as eight waves hold, but no more than twice what a prefix
+// has members on the average, so that the scratch, a place for every column of a block, does not grow with what blocks leave empty.
+int block_columns(int batch, int n_prefixes, int rep, bool codes) {
+  if (codes) return kColumns;
+  const int64_t used = n_prefixes < batch ? n_prefixes : batch;
+  const int64_t mean = ((used > 1 ? 2 : 1) * (int64_t)batch * rep + used - 1) / used;
+  const int64_t n = (mean + 31) / 32 * 32;
+  return (int)(n < kWideColumns ? n : kWideColumns);
 }
 
-// Pieces: a call has at most max(kGroups, kGroups / 2 + units), see `share`.
-int64_t shared_pieces(int batch, int n_prefixes, int n_kv, int rep) {
-  const int64_t n = kGroups / 2 + shared_units(batch, n_prefixes, n_kv, rep);
-  return n > kGroups ? n : kGroups;
+// Pieces of `units` units: a call has at most max(kGroups, kGroups / 2 + units), see `share`.
+int64_t pieces_of(int64_t units) { return kGroups / 2 + units > kGroups ? kGroups / 2 + units : kGroups; }
+
+// Blocks of members, at most (every prefix may have one that is not full), of every KV head.
+int64_t prefix_units(int batch, int n_prefixes, int n_kv, int rep, int block) {
+  const int rows_a_block = block / rep;
+  const int used = n_prefixes < batch ? n_prefixes : batch;
+  return (int64_t)n_kv * ((batch + (int64_t)used * (rows_a_block - 1)) / rows_a_block);
 }
 
 struct SharedScratch {
-  int64_t prefix_slots, own_slots;  // every query has a piece of its own, at least
+  int block;
+  int64_t pieces, prefix_pieces;           // workgroups of the two kernels (8-bit rows: of the one)
+  int64_t prefix_slots, own_slots;         // places for partials
   size_t pre, pre_ml, own, own_ml, parts;  // bytes
   size_t total() const { return pre + pre_ml + own + own_ml + parts; }
 };
-SharedScratch shared_scratch(int batch, int n_prefixes, int n_kv, int rep) {
+SharedScratch shared_scratch(int batch, int n_prefixes, int n_kv, int rep, bool codes) {
   SharedScratch s;
-  const int64_t pieces = shared_pieces(batch, n_prefixes, n_kv, rep), own = (int64_t)batch * n_kv;
-  s.prefix_slots = pieces > own ? pieces - own : 0;
-  s.own_slots = kGroups / 2 + own > kGroups ? kGroups / 2 + own : kGroups;
-  s.pre = (size_t)s.prefix_slots * kColumns * kD * sizeof(float);
-  s.pre_ml = (size_t)s.prefix_slots * kColumns * 2 * sizeof(float);
+  s.block = block_columns(batch, n_prefixes, rep, codes);
+  const int64_t own = (int64_t)batch * n_kv, blocks = prefix_units(batch, n_prefixes, n_kv, rep, s.block);
+  s.pieces = pieces_of(codes ? own + blocks : own);
+  s.prefix_pieces = codes ? 0 : pieces_of(blocks);
+  s.prefix_slots = codes ? s.pieces - own : s.prefix_pieces;  // (every query has a piece of its own, at least)
+  s.own_slots = pieces_of(own);
+  s.pre = (size_t)s.prefix_slots * s.block * kD * sizeof(float);
+  s.pre_ml = (size_t)s.prefix_slots * s.block * 2 * sizeof(float);
   s.own = (size_t)s.own_slots * rep * kD * sizeof(float);
   s.own_ml = (size_t)s.own_slots * 16 * 2 * sizeof(float);
   s.parts = (size_t)own * 8 * sizeof(int32_t);
   return s;
 }
 
+// The LDS of a kernel beyond what every launch may have, asked for once a device.
+template <typename K>
+int reserve_lds(K* kernel, int bytes, bool (&done)[64]) {
+  int device = 0;
+  if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64 || !done[device]) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) {
+      mspr_set_error("sdpa_decode_paged_shared: cannot reserve %d bytes of LDS: %s", bytes, hipGetErrorString(e));
+      return MSPR_ERR_LAUNCH;
+    }
+    if (device >= 0 && device < 64) done[device] = true;
+  }
+  return MSPR_OK;
+}
+
 template <int QDT, int FMT, int SDT>
 int shared_launch(const SharedArgs& a, hipStream_t st) {
   constexpr int kLds = shared_lds(QDT, FMT);
-  static bool attr_set[64] = {};  // by device
-  int device = 0;
-  if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64 || !attr_set[device]) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_shared_kernel<QDT, FMT, SDT>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-    if (e != hipSuccess) {
-      mspr_set_error("sdpa_decode_paged_shared: cannot reserve %d bytes of LDS: %s", kLds, hipGetErrorString(e));
-      return MSPR_ERR_LAUNCH;
-    }
-    if (device >= 0 && device < 64) attr_set[device] = true;
-  }
+  static bool reserved[2][64] = {};
   const SharedRest& r = a.rest;
+  if constexpr (FMT != kAffine) {
+    if (int rc = reserve_lds(&paged_prefix_kernel<FMT>, kWideLds, reserved[0])) return rc;
+    paged_prefix_kernel<FMT><<<dim3((unsigned)a.prefix_pieces), dim3(kWideThreads), kWideLds, st>>>(
+        a.requests, a.groups, a.prefix_lens, a.batch, a.n_prefixes, a.n_tables, a.n_kv, a.rep, r);
+    MSPR_CHECK_LAUNCH("sdpa_decode_paged_shared (prefixes)");
+  }
+  if (int rc = reserve_lds(&paged_shared_kernel<QDT, FMT, SDT>, kLds, reserved[1])) return rc;
   paged_shared_kernel<QDT, FMT, SDT><<<dim3((unsigned)a.pieces), dim3(kThreads), kLds, st>>>(
       a.requests, a.groups, a.lens, a.prefix_lens, a.batch, a.n_prefixes, a.n_tables, a.n_kv, a.rep, r);
   MSPR_CHECK_LAUNCH("sdpa_decode_paged_shared");
@@ -895,7 +1370,7 @@ int shared_launch(const SharedArgs& a, hipStream_t st) {
   auto merge = [&](auto waves) {
     constexpr int kWavesAHead = decltype(waves)::value, kHeads = kMergeWaves / kWavesAHead;
     paged_shared_merge_kernel<QDT, kWavesAHead><<<dim3((unsigned)((heads + kHeads - 1) / kHeads)), dim3(64 * kMergeWaves), 0, st>>>(
-        r.parts, r.ws_pre, r.ws_pre_ml, r.ws_own, r.ws_own_ml, a.rep, a.n_kv, heads, r.prefix_slots, r.own_slots, r.out);
+        r.parts, r.ws_pre, r.ws_pre_ml, r.ws_own, r.ws_own_ml, a.rep, a.n_kv, heads, r.block, r.prefix_slots, r.own_slots, r.out);
   };
   // (a head has as many pieces as compute units divided by blocks: few where heads are many)
   if (heads <= 1024) merge(std::integral_constant<int, 8>{});
@@ -904,7 +1379,7 @@ int shared_launch(const SharedArgs& a, hipStream_t st) {
   return MSPR_OK;
 }
 
-int shared_fill(const char* what, SharedArgs& a, const void* q, const void* k, const void* v, const int32_t* prefix_tables,
+int shared_fill(const char* what, SharedArgs& a, bool codes, const void* q, const void* k, const void* v, const int32_t* prefix_tables,
                 const int32_t* prefix_lens, const int32_t* groups, const int32_t* tables, const int32_t* lens,
                 const int32_t* requests, int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_pages, int page_size,
                 int n_prefixes, int prefix_width, int n_tables, int table_width, float scale, void* out, void* workspace,
@@ -926,11 +1401,11 @@ int shared_fill(const char* what, SharedArgs& a, const void* q, const void* k, c
   const int rep = n_q_heads / n_kv_heads;
   const int64_t most = (int64_t)table_width * page_size > (int64_t)prefix_width * page_size ? (int64_t)table_width * page_size
                                                                                            : (int64_t)prefix_width * page_size;
-  MSPR_REQUIRE(shared_units(batch, n_prefixes, n_kv_heads, rep) * ((most + kTileKeys - 1) / kTileKeys + 1) <= 0x3FFFFFFF,
+  const SharedScratch s = shared_scratch(batch, n_prefixes, n_kv_heads, rep, codes);
+  MSPR_REQUIRE((prefix_units(batch, n_prefixes, n_kv_heads, rep, s.block) + (int64_t)batch * n_kv_heads) * ((most + kTileKeys - 1) / kTileKeys + 1) <= 0x3FFFFFFF,
                "%s: the tables hold too many tokens together", what);
   MSPR_REQUIRE(mspr_aligned(q, 16) && mspr_aligned(k, 16) && mspr_aligned(v, 16) && mspr_aligned(out, 16),
                "%s: pointers must be 16-byte aligned", what);
-  const SharedScratch s = shared_scratch(batch, n_prefixes, n_kv_heads, rep);
   MSPR_REQUIRE(workspace && workspace_bytes >= s.total() && mspr_aligned(workspace, 16),
                "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", what, s.total(), workspace_bytes);
   a = SharedArgs{};
@@ -943,7 +1418,8 @@ int shared_fill(const char* what, SharedArgs& a, const void* q, const void* k, c
   a.n_tables = n_tables;
   a.n_kv = n_kv_heads;
   a.rep = rep;
-  a.pieces = (int)shared_pieces(batch, n_prefixes, n_kv_heads, rep);
+  a.pieces = (int)s.pieces;
+  a.prefix_pieces = (int)s.prefix_pieces;
   SharedRest& r = a.rest;
   r.q = q;
   r.k = k;
@@ -956,6 +1432,7 @@ int shared_fill(const char* what, SharedArgs& a, const void* q, const void* k, c
   r.width = table_width;
   r.prefix_slots = (int)s.prefix_slots;
   r.own_slots = (int)s.own_slots;
+  r.block = s.block;
   r.scale_log2 = (float)((double)scale * 1.4426950408889634);
   uint8_t* at = reinterpret_cast<uint8_t*>(workspace);
   r.ws_pre = reinterpret_cast<float*>(at);
@@ -976,9 +1453,12 @@ int shared_q8_launch(const SharedArgs& a, int sb_dtype, hipStream_t st) {
 
 }  // namespace
 
+// (of both page formats, whichever needs more)
 extern "C" size_t mspr_sdpa_decode_paged_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int n_prefixes) {
   if (batch < 1 || n_kv_heads < 1 || n_q_heads < n_kv_heads || n_q_heads / n_kv_heads > 16 || n_prefixes < 1) return 0;
-  return shared_scratch(batch, n_prefixes, n_kv_heads, n_q_heads / n_kv_heads).total();
+  const size_t rows = shared_scratch(batch, n_prefixes, n_kv_heads, n_q_heads / n_kv_heads, false).total();
+  const size_t codes = shared_scratch(batch, n_prefixes, n_kv_heads, n_q_heads / n_kv_heads, true).total();
+  return rows > codes ? rows : codes;
 }
 
 extern "C" int mspr_sdpa_decode_paged_shared(const void* queries, const void* k_pages, const void* v_pages, int dtype,
@@ -989,7 +1469,7 @@ extern "C" int mspr_sdpa_decode_paged_shared(const void* queries, const void* k_
                                              void* out, void* workspace, size_t workspace_bytes, void* stream) {
   MSPR_REQUIRE(dtype == MSPR_F16 || dtype == MSPR_BF16, "sdpa_decode_paged_shared: dtype must be f16 or bf16");
   SharedArgs a;
-  if (int rc = shared_fill("sdpa_decode_paged_shared", a, queries, k_pages, v_pages, prefix_tables, prefix_lens, groups, tables,
+  if (int rc = shared_fill("sdpa_decode_paged_shared", a, false, queries, k_pages, v_pages, prefix_tables, prefix_lens, groups, tables,
                            lens, requests, batch, n_q_heads, n_kv_heads, head_dim, n_pages, page_size, n_prefixes, prefix_width,
                            n_tables, table_width, scale, out, workspace, workspace_bytes))
     return rc;
@@ -1013,7 +1493,7 @@ extern "C" int mspr_sdpa_decode_paged_shared_q8(const void* queries, int q_dtype
                    mspr_aligned(v_biases, 16),
                "sdpa_decode_paged_shared_q8: pointers must be 16-byte aligned");
   SharedArgs a;
-  if (int rc = shared_fill("sdpa_decode_paged_shared_q8", a, queries, k_wq, v_wq, prefix_tables, prefix_lens, groups, tables, lens,
+  if (int rc = shared_fill("sdpa_decode_paged_shared_q8", a, true, queries, k_wq, v_wq, prefix_tables, prefix_lens, groups, tables, lens,
                            requests, batch, n_q_heads, n_kv_heads, head_dim, n_pages, page_size, n_prefixes, prefix_width,
                            n_tables, table_width, scale, out, workspace, workspace_bytes))
     return rc;
