@@ -412,12 +412,13 @@ int mspr_sdpa_decode_paged_q8(const void* queries, int q_dtype, const void* k_wq
                               size_t workspace_bytes, void* stream);
 
 /* Scratch bytes of the two entry points below. */
-size_t mspr_sdpa_decode_paged_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int n_prefixes);
+size_t mspr_sdpa_decode_paged_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int page_size, int table_width,
+                                                     int n_prefixes);
 
 /* mspr_sdpa_decode_paged for requests that continue a shared prefix: out[b] is attention over the first prefix_lens[g] rows that
  * prefix_tables[g] (int32 [n_prefixes][prefix_width]) names, g = groups[request of b] (int32 [n_tables]; none of the prefixes:
  * no prefix), and the first lens[b] rows of the request's own table behind them. Rows of a prefix are read once for the members
- * of a group together (for as many query heads as 32 columns hold at a time). What lens, tables, requests and pages may hold is
+ * of a group together. What lens, tables, requests and pages may hold is
  * as there; all are read on the device. batch and n_prefixes <= 2048. */
 int mspr_sdpa_decode_paged_shared(const void* queries, const void* k_pages, const void* v_pages, int dtype,
                                   const int32_t* prefix_tables, const int32_t* prefix_lens, const int32_t* groups,

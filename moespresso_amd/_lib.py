@@ -152,7 +152,7 @@ SIGNATURES = {
         c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
                 c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p,
                 c_size_t, c_void_p]),
-    "mspr_sdpa_decode_paged_shared_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "mspr_sdpa_decode_paged_shared_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "mspr_sdpa_decode_paged_shared": (
         c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
                 c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
@@ -229,9 +229,11 @@ def paged_decode_workspace(batch: int, n_q_heads: int, n_kv_heads: int, page_siz
     return torch.empty((max(nbytes, 16) + 3) // 4, dtype=torch.float32, device=device)
 
 
-def paged_shared_workspace(batch: int, n_q_heads: int, n_kv_heads: int, n_prefixes: int, device) -> torch.Tensor:
+def paged_shared_workspace(batch: int, n_q_heads: int, n_kv_heads: int, page_size: int, table_width: int, n_prefixes: int,
+                           device) -> torch.Tensor:
     """Scratch tensor for the decode entry points over shared prefixes (partials of every piece, and which a query has)."""
-    nbytes = int(lib().mspr_sdpa_decode_paged_shared_workspace_bytes(int(batch), int(n_q_heads), int(n_kv_heads), int(n_prefixes)))
+    nbytes = int(lib().mspr_sdpa_decode_paged_shared_workspace_bytes(int(batch), int(n_q_heads), int(n_kv_heads), int(page_size),
+                                                                     int(table_width), int(n_prefixes)))
     return torch.empty((max(nbytes, 16) + 3) // 4, dtype=torch.float32, device=device)
 
 

@@ -936,8 +936,9 @@ bool shared_operands(PyObject* queries, PyObject* const* rest, const Pages& p, S
   if (d->R > 2048 || d->G < 1 || d->G > 2048 || d->width < 1 || d->width > INT32_MAX || d->prefix_lens->size(0) != d->G ||
       d->groups->size(0) != d->B || !here({d->q, d->prefix_tables, d->prefix_lens, d->groups}))
     return false;
-  return take_workspace(rest[7], mspr_sdpa_decode_paged_shared_workspace_bytes((int)d->R, (int)d->Hq, (int)p.heads, (int)d->G), *d->q,
-                        ws);
+  return take_workspace(rest[7], mspr_sdpa_decode_paged_shared_workspace_bytes((int)d->R, (int)d->Hq, (int)p.heads, (int)p.page, (int)d->P,
+                                                                               (int)d->G),
+                        *d->q, ws);
 }
 
 const int32_t* ints(const Tensor* t) { return (const int32_t*)at_or_null(t); }

@@ -34,7 +34,7 @@
 // it has fewer digits than one float16 term: the sums over codes and over biases, which take the weights apart, may be many
 // times the result (a key whose scale is 10^4 of the others' left results 1.8e-2 of the values' sum off; one term took 186 us
 // for 16 ragged requests where two take 193).
-#include "paged_rows.h"
+#include "paged_parts.h"
 
 namespace {
 
@@ -68,7 +68,9 @@ struct PagedRest {
   float* ws_ml;   // their statistics [2 shares][16][2]
   int32_t* cut;   // {row, its first share, its last share} of a row that was cut, row -1 of none: by row where there are no
                   // more of them than shares, else by the share that begins the row
-  void* out;      // [B, Hq, D]
+  void* out;      // [B, Hq, D]; or, where other keys of the same queries are joined with these,
+  float* own;     // [B * n_kv * rep][256] sums, relative to their reference maximum, of rows that are not cut (else null)
+  float* own_ml;  // [B * n_kv * rep][2]
 };
 
 struct PagedArgs {
@@ -624,7 +626,9 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
     float m_all = m_run, l_all = l_run;
     auto write = [&](int mt, f32x4_t acc) {
       if (n >= rep) return;
-      if (whole) store_out<QDT>(a.out, ((int64_t)row * rep + n) * kD + 16 * mt + 4 * g, acc, l_all);
+      const int64_t at = ((int64_t)row * rep + n) * kD + 16 * mt + 4 * g;
+      if (whole && a.own) *reinterpret_cast<f32x4_t*>(a.own + at) = acc;
+      else if (whole) store_out<QDT>(a.out, at, acc, l_all);
       else window_store<kStoreThrough>(po, (n * kD + 16 * mt + 4 * g) * 4, __builtin_bit_cast(u32x4_t, acc));
     };
     if constexpr (ALONE) {
@@ -665,6 +669,7 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
     }
     if (first_tile == 0 && g == 0) {
       if (!whole) *reinterpret_cast<f32x2_t*>(a.ws_ml + (part * 16 + n) * 2) = f32x2_t{m_all, l_all};
+      else if (a.own && n < rep) *reinterpret_cast<f32x2_t*>(a.own_ml + ((int64_t)row * rep + n) * 2) = f32x2_t{m_all, l_all};
       if (n == 0 && tile0 == 0 && (by_row || !whole)) {
         int32_t* c = a.cut + 3 * (int64_t)(by_row ? row : number);
         c[0] = whole ? -1 : row;
@@ -677,9 +682,6 @@ __global__ __launch_bounds__(64 * kWaves, FMT == kAffine && QDT != MSPR_F32 ? 2 
     else __syncthreads();
   }
 }
-
-// Where part i of a row lies whose first part is share `first`'s: that began the row, the others go on with it.
-__device__ __forceinline__ int64_t part_of(int first, int i) { return 2 * (int64_t)(first + i) + (i == 0 ? 1 : 0); }
 
 constexpr int kAtOnce = 16;  // parts that a wave joins at a time
 
@@ -722,9 +724,21 @@ struct Join {
   }
 };
 
+// A head's four channels: the result, or (with own_ml) what is joined with other keys.
+template <int ODT>
+__device__ __forceinline__ void store_joined(void* out, int64_t at, f32x4_t o, float m, float l, float* own_ml) {
+  const int lane = threadIdx.x & 63;
+  if (!own_ml) {
+    store_out<ODT>(out, at + 4 * lane, o, l);
+  } else {
+    *reinterpret_cast<f32x4_t*>(reinterpret_cast<float*>(out) + at + 4 * lane) = o;
+    if (lane == 0) *reinterpret_cast<f32x2_t*>(own_ml + at / kD * 2) = f32x2_t{m, l};
+  }
+}
+
 // Parts of a row that a workgroup's waves took every WAVES-th of, joined in LDS and written by the first wave.
 template <int ODT, int WAVES>
-__device__ __forceinline__ void join_waves(const Join& part, float (*xo)[kD + 2], void* out, int64_t at) {
+__device__ __forceinline__ void join_waves(const Join& part, float (*xo)[kD + 2], void* out, int64_t at, float* own_ml) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (lane == 0) {
@@ -748,20 +762,8 @@ __device__ __forceinline__ void join_waves(const Join& part, float (*xo)[kD + 2]
 #pragma unroll
     for (int i = 0; i < 4; i++) o_all[i] += xo[w][4 * lane + i] * wt;
   }
-  store_out<ODT>(out, at + 4 * lane, o_all, l_all);
+  store_joined<ODT>(out, at, o_all, m_all, l_all, own_ml);
 }
-
-// An entry of `cut`: a row and how many parts it has, none where no row was cut. (Bounded by the call's rows and shares,
-// whatever is there.)
-struct Cut {
-  int row, first, count;
-  __device__ __forceinline__ void load(const int32_t* cut, int entry, int rows, int shares) {
-    row = cut[3 * entry];
-    first = cut[3 * entry + 1];
-    const int last = min(cut[3 * entry + 2], shares - 1);
-    count = row < 0 || row >= rows || first < 0 || first > last ? 0 : last - first + 1;
-  }
-};
 
 // Joins the parts of one row that was cut, for one query head: eight waves take every eighth part.
 // grid: (rows, query heads of a KV head)
@@ -778,7 +780,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const int
   Join join;
   for (int p0 = wave; p0 < c.count; p0 += kAtOnce * kMergeWaves)
     join.add(ws_o, ws_ml, c.first, p0, kMergeWaves, c.count, rep, hn);
-  join_waves<ODT, kMergeWaves>(join, xo, out, ((int64_t)c.row * rep + hn) * kD);
+  join_waves<ODT, kMergeWaves>(join, xo, out, ((int64_t)c.row * rep + hn) * kD, nullptr);
 }
 
 // The same for many rows, of which most have few parts: a wave takes an entry, and the four of a workgroup together those of
@@ -787,7 +789,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const int
 template <int ODT>
 __global__ __launch_bounds__(64 * kWaves) void paged_merge_many_kernel(const int32_t* cut, const float* ws_o, const float* ws_ml,
                                                                        int rep, int rows, int shares, unsigned entries,
-                                                                       void* out) {
+                                                                       void* out, float* own_ml) {
   __shared__ __attribute__((aligned(16))) float xo[kWaves][kD + 2];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hn = blockIdx.y;
@@ -799,7 +801,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_merge_many_kernel(const int
   if (c.count > 0 && c.count <= kAtOnce) {
     Join join;
     join.add(ws_o, ws_ml, c.first, 0, 1, c.count, rep, hn);
-    store_out<ODT>(out, ((int64_t)c.row * rep + hn) * kD + 4 * (threadIdx.x & 63), join.o, join.l);
+    store_joined<ODT>(out, ((int64_t)c.row * rep + hn) * kD, join.o, join.m, join.l, own_ml);
   }
   __syncthreads();
 #pragma unroll 1
@@ -809,7 +811,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_merge_many_kernel(const int
     const int first = __builtin_amdgcn_readfirstlane(entry[w].first);
     Join join;
     for (int p0 = wave; p0 < count; p0 += kAtOnce * kWaves) join.add(ws_o, ws_ml, first, p0, kWaves, count, rep, hn);
-    join_waves<ODT, kWaves>(join, xo, out, ((int64_t)__builtin_amdgcn_readfirstlane(entry[w].row) * rep + hn) * kD);
+    join_waves<ODT, kWaves>(join, xo, out, ((int64_t)__builtin_amdgcn_readfirstlane(entry[w].row) * rep + hn) * kD, own_ml);
     __syncthreads();
   }
 }
@@ -861,11 +863,12 @@ int paged_launch_form(const PagedArgs& a, hipStream_t st) {
   // (rows of kMinTiles tiles are cut only where there are more of them than shares)
   const int rows = a.batch * a.n_kv;
   const bool more = ALONE && rows > kMaxGroups * kWaves;
+  if (r.own && !more) return MSPR_OK;  // (the caller joins the parts, which it finds row by row)
   if (row_tiles_most(cap) > kMinTiles || more) {
     if constexpr (ALONE) {
       const unsigned entries = (unsigned)(more ? shares : rows);
       paged_merge_many_kernel<QDT><<<dim3((entries + kWaves - 1) / kWaves, (unsigned)a.rep), dim3(64 * kWaves), 0, st>>>(
-          r.cut, r.ws_o, r.ws_ml, a.rep, rows, shares, entries, r.out);
+          r.cut, r.ws_o, r.ws_ml, a.rep, rows, shares, entries, r.own ? r.own : r.out, r.own_ml);
     } else {
       paged_merge_kernel<QDT><<<dim3((unsigned)rows, (unsigned)a.rep), dim3(64 * kMergeWaves), 0, st>>>(r.cut, r.ws_o, r.ws_ml, a.rep,
                                                                                                         rows, shares, r.out);
@@ -935,7 +938,42 @@ int paged_q8_launch(const PagedArgs& a, int sb_dtype, hipStream_t st) {
   return paged_launch<QDT, kAffine, MSPR_BF16>(a, st);
 }
 
+// The entry points' launches, of 16-bit rows and of 8-bit ones.
+int rows_launch(const PagedArgs& a, int dtype, hipStream_t st) {
+  if (dtype == MSPR_F16) return paged_launch<MSPR_F16, MSPR_F16, MSPR_F16>(a, st);
+  return paged_launch<MSPR_BF16, MSPR_BF16, MSPR_BF16>(a, st);
+}
+int codes_launch(const PagedArgs& a, int q_dtype, int sb_dtype, hipStream_t st) {
+  if (q_dtype == MSPR_F32) return paged_q8_launch<MSPR_F32>(a, sb_dtype, st);
+  if (q_dtype == MSPR_F16) return paged_q8_launch<MSPR_F16>(a, sb_dtype, st);
+  return paged_q8_launch<MSPR_BF16>(a, sb_dtype, st);
+}
+
 }  // namespace
+
+int mspr_paged_decode_parts(const char* what, const PagedPartsCall& c, PagedParts* parts, hipStream_t st) {
+  PagedArgs a;
+  if (int rc = paged_fill(what, a, c.q, c.k, c.v, c.tables, c.lens, c.requests, c.batch, c.rep * c.n_kv, c.n_kv, kD, c.n_pages,
+                          1 << c.page_shift, c.n_tables, c.width, 1.0f, c.own, c.workspace, c.workspace_bytes))
+    return rc;
+  a.rest.scale_log2 = c.scale_log2;
+  a.rest.k_scales = c.k_scales;
+  a.rest.k_biases = c.k_biases;
+  a.rest.v_scales = c.v_scales;
+  a.rest.v_biases = c.v_biases;
+  a.rest.own = c.own;
+  a.rest.own_ml = c.own_ml;
+  const int rows = c.batch * c.n_kv;
+  const int64_t cap = (int64_t)c.width << c.page_shift;
+  // (of more rows than shares parts are not found row by row, and have been joined; of rows that are never cut there are none)
+  const bool joined = paged_alone(c.batch, c.n_kv) ? rows > kMaxGroups * kWaves : false;
+  parts->cut = joined || row_tiles_most(cap) <= kMinTiles ? nullptr : a.rest.cut;
+  parts->o = a.rest.ws_o;
+  parts->ml = a.rest.ws_ml;
+  parts->shares = paged_shares(c.batch, c.n_kv, cap);
+  if (c.k_scales) return codes_launch(a, c.q_dtype, c.sb_dtype, st);
+  return rows_launch(a, c.q_dtype, st);
+}
 
 extern "C" size_t mspr_sdpa_decode_paged_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int page_size,
                                                          int table_width) {
@@ -953,8 +991,7 @@ extern "C" int mspr_sdpa_decode_paged(const void* queries, const void* k_pages, 
   if (int rc = paged_fill("sdpa_decode_paged", a, queries, k_pages, v_pages, tables, lens, requests, batch, n_q_heads, n_kv_heads,
                           head_dim, n_pages, page_size, n_tables, table_width, scale, out, workspace, workspace_bytes))
     return rc;
-  if (dtype == MSPR_F16) return paged_launch<MSPR_F16, MSPR_F16, MSPR_F16>(a, (hipStream_t)stream);
-  return paged_launch<MSPR_BF16, MSPR_BF16, MSPR_BF16>(a, (hipStream_t)stream);
+  return rows_launch(a, dtype, (hipStream_t)stream);
 }
 
 extern "C" int mspr_sdpa_decode_paged_q8(const void* queries, int q_dtype, const void* k_wq, const void* k_scales,
@@ -978,8 +1015,5 @@ extern "C" int mspr_sdpa_decode_paged_q8(const void* queries, int q_dtype, const
   a.rest.k_biases = k_biases;
   a.rest.v_scales = v_scales;
   a.rest.v_biases = v_biases;
-  hipStream_t st = (hipStream_t)stream;
-  if (q_dtype == MSPR_F32) return paged_q8_launch<MSPR_F32>(a, sb_dtype, st);
-  if (q_dtype == MSPR_F16) return paged_q8_launch<MSPR_F16>(a, sb_dtype, st);
-  return paged_q8_launch<MSPR_BF16>(a, sb_dtype, st);
+  return codes_launch(a, q_dtype, sb_dtype, (hipStream_t)stream);
 }

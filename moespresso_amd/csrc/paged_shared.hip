@@ -12,13 +12,14 @@
 // so that a piece falls to every compute unit; the number of a piece says what it is. Blocks of one range lie eight workgroups
 // apart, on one XCD, whose L2 then has the rows for the second block. A last kernel joins a query's pieces.
 //
-// Prefixes of 16-bit rows (paged_prefix_kernel): up to 256 columns a block. Tiles of 32 keys come by asynchronous copies into a
-// ring of LDS that eight waves share, 32 columns a wave: read from HBM once, from LDS by every wave (the layout and the order of
-// flash_prefill.hip). Up to 128 columns the waves take two tiles at a time, four each.
+// Two forms. Where one block of 32 columns does not hold all queries' heads, prefixes of 16-bit rows are a kernel's own
+// (paged_prefix_kernel), with up to 256 columns a block: tiles of 32 keys come by asynchronous copies into a ring of LDS that eight
+// waves share, 32 columns a wave, read from HBM once and from LDS by every wave (the layout and the order of flash_prefill.hip; up to 128
+// columns the waves take two tiles at a time, four each). Own rows are paged_decode.hip's then.
 //
-// Own rows (and prefixes of 8-bit rows, in blocks of 32 columns; paged_shared_kernel): a tile is a wave's own, in registers, and the
-// four waves of a workgroup, which take the tiles of a piece in turn, meet in LDS.
-#include "paged_rows.h"
+// Else (few queries, or 8-bit rows; paged_shared_kernel) prefixes and own rows are one launch's: a tile is a wave's own, in registers,
+// and the four waves of a workgroup, which take the tiles of a piece in turn, meet in LDS.
+#include "paged_parts.h"
 
 namespace {
 
@@ -52,7 +53,10 @@ struct SharedRest {
 struct SharedArgs {
   const int32_t *requests, *groups, *lens, *prefix_lens;
   int batch, n_prefixes, n_tables, n_kv, rep;
-  int pieces, prefix_pieces;  // workgroups: no less than the pieces there can be (of own rows and prefixes, or each)
+  int pieces;  // workgroups: no less than the pieces there can be
+  void* decode;
+  size_t decode_bytes;
+  bool wide;
   SharedRest rest;
 };
 
@@ -565,7 +569,6 @@ __global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(const int32_t
                                                                    const int32_t* prefix_lens, int batch, int n_prefixes,
                                                                    int n_tables, int n_kv, int rep, SharedRest a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-  constexpr bool kPrefixes = FMT == kAffine;  // else another kernel's
   __shared__ int wave_sums[3][kWaves];
   __shared__ int members[kColumns];
   __shared__ Piece found;
@@ -596,7 +599,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(const int32_t
   if (t == 0) found.kvh = -1;
   __syncthreads();
   const int rows_a_block = kColumns / rep;
-  auto blocks_of = [&](int e) { return e >= n_prefixes ? 1 : kPrefixes ? ceil_div(count[e], rows_a_block) : 0; };
+  auto blocks_of = [&](int e) { return e >= n_prefixes ? 1 : ceil_div(count[e], rows_a_block); };
   const int entries = n_prefixes + batch, per = ceil_div(entries, kThreads);
   const int e0 = min(t * per, entries), e1 = min(e0 + per, entries);
   int sum = 0, units = 0;
@@ -696,7 +699,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(const int32_t
   int n_members = 1, n_tiles, len;
   const int32_t* table;
   bool whole = false;
-  if (kPrefixes && p.prefix >= 0) {
+  if (p.prefix >= 0) {
     const int per_row = ceil_div(batch, kThreads);
     const int r0 = min(t * per_row, batch), r1 = min(r0 + per_row, batch);
     int mine = 0;
@@ -750,9 +753,9 @@ __global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(const int32_t
   if (p.slot >= (p.prefix >= 0 ? a.prefix_slots : a.own_slots)) return;  // (cannot be, unless lengths change meanwhile)
   const int tile0 = (int)((int64_t)n_tiles * p.range / p.ranges), tile1 = (int)((int64_t)n_tiles * (p.range + 1) / p.ranges);
   const int columns = n_members * rep;
-  if (!kPrefixes || columns <= 16)
+  if (columns <= 16)
     attend_piece<QDT, FMT, SDT, 1>(a, p, table, len, tile0, tile1, n_kv, rep, columns, whole, members, lds);
-  else if constexpr (kPrefixes)
+  else
     attend_piece<QDT, FMT, SDT, 2>(a, p, table, len, tile0, tile1, n_kv, rep, columns, whole, members, lds);
 }
 
@@ -1087,6 +1090,8 @@ __global__ __launch_bounds__(kWideThreads, 1) void paged_prefix_kernel(const int
     if (group < 0 || group >= n_prefixes || tiles[group] == 0) group = -1;
     row_group[r] = group;
     if (group >= 0) atomicAdd(&count[group], 1);
+    else if (number == 0)
+      for (int kvh = 0; kvh < n_kv; kvh++) a.parts[8 * ((int64_t)r * n_kv + kvh) + 3] = 0;
   }
   __syncthreads();
   const int most = a.block / rep;  // members of a block
@@ -1197,14 +1202,16 @@ __global__ __launch_bounds__(kWideThreads, 1) void paged_prefix_kernel(const int
 
 constexpr int kAtOnce = 16;  // pieces that a wave joins at a time
 
-// Joins the pieces of one query head: WAVES of them a head take every WAVES-th, and meet in LDS.
+// Joins the pieces of one query head: WAVES of them a head take every WAVES-th, and meet in LDS. PARTS: own rows are
+// paged_decode.hip's parts (own: of rows that are not cut), else pieces of paged_shared_kernel.
 // grid: heads / (kMergeWaves / WAVES)
 constexpr int kMergeWaves = 8;
-template <int ODT, int WAVES>
+template <int ODT, int WAVES, bool PARTS>
 __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(const int32_t* parts, const float* ws_pre,
                                                                               const float* ws_pre_ml, const float* ws_own,
-                                                                              const float* ws_own_ml, int rep, int n_kv, int heads, int block,
-                                                                              int prefix_slots, int own_slots, void* out) {
+                                                                              const float* ws_own_ml, int rep, int n_kv, int heads,
+                                                                              int block, int prefix_slots, int own_slots,
+                                                                              PagedParts own, void* out) {
   __shared__ __attribute__((aligned(16))) float xo[kMergeWaves][kD + 2];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1213,41 +1220,44 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
   const bool here = head < heads;
   const int row = here ? head / rep : 0, hn = here ? head - row * rep : 0;
   const int32_t* at = parts + 8 * (int64_t)row;
-  const int n_own = here ? at[1] : 0, ranges = here ? at[3] : 0;
+  Cut cut = {-1, 0, 0};
+  if constexpr (PARTS)
+    if (own.cut) cut.load(own.cut, row, heads / rep, own.shares);
+  const int n_own = !here ? 0 : !PARTS ? at[1] : cut.count > 0 ? cut.count : 1, ranges = here ? at[3] : 0;
   const int total = n_own + ranges;
-  const int own_first = at[0], pre_first = at[2], blocks = at[4], column = at[5] + hn;
+  const int own_first = PARTS ? 0 : at[0], pre_first = at[2], blocks = at[4], column = at[5] + hn;
   const int kvh = row % n_kv;
-  // (bounded by the workspace, whatever is there)
-  auto slot_of = [&](int i, int& col) {
-    if (i < n_own) {
-      col = hn;
-      const int s = own_first + i;
-      return s >= 0 && s < own_slots ? s : 0;
+  // Sums and statistics of piece i (bounded by the workspace, whatever is there)
+  struct From {
+    const float *o, *ml;
+  };
+  auto piece = [&](int i) {
+    if (i >= n_own) {
+      int s = pre_first + bundle_piece(kvh * ranges + (i - n_own), column / block, n_kv * ranges, blocks);
+      s = s >= 0 && s < prefix_slots ? s : 0;
+      const int64_t r = (int64_t)s * block + column % block;
+      return From{ws_pre + r * kD, ws_pre_ml + r * 2};
     }
-    col = column % block;
-    const int s = pre_first + bundle_piece(kvh * ranges + (i - n_own), column / block, n_kv * ranges, blocks);
-    return s >= 0 && s < prefix_slots ? s : 0;
+    if constexpr (PARTS) {
+      if (cut.count > 0) {
+        const int64_t p = part_of(cut.first, i);
+        return From{own.o + (p * rep + hn) * kD, own.ml + (p * 16 + hn) * 2};
+      }
+      return From{ws_own + (int64_t)head * kD, ws_own_ml + (int64_t)head * 2};
+    }
+    const int s = own_first + i >= 0 && own_first + i < own_slots ? own_first + i : 0;
+    return From{ws_own + ((int64_t)s * rep + hn) * kD, ws_own_ml + ((int64_t)s * 16 + hn) * 2};
   };
   float m = -__builtin_inff(), l = 0.0f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   for (int p0 = part; p0 < total; p0 += kAtOnce * WAVES) {
     const int mine = p0 + WAVES * (lane % kAtOnce);
     f32x2_t stat = {-__builtin_inff(), 0.0f};
-    if (mine < total) {
-      int col;
-      const int s = slot_of(mine, col);
-      stat = mine < n_own ? *reinterpret_cast<const f32x2_t*>(ws_own_ml + ((int64_t)s * 16 + col) * 2)
-                          : *reinterpret_cast<const f32x2_t*>(ws_pre_ml + ((int64_t)s * block + col) * 2);
-    }
+    if (mine < total) stat = *reinterpret_cast<const f32x2_t*>(piece(mine).ml);
     f32x4_t ov[kAtOnce];
 #pragma unroll
     for (int j = 0; j < kAtOnce; j++)  // (wave-uniform: pieces past the end cost no load)
-      if (p0 + WAVES * j < total) {
-        int col;
-        const int s = slot_of(p0 + WAVES * j, col);
-        const float* from = p0 + WAVES * j < n_own ? ws_own + ((int64_t)s * rep + col) * kD : ws_pre + ((int64_t)s * block + col) * kD;
-        ov[j] = *reinterpret_cast<const f32x4_t*>(from + 4 * lane);
-      }
+      if (p0 + WAVES * j < total) ov[j] = *reinterpret_cast<const f32x4_t*>(piece(p0 + WAVES * j).o + 4 * lane);
     float m_new = stat.x;
     m_new = fmaxf(m_new, lane_xor<1>(m_new));
     m_new = fmaxf(m_new, lane_xor<2>(m_new));
@@ -1293,10 +1303,13 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
   if (total > 0) store_out<ODT>(out, ((int64_t)row * rep + hn) * kD + 4 * lane, o, l);
 }
 
-// Columns of a block of members. Of 8-bit rows 32; of 16-bit ones as many as eight waves hold, but no more than twice what a prefix
-// has members on the average, so that the scratch, a place for every column of a block, does not grow with what blocks leave empty.
-int block_columns(int batch, int n_prefixes, int rep, bool codes) {
-  if (codes) return kColumns;
+// Prefixes are a kernel's own where a block of 32 columns does not hold the call's query heads of a KV head.
+bool wide_prefixes(int batch, int rep, bool codes) { return !codes && (int64_t)batch * rep > kColumns; }
+
+// Columns of a block of members: 32, or as many as eight waves hold, but no more than twice what a prefix has members on the
+// average, so that the scratch, a place for every column of a block, does not grow with what blocks leave empty.
+int block_columns(int batch, int n_prefixes, int rep, bool wide) {
+  if (!wide) return kColumns;
   const int64_t used = n_prefixes < batch ? n_prefixes : batch;
   const int64_t mean = ((used > 1 ? 2 : 1) * (int64_t)batch * rep + used - 1) / used;
   const int64_t n = (mean + 31) / 32 * 32;
@@ -1314,25 +1327,27 @@ int64_t prefix_units(int batch, int n_prefixes, int n_kv, int rep, int block) {
 }
 
 struct SharedScratch {
+  bool wide;
   int block;
-  int64_t pieces, prefix_pieces;           // workgroups of the two kernels (8-bit rows: of the one)
-  int64_t prefix_slots, own_slots;         // places for partials
-  size_t pre, pre_ml, own, own_ml, parts;  // bytes
-  size_t total() const { return pre + pre_ml + own + own_ml + parts; }
+  int64_t pieces;                                  // workgroups: of prefixes, and of own rows where one launch has both
+  int64_t prefix_slots, own_slots;                 // places for partials; wide: own_slots query heads
+  size_t pre, pre_ml, own, own_ml, parts, decode;  // bytes
+  size_t total() const { return pre + pre_ml + own + own_ml + parts + decode; }
 };
-SharedScratch shared_scratch(int batch, int n_prefixes, int n_kv, int rep, bool codes) {
+SharedScratch shared_scratch(int batch, int n_prefixes, int n_kv, int rep, int page_size, int width, bool codes) {
   SharedScratch s;
-  s.block = block_columns(batch, n_prefixes, rep, codes);
+  s.wide = wide_prefixes(batch, rep, codes);
+  s.block = block_columns(batch, n_prefixes, rep, s.wide);
   const int64_t own = (int64_t)batch * n_kv, blocks = prefix_units(batch, n_prefixes, n_kv, rep, s.block);
-  s.pieces = pieces_of(codes ? own + blocks : own);
-  s.prefix_pieces = codes ? 0 : pieces_of(blocks);
-  s.prefix_slots = codes ? s.pieces - own : s.prefix_pieces;  // (every query has a piece of its own, at least)
-  s.own_slots = pieces_of(own);
+  s.pieces = pieces_of(s.wide ? blocks : own + blocks);
+  s.prefix_slots = s.wide ? s.pieces : s.pieces - own;  // (every query has a piece of its own, at least)
+  s.own_slots = s.wide ? own * rep : pieces_of(own);
   s.pre = (size_t)s.prefix_slots * s.block * kD * sizeof(float);
   s.pre_ml = (size_t)s.prefix_slots * s.block * 2 * sizeof(float);
-  s.own = (size_t)s.own_slots * rep * kD * sizeof(float);
-  s.own_ml = (size_t)s.own_slots * 16 * 2 * sizeof(float);
+  s.own = (size_t)s.own_slots * (s.wide ? 1 : rep) * kD * sizeof(float);
+  s.own_ml = ((size_t)s.own_slots * (s.wide ? 1 : 16) * 2 * sizeof(float) + 15) / 16 * 16;
   s.parts = (size_t)own * 8 * sizeof(int32_t);
+  s.decode = s.wide ? mspr_sdpa_decode_paged_workspace_bytes(batch, n_kv * rep, n_kv, page_size, width) : 0;
   return s;
 }
 
@@ -1351,32 +1366,66 @@ int reserve_lds(K* kernel, int bytes, bool (&done)[64]) {
   return MSPR_OK;
 }
 
-template <int QDT, int FMT, int SDT>
-int shared_launch(const SharedArgs& a, hipStream_t st) {
-  constexpr int kLds = shared_lds(QDT, FMT);
-  static bool reserved[2][64] = {};
+// Joins the pieces of `heads` query heads: eight waves a head where they are few and have many pieces, else one.
+template <int QDT, bool PARTS>
+int merge_launch(const SharedArgs& a, const PagedParts& own, hipStream_t st) {
   const SharedRest& r = a.rest;
-  if constexpr (FMT != kAffine) {
-    if (int rc = reserve_lds(&paged_prefix_kernel<FMT>, kWideLds, reserved[0])) return rc;
-    paged_prefix_kernel<FMT><<<dim3((unsigned)a.prefix_pieces), dim3(kWideThreads), kWideLds, st>>>(
-        a.requests, a.groups, a.prefix_lens, a.batch, a.n_prefixes, a.n_tables, a.n_kv, a.rep, r);
-    MSPR_CHECK_LAUNCH("sdpa_decode_paged_shared (prefixes)");
-  }
-  if (int rc = reserve_lds(&paged_shared_kernel<QDT, FMT, SDT>, kLds, reserved[1])) return rc;
-  paged_shared_kernel<QDT, FMT, SDT><<<dim3((unsigned)a.pieces), dim3(kThreads), kLds, st>>>(
-      a.requests, a.groups, a.lens, a.prefix_lens, a.batch, a.n_prefixes, a.n_tables, a.n_kv, a.rep, r);
-  MSPR_CHECK_LAUNCH("sdpa_decode_paged_shared");
   const int heads = a.batch * a.n_kv * a.rep;
   auto merge = [&](auto waves) {
     constexpr int kWavesAHead = decltype(waves)::value, kHeads = kMergeWaves / kWavesAHead;
-    paged_shared_merge_kernel<QDT, kWavesAHead><<<dim3((unsigned)((heads + kHeads - 1) / kHeads)), dim3(64 * kMergeWaves), 0, st>>>(
-        r.parts, r.ws_pre, r.ws_pre_ml, r.ws_own, r.ws_own_ml, a.rep, a.n_kv, heads, r.block, r.prefix_slots, r.own_slots, r.out);
+    paged_shared_merge_kernel<QDT, kWavesAHead, PARTS><<<dim3((unsigned)((heads + kHeads - 1) / kHeads)), dim3(64 * kMergeWaves), 0, st>>>(
+        r.parts, r.ws_pre, r.ws_pre_ml, r.ws_own, r.ws_own_ml, a.rep, a.n_kv, heads, r.block, r.prefix_slots, r.own_slots, own, r.out);
   };
   // (a head has as many pieces as compute units divided by blocks: few where heads are many)
   if (heads <= 1024) merge(std::integral_constant<int, 8>{});
   else merge(std::integral_constant<int, 1>{});
   MSPR_CHECK_LAUNCH("sdpa_decode_paged_shared (merge)");
   return MSPR_OK;
+}
+
+template <int QDT, int FMT, int SDT>
+int shared_launch(const SharedArgs& a, hipStream_t st) {
+  constexpr int kLds = shared_lds(QDT, FMT);
+  static bool reserved[64] = {};
+  if (int rc = reserve_lds(&paged_shared_kernel<QDT, FMT, SDT>, kLds, reserved)) return rc;
+  paged_shared_kernel<QDT, FMT, SDT><<<dim3((unsigned)a.pieces), dim3(kThreads), kLds, st>>>(
+      a.requests, a.groups, a.lens, a.prefix_lens, a.batch, a.n_prefixes, a.n_tables, a.n_kv, a.rep, a.rest);
+  MSPR_CHECK_LAUNCH("sdpa_decode_paged_shared");
+  return merge_launch<QDT, false>(a, PagedParts{}, st);
+}
+
+// Own rows, then prefixes.
+template <int FMT>
+int wide_launch(const char* what, const SharedArgs& a, hipStream_t st) {
+  static bool reserved[64] = {};
+  if (int rc = reserve_lds(&paged_prefix_kernel<FMT>, kWideLds, reserved)) return rc;
+  const SharedRest& r = a.rest;
+  PagedPartsCall c = {};
+  c.q = r.q;
+  c.k = r.k;
+  c.v = r.v;
+  c.q_dtype = FMT;
+  c.tables = r.tables;
+  c.lens = a.lens;
+  c.requests = a.requests;
+  c.batch = a.batch;
+  c.n_kv = a.n_kv;
+  c.rep = a.rep;
+  c.n_pages = r.n_pages;
+  c.page_shift = r.page_shift;
+  c.n_tables = a.n_tables;
+  c.width = r.width;
+  c.scale_log2 = r.scale_log2;
+  c.own = r.ws_own;
+  c.own_ml = r.ws_own_ml;
+  c.workspace = a.decode;
+  c.workspace_bytes = a.decode_bytes;
+  PagedParts own;
+  if (int rc = mspr_paged_decode_parts(what, c, &own, st)) return rc;
+  paged_prefix_kernel<FMT><<<dim3((unsigned)a.pieces), dim3(kWideThreads), kWideLds, st>>>(
+      a.requests, a.groups, a.prefix_lens, a.batch, a.n_prefixes, a.n_tables, a.n_kv, a.rep, r);
+  MSPR_CHECK_LAUNCH("sdpa_decode_paged_shared (prefixes)");
+  return merge_launch<FMT, true>(a, own, st);
 }
 
 int shared_fill(const char* what, SharedArgs& a, bool codes, const void* q, const void* k, const void* v, const int32_t* prefix_tables,
@@ -1401,7 +1450,7 @@ int shared_fill(const char* what, SharedArgs& a, bool codes, const void* q, cons
   const int rep = n_q_heads / n_kv_heads;
   const int64_t most = (int64_t)table_width * page_size > (int64_t)prefix_width * page_size ? (int64_t)table_width * page_size
                                                                                            : (int64_t)prefix_width * page_size;
-  const SharedScratch s = shared_scratch(batch, n_prefixes, n_kv_heads, rep, codes);
+  const SharedScratch s = shared_scratch(batch, n_prefixes, n_kv_heads, rep, page_size, table_width, codes);
   MSPR_REQUIRE((prefix_units(batch, n_prefixes, n_kv_heads, rep, s.block) + (int64_t)batch * n_kv_heads) * ((most + kTileKeys - 1) / kTileKeys + 1) <= 0x3FFFFFFF,
                "%s: the tables hold too many tokens together", what);
   MSPR_REQUIRE(mspr_aligned(q, 16) && mspr_aligned(k, 16) && mspr_aligned(v, 16) && mspr_aligned(out, 16),
@@ -1419,7 +1468,8 @@ int shared_fill(const char* what, SharedArgs& a, bool codes, const void* q, cons
   a.n_kv = n_kv_heads;
   a.rep = rep;
   a.pieces = (int)s.pieces;
-  a.prefix_pieces = (int)s.prefix_pieces;
+  a.wide = s.wide;
+  a.decode_bytes = s.decode;
   SharedRest& r = a.rest;
   r.q = q;
   r.k = k;
@@ -1439,7 +1489,8 @@ int shared_fill(const char* what, SharedArgs& a, bool codes, const void* q, cons
   r.ws_pre_ml = reinterpret_cast<float*>(at += s.pre);
   r.ws_own = reinterpret_cast<float*>(at += s.pre_ml);
   r.ws_own_ml = reinterpret_cast<float*>(at += s.own);
-  r.parts = reinterpret_cast<int32_t*>(at + s.own_ml);
+  r.parts = reinterpret_cast<int32_t*>(at += s.own_ml);
+  a.decode = at + s.parts;
   r.out = out;
   return MSPR_OK;
 }
@@ -1454,10 +1505,14 @@ int shared_q8_launch(const SharedArgs& a, int sb_dtype, hipStream_t st) {
 }  // namespace
 
 // (of both page formats, whichever needs more)
-extern "C" size_t mspr_sdpa_decode_paged_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int n_prefixes) {
-  if (batch < 1 || n_kv_heads < 1 || n_q_heads < n_kv_heads || n_q_heads / n_kv_heads > 16 || n_prefixes < 1) return 0;
-  const size_t rows = shared_scratch(batch, n_prefixes, n_kv_heads, n_q_heads / n_kv_heads, false).total();
-  const size_t codes = shared_scratch(batch, n_prefixes, n_kv_heads, n_q_heads / n_kv_heads, true).total();
+extern "C" size_t mspr_sdpa_decode_paged_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int page_size,
+                                                                int table_width, int n_prefixes) {
+  if (batch < 1 || n_kv_heads < 1 || n_q_heads < n_kv_heads || n_q_heads / n_kv_heads > 16 || n_prefixes < 1 || page_size < 1 ||
+      table_width < 1)
+    return 0;
+  const int rep = n_q_heads / n_kv_heads;
+  const size_t rows = shared_scratch(batch, n_prefixes, n_kv_heads, rep, page_size, table_width, false).total();
+  const size_t codes = shared_scratch(batch, n_prefixes, n_kv_heads, rep, page_size, table_width, true).total();
   return rows > codes ? rows : codes;
 }
 
@@ -1473,8 +1528,10 @@ extern "C" int mspr_sdpa_decode_paged_shared(const void* queries, const void* k_
                            lens, requests, batch, n_q_heads, n_kv_heads, head_dim, n_pages, page_size, n_prefixes, prefix_width,
                            n_tables, table_width, scale, out, workspace, workspace_bytes))
     return rc;
-  if (dtype == MSPR_F16) return shared_launch<MSPR_F16, MSPR_F16, MSPR_F16>(a, (hipStream_t)stream);
-  return shared_launch<MSPR_BF16, MSPR_BF16, MSPR_BF16>(a, (hipStream_t)stream);
+  hipStream_t st = (hipStream_t)stream;
+  if (a.wide) return dtype == MSPR_F16 ? wide_launch<MSPR_F16>("sdpa_decode_paged_shared", a, st) : wide_launch<MSPR_BF16>("sdpa_decode_paged_shared", a, st);
+  if (dtype == MSPR_F16) return shared_launch<MSPR_F16, MSPR_F16, MSPR_F16>(a, st);
+  return shared_launch<MSPR_BF16, MSPR_BF16, MSPR_BF16>(a, st);
 }
 
 extern "C" int mspr_sdpa_decode_paged_shared_q8(const void* queries, int q_dtype, const void* k_wq, const void* k_scales,

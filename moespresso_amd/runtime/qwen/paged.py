@@ -423,7 +423,7 @@ def sdpa_decode_paged_shared(queries, keys, values, prefix_tables, prefix_lens, 
         return out
     q = _aligned(queries.contiguous())
     if workspace is None:
-        workspace = _lib.paged_shared_workspace(R, Hq, heads, G, dev)
+        workspace = _lib.paged_shared_workspace(R, Hq, heads, page_size, int(tables.shape[1]), G, dev)
     _lib.check(_lib.launch(
         dev, "mspr_sdpa_decode_paged_shared", _lib.ptr(q), _lib.ptr(keys), _lib.ptr(values), _lib.DTYPE_CODE[q.dtype],
         _lib.ptr(prefix_tables), _lib.ptr(prefix_lens), _lib.ptr(groups), _lib.ptr(tables), _lib.ptr(lens), _lib.ptr(requests), R,
@@ -461,7 +461,7 @@ def sdpa_decode_paged_shared_q8(queries, k_wq, k_scales, k_biases, v_wq, v_scale
         return out
     q = _aligned(queries.contiguous())
     if workspace is None:
-        workspace = _lib.paged_shared_workspace(R, Hq, heads, G, dev)
+        workspace = _lib.paged_shared_workspace(R, Hq, heads, page_size, int(tables.shape[1]), G, dev)
     _lib.check(_lib.launch(
         dev, "mspr_sdpa_decode_paged_shared_q8", _lib.ptr(q), _lib.DTYPE_CODE[q.dtype], *(_lib.ptr(t) for t in parts),
         _lib.DTYPE_CODE[k_scales.dtype], _lib.ptr(prefix_tables), _lib.ptr(prefix_lens), _lib.ptr(groups), _lib.ptr(tables),

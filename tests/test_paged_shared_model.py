@@ -1,8 +1,6 @@
 """CPU model of how the kernel of shared prefixes deals out its work: every tile of every prefix meets every member once, every
 tile of own rows its query, every partial has a place of its own, and the second kernel finds them."""
 
-import ctypes
-
 import numpy as np
 import pytest
 
@@ -15,23 +13,22 @@ def _ceil(a, b):
     return -(-a // b)
 
 
-def _block(batch, n_prefixes, rep, codes):
+def _block(batch, n_prefixes, rep, wide):
     """Columns of a block of members, at most."""
     used = min(n_prefixes, batch)
-    return NARROW if codes else min(WIDE, _ceil(_ceil((2 if used > 1 else 1) * batch * rep, used), 32) * 32)
+    return min(WIDE, _ceil(_ceil((2 if used > 1 else 1) * batch * rep, used), 32) * 32) if wide else NARROW
 
 
 def _pieces_of(units):
     return max(GROUPS, GROUPS // 2 + units)
 
 
-def _slots(batch, n_prefixes, n_kv, rep, codes):
-    """Workgroups of the kernel of own rows and of the one of prefixes, places for partials of prefixes and of own rows."""
-    per = _block(batch, n_prefixes, rep, codes) // rep
+def _slots(batch, n_prefixes, n_kv, rep, wide):
+    """Workgroups, places for partials of prefixes, and of own rows."""
+    per = _block(batch, n_prefixes, rep, wide) // rep
     own, blocks = batch * n_kv, n_kv * ((batch + min(n_prefixes, batch) * (per - 1)) // per)
-    if codes:
-        return _pieces_of(own + blocks), 0, _pieces_of(own + blocks) - own, _pieces_of(own)
-    return _pieces_of(own), _pieces_of(blocks), _pieces_of(blocks), _pieces_of(own)
+    pieces = _pieces_of(blocks if wide else own + blocks)
+    return pieces, pieces if wide else pieces - own, own * rep if wide else _pieces_of(own)
 
 
 def _plan(tiles, blocks, n_kv, least):
@@ -51,24 +48,24 @@ def _bundle_piece(bundle, block, bundles, blocks):
     return 8 * blocks * q + block * min(8, bundles - 8 * q) + bundle % 8
 
 
-@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("batch,n_prefixes,n_kv,rep,most_prefix,most", [
     (1, 1, 1, 1, 40, 40), (2, 1, 2, 8, 137, 40), (16, 1, 2, 8, 32768, 512), (61, 5, 2, 8, 9001, 2000), (256, 1, 2, 8, 8192, 700),
     (33, 1, 2, 8, 20001, 300), (7, 20, 4, 5, 900, 90), (300, 300, 1, 16, 2000, 10), (2048, 3, 8, 1, 300, 60), (40, 2, 1, 3, 0, 500),
     (9, 2, 2, 7, 60000, 0), (100, 100, 8, 4, 70, 70)])
-def test_every_tile_is_met_once_and_every_partial_has_a_place(batch, n_prefixes, n_kv, rep, most_prefix, most, codes):
+def test_every_tile_is_met_once_and_every_partial_has_a_place(batch, n_prefixes, n_kv, rep, most_prefix, most, wide):
     rng = np.random.default_rng(batch + n_prefixes)
     prefix_lens = [int(n) for n in rng.integers(0, most_prefix + 1, n_prefixes)]
     prefix_lens[-1] = most_prefix
     lens = [int(n) for n in rng.integers(0, most + 1, batch)]
     groups = [g if 0 <= g < n_prefixes and prefix_lens[g] > 0 else -1 for g in (int(g) for g in rng.integers(-1, n_prefixes + 1, batch))]
-    block = _block(batch, n_prefixes, rep, codes)
+    block = _block(batch, n_prefixes, rep, wide)
     per = block // rep
     members = [[r for r in range(batch) if groups[r] == g] for g in range(n_prefixes)]
     blocks = [_ceil(len(m), per) for m in members]
     prefix_tiles, own_tiles = ([_ceil(n, TILE) for n in ns] for ns in (prefix_lens, lens))
-    grid, prefix_grid, prefix_slots, own_slots = _slots(batch, n_prefixes, n_kv, rep, codes)
-    if codes:  # one kernel: prefixes, then own rows
+    grid, prefix_slots, own_slots = _slots(batch, n_prefixes, n_kv, rep, wide)
+    if not wide:  # one kernel: prefixes, then own rows
         entries, pieces = _plan(prefix_tiles + own_tiles, blocks + [1] * batch, n_kv, 1)
         prefixes, own = entries[:n_prefixes], entries[n_prefixes:]
         of_prefixes = own[0][3]
@@ -76,11 +73,11 @@ def test_every_tile_is_met_once_and_every_partial_has_a_place(batch, n_prefixes,
         assert pieces <= grid and of_prefixes <= prefix_slots and pieces - of_prefixes <= own_slots
     else:
         prefixes, of_prefixes = _plan(prefix_tiles, blocks, n_kv, 0)
-        own, pieces = _plan(own_tiles, [1] * batch, n_kv, 1)
-        assert of_prefixes <= prefix_grid and of_prefixes <= prefix_slots and pieces <= grid and pieces <= own_slots
+        own = []  # (dealt out as test_paged_decode_model.py has it)
+        assert of_prefixes <= grid and of_prefixes <= prefix_slots
     met, places = {}, set()
     for g, (n_blocks, ranges, tiles, at) in enumerate(prefixes):
-        a_block = _ceil(len(members[g]), n_blocks) if n_blocks and not codes else per  # (of 16-bit rows about equal)
+        a_block = _ceil(len(members[g]), n_blocks) if n_blocks and wide else per  # (wide ones about equal)
         bundles = n_kv * ranges
         for i in range(n_blocks * bundles):
             q = i // (8 * n_blocks)
@@ -113,14 +110,16 @@ def test_every_tile_is_met_once_and_every_partial_has_a_place(batch, n_prefixes,
 
 
 @pytest.mark.skipif(not _lib.library_available(), reason="the library is not built")
-@pytest.mark.parametrize("batch,hq,hkv,n_prefixes", [(1, 1, 1, 1), (16, 16, 2, 1), (2048, 64, 4, 2048), (100, 48, 3, 7), (5, 15, 3, 9)])
-def test_the_workspace_holds_every_place(batch, hq, hkv, n_prefixes):
-    rep = hq // hkv
+@pytest.mark.parametrize("batch,hq,hkv,page,width,n_prefixes", [(1, 1, 1, 16, 1, 1), (16, 16, 2, 64, 8, 1), (2048, 64, 4, 16, 100, 2048),
+                                                                (100, 48, 3, 256, 7, 7), (5, 15, 3, 16, 3, 9), (4, 16, 2, 64, 9, 1)])
+def test_the_workspace_holds_every_place(batch, hq, hkv, page, width, n_prefixes):
+    rep, lib = hq // hkv, _lib.lib()
 
-    def words(codes):
-        _, _, prefix_slots, own_slots = _slots(batch, n_prefixes, hkv, rep, codes)
-        return prefix_slots * _block(batch, n_prefixes, rep, codes) * (DIM + 2) + own_slots * (rep * DIM + 32) + batch * hkv * 8
+    def bytes_of(wide):
+        _, prefix_slots, own_slots = _slots(batch, n_prefixes, hkv, rep, wide)
+        n = prefix_slots * _block(batch, n_prefixes, rep, wide) * (DIM + 2) + own_slots * (DIM if wide else rep * DIM)
+        n = 4 * n + _ceil(own_slots * (8 if wide else 128), 16) * 16 + batch * hkv * 32
+        return n + (lib.mspr_sdpa_decode_paged_workspace_bytes(batch, hq, hkv, page, width) if wide else 0)
 
-    lib = _lib.lib()
-    lib.mspr_sdpa_decode_paged_shared_workspace_bytes.restype = ctypes.c_size_t
-    assert lib.mspr_sdpa_decode_paged_shared_workspace_bytes(batch, hq, hkv, n_prefixes) == 4 * max(words(False), words(True))
+    most = max(bytes_of(False), bytes_of(True) if batch * rep > NARROW else 0)
+    assert lib.mspr_sdpa_decode_paged_shared_workspace_bytes(batch, hq, hkv, page, width, n_prefixes) == most
