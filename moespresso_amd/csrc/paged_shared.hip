@@ -42,8 +42,8 @@ struct SharedRest {
   int n_pages, page_shift, prefix_width, width, prefix_slots, own_slots;
   int block;          // columns of a block of a prefix's members, at most
   float scale_log2;
-  float* ws_pre;      // partial outputs of prefix pieces [prefix_slots][block columns][256]
-  float* ws_pre_ml;   // their statistics [prefix_slots][block][2]
+  void* ws_pre;       // partial outputs of prefix pieces [prefix_slots][block columns][256], float32 or scaled float16
+  float* ws_pre_ml;   // their statistics [prefix_slots][block][4]: maximum, sum of weights, scale
   float* ws_own;      // of own pieces [own_slots][rep][256]
   float* ws_own_ml;   // [own_slots][16][2]
   int32_t* parts;     // [B * n_kv][8]: of own pieces the first and how many; of prefix pieces the first, ranges, blocks, first column
@@ -516,8 +516,8 @@ __device__ __forceinline__ void attend_piece(const SharedRest& a, const Piece& p
   float* xo = reinterpret_cast<float*>(lds);   // [waves][16 mt][64 lanes][4]
   float* xml = xo + kWaves * 16 * 64 * 4;      // [waves][16 columns][2]
   const int width = p.prefix >= 0 ? a.block : rep;  // columns of a partial
-  const auto po = store_window((p.prefix >= 0 ? a.ws_pre : a.ws_own) + (int64_t)p.slot * width * kD, width * kD * (int)sizeof(float));
-  float* ml = p.prefix >= 0 ? a.ws_pre_ml + (int64_t)p.slot * a.block * 2 : a.ws_own_ml + (int64_t)p.slot * 16 * 2;
+  const auto po = store_window((p.prefix >= 0 ? reinterpret_cast<float*>(a.ws_pre) : a.ws_own) + (int64_t)p.slot * width * kD, width * kD * (int)sizeof(float));
+  float* ml = p.prefix >= 0 ? a.ws_pre_ml + (int64_t)p.slot * a.block * 4 : a.ws_own_ml + (int64_t)p.slot * 16 * 2;
 #pragma unroll
   for (int b = 0; b < NB; b++) {
     l_run[b] += __shfl_xor(l_run[b], 16, MSPR_WAVE);
@@ -559,7 +559,10 @@ __device__ __forceinline__ void attend_piece(const SharedRest& a, const Piece& p
       if (whole) store_out<QDT>(a.out, (((int64_t)p.row * n_kv + p.kvh) * rep + column) * kD + 16 * mt + 4 * g, acc, l_all);
       else window_store<kStoreThrough>(po, (column * kD + 16 * mt + 4 * g) * 4, __builtin_bit_cast(u32x4_t, acc));
     }
-    if (!whole && wave == 0 && g == 0 && mine[b]) *reinterpret_cast<f32x2_t*>(ml + 2 * column) = f32x2_t{m_all, l_all};
+    if (!whole && wave == 0 && g == 0 && mine[b]) {
+      if (p.prefix >= 0) *reinterpret_cast<f32x4_t*>(ml + 4 * column) = f32x4_t{m_all, l_all, 1.0f, 0.0f};
+      else *reinterpret_cast<f32x2_t*>(ml + 2 * column) = f32x2_t{m_all, l_all};
+    }
   }
 }
 
@@ -767,7 +770,7 @@ constexpr int kStageBytes = 2 * kTileBytes;
 constexpr int kStages = 4;                         // tiles of the ring
 constexpr int kWideLds = kStages * kStageBytes;    // 128 KB
 constexpr int kChunk = 30;                         // tiles whose pages a wave has at hand, with two more behind them
-static_assert(kWideLds >= 3 * kMaxRows * 4, "the plan fits into the ring");
+static_assert(2 * kStageBytes >= 3 * kMaxRows * 4, "the plan fits into half of the ring");
 
 __device__ const uint32_t g_no_rows[kRowBytes / 4] = {};  // what half tiles without rows are copied from
 
@@ -783,6 +786,8 @@ template <int N>
 __device__ __forceinline__ void wait_copies_and_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
+// The waves' LDS accesses only: copies and loads stay under way.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 // Lane i's 16 bytes at base + offset land at lds_base + 16 i. In an asm statement, so that the compiler does not wait for it in
 // front of other LDS reads (s_nop: an instruction has to lie between the scalar write of M0 and the copy).
 __device__ __forceinline__ void copy_16(uint64_t base, uint32_t offset, uint32_t lds_base) {
@@ -797,9 +802,10 @@ __device__ __forceinline__ int swizzle(int r) { return ((r & 7) << 1) | ((r >> 3
 
 // One piece: `columns` columns (head rows of q in `column_row`) over tiles [tile0, tile1). KS tiles at a time: wave w has columns 32 (w %
 // (8 / KS)) on and every KS-th tile.
-template <int FMT, int KS>
+template <int FMT, int KS, typename F>
 __device__ __forceinline__ void prefix_piece(const SharedRest& a, const int32_t* table, int len, int tile0, int tile1, int n_kv, int kvh,
-                                             int slot, int columns, const int* column_row, unsigned char* lds, float (*xml)[32][2]) {
+                                             int slot, int columns, const int* column_row, F&& find_members, unsigned char* lds,
+                                             float (*xml)[32][2]) {
   constexpr float kLag = 4.0f;                              // (as in paged_decode.hip)
   constexpr float kUp = FMT == MSPR_F16 ? 11.0f : 0.0f;
   constexpr int kAhead = 2 / KS;                            // steps whose copies are under way behind the present one
@@ -857,6 +863,7 @@ __device__ __forceinline__ void prefix_piece(const SharedRest& a, const int32_t*
 #pragma unroll
   for (int i = 0; i < kAhead; i++) ahead[i] = issue_step(ids, tile0, i);
   int ids_next = load_ids(tile0 + kChunk);
+  find_members();  // (under the first copies)
 
   // ---- Q^T operand: lane (n, g) holds q[column][16 s + 8 g ...] for step s. The wave's rows come in halves of 128 channels, in whole
   //      runs of 256 bytes, and change lanes in 8 KB of LDS that no tile uses yet (piece p of row r at p ^ (r & 15)).
@@ -871,6 +878,7 @@ __device__ __forceinline__ void prefix_piece(const SharedRest& a, const int32_t*
 #pragma unroll
       for (int h = 0; h < 2; h++) raw[h][i] = reinterpret_cast<const u32x4_t*>(a.q)[row * 32 + h * 16 + xc];
     }
+    lds_barrier();  // (the plan lies there)
     unsigned char* xq = lds + 2 * kStageBytes + (wave << 13);
 #pragma unroll
     for (int h = 0; h < 2; h++) {
@@ -1036,25 +1044,56 @@ __device__ __forceinline__ void prefix_piece(const SharedRest& a, const int32_t*
   if (mine == 0) return;
   int row0 = slot * a.block + column0;  // (a scalar by hand: with the lanes' addresses below, the compiler takes it for one of each lane's)
   asm volatile("" : "+s"(row0));
-  if (eg == 0 && en < mine) *reinterpret_cast<f32x2_t*>(a.ws_pre_ml + 2 * (int64_t)(row0 + en)) = f32x2_t{m_run, l_run};
   unsigned char* xo = lds + (wave << (KS == 2 ? 15 : 14));  // (of two parts, where the wave's own exchange was)
-  const auto to = store_window(a.ws_pre + (int64_t)row0 * kD, mine * kD * 4);
+  if constexpr (FMT == MSPR_BF16) {
+    // As float16, scaled by a power of two that brings a column's largest sum to [1/2, 1): partials are as many bytes as the rows
+    // themselves where a compute unit has few tiles (16 queries over 32768 rows, 29 MB), and eleven digits of a part are more
+    // than the result has (one rounding of 2^-12 of the attention over |V| beside its 2^-9).
+    float top = 0.0f;
 #pragma unroll
-  for (int h = 0; h < 2; h++) {
+    for (int mt = 0; mt < 8; mt++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) top = fmaxf(top, fabsf(oacc[mt][i]));
+    top = half_wave_max(top);
+    const int e = top > 0.0f && top < __builtin_inff() ? max(__builtin_amdgcn_frexp_expf(top), -120) : 0;
+    const float by = __builtin_amdgcn_ldexpf(1.0f, -e);
+    if (eg == 0 && en < mine)
+      *reinterpret_cast<f32x4_t*>(a.ws_pre_ml + 4 * (int64_t)(row0 + en)) = f32x4_t{m_run, l_run, __builtin_amdgcn_ldexpf(1.0f, e), 0.0f};
+    const auto to = store_window(reinterpret_cast<uint16_t*>(a.ws_pre) + (int64_t)row0 * kD, mine * kD * 2);
     if constexpr (KS == 2) __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int mt = 0; mt < 4; mt++)
+    for (int mt = 0; mt < 8; mt++)
 #pragma unroll
       for (int c = 0; c < 4; c++) {
-        const f32x16_t& o = oacc[4 * h + mt];
-        *reinterpret_cast<f32x4_t*>(xo + en * 512 + 16 * ((8 * mt + 2 * c + eg) ^ (en & 15))) =
-            f32x4_t{o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]};
+        const h2_t lo = {(_Float16)(oacc[mt][4 * c] * by), (_Float16)(oacc[mt][4 * c + 1] * by)};
+        const h2_t hi = {(_Float16)(oacc[mt][4 * c + 2] * by), (_Float16)(oacc[mt][4 * c + 3] * by)};
+        *reinterpret_cast<u32x2_t*>(xo + en * 512 + 16 * ((4 * mt + c) ^ (en & 15)) + 8 * eg) = u32x2_t{h2_bits(lo), h2_bits(hi)};
       }
 #pragma unroll
     for (int i = 0; i < 16; i++) {
       const int r = 2 * i + eg;
-      const f32x4_t v = *reinterpret_cast<const f32x4_t*>(xo + r * 512 + 16 * (en ^ (r & 15)));
-      window_store<kStoreThrough>(to, r * kD * 4 + 512 * h + 16 * en, __builtin_bit_cast(u32x4_t, v));
+      window_store<kStoreThrough>(to, r * kD * 2 + 16 * en, *reinterpret_cast<const u32x4_t*>(xo + r * 512 + 16 * (en ^ (r & 15))));
+    }
+  } else {
+    if (eg == 0 && en < mine) *reinterpret_cast<f32x4_t*>(a.ws_pre_ml + 4 * (int64_t)(row0 + en)) = f32x4_t{m_run, l_run, 1.0f, 0.0f};
+    const auto to = store_window(reinterpret_cast<float*>(a.ws_pre) + (int64_t)row0 * kD, mine * kD * 4);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      if constexpr (KS == 2) __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int mt = 0; mt < 4; mt++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          const f32x16_t& o = oacc[4 * h + mt];
+          *reinterpret_cast<f32x4_t*>(xo + en * 512 + 16 * ((8 * mt + 2 * c + eg) ^ (en & 15))) =
+              f32x4_t{o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]};
+        }
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const int r = 2 * i + eg;
+        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(xo + r * 512 + 16 * (en ^ (r & 15)));
+        window_store<kStoreThrough>(to, r * kD * 4 + 512 * h + 16 * en, __builtin_bit_cast(u32x4_t, v));
+      }
     }
   }
 }
@@ -1065,123 +1104,122 @@ __global__ __launch_bounds__(kWideThreads, 1) void paged_prefix_kernel(const int
                                                                        const int32_t* prefix_lens, int batch, int n_prefixes,
                                                                        int n_tables, int n_kv, int rep, SharedRest a) {
   extern __shared__ __attribute__((aligned(256))) unsigned char lds[];  // tile bases: zero low bits under the address XORs
-  __shared__ int wave_sums[2][kWideWaves];
+  __shared__ int wave_members[kWideWaves];
   __shared__ int column_row[kWideColumns];
   __shared__ float xml[kWideWaves / 2][32][2];
-  __shared__ Piece found;
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int number = blockIdx.x;
 
-  // ---- the plan: members of every prefix, tiles, the length of a range
-  int* row_group = reinterpret_cast<int*>(lds);  // [batch]
-  int* tiles = row_group + kMaxRows;             // [n_prefixes]
-  int* count = tiles + kMaxRows;                 // [n_prefixes]
+  // ---- members of every prefix (where no first tile goes)
+  int* row_group = reinterpret_cast<int*>(lds + 2 * kStageBytes);  // [batch]
+  int* length = row_group + kMaxRows;                              // [n_prefixes]
+  int* count = length + kMaxRows;                                  // [n_prefixes]
   const int prefix_cap = a.prefix_width << a.page_shift;
+  auto group_of = [&](int r) {
+    if (r >= batch) return -1;
+    const int request = requests ? requests[r] : r;
+    return request >= 0 && request < n_tables ? groups[request] : -1;
+  };
+  int group = group_of(t);  // (asked for together with the lengths)
   for (int i = t; i < n_prefixes; i += kWideThreads) {
-    tiles[i] = ceil_div(length_of(prefix_lens, n_prefixes, i, prefix_cap), kTileKeys);
+    length[i] = length_of(prefix_lens, n_prefixes, i, prefix_cap);
     count[i] = 0;
   }
-  if (t == 0) found.kvh = -1;
-  __syncthreads();
+  lds_barrier();
   for (int r = t; r < batch; r += kWideThreads) {
-    const int request = requests ? requests[r] : r;
-    int group = request >= 0 && request < n_tables ? groups[request] : -1;
-    if (group < 0 || group >= n_prefixes || tiles[group] == 0) group = -1;
+    if (r > t) group = group_of(r);
+    if (group < 0 || group >= n_prefixes || length[group] == 0) group = -1;
     row_group[r] = group;
     if (group >= 0) atomicAdd(&count[group], 1);
     else if (number == 0)
       for (int kvh = 0; kvh < n_kv; kvh++) a.parts[8 * ((int64_t)r * n_kv + kvh) + 3] = 0;
   }
-  __syncthreads();
+  lds_barrier();
+
+  // ---- the plan, by every wave for itself: 64 prefixes at a time, one a lane
   const int most = a.block / rep;  // members of a block
-  const int per = ceil_div(n_prefixes, kWideThreads);
-  const int e0 = min(t * per, n_prefixes), e1 = min(e0 + per, n_prefixes);
-  auto total = [&](int v, int which) {
-    const int sum = wave_scan(v);
-    if (lane == 63) wave_sums[which][wave] = sum;
-    return sum;
+  const int chunks = ceil_div(n_prefixes, MSPR_WAVE);
+  struct Load {
+    int blocks, tiles;
   };
-  int sum = 0, units = 0;
-  for (int e = e0; e < e1; e++) {
-    const int blocks = ceil_div(count[e], most);
-    sum += blocks * tiles[e];
-    units += blocks;
+  auto load_of = [&](int chunk) {
+    const int e = chunk * MSPR_WAVE + lane;
+    return e < n_prefixes ? Load{ceil_div(count[e], most), ceil_div(length[e], kTileKeys)} : Load{0, 0};
+  };
+  Load first = load_of(0);
+  int all = 0, units = 0;
+  for (int c = 0; c < chunks; c++) {
+    const Load p = c == 0 ? first : load_of(c);
+    all += __builtin_amdgcn_readlane(wave_scan(p.blocks * p.tiles), 63);
+    units += __builtin_amdgcn_readlane(wave_scan(p.blocks), 63);
   }
-  total(sum, 0);
-  total(units, 1);
-  __syncthreads();
-  int all = 0, all_units = 0;
-#pragma unroll
-  for (int w = 0; w < kWideWaves; w++) {
-    all += wave_sums[0][w];
-    all_units += wave_sums[1][w];
-  }
-  all = __builtin_amdgcn_readfirstlane(all) * n_kv;
-  all_units = __builtin_amdgcn_readfirstlane(all_units) * n_kv;
   if (all == 0) return;
-  const int share = max(kMinShare, ceil_div(all, max(kGroups - all_units, kGroups / 2)));
-  int pieces = 0;
-  for (int e = e0; e < e1; e++) pieces += n_kv * ceil_div(count[e], most) * ceil_div(tiles[e], share);
-  __syncthreads();
-  int before = total(pieces, 0) - pieces;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWideWaves; w++)
-    if (w < wave) before += wave_sums[0][w];
-  if (number >= before && number < before + pieces) {
-    for (int e = e0; e < e1; e++) {
-      const int blocks = ceil_div(count[e], most), ranges = ceil_div(tiles[e], share);
-      const int own = n_kv * blocks * ranges;
-      if (number < before + own) {
-        const int i = number - before, bundles = n_kv * ranges;
-        const int q = i / (8 * blocks), j = i - 8 * blocks * q, m = min(8, bundles - 8 * q);
-        const int bundle = 8 * q + j % m;
-        Piece p;
-        p.prefix = e;
-        p.row = 0;
-        p.block = j / m;
-        p.blocks = blocks;
-        p.kvh = bundle / ranges;
-        p.range = bundle - p.kvh * ranges;
-        p.ranges = ranges;
-        p.first = before;
-        p.slot = number;
-        found = p;
-        break;
-      }
-      before += own;
+  all *= n_kv;
+  units *= n_kv;
+  // A range's tiles: so many that there are no more pieces than compute units, as a unit has at most one piece that is not full; where
+  // there are too many units for that, half as many again. Of few prefixes the least of 64 lengths that does it, tried one a
+  // lane (16 queries over 32768 rows of two KV heads: 256 pieces of eight tiles, not 228 of nine).
+  const int step = a.block <= kWideColumns / 2 ? 2 : 1;  // (tiles that the waves take at a time)
+  int share = max(kMinShare, ceil_div(all, max(kGroups - units, kGroups / 2)));
+  if (n_prefixes <= 16 && all < (1 << 21)) {
+    const int tried = (max(kMinShare, ceil_div(all, kGroups)) + step - 1) / step * step + step * lane;
+    const float inverse = 1.0f / (float)tried;  // (exact enough: quotients below 2^21, a half away from whole numbers)
+    int pieces = 0;
+    for (int e = 0; e < n_prefixes; e++) {
+      const int tiles = __builtin_amdgcn_readlane(first.tiles, e), blocks = __builtin_amdgcn_readlane(first.blocks, e);
+      pieces += blocks * (int)(((float)(tiles + tried - 1) + 0.5f) * inverse);
+    }
+    const uint64_t fits = __ballot(pieces * n_kv <= kGroups);
+    if (fits) share = min(share, __builtin_amdgcn_readlane(tried, __builtin_ctzll(fits)));
+  }
+  int before = 0, prefix = -1, blocks = 0, ranges = 0;
+  for (int c = 0; c < chunks && prefix < 0; c++) {
+    const Load p = c == 0 ? first : load_of(c);
+    const int p_ranges = ceil_div(p.tiles, share), pieces = n_kv * p.blocks * p_ranges;
+    const int upto = before + wave_scan(pieces);
+    const uint64_t beyond = __ballot(upto > number);
+    if (beyond) {
+      const int i = __builtin_ctzll(beyond);
+      prefix = c * MSPR_WAVE + i;
+      blocks = __builtin_amdgcn_readlane(p.blocks, i);
+      ranges = __builtin_amdgcn_readlane(p_ranges, i);
+      before = __builtin_amdgcn_readlane(upto - pieces, i);
+    } else {
+      before = __builtin_amdgcn_readlane(upto, 63);
     }
   }
-  __syncthreads();
-  const int kvh = __builtin_amdgcn_readfirstlane(found.kvh);
-  if (kvh < 0 || number >= a.prefix_slots) return;  // (more workgroups than pieces)
-  const int prefix = __builtin_amdgcn_readfirstlane(found.prefix);
-  const int block = __builtin_amdgcn_readfirstlane(found.block), blocks = __builtin_amdgcn_readfirstlane(found.blocks);
-  const int range = __builtin_amdgcn_readfirstlane(found.range), ranges = __builtin_amdgcn_readfirstlane(found.ranges);
+  if (prefix < 0 || number >= a.prefix_slots) return;  // (more workgroups than pieces)
+  const int piece = number - before, bundles = n_kv * ranges;
+  const int eights = piece / (8 * blocks), in_eights = piece - 8 * blocks * eights, wide = min(8, bundles - 8 * eights);
+  const int block = __builtin_amdgcn_readfirstlane(in_eights / wide);
+  const int bundle = 8 * eights + in_eights - block * wide;
+  const int kvh = __builtin_amdgcn_readfirstlane(bundle / ranges), range = __builtin_amdgcn_readfirstlane(bundle - kvh * ranges);
 
   // ---- its queries: members block by block, as many in each as it takes to have them about equal
   const int members = __builtin_amdgcn_readfirstlane(count[prefix]);
-  const int a_block = ceil_div(members, blocks);
+  const int a_block = __builtin_amdgcn_readfirstlane(ceil_div(members, blocks));
   const int n_members = min(a_block, members - block * a_block);
-  const int n_tiles = __builtin_amdgcn_readfirstlane(tiles[prefix]);
-  {
+  const int len = __builtin_amdgcn_readfirstlane(length[prefix]), n_tiles = ceil_div(len, kTileKeys);
+  auto find_members = [&]() {
     const int per_row = ceil_div(batch, kWideThreads);
     const int r0 = min(t * per_row, batch), r1 = min(r0 + per_row, batch);
     int mine = 0;
     for (int r = r0; r < r1; r++) mine += row_group[r] == prefix;
-    int rank = total(mine, 1) - mine - block * a_block;
-    __syncthreads();
+    const int sum = wave_scan(mine);
+    if (lane == 63) wave_members[wave] = sum;
+    lds_barrier();
+    int rank = sum - mine - block * a_block;
 #pragma unroll
     for (int w = 0; w < kWideWaves; w++)
-      if (w < wave) rank += wave_sums[1][w];
+      if (w < wave) rank += wave_members[w];
     for (int r = r0; r < r1; r++)
       if (row_group[r] == prefix) {
         if (rank >= 0 && rank < a_block) {
           for (int h = 0; h < rep; h++) column_row[rank * rep + h] = (r * n_kv + kvh) * rep + h;
           if (range == 0) {
             int32_t* at = a.parts + 8 * ((int64_t)r * n_kv + kvh);
-            at[2] = found.first;
+            at[2] = before;
             at[3] = ranges;
             at[4] = blocks;
             at[5] = block * a.block + rank * rep;
@@ -1189,15 +1227,16 @@ __global__ __launch_bounds__(kWideThreads, 1) void paged_prefix_kernel(const int
         }
         rank++;
       }
-  }
-  const int len = __builtin_amdgcn_readfirstlane(length_of(prefix_lens, n_prefixes, prefix, prefix_cap));
+    lds_barrier();
+  };
   const int32_t* table = a.prefix_tables + (int64_t)prefix * a.prefix_width;
-  __syncthreads();  // (the plan lies where the tiles will be)
   const int tile0 = __builtin_amdgcn_readfirstlane((int)((int64_t)n_tiles * range / ranges));
   const int tile1 = __builtin_amdgcn_readfirstlane((int)((int64_t)n_tiles * (range + 1) / ranges));
   const int columns = __builtin_amdgcn_readfirstlane(n_members * rep);
-  if (columns <= kWideColumns / 2) prefix_piece<FMT, 2>(a, table, len, tile0, tile1, n_kv, kvh, number, columns, column_row, lds, xml);
-  else prefix_piece<FMT, 1>(a, table, len, tile0, tile1, n_kv, kvh, number, columns, column_row, lds, xml);
+  if (columns <= kWideColumns / 2)
+    prefix_piece<FMT, 2>(a, table, len, tile0, tile1, n_kv, kvh, number, columns, column_row, find_members, lds, xml);
+  else
+    prefix_piece<FMT, 1>(a, table, len, tile0, tile1, n_kv, kvh, number, columns, column_row, find_members, lds, xml);
 }
 
 constexpr int kAtOnce = 16;  // pieces that a wave joins at a time
@@ -1206,8 +1245,8 @@ constexpr int kAtOnce = 16;  // pieces that a wave joins at a time
 // paged_decode.hip's parts (own: of rows that are not cut), else pieces of paged_shared_kernel.
 // grid: heads / (kMergeWaves / WAVES)
 constexpr int kMergeWaves = 8;
-template <int ODT, int WAVES, bool PARTS>
-__global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(const int32_t* parts, const float* ws_pre,
+template <int ODT, int WAVES, bool PARTS>  // (partials of prefixes are float16 where PARTS and bfloat16 results)
+__global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(const int32_t* parts, const void* ws_pre,
                                                                               const float* ws_pre_ml, const float* ws_own,
                                                                               const float* ws_own_ml, int rep, int n_kv, int heads,
                                                                               int block, int prefix_slots, int own_slots,
@@ -1227,17 +1266,16 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
   const int total = n_own + ranges;
   const int own_first = PARTS ? 0 : at[0], pre_first = at[2], blocks = at[4], column = at[5] + hn;
   const int kvh = row % n_kv;
-  // Sums and statistics of piece i (bounded by the workspace, whatever is there)
+  constexpr bool kHalf = PARTS && ODT == MSPR_BF16;
+  // Row of prefix piece i (bounded by the workspace, whatever is there), sums and statistics of own piece i
+  auto prefix_row = [&](int i) {
+    const int s = pre_first + bundle_piece(kvh * ranges + i, column / block, n_kv * ranges, blocks);
+    return (int64_t)(s >= 0 && s < prefix_slots ? s : 0) * block + column % block;
+  };
   struct From {
     const float *o, *ml;
   };
-  auto piece = [&](int i) {
-    if (i >= n_own) {
-      int s = pre_first + bundle_piece(kvh * ranges + (i - n_own), column / block, n_kv * ranges, blocks);
-      s = s >= 0 && s < prefix_slots ? s : 0;
-      const int64_t r = (int64_t)s * block + column % block;
-      return From{ws_pre + r * kD, ws_pre_ml + r * 2};
-    }
+  auto own_piece = [&](int i) {
     if constexpr (PARTS) {
       if (cut.count > 0) {
         const int64_t p = part_of(cut.first, i);
@@ -1253,11 +1291,29 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
   for (int p0 = part; p0 < total; p0 += kAtOnce * WAVES) {
     const int mine = p0 + WAVES * (lane % kAtOnce);
     f32x2_t stat = {-__builtin_inff(), 0.0f};
-    if (mine < total) stat = *reinterpret_cast<const f32x2_t*>(piece(mine).ml);
-    f32x4_t ov[kAtOnce];
+    float scale = 1.0f;
+    if (mine < n_own) {
+      stat = *reinterpret_cast<const f32x2_t*>(own_piece(mine).ml);
+    } else if (mine < total) {
+      const f32x4_t s = *reinterpret_cast<const f32x4_t*>(ws_pre_ml + 4 * prefix_row(mine - n_own));
+      stat = f32x2_t{s.x, s.y};
+      scale = s.z;
+    }
+    u32x4_t ov[kAtOnce];
 #pragma unroll
-    for (int j = 0; j < kAtOnce; j++)  // (wave-uniform: pieces past the end cost no load)
-      if (p0 + WAVES * j < total) ov[j] = *reinterpret_cast<const f32x4_t*>(piece(p0 + WAVES * j).o + 4 * lane);
+    for (int j = 0; j < kAtOnce; j++) {  // (wave-uniform: pieces past the end cost no load)
+      const int i = p0 + WAVES * j;
+      if (i >= total) continue;
+      if (i < n_own) {
+        ov[j] = *reinterpret_cast<const u32x4_t*>(own_piece(i).o + 4 * lane);
+      } else if constexpr (kHalf) {
+        const u32x2_t h = *reinterpret_cast<const u32x2_t*>(reinterpret_cast<const uint16_t*>(ws_pre) + prefix_row(i - n_own) * kD + 4 * lane);
+        ov[j].x = h.x;
+        ov[j].y = h.y;
+      } else {
+        ov[j] = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const float*>(ws_pre) + prefix_row(i - n_own) * kD + 4 * lane);
+      }
+    }
     float m_new = stat.x;
     m_new = fmaxf(m_new, lane_xor<1>(m_new));
     m_new = fmaxf(m_new, lane_xor<2>(m_new));
@@ -1272,9 +1328,18 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
     lw += lane_xor<4>(lw);
     l = l * alpha + (lw + lane_xor<8>(lw));
     o = o * alpha;
+    const float of_sums = w * scale;
 #pragma unroll
-    for (int j = 0; j < kAtOnce; j++)
-      if (p0 + WAVES * j < total) o += ov[j] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), j));
+    for (int j = 0; j < kAtOnce; j++) {
+      const int i = p0 + WAVES * j;
+      if (i >= total) continue;
+      f32x4_t v = __builtin_bit_cast(f32x4_t, ov[j]);
+      if (kHalf && i >= n_own) {
+        const h2_t lo = bits_h2(ov[j].x), hi = bits_h2(ov[j].y);
+        v = f32x4_t{(float)lo.x, (float)lo.y, (float)hi.x, (float)hi.y};
+      }
+      o += v * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(of_sums), j));
+    }
     m = m_new;
   }
   if constexpr (WAVES > 1) {
@@ -1343,7 +1408,7 @@ SharedScratch shared_scratch(int batch, int n_prefixes, int n_kv, int rep, int p
   s.prefix_slots = s.wide ? s.pieces : s.pieces - own;  // (every query has a piece of its own, at least)
   s.own_slots = s.wide ? own * rep : pieces_of(own);
   s.pre = (size_t)s.prefix_slots * s.block * kD * sizeof(float);
-  s.pre_ml = (size_t)s.prefix_slots * s.block * 2 * sizeof(float);
+  s.pre_ml = (size_t)s.prefix_slots * s.block * 4 * sizeof(float);
   s.own = (size_t)s.own_slots * (s.wide ? 1 : rep) * kD * sizeof(float);
   s.own_ml = ((size_t)s.own_slots * (s.wide ? 1 : 16) * 2 * sizeof(float) + 15) / 16 * 16;
   s.parts = (size_t)own * 8 * sizeof(int32_t);
@@ -1485,7 +1550,7 @@ int shared_fill(const char* what, SharedArgs& a, bool codes, const void* q, cons
   r.block = s.block;
   r.scale_log2 = (float)((double)scale * 1.4426950408889634);
   uint8_t* at = reinterpret_cast<uint8_t*>(workspace);
-  r.ws_pre = reinterpret_cast<float*>(at);
+  r.ws_pre = at;
   r.ws_pre_ml = reinterpret_cast<float*>(at += s.pre);
   r.ws_own = reinterpret_cast<float*>(at += s.pre_ml);
   r.ws_own_ml = reinterpret_cast<float*>(at += s.own);

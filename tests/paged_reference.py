@@ -69,8 +69,10 @@ def places(table, n, page, n_pages):
     return [(p, o) for p, o in at if 0 <= p < n_pages]
 
 
-def attention(q, keys, values, at, scale):
-    """(float64 results, bound without the last rounding) of queries ``[R, Hq, 256]``; ``at[r][g]``: the places that r attends."""
+def attention(q, keys, values, at, scale, half_parts=False):
+    """(float64 results, bound without the last rounding) of queries ``[R, Hq, 256]``; ``at[r][g]``: the places that r attends.
+    ``half_parts``: partial sums may be stored as float16 numbers of a column's largest, each off by half a step (2^-11 of it, or, below
+    2^-14 of the largest, 2^-25 of a power of two that is at most twice that); joined, they are off by the same of the attention over |V|."""
     out, bound = (torch.zeros(q.shape, dtype=torch.float64, device="cuda") for _ in range(2))
     G = (keys if torch.is_tensor(keys) else keys[0]).shape[1]
     rep = q.shape[1] // G
@@ -87,15 +89,18 @@ def attention(q, keys, values, at, scale):
             most = (x.abs() @ k_size.t()).amax(-1, keepdim=True) * abs(scale)
             h = slice(g * rep, (g + 1) * rep)
             out[r, h] = w @ v
-            bound[r, h] = (w @ v_size) * (2 * 260 * 2.0 ** -24 * most + terms + 2 * (len(at[r][g]) / 8 + 36) * 2.0 ** -24)
+            size = w @ v_size
+            if half_parts:
+                bound[r, h] = size * 2.0 ** -11 + size.amax(-1, keepdim=True) * 2.0 ** -24
+            bound[r, h] += size * (2 * 260 * 2.0 ** -24 * most + terms + 2 * (len(at[r][g]) / 8 + 36) * 2.0 ** -24)
             if q.dtype != BF16 or not torch.is_tensor(keys):
                 bound[r, h] += len(at[r][g]) * 2.0 ** -36 * v_most
     return out, bound
 
 
-def check(got, q, keys, values, at, scale):
+def check(got, q, keys, values, at, scale, half_parts=False):
     assert got.dtype == q.dtype and got.shape == q.shape
-    want, bound = attention(q, keys, values, at, scale)
+    want, bound = attention(q, keys, values, at, scale, half_parts)
     bound = bound + torch.finfo(q.dtype).eps / 2 * want.abs() + torch.finfo(q.dtype).tiny
     err = (got.double() - want).abs()
     assert (err <= bound).all(), ((err / bound).nan_to_num(9e9).max(), err.max())

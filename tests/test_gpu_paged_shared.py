@@ -37,11 +37,16 @@ def _places(prefix_tables, prefix_lens, groups, tables, lens, requests, R, page,
     return out
 
 
+def _half_parts(q, keys):
+    """Blocks of more than 32 columns of bfloat16 rows leave partial sums of eleven digits."""
+    return torch.is_tensor(keys) and q.dtype == BF16 and q.shape[0] * (q.shape[1] // keys.shape[1]) > 32
+
+
 def _check(q, keys, values, prefix_tables, prefix_lens, groups, tables, lens, scale=SCALE, requests=None):
     n_pages, G, page = (keys if torch.is_tensor(keys) else keys[0]).shape[:3]
     got = _call(q, keys, values, prefix_tables, prefix_lens, groups, tables, lens, scale, requests)
     at = _places(prefix_tables, prefix_lens, groups, tables, lens, requests, q.shape[0], page, n_pages, G)
-    ref.check(got, q, keys, values, at, scale)
+    ref.check(got, q, keys, values, at, scale, _half_parts(q, keys))
     return got
 
 
@@ -155,7 +160,7 @@ def test_as_many_queries_and_prefixes_as_a_call_takes(R, n_prefixes):
     got = _call(q, keys, values, prefix_tables, prefix_lens, groups, tables, lens, requests=requests)
     some = sorted({0, R - 1, *(int(i) for i in rng.choice(R, 40, replace=False))})
     at = _places(prefix_tables, prefix_lens, groups, tables, lens[some], requests[some], len(some), 16, 40, 2)
-    ref.check(got[some], q[some], keys, values, at, SCALE)
+    ref.check(got[some], q[some], keys, values, at, SCALE, _half_parts(q, keys))
     assert not got.isnan().any()
 
 
@@ -193,6 +198,16 @@ def test_large_queries_and_scales_of_very_different_size():
     args = keys, values, [[0, 1, 2, 3]], [120], [0, 0, 0], [[4], [5], [5]], [20, 32, 0]
     _check(q, *args)
     _check(q.bfloat16(), *args)
+
+
+def test_values_of_any_size():
+    """Beyond float16's range and below it, a prefix's and own rows' of very different size."""
+    q, keys, values, prefix_tables, *rest = _case(22, 16, 2, 16, [300, 40], [0] * 9 + [1] * 5, [50, 1, 0, 70, 16, 17, 3] * 2, BF16, "rows")
+    for of_prefixes, of_others in ((1e30, 1e30), (1e-30, 1e-30), (1e30, 1e-6), (1e-30, 1.0), (0.0, 1.0), (1.0, 0.0)):
+        v = values * of_others
+        for p in prefix_tables[0][:19].tolist() + prefix_tables[1][:3].tolist():
+            v[p] = values[p] * of_prefixes
+        _check(q, keys, v, prefix_tables, *rest)
 
 
 def test_a_negative_scale_and_one_of_zero():

@@ -31,10 +31,21 @@ def _slots(batch, n_prefixes, n_kv, rep, wide):
     return pieces, pieces if wide else pieces - own, own * rep if wide else _pieces_of(own)
 
 
-def _plan(tiles, blocks, n_kv, least):
-    """Ranges and first piece of every entry of so many tiles and blocks, and the number of pieces."""
+def _plan(tiles, blocks, n_kv, least, step=None):
+    """Ranges and first piece of every entry of so many tiles and blocks, and the number of pieces. ``step``: of few prefixes lengths in
+    such steps are tried."""
     total, units = n_kv * sum(b * t for b, t in zip(blocks, tiles)), n_kv * sum(blocks)
     share = max(MIN_SHARE, _ceil(total, max(GROUPS - units, GROUPS // 2)))
+    if step and len(tiles) <= 16:
+        first = _ceil(max(MIN_SHARE, _ceil(total, GROUPS)), step) * step
+        tried = np.arange(first, first + 64 * step, step)
+        pieces = np.zeros(64, dtype=int)
+        for b, t in zip(blocks, tiles):  # (in float32, as the kernel's)
+            q = (np.float32(t) + tried.astype(np.float32) - np.float32(0.5)) * (np.float32(1) / tried.astype(np.float32))
+            assert (q.astype(int) == -(-t // tried)).all()
+            pieces += b * q.astype(int)
+        if (pieces * n_kv <= GROUPS).any():
+            share = min(share, int(tried[np.argmax(pieces * n_kv <= GROUPS)]))
     entries, at = [], 0
     for b, t in zip(blocks, tiles):
         ranges = max(least, _ceil(t, share))
@@ -72,7 +83,7 @@ def test_every_tile_is_met_once_and_every_partial_has_a_place(batch, n_prefixes,
         own = [(b, r, t, at - of_prefixes) for b, r, t, at in own]
         assert pieces <= grid and of_prefixes <= prefix_slots and pieces - of_prefixes <= own_slots
     else:
-        prefixes, of_prefixes = _plan(prefix_tiles, blocks, n_kv, 0)
+        prefixes, of_prefixes = _plan(prefix_tiles, blocks, n_kv, 0, 2 if block <= 128 else 1)
         own = []  # (dealt out as test_paged_decode_model.py has it)
         assert of_prefixes <= grid and of_prefixes <= prefix_slots
     met, places = {}, set()
@@ -117,7 +128,7 @@ def test_the_workspace_holds_every_place(batch, hq, hkv, page, width, n_prefixes
 
     def bytes_of(wide):
         _, prefix_slots, own_slots = _slots(batch, n_prefixes, hkv, rep, wide)
-        n = prefix_slots * _block(batch, n_prefixes, rep, wide) * (DIM + 2) + own_slots * (DIM if wide else rep * DIM)
+        n = prefix_slots * _block(batch, n_prefixes, rep, wide) * (DIM + 4) + own_slots * (DIM if wide else rep * DIM)
         n = 4 * n + _ceil(own_slots * (8 if wide else 128), 16) * 16 + batch * hkv * 32
         return n + (lib.mspr_sdpa_decode_paged_workspace_bytes(batch, hq, hkv, page, width) if wide else 0)
 
