@@ -11,8 +11,8 @@
 // Sums are whole numbers below 2^24 and scales powers of two, so that a bound is exact in float32, and the selection does not
 // depend on the order of anything.
 //
-// Two launches: bounds of 16 pages a wave and step, read at the rate of HBM (516 bytes a page and KV head) with their maxima, and the
-// choice, a workgroup a query and KV head, in LDS. The pages of a KV head are then pages of a pool of its own (page * n_kv + head,
+// Two launches: bounds of 16 pages a wave and step, read at the rate of HBM (516 bytes a page and KV head), and the choice, a workgroup a
+// query and KV head. The pages of a KV head are then pages of a pool of its own (page * n_kv + head,
 // one head a page), over which paged_decode.hip attends.
 #include "page_bounds.h"
 
@@ -24,7 +24,7 @@ constexpr int kTile = 16;          // pages of a matrix instruction
 constexpr int kScoreWaves = 4;
 constexpr int kTilesAWave = 2;
 constexpr int kPagesAGroup = kTile * kScoreWaves * kTilesAWave;
-constexpr int kMaxTablePages = 32768;  // their keys fit into LDS
+constexpr int kMaxTablePages = 32768;  // a workgroup of 1024 threads has 32 a thread
 constexpr int kMaxSelected = 4096;
 
 struct SelectArgs {
@@ -36,7 +36,6 @@ struct SelectArgs {
   const float* scales;      // [n_pages, n_kv]
   int rows, n_kv, rep, width, n_tables, n_pages, page_shift, selected, first, recent;
   float* bounds;            // [R * n_kv][rep][padded]
-  float* most;              // [R * n_kv][padded / 16][rep], maxima of 16 pages
   int padded;               // width, up to a multiple of 16
   int32_t* out;             // [R * n_kv][selected]
   int32_t* out_lens;        // [R * n_kv]
@@ -139,146 +138,275 @@ __global__ __launch_bounds__(64 * kScoreWaves) void page_score_kernel(SelectArgs
     }
     // page 4 g + j of the tile, head `head`
     f32x4_t b;
-    float best = -__builtin_inff();
     const float of_page = good[i] ? scale[i] : 0.0f;  // (bounds of a page that is not in the pool: none)
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const float s = __shfl(of_page, 4 * g + j, MSPR_WAVE);
       const bool there = __shfl((int)good[i], 4 * g + j, MSPR_WAVE) != 0;
       b[j] = there ? (float)acc[j] * unit * s : -__builtin_inff();
-      best = fmaxf(best, b[j]);
     }
-    best = half_wave_max(row_pair_max(best));
-    if (mine) {
-      *reinterpret_cast<f32x4_t*>(a.bounds + ((int64_t)row * a.rep + head) * a.padded + p0 + 4 * g) = b;
-      if (g == 0) a.most[((int64_t)row * (a.padded / kTile) + tile0 + i) * a.rep + head] = best;
-    }
+    if (mine) *reinterpret_cast<f32x4_t*>(a.bounds + ((int64_t)row * a.rep + head) * a.padded + p0 + 4 * g) = b;
   }
 }
 
-constexpr int kChooseThreads = 1024;
-constexpr int kChooseWaves = kChooseThreads / 64;
-constexpr int kBins = 2048;
+constexpr int kBins = 1024;
+constexpr int kRanked = 512;  // keys of a bin that are ranked one by one
 
-__device__ __forceinline__ int scan_up(int v) {  // sums over this lane and those before it
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const int o = __shfl_up(v, m, MSPR_WAVE);
-    if ((int)(threadIdx.x & 63) >= m) v += o;
-  }
+// Largest value over the wave, in all lanes.
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, lane_xor<1>(v));
+  v = fmaxf(v, lane_xor<2>(v));
+  v = fmaxf(v, lane_xor<4>(v));
+  v = fmaxf(v, lane_xor<8>(v));
+  return half_wave_max(row_pair_max(v));
+}
+__device__ __forceinline__ int wave_sum_upto(int v) {  // sums over this lane and those before it, by data-parallel moves
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
   return v;
 }
 
-// One workgroup a query and KV head. LDS: keys of all pages.
-__global__ __launch_bounds__(kChooseThreads) void page_choose_kernel(SelectArgs a) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-  uint32_t* keys = reinterpret_cast<uint32_t*>(lds);  // [width]
+// A workgroup a query and KV head, PER pages a thread, one behind the other, whose worths stay in registers. The worth of rank
+// `selected` lies in one of 1024 bins over the range that worths have (a monotone map); the keys of that bin are ranked one by one, or,
+// where they are too many (worths that are alike), the bin is found again among their 32-bit keys, ten bits at a time.
+// HEADS: rows of bounds that are read, the query heads or, of fewer, the first again (without branches between them, their loads and
+// reductions go on at once).
+template <int THREADS, int PER, int HEADS>
+__global__ __launch_bounds__(THREADS) void page_choose_kernel(SelectArgs a) {
+  constexpr int kWaves = THREADS / 64;
+  constexpr bool kHold = PER <= 8 && THREADS <= 512;  // all heads' bounds stay in registers between the best one and the worths
+  static_assert(kWaves <= 16, "the waves' best bounds are sixteen a head");
   __shared__ int bins[kBins];
-  __shared__ float tops[16];
-  __shared__ int sums[kChooseWaves];
-  __shared__ int found[2];
+  __shared__ float tops[kWaves][16], lows[kWaves];
+  __shared__ int sums[2][kWaves];
+  __shared__ int found[2], listed;
+  __shared__ uint32_t list_key[kRanked];
+  __shared__ int list_page[kRanked];
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int row = blockIdx.x, r = row / a.n_kv, kvh = row - r * a.n_kv;
+  const int p0 = t * PER;
+  const float* bounds = a.bounds + (int64_t)row * a.rep * a.padded;
+  // Bounds of head h, asked for ahead of the lengths and masked behind them (what lies behind the last page was not written; rows are
+  // `padded`, a multiple of four, long).
+  auto load_bounds = [&](int h, float* b) {
+#pragma unroll
+    for (int q = 0; q < PER / 4; q++) {
+      const f32x4_t v = *reinterpret_cast<const f32x4_t*>(bounds + (int64_t)(h < a.rep ? h : 0) * a.padded + min(p0 + 4 * q, a.padded - 4));
+#pragma unroll
+      for (int i = 0; i < 4; i++) b[4 * q + i] = v[i];
+    }
+  };
+  float held[kHold ? HEADS : 1][PER];
+  if constexpr (kHold) {
+#pragma unroll
+    for (int h = 0; h < HEADS; h++) load_bounds(h, held[h]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
   const Seen seen = seen_by(a, r);
   const int page_size = 1 << a.page_shift;
-  const int n = (seen.len + page_size - 1) >> a.page_shift;
+  const int n = __builtin_amdgcn_readfirstlane((seen.len + page_size - 1) >> a.page_shift);
   const int32_t* table = a.tables + (int64_t)seen.request * a.width;
   int32_t* out = a.out + (int64_t)row * a.selected;
-  auto id_of = [&](int p) {
-    const int page = table[p];
-    return page >= 0 && page < a.n_pages ? page * a.n_kv + kvh : -1;
-  };
+  auto id_of = [&](int page) { return page >= 0 && page < a.n_pages ? page * a.n_kv + kvh : -1; };
   if (t == 0) a.out_lens[row] = n > a.selected ? seen.len - ((n - a.selected) << a.page_shift) : seen.len;
   if (n <= a.selected) {
-    for (int i = t; i < a.selected; i += kChooseThreads) out[i] = i < n ? id_of(i) : -1;
+    for (int i = t; i < a.selected; i += THREADS) out[i] = i < n ? id_of(table[i]) : -1;
     return;
   }
+  auto mask_bounds = [&](float* b) {
+#pragma unroll
+    for (int i = 0; i < PER; i++) b[i] = p0 + i < n ? b[i] : -__builtin_inff();
+  };
   // ---- every head's best bound
-  for (int h = wave; h < a.rep; h += kChooseWaves) {
-    float best = -__builtin_inff();
-    const float* most = a.most + (int64_t)row * (a.padded / kTile) * a.rep + h;
-    for (int i = lane; i * kTile < n; i += 64) best = fmaxf(best, most[(int64_t)i * a.rep]);
-    for (int m = 32; m > 0; m >>= 1) best = fmaxf(best, __shfl_xor(best, m, MSPR_WAVE));
-    if (lane == 0) tops[h] = best == -__builtin_inff() ? 0.0f : best;
-  }
-  __syncthreads();
-  // ---- keys in the order of worth: 32 bits that grow with it
-  for (int p = t; p < n; p += kChooseThreads) {
-    float worth = -__builtin_inff();
-    for (int h = 0; h < a.rep; h++) worth = fmaxf(worth, a.bounds[((int64_t)row * a.rep + h) * a.padded + p] - tops[h]);
-    keys[p] = p < a.first || p >= n - a.recent ? 0xFFFFFFFFu : score_key(worth);
-  }
-  // ---- the key of rank `selected`, eleven, eleven and ten bits at a time
-  uint32_t prefix = 0, known = 0;
-  int want = a.selected;  // rank of the key among those with this prefix
+  auto best_of = [&](const float* b) {
+    float best = b[0];
+#pragma unroll
+    for (int i = 1; i < PER; i++) best = fmaxf(best, b[i]);
+    return best;
+  };
+  if constexpr (kHold) {
+    float best[HEADS];
+#pragma unroll
+    for (int h = 0; h < HEADS; h++) {
+      mask_bounds(held[h]);
+      best[h] = best_of(held[h]);
+    }
+#pragma unroll
+    for (int h = 0; h < HEADS; h++) {
+      best[h] = wave_max(best[h]);
+      if (lane == 0) tops[wave][h] = best[h];
+    }
+  } else {
 #pragma unroll 1
-  for (int pass = 0; pass < 3; pass++) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    const uint32_t mask = pass == 2 ? 1023u : 2047u;
-    for (int i = t; i < kBins; i += kChooseThreads) bins[i] = 0;
-    __syncthreads();
-    for (int p = t; p < n; p += kChooseThreads)
-      if ((keys[p] & known) == prefix) atomicAdd(&bins[keys[p] >> shift & mask], 1);
-    __syncthreads();
-    // from the highest bin down: thread t has bins 2047 - 2 t and the one below
-    const int b0 = bins[kBins - 1 - 2 * t], b1 = bins[kBins - 2 - 2 * t];
-    const int upto = scan_up(b0 + b1);
-    if (lane == 63) sums[wave] = upto;
-    __syncthreads();
-    int before = upto - b0 - b1;
-    for (int w = 0; w < wave; w++) before += sums[w];
-    if (before < want && want <= before + b0 + b1) {
-      const bool second = want > before + b0;
-      found[0] = kBins - 1 - 2 * t - (second ? 1 : 0);
-      found[1] = want - before - (second ? b0 : 0);
+    for (int h = 0; h < HEADS; h++) {
+      load_bounds(h, held[0]);
+      mask_bounds(held[0]);
+      const float best = wave_max(best_of(held[0]));
+      if (lane == 0) tops[wave][h] = best;
     }
-    __syncthreads();
-    prefix |= (uint32_t)found[0] << shift;
-    known |= mask << shift;
-    want = found[1];
   }
-  // ---- pages above that key, and the first `want` with it, in order: a stretch of pages a thread
-  const int per = (n + kChooseThreads - 1) / kChooseThreads;
-  const int p0 = min(t * per, n), p1 = min(p0 + per, n);
-  int above = 0, ties = 0;
-  for (int p = p0; p < p1; p++) {
-    above += keys[p] > prefix;
-    ties += keys[p] == prefix;
-  }
-  const int upto = scan_up(above), ties_upto = scan_up(ties);
+  for (int i = t; i < kBins; i += THREADS) bins[i] = 0;
+  if (t == 0) listed = 0;
   __syncthreads();
-  if (lane == 63) {
-    sums[wave] = upto;
-    bins[wave] = ties_upto;
-  }
-  __syncthreads();
-  int at = upto - above, tied = ties_upto - ties;
-  for (int w = 0; w < wave; w++) {
-    at += sums[w];
-    tied += bins[w];
-  }
-  for (int p = p0; p < p1; p++) {
-    const bool tie = keys[p] == prefix;
-    if (keys[p] > prefix || (tie && tied < want)) {
-      const int i = at + min(tied, want);
-      if (i < a.selected) out[i] = id_of(p);
+  // ---- worths
+  float worth[PER];
+#pragma unroll
+  for (int i = 0; i < PER; i++) worth[i] = -__builtin_inff();
+  float of_head = -__builtin_inff();  // lane h: of head h
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) of_head = fmaxf(of_head, tops[w][lane % HEADS]);
+  of_head = of_head == -__builtin_inff() ? 0.0f : of_head;
+  auto take = [&](int h, const float* b) {
+    const float top = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(of_head), h));
+#pragma unroll
+    for (int i = 0; i < PER; i++) worth[i] = fmaxf(worth[i], b[i] - top);
+  };
+  if constexpr (kHold) {
+#pragma unroll
+    for (int h = 0; h < HEADS; h++) take(h, held[h]);
+  } else {
+#pragma unroll 1
+    for (int h = 0; h < HEADS; h++) {
+      load_bounds(h, held[0]);
+      mask_bounds(held[0]);
+      take(h, held[0]);
     }
-    at += keys[p] > prefix;
-    tied += tie;
   }
+  auto always = [&](int p) { return p < a.first || p >= n - a.recent; };
+  float low = 0.0f;  // (the best page of a head is worth nothing less)
+#pragma unroll
+  for (int i = 0; i < PER; i++)  // (a last page of few rows may lie far below the others)
+    low = fminf(low, worth[i] == -__builtin_inff() || always(p0 + i) ? 0.0f : worth[i]);
+  low = -wave_max(-low);
+  if (lane == 0) lows[wave] = low;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) low = fminf(low, lows[w]);
+  // ---- the bin of the page of rank `selected`: from the last one down, in which the pages are that are taken whatever they are worth
+  const float by = low < 0.0f ? (float)(kBins - 2) / -low : 0.0f;
+  int bin[PER];
+#pragma unroll
+  for (int i = 0; i < PER; i++) {
+    const int p = p0 + i;
+    const float place = (worth[i] - low) * by;
+    bin[i] = p >= n ? -1 : always(p) ? kBins - 1 : worth[i] == -__builtin_inff() ? 0 : min((int)place, kBins - 2);
+    if (bin[i] >= 0) atomicAdd(&bins[bin[i]], 1);
+  }
+  // Which bin has the key of rank `want`, and its rank in it: thread t of 256 has four bins, from the highest down.
+  auto find_bin = [&](int want) {
+    __syncthreads();
+    int own[4] = {}, mine = 0;
+    if (t < kBins / 4)
+#pragma unroll
+      for (int i = 0; i < 4; i++) mine += own[i] = bins[kBins - 1 - 4 * t - i];
+    const int upto = wave_sum_upto(mine);
+    if (lane == 63) sums[0][wave] = upto;
+    __syncthreads();
+    int before = upto - mine;
+    for (int w = 0; w < min(wave, 4); w++) before += sums[0][w];
+    if (t < kBins / 4 && before < want && want <= before + mine)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if (before < want && want <= before + own[i]) {
+          found[0] = kBins - 1 - 4 * t - i;
+          found[1] = want - before;
+        }
+        before += own[i];
+      }
+    __syncthreads();
+  };
+  find_bin(a.selected);
+  const int last = found[0];
+  int want = found[1];  // of that bin's pages
+  const int in_bin = bins[last];
+  static_assert(PER <= 32, "a bit a page");
+  uint32_t taken = 0;
+#pragma unroll
+  for (int i = 0; i < PER; i++) taken |= (uint32_t)(bin[i] > last) << i;
+  if (in_bin == want) {
+#pragma unroll
+    for (int i = 0; i < PER; i++) taken |= (uint32_t)(bin[i] == last) << i;
+  } else if (in_bin <= kRanked) {
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+      if (bin[i] == last) {
+        const int at = atomicAdd(&listed, 1);
+        list_key[at] = score_key(worth[i]);
+        list_page[at] = p0 + i;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+      if (bin[i] == last) {
+        const uint32_t key = score_key(worth[i]);
+        int ahead = 0;  // pages of the bin that are worth more, or as much and lower
+        for (int k = 0; k < in_bin; k++) ahead += list_key[k] > key || (list_key[k] == key && list_page[k] < p0 + i);
+        taken |= (uint32_t)(ahead < want) << i;
+      }
+  } else {
+    uint32_t prefix = 0, known = 0;
+#pragma unroll 1
+    for (int shift = 22; shift >= 0; shift = shift == 2 ? 0 : shift - 10) {  // bits 22 to 31, 12 to 21, 2 to 11, 0 and 1
+      const uint32_t mask = shift == 0 ? 3u : 1023u;
+      __syncthreads();
+      for (int i = t; i < kBins; i += THREADS) bins[i] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < PER; i++) {
+        const uint32_t key = score_key(worth[i]);
+        if (bin[i] == last && (key & known) == prefix) atomicAdd(&bins[key >> shift & mask], 1);
+      }
+      find_bin(want);
+      prefix |= (uint32_t)found[0] << shift;
+      known |= mask << shift;
+      want = found[1];
+      if (shift == 0) break;
+    }
+    // the first `want` pages with that key
+    int ties = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) ties += bin[i] == last && score_key(worth[i]) == prefix;
+    const int upto = wave_sum_upto(ties);
+    if (lane == 63) sums[1][wave] = upto;
+    __syncthreads();
+    int before = upto - ties;
+    for (int w = 0; w < wave; w++) before += sums[1][w];
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+      if (bin[i] == last) {
+        const uint32_t key = score_key(worth[i]);
+        taken |= (uint32_t)(key > prefix || (key == prefix && before++ < want)) << i;
+      }
+  }
+  // ---- in the order of their positions
+  const int mine = __builtin_popcount(taken);
+  const int upto = wave_sum_upto(mine);
+  __syncthreads();
+  if (lane == 63) sums[0][wave] = upto;
+  __syncthreads();
+  int at = upto - mine;
+  for (int w = 0; w < wave; w++) at += sums[0][w];
+#pragma unroll
+  for (int i = 0; i < PER; i++)
+    if (taken >> i & 1) {
+      if (at < a.selected) out[at] = id_of(table[p0 + i]);
+      at++;
+    }
 }
 
 struct SelectScratch {
   int padded;
-  size_t bounds, most;  // bytes
-  size_t total() const { return bounds + most; }
+  size_t bytes;
 };
 SelectScratch select_scratch(int64_t rows, int rep, int width) {
   SelectScratch s;
   s.padded = (width + kTile - 1) / kTile * kTile;
-  s.bounds = (size_t)rows * rep * s.padded * sizeof(float);
-  s.most = ((size_t)rows * rep * (s.padded / kTile) * sizeof(float) + 15) / 16 * 16;
+  s.bytes = (size_t)rows * rep * s.padded * sizeof(float);
   return s;
 }
 
@@ -304,8 +432,8 @@ int select_fill(const char* what, SelectArgs& a, const void* q, int q_dtype, con
   MSPR_REQUIRE(mspr_aligned(q, 16) && mspr_aligned(codes, 16) && mspr_aligned(scales, 4), "%s: pointers must be 16-byte aligned", what);
   const int rep = n_q_heads / n_kv_heads;
   const SelectScratch s = select_scratch((int64_t)rows * n_kv_heads, rep, table_width);
-  MSPR_REQUIRE(workspace && workspace_bytes >= s.total() && mspr_aligned(workspace, 16),
-               "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", what, s.total(), workspace_bytes);
+  MSPR_REQUIRE(workspace && workspace_bytes >= s.bytes && mspr_aligned(workspace, 16),
+               "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", what, s.bytes, workspace_bytes);
   a = SelectArgs{};
   a.q = q;
   a.requests = requests;
@@ -325,24 +453,11 @@ int select_fill(const char* what, SelectArgs& a, const void* q, int q_dtype, con
   a.recent = recent;
   a.padded = s.padded;
   a.bounds = reinterpret_cast<float*>(workspace);
-  a.most = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + s.bounds);
   return MSPR_OK;
 }
 
 int select_launch(const char* what, const SelectArgs& a, int q_dtype, hipStream_t st) {
   const unsigned rows = (unsigned)(a.rows * a.n_kv);
-  static bool attr_set[64] = {};  // by device
-  constexpr int kMostLds = kMaxTablePages * (int)sizeof(uint32_t);
-  int device = 0;
-  if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64 || !attr_set[device]) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&page_choose_kernel),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, kMostLds);
-    if (e != hipSuccess) {
-      mspr_set_error("%s: cannot reserve %d bytes of LDS: %s", what, kMostLds, hipGetErrorString(e));
-      return MSPR_ERR_LAUNCH;
-    }
-    if (device >= 0 && device < 64) attr_set[device] = true;
-  }
   if (a.width > a.selected) {
     const dim3 grid((unsigned)((a.width + kPagesAGroup - 1) / kPagesAGroup), rows);
     if (q_dtype == MSPR_F32) page_score_kernel<MSPR_F32><<<grid, dim3(64 * kScoreWaves), 0, st>>>(a);
@@ -350,7 +465,15 @@ int select_launch(const char* what, const SelectArgs& a, int q_dtype, hipStream_
     else page_score_kernel<MSPR_BF16><<<grid, dim3(64 * kScoreWaves), 0, st>>>(a);
     MSPR_CHECK_LAUNCH(what);
   }
-  page_choose_kernel<<<dim3(rows), dim3(kChooseThreads), (size_t)a.width * sizeof(uint32_t), st>>>(a);
+  auto choose = [&](auto heads) {
+    constexpr int kHeads = decltype(heads)::value;
+    if (a.width <= 1024) page_choose_kernel<256, 4, kHeads><<<dim3(rows), dim3(256), 0, st>>>(a);
+    else if (a.width <= 4096) page_choose_kernel<512, 8, kHeads><<<dim3(rows), dim3(512), 0, st>>>(a);
+    else if (a.width <= 8192) page_choose_kernel<1024, 8, kHeads><<<dim3(rows), dim3(1024), 0, st>>>(a);
+    else page_choose_kernel<1024, 32, kHeads><<<dim3(rows), dim3(1024), 0, st>>>(a);
+  };
+  if (a.rep <= 8) choose(std::integral_constant<int, 8>{});
+  else choose(std::integral_constant<int, 16>{});
   MSPR_CHECK_LAUNCH(what);
   return MSPR_OK;
 }
@@ -363,7 +486,7 @@ struct SparseScratch {
 SparseScratch sparse_scratch(int rows, int n_q_heads, int n_kv_heads, int page_size, int table_width, int selected) {
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   SparseScratch s;
-  s.select = up(select_scratch((int64_t)rows * n_kv_heads, n_q_heads / n_kv_heads, table_width).total());
+  s.select = up(select_scratch((int64_t)rows * n_kv_heads, n_q_heads / n_kv_heads, table_width).bytes);
   s.tables = up((size_t)rows * n_kv_heads * selected * sizeof(int32_t));
   s.lens = up((size_t)rows * n_kv_heads * sizeof(int32_t));
   s.decode = mspr_sdpa_decode_paged_workspace_bytes(rows * n_kv_heads, n_q_heads / n_kv_heads, 1, page_size, selected);
@@ -409,7 +532,7 @@ int sparse_select(const char* what, const void* q, int q_dtype, const int8_t* co
 
 extern "C" size_t mspr_select_pages_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int table_width) {
   if (!sparse_sizes_ok(batch, n_q_heads, n_kv_heads, 16, table_width, 1)) return 0;
-  return select_scratch((int64_t)batch * n_kv_heads, n_q_heads / n_kv_heads, table_width).total();
+  return select_scratch((int64_t)batch * n_kv_heads, n_q_heads / n_kv_heads, table_width).bytes;
 }
 
 extern "C" int mspr_select_pages(const void* queries, int q_dtype, const int8_t* codes, const float* scales, const int32_t* tables,

@@ -167,6 +167,22 @@ def test_ties_go_to_the_lower_page():
     assert (lens.cpu().numpy()[:, 0] == [592, 585, 581]).all()
 
 
+@pytest.mark.parametrize("width", [1000, 4000, 8000, 20000])
+def test_worths_that_are_alike(width):
+    """Most pages within a hair of each other and one far below, so that they fall into one bin; many of them the same."""
+    rng = np.random.default_rng(width)
+    codes, scales = _some_bounds(rng, 40, 1)
+    codes[1:] = codes[0]
+    codes[1:39, 0, 1, 0] = torch.arange(38, device="cuda").to(torch.int8) + 80
+    scales[:] = 2.0 ** -6
+    codes[39], scales[39] = torch.where(codes[0] > 0, -127, -126), 2.0 ** 20
+    tables = rng.integers(0, 39, (3, width))
+    tables[0, 77], tables[1, 5:50], tables[2, 100:] = 39, -1, 7
+    q = ref.rows(rng, (3, 4, 256), F32).abs()
+    for selected in (3, 30, 700):
+        _check_select(q, codes, scales, tables, [16 * width, 16 * width - 5, 16 * width - 16], 16, selected, 1, 2)
+
+
 def test_pages_that_are_not_in_the_pool_come_last():
     rng = np.random.default_rng(2)
     codes, scales = _some_bounds(rng, 30, 2)
@@ -199,7 +215,7 @@ def test_queries_of_any_size():
         assert at == sorted(set(at)) and at[0] == 0 and at[-2:] == ([62, 63] if r == 0 else [61, 62])
 
 
-@pytest.mark.parametrize("width", [300, 2048, 32768])
+@pytest.mark.parametrize("width", [300, 1024, 1025, 2048, 4100, 8192, 32768])
 def test_long_tables(width):
     rng = np.random.default_rng(width)
     codes, scales = _some_bounds(rng, 700, 2)
