@@ -7,7 +7,7 @@
 //
 // Bound by latency for single tokens (slots, rows, codes one after the other), by HBM for prompts: a key row is read once. A
 // workgroup takes the runs of rows (consecutive slots of one page) that end among `span` rows of the step, of one KV head; its
-// four waves take a run's rows in turn, two 16-bit rows or four 8-bit ones a load, and meet in LDS. 8-bit rows are code * scale +
+// four waves take a run's rows in turn, two 16-bit rows or one 8-bit row a load, and meet in LDS. 8-bit rows are code * scale +
 // bias in 64 bits, where that is exact: a value next to a whole number of steps must not be rounded to it.
 #include "page_bounds.h"
 
@@ -36,10 +36,10 @@ __global__ __launch_bounds__(64 * kWaves) void page_bounds_kernel(const int32_t*
                                                                   int span, int page_shift, int n_pages) {
   constexpr bool kCodes = FMT == kAffineRows;
   using T = std::conditional_t<kCodes, double, float>;
-  constexpr int kElements = kCodes ? 16 : 8;    // channels a lane has of a row
+  constexpr int kElements = kCodes ? 4 : 8;     // channels a lane has of a row
   constexpr int kLanes = 256 / kElements;       // lanes of a row
   constexpr int kRows = 64 / kLanes;            // rows a load
-  constexpr int kAhead = kCodes ? 2 : 8;        // loads in flight
+  constexpr int kAhead = kCodes ? 16 : 8;       // loads in flight: sixteen rows a wave
   const T inf = (T)__builtin_inff();
   __shared__ T edge[2][kWaves * kRows][256];
   __shared__ float tops[kWaves];
@@ -47,14 +47,16 @@ __global__ __launch_bounds__(64 * kWaves) void page_bounds_kernel(const int32_t*
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int n_kv = gridDim.y, kvh = blockIdx.y;
   const int page_mask = (1 << page_shift) - 1;
-  const int r_end = min((int)(blockIdx.x + 1) * span, n_rows);
+  const int r0 = blockIdx.x * span;
   const int mine = lane / kLanes, channel = kElements * (lane % kLanes);
   auto slot_at = [&](int r) { return r >= 0 && r < n_rows ? slots[r] : -1; };
-  for (int r = blockIdx.x * span; r < r_end; r++) {
-    const int slot = __builtin_amdgcn_readfirstlane(slots[r]);
-    const int next = __builtin_amdgcn_readfirstlane(slot_at(r + 1));
+  // which of the span's rows are the last of their run, all at once
+  const int here = lane < span ? slot_at(r0 + lane) : -1, behind = slot_at(r0 + lane + 1);
+  uint64_t ends = __ballot(here >= 0 && here >> page_shift < n_pages && (behind != here + 1 || (here & page_mask) == page_mask));
+  for (; ends; ends &= ends - 1) {
+    const int i_end = __builtin_ctzll(ends), r = r0 + i_end;
+    const int slot = __builtin_amdgcn_readlane(here, i_end);
     const int page = slot >> page_shift, row = slot & page_mask;
-    if (slot < 0 || page >= n_pages || (next == slot + 1 && row != page_mask)) continue;  // (not the last of its run)
     int count = 0;  // rows of the run
     for (int back = 0; back <= row; back += 64) {
       const uint64_t broken = __ballot(back + lane > row || slot_at(r - back - lane) != slot - back - lane);
@@ -81,13 +83,14 @@ __global__ __launch_bounds__(64 * kWaves) void page_bounds_kernel(const int32_t*
       hi[j] = -inf;
     }
     for (int i0 = kRows * wave; i0 < count; i0 += kRows * kWaves * kAhead) {
-      u32x4_t raw[kAhead];
+      std::conditional_t<kCodes, uint32_t, u32x4_t> raw[kAhead];
       float scale[kAhead], bias[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; k++) {
         // (behind the last, the last again)
         const int64_t from = first + min(i0 + kRows * kWaves * k + mine, count - 1);
-        raw[k] = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint8_t*>(keys) + from * (kCodes ? 256 : 512) + 16 * (lane % kLanes));
+        const uint8_t* row_of = reinterpret_cast<const uint8_t*>(keys) + from * (kCodes ? 256 : 512);
+        raw[k] = reinterpret_cast<const std::conditional_t<kCodes, uint32_t, u32x4_t>*>(row_of)[lane % kLanes];
         if constexpr (kCodes) {
           scale[k] = load_as_f32<SDT>(key_scales, from * 4 + channel / 64);
           bias[k] = load_as_f32<SDT>(key_biases, from * 4 + channel / 64);
@@ -98,7 +101,7 @@ __global__ __launch_bounds__(64 * kWaves) void page_bounds_kernel(const int32_t*
 #pragma unroll
         for (int j = 0; j < kElements; j++) {
           T x;
-          if constexpr (kCodes) x = fma((double)((raw[k][j / 4] >> 8 * (j % 4)) & 0xFFu), (double)scale[k], (double)bias[k]);
+          if constexpr (kCodes) x = fma((double)(raw[k] >> 8 * j & 0xFFu), (double)scale[k], (double)bias[k]);
           else if constexpr (FMT == MSPR_F16) x = f16_bits_to_f32((uint16_t)(raw[k][j / 2] >> 16 * (j % 2)));
           else x = bf16_bits_to_f32((uint16_t)(raw[k][j / 2] >> 16 * (j % 2)));
           lo[j] = min_of(lo[j], x);
@@ -156,7 +159,7 @@ __global__ __launch_bounds__(64 * kWaves) void page_bounds_kernel(const int32_t*
   }
 }
 
-// Rows of a step from which on a workgroup looks after sixteen of them.
+// Rows of a step from which on a workgroup looks after sixteen of them (fewer: each after one, which may end a run).
 constexpr int kManyRows = 2048;
 
 template <int FMT, int SDT>
