@@ -1098,23 +1098,20 @@ __device__ __forceinline__ void prefix_piece(const SharedRest& a, const int32_t*
   }
 }
 
-// A piece of a prefix a workgroup.
-template <int FMT>
-__global__ __launch_bounds__(kWideThreads, 1) void paged_prefix_kernel(const int32_t* requests, const int32_t* groups,
-                                                                       const int32_t* prefix_lens, int batch, int n_prefixes,
-                                                                       int n_tables, int n_kv, int rep, SharedRest a) {
-  extern __shared__ __attribute__((aligned(256))) unsigned char lds[];  // tile bases: zero low bits under the address XORs
-  __shared__ int wave_members[kWideWaves];
-  __shared__ int column_row[kWideColumns];
-  __shared__ float xml[kWideWaves / 2][32][2];
+// What a workgroup of the kernels for prefixes does: the plan, in `plan` (LDS where no first copy goes), then its piece by `run`(table, rows,
+// first tile, last, KV head, columns, what finds its members).
+template <typename F>
+__device__ __forceinline__ void prefix_workgroup(const int32_t* requests, const int32_t* groups, const int32_t* prefix_lens, int batch,
+                                                 int n_prefixes, int n_tables, int n_kv, int rep, const SharedRest& a, int step,
+                                                 unsigned char* plan, int* wave_members, int* column_row, F&& run) {
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int number = blockIdx.x;
 
-  // ---- members of every prefix (where no first tile goes)
-  int* row_group = reinterpret_cast<int*>(lds + 2 * kStageBytes);  // [batch]
-  int* length = row_group + kMaxRows;                              // [n_prefixes]
-  int* count = length + kMaxRows;                                  // [n_prefixes]
+  // ---- members of every prefix
+  int* row_group = reinterpret_cast<int*>(plan);  // [batch]
+  int* length = row_group + kMaxRows;             // [n_prefixes]
+  int* count = length + kMaxRows;                 // [n_prefixes]
   const int prefix_cap = a.prefix_width << a.page_shift;
   auto group_of = [&](int r) {
     if (r >= batch) return -1;
@@ -1160,7 +1157,6 @@ __global__ __launch_bounds__(kWideThreads, 1) void paged_prefix_kernel(const int
   // A range's tiles: so many that there are no more pieces than compute units, as a unit has at most one piece that is not full; where
   // there are too many units for that, half as many again. Of few prefixes the least of 64 lengths that does it, tried one a
   // lane (16 queries over 32768 rows of two KV heads: 256 pieces of eight tiles, not 228 of nine).
-  const int step = a.block <= kWideColumns / 2 ? 2 : 1;  // (tiles that the waves take at a time)
   int share = max(kMinShare, ceil_div(all, max(kGroups - units, kGroups / 2)));
   if (n_prefixes <= 16 && all < (1 << 21)) {
     const int tried = (max(kMinShare, ceil_div(all, kGroups)) + step - 1) / step * step + step * lane;
@@ -1233,10 +1229,374 @@ __global__ __launch_bounds__(kWideThreads, 1) void paged_prefix_kernel(const int
   const int tile0 = __builtin_amdgcn_readfirstlane((int)((int64_t)n_tiles * range / ranges));
   const int tile1 = __builtin_amdgcn_readfirstlane((int)((int64_t)n_tiles * (range + 1) / ranges));
   const int columns = __builtin_amdgcn_readfirstlane(n_members * rep);
-  if (columns <= kWideColumns / 2)
-    prefix_piece<FMT, 2>(a, table, len, tile0, tile1, n_kv, kvh, number, columns, column_row, find_members, lds, xml);
-  else
-    prefix_piece<FMT, 1>(a, table, len, tile0, tile1, n_kv, kvh, number, columns, column_row, find_members, lds, xml);
+  run(table, len, tile0, tile1, kvh, columns, find_members);
+}
+
+// A piece of a prefix of 16-bit rows a workgroup.
+template <int FMT>
+__global__ __launch_bounds__(kWideThreads, 1) void paged_prefix_kernel(const int32_t* requests, const int32_t* groups,
+                                                                       const int32_t* prefix_lens, int batch, int n_prefixes,
+                                                                       int n_tables, int n_kv, int rep, SharedRest a) {
+  // (a name of its own: declarations of one name share an alignment, and the tiles' bases need zero low bits under the address XORs)
+  extern __shared__ __attribute__((aligned(256))) unsigned char ring[];
+  __shared__ int wave_members[kWideWaves];
+  __shared__ int column_row[kWideColumns];
+  __shared__ float xml[kWideWaves / 2][32][2];
+  const int step = a.block <= kWideColumns / 2 ? 2 : 1;  // (tiles that the waves take at a time)
+  prefix_workgroup(requests, groups, prefix_lens, batch, n_prefixes, n_tables, n_kv, rep, a, step, ring + 2 * kStageBytes, wave_members,
+                   column_row, [&](const int32_t* table, int len, int tile0, int tile1, int kvh, int columns, auto&& find_members) {
+                     if (columns <= kWideColumns / 2)
+                       prefix_piece<FMT, 2>(a, table, len, tile0, tile1, n_kv, kvh, blockIdx.x, columns, column_row, find_members, ring, xml);
+                     else
+                       prefix_piece<FMT, 1>(a, table, len, tile0, tile1, n_kv, kvh, blockIdx.x, columns, column_row, find_members, ring, xml);
+                   });
+}
+
+// ---------------------------------------------------------------------------------------------- prefixes of 8-bit rows
+
+// Sixteen columns a wave, 128 a block, by 16x16x32 products of codes and queries, as paged_decode.hip makes them. Raw rows come by
+// asynchronous copies into a ring of four tiles; the eight waves together make a tile's codes float16 numbers, a tile ahead of the
+// one they multiply, so that what unpacking costs is shared. Scales and biases are read where the copies put them.
+constexpr int kCodeColumns = 16 * kWideWaves;
+constexpr int kCodeTile = kTileKeys * kD;                  // 8 KB of codes, K and V each
+constexpr int kScaleBytes = 256;                           // sixteen rows of scales or biases (of 16-bit ones half of it)
+constexpr int kRawBytes = 2 * kCodeTile + 8 * kScaleBytes;
+constexpr int kRawSlots = 4;
+constexpr int kRawBase = 2 * kStageBytes;
+constexpr int kCodeLds = kRawBase + kRawSlots * kRawBytes;  // 136 KB
+constexpr int kCodeChunk = 28;                             // tiles whose pages a wave has at hand, with three more behind them
+
+// Lane i's four bytes at base + offset land at lds_base + 4 i.
+__device__ __forceinline__ void copy_4(uint64_t base, uint32_t offset, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, %0" ::"s"(base), "v"(offset), "s"(lds_base) : "memory", "m0");
+}
+// Sixteen-byte piece p of row r lies at place p ^ turn(r): eight rows' pieces, and four rows' pairs of pieces, on all banks.
+__device__ __forceinline__ int turn(int r) { return ((r & 3) << 1) | (r >> 2 & 1); }
+
+template <int SDT>
+__device__ __forceinline__ float scale_at(const unsigned char* region, int i) { return load_as_f32<SDT>(region, i); }
+
+template <int QDT, int SDT, typename F>
+__device__ __forceinline__ void codes_piece(const SharedRest& a, const int32_t* table, int len, int tile0, int tile1, int n_kv, int kvh,
+                                            int slot, int columns, const int* column_row, F&& find_members, unsigned char* lds) {
+  constexpr float kLag = 4.0f, kUp = 11.0f;           // (as in paged_decode.hip)
+  constexpr int kQTerms = QDT == MSPR_F32 ? 2 : 1;
+  constexpr int kSB = SDT == MSPR_F32 ? 4 : 2;
+  constexpr int kCopies = 3;                           // of a wave and tile
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, g = lane >> 4;  // column of the wave's sixteen, key of the K operand; quarter of an operand's depth
+  const int column0 = 16 * wave;
+  const int mine = __builtin_amdgcn_readfirstlane(min(max(columns - column0, 0), 16));
+  const int page_mask = (1 << a.page_shift) - 1;
+
+  // ---- copies: a wave has a quarter of half a tile's K and V codes, and one of the four kinds of scales of that half
+  const int half = wave >> 2, kind = wave & 3;
+  const int c_row = (tid & 255) >> 4, s_row = kSB == 4 ? lane >> 2 : (lane & 31) >> 1;
+  const uint64_t scales = (uint64_t)(kind == 0 ? a.k_scales : kind == 1 ? a.k_biases : kind == 2 ? a.v_scales : a.v_biases);
+  const uint32_t raw0 = __builtin_amdgcn_readfirstlane(lds_address(lds)) + kRawBase;
+  auto load_ids = [&](int t0) {  // lane i: page of half tile i from tile t0 on
+    const int t = t0 + (lane >> 1), key = t * kTileKeys + 16 * (lane & 1);
+    const int e = t < tile1 && key < len ? key >> a.page_shift : -1;
+    return e >= 0 ? table[e] : -1;
+  };
+  // (rows that count, as of the 16-bit form; rows behind them are copies of the last, of half tiles without any codes and scales of zero)
+  auto issue_tile = [&](int ids, int t0, int t) {
+    uint32_t rows = 0;
+    int64_t row = 0;
+    int count = 0;
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const int page = __builtin_amdgcn_readlane(ids, 2 * (t - t0) + u);
+      const int key = t * kTileKeys + 16 * u;
+      const bool good = page >= 0 && page < a.n_pages && t < tile1;
+      const int c = !good ? 0 : len - key >= 16 ? 16 : len - key < 0 ? 0 : len - key;
+      if (u == half) {
+        row = ((((int64_t)(good ? page : 0) * n_kv + kvh) << a.page_shift) + (key & page_mask));
+        count = c;
+      }
+      rows |= (uint32_t)c << 8 * u;
+    }
+    const uint64_t none = (uint64_t)(const void*)g_no_rows;
+    const uint64_t kb = count > 0 ? (uint64_t)a.k + row * kD : none, vb = count > 0 ? (uint64_t)a.v + row * kD : none;
+    const uint64_t sb = count > 0 ? scales + row * 4 * kSB : none;
+    const int last = max(count, 1) - 1;
+    const uint32_t offset = (uint32_t)(min(c_row, last) * kD + (tid & 15) * 16);
+    const uint32_t s_offset = (uint32_t)(min(s_row, last) * 4 * kSB + (lane & (kSB - 1)) * 4);
+    const uint32_t to = raw0 + ((t - tile0) % kRawSlots) * kRawBytes;
+    copy_16(kb, offset, to + wave * 1024);
+    copy_16(vb, offset, to + kCodeTile + wave * 1024);
+    copy_4(sb, s_offset, to + 2 * kCodeTile + (2 * kind + half) * kScaleBytes);
+    return rows;
+  };
+  uint32_t ahead[4];  // rows of the present tile and of the three behind it
+  int ids = load_ids(tile0);
+#pragma unroll
+  for (int i = 0; i < 3; i++) ahead[i] = issue_tile(ids, tile0, tile0 + i);
+  int ids_next = load_ids(tile0 + kCodeChunk);
+  find_members();  // (under the first copies)
+
+  // ---- Q^T operands in registers: lane (n, g) has channels 32 s + 8 g on of step s, scaled by a power of two that brings the
+  //      column's largest element to [2^14, 2^15) (float16 queries as they are)
+  u32x4_t qf[8][kQTerms];
+  float q_unit = a.scale_log2, qsum = 0.0f;  // (sums of the query over group g, for the biases)
+  {
+    constexpr int kWords = QDT == MSPR_F32 ? 2 : 1;
+    u32x4_t raw[8][kWords];
+    const int64_t row = column_row[column0 + n < columns ? column0 + n : 0];
+#pragma unroll
+    for (int s = 0; s < 8; s++)
+#pragma unroll
+      for (int w = 0; w < kWords; w++)
+        raw[s][w] = reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint8_t*>(a.q) +
+                                                     (row * kD + 32 * s + 8 * g) * (QDT == MSPR_F32 ? 4 : 2))[w];
+    auto element = [&](int s, float* x) {
+      if constexpr (QDT == MSPR_F32) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = __uint_as_float(raw[s][j / 4][j % 4]);
+      } else {
+        widen8<QDT>(raw[s][0], x);
+      }
+    };
+    int e = 0;
+    if constexpr (QDT != MSPR_F16) {
+      float top = 0.0f;
+#pragma unroll
+      for (int s = 0; s < 8; s++) {
+        float x[8];
+        element(s, x);
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[j]));
+      }
+      top = half_wave_max(row_pair_max(top));
+      if (top > 0.0f && top < __builtin_inff()) e = __builtin_amdgcn_frexp_expf(top) - 15;
+    }
+    float sums[4] = {};
+#pragma unroll
+    for (int s = 0; s < 8; s++) {
+      float x[8];
+      element(s, x);
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] = __builtin_amdgcn_ldexpf(x[j], -e);
+      split_terms<MSPR_F16, kQTerms>(x, qf[s]);
+#pragma unroll
+      for (int t = 0; t < kQTerms; t++) {  // (of the terms, as the products are)
+        float y[8];
+        widen8<MSPR_F16>(qf[s][t], y);
+#pragma unroll
+        for (int j = 0; j < 8; j++) sums[s / 2] += y[j];
+      }
+    }
+    q_unit = __builtin_amdgcn_ldexpf(q_unit, e);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      sums[j] += __shfl_xor(sums[j], 16, MSPR_WAVE);
+      sums[j] += __shfl_xor(sums[j], 32, MSPR_WAVE);
+    }
+    qsum = g == 0 ? sums[0] : g == 1 ? sums[1] : g == 2 ? sums[2] : sums[3];
+  }
+
+  f32x4_t oacc[16], bacc = {0.f, 0.f, 0.f, 0.f};  // bacc: weighted biases, lane n (g = 0) has those of column n and the four groups
+#pragma unroll
+  for (int mt = 0; mt < 16; mt++) oacc[mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float m_run = -__builtin_inff(), l_run = 0.0f, v_unit = 0x1p-126f;
+  bool begun = false;
+
+  // A tile's codes as float16 numbers, less 128: a thread has sixteen of K and of V.
+  auto unpack = [&](int i) {
+    int tl = tid;
+    asm volatile("" : "+v"(tl));  // (offsets are made here, not carried through the loop)
+    const unsigned char* raw = lds + kRawBase + (i % kRawSlots) * kRawBytes + tl * 16;
+    const int row = tl >> 4, piece = 2 * (tl & 15), f = turn(row);
+    unsigned char* to = lds + (i & 1) * kStageBytes + row * kRowBytes;
+#pragma unroll
+    for (int side = 0; side < 2; side++) {
+      const u32x4_t c = *reinterpret_cast<const u32x4_t*>(raw + side * kCodeTile);
+      u32x4_t p[2];
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        h2_t lo, hi;
+        centred_to_h(c[w], lo, hi);
+        p[w >> 1][2 * (w & 1)] = h2_bits(lo);
+        p[w >> 1][2 * (w & 1) + 1] = h2_bits(hi);
+      }
+      *reinterpret_cast<u32x4_t*>(to + side * kTileBytes + 16 * (piece ^ f)) = p[0];
+      *reinterpret_cast<u32x4_t*>(to + side * kTileBytes + 16 * ((piece + 1) ^ f)) = p[1];
+    }
+  };
+
+  const int k_off0 = n * kRowBytes + 16 * (g ^ turn(n)), k_off1 = n * kRowBytes + 16 * ((4 + g) ^ turn(n));  // + 8192 half + 128 group
+  const int tr_row = 4 * g + (n >> 2);
+  const uint32_t v_off = kTileBytes + tr_row * kRowBytes + 16 * (((n & 3) >> 1) ^ turn(tr_row)) + 8 * (n & 1);
+  auto attend_tile = [&](int i, uint32_t rows) {
+    const unsigned char* st = lds + (i & 1) * kStageBytes;
+    const unsigned char* sc = lds + kRawBase + (i % kRawSlots) * kRawBytes + 2 * kCodeTile;
+    // ---- S^T = K . Q^T: a group's sum takes its scale, biases are products with the query's sums
+    float s[8];  // key 16 u + 4 g + i at 4 u + i
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+      const float ksf = scale_at<SDT>(sc + u * kScaleBytes, 16 * g + n);
+      const float bias = fmaf(128.0f, scale_at<SDT>(sc + u * kScaleBytes, 4 * n + g), scale_at<SDT>(sc + (2 + u) * kScaleBytes, 4 * n + g));
+      f32x4_t sum = __builtin_amdgcn_mfma_f32_16x16x4f32(bias, qsum, zero, 0, 0, 0);
+      static_for<4>([&](auto jc) {
+        constexpr int j = decltype(jc)::value;
+        f32x4_t acc = zero;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const u32x4_t c = *reinterpret_cast<const u32x4_t*>(st + (h ? k_off1 : k_off0) + 8192 * u + 128 * j);
+#pragma unroll
+          for (int t = 0; t < kQTerms; t++) acc = mfma<MSPR_F16>(c, qf[2 * j + h][t], acc);
+        }
+        static_for<4>([&](auto ic) {
+          constexpr int k = decltype(ic)::value;
+          sum[k] = fmaf(of_lane<4 * k + j>(ksf), acc[k], sum[k]);
+        });
+      });
+#pragma unroll
+      for (int k = 0; k < 4; k++) s[4 * u + k] = sum[k] * q_unit;
+    }
+    // ---- online softmax
+    float tmax = -__builtin_inff();
+    if (rows != 0x1010u) {
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        if (4 * g + (k & 3) >= (int)(k < 4 ? rows & 0xFFu : rows >> 8)) s[k] = -__builtin_inff();
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++) tmax = fmaxf(tmax, s[k]);
+    tmax = half_wave_max(row_pair_max(tmax));
+    const bool grow = tmax > m_run + kLag;
+    if (__any(grow)) {
+      const float m_new = grow ? tmax : m_run;
+      if (begun) {
+        const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+        l_run *= alpha;
+#pragma unroll
+        for (int mt = 0; mt < 16; mt++) oacc[mt] = oacc[mt] * alpha;
+        bacc = bacc * alpha;
+      }
+      m_run = m_new;
+    }
+    const float m_safe = (m_run == -__builtin_inff() ? 0.0f : m_run) - kUp;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      s[k] = __builtin_amdgcn_exp2f(s[k] - m_safe);
+      l_run += s[k];
+    }
+    // ---- O^T += V^T . P^T: weights take V's scales, as multiples of a power of two that is as large as any of their group
+    float vsf[2], vbf[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      vsf[u] = scale_at<SDT>(sc + (4 + u) * kScaleBytes, 16 * g + n);
+      vbf[u] = fmaf(128.0f, vsf[u], scale_at<SDT>(sc + (6 + u) * kScaleBytes, 16 * g + n));
+    }
+    const float largest = fmaxf(fabsf(vsf[0]), fabsf(vsf[1]));
+    if (__any(largest > v_unit)) {
+      float top = largest;
+      top = fmaxf(top, lane_xor<4>(top));
+      top = fmaxf(top, lane_xor<8>(top));
+      top = half_wave_max(row_pair_max(top));
+      const int e = top < 0x1p126f ? __builtin_amdgcn_frexp_expf(top) : 126;
+      const float unit = top > v_unit ? __builtin_amdgcn_ldexpf(1.0f, e) : v_unit;
+      if (begun) {
+        const float by = v_unit / unit;
+        static_for<16>([&](auto mt) { oacc[mt] = oacc[mt] * of_lane<decltype(mt)::value / 4>(by); });
+      }
+      v_unit = unit;
+    }
+    begun = true;
+    const float per_unit = 1.0f / v_unit;
+    vsf[0] *= per_unit;
+    vsf[1] *= per_unit;
+    static_for<8>([&](auto ic) {
+      constexpr int k = decltype(ic)::value;
+      float bias = vbf[k >> 2];
+      if constexpr ((k & 3) != 0)
+        bias = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(bias), 0x100 + 4 * (k & 3), 0xF, 0xF, true));  // row_shl
+      bacc = __builtin_amdgcn_mfma_f32_16x16x4f32(bias, s[k], bacc, 0, 0, 0);
+    });
+    const uint32_t vb = lds_address(st) + v_off;
+    static_for<4>([&](auto jc) {  // the weights of group j, which has channels 64 j on
+      constexpr int j = decltype(jc)::value;
+      u32x4_t vf[4], pf[2];
+#pragma unroll
+      for (int m = 0; m < 4; m++) {
+        const uint32_t at = (vb ^ (uint32_t)(m << 5)) + 128 * j;
+        const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, (uintptr_t)at)));
+        const u32x2_t hi =
+            __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, (uintptr_t)(at + 16 * kRowBytes))));
+        vf[m] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
+      }
+      float w[8];
+      static_for<8>([&](auto ic) {
+        constexpr int k = decltype(ic)::value;
+        w[k] = of_lane<4 * (k & 3) + j>(vsf[k >> 2]) * s[k];
+        asm("" : "+v"(w[k]));  // (a rounded product, see paged_decode.hip)
+      });
+      split_terms<MSPR_F16, 2>(w, pf);
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int m = 0; m < 4; m++) oacc[4 * j + m] = mfma<MSPR_F16>(vf[m], pf[t], oacc[4 * j + m]);
+    });
+  };
+
+  // Steps of a wave: what tile i + 1 is made of has landed once its copies have (three a tile, in order) and every wave got here; the
+  // stage and the slot of tile i - 1 are free then.
+  wait_copies_and_barrier<2 * kCopies>();  // (and the plan, where the stages lie, is no longer read)
+  unpack(0);
+  const int n_tiles = tile1 - tile0;
+  for (int i0 = 0; i0 < n_tiles; i0 += kCodeChunk) {
+    const int i_end = min(i0 + kCodeChunk, n_tiles);
+    for (int i = i0; i < i_end; i++) {
+      wait_copies_and_barrier<kCopies>();
+      ahead[3] = issue_tile(ids, tile0 + i0, tile0 + i + 3);  // (behind the last, tiles without rows: what is under way is the same)
+      if (i + 1 < n_tiles) unpack(i + 1);
+      const uint32_t rows = ahead[0];
+#pragma unroll
+      for (int k = 0; k < 3; k++) ahead[k] = ahead[k + 1];
+      if (mine > 0 && rows != 0) attend_tile(i, rows);
+    }
+    ids = ids_next;
+    ids_next = load_ids(tile0 + i0 + 2 * kCodeChunk);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the last copies must not outlive the piece)
+
+  // ---- a wave's columns leave in whole rows, through 16 KB of LDS
+  __syncthreads();  // every wave has left the tiles
+  if (mine == 0) return;
+  l_run += __shfl_xor(l_run, 16, MSPR_WAVE);
+  l_run += __shfl_xor(l_run, 32, MSPR_WAVE);
+  float bias[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) bias[j] = __shfl(bacc[j], n, MSPR_WAVE);
+  int row0 = slot * a.block + column0;  // (a scalar by hand, as of the 16-bit form)
+  asm volatile("" : "+s"(row0));
+  if (g == 0 && n < mine) *reinterpret_cast<f32x4_t*>(a.ws_pre_ml + 4 * (int64_t)(row0 + n)) = f32x4_t{m_run, l_run, 1.0f, 0.0f};
+  unsigned char* xo = lds + (wave << 14);
+  static_for<16>([&](auto mt) {
+    constexpr int m = decltype(mt)::value;
+    *reinterpret_cast<f32x4_t*>(xo + n * 1024 + 16 * ((4 * m + g) ^ n)) = oacc[m] * of_lane<m / 4>(v_unit) + bias[m / 4];
+  });
+  const auto to = store_window(reinterpret_cast<float*>(a.ws_pre) + (int64_t)row0 * kD, mine * kD * 4);
+#pragma unroll
+  for (int r = 0; r < 16; r++)
+    window_store<kStoreThrough>(to, r * 1024 + 16 * lane, *reinterpret_cast<const u32x4_t*>(xo + r * 1024 + 16 * (lane ^ r)));
+}
+
+// A piece of a prefix of 8-bit rows a workgroup.
+template <int QDT, int SDT>
+__global__ __launch_bounds__(kWideThreads, 1) void paged_prefix_codes_kernel(const int32_t* requests, const int32_t* groups,
+                                                                             const int32_t* prefix_lens, int batch, int n_prefixes,
+                                                                             int n_tables, int n_kv, int rep, SharedRest a) {
+  extern __shared__ __attribute__((aligned(256))) unsigned char ring[];
+  __shared__ int wave_members[kWideWaves];
+  __shared__ int column_row[kCodeColumns];
+  prefix_workgroup(requests, groups, prefix_lens, batch, n_prefixes, n_tables, n_kv, rep, a, 1, ring, wave_members, column_row,
+                   [&](const int32_t* table, int len, int tile0, int tile1, int kvh, int columns, auto&& find_members) {
+                     codes_piece<QDT, SDT>(a, table, len, tile0, tile1, n_kv, kvh, blockIdx.x, columns, column_row, find_members, ring);
+                   });
 }
 
 constexpr int kAtOnce = 16;  // pieces that a wave joins at a time
@@ -1245,7 +1605,7 @@ constexpr int kAtOnce = 16;  // pieces that a wave joins at a time
 // paged_decode.hip's parts (own: of rows that are not cut), else pieces of paged_shared_kernel.
 // grid: heads / (kMergeWaves / WAVES)
 constexpr int kMergeWaves = 8;
-template <int ODT, int WAVES, bool PARTS>  // (partials of prefixes are float16 where PARTS and bfloat16 results)
+template <int ODT, int WAVES, bool PARTS, bool HALF>  // HALF: partials of prefixes are scaled float16 numbers
 __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(const int32_t* parts, const void* ws_pre,
                                                                               const float* ws_pre_ml, const float* ws_own,
                                                                               const float* ws_own_ml, int rep, int n_kv, int heads,
@@ -1266,7 +1626,6 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
   const int total = n_own + ranges;
   const int own_first = PARTS ? 0 : at[0], pre_first = at[2], blocks = at[4], column = at[5] + hn;
   const int kvh = row % n_kv;
-  constexpr bool kHalf = PARTS && ODT == MSPR_BF16;
   // Row of prefix piece i (bounded by the workspace, whatever is there), sums and statistics of own piece i
   auto prefix_row = [&](int i) {
     const int s = pre_first + bundle_piece(kvh * ranges + i, column / block, n_kv * ranges, blocks);
@@ -1306,7 +1665,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
       if (i >= total) continue;
       if (i < n_own) {
         ov[j] = *reinterpret_cast<const u32x4_t*>(own_piece(i).o + 4 * lane);
-      } else if constexpr (kHalf) {
+      } else if constexpr (HALF) {
         const u32x2_t h = *reinterpret_cast<const u32x2_t*>(reinterpret_cast<const uint16_t*>(ws_pre) + prefix_row(i - n_own) * kD + 4 * lane);
         ov[j].x = h.x;
         ov[j].y = h.y;
@@ -1334,7 +1693,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
       const int i = p0 + WAVES * j;
       if (i >= total) continue;
       f32x4_t v = __builtin_bit_cast(f32x4_t, ov[j]);
-      if (kHalf && i >= n_own) {
+      if (HALF && i >= n_own) {
         const h2_t lo = bits_h2(ov[j].x), hi = bits_h2(ov[j].y);
         v = f32x4_t{(float)lo.x, (float)lo.y, (float)hi.x, (float)hi.y};
       }
@@ -1369,16 +1728,17 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
 }
 
 // Prefixes are a kernel's own where a block of 32 columns does not hold the call's query heads of a KV head.
-bool wide_prefixes(int batch, int rep, bool codes) { return !codes && (int64_t)batch * rep > kColumns; }
+bool wide_prefixes(int batch, int rep) { return (int64_t)batch * rep > kColumns; }
 
 // Columns of a block of members: 32, or as many as eight waves hold, but no more than twice what a prefix has members on the
 // average, so that the scratch, a place for every column of a block, does not grow with what blocks leave empty.
-int block_columns(int batch, int n_prefixes, int rep, bool wide) {
+int block_columns(int batch, int n_prefixes, int rep, bool wide, bool codes) {
   if (!wide) return kColumns;
+  const int most = codes ? kCodeColumns : kWideColumns;
   const int64_t used = n_prefixes < batch ? n_prefixes : batch;
   const int64_t mean = ((used > 1 ? 2 : 1) * (int64_t)batch * rep + used - 1) / used;
   const int64_t n = (mean + 31) / 32 * 32;
-  return (int)(n < kWideColumns ? n : kWideColumns);
+  return (int)(n < most ? n : most);
 }
 
 // Pieces of `units` units: a call has at most max(kGroups, kGroups / 2 + units), see `share`.
@@ -1401,8 +1761,8 @@ struct SharedScratch {
 };
 SharedScratch shared_scratch(int batch, int n_prefixes, int n_kv, int rep, int page_size, int width, bool codes) {
   SharedScratch s;
-  s.wide = wide_prefixes(batch, rep, codes);
-  s.block = block_columns(batch, n_prefixes, rep, s.wide);
+  s.wide = wide_prefixes(batch, rep);
+  s.block = block_columns(batch, n_prefixes, rep, s.wide, codes);
   const int64_t own = (int64_t)batch * n_kv, blocks = prefix_units(batch, n_prefixes, n_kv, rep, s.block);
   s.pieces = pieces_of(s.wide ? blocks : own + blocks);
   s.prefix_slots = s.wide ? s.pieces : s.pieces - own;  // (every query has a piece of its own, at least)
@@ -1432,13 +1792,13 @@ int reserve_lds(K* kernel, int bytes, bool (&done)[64]) {
 }
 
 // Joins the pieces of `heads` query heads: eight waves a head where they are few and have many pieces, else one.
-template <int QDT, bool PARTS>
+template <int QDT, bool PARTS, bool HALF>
 int merge_launch(const SharedArgs& a, const PagedParts& own, hipStream_t st) {
   const SharedRest& r = a.rest;
   const int heads = a.batch * a.n_kv * a.rep;
   auto merge = [&](auto waves) {
     constexpr int kWavesAHead = decltype(waves)::value, kHeads = kMergeWaves / kWavesAHead;
-    paged_shared_merge_kernel<QDT, kWavesAHead, PARTS><<<dim3((unsigned)((heads + kHeads - 1) / kHeads)), dim3(64 * kMergeWaves), 0, st>>>(
+    paged_shared_merge_kernel<QDT, kWavesAHead, PARTS, HALF><<<dim3((unsigned)((heads + kHeads - 1) / kHeads)), dim3(64 * kMergeWaves), 0, st>>>(
         r.parts, r.ws_pre, r.ws_pre_ml, r.ws_own, r.ws_own_ml, a.rep, a.n_kv, heads, r.block, r.prefix_slots, r.own_slots, own, r.out);
   };
   // (a head has as many pieces as compute units divided by blocks: few where heads are many)
@@ -1456,20 +1816,24 @@ int shared_launch(const SharedArgs& a, hipStream_t st) {
   paged_shared_kernel<QDT, FMT, SDT><<<dim3((unsigned)a.pieces), dim3(kThreads), kLds, st>>>(
       a.requests, a.groups, a.lens, a.prefix_lens, a.batch, a.n_prefixes, a.n_tables, a.n_kv, a.rep, a.rest);
   MSPR_CHECK_LAUNCH("sdpa_decode_paged_shared");
-  return merge_launch<QDT, false>(a, PagedParts{}, st);
+  return merge_launch<QDT, false, false>(a, PagedParts{}, st);
 }
 
-// Own rows, then prefixes.
-template <int FMT>
-int wide_launch(const char* what, const SharedArgs& a, hipStream_t st) {
-  static bool reserved[64] = {};
-  if (int rc = reserve_lds(&paged_prefix_kernel<FMT>, kWideLds, reserved)) return rc;
+// Own rows, then prefixes by `kernel`.
+template <int QDT, bool HALF, typename K>
+int wide_launch(const char* what, const SharedArgs& a, int sb_dtype, K* kernel, int lds, bool (&reserved)[64], hipStream_t st) {
+  if (int rc = reserve_lds(kernel, lds, reserved)) return rc;
   const SharedRest& r = a.rest;
   PagedPartsCall c = {};
   c.q = r.q;
   c.k = r.k;
   c.v = r.v;
-  c.q_dtype = FMT;
+  c.k_scales = r.k_scales;
+  c.k_biases = r.k_biases;
+  c.v_scales = r.v_scales;
+  c.v_biases = r.v_biases;
+  c.q_dtype = QDT;
+  c.sb_dtype = sb_dtype;
   c.tables = r.tables;
   c.lens = a.lens;
   c.requests = a.requests;
@@ -1487,10 +1851,22 @@ int wide_launch(const char* what, const SharedArgs& a, hipStream_t st) {
   c.workspace_bytes = a.decode_bytes;
   PagedParts own;
   if (int rc = mspr_paged_decode_parts(what, c, &own, st)) return rc;
-  paged_prefix_kernel<FMT><<<dim3((unsigned)a.pieces), dim3(kWideThreads), kWideLds, st>>>(
-      a.requests, a.groups, a.prefix_lens, a.batch, a.n_prefixes, a.n_tables, a.n_kv, a.rep, r);
+  kernel<<<dim3((unsigned)a.pieces), dim3(kWideThreads), lds, st>>>(a.requests, a.groups, a.prefix_lens, a.batch, a.n_prefixes, a.n_tables,
+                                                                    a.n_kv, a.rep, r);
   MSPR_CHECK_LAUNCH("sdpa_decode_paged_shared (prefixes)");
-  return merge_launch<FMT, true>(a, own, st);
+  return merge_launch<QDT, true, HALF>(a, own, st);
+}
+template <int FMT>
+int rows_launch(const SharedArgs& a, hipStream_t st) {
+  static bool reserved[64] = {};
+  if (!a.wide) return shared_launch<FMT, FMT, FMT>(a, st);
+  return wide_launch<FMT, FMT == MSPR_BF16>("sdpa_decode_paged_shared", a, FMT, &paged_prefix_kernel<FMT>, kWideLds, reserved, st);
+}
+template <int QDT, int SDT>
+int codes_launch(const SharedArgs& a, hipStream_t st) {
+  static bool reserved[64] = {};
+  if (!a.wide) return shared_launch<QDT, kAffine, SDT>(a, st);
+  return wide_launch<QDT, false>("sdpa_decode_paged_shared_q8", a, SDT, &paged_prefix_codes_kernel<QDT, SDT>, kCodeLds, reserved, st);
 }
 
 int shared_fill(const char* what, SharedArgs& a, bool codes, const void* q, const void* k, const void* v, const int32_t* prefix_tables,
@@ -1562,9 +1938,9 @@ int shared_fill(const char* what, SharedArgs& a, bool codes, const void* q, cons
 
 template <int QDT>
 int shared_q8_launch(const SharedArgs& a, int sb_dtype, hipStream_t st) {
-  if (sb_dtype == MSPR_F32) return shared_launch<QDT, kAffine, MSPR_F32>(a, st);
-  if (sb_dtype == MSPR_F16) return shared_launch<QDT, kAffine, MSPR_F16>(a, st);
-  return shared_launch<QDT, kAffine, MSPR_BF16>(a, st);
+  if (sb_dtype == MSPR_F32) return codes_launch<QDT, MSPR_F32>(a, st);
+  if (sb_dtype == MSPR_F16) return codes_launch<QDT, MSPR_F16>(a, st);
+  return codes_launch<QDT, MSPR_BF16>(a, st);
 }
 
 }  // namespace
@@ -1594,9 +1970,7 @@ extern "C" int mspr_sdpa_decode_paged_shared(const void* queries, const void* k_
                            n_tables, table_width, scale, out, workspace, workspace_bytes))
     return rc;
   hipStream_t st = (hipStream_t)stream;
-  if (a.wide) return dtype == MSPR_F16 ? wide_launch<MSPR_F16>("sdpa_decode_paged_shared", a, st) : wide_launch<MSPR_BF16>("sdpa_decode_paged_shared", a, st);
-  if (dtype == MSPR_F16) return shared_launch<MSPR_F16, MSPR_F16, MSPR_F16>(a, st);
-  return shared_launch<MSPR_BF16, MSPR_BF16, MSPR_BF16>(a, st);
+  return dtype == MSPR_F16 ? rows_launch<MSPR_F16>(a, st) : rows_launch<MSPR_BF16>(a, st);
 }
 
 extern "C" int mspr_sdpa_decode_paged_shared_q8(const void* queries, int q_dtype, const void* k_wq, const void* k_scales,

@@ -6,7 +6,8 @@ import pytest
 
 from moespresso_amd import _lib
 
-TILE, GROUPS, MIN_SHARE, DIM, WIDE, NARROW = 32, 256, 4, 256, 256, 32
+TILE, GROUPS, MIN_SHARE, DIM, NARROW = 32, 256, 4, 256, 32
+ROWS, CODES = 256, 128  # columns of a block where prefixes are a kernel's own, of 16-bit and of 8-bit rows
 
 
 def _ceil(a, b):
@@ -14,9 +15,9 @@ def _ceil(a, b):
 
 
 def _block(batch, n_prefixes, rep, wide):
-    """Columns of a block of members, at most."""
+    """Columns of a block of members, at most (wide: as many; 0: both kinds of rows in one launch)."""
     used = min(n_prefixes, batch)
-    return min(WIDE, _ceil(_ceil((2 if used > 1 else 1) * batch * rep, used), 32) * 32) if wide else NARROW
+    return min(wide, _ceil(_ceil((2 if used > 1 else 1) * batch * rep, used), 32) * 32) if wide else NARROW
 
 
 def _pieces_of(units):
@@ -59,7 +60,7 @@ def _bundle_piece(bundle, block, bundles, blocks):
     return 8 * blocks * q + block * min(8, bundles - 8 * q) + bundle % 8
 
 
-@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("wide", [0, CODES, ROWS])
 @pytest.mark.parametrize("batch,n_prefixes,n_kv,rep,most_prefix,most", [
     (1, 1, 1, 1, 40, 40), (2, 1, 2, 8, 137, 40), (16, 1, 2, 8, 32768, 512), (61, 5, 2, 8, 9001, 2000), (256, 1, 2, 8, 8192, 700),
     (33, 1, 2, 8, 20001, 300), (7, 20, 4, 5, 900, 90), (300, 300, 1, 16, 2000, 10), (2048, 3, 8, 1, 300, 60), (40, 2, 1, 3, 0, 500),
@@ -83,7 +84,7 @@ def test_every_tile_is_met_once_and_every_partial_has_a_place(batch, n_prefixes,
         own = [(b, r, t, at - of_prefixes) for b, r, t, at in own]
         assert pieces <= grid and of_prefixes <= prefix_slots and pieces - of_prefixes <= own_slots
     else:
-        prefixes, of_prefixes = _plan(prefix_tiles, blocks, n_kv, 0, 2 if block <= 128 else 1)
+        prefixes, of_prefixes = _plan(prefix_tiles, blocks, n_kv, 0, 2 if wide == ROWS and block <= 128 else 1)
         own = []  # (dealt out as test_paged_decode_model.py has it)
         assert of_prefixes <= grid and of_prefixes <= prefix_slots
     met, places = {}, set()
@@ -132,5 +133,5 @@ def test_the_workspace_holds_every_place(batch, hq, hkv, page, width, n_prefixes
         n = 4 * n + _ceil(own_slots * (8 if wide else 128), 16) * 16 + batch * hkv * 32
         return n + (lib.mspr_sdpa_decode_paged_workspace_bytes(batch, hq, hkv, page, width) if wide else 0)
 
-    most = max(bytes_of(False), bytes_of(True) if batch * rep > NARROW else 0)
+    most = bytes_of(0) if batch * rep <= NARROW else max(bytes_of(CODES), bytes_of(ROWS))
     assert lib.mspr_sdpa_decode_paged_shared_workspace_bytes(batch, hq, hkv, page, width, n_prefixes) == most
