@@ -1273,6 +1273,18 @@ __device__ __forceinline__ void copy_4(uint64_t base, uint32_t offset, uint32_t 
 // Sixteen-byte piece p of row r lies at place p ^ turn(r): eight rows' pieces, and four rows' pairs of pieces, on all banks.
 __device__ __forceinline__ int turn(int r) { return ((r & 3) << 1) | (r >> 2 & 1); }
 
+// Eight weights as two float16 terms each: the first cut off instead of rounded (half the instructions), which the second, a rounded
+// rest of at most 2^-10 of the weight, makes up for.
+__device__ __forceinline__ void cut_terms(const float* x, u32x4_t* t) {
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const h2_t h = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(x[2 * j], x[2 * j + 1]));
+    t[0][j] = h2_bits(h);
+    const h2_t rest = {(_Float16)fmaf((float)h.x, -1.0f, x[2 * j]), (_Float16)fmaf((float)h.y, -1.0f, x[2 * j + 1])};
+    t[1][j] = h2_bits(rest);
+  }
+}
+
 template <int SDT>
 __device__ __forceinline__ float scale_at(const unsigned char* region, int i) { return load_as_f32<SDT>(region, i); }
 
@@ -1428,29 +1440,38 @@ __device__ __forceinline__ void codes_piece(const SharedRest& a, const int32_t* 
   const int k_off0 = n * kRowBytes + 16 * (g ^ turn(n)), k_off1 = n * kRowBytes + 16 * ((4 + g) ^ turn(n));  // + 8192 half + 128 group
   const int tr_row = 4 * g + (n >> 2);
   const uint32_t v_off = kTileBytes + tr_row * kRowBytes + 16 * (((n & 3) >> 1) ^ turn(tr_row)) + 8 * (n & 1);
-  auto attend_tile = [&](int i, uint32_t rows) {
+  // K operands of half a tile: [step]
+  auto read_k = [&](int i, int u, u32x4_t* kf) {
+    const unsigned char* st = lds + (i & 1) * kStageBytes + 8192 * u;
+#pragma unroll
+    for (int s = 0; s < 8; s++) kf[s] = *reinterpret_cast<const u32x4_t*>(st + ((s & 1) ? k_off1 : k_off0) + 128 * (s >> 1));
+  };
+  auto attend_tile = [&](int i, uint32_t rows, u32x4_t (*kf)[8]) {
     const unsigned char* st = lds + (i & 1) * kStageBytes;
     const unsigned char* sc = lds + kRawBase + (i % kRawSlots) * kRawBytes + 2 * kCodeTile;
     // ---- S^T = K . Q^T: a group's sum takes its scale, biases are products with the query's sums
     float s[8];  // key 16 u + 4 g + i at 4 u + i
+    read_k(i, 1, kf[1]);
 #pragma unroll
     for (int u = 0; u < 2; u++) {
       const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
       const float ksf = scale_at<SDT>(sc + u * kScaleBytes, 16 * g + n);
       const float bias = fmaf(128.0f, scale_at<SDT>(sc + u * kScaleBytes, 4 * n + g), scale_at<SDT>(sc + (2 + u) * kScaleBytes, 4 * n + g));
+      f32x4_t acc[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) acc[j] = zero;
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int t = 0; t < kQTerms; t++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) acc[j] = mfma<MSPR_F16>(kf[u][2 * j + h], qf[2 * j + h][t], acc[j]);
       f32x4_t sum = __builtin_amdgcn_mfma_f32_16x16x4f32(bias, qsum, zero, 0, 0, 0);
       static_for<4>([&](auto jc) {
         constexpr int j = decltype(jc)::value;
-        f32x4_t acc = zero;
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const u32x4_t c = *reinterpret_cast<const u32x4_t*>(st + (h ? k_off1 : k_off0) + 8192 * u + 128 * j);
-#pragma unroll
-          for (int t = 0; t < kQTerms; t++) acc = mfma<MSPR_F16>(c, qf[2 * j + h][t], acc);
-        }
         static_for<4>([&](auto ic) {
           constexpr int k = decltype(ic)::value;
-          sum[k] = fmaf(of_lane<4 * k + j>(ksf), acc[k], sum[k]);
+          sum[k] = fmaf(of_lane<4 * k + j>(ksf), acc[j][k], sum[k]);
         });
       });
 #pragma unroll
@@ -1516,29 +1537,35 @@ __device__ __forceinline__ void codes_piece(const SharedRest& a, const int32_t* 
         bias = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(bias), 0x100 + 4 * (k & 3), 0xF, 0xF, true));  // row_shl
       bacc = __builtin_amdgcn_mfma_f32_16x16x4f32(bias, s[k], bacc, 0, 0, 0);
     });
+    // (operands of the next group of channels are read while this one's weights are made)
     const uint32_t vb = lds_address(st) + v_off;
-    static_for<4>([&](auto jc) {  // the weights of group j, which has channels 64 j on
-      constexpr int j = decltype(jc)::value;
-      u32x4_t vf[4], pf[2];
+    u32x4_t vf[2][4];
+    auto read_v = [&](int j) {
 #pragma unroll
       for (int m = 0; m < 4; m++) {
         const uint32_t at = (vb ^ (uint32_t)(m << 5)) + 128 * j;
         const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, (uintptr_t)at)));
         const u32x2_t hi =
             __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(MSPR_LDS_PTR(s16x4_t, (uintptr_t)(at + 16 * kRowBytes))));
-        vf[m] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
+        vf[j & 1][m] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
       }
+    };
+    read_v(0);
+    static_for<4>([&](auto jc) {  // the weights of group j, which has channels 64 j on
+      constexpr int j = decltype(jc)::value;
+      if constexpr (j < 3) read_v(j + 1);
       float w[8];
       static_for<8>([&](auto ic) {
         constexpr int k = decltype(ic)::value;
         w[k] = of_lane<4 * (k & 3) + j>(vsf[k >> 2]) * s[k];
         asm("" : "+v"(w[k]));  // (a rounded product, see paged_decode.hip)
       });
-      split_terms<MSPR_F16, 2>(w, pf);
+      u32x4_t pf[2];
+      cut_terms(w, pf);
 #pragma unroll
       for (int t = 0; t < 2; t++)
 #pragma unroll
-        for (int m = 0; m < 4; m++) oacc[4 * j + m] = mfma<MSPR_F16>(vf[m], pf[t], oacc[4 * j + m]);
+        for (int m = 0; m < 4; m++) oacc[4 * j + m] = mfma<MSPR_F16>(vf[j & 1][m], pf[t], oacc[4 * j + m]);
     });
   };
 
@@ -1552,11 +1579,13 @@ __device__ __forceinline__ void codes_piece(const SharedRest& a, const int32_t* 
     for (int i = i0; i < i_end; i++) {
       wait_copies_and_barrier<kCopies>();
       ahead[3] = issue_tile(ids, tile0 + i0, tile0 + i + 3);  // (behind the last, tiles without rows: what is under way is the same)
+      u32x4_t kf[2][8];
+      if (mine > 0) read_k(i, 0, kf[0]);  // (under the unpacking)
       if (i + 1 < n_tiles) unpack(i + 1);
       const uint32_t rows = ahead[0];
 #pragma unroll
       for (int k = 0; k < 3; k++) ahead[k] = ahead[k + 1];
-      if (mine > 0 && rows != 0) attend_tile(i, rows);
+      if (mine > 0 && rows != 0) attend_tile(i, rows, kf);
     }
     ids = ids_next;
     ids_next = load_ids(tile0 + i0 + 2 * kCodeChunk);
