@@ -9,9 +9,14 @@ A step of a server, every part of it enqueued without waiting for the device:
 
 * ``page_step`` takes and gives back pages and names a slot for every new row,
 * ``qk_norm_rope_append`` (each layer) normalises and rotates queries and keys and writes keys and values to their slots,
-* ``sdpa_decode_paged`` / ``sdpa_decode_paged_q8`` (each layer) attends every new query over its request's pages.
+* ``sdpa_decode_paged`` / ``sdpa_decode_paged_q8`` (each layer) attends every new query over its request's pages,
+* in its place, for requests that continue a prefix they share (a system prompt, a document): ``sdpa_decode_paged_shared`` and
+  ``_q8``, which read the rows of a prefix once for all of them,
+* or, for long requests, ``page_bounds`` (each layer, behind the append) and ``sdpa_decode_paged_sparse`` and ``_q8``, which attend
+  the pages alone that ``select_pages`` finds to matter most.
 
-``PageTables``, ``PagedKVCache`` and ``PagedAttention`` hold what such a server keeps: the tables, a layer's pages, a layer.
+``PageTables``, ``PagedKVCache`` and ``PagedAttention`` hold what such a server keeps: the tables (and the prefixes), a layer's
+pages (and their bounds), a layer.
 """
 
 from __future__ import annotations
@@ -521,10 +526,15 @@ def page_bounds(slots, keys, codes, scales):
     _lib.check(rc, "page_bounds")
 
 
-def _check_selection(R, heads, tables, n_selected, first, recent):
+def _check_selected(n_selected, first, recent):
     n_selected, first, recent = int(n_selected), int(first), int(recent)
     if not 1 <= n_selected <= MAX_SELECTED or first < 0 or recent < 1 or first + recent > n_selected:
         raise ValueError(f"n_selected must be 1 to {MAX_SELECTED}, first 0 or more, recent 1 or more, and both together no more than n_selected")
+    return n_selected, first, recent
+
+
+def _check_selection(R, heads, tables, n_selected, first, recent):
+    n_selected, first, recent = _check_selected(n_selected, first, recent)
     if int(tables.shape[1]) > MAX_TABLE_PAGES:
         raise ValueError(f"tables must hold at most {MAX_TABLE_PAGES} pages a request")
     if R * heads > 65535:
@@ -661,29 +671,64 @@ def sdpa_decode_paged_sparse_q8(queries, k_wq, k_scales, k_biases, v_wq, v_scale
 
 
 class PageTables:
-    """Lengths, tables and the stack of free pages of up to ``batch`` requests, shared by the layers of a model."""
+    """Lengths, tables and the stack of free pages of up to ``batch`` requests, shared by the layers of a model.
 
-    def __init__(self, batch: int, n_pages: int, page_size: int = 64, max_tokens: int = 131072, device="cuda"):
+    With ``n_prefixes`` there are as many requests more, behind the others, which hold prefixes: places ``batch`` to ``batch +
+    n_prefixes - 1`` of ``new_lens``. A prefix gets its rows like any request (in one step or some) and gives its pages back
+    like any; a request that ``continue_prefix`` named to continue it sees its rows in front of its own, and is counted on from
+    its length. It has to stay as it is while requests continue it. (``n_prefixes=0``: none, and nothing is computed for them.)
+    """
+
+    def __init__(self, batch: int, n_pages: int, page_size: int = 64, max_tokens: int = 131072, device="cuda", *,
+                 n_prefixes: int = 0):
         _check_page_size(page_size)
-        self.page_size = page_size
+        if n_prefixes < 0 or (n_prefixes > 0 and not 1 <= batch <= MAX_REQUESTS - n_prefixes):
+            raise ValueError(f"requests and prefixes must be 1 to {MAX_REQUESTS} together")
+        self.page_size, self.batch, self.n_prefixes = page_size, batch, n_prefixes
+        batch += n_prefixes
         self.lens = torch.zeros((batch,), dtype=torch.int32, device=device)
         self.tables = torch.full((batch, -(-max_tokens // page_size)), -1, dtype=torch.int32, device=device)
         self.free_pages = torch.arange(n_pages, dtype=torch.int32, device=device)
         self.head = torch.zeros((1,), dtype=torch.int32, device=device)
+        # the prefix that a request continues, -1: none
+        self.groups = torch.full((batch,), -1, dtype=torch.int32, device=device) if n_prefixes else None
+
+    def continue_prefix(self, request: int, prefix):
+        """``request`` continues ``prefix`` (from 0 on; None: none) from now on: before its first row. It stays so until said otherwise."""
+        if self.groups is None or not 0 <= request < self.batch or not (prefix is None or 0 <= prefix < self.n_prefixes):
+            raise ValueError(f"{request} is no request, or {prefix} no prefix, of these tables")
+        self.groups[request] = -1 if prefix is None else prefix
+
+    @property
+    def prefixes(self):
+        """``(prefix_tables, prefix_lens, groups)`` of ``sdpa_decode_paged_shared``; None without prefixes."""
+        return None if self.groups is None else (self.tables[self.batch:], self.lens[self.batch:], self.groups)
 
     def step(self, new_lens, n_rows: int) -> PageStep:
-        """``page_step`` that carries the lengths and the stack on (in place, so that a captured step follows them)."""
+        """``page_step`` that carries the lengths and the stack on (in place, so that a captured step follows them); positions
+        of requests that continue a prefix are counted from its first row. (Rows without a slot belong to no request then: they
+        would see the prefix.)"""
         step = page_step(self.lens, new_lens, self.tables, self.free_pages, self.head, page_size=self.page_size, n_rows=n_rows)
         self.lens.copy_(step.lens)
         self.head.copy_(step.head)
-        return step
+        if self.groups is None:
+            return step
+        # (places that are none wrap round and are masked; a prefix outside the tables is none, as for the operators)
+        known = (self.groups >= 0) & (self.groups < self.n_prefixes)
+        before = torch.where(known, self.lens[self.batch:][torch.where(known, self.groups, 0)], 0)
+        return step._replace(positions=step.positions + torch.where(step.requests >= 0, before[step.requests], 0),
+                             requests=torch.where(step.slots >= 0, step.requests, -1))
 
 
 class PagedKVCache:
-    """The pages of one layer: 16-bit rows of ``dtype``, or affine 8-bit rows with scales of ``dtype`` (``quantized``)."""
+    """The pages of one layer: 16-bit rows of ``dtype``, or affine 8-bit rows with scales of ``dtype`` (``quantized``).
+
+    With ``bounds`` every append keeps up the bounds of the pages' keys (``codes`` and ``scales`` of ``page_bounds``: 516 bytes a page
+    and KV head), from which ``attend`` can select pages.
+    """
 
     def __init__(self, n_pages: int, n_kv_heads: int, page_size: int = 64, dtype=torch.bfloat16, quantized: bool = False,
-                 device="cuda"):
+                 device="cuda", *, bounds: bool = False):
         _check_page_size(page_size)
         self.quantized = quantized
         shape = (n_pages, n_kv_heads, page_size)
@@ -696,21 +741,44 @@ class PagedKVCache:
                     torch.zeros(shape + (_HEAD_DIM // _GROUP,), dtype=dtype, device=device))
 
         self.keys, self.values = side(), side()
+        self.codes = torch.zeros((n_pages, n_kv_heads, 2, _HEAD_DIM), dtype=torch.int8, device=device) if bounds else None
+        self.scales = torch.ones((n_pages, n_kv_heads), dtype=torch.float32, device=device) if bounds else None
 
     def append(self, q, k, v, q_weight, k_weight, positions, inv_freq, slots, *, eps: float = 1e-6, sections=None):
-        """``qk_norm_rope_append`` into these pages."""
-        return qk_norm_rope_append(q, k, v, q_weight, k_weight, positions, inv_freq, slots, self.keys, self.values, eps=eps,
-                                   sections=sections)
+        """``qk_norm_rope_append`` into these pages, and ``page_bounds`` where they have bounds."""
+        q = qk_norm_rope_append(q, k, v, q_weight, k_weight, positions, inv_freq, slots, self.keys, self.values, eps=eps,
+                                sections=sections)
+        if self.codes is not None:
+            page_bounds(slots, self.keys, self.codes, self.scales)
+        return q
 
-    def attend(self, queries, tables, lens, scale, *, requests=None, workspace=None):
-        """One query a request over these pages (float32 queries over 16-bit rows are rounded to the rows' type)."""
+    def attend(self, queries, tables, lens, scale, *, requests=None, workspace=None, prefixes=None, selected=None):
+        """One query a request over these pages (float32 queries over 16-bit rows are rounded to the rows' type).
+
+        Args:
+            prefixes: ``(prefix_tables, prefix_lens, groups)``, for ``sdpa_decode_paged_shared``.
+            selected: ``(n_selected, first, recent)``, for ``sdpa_decode_paged_sparse`` over the pages' bounds. Not with ``prefixes``.
+        """
+        kind, extra, where, kwargs = "", (), (), dict(requests=requests, workspace=workspace)
+        if prefixes is not None:
+            kind, where = "_shared", tuple(prefixes)
+        if selected is not None:
+            if prefixes is not None:
+                raise ValueError("pages are selected of requests that continue no prefix")
+            if self.codes is None:
+                raise ValueError("pages without bounds cannot be selected from")
+            n_selected, kwargs["first"], kwargs["recent"] = selected
+            kind, where, extra = "_sparse", (self.codes, self.scales), (n_selected,)
         if self.quantized:
-            return sdpa_decode_paged_q8(queries, *self.keys, *self.values, tables, lens, scale, requests=requests,
-                                        workspace=workspace)
-        if queries.dtype != torch.float32:
-            return sdpa_decode_paged(queries, self.keys, self.values, tables, lens, scale, requests=requests, workspace=workspace)
-        return sdpa_decode_paged(queries.to(self.keys.dtype), self.keys, self.values, tables, lens, scale, requests=requests,
-                                 workspace=workspace).float()
+            return _ATTEND[kind + "_q8"](queries, *self.keys, *self.values, *where, tables, lens, scale, *extra, **kwargs)
+        asked = queries.to(self.keys.dtype) if queries.dtype == torch.float32 else queries
+        out = _ATTEND[kind](asked, self.keys, self.values, *where, tables, lens, scale, *extra, **kwargs)
+        return out.float() if queries.dtype == torch.float32 else out
+
+
+# what a cache attends with, by what is to be left out or shared
+_ATTEND = {"": sdpa_decode_paged, "_q8": sdpa_decode_paged_q8, "_shared": sdpa_decode_paged_shared,
+           "_shared_q8": sdpa_decode_paged_shared_q8, "_sparse": sdpa_decode_paged_sparse, "_sparse_q8": sdpa_decode_paged_sparse_q8}
 
 
 class _NoGradient(torch.autograd.Function):
@@ -779,11 +847,15 @@ class PagedAttention(torch.nn.Module):
     anew from these: a norm or rope that can be called and gives something else is refused, and so are hooks on them. A block
     may come without ``eps``, ``inv_freq`` or ``sections`` where only the wrapper uses it; this layer needs them.
 
+    Where the tables hold prefixes (``n_prefixes`` of ``PageTables``), requests attend the prefix they continue and their own rows. With
+    ``n_selected`` (and a cache with ``bounds``) every row attends the pages alone that ``select_pages`` takes for it, ``first`` and
+    ``recent`` ones among them: all there are while a request has no more.
+
     The layer serves: a backward pass that would have to go through its attention raises (the gate and the projection behind it
     alone would leave gradients that lack a part).
     """
 
-    def __init__(self, inner, cache: PagedKVCache):
+    def __init__(self, inner, cache: PagedKVCache, *, n_selected=None, first: int = 1, recent: int = 2):
         super().__init__()
         if inner.q_norm.eps != inner.k_norm.eps:
             raise ValueError("q_norm and k_norm must share an eps")
@@ -793,11 +865,41 @@ class PagedAttention(torch.nn.Module):
         if inner.num_attention_heads % kv_heads != 0 or not 1 <= inner.num_attention_heads // kv_heads <= 16:
             raise ValueError("query heads must be a multiple (at most 16x) of the KV heads")
         _check_modules(inner)
+        self.selected = None
+        if n_selected is not None:
+            self.selected = _check_selected(n_selected, first, recent)
+            if cache.codes is None:
+                raise ValueError("pages are selected by their bounds: the cache must have them")
+            if inner.scale < 0:
+                raise ValueError("pages are selected where the softmax scale is not negative")
+            if self.n_pages * kv_heads * self.page_size > 0x7FFFFFFF:
+                raise ValueError("pages are selected of pools of fewer than 2^31 tokens times KV heads")
         self.inner = inner
         self.cache = cache
 
-    def forward(self, x, step: PageStep, tables: PageTables, positions=None):
-        """``x``: ``[n_rows, hidden]``, the rows of ``step``. ``positions``: int32 ``[3, n_rows]`` where the rope has sections."""
+    def _most(self, tables, selected):
+        """Queries of one call; none of them without a reason that is raised, before anything is written."""
+        kv_heads, width = self.inner.num_key_value_heads, int(tables.tables.shape[1])
+        most = _queries_a_call(kv_heads, tables.page_size, width)
+        if tables.groups is not None:
+            if selected is not None:
+                raise ValueError("pages are selected of requests that continue no prefix: ask for dense=True, or for tables without")
+            # (at most a block of columns a query and KV head, and its own rows)
+            most = min(MAX_SHARED, 0x3FFFFFFF // (2 * kv_heads * (-(-width * tables.page_size // 32) + 1)))
+        if selected is not None:
+            if width > MAX_TABLE_PAGES:
+                raise ValueError(f"pages are selected from tables of at most {MAX_TABLE_PAGES} pages")
+            # (a query and KV head is a request to the attention over its pages; 2048 queries keep the scratch, a word for every
+            # query head and page of its table, within reach)
+            tiles = -(-selected[0] * tables.page_size // 32) + 1
+            most = min(2048, 65535 // kv_heads, 0x3FFFFFFF // (kv_heads * tiles)) if tiles <= 0x2000000 else 0
+        if most < 1:
+            raise ValueError("the tables hold too many tokens together")
+        return most
+
+    def forward(self, x, step: PageStep, tables: PageTables, positions=None, *, dense: bool = False):
+        """``x``: ``[n_rows, hidden]``, the rows of ``step``. ``positions``: int32 ``[3, n_rows]`` where the rope has sections.
+        ``dense``: this step attends all pages, also where the layer selects (the steps of a prompt)."""
         inner = self.inner
         for module in (inner.q_norm, inner.k_norm, inner.rope):
             if getattr(module, "_forward_hooks", None) or getattr(module, "_forward_pre_hooks", None):
@@ -806,9 +908,13 @@ class PagedAttention(torch.nn.Module):
         heads, kv_heads = inner.num_attention_heads, inner.num_key_value_heads
         if tables.page_size != self.page_size or int(tables.free_pages.shape[0]) > self.n_pages:
             raise ValueError("the tables name pages of another size, or more of them, than the cache has")
-        most = _queries_a_call(kv_heads, tables.page_size, int(tables.tables.shape[1]))
-        if most < 1:  # (before anything is written)
-            raise ValueError("the tables hold too many tokens together")
+        selected = None if dense else self.selected
+        most = self._most(tables, selected)
+        asked = {}
+        if tables.groups is not None:
+            asked["prefixes"] = tables.prefixes
+        if selected is not None:
+            asked["selected"] = selected
         # (widths in full: a step in which every request ends has no rows, of which a width could not be told)
         q, gate = inner.q_proj(x).reshape(T, heads, 2 * _HEAD_DIM).chunk(2, dim=-1)
         k = inner.k_proj(x).reshape(T, kv_heads, _HEAD_DIM)
@@ -818,10 +924,10 @@ class PagedAttention(torch.nn.Module):
                               step.positions if positions is None else positions, inner.rope.inv_freq, step.slots,
                               eps=inner.q_norm.eps, sections=None if positions is None else inner.rope.sections)
         if T <= most:
-            out = self.cache.attend(q, tables.tables, step.visible, inner.scale, requests=step.requests)
+            out = self.cache.attend(q, tables.tables, step.visible, inner.scale, requests=step.requests, **asked)
         else:
             out = torch.cat([self.cache.attend(q[i:i + most], tables.tables, step.visible[i:i + most], inner.scale,
-                                               requests=step.requests[i:i + most]) for i in range(0, T, most)])
+                                               requests=step.requests[i:i + most], **asked) for i in range(0, T, most)])
         if torch.is_grad_enabled() and any(t.requires_grad for t in made_from):
             out = _NoGradient.apply(out, *made_from)
         return inner.o_proj((out * torch.sigmoid(gate)).reshape(T, heads * _HEAD_DIM))
