@@ -39,7 +39,7 @@ struct Cut {
     row = cut[3 * entry];
     first = cut[3 * entry + 1];
     const int last = min(cut[3 * entry + 2], shares - 1);
-    count = row < 0 || row >= rows || first < 0 || first > last ? 0 : last - first + 1;
+    count = ((row < 0) | (row >= rows) | (first < 0) | (first > last)) ? 0 : last - first + 1;  // (one wait for the three)
   }
 };
 

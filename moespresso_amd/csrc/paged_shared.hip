@@ -1264,6 +1264,7 @@ constexpr int kRawBytes = 2 * kCodeTile + 8 * kScaleBytes;
 constexpr int kRawSlots = 4;
 constexpr int kRawBase = 2 * kStageBytes;
 constexpr int kCodeLds = kRawBase + kRawSlots * kRawBytes;  // 136 KB
+constexpr int kFewestHelpers = 1;                          // waves without columns that unpack for the others
 constexpr int kCodeChunk = 28;                             // tiles whose pages a wave has at hand, with three more behind them
 
 // Lane i's four bytes at base + offset land at lds_base + 4 i.
@@ -1411,12 +1412,12 @@ __device__ __forceinline__ void codes_piece(const SharedRest& a, const int32_t* 
   f32x4_t oacc[16], bacc = {0.f, 0.f, 0.f, 0.f};  // bacc: weighted biases, lane n (g = 0) has those of column n and the four groups
 #pragma unroll
   for (int mt = 0; mt < 16; mt++) oacc[mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float m_run = -__builtin_inff(), l_run = 0.0f, v_unit = 0x1p-126f;
+  float m_run = -__builtin_inff(), l_run = 0.0f, v_unit = 0x1p-126f, per_unit = 0x1p126f;
   bool begun = false;
 
-  // A tile's codes as float16 numbers, less 128: a thread has sixteen of K and of V.
-  auto unpack = [&](int i) {
-    int tl = tid;
+  // A tile's codes as float16 numbers, less 128: a thread has sixteen of K and of V in each eighth that its wave unpacks.
+  auto unpack_part = [&](int i, int part) {
+    int tl = lane + 64 * part;
     asm volatile("" : "+v"(tl));  // (offsets are made here, not carried through the loop)
     const unsigned char* raw = lds + kRawBase + (i % kRawSlots) * kRawBytes + tl * 16;
     const int row = tl >> 4, piece = 2 * (tl & 15), f = turn(row);
@@ -1434,6 +1435,15 @@ __device__ __forceinline__ void codes_piece(const SharedRest& a, const int32_t* 
       }
       *reinterpret_cast<u32x4_t*>(to + side * kTileBytes + 16 * (piece ^ f)) = p[0];
       *reinterpret_cast<u32x4_t*>(to + side * kTileBytes + 16 * ((piece + 1) ^ f)) = p[1];
+    }
+  };
+
+  const int busy = (columns + 15) >> 4, idle = kWideWaves - busy;
+  auto unpack = [&](int i) {
+    if (idle < kFewestHelpers) {
+      unpack_part(i, wave);
+    } else {
+      for (int part = wave - busy; part >= 0 && part < kWideWaves; part += idle) unpack_part(i, part);
     }
   };
 
@@ -1525,9 +1535,9 @@ __device__ __forceinline__ void codes_piece(const SharedRest& a, const int32_t* 
         static_for<16>([&](auto mt) { oacc[mt] = oacc[mt] * of_lane<decltype(mt)::value / 4>(by); });
       }
       v_unit = unit;
+      per_unit = 1.0f / unit;
     }
     begun = true;
-    const float per_unit = 1.0f / v_unit;
     vsf[0] *= per_unit;
     vsf[1] *= per_unit;
     static_for<8>([&](auto ic) {
@@ -1572,7 +1582,7 @@ __device__ __forceinline__ void codes_piece(const SharedRest& a, const int32_t* 
   // Steps of a wave: what tile i + 1 is made of has landed once its copies have (three a tile, in order) and every wave got here; the
   // stage and the slot of tile i - 1 are free then.
   wait_copies_and_barrier<2 * kCopies>();  // (and the plan, where the stages lie, is no longer read)
-  unpack(0);
+  unpack_part(0, wave);
   const int n_tiles = tile1 - tile0;
   for (int i0 = 0; i0 < n_tiles; i0 += kCodeChunk) {
     const int i_end = min(i0 + kCodeChunk, n_tiles);
@@ -1629,77 +1639,87 @@ __global__ __launch_bounds__(kWideThreads, 1) void paged_prefix_codes_kernel(con
 }
 
 constexpr int kAtOnce = 16;  // pieces that a wave joins at a time
+typedef __attribute__((address_space(1))) u32x2_t global_words_t;
+typedef __attribute__((address_space(1))) u32x4_t global_quads_t;
 
 // Joins the pieces of one query head: WAVES of them a head take every WAVES-th, and meet in LDS. PARTS: own rows are
 // paged_decode.hip's parts (own: of rows that are not cut), else pieces of paged_shared_kernel.
 // grid: heads / (kMergeWaves / WAVES)
 constexpr int kMergeWaves = 8;
 template <int ODT, int WAVES, bool PARTS, bool HALF>  // HALF: partials of prefixes are scaled float16 numbers
-__global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(const int32_t* parts, const void* ws_pre,
-                                                                              const float* ws_pre_ml, const float* ws_own,
-                                                                              const float* ws_own_ml, int rep, int n_kv, int heads,
-                                                                              int block, int prefix_slots, int own_slots,
-                                                                              PagedParts own, void* out) {
+__global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(const int32_t* parts, const int32_t* cuts, int rep, int n_kv,
+                                                                              int rows, int block, int prefix_slots, int own_slots,
+                                                                              int shares, bool cut_rows, const void* ws_pre, const float* ws_pre_ml,
+                                                                              const float* ws_own, const float* ws_own_ml,
+                                                                              const float* part_o, const float* part_ml, void* out) {
   __shared__ __attribute__((aligned(16))) float xo[kMergeWaves][kD + 2];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int head = (int)blockIdx.x * (kMergeWaves / WAVES) + wave / WAVES;
   const int part = wave % WAVES;
-  const bool here = head < heads;
+  const bool here = head < rows * rep;
   const int row = here ? head / rep : 0, hn = here ? head - row * rep : 0;
+  // (both entries of the row are read at once, whether it has a cut or not: waits one behind the other are what this kernel's time
+  // is made of)
   const int32_t* at = parts + 8 * (int64_t)row;
+  const int own_first = PARTS ? 0 : at[0], own_count = at[1], pre_first = at[2], pre_ranges = at[3], blocks = at[4], column = at[5] + hn;
   Cut cut = {-1, 0, 0};
-  if constexpr (PARTS)
-    if (own.cut) cut.load(own.cut, row, heads / rep, own.shares);
-  const int n_own = !here ? 0 : !PARTS ? at[1] : cut.count > 0 ? cut.count : 1, ranges = here ? at[3] : 0;
+  if constexpr (PARTS) cut.load(cuts, row, rows, shares);
+  const bool is_cut = PARTS && cut_rows && cut.count > 0;
+  const int n_own = !here ? 0 : !PARTS ? own_count : is_cut ? cut.count : 1, ranges = here ? pre_ranges : 0;
   const int total = n_own + ranges;
-  const int own_first = PARTS ? 0 : at[0], pre_first = at[2], blocks = at[4], column = at[5] + hn;
-  const int kvh = row % n_kv;
-  // Row of prefix piece i (bounded by the workspace, whatever is there), sums and statistics of own piece i
-  auto prefix_row = [&](int i) {
-    const int s = pre_first + bundle_piece(kvh * ranges + i, column / block, n_kv * ranges, blocks);
-    return (int64_t)(s >= 0 && s < prefix_slots ? s : 0) * block + column % block;
-  };
+  const int kvh = row % n_kv, column_block = column / block, column_at = column - column_block * block;
   struct From {
-    const float *o, *ml;
+    const void* o;
+    const float* ml;
   };
+  // Sums and statistics of own piece i, of prefix piece i (bounded by the workspace, whatever is there)
   auto own_piece = [&](int i) {
-    if constexpr (PARTS) {
-      if (cut.count > 0) {
-        const int64_t p = part_of(cut.first, i);
-        return From{own.o + (p * rep + hn) * kD, own.ml + (p * 16 + hn) * 2};
-      }
-      return From{ws_own + (int64_t)head * kD, ws_own_ml + (int64_t)head * 2};
+    if (is_cut) {
+      const int64_t p = part_of(cut.first, i);
+      return From{part_o + (p * rep + hn) * kD, part_ml + (p * 16 + hn) * 2};
     }
+    if constexpr (PARTS) return From{ws_own + (int64_t)head * kD, ws_own_ml + (int64_t)head * 2};
     const int s = own_first + i >= 0 && own_first + i < own_slots ? own_first + i : 0;
     return From{ws_own + ((int64_t)s * rep + hn) * kD, ws_own_ml + ((int64_t)s * 16 + hn) * 2};
+  };
+  auto prefix_piece = [&](int i) {
+    const int s = pre_first + bundle_piece(kvh * ranges + i, column_block, n_kv * ranges, blocks);
+    const int64_t r = (int64_t)(s >= 0 && s < prefix_slots ? s : 0) * block + column_at;
+    return From{reinterpret_cast<const uint8_t*>(ws_pre) + r * kD * (HALF ? 2 : 4), ws_pre_ml + 4 * r};
   };
   float m = -__builtin_inff(), l = 0.0f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   for (int p0 = part; p0 < total; p0 += kAtOnce * WAVES) {
-    const int mine = p0 + WAVES * (lane % kAtOnce);
-    f32x2_t stat = {-__builtin_inff(), 0.0f};
-    float scale = 1.0f;
-    if (mine < n_own) {
-      stat = *reinterpret_cast<const f32x2_t*>(own_piece(mine).ml);
-    } else if (mine < total) {
-      const f32x4_t s = *reinterpret_cast<const f32x4_t*>(ws_pre_ml + 4 * prefix_row(mine - n_own));
-      stat = f32x2_t{s.x, s.y};
-      scale = s.z;
-    }
+    // Lane j finds piece j, of those past the end the last. (One load of either kind of piece, so that none waits for the other.)
+    const int mine = p0 + WAVES * (lane % kAtOnce), near = min(mine, total - 1);
+    const bool pre = near >= n_own;
+    const From from = pre ? prefix_piece(near - n_own) : own_piece(near);
+    f32x2_t stat = *reinterpret_cast<const f32x2_t*>(from.ml);
+    float scale = HALF ? from.ml[pre ? 2 : 0] : 1.0f;
+    if (!pre) scale = 1.0f;
+    if (mine >= total) stat = f32x2_t{-__builtin_inff(), 0.0f};
+    const uint64_t o_at = reinterpret_cast<uint64_t>(from.o);
     u32x4_t ov[kAtOnce];
 #pragma unroll
     for (int j = 0; j < kAtOnce; j++) {  // (wave-uniform: pieces past the end cost no load)
       const int i = p0 + WAVES * j;
       if (i >= total) continue;
-      if (i < n_own) {
-        ov[j] = *reinterpret_cast<const u32x4_t*>(own_piece(i).o + 4 * lane);
-      } else if constexpr (HALF) {
-        const u32x2_t h = *reinterpret_cast<const u32x2_t*>(reinterpret_cast<const uint16_t*>(ws_pre) + prefix_row(i - n_own) * kD + 4 * lane);
-        ov[j].x = h.x;
-        ov[j].y = h.y;
+      const uint64_t o_j = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)o_at, j) |
+                           (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(o_at >> 32), j) << 32;
+      if constexpr (HALF) {
+        const bool whole = i < n_own;  // (four floats a lane, or four float16 numbers)
+        const uint64_t o_lane = o_j + (uint32_t)((whole ? 16 : 8) * lane);
+        const u32x2_t lo = *reinterpret_cast<const global_words_t*>(o_lane);
+        ov[j].x = lo.x;
+        ov[j].y = lo.y;
+        if (whole) {
+          const u32x2_t hi = *reinterpret_cast<const global_words_t*>(o_lane + 8);
+          ov[j].z = hi.x;
+          ov[j].w = hi.y;
+        }
       } else {
-        ov[j] = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const float*>(ws_pre) + prefix_row(i - n_own) * kD + 4 * lane);
+        ov[j] = reinterpret_cast<const global_quads_t*>(o_j)[lane];
       }
     }
     float m_new = stat.x;
@@ -1828,7 +1848,8 @@ int merge_launch(const SharedArgs& a, const PagedParts& own, hipStream_t st) {
   auto merge = [&](auto waves) {
     constexpr int kWavesAHead = decltype(waves)::value, kHeads = kMergeWaves / kWavesAHead;
     paged_shared_merge_kernel<QDT, kWavesAHead, PARTS, HALF><<<dim3((unsigned)((heads + kHeads - 1) / kHeads)), dim3(64 * kMergeWaves), 0, st>>>(
-        r.parts, r.ws_pre, r.ws_pre_ml, r.ws_own, r.ws_own_ml, a.rep, a.n_kv, heads, r.block, r.prefix_slots, r.own_slots, own, r.out);
+        r.parts, own.cut ? own.cut : r.parts, a.rep, a.n_kv, a.batch * a.n_kv, r.block, r.prefix_slots, r.own_slots, own.shares,
+        own.cut != nullptr, r.ws_pre, r.ws_pre_ml, r.ws_own, r.ws_own_ml, own.o, own.ml, r.out);
   };
   // (a head has as many pieces as compute units divided by blocks: few where heads are many)
   if (heads <= 1024) merge(std::integral_constant<int, 8>{});
