@@ -312,3 +312,99 @@ def test_a_step_of_more_rows_than_a_call_takes(selects):
             parts.append(paged.sdpa_decode_paged_shared(q[at], layer.cache.keys, layer.cache.values, *tables.prefixes, *args,
                                                         requests=step.requests[at]))
     assert got.equal(layer.inner.o_proj((torch.cat(parts) * torch.sigmoid(gate)).reshape(2100, -1)))
+
+
+def _calls(gen, quantized=False):
+    """Calls of every operator, small and large: (function of a workspace, floats of it that are enough)."""
+    n_kv, rep, page, pool = 2, 8, 64, 160
+    if quantized:
+        def side():
+            scales = 0.02 * torch.rand(pool, n_kv, page, 4, device="cuda", generator=gen)
+            return (torch.randint(-2 ** 31, 2 ** 31 - 1, (pool, n_kv, page, 64), device="cuda", generator=gen, dtype=torch.int32).view(torch.uint32),
+                    scales.to(BF16), (-128 * scales).to(BF16))
+        keys, values = side(), side()
+        pages = (*keys, *values)
+        shared, sparse = paged.sdpa_decode_paged_shared_q8, paged.sdpa_decode_paged_sparse_q8
+    else:
+        keys, values = (torch.randn(pool, n_kv, page, 256, device="cuda", generator=gen).to(BF16) for _ in range(2))
+        pages = (keys, values)
+        shared, sparse = paged.sdpa_decode_paged_shared, paged.sdpa_decode_paged_sparse
+    codes, scales = torch.zeros(pool, n_kv, 2, 256, dtype=torch.int8, device="cuda"), torch.ones(pool, n_kv, device="cuda")
+    paged.page_bounds(torch.arange(pool * page, dtype=torch.int32, device="cuda"), keys, codes, scales)
+
+    def ints(high, *shape):
+        return torch.randint(0, high, shape, device="cuda", generator=gen, dtype=torch.int32)
+
+    calls = []
+    for R in (2, 37):
+        q = torch.randn(R, n_kv * rep, 256, device="cuda", generator=gen).to(BF16)
+        own = ints(pool, R, 30), ints(1900, R)
+        prefixes = ints(pool, 3, 40), ints(2500, 3), ints(4, R)
+        calls += [lambda ws, a=(q, *pages, *prefixes, *own, 0.0625): (shared(*a, workspace=ws),),
+                  lambda ws, a=(q, *pages, codes, scales, *own, 0.0625, 6): (sparse(*a, workspace=ws),),
+                  lambda ws, a=(q, codes, scales, *own, 6): paged.select_pages(*a, page_size=page, workspace=ws)]
+    return calls
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_captured_graphs_share_a_workspace(quantized):
+    """One after the other, of different operators and sizes, over memory that holds what the last one left (at first: not a number)."""
+    calls, graphs = _calls(torch.Generator(device="cuda").manual_seed(12), quantized), []
+    ws = torch.full((1 << 24,), float("nan"), device="cuda")
+    for call in calls:
+        want = call(None)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(ws)
+        graphs.append((graph, out, want))
+    for _ in range(3):
+        for graph, out, want in graphs:
+            for o in out:
+                o.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(o.equal(w) for o, w in zip(out, want))
+
+
+def test_calls_of_several_operators_on_streams_of_their_own():
+    calls = _calls(torch.Generator(device="cuda").manual_seed(13))
+    wants = [call(None) for call in calls]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in calls], [[] for _ in calls]
+    for _ in range(10):
+        for call, stream, outs in zip(calls, streams, got):
+            with torch.cuda.stream(stream):
+                outs.append(call(None))
+    torch.cuda.synchronize()
+    for want, outs in zip(wants, got):
+        assert all(o.equal(w) for out in outs for o, w in zip(out, want))
+
+
+def test_a_workspace_that_is_too_small_is_refused():
+    for call in _calls(torch.Generator(device="cuda").manual_seed(14)):
+        with pytest.raises((RuntimeError, ValueError), match="workspace"):
+            call(torch.empty(4, device="cuda"))
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_calls_and_steps_without_rows(quantized):
+    cache = _cache(8, BF16, quantized, bounds=True)
+    sides = (*cache.keys, *cache.values) if quantized else (cache.keys, cache.values)
+    shared, sparse = ((paged.sdpa_decode_paged_shared_q8, paged.sdpa_decode_paged_sparse_q8) if quantized else
+                      (paged.sdpa_decode_paged_shared, paged.sdpa_decode_paged_sparse))
+    q, none, t = torch.empty(0, HEADS, 256, device="cuda", dtype=BF16), _ints([]), torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    two, bounds = _ints([0, 0]), (cache.codes, cache.scales)
+    assert shared(q, *sides, t, two, two, t, none, 0.1, requests=none).shape == q.shape
+    assert sparse(q, *sides, *bounds, t, none, 0.1, 4, requests=none).shape == q.shape
+    of, n = paged.select_pages(q, *bounds, t, none, 4, page_size=16, requests=none)
+    assert of.shape == (0, KV_HEADS, 4) and n.shape == (0, KV_HEADS)
+    before = cache.codes.clone()
+    paged.page_bounds(none, cache.keys, *bounds)
+    assert cache.codes.equal(before)
+    block, x = _Block(8, BF16), torch.empty(0, HIDDEN, device="cuda", dtype=BF16)
+    for tables, kwargs in ((paged.PageTables(2, 8, page_size=16, max_tokens=48, n_prefixes=1), {}),
+                           (paged.PageTables(2, 8, page_size=16, max_tokens=48), dict(n_selected=4))):
+        layer = paged.PagedAttention(block, cache, **kwargs)
+        step = tables.step(_ints([0] * (2 + tables.n_prefixes)), 0)
+        assert layer(x, step, tables).shape == (0, HIDDEN)
