@@ -22,8 +22,10 @@ typedef __attribute__((ext_vector_type(4))) int i32x4_t;
 
 constexpr int kTile = 16;          // pages of a matrix instruction
 constexpr int kScoreWaves = 4;
-constexpr int kTilesAWave = 2;
-constexpr int kPagesAGroup = kTile * kScoreWaves * kTilesAWave;
+// Tiles of all tables, as wide as they are, from which on a wave takes two (fewer: one, on as many more compute units). In us, with one
+// and with two: a request of 256 pages 8.7 and 9.9, 16 of up to 2048 20.0 and 18.5, 64 such 38.7 and 34.8 (with four 34.1, but 11.6
+// for the first).
+constexpr int kManyTiles = 1024;
 constexpr int kMaxTablePages = 32768;  // a workgroup of 1024 threads has 32 a thread
 constexpr int kMaxSelected = 4096;
 
@@ -54,7 +56,7 @@ __device__ __forceinline__ Seen seen_by(const SelectArgs& a, int r) {
 }
 
 // grid: (groups of pages, queries x KV heads)
-template <int QDT>
+template <int QDT, int TILES>
 __global__ __launch_bounds__(64 * kScoreWaves) void page_score_kernel(SelectArgs a) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -62,15 +64,15 @@ __global__ __launch_bounds__(64 * kScoreWaves) void page_score_kernel(SelectArgs
   const Seen seen = seen_by(a, r);
   const int n = (seen.len + (1 << a.page_shift) - 1) >> a.page_shift;
   if (n <= a.selected) return;  // (all of them are taken)
-  const int tile0 = ((int)blockIdx.x * kScoreWaves + wave) * kTilesAWave;
+  const int tile0 = ((int)blockIdx.x * kScoreWaves + wave) * TILES;
   if (tile0 * kTile >= n) return;
   const int head = lane & 15, g = lane >> 4;
   // ---- page numbers, then the bounds of two tiles; the query in the meantime
   const int32_t* table = a.tables + (int64_t)seen.request * a.width;
-  int page[kTilesAWave];
-  bool good[kTilesAWave];
+  int page[TILES];
+  bool good[TILES];
 #pragma unroll
-  for (int i = 0; i < kTilesAWave; i++) {
+  for (int i = 0; i < TILES; i++) {
     const int p = (tile0 + i) * kTile + head;
     page[i] = p < n ? table[p] : -1;
   }
@@ -93,10 +95,10 @@ __global__ __launch_bounds__(64 * kScoreWaves) void page_score_kernel(SelectArgs
       }
     }
   }
-  i32x4_t tile[kTilesAWave][8];
-  float scale[kTilesAWave];
+  i32x4_t tile[TILES][8];
+  float scale[TILES];
 #pragma unroll
-  for (int i = 0; i < kTilesAWave; i++) {
+  for (int i = 0; i < TILES; i++) {
     good[i] = page[i] >= 0 && page[i] < a.n_pages;
     const int64_t at = (int64_t)(good[i] ? page[i] : 0) * a.n_kv + kvh;
     const i32x4_t* from = reinterpret_cast<const i32x4_t*>(a.codes + at * kBoundBytes + 16 * g);
@@ -127,7 +129,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void page_score_kernel(SelectArgs
     }
   const float unit = __builtin_amdgcn_ldexpf(1.0f, e);
 #pragma unroll
-  for (int i = 0; i < kTilesAWave; i++) {
+  for (int i = 0; i < TILES; i++) {
     const int p0 = (tile0 + i) * kTile;
     if (p0 >= n) break;
     i32x4_t acc = {0, 0, 0, 0};
@@ -459,12 +461,19 @@ int select_fill(const char* what, SelectArgs& a, const void* q, int q_dtype, con
 int select_launch(const char* what, const SelectArgs& a, int q_dtype, hipStream_t st) {
   const unsigned rows = (unsigned)(a.rows * a.n_kv);
   if (a.width > a.selected) {
-    const dim3 grid((unsigned)((a.width + kPagesAGroup - 1) / kPagesAGroup), rows);
-    if (q_dtype == MSPR_F32) page_score_kernel<MSPR_F32><<<grid, dim3(64 * kScoreWaves), 0, st>>>(a);
-    else if (q_dtype == MSPR_F16) page_score_kernel<MSPR_F16><<<grid, dim3(64 * kScoreWaves), 0, st>>>(a);
-    else page_score_kernel<MSPR_BF16><<<grid, dim3(64 * kScoreWaves), 0, st>>>(a);
+    auto score = [&](auto tiles) {
+      constexpr int kTiles = decltype(tiles)::value, kPages = kTile * kScoreWaves * kTiles;
+      const dim3 grid((unsigned)((a.width + kPages - 1) / kPages), rows);
+      if (q_dtype == MSPR_F32) page_score_kernel<MSPR_F32, kTiles><<<grid, dim3(64 * kScoreWaves), 0, st>>>(a);
+      else if (q_dtype == MSPR_F16) page_score_kernel<MSPR_F16, kTiles><<<grid, dim3(64 * kScoreWaves), 0, st>>>(a);
+      else page_score_kernel<MSPR_BF16, kTiles><<<grid, dim3(64 * kScoreWaves), 0, st>>>(a);
+    };
+    if ((int64_t)rows * ((a.width + kTile - 1) / kTile) < kManyTiles) score(std::integral_constant<int, 1>{});
+    else score(std::integral_constant<int, 2>{});
     MSPR_CHECK_LAUNCH(what);
   }
+  // (In us: 256 pages by 256 threads 9.9, by 512 12.1, by 1024 16.0; 16 requests of up to 2048 pages by 512 18.2, by 1024 22.2. Rows of bounds
+  // for 16 heads where there are 8: 256 pages 11.1, 2048 20.9.)
   auto choose = [&](auto heads) {
     constexpr int kHeads = decltype(heads)::value;
     if (a.width <= 1024) page_choose_kernel<256, 4, kHeads><<<dim3(rows), dim3(256), 0, st>>>(a);

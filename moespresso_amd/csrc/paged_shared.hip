@@ -12,13 +12,17 @@
 // so that a piece falls to every compute unit; the number of a piece says what it is. Blocks of one range lie eight workgroups
 // apart, on one XCD, whose L2 then has the rows for the second block. A last kernel joins a query's pieces.
 //
-// Two forms. Where one block of 32 columns does not hold all queries' heads, prefixes of 16-bit rows are a kernel's own
-// (paged_prefix_kernel), with up to 256 columns a block: tiles of 32 keys come by asynchronous copies into a ring of LDS that eight
-// waves share, 32 columns a wave, read from HBM once and from LDS by every wave (the layout and the order of flash_prefill.hip; up to 128
-// columns the waves take two tiles at a time, four each). Own rows are paged_decode.hip's then.
+// Two forms. Of few query heads or short prefixes one launch (paged_shared_kernel) has prefixes, in blocks of 32 columns, and own
+// rows: a tile is a wave's own, in registers, and the four waves of a workgroup, which take the tiles of a piece in turn, meet in
+// LDS. Else prefixes are a kernel's own, with up to 128 columns a block, and own rows paged_decode.hip's: tiles of 32 keys come by
+// asynchronous copies into a ring of LDS, read from HBM once a block and from LDS by every wave. Of 16-bit rows (paged_prefix_kernel) a
+// wave has 32 columns of every second tile, of 8-bit ones (paged_prefix_codes_kernel) sixteen of every tile.
 //
-// Else (few queries, or 8-bit rows; paged_shared_kernel) prefixes and own rows are one launch's: a tile is a wave's own, in registers,
-// and the four waves of a workgroup, which take the tiles of a piece in turn, meet in LDS.
+// What bounds it: few queries the chain of accesses (requests, groups, lengths, table, rows) and two launches; long prefixes of few
+// queries HBM (16 queries over 32768 rows: the tiles' loop reads 6.4 TB/s, 10 of the kernel's 25 us; the others are the plan, the first
+// tiles, and 16 MB of partials); many columns the matrix units (256 queries over 8192 rows: 45 us at the rate of a library's product
+// with two terms a weight, 57 taken); 8-bit rows a wave's own chain of scales, terms and cross-lane moves (60 us for 33 queries over
+// 20001 rows).
 #include "paged_parts.h"
 
 namespace {
@@ -27,9 +31,10 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kGroups = 256;    // workgroups that run at once: one a compute unit
 constexpr int kColumns = 32;    // of a piece, in blocks of 16
-constexpr int kWideWaves = 8;   // of the kernel for prefixes of 16-bit rows
+constexpr int kWideWaves = 8;   // of the kernels for prefixes alone
 constexpr int kWideThreads = 64 * kWideWaves;
-constexpr int kWideColumns = 32 * kWideWaves;
+constexpr int kAtATime = 2;     // tiles that the waves of a kernel for 16-bit rows take at a time
+constexpr int kWideColumns = 128;  // of a block: 32 a wave and tile, of 8-bit rows 16 a wave
 constexpr int kBlocks = kColumns / 16;
 constexpr int kMinShare = 4;    // tiles of a range, at least: one a wave
 constexpr int kMaxRows = 2048;  // queries, and prefixes, of a call
@@ -800,19 +805,20 @@ __device__ __forceinline__ uint32_t lds_address(const unsigned char* p) {
 // transposed ones of V meet a bank twice.
 __device__ __forceinline__ int swizzle(int r) { return ((r & 7) << 1) | ((r >> 3) & 1); }
 
-// One piece: `columns` columns (head rows of q in `column_row`) over tiles [tile0, tile1). KS tiles at a time: wave w has columns 32 (w %
-// (8 / KS)) on and every KS-th tile.
-template <int FMT, int KS, typename F>
+// One piece: `columns` columns (head rows of q in `column_row`) over tiles [tile0, tile1), two at a time: wave w has columns 32 (w % 4)
+// on and every second tile. (Blocks of 256 columns, which read a prefix half as often, a tile at a time: 2048 query heads a KV head over
+// 8192 rows 108.6 us instead of 109.1, over 20000 rows 160 instead of 164, but 256 over 32768 rows 55.7 instead of 52.0, 200 ragged queries
+// 127 instead of 123. One tile at a time for blocks of 128: 42.4 us instead of 42.0 for 16 queries over 32768 rows.)
+template <int FMT, typename F>
 __device__ __forceinline__ void prefix_piece(const SharedRest& a, const int32_t* table, int len, int tile0, int tile1, int n_kv, int kvh,
                                              int slot, int columns, const int* column_row, F&& find_members, unsigned char* lds,
                                              float (*xml)[32][2]) {
   constexpr float kLag = 4.0f;                              // (as in paged_decode.hip)
   constexpr float kUp = FMT == MSPR_F16 ? 11.0f : 0.0f;
-  constexpr int kAhead = 2 / KS;                            // steps whose copies are under way behind the present one
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 31, g = lane >> 5;  // column within the wave's; key of the K operand
-  constexpr int kColumnWaves = kWideWaves / KS;
+  constexpr int kColumnWaves = kWideWaves / kAtATime;
   const int column0 = 32 * (wave % kColumnWaves), part = wave / kColumnWaves;
   const int mine = __builtin_amdgcn_readfirstlane(min(max(columns - column0, 0), 32));  // columns of this wave
   const int page_mask = (1 << a.page_shift) - 1;
@@ -847,21 +853,19 @@ __device__ __forceinline__ void prefix_piece(const SharedRest& a, const int32_t*
     }
     return rows;
   };
-  uint32_t ahead[kAhead + 1];  // rows of this wave's tile in the steps under way
   auto issue_step = [&](int ids, int t0, int step) {
     uint32_t rows = 0;
 #pragma unroll
-    for (int i = 0; i < KS; i++) {
-      const int t = tile0 + step * KS + i;
-      const uint32_t r = issue_tile(ids, t0, t, (step * KS + i) % kStages);
+    for (int i = 0; i < kAtATime; i++) {
+      const int t = tile0 + step * kAtATime + i;
+      const uint32_t r = issue_tile(ids, t0, t, (step * kAtATime + i) % kStages);
       if (i == part) rows = r;
     }
     return rows;
   };
-  const int n_steps = __builtin_amdgcn_readfirstlane((tile1 - tile0 + KS - 1) / KS);
+  const int n_steps = __builtin_amdgcn_readfirstlane((tile1 - tile0 + kAtATime - 1) / kAtATime);
   int ids = load_ids(tile0);
-#pragma unroll
-  for (int i = 0; i < kAhead; i++) ahead[i] = issue_step(ids, tile0, i);
+  uint32_t ahead = issue_step(ids, tile0, 0);  // rows of this wave's tile in the step under way
   int ids_next = load_ids(tile0 + kChunk);
   find_members();  // (under the first copies)
 
@@ -989,17 +993,15 @@ __device__ __forceinline__ void prefix_piece(const SharedRest& a, const int32_t*
     }
   };
 
-  for (int s0 = 0; s0 < n_steps; s0 += kChunk / KS) {
-    const int s_end = min(s0 + kChunk / KS, n_steps), t0 = tile0 + s0 * KS;
+  for (int s0 = 0; s0 < n_steps; s0 += kChunk / kAtATime) {
+    const int s_end = min(s0 + kChunk / kAtATime, n_steps), t0 = tile0 + s0 * kAtATime;
     for (int step = s0; step < s_end; step++) {
-      // This step's tiles have landed once the wave's copies of them have (four a tile, in order) and every wave got here; the
-      // stages of the step before are free then.
-      wait_copies_and_barrier<4 * KS * (kAhead - 1)>();
-      ahead[kAhead] = issue_step(ids, t0, step + kAhead);  // (behind the last, tiles without rows: what is under way is the same)
-      const uint32_t rows = ahead[0];
-#pragma unroll
-      for (int i = 0; i < kAhead; i++) ahead[i] = ahead[i + 1];
-      if (mine > 0 && rows != 0) attend_tile(lds + ((step * KS + part) % kStages) * kStageBytes, rows);
+      // This step's tiles have landed once the wave's copies of them have and every wave got here; the stages of the step before are
+      // free then.
+      wait_copies_and_barrier<0>();
+      const uint32_t rows = ahead;
+      ahead = issue_step(ids, t0, step + 1);  // (behind the last, tiles without rows)
+      if (mine > 0 && rows != 0) attend_tile(lds + ((step * kAtATime + part) % kStages) * kStageBytes, rows);
     }
     ids = ids_next;
     ids_next = load_ids(t0 + 2 * kChunk);
@@ -1012,7 +1014,7 @@ __device__ __forceinline__ void prefix_piece(const SharedRest& a, const int32_t*
   int tl = tid;
   asm volatile("" : "+v"(tl));  // (the offsets below are made here, not carried through the tile loop)
   const int en = tl & 31, eg = (tl >> 5) & 1;
-  if constexpr (KS == 2) {
+  {
     f32x4_t* xo = reinterpret_cast<f32x4_t*>(lds + (wave % kColumnWaves) * 32768) + (tl & 63);  // [32 quads][64 lanes]
     if (part == 1 && mine > 0) {
 #pragma unroll
@@ -1041,14 +1043,14 @@ __device__ __forceinline__ void prefix_piece(const SharedRest& a, const int32_t*
         for (int i = 0; i < 4; i++) oacc[mt][4 * c + i] = oacc[mt][4 * c + i] * w1 + o[i] * w2;
       }
   }
-  if (mine == 0) return;
   int row0 = slot * a.block + column0;  // (a scalar by hand: with the lanes' addresses below, the compiler takes it for one of each lane's)
   asm volatile("" : "+s"(row0));
-  unsigned char* xo = lds + (wave << (KS == 2 ? 15 : 14));  // (of two parts, where the wave's own exchange was)
+  unsigned char* xo = lds + (wave << 15);  // (where the wave's own exchange was)
   if constexpr (FMT == MSPR_BF16) {
     // As float16, scaled by a power of two that brings a column's largest sum to [1/2, 1): partials are as many bytes as the rows
     // themselves where a compute unit has few tiles (16 queries over 32768 rows, 29 MB), and eleven digits of a part are more
-    // than the result has (one rounding of 2^-12 of the attention over |V| beside its 2^-9).
+    // than the result has (one rounding of 2^-12 of the attention over |V| beside its 2^-9). Float32 ones: 46.4 us instead of 42.0, 256
+    // queries over 8192 rows 116 instead of 108.
     float top = 0.0f;
 #pragma unroll
     for (int mt = 0; mt < 8; mt++)
@@ -1060,7 +1062,7 @@ __device__ __forceinline__ void prefix_piece(const SharedRest& a, const int32_t*
     if (eg == 0 && en < mine)
       *reinterpret_cast<f32x4_t*>(a.ws_pre_ml + 4 * (int64_t)(row0 + en)) = f32x4_t{m_run, l_run, __builtin_amdgcn_ldexpf(1.0f, e), 0.0f};
     const auto to = store_window(reinterpret_cast<uint16_t*>(a.ws_pre) + (int64_t)row0 * kD, mine * kD * 2);
-    if constexpr (KS == 2) __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int mt = 0; mt < 8; mt++)
 #pragma unroll
@@ -1079,7 +1081,7 @@ __device__ __forceinline__ void prefix_piece(const SharedRest& a, const int32_t*
     const auto to = store_window(reinterpret_cast<float*>(a.ws_pre) + (int64_t)row0 * kD, mine * kD * 4);
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      if constexpr (KS == 2) __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int mt = 0; mt < 4; mt++)
 #pragma unroll
@@ -1155,8 +1157,8 @@ __device__ __forceinline__ void prefix_workgroup(const int32_t* requests, const 
   all *= n_kv;
   units *= n_kv;
   // A range's tiles: so many that there are no more pieces than compute units, as a unit has at most one piece that is not full; where
-  // there are too many units for that, half as many again. Of few prefixes the least of 64 lengths that does it, tried one a
-  // lane (16 queries over 32768 rows of two KV heads: 256 pieces of eight tiles, not 228 of nine).
+  // there are too many units for that, half as many again. Of few prefixes the least of 64 lengths that does it, tried one a lane (256
+  // queries over 8192 rows of two KV heads: 256 pieces of 32 tiles, not 224 of 37; the kernel 57 us, not 65).
   int share = max(kMinShare, ceil_div(all, max(kGroups - units, kGroups / 2)));
   if (n_prefixes <= 16 && all < (1 << 21)) {
     const int tried = (max(kMinShare, ceil_div(all, kGroups)) + step - 1) / step * step + step * lane;
@@ -1242,29 +1244,24 @@ __global__ __launch_bounds__(kWideThreads, 1) void paged_prefix_kernel(const int
   __shared__ int wave_members[kWideWaves];
   __shared__ int column_row[kWideColumns];
   __shared__ float xml[kWideWaves / 2][32][2];
-  const int step = a.block <= kWideColumns / 2 ? 2 : 1;  // (tiles that the waves take at a time)
-  prefix_workgroup(requests, groups, prefix_lens, batch, n_prefixes, n_tables, n_kv, rep, a, step, ring + 2 * kStageBytes, wave_members,
-                   column_row, [&](const int32_t* table, int len, int tile0, int tile1, int kvh, int columns, auto&& find_members) {
-                     if (columns <= kWideColumns / 2)
-                       prefix_piece<FMT, 2>(a, table, len, tile0, tile1, n_kv, kvh, blockIdx.x, columns, column_row, find_members, ring, xml);
-                     else
-                       prefix_piece<FMT, 1>(a, table, len, tile0, tile1, n_kv, kvh, blockIdx.x, columns, column_row, find_members, ring, xml);
+  prefix_workgroup(requests, groups, prefix_lens, batch, n_prefixes, n_tables, n_kv, rep, a, kAtATime, ring + 2 * kStageBytes, wave_members, column_row,
+                   [&](const int32_t* table, int len, int tile0, int tile1, int kvh, int columns, auto&& find_members) {
+                     prefix_piece<FMT>(a, table, len, tile0, tile1, n_kv, kvh, blockIdx.x, columns, column_row, find_members, ring, xml);
                    });
 }
 
 // ---------------------------------------------------------------------------------------------- prefixes of 8-bit rows
 
-// Sixteen columns a wave, 128 a block, by 16x16x32 products of codes and queries, as paged_decode.hip makes them. Raw rows come by
+// Sixteen columns a wave by 16x16x32 products of codes and queries, as paged_decode.hip makes them. Raw rows come by
 // asynchronous copies into a ring of four tiles; the eight waves together make a tile's codes float16 numbers, a tile ahead of the
 // one they multiply, so that what unpacking costs is shared. Scales and biases are read where the copies put them.
-constexpr int kCodeColumns = 16 * kWideWaves;
+static_assert(kWideColumns == 16 * kWideWaves && kWideColumns == 32 * kWideWaves / kAtATime, "a block's columns are the waves'");
 constexpr int kCodeTile = kTileKeys * kD;                  // 8 KB of codes, K and V each
 constexpr int kScaleBytes = 256;                           // sixteen rows of scales or biases (of 16-bit ones half of it)
 constexpr int kRawBytes = 2 * kCodeTile + 8 * kScaleBytes;
 constexpr int kRawSlots = 4;
 constexpr int kRawBase = 2 * kStageBytes;
 constexpr int kCodeLds = kRawBase + kRawSlots * kRawBytes;  // 136 KB
-constexpr int kFewestHelpers = 1;                          // waves without columns that unpack for the others
 constexpr int kCodeChunk = 28;                             // tiles whose pages a wave has at hand, with three more behind them
 
 // Lane i's four bytes at base + offset land at lds_base + 4 i.
@@ -1440,9 +1437,9 @@ __device__ __forceinline__ void codes_piece(const SharedRest& a, const int32_t* 
 
   const int busy = (columns + 15) >> 4, idle = kWideWaves - busy;
   auto unpack = [&](int i) {
-    if (idle < kFewestHelpers) {
+    if (idle == 0) {
       unpack_part(i, wave);
-    } else {
+    } else {  // (waves without columns unpack for the others: 33 queries, of which six waves have 88 heads, 84.0 -> 79.7 us)
       for (int part = wave - busy; part >= 0 && part < kWideWaves; part += idle) unpack_part(i, part);
     }
   };
@@ -1631,7 +1628,7 @@ __global__ __launch_bounds__(kWideThreads, 1) void paged_prefix_codes_kernel(con
                                                                              int n_tables, int n_kv, int rep, SharedRest a) {
   extern __shared__ __attribute__((aligned(256))) unsigned char ring[];
   __shared__ int wave_members[kWideWaves];
-  __shared__ int column_row[kCodeColumns];
+  __shared__ int column_row[kWideColumns];
   prefix_workgroup(requests, groups, prefix_lens, batch, n_prefixes, n_tables, n_kv, rep, a, 1, ring, wave_members, column_row,
                    [&](const int32_t* table, int len, int tile0, int tile1, int kvh, int columns, auto&& find_members) {
                      codes_piece<QDT, SDT>(a, table, len, tile0, tile1, n_kv, kvh, blockIdx.x, columns, column_row, find_members, ring);
@@ -1776,18 +1773,26 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
   if (total > 0) store_out<ODT>(out, ((int64_t)row * rep + hn) * kD + 4 * lane, o, l);
 }
 
-// Prefixes are a kernel's own where a block of 32 columns does not hold the call's query heads of a KV head.
-bool wide_prefixes(int batch, int rep) { return (int64_t)batch * rep > kColumns; }
+// Whether prefixes are a kernel's own: from so many columns times rows that their tables hold (the lengths are on the device) on, and of
+// many columns always. A second kernel costs 9 to 11 us; blocks of 32 columns read a prefix again and again, and own rows of many
+// queries are better dealt out by paged_decode.hip. In us, one launch and two, 8 query heads a KV head: 16-bit rows, 8 queries over 32768
+// rows 35.7 and 37.4, 12 over them 44.3 and 39.5; 32 over 4000 29.3 and 36.1, 128 over 1000 44.1 and 49.5, 256 over 1000 75.0 and 67.5; 20 ragged
+// ones behind 5 prefixes of up to 9001 33.4 and 39.1, 40 such 59.3 and 51.6. 8-bit rows: 24 queries over 20000 rows 60.6 and 61.5, 32 over
+// them 79.7 and 68.9, 48 over 4000 49.5 and 49.7, 96 over 1000 34.6 and 49.3, 200 over 1000 52.6 and 54.4.
+constexpr int kManyColumns = 1024;
+bool wide_prefixes(int batch, int rep, int64_t prefix_cap, bool codes) {
+  const int64_t columns = (int64_t)batch * rep;
+  return columns > kManyColumns || (columns > kColumns && columns * prefix_cap >= (codes ? 4 << 20 : 5 << 19));
+}
 
 // Columns of a block of members: 32, or as many as eight waves hold, but no more than twice what a prefix has members on the
 // average, so that the scratch, a place for every column of a block, does not grow with what blocks leave empty.
-int block_columns(int batch, int n_prefixes, int rep, bool wide, bool codes) {
+int block_columns(int batch, int n_prefixes, int rep, bool wide) {
   if (!wide) return kColumns;
-  const int most = codes ? kCodeColumns : kWideColumns;
   const int64_t used = n_prefixes < batch ? n_prefixes : batch;
   const int64_t mean = ((used > 1 ? 2 : 1) * (int64_t)batch * rep + used - 1) / used;
   const int64_t n = (mean + 31) / 32 * 32;
-  return (int)(n < most ? n : most);
+  return (int)(n < kWideColumns ? n : kWideColumns);
 }
 
 // Pieces of `units` units: a call has at most max(kGroups, kGroups / 2 + units), see `share`.
@@ -1808,10 +1813,10 @@ struct SharedScratch {
   size_t pre, pre_ml, own, own_ml, parts, decode;  // bytes
   size_t total() const { return pre + pre_ml + own + own_ml + parts + decode; }
 };
-SharedScratch shared_scratch(int batch, int n_prefixes, int n_kv, int rep, int page_size, int width, bool codes) {
+SharedScratch shared_scratch(int batch, int n_prefixes, int n_kv, int rep, int page_size, int width, bool wide) {
   SharedScratch s;
-  s.wide = wide_prefixes(batch, rep);
-  s.block = block_columns(batch, n_prefixes, rep, s.wide, codes);
+  s.wide = wide;
+  s.block = block_columns(batch, n_prefixes, rep, s.wide);
   const int64_t own = (int64_t)batch * n_kv, blocks = prefix_units(batch, n_prefixes, n_kv, rep, s.block);
   s.pieces = pieces_of(s.wide ? blocks : own + blocks);
   s.prefix_slots = s.wide ? s.pieces : s.pieces - own;  // (every query has a piece of its own, at least)
@@ -1840,7 +1845,8 @@ int reserve_lds(K* kernel, int bytes, bool (&done)[64]) {
   return MSPR_OK;
 }
 
-// Joins the pieces of `heads` query heads: eight waves a head where they are few and have many pieces, else one.
+// Joins the pieces of `heads` query heads: eight waves a head where they are few and have many pieces, else one. (In us, with eight and with
+// one: 256 heads of 129 pieces 42.0 and 54.8 the call, 1024 of 33 83.0 and 83.9, 2048 133 and 129, 4096 120 and 107.)
 template <int QDT, bool PARTS, bool HALF>
 int merge_launch(const SharedArgs& a, const PagedParts& own, hipStream_t st) {
   const SharedRest& r = a.rest;
@@ -1941,7 +1947,8 @@ int shared_fill(const char* what, SharedArgs& a, bool codes, const void* q, cons
   const int rep = n_q_heads / n_kv_heads;
   const int64_t most = (int64_t)table_width * page_size > (int64_t)prefix_width * page_size ? (int64_t)table_width * page_size
                                                                                            : (int64_t)prefix_width * page_size;
-  const SharedScratch s = shared_scratch(batch, n_prefixes, n_kv_heads, rep, page_size, table_width, codes);
+  const SharedScratch s = shared_scratch(batch, n_prefixes, n_kv_heads, rep, page_size, table_width,
+                                         wide_prefixes(batch, rep, (int64_t)prefix_width * page_size, codes));
   MSPR_REQUIRE((prefix_units(batch, n_prefixes, n_kv_heads, rep, s.block) + (int64_t)batch * n_kv_heads) * ((most + kTileKeys - 1) / kTileKeys + 1) <= 0x3FFFFFFF,
                "%s: the tables hold too many tokens together", what);
   MSPR_REQUIRE(mspr_aligned(q, 16) && mspr_aligned(k, 16) && mspr_aligned(v, 16) && mspr_aligned(out, 16),
@@ -1995,16 +2002,17 @@ int shared_q8_launch(const SharedArgs& a, int sb_dtype, hipStream_t st) {
 
 }  // namespace
 
-// (of both page formats, whichever needs more)
+// (of both forms, whichever needs more: which it is depends on the prefixes' tables too)
 extern "C" size_t mspr_sdpa_decode_paged_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int page_size,
                                                                 int table_width, int n_prefixes) {
   if (batch < 1 || n_kv_heads < 1 || n_q_heads < n_kv_heads || n_q_heads / n_kv_heads > 16 || n_prefixes < 1 || page_size < 1 ||
       table_width < 1)
     return 0;
   const int rep = n_q_heads / n_kv_heads;
-  const size_t rows = shared_scratch(batch, n_prefixes, n_kv_heads, rep, page_size, table_width, false).total();
-  const size_t codes = shared_scratch(batch, n_prefixes, n_kv_heads, rep, page_size, table_width, true).total();
-  return rows > codes ? rows : codes;
+  const size_t narrow = shared_scratch(batch, n_prefixes, n_kv_heads, rep, page_size, table_width, false).total();
+  if ((int64_t)batch * rep <= kColumns) return narrow;
+  const size_t wide = shared_scratch(batch, n_prefixes, n_kv_heads, rep, page_size, table_width, true).total();
+  return narrow > wide ? narrow : wide;
 }
 
 extern "C" int mspr_sdpa_decode_paged_shared(const void* queries, const void* k_pages, const void* v_pages, int dtype,

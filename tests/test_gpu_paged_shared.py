@@ -1,4 +1,7 @@
-"""GPU parity of decode attention behind shared prefixes with float64 attention over the rows as stored (bound: paged_reference.py)."""
+"""GPU parity of decode attention behind shared prefixes with float64 attention over the rows as stored (bound: paged_reference.py).
+
+Every test runs twice: with prefixes' tables as they are, and with so many entries behind them that prefixes are a kernel's own (of more
+than 32 query heads a KV head; which form a call takes goes by these and by the rows that the tables hold)."""
 
 import numpy as np
 import pytest
@@ -16,7 +19,35 @@ FORMS = [(F16, "rows"), (BF16, "rows"), (F32, F32), (F32, BF16), (F16, F16), (F1
 FEW = [(BF16, "rows"), (F16, "rows"), (F32, F32), (BF16, BF16)]
 
 
+@pytest.fixture(params=["tables", "long_tables"], autouse=True)
+def long_tables(request):
+    global LONG
+    LONG = request.param == "long_tables"
+    return LONG
+
+
+def _wide(prefix_tables, columns, page, codes):
+    return columns > 1024 or columns > 32 and columns * np.shape(prefix_tables)[1] * page >= (4 << 20 if codes else 5 << 19)
+
+
+def _tables_of(prefix_tables, columns, page):
+    """The tables, or with so many entries that name no page behind them that the form of many columns takes them."""
+    prefix_tables = np.asarray(prefix_tables)
+    if LONG and columns > 32:
+        width = -(-(4 << 20) // (columns * page))
+        prefix_tables = np.pad(prefix_tables, ((0, 0), (0, max(0, width - prefix_tables.shape[1]))), constant_values=-1)
+        assert _wide(prefix_tables, columns, page, True)
+    return prefix_tables
+
+
+def _shape_of(q, keys):
+    """Query heads of all queries and one KV head, and the page size."""
+    shape = (keys if torch.is_tensor(keys) else keys[0]).shape
+    return q.shape[0] * (q.shape[1] // shape[1]), shape[2]
+
+
 def _call(q, keys, values, prefix_tables, prefix_lens, groups, tables, lens, scale=SCALE, requests=None, **kw):
+    prefix_tables = _tables_of(prefix_tables, *_shape_of(q, keys))
     rest = (i32(prefix_tables), i32(prefix_lens), i32(groups), i32(tables), i32(lens), scale)
     kw["requests"] = None if requests is None else i32(requests)
     if torch.is_tensor(keys):
@@ -37,16 +68,17 @@ def _places(prefix_tables, prefix_lens, groups, tables, lens, requests, R, page,
     return out
 
 
-def _half_parts(q, keys):
-    """Blocks of more than 32 columns of bfloat16 rows leave partial sums of eleven digits."""
-    return torch.is_tensor(keys) and q.dtype == BF16 and q.shape[0] * (q.shape[1] // keys.shape[1]) > 32
+def _half_parts(q, keys, prefix_tables):
+    """Where prefixes are a kernel's own, bfloat16 rows leave partial sums of eleven digits."""
+    columns, page = _shape_of(q, keys)
+    return torch.is_tensor(keys) and q.dtype == BF16 and _wide(_tables_of(prefix_tables, columns, page), columns, page, False)
 
 
 def _check(q, keys, values, prefix_tables, prefix_lens, groups, tables, lens, scale=SCALE, requests=None):
     n_pages, G, page = (keys if torch.is_tensor(keys) else keys[0]).shape[:3]
     got = _call(q, keys, values, prefix_tables, prefix_lens, groups, tables, lens, scale, requests)
     at = _places(prefix_tables, prefix_lens, groups, tables, lens, requests, q.shape[0], page, n_pages, G)
-    ref.check(got, q, keys, values, at, scale, _half_parts(q, keys))
+    ref.check(got, q, keys, values, at, scale, _half_parts(q, keys, prefix_tables))
     return got
 
 
@@ -160,7 +192,7 @@ def test_as_many_queries_and_prefixes_as_a_call_takes(R, n_prefixes):
     got = _call(q, keys, values, prefix_tables, prefix_lens, groups, tables, lens, requests=requests)
     some = sorted({0, R - 1, *(int(i) for i in rng.choice(R, 40, replace=False))})
     at = _places(prefix_tables, prefix_lens, groups, tables, lens[some], requests[some], len(some), 16, 40, 2)
-    ref.check(got[some], q[some], keys, values, at, SCALE, _half_parts(q, keys))
+    ref.check(got[some], q[some], keys, values, at, SCALE, _half_parts(q, keys, prefix_tables))
     assert not got.isnan().any()
 
 
@@ -225,7 +257,7 @@ def test_the_same_call_gives_the_same_bits():
     ws = torch.full((1 << 24,), float("nan"), device="cuda")
     assert all(_call(q, keys, values, *rest, workspace=ws).equal(want) for _ in range(4))
     lens_dev = i32(rest[4])
-    args = (i32(rest[0]), i32(rest[1]), i32(rest[2]), i32(rest[3]), lens_dev, SCALE)
+    args = (i32(_tables_of(rest[0], 160, 16)), i32(rest[1]), i32(rest[2]), i32(rest[3]), lens_dev, SCALE)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         out = paged.sdpa_decode_paged_shared(q, keys, values, *args)
@@ -260,7 +292,7 @@ def test_pages_beyond_4_gb():
 
 def test_two_streams_at_once():
     cases = [_case(s, 16, 2, 64, [3000], [0] * 8, [100 * s + i for i in range(8)], BF16, "rows") for s in (1, 2)]
-    ints = [tuple(i32(a) for a in c[3:]) for c in cases]
+    ints = [(i32(_tables_of(c[3], 64, 64)), *(i32(a) for a in c[4:])) for c in cases]
     want = [paged.sdpa_decode_paged_shared(*c[:3], *i, SCALE) for c, i in zip(cases, ints)]
     torch.cuda.synchronize()
     streams, got = [torch.cuda.Stream() for _ in cases], [[], []]

@@ -145,15 +145,16 @@ def test_a_server_whose_requests_continue_prefixes(dtype, quantized, axes):
         assert (got[rows:] == 0).all()
 
 
+@pytest.mark.parametrize("max_tokens", [320, 150000])
 @pytest.mark.parametrize("dtype,quantized", FORMS)
-def test_a_prefix_once_is_a_history_of_every_request(dtype, quantized):
+def test_a_prefix_once_is_a_history_of_every_request(dtype, quantized, max_tokens):
     """Twenty requests behind a prefix of 300 rows, and the same where every request holds those rows itself: the same keys, and
-    results that are each off by no more than the bound (prompts of many rows and single tokens: both forms of the kernels)."""
+    results that are each off by no more than the bound (tables of few and of many pages: both forms of the kernels)."""
     gen = torch.Generator(device="cuda").manual_seed(6)
     block, n = _Block(2, dtype), 20
     shared = paged.PagedAttention(block, _cache(19 + 6 * n, dtype, quantized))
     apart = paged.PagedAttention(block, _cache(26 * n, dtype, quantized))
-    tables = paged.PageTables(n, 19 + 6 * n, page_size=16, max_tokens=320, n_prefixes=1)
+    tables = paged.PageTables(n, 19 + 6 * n, page_size=16, max_tokens=max_tokens, n_prefixes=1)
     others = paged.PageTables(n, 26 * n, page_size=16, max_tokens=416)
     x = torch.randn(300, HIDDEN, device="cuda", generator=gen).to(dtype)
     shared(x, tables.step(_ints([0] * n + [300]), 300), tables)
@@ -339,7 +340,7 @@ def _calls(gen, quantized=False):
     for R in (2, 37):
         q = torch.randn(R, n_kv * rep, 256, device="cuda", generator=gen).to(BF16)
         own = ints(pool, R, 30), ints(1900, R)
-        prefixes = ints(pool, 3, 40), ints(2500, 3), ints(4, R)
+        prefixes = ints(pool, 3, 40 if R == 2 else 300), ints(2500, 3), ints(4, R)  # (one launch, and prefixes by themselves)
         calls += [lambda ws, a=(q, *pages, *prefixes, *own, 0.0625): (shared(*a, workspace=ws),),
                   lambda ws, a=(q, *pages, codes, scales, *own, 0.0625, 6): (sparse(*a, workspace=ws),),
                   lambda ws, a=(q, codes, scales, *own, 6): paged.select_pages(*a, page_size=page, workspace=ws)]

@@ -7,7 +7,7 @@ import pytest
 from moespresso_amd import _lib
 
 TILE, GROUPS, MIN_SHARE, DIM, NARROW = 32, 256, 4, 256, 32
-ROWS, CODES = 256, 128  # columns of a block where prefixes are a kernel's own, of 16-bit and of 8-bit rows
+WIDE = 128  # columns of a block where prefixes are a kernel's own
 
 
 def _ceil(a, b):
@@ -60,12 +60,12 @@ def _bundle_piece(bundle, block, bundles, blocks):
     return 8 * blocks * q + block * min(8, bundles - 8 * q) + bundle % 8
 
 
-@pytest.mark.parametrize("wide", [0, CODES, ROWS])
+@pytest.mark.parametrize("wide,step", [(0, None), (WIDE, 1), (WIDE, 2)])
 @pytest.mark.parametrize("batch,n_prefixes,n_kv,rep,most_prefix,most", [
     (1, 1, 1, 1, 40, 40), (2, 1, 2, 8, 137, 40), (16, 1, 2, 8, 32768, 512), (61, 5, 2, 8, 9001, 2000), (256, 1, 2, 8, 8192, 700),
     (33, 1, 2, 8, 20001, 300), (7, 20, 4, 5, 900, 90), (300, 300, 1, 16, 2000, 10), (2048, 3, 8, 1, 300, 60), (40, 2, 1, 3, 0, 500),
     (9, 2, 2, 7, 60000, 0), (100, 100, 8, 4, 70, 70)])
-def test_every_tile_is_met_once_and_every_partial_has_a_place(batch, n_prefixes, n_kv, rep, most_prefix, most, wide):
+def test_every_tile_is_met_once_and_every_partial_has_a_place(batch, n_prefixes, n_kv, rep, most_prefix, most, wide, step):
     rng = np.random.default_rng(batch + n_prefixes)
     prefix_lens = [int(n) for n in rng.integers(0, most_prefix + 1, n_prefixes)]
     prefix_lens[-1] = most_prefix
@@ -84,7 +84,7 @@ def test_every_tile_is_met_once_and_every_partial_has_a_place(batch, n_prefixes,
         own = [(b, r, t, at - of_prefixes) for b, r, t, at in own]
         assert pieces <= grid and of_prefixes <= prefix_slots and pieces - of_prefixes <= own_slots
     else:
-        prefixes, of_prefixes = _plan(prefix_tiles, blocks, n_kv, 0, 2 if wide == ROWS and block <= 128 else 1)
+        prefixes, of_prefixes = _plan(prefix_tiles, blocks, n_kv, 0, step)
         own = []  # (dealt out as test_paged_decode_model.py has it)
         assert of_prefixes <= grid and of_prefixes <= prefix_slots
     met, places = {}, set()
@@ -133,5 +133,5 @@ def test_the_workspace_holds_every_place(batch, hq, hkv, page, width, n_prefixes
         n = 4 * n + _ceil(own_slots * (8 if wide else 128), 16) * 16 + batch * hkv * 32
         return n + (lib.mspr_sdpa_decode_paged_workspace_bytes(batch, hq, hkv, page, width) if wide else 0)
 
-    most = bytes_of(0) if batch * rep <= NARROW else max(bytes_of(CODES), bytes_of(ROWS))
+    most = bytes_of(0) if batch * rep <= NARROW else max(bytes_of(0), bytes_of(WIDE))
     assert lib.mspr_sdpa_decode_paged_shared_workspace_bytes(batch, hq, hkv, page, width, n_prefixes) == most
