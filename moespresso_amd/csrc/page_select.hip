@@ -220,6 +220,12 @@ __global__ __launch_bounds__(THREADS) void page_choose_kernel(SelectArgs a) {
     for (int i = t; i < a.selected; i += THREADS) out[i] = i < n ? id_of(table[i]) : -1;
     return;
   }
+  // (asked for now: behind the choice each would be one more access to wait for)
+  int page[kHold ? PER : 1];
+  if constexpr (kHold) {
+#pragma unroll
+    for (int i = 0; i < PER; i++) page[i] = table[min(p0 + i, n - 1)];
+  }
   auto mask_bounds = [&](float* b) {
 #pragma unroll
     for (int i = 0; i < PER; i++) b[i] = p0 + i < n ? b[i] : -__builtin_inff();
@@ -396,7 +402,7 @@ __global__ __launch_bounds__(THREADS) void page_choose_kernel(SelectArgs a) {
 #pragma unroll
   for (int i = 0; i < PER; i++)
     if (taken >> i & 1) {
-      if (at < a.selected) out[at] = id_of(table[p0 + i]);
+      if (at < a.selected) out[at] = id_of(kHold ? page[i] : table[p0 + i]);
       at++;
     }
 }
