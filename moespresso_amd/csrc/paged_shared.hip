@@ -74,7 +74,7 @@ __device__ __forceinline__ int bundle_piece(int bundle, int block, int bundles, 
   return 8 * blocks * q + block * min(8, bundles - 8 * q) + bundle % 8;
 }
 
-constexpr int kPlanInts = 3 * kMaxRows + 2 * kMaxRows;  // groups of rows; tiles of prefixes and rows; members of prefixes
+constexpr int kPlanInts = 5 * kMaxRows;  // groups and requests of queries; lengths of prefixes and queries; members of prefixes
 
 __host__ __device__ constexpr int shared_query_bytes(int qdt, int fmt) {
   return kBlocks * 8 * 64 * 16 * (fmt == kAffine && qdt == MSPR_F32 ? 2 : 1);
@@ -587,23 +587,36 @@ __global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(const int32_t
 
   // ---- the plan: which query belongs to which prefix, and how many tiles there are
   int* row_group = reinterpret_cast<int*>(lds);       // [batch]
-  int* tiles = row_group + kMaxRows;                  // [n_prefixes, then batch]
-  int* count = tiles + 2 * kMaxRows;                  // [n_prefixes]
+  int* row_request = row_group + kMaxRows;            // [batch]
+  int* length = row_request + kMaxRows;               // [n_prefixes, then batch]
+  int* count = length + 2 * kMaxRows;                 // [n_prefixes]
   const int prefix_cap = a.prefix_width << a.page_shift, cap = a.width << a.page_shift;
+  // (what a thread's first query and prefix need is asked for at once; the plan keeps all of it, so that a piece asks for no length again)
+  auto request_of = [&](int r) { return r >= batch ? -1 : requests ? requests[r] : r; };
+  auto group_of = [&](int request) { return request >= 0 && request < n_tables ? groups[request] : -1; };
+  int request = request_of(t);
+  int row_length = t < batch ? length_of(lens, batch, t, cap) : 0;
+  const int first_length = t < n_prefixes ? length_of(prefix_lens, n_prefixes, t, prefix_cap) : 0;
+  int group = group_of(request);
   for (int i = t; i < n_prefixes; i += kThreads) {
-    tiles[i] = ceil_div(length_of(prefix_lens, n_prefixes, i, prefix_cap), kTileKeys);
+    length[i] = i == t ? first_length : length_of(prefix_lens, n_prefixes, i, prefix_cap);
     count[i] = 0;
   }
   __syncthreads();
   for (int r = t; r < batch; r += kThreads) {
-    const int request = requests ? requests[r] : r;
-    const bool known = request >= 0 && request < n_tables;
-    int group = known ? groups[request] : -1;
-    if (group < 0 || group >= n_prefixes || tiles[group] == 0) group = -1;
+    if (r > t) {
+      request = request_of(r);
+      group = group_of(request);
+      row_length = length_of(lens, batch, r, cap);
+    }
+    if (group < 0 || group >= n_prefixes || length[group] == 0) group = -1;
     row_group[r] = group;
-    tiles[n_prefixes + r] = known ? ceil_div(length_of(lens, batch, r, cap), kTileKeys) : 0;
+    const bool known = request >= 0 && request < n_tables;
+    row_request[r] = known ? request : 0;
+    length[n_prefixes + r] = known ? row_length : 0;
     if (group >= 0) atomicAdd(&count[group], 1);
   }
+  auto tiles_of = [&](int e) { return ceil_div(length[e], kTileKeys); };
   if (t == 0) found.kvh = -1;
   __syncthreads();
   const int rows_a_block = kColumns / rep;
@@ -613,7 +626,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(const int32_t
   int sum = 0, units = 0;
   for (int e = e0; e < e1; e++) {
     const int blocks = blocks_of(e);
-    sum += blocks * tiles[e];
+    sum += blocks * tiles_of(e);
     units += blocks;
   }
   sum = wave_scan(sum);
@@ -636,7 +649,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(const int32_t
   const int share = max(kMinShare, ceil_div(all, max(kGroups - all_units, kGroups / 2)));
   int pieces = 0, of_prefixes = 0;
   for (int e = e0; e < e1; e++) {
-    const int ranges = max(1, ceil_div(tiles[e], share));
+    const int ranges = max(1, ceil_div(tiles_of(e), share));
     const int blocks = blocks_of(e);
     pieces += n_kv * blocks * ranges;
     if (e < n_prefixes) of_prefixes += n_kv * blocks * ranges;
@@ -657,7 +670,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(const int32_t
   }
   if (number >= before && number < before + pieces) {
     for (int e = e0; e < e1; e++) {
-      const int ranges = max(1, ceil_div(tiles[e], share));
+      const int ranges = max(1, ceil_div(tiles_of(e), share));
       const int blocks = blocks_of(e);
       const int own = n_kv * blocks * ranges;
       if (number < before + own) {
@@ -734,18 +747,16 @@ __global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(const int32_t
         rank++;
       }
     n_members = min(rows_a_block, __builtin_amdgcn_readfirstlane(count[p.prefix]) - p.block * rows_a_block);
-    n_tiles = __builtin_amdgcn_readfirstlane(tiles[p.prefix]);
-    len = __builtin_amdgcn_readfirstlane(length_of(prefix_lens, n_prefixes, p.prefix, prefix_cap));
+    len = __builtin_amdgcn_readfirstlane(length[p.prefix]);
+    n_tiles = ceil_div(len, kTileKeys);
     table = a.prefix_tables + (int64_t)p.prefix * a.prefix_width;
   } else {
-    n_tiles = __builtin_amdgcn_readfirstlane(tiles[n_prefixes + p.row]);
+    len = __builtin_amdgcn_readfirstlane(length[n_prefixes + p.row]);
+    n_tiles = ceil_div(len, kTileKeys);
     const bool alone = __builtin_amdgcn_readfirstlane(row_group[p.row]) < 0;
     whole = alone && p.ranges == 1;
     const bool some = !whole && n_tiles > 0;
-    const int request = requests ? __builtin_amdgcn_readfirstlane(requests[p.row]) : p.row;
-    len = __builtin_amdgcn_readfirstlane(length_of(lens, batch, p.row, cap));
-    table = a.tables + (int64_t)(n_tiles > 0 ? request : 0) * a.width;
-    if (n_tiles == 0) len = 0;
+    table = a.tables + (int64_t)__builtin_amdgcn_readfirstlane(row_request[p.row]) * a.width;
     if (t == 0) {
       members[0] = p.row;
       if (p.range == 0) {
