@@ -11,9 +11,10 @@
 // Sums are whole numbers below 2^24 and scales powers of two, so that a bound is exact in float32, and the selection does not
 // depend on the order of anything.
 //
-// Two launches: bounds of 16 pages a wave and step, read at the rate of HBM (516 bytes a page and KV head), and the choice, a workgroup a
-// query and KV head. The pages of a KV head are then pages of a pool of its own (page * n_kv + head,
-// one head a page), over which paged_decode.hip attends.
+// Two launches: bounds of 16 pages a wave (516 bytes a page and KV head), and the choice, a workgroup a query and KV head. Bound by
+// latency: requests and lengths, table, bounds one after the other (4.7 us for one request of 256 or of 2048 pages), then the choice's
+// barriers (4.2 us for 256 pages, 7.6 for 2048); 48 ragged requests read 49 MB of bounds in 14.2 us, 3.4 TB/s. The pages of a KV head are then
+// pages of a pool of its own (page * n_kv + head, one head a page), over which paged_decode.hip attends.
 #include "page_bounds.h"
 
 namespace {
