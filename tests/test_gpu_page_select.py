@@ -308,3 +308,28 @@ def test_pages_beyond_2_gb_of_bounds():
     want, _ = oracle.select_pages(q.double().cpu().numpy(), b.cpu().numpy(), s.cpu().numpy(), order[None], [80 * 16], 16, 7, 1, 2)
     at = want // n_kv
     assert (got.cpu().numpy() == some[at].astype(np.int64) * n_kv + want % n_kv).all()
+
+
+def test_a_query_that_is_not_a_number_stays_alone():
+    """Its own pages are some of its request's, those of the others what they were."""
+    rng = np.random.default_rng(40)
+    n_pages, page = 90, 16
+    keys, values = ref.cache(rng, (n_pages, 2, page, 256), BF16, "rows")
+    codes, scales = _empty(n_pages, 2)
+    paged.page_bounds(i32(np.arange(n_pages * page)), keys, codes, scales)
+    tables = i32(rng.permutation(n_pages)[:80].reshape(4, 20))
+    lens = i32([320, 300, 319, 33])
+    q = ref.rows(rng, (4, 16, 256), BF16)
+    args = (codes, scales, tables, lens)
+    want = paged.select_pages(q, *args, 6, page_size=page)
+    out = paged.sdpa_decode_paged_sparse(q, keys, values, *args, SCALE, 6)
+    odd = q.clone()
+    odd[1], odd[2, 3, 7], odd[2, 9, 8] = float("nan"), float("inf"), float("-inf")
+    got = paged.select_pages(odd, *args, 6, page_size=page)
+    assert got[1].equal(want[1]) and got[0][[0, 3]].equal(want[0][[0, 3]])
+    for r in (1, 2):
+        for g in range(2):
+            at = [int(p) // 2 for p in got[0][r, g]]
+            assert len(set(at)) == 6 and set(at) <= set(tables[r].tolist()) and all(int(p) % 2 == g for p in got[0][r, g])
+    after = paged.sdpa_decode_paged_sparse(odd, keys, values, *args, SCALE, 6)
+    assert after[[0, 3]].equal(out[[0, 3]]) and after[1].isnan().all()

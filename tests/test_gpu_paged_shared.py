@@ -284,10 +284,10 @@ def test_pages_beyond_4_gb():
     rng = np.random.default_rng(13)
     n_pages, page = 20000, 256
     keys, values = (torch.empty(n_pages, 2, page, 256, dtype=BF16, device="cuda") for _ in range(2))
-    tables, prefix = np.array([[n_pages - 1, 2], [n_pages - 2, n_pages - 4]]), np.array([[n_pages - 3, 5, n_pages - 5]])
+    tables, prefix = np.array([[n_pages - 1, 2], [n_pages - 2, n_pages - 4]] * 3), np.array([[n_pages - 3, 5, n_pages - 5]])
     for p in [*tables.reshape(-1), *prefix.reshape(-1)]:
         keys[p], values[p] = ref.rows(rng, (2, page, 256), BF16), ref.rows(rng, (2, page, 256), BF16)
-    _check(ref.rows(rng, (2, 16, 256), BF16), keys, values, prefix, [700], [0, 0], tables, [300, 512])
+    _check(ref.rows(rng, (6, 16, 256), BF16), keys, values, prefix, [700], [0] * 6, tables, [300, 512, 0, 1, 257, 256])
 
 
 def test_two_streams_at_once():
@@ -302,3 +302,22 @@ def test_two_streams_at_once():
                 got[k].append(paged.sdpa_decode_paged_shared(*cases[k][:3], *ints[k], SCALE))
     torch.cuda.synchronize()
     assert all(g.equal(want[k]) for k in (0, 1) for g in got[k])
+
+
+@pytest.mark.parametrize("dtype,form", FEW)
+def test_what_is_no_number_stays_with_its_query(dtype, form):
+    """A query, a prefix's row and a request's own row that hold NaN or infinities: the results of all others keep their bits."""
+    q, keys, values, prefix_tables, prefix_lens, groups, tables, lens = _case(31, 16, 2, 16, [300, 50, 40], [0] * 7 + [1] * 7 + [2, -1, 2], [40, 1, 0, 17, 70] * 3 + [9, 5], dtype, form)
+    args = prefix_tables, prefix_lens, groups, tables, lens
+    want = _call(q, keys, values, *args)
+    odd = q.clone()
+    odd[3], odd[8, ::2], odd[9, :, 5] = float("nan"), float("inf"), float("-inf")
+    got = _call(odd, keys, values, *args)
+    others = [r for r in range(len(lens)) if r not in (3, 8, 9)]
+    assert got[others].equal(want[others]) and got[8, 1::2].equal(want[8, 1::2]) and got[3].isnan().all()
+    for side in (keys, values):
+        for t in (side,) if torch.is_tensor(side) else side[1:]:
+            t[int(prefix_tables[2][1]), :, 3], t[int(tables[15][0]), :, 2] = float("nan"), float("inf")
+    got = _call(q, keys, values, *args)
+    others = [r for r in range(len(lens)) if r not in (14, 15, 16)]
+    assert got[others].equal(want[others]) and not got[14].isfinite().any() and not got[16].isfinite().any()
