@@ -163,6 +163,16 @@ __device__ __forceinline__ float wave_max(float v) {
   v = fmaxf(v, lane_xor<8>(v));
   return half_wave_max(row_pair_max(v));
 }
+// One step of the largest values of 2 HALF numbers a lane: lanes that differ in bit X exchange, and keep half of the numbers each.
+template <int HALF, int X>
+__device__ __forceinline__ void fold_max(float* v, int lane) {
+  const bool up = (lane & X) != 0;
+#pragma unroll
+  for (int j = 0; j < HALF; j++) {
+    const float keep = up ? v[HALF + j] : v[j], give = up ? v[j] : v[HALF + j];
+    v[j] = fmaxf(keep, lane_xor<X>(give));
+  }
+}
 __device__ __forceinline__ int wave_sum_upto(int v) {  // sums over this lane and those before it, by data-parallel moves
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
   v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
@@ -242,14 +252,19 @@ __global__ __launch_bounds__(THREADS) void page_choose_kernel(SelectArgs a) {
     float best[HEADS];
 #pragma unroll
     for (int h = 0; h < HEADS; h++) {
-      mask_bounds(held[h]);
+      if (64 * PER * (wave + 1) > n) mask_bounds(held[h]);  // (wave-uniform: of the others all are there)
       best[h] = best_of(held[h]);
     }
-#pragma unroll
-    for (int h = 0; h < HEADS; h++) {
-      best[h] = wave_max(best[h]);
-      if (lane == 0) tops[wave][h] = best[h];
-    }
+    // (all heads together: a third of the instructions of one reduction a head)
+    fold_max<HEADS / 2, 1>(best, lane);
+    fold_max<HEADS / 4, 2>(best, lane);
+    fold_max<HEADS / 8, 4>(best, lane);
+    if constexpr (HEADS == 16) fold_max<1, 8>(best, lane);
+    else best[0] = fmaxf(best[0], lane_xor<8>(best[0]));
+    best[0] = half_wave_max(row_pair_max(best[0]));
+    const int head = HEADS == 16 ? 8 * (lane & 1) + 4 * (lane >> 1 & 1) + 2 * (lane >> 2 & 1) + (lane >> 3 & 1)
+                                 : 4 * (lane & 1) + 2 * (lane >> 1 & 1) + (lane >> 2 & 1);
+    if (lane < HEADS) tops[wave][head] = best[0];
   } else {
 #pragma unroll 1
     for (int h = 0; h < HEADS; h++) {
