@@ -21,7 +21,7 @@
 // What bounds it: few queries the chain of accesses (requests, groups, lengths, table, rows) and two launches; long prefixes of few
 // queries HBM (16 queries over 32768 rows: the tiles' loop reads 6.4 TB/s, 10 of the kernel's 25 us; the others are the plan, the first
 // tiles, and 16 MB of partials); many columns the matrix units (256 queries over 8192 rows: 45 us at the rate of a library's product
-// with two terms a weight, 57 taken); 8-bit rows a wave's own chain of scales, terms and cross-lane moves (60 us for 33 queries over
+// with two terms a weight, 55 to 65 taken); 8-bit rows a wave's own chain of scales, terms and cross-lane moves (60 us for 33 queries over
 // 20001 rows).
 #include "paged_parts.h"
 
