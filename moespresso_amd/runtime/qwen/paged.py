@@ -677,11 +677,15 @@ class PageTables:
     n_prefixes - 1`` of ``new_lens``. A prefix gets its rows like any request (in one step or some) and gives its pages back
     like any; a request that ``continue_prefix`` named to continue it sees its rows in front of its own, and is counted on from
     its length. It has to stay as it is while requests continue it. (``n_prefixes=0``: none, and nothing is computed for them.)
+    ``max_prefix_tokens``: what a prefix has at most, in whole pages; rows behind that are no part of it. Where it is far less than
+    ``max_tokens`` the attention takes a form for short prefixes (how long they are is known on the device only).
     """
 
     def __init__(self, batch: int, n_pages: int, page_size: int = 64, max_tokens: int = 131072, device="cuda", *,
-                 n_prefixes: int = 0):
+                 n_prefixes: int = 0, max_prefix_tokens: int | None = None):
         _check_page_size(page_size)
+        if max_prefix_tokens is not None and (n_prefixes == 0 or not 1 <= max_prefix_tokens <= max_tokens):
+            raise ValueError("max_prefix_tokens must be 1 to max_tokens, of tables with prefixes")
         if n_prefixes < 0 or (n_prefixes > 0 and not 1 <= batch <= MAX_REQUESTS - n_prefixes):
             raise ValueError(f"requests and prefixes must be 1 to {MAX_REQUESTS} together")
         self.page_size, self.batch, self.n_prefixes = page_size, batch, n_prefixes
@@ -692,6 +696,9 @@ class PageTables:
         self.head = torch.zeros((1,), dtype=torch.int32, device=device)
         # the prefix that a request continues, -1: none
         self.groups = torch.full((batch,), -1, dtype=torch.int32, device=device) if n_prefixes else None
+        # the first pages of the prefixes' tables, where these are wider
+        self.prefix_tables = None if max_prefix_tokens is None else torch.full(
+            (n_prefixes, -(-max_prefix_tokens // page_size)), -1, dtype=torch.int32, device=device)
 
     def continue_prefix(self, request: int, prefix):
         """``request`` continues ``prefix`` (from 0 on; None: none) from now on: before its first row. It stays so until said otherwise."""
@@ -702,7 +709,9 @@ class PageTables:
     @property
     def prefixes(self):
         """``(prefix_tables, prefix_lens, groups)`` of ``sdpa_decode_paged_shared``; None without prefixes."""
-        return None if self.groups is None else (self.tables[self.batch:], self.lens[self.batch:], self.groups)
+        if self.groups is None:
+            return None
+        return self.tables[self.batch:] if self.prefix_tables is None else self.prefix_tables, self.lens[self.batch:], self.groups
 
     def step(self, new_lens, n_rows: int) -> PageStep:
         """``page_step`` that carries the lengths and the stack on (in place, so that a captured step follows them); positions
@@ -715,7 +724,12 @@ class PageTables:
             return step
         # (places that are none wrap round and are masked; a prefix outside the tables is none, as for the operators)
         known = (self.groups >= 0) & (self.groups < self.n_prefixes)
-        before = torch.where(known, self.lens[self.batch:][torch.where(known, self.groups, 0)], 0)
+        lens = self.lens[self.batch:]
+        if self.prefix_tables is not None:
+            width = int(self.prefix_tables.shape[1])
+            self.prefix_tables.copy_(self.tables[self.batch:, :width])
+            lens = lens.clamp(max=width * self.page_size)
+        before = torch.where(known, lens[torch.where(known, self.groups, 0)], 0)
         return step._replace(positions=step.positions + torch.where(step.requests >= 0, before[step.requests], 0),
                              requests=torch.where(step.slots >= 0, step.requests, -1))
 

@@ -145,16 +145,16 @@ def test_a_server_whose_requests_continue_prefixes(dtype, quantized, axes):
         assert (got[rows:] == 0).all()
 
 
-@pytest.mark.parametrize("max_tokens", [320, 150000])
+@pytest.mark.parametrize("max_tokens,max_prefix", [(320, None), (150000, None), (150000, 301)])
 @pytest.mark.parametrize("dtype,quantized", FORMS)
-def test_a_prefix_once_is_a_history_of_every_request(dtype, quantized, max_tokens):
+def test_a_prefix_once_is_a_history_of_every_request(dtype, quantized, max_tokens, max_prefix):
     """Twenty requests behind a prefix of 300 rows, and the same where every request holds those rows itself: the same keys, and
     results that are each off by no more than the bound (tables of few and of many pages: both forms of the kernels)."""
     gen = torch.Generator(device="cuda").manual_seed(6)
     block, n = _Block(2, dtype), 20
     shared = paged.PagedAttention(block, _cache(19 + 6 * n, dtype, quantized))
     apart = paged.PagedAttention(block, _cache(26 * n, dtype, quantized))
-    tables = paged.PageTables(n, 19 + 6 * n, page_size=16, max_tokens=max_tokens, n_prefixes=1)
+    tables = paged.PageTables(n, 19 + 6 * n, page_size=16, max_tokens=max_tokens, n_prefixes=1, max_prefix_tokens=max_prefix)
     others = paged.PageTables(n, 26 * n, page_size=16, max_tokens=416)
     x = torch.randn(300, HIDDEN, device="cuda", generator=gen).to(dtype)
     shared(x, tables.step(_ints([0] * n + [300]), 300), tables)
@@ -247,7 +247,7 @@ def test_a_captured_step_follows_prefixes_and_bounds(quantized, selects):
     places = 7 if not selects else 5
 
     def server():
-        return (paged.PageTables(5, 60, page_size=16, max_tokens=256, n_prefixes=0 if selects else 2),
+        return (paged.PageTables(5, 60, page_size=16, max_tokens=256, **({} if selects else dict(n_prefixes=2, max_prefix_tokens=40))),
                 [paged.PagedAttention(b, _cache(60, BF16, quantized, bounds=selects), **kwargs) for b in blocks])
 
     gen = torch.Generator(device="cuda").manual_seed(9)

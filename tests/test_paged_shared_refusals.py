@@ -336,6 +336,27 @@ def test_tables_refuse_prefixes_they_have_no_place_for():
             paged.PageTables(batch, 4, page_size=16, max_tokens=64, device="cpu", n_prefixes=n)
 
 
+def test_tables_refuse_lengths_of_prefixes():
+    for kwargs in (dict(max_prefix_tokens=16), dict(n_prefixes=1, max_prefix_tokens=0), dict(n_prefixes=1, max_prefix_tokens=65)):
+        with pytest.raises(ValueError, match="max_prefix_tokens"):
+            _tables(**kwargs)
+    assert [tuple(t.shape) for t in _tables(n_prefixes=2, max_prefix_tokens=17).prefixes] == [(2, 2), (2,), (4,)]
+
+
+def test_a_prefix_ends_with_its_pages(monkeypatch):
+    """Rows behind ``max_prefix_tokens`` are seen by nobody, and positions count on from there."""
+    tables = _tables(n_prefixes=2, max_prefix_tokens=20)
+    ints = lambda *a: torch.tensor(a, dtype=I32)
+    step = paged.PageStep(ints(5, 2, 40, 7), ints(3), ints(0, 2, 3, 3, 3), ints(3, 4, 5), ints(3, 4, 1), ints(4, 5, 2), ints(0, 0, 1), ints(0, 0, 0, 0))
+    monkeypatch.setattr(paged, "page_step", lambda *a, **k: step)
+    tables.tables.copy_(torch.arange(16, dtype=I32).reshape(4, 4))
+    tables.continue_prefix(0, 0)
+    tables.continue_prefix(1, 1)
+    held = tables.prefix_tables
+    got = tables.step(ints(2, 1, 0, 0), 3)
+    assert got.positions.tolist() == [35, 36, 8] and tables.prefixes[0] is held and held.tolist() == [[8, 9], [12, 13]]
+
+
 def test_positions_are_counted_from_the_prefix(monkeypatch):
     """(The step itself is stood in for.) Places that name no prefix, and rows of no request, are left as they are."""
     tables = _tables(n_prefixes=2)
