@@ -238,7 +238,7 @@ def paged_shared_workspace(batch: int, n_q_heads: int, n_kv_heads: int, page_siz
 
 
 def select_pages_workspace(batch: int, n_q_heads: int, n_kv_heads: int, table_width: int, device) -> torch.Tensor:
-    """Scratch tensor for mspr_select_pages (bounds of every page, query head and query, and maxima of sixteen pages)."""
+    """Scratch tensor for mspr_select_pages (bounds of every page, query head and query)."""
     nbytes = int(lib().mspr_select_pages_workspace_bytes(int(batch), int(n_q_heads), int(n_kv_heads), int(table_width)))
     return torch.empty((max(nbytes, 16) + 3) // 4, dtype=torch.float32, device=device)
 
