@@ -20,7 +20,7 @@
 //
 // What bounds it: few queries the chain of accesses (requests, groups, lengths, table, rows) and two launches; long prefixes of few
 // queries HBM (16 queries over 32768 rows: the tiles' loop reads 6.4 TB/s, 10 of the kernel's 25 us; the others are the plan, the first
-// tiles, and 16 MB of partials); many columns the matrix units (256 queries over 8192 rows: 45 us at the rate of a library's product
+// tiles, and 34 MB of partials); many columns the matrix units (256 queries over 8192 rows: 45 us at the rate of a library's product
 // with two terms a weight, 55 to 65 taken); 8-bit rows a wave's own chain of scales, terms and cross-lane moves (60 us for 33 queries over
 // 20001 rows).
 #include "paged_parts.h"
@@ -47,8 +47,8 @@ struct SharedRest {
   int n_pages, page_shift, prefix_width, width, prefix_slots, own_slots;
   int block;          // columns of a block of a prefix's members, at most
   float scale_log2;
-  void* ws_pre;       // partial outputs of prefix pieces [prefix_slots][block columns][256], float32 or scaled float16
-  float* ws_pre_ml;   // their statistics [prefix_slots][block][4]: maximum, sum of weights, scale
+  float* ws_pre;      // partial outputs of prefix pieces [prefix_slots][block columns][256]
+  float* ws_pre_ml;   // their statistics [prefix_slots][block][4]: maximum, sum of weights, two that nothing uses
   float* ws_own;      // of own pieces [own_slots][rep][256]
   float* ws_own_ml;   // [own_slots][16][2]
   int32_t* parts;     // [B * n_kv][8]: of own pieces the first and how many; of prefix pieces the first, ranges, blocks, first column
@@ -521,8 +521,9 @@ __device__ __forceinline__ void attend_piece(const SharedRest& a, const Piece& p
   float* xo = reinterpret_cast<float*>(lds);   // [waves][16 mt][64 lanes][4]
   float* xml = xo + kWaves * 16 * 64 * 4;      // [waves][16 columns][2]
   const int width = p.prefix >= 0 ? a.block : rep;  // columns of a partial
-  const auto po = store_window((p.prefix >= 0 ? reinterpret_cast<float*>(a.ws_pre) : a.ws_own) + (int64_t)p.slot * width * kD, width * kD * (int)sizeof(float));
+  const auto po = store_window((p.prefix >= 0 ? a.ws_pre : a.ws_own) + (int64_t)p.slot * width * kD, width * kD * (int)sizeof(float));
   float* ml = p.prefix >= 0 ? a.ws_pre_ml + (int64_t)p.slot * a.block * 4 : a.ws_own_ml + (int64_t)p.slot * 16 * 2;
+  const int ml_pitch = p.prefix >= 0 ? 4 : 2;
 #pragma unroll
   for (int b = 0; b < NB; b++) {
     l_run[b] += __shfl_xor(l_run[b], 16, MSPR_WAVE);
@@ -564,10 +565,7 @@ __device__ __forceinline__ void attend_piece(const SharedRest& a, const Piece& p
       if (whole) store_out<QDT>(a.out, (((int64_t)p.row * n_kv + p.kvh) * rep + column) * kD + 16 * mt + 4 * g, acc, l_all);
       else window_store<kStoreThrough>(po, (column * kD + 16 * mt + 4 * g) * 4, __builtin_bit_cast(u32x4_t, acc));
     }
-    if (!whole && wave == 0 && g == 0 && mine[b]) {
-      if (p.prefix >= 0) *reinterpret_cast<f32x4_t*>(ml + 4 * column) = f32x4_t{m_all, l_all, 1.0f, 0.0f};
-      else *reinterpret_cast<f32x2_t*>(ml + 2 * column) = f32x2_t{m_all, l_all};
-    }
+    if (!whole && wave == 0 && g == 0 && mine[b]) *reinterpret_cast<f32x2_t*>(ml + ml_pitch * column) = f32x2_t{m_all, l_all};
   }
 }
 
@@ -1025,88 +1023,54 @@ __device__ __forceinline__ void prefix_piece(const SharedRest& a, const int32_t*
   int tl = tid;
   asm volatile("" : "+v"(tl));  // (the offsets below are made here, not carried through the tile loop)
   const int en = tl & 31, eg = (tl >> 5) & 1;
-  {
-    f32x4_t* xo = reinterpret_cast<f32x4_t*>(lds + (wave % kColumnWaves) * 32768) + (tl & 63);  // [32 quads][64 lanes]
-    if (part == 1 && mine > 0) {
-#pragma unroll
-      for (int mt = 0; mt < 8; mt++)
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-          xo[64 * (4 * mt + c)] = f32x4_t{oacc[mt][4 * c], oacc[mt][4 * c + 1], oacc[mt][4 * c + 2], oacc[mt][4 * c + 3]};
-      if (eg == 0) {
-        xml[wave % kColumnWaves][en][0] = m_run;
-        xml[wave % kColumnWaves][en][1] = l_run;
-      }
-    }
-    __syncthreads();
-    if (part == 1 || mine == 0) return;
-    const float m2 = xml[wave][en][0], l2 = xml[wave][en][1];
-    const float m_all = fmaxf(m_run, m2), m_safe = m_all == -__builtin_inff() ? 0.0f : m_all;
-    const float w1 = __builtin_amdgcn_exp2f(m_run - m_safe), w2 = __builtin_amdgcn_exp2f(m2 - m_safe);
-    m_run = m_all;
-    l_run = l_run * w1 + l2 * w2;
+  unsigned char* region = lds + (wave % kColumnWaves) * 32768;
+  f32x4_t* xo = reinterpret_cast<f32x4_t*>(region) + (tl & 63);  // [32 quads][64 lanes]
+  if (part == 1 && mine > 0) {
 #pragma unroll
     for (int mt = 0; mt < 8; mt++)
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        const f32x4_t o = xo[64 * (4 * mt + c)];
-#pragma unroll
-        for (int i = 0; i < 4; i++) oacc[mt][4 * c + i] = oacc[mt][4 * c + i] * w1 + o[i] * w2;
-      }
+      for (int c = 0; c < 4; c++)
+        xo[64 * (4 * mt + c)] = f32x4_t{oacc[mt][4 * c], oacc[mt][4 * c + 1], oacc[mt][4 * c + 2], oacc[mt][4 * c + 3]};
+    if (eg == 0) {
+      xml[wave % kColumnWaves][en][0] = m_run;
+      xml[wave % kColumnWaves][en][1] = l_run;
+    }
   }
+  __syncthreads();
+  if (part == 1 || mine == 0) return;
+  const float m2 = xml[wave][en][0], l2 = xml[wave][en][1];
+  const float m_all = fmaxf(m_run, m2), m_safe = m_all == -__builtin_inff() ? 0.0f : m_all;
+  const float w1 = __builtin_amdgcn_exp2f(m_run - m_safe), w2 = __builtin_amdgcn_exp2f(m2 - m_safe);
   int row0 = slot * a.block + column0;  // (a scalar by hand: with the lanes' addresses below, the compiler takes it for one of each lane's)
   asm volatile("" : "+s"(row0));
-  unsigned char* xo = lds + (wave << 15);  // (where the wave's own exchange was)
-  if constexpr (FMT == MSPR_BF16) {
-    // As float16, scaled by a power of two that brings a column's largest sum to [1/2, 1): partials are as many bytes as the rows
-    // themselves where a compute unit has few tiles (16 queries over 32768 rows, 29 MB), and eleven digits of a part are more
-    // than the result has (one rounding of 2^-12 of the attention over |V| beside its 2^-9). Float32 ones: 46.4 us instead of 42.0, 256
-    // queries over 8192 rows 116 instead of 108.
-    float top = 0.0f;
+  if (eg == 0 && en < mine) *reinterpret_cast<f32x2_t*>(a.ws_pre_ml + 4 * (int64_t)(row0 + en)) = f32x2_t{m_all, l_run * w1 + l2 * w2};
+  const auto to = store_window(a.ws_pre + (int64_t)row0 * kD, mine * kD * 4);
+  // (half of the channels at a time: the first half's exchange is over when its rows take the place)
 #pragma unroll
-    for (int mt = 0; mt < 8; mt++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) top = fmaxf(top, fabsf(oacc[mt][i]));
-    top = half_wave_max(top);
-    const int e = top > 0.0f && top < __builtin_inff() ? max(__builtin_amdgcn_frexp_expf(top), -120) : 0;
-    const float by = __builtin_amdgcn_ldexpf(1.0f, -e);
-    if (eg == 0 && en < mine)
-      *reinterpret_cast<f32x4_t*>(a.ws_pre_ml + 4 * (int64_t)(row0 + en)) = f32x4_t{m_run, l_run, __builtin_amdgcn_ldexpf(1.0f, e), 0.0f};
-    const auto to = store_window(reinterpret_cast<uint16_t*>(a.ws_pre) + (int64_t)row0 * kD, mine * kD * 2);
+  for (int h = 0; h < 2; h++) {
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int mt = 0; mt < 8; mt++)
+    for (int mt = 0; mt < 4; mt++)
 #pragma unroll
       for (int c = 0; c < 4; c++) {
-        const h2_t lo = {(_Float16)(oacc[mt][4 * c] * by), (_Float16)(oacc[mt][4 * c + 1] * by)};
-        const h2_t hi = {(_Float16)(oacc[mt][4 * c + 2] * by), (_Float16)(oacc[mt][4 * c + 3] * by)};
-        *reinterpret_cast<u32x2_t*>(xo + en * 512 + 16 * ((4 * mt + c) ^ (en & 15)) + 8 * eg) = u32x2_t{h2_bits(lo), h2_bits(hi)};
+        const f32x4_t other = xo[64 * (16 * h + 4 * mt + c)];
+#pragma unroll
+        for (int i = 0; i < 4; i++) oacc[4 * h + mt][4 * c + i] = oacc[4 * h + mt][4 * c + i] * w1 + other[i] * w2;
+      }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int mt = 0; mt < 4; mt++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const f32x16_t& o = oacc[4 * h + mt];
+        *reinterpret_cast<f32x4_t*>(region + en * 512 + 16 * ((8 * mt + 2 * c + eg) ^ (en & 15))) =
+            f32x4_t{o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]};
       }
 #pragma unroll
     for (int i = 0; i < 16; i++) {
       const int r = 2 * i + eg;
-      window_store<kStoreThrough>(to, r * kD * 2 + 16 * en, *reinterpret_cast<const u32x4_t*>(xo + r * 512 + 16 * (en ^ (r & 15))));
-    }
-  } else {
-    if (eg == 0 && en < mine) *reinterpret_cast<f32x4_t*>(a.ws_pre_ml + 4 * (int64_t)(row0 + en)) = f32x4_t{m_run, l_run, 1.0f, 0.0f};
-    const auto to = store_window(reinterpret_cast<float*>(a.ws_pre) + (int64_t)row0 * kD, mine * kD * 4);
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int mt = 0; mt < 4; mt++)
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          const f32x16_t& o = oacc[4 * h + mt];
-          *reinterpret_cast<f32x4_t*>(xo + en * 512 + 16 * ((8 * mt + 2 * c + eg) ^ (en & 15))) =
-              f32x4_t{o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]};
-        }
-#pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const int r = 2 * i + eg;
-        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(xo + r * 512 + 16 * (en ^ (r & 15)));
-        window_store<kStoreThrough>(to, r * kD * 4 + 512 * h + 16 * en, __builtin_bit_cast(u32x4_t, v));
-      }
+      const f32x4_t v = *reinterpret_cast<const f32x4_t*>(region + r * 512 + 16 * (en ^ (r & 15)));
+      window_store<kStoreThrough>(to, r * kD * 4 + 512 * h + 16 * en, __builtin_bit_cast(u32x4_t, v));
     }
   }
 }
@@ -1624,13 +1588,13 @@ __device__ __forceinline__ void codes_piece(const SharedRest& a, const int32_t* 
   for (int j = 0; j < 4; j++) bias[j] = __shfl(bacc[j], n, MSPR_WAVE);
   int row0 = slot * a.block + column0;  // (a scalar by hand, as of the 16-bit form)
   asm volatile("" : "+s"(row0));
-  if (g == 0 && n < mine) *reinterpret_cast<f32x4_t*>(a.ws_pre_ml + 4 * (int64_t)(row0 + n)) = f32x4_t{m_run, l_run, 1.0f, 0.0f};
+  if (g == 0 && n < mine) *reinterpret_cast<f32x4_t*>(a.ws_pre_ml + 4 * (int64_t)(row0 + n)) = f32x4_t{m_run, l_run, 0.0f, 0.0f};
   unsigned char* xo = lds + (wave << 14);
   static_for<16>([&](auto mt) {
     constexpr int m = decltype(mt)::value;
     *reinterpret_cast<f32x4_t*>(xo + n * 1024 + 16 * ((4 * m + g) ^ n)) = oacc[m] * of_lane<m / 4>(v_unit) + bias[m / 4];
   });
-  const auto to = store_window(reinterpret_cast<float*>(a.ws_pre) + (int64_t)row0 * kD, mine * kD * 4);
+  const auto to = store_window(a.ws_pre + (int64_t)row0 * kD, mine * kD * 4);
 #pragma unroll
   for (int r = 0; r < 16; r++)
     window_store<kStoreThrough>(to, r * 1024 + 16 * lane, *reinterpret_cast<const u32x4_t*>(xo + r * 1024 + 16 * (lane ^ r)));
@@ -1651,17 +1615,16 @@ __global__ __launch_bounds__(kWideThreads, 1) void paged_prefix_codes_kernel(con
 }
 
 constexpr int kAtOnce = 16;  // pieces that a wave joins at a time
-typedef __attribute__((address_space(1))) u32x2_t global_words_t;
 typedef __attribute__((address_space(1))) u32x4_t global_quads_t;
 
 // Joins the pieces of one query head: WAVES of them a head take every WAVES-th, and meet in LDS. PARTS: own rows are
 // paged_decode.hip's parts (own: of rows that are not cut), else pieces of paged_shared_kernel.
 // grid: heads / (kMergeWaves / WAVES)
 constexpr int kMergeWaves = 8;
-template <int ODT, int WAVES, bool PARTS, bool HALF>  // HALF: partials of prefixes are scaled float16 numbers
+template <int ODT, int WAVES, bool PARTS>
 __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(const int32_t* parts, const int32_t* cuts, int rep, int n_kv,
                                                                               int rows, int block, int prefix_slots, int own_slots,
-                                                                              int shares, bool cut_rows, const void* ws_pre, const float* ws_pre_ml,
+                                                                              int shares, bool cut_rows, const float* ws_pre, const float* ws_pre_ml,
                                                                               const float* ws_own, const float* ws_own_ml,
                                                                               const float* part_o, const float* part_ml, void* out) {
   __shared__ __attribute__((aligned(16))) float xo[kMergeWaves][kD + 2];
@@ -1682,8 +1645,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
   const int total = n_own + ranges;
   const int kvh = row % n_kv, column_block = column / block, column_at = column - column_block * block;
   struct From {
-    const void* o;
-    const float* ml;
+    const float *o, *ml;
   };
   // Sums and statistics of own piece i, of prefix piece i (bounded by the workspace, whatever is there)
   auto own_piece = [&](int i) {
@@ -1698,18 +1660,15 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
   auto prefix_piece = [&](int i) {
     const int s = pre_first + bundle_piece(kvh * ranges + i, column_block, n_kv * ranges, blocks);
     const int64_t r = (int64_t)(s >= 0 && s < prefix_slots ? s : 0) * block + column_at;
-    return From{reinterpret_cast<const uint8_t*>(ws_pre) + r * kD * (HALF ? 2 : 4), ws_pre_ml + 4 * r};
+    return From{ws_pre + r * kD, ws_pre_ml + 4 * r};
   };
   float m = -__builtin_inff(), l = 0.0f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   for (int p0 = part; p0 < total; p0 += kAtOnce * WAVES) {
     // Lane j finds piece j, of those past the end the last. (One load of either kind of piece, so that none waits for the other.)
     const int mine = p0 + WAVES * (lane % kAtOnce), near = min(mine, total - 1);
-    const bool pre = near >= n_own;
-    const From from = pre ? prefix_piece(near - n_own) : own_piece(near);
+    const From from = near >= n_own ? prefix_piece(near - n_own) : own_piece(near);
     f32x2_t stat = *reinterpret_cast<const f32x2_t*>(from.ml);
-    float scale = HALF ? from.ml[pre ? 2 : 0] : 1.0f;
-    if (!pre) scale = 1.0f;
     if (mine >= total) stat = f32x2_t{-__builtin_inff(), 0.0f};
     const uint64_t o_at = reinterpret_cast<uint64_t>(from.o);
     u32x4_t ov[kAtOnce];
@@ -1719,20 +1678,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
       if (i >= total) continue;
       const uint64_t o_j = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)o_at, j) |
                            (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(o_at >> 32), j) << 32;
-      if constexpr (HALF) {
-        const bool whole = i < n_own;  // (four floats a lane, or four float16 numbers)
-        const uint64_t o_lane = o_j + (uint32_t)((whole ? 16 : 8) * lane);
-        const u32x2_t lo = *reinterpret_cast<const global_words_t*>(o_lane);
-        ov[j].x = lo.x;
-        ov[j].y = lo.y;
-        if (whole) {
-          const u32x2_t hi = *reinterpret_cast<const global_words_t*>(o_lane + 8);
-          ov[j].z = hi.x;
-          ov[j].w = hi.y;
-        }
-      } else {
-        ov[j] = reinterpret_cast<const global_quads_t*>(o_j)[lane];
-      }
+      ov[j] = reinterpret_cast<const global_quads_t*>(o_j)[lane];
     }
     float m_new = stat.x;
     m_new = fmaxf(m_new, lane_xor<1>(m_new));
@@ -1748,17 +1694,11 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
     lw += lane_xor<4>(lw);
     l = l * alpha + (lw + lane_xor<8>(lw));
     o = o * alpha;
-    const float of_sums = w * scale;
 #pragma unroll
     for (int j = 0; j < kAtOnce; j++) {
       const int i = p0 + WAVES * j;
       if (i >= total) continue;
-      f32x4_t v = __builtin_bit_cast(f32x4_t, ov[j]);
-      if (HALF && i >= n_own) {
-        const h2_t lo = bits_h2(ov[j].x), hi = bits_h2(ov[j].y);
-        v = f32x4_t{(float)lo.x, (float)lo.y, (float)hi.x, (float)hi.y};
-      }
-      o += v * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(of_sums), j));
+      o += __builtin_bit_cast(f32x4_t, ov[j]) * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), j));
     }
     m = m_new;
   }
@@ -1862,13 +1802,13 @@ int reserve_lds(K* kernel, int bytes, bool (&done)[64]) {
 
 // Joins the pieces of `heads` query heads: eight waves a head where they are few and have many pieces, else one. (In us, with eight and with
 // one: 256 heads of 129 pieces 42.0 and 54.8 the call, 1024 of 33 83.0 and 83.9, 2048 133 and 129, 4096 120 and 107.)
-template <int QDT, bool PARTS, bool HALF>
+template <int QDT, bool PARTS>
 int merge_launch(const SharedArgs& a, const PagedParts& own, hipStream_t st) {
   const SharedRest& r = a.rest;
   const int heads = a.batch * a.n_kv * a.rep;
   auto merge = [&](auto waves) {
     constexpr int kWavesAHead = decltype(waves)::value, kHeads = kMergeWaves / kWavesAHead;
-    paged_shared_merge_kernel<QDT, kWavesAHead, PARTS, HALF><<<dim3((unsigned)((heads + kHeads - 1) / kHeads)), dim3(64 * kMergeWaves), 0, st>>>(
+    paged_shared_merge_kernel<QDT, kWavesAHead, PARTS><<<dim3((unsigned)((heads + kHeads - 1) / kHeads)), dim3(64 * kMergeWaves), 0, st>>>(
         r.parts, own.cut ? own.cut : r.parts, a.rep, a.n_kv, a.batch * a.n_kv, r.block, r.prefix_slots, r.own_slots, own.shares,
         own.cut != nullptr, r.ws_pre, r.ws_pre_ml, r.ws_own, r.ws_own_ml, own.o, own.ml, r.out);
   };
@@ -1887,11 +1827,11 @@ int shared_launch(const SharedArgs& a, hipStream_t st) {
   paged_shared_kernel<QDT, FMT, SDT><<<dim3((unsigned)a.pieces), dim3(kThreads), kLds, st>>>(
       a.requests, a.groups, a.lens, a.prefix_lens, a.batch, a.n_prefixes, a.n_tables, a.n_kv, a.rep, a.rest);
   MSPR_CHECK_LAUNCH("sdpa_decode_paged_shared");
-  return merge_launch<QDT, false, false>(a, PagedParts{}, st);
+  return merge_launch<QDT, false>(a, PagedParts{}, st);
 }
 
 // Own rows, then prefixes by `kernel`.
-template <int QDT, bool HALF, typename K>
+template <int QDT, typename K>
 int wide_launch(const char* what, const SharedArgs& a, int sb_dtype, K* kernel, int lds, bool (&reserved)[64], hipStream_t st) {
   if (int rc = reserve_lds(kernel, lds, reserved)) return rc;
   const SharedRest& r = a.rest;
@@ -1925,19 +1865,19 @@ int wide_launch(const char* what, const SharedArgs& a, int sb_dtype, K* kernel, 
   kernel<<<dim3((unsigned)a.pieces), dim3(kWideThreads), lds, st>>>(a.requests, a.groups, a.prefix_lens, a.batch, a.n_prefixes, a.n_tables,
                                                                     a.n_kv, a.rep, r);
   MSPR_CHECK_LAUNCH("sdpa_decode_paged_shared (prefixes)");
-  return merge_launch<QDT, true, HALF>(a, own, st);
+  return merge_launch<QDT, true>(a, own, st);
 }
 template <int FMT>
 int rows_launch(const SharedArgs& a, hipStream_t st) {
   static bool reserved[64] = {};
   if (!a.wide) return shared_launch<FMT, FMT, FMT>(a, st);
-  return wide_launch<FMT, FMT == MSPR_BF16>("sdpa_decode_paged_shared", a, FMT, &paged_prefix_kernel<FMT>, kWideLds, reserved, st);
+  return wide_launch<FMT>("sdpa_decode_paged_shared", a, FMT, &paged_prefix_kernel<FMT>, kWideLds, reserved, st);
 }
 template <int QDT, int SDT>
 int codes_launch(const SharedArgs& a, hipStream_t st) {
   static bool reserved[64] = {};
   if (!a.wide) return shared_launch<QDT, kAffine, SDT>(a, st);
-  return wide_launch<QDT, false>("sdpa_decode_paged_shared_q8", a, SDT, &paged_prefix_codes_kernel<QDT, SDT>, kCodeLds, reserved, st);
+  return wide_launch<QDT>("sdpa_decode_paged_shared_q8", a, SDT, &paged_prefix_codes_kernel<QDT, SDT>, kCodeLds, reserved, st);
 }
 
 int shared_fill(const char* what, SharedArgs& a, bool codes, const void* q, const void* k, const void* v, const int32_t* prefix_tables,
@@ -1998,7 +1938,7 @@ int shared_fill(const char* what, SharedArgs& a, bool codes, const void* q, cons
   r.block = s.block;
   r.scale_log2 = (float)((double)scale * 1.4426950408889634);
   uint8_t* at = reinterpret_cast<uint8_t*>(workspace);
-  r.ws_pre = at;
+  r.ws_pre = reinterpret_cast<float*>(at);
   r.ws_pre_ml = reinterpret_cast<float*>(at += s.pre);
   r.ws_own = reinterpret_cast<float*>(at += s.pre_ml);
   r.ws_own_ml = reinterpret_cast<float*>(at += s.own);
