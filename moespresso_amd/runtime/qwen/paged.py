@@ -35,6 +35,7 @@ MAX_REQUESTS = 2048  # requests of one page_step
 MAX_SHARED = 2048    # queries, and prefixes, of one call over shared prefixes
 MAX_SELECTED = 4096      # pages that a query may select
 MAX_TABLE_PAGES = 32768  # pages of a request of which some are selected
+_SELECTION_BYTES = 256 << 20  # scratch of one selection of a layer, about (more than a query's own: a query a call)
 
 
 def _check_page_size(page_size: int):
@@ -903,10 +904,12 @@ class PagedAttention(torch.nn.Module):
         if selected is not None:
             if width > MAX_TABLE_PAGES:
                 raise ValueError(f"pages are selected from tables of at most {MAX_TABLE_PAGES} pages")
-            # (a query and KV head is a request to the attention over its pages; 2048 queries keep the scratch, a word for every
-            # query head and page of its table, within reach)
+            # (a query and KV head is a request to the attention over its pages)
             tiles = -(-selected[0] * tables.page_size // 32) + 1
             most = min(2048, 65535 // kv_heads, 0x3FFFFFFF // (kv_heads * tiles)) if tiles <= 0x2000000 else 0
+            # (of a query: a bound for every query head and page that its table could name, and the selected pages)
+            scratch = 4 * (self.inner.num_attention_heads * (-(-width // 16) * 16) + kv_heads * selected[0])
+            most = min(most, max(1, _SELECTION_BYTES // scratch))
         if most < 1:
             raise ValueError("the tables hold too many tokens together")
         return most
