@@ -196,8 +196,9 @@ __global__ __launch_bounds__(64 * kWaves) void page_bounds_kernel(const int32_t*
         code_lo = (int)fmin(fmax(floor(ldexp(low, -e)), -127.0), 127.0);
         code_hi = (int)fmin(fmax(ceil(ldexp(high, -e)), -127.0), 127.0);
       } else {
-        code_lo = bound_code(floorf(__builtin_amdgcn_ldexpf(low, -e)));
-        code_hi = bound_code(ceilf(__builtin_amdgcn_ldexpf(high, -e)));
+        // (a bfloat16 number 2^-150 of the step becomes zero, but stays on its side of it)
+        code_lo = min(bound_code(floorf(__builtin_amdgcn_ldexpf(low, -e))), low < 0.0f ? -1 : 127);
+        code_hi = max(bound_code(ceilf(__builtin_amdgcn_ldexpf(high, -e))), high > 0.0f ? 1 : -127);
       }
     }
     if (!fresh) {

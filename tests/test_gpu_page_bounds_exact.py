@@ -89,3 +89,15 @@ def test_scales_and_biases_of_any_size(dtype):
         t.copy_(torch.tensor(x))
     biases[:4] = biases[:4].float().clamp(-127, 127).round().to(dtype)
     _check((codes.view(torch.int32).view(torch.uint32), scales, biases), [3, 13])
+
+
+def test_rows_of_16_bits_far_below_the_step():
+    """Negative keys lie below zero, positive ones above it, however small they are beside the largest."""
+    keys = torch.zeros(3, 1, PAGE, 256, dtype=BF16, device="cuda")
+    for p, top in enumerate((2.0 ** 100, 2.0 ** 57, 1.0)):
+        keys[p, 0, :, 0] = top
+        for c, x in enumerate((1e-30, -1e-30, 2.0 ** -126, -2.0 ** -126, 2.0 ** -133, -2.0 ** -133), 1):
+            keys[p, 0, 5, c], keys[p, 0, 9, 10 + c] = x, -x
+            keys[p, 0, :, 20 + c] = x
+    _check(keys, [16])
+    _check(keys, [2, 7, 7])
