@@ -314,6 +314,13 @@ def ptr(t: torch.Tensor | None) -> c_void_p:
     return c_void_p(t.data_ptr())
 
 
+def workspace_args(workspace: torch.Tensor, dev: torch.device) -> tuple[c_void_p, int]:
+    """Address and bytes of a call's scratch, which the kernels write to without asking whose memory it is."""
+    if not torch.is_tensor(workspace) or workspace.device != dev or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous tensor on the device of the operands, {dev}")
+    return ptr(workspace), workspace.numel() * workspace.element_size()
+
+
 def launch(dev: torch.device, entry: str, *args) -> int:
     """One entry point of the library on the current stream of ``dev``, the device of its operands."""
     if dev.index == torch.cuda.current_device():

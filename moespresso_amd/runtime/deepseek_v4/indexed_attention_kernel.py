@@ -112,8 +112,7 @@ def indexed_mixed_attention_decode(q, raw_kv, comp_kv, topk, sinks, *, pos0: int
     rc = _lib.launch(
         dev, "mspr_indexed_mixed_attention_decode",
         _lib.ptr(qc), n_heads, _lib.ptr(rc_), raw_cap, _lib.ptr(cc), n_comp, _lib.ptr(tc), top_k,
-        _lib.ptr(sc), int(pos0), int(window), int(ratio), int(raw_start), _lib.ptr(out), _lib.ptr(ws),
-        ws.numel() * 4)
+        _lib.ptr(sc), int(pos0), int(window), int(ratio), int(raw_start), _lib.ptr(out), *_lib.workspace_args(ws, dev))
     _lib.check(rc, "indexed_mixed_attention_decode")
     return out
 
@@ -182,8 +181,7 @@ def sparse_mla_decode(q, kv, rows, *, scale: float, v_dim: int = 512, window_sta
     rc = _lib.launch(
         dev, "mspr_sparse_mla_decode",
         _lib.ptr(qc), _lib.ptr(kc), _lib.ptr(rc_), _lib.ptr(sinks), _lib.DTYPE_CODE[q.dtype], batch, n_heads,
-        k_dim, 512, n_pool, n_rows, int(row_mul), int(row_add), win_start, window_rows, float(scale), _lib.ptr(out), _lib.ptr(ws),
-        ws.numel() * 4)
+        k_dim, 512, n_pool, n_rows, int(row_mul), int(row_add), win_start, window_rows, float(scale), _lib.ptr(out), *_lib.workspace_args(ws, dev))
     _lib.check(rc, "sparse_mla_decode")
     return out
 
@@ -201,8 +199,7 @@ def _run_prefill(q, raw_kv, comp_kv, topk, sinks, *, batch, n_heads, n_tokens, s
         dev, "mspr_indexed_mixed_attention_prefill",
         _lib.ptr(q), _lib.DTYPE_CODE[q.dtype], batch, n_heads, n_tokens, strides[0], strides[1], strides[2],
         _lib.ptr(raw_kv), raw_cap, _lib.ptr(comp_kv), n_comp, _lib.ptr(topk) if top_k else None, top_k,
-        _lib.ptr(sinks), int(pos0), int(window), int(ratio), int(raw_start), _lib.ptr(out), _lib.ptr(ws),
-        ws.numel() * 4)
+        _lib.ptr(sinks), int(pos0), int(window), int(ratio), int(raw_start), _lib.ptr(out), *_lib.workspace_args(ws, dev))
     _lib.check(rc, "indexed_mixed_attention_prefill")
     return out
 

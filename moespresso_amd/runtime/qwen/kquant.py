@@ -243,7 +243,7 @@ def sdpa_decode_q8(queries, k_wq, k_scales, k_biases, v_wq, v_scales, v_biases, 
         dev, "mspr_sdpa_decode_q8",
         _lib.ptr(q), _lib.DTYPE_CODE[q.dtype], _lib.ptr(kw), _lib.ptr(ks), _lib.ptr(kb), _lib.ptr(vw), _lib.ptr(vs),
         _lib.ptr(vb), _lib.DTYPE_CODE[ks.dtype], B, Hq, Hkv, _HEAD_DIM, N, kv_rows, float(scale), 64, 8, _lib.ptr(out),
-        _lib.ptr(workspace), workspace.numel() * workspace.element_size()), "sdpa_decode_q8")
+        *_lib.workspace_args(workspace, dev)), "sdpa_decode_q8")
     return out
 
 
@@ -288,8 +288,7 @@ def sdpa_decode_q8_0(queries, k_codes, k_scales, v_codes, v_scales, scale, *, wo
     _lib.check(_lib.launch(
         dev, "mspr_sdpa_decode_q8_0",
         _lib.ptr(q), _lib.DTYPE_CODE[q.dtype], _lib.ptr(kc), _lib.ptr(ks), _lib.ptr(vc), _lib.ptr(vs), B, Hq, Hkv,
-        _HEAD_DIM, N, kv_rows, float(scale), _lib.ptr(out), _lib.ptr(workspace),
-        workspace.numel() * workspace.element_size()), "sdpa_decode_q8_0")
+        _HEAD_DIM, N, kv_rows, float(scale), _lib.ptr(out), *_lib.workspace_args(workspace, dev)), "sdpa_decode_q8_0")
     return out
 
 
@@ -345,8 +344,7 @@ def sdpa_fa_prefill_q8(queries, pk_wq, pk_scales, pk_biases, pv_wq, pv_scales, p
         dev, "mspr_sdpa_fa_prefill_q8",
         _lib.ptr(q), _lib.ptr(kw), _lib.ptr(ks), _lib.ptr(kb), _lib.ptr(vw), _lib.ptr(vs), _lib.ptr(vb),
         _lib.DTYPE_CODE[ks.dtype], _lib.ptr(sk), _lib.ptr(sv), _lib.DTYPE_CODE[sk.dtype], B, Hq, Hkv, _HEAD_DIM, L, P,
-        past_rows, float(scale), 64, 8, _lib.ptr(out), _lib.ptr(workspace),
-        workspace.numel() * workspace.element_size()), "sdpa_fa_prefill_q8")
+        past_rows, float(scale), 64, 8, _lib.ptr(out), *_lib.workspace_args(workspace, dev)), "sdpa_fa_prefill_q8")
     return out
 
 
@@ -390,5 +388,5 @@ def flash_prefill(queries, keys, values, scale, *, past_len: int, workspace=None
     _lib.check(_lib.launch(
         dev, "mspr_flash_prefill",
         _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.DTYPE_CODE[q.dtype], B, Hq, Hkv, _HEAD_DIM, L, past_len, rows,
-        float(scale), _lib.ptr(out), _lib.ptr(workspace), workspace.numel() * workspace.element_size()), "flash_prefill")
+        float(scale), _lib.ptr(out), *_lib.workspace_args(workspace, dev)), "flash_prefill")
     return out

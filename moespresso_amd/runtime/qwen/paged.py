@@ -338,8 +338,7 @@ def sdpa_decode_paged(queries, keys, values, tables, lens, scale, *, requests=No
     _lib.check(_lib.launch(
         dev, "mspr_sdpa_decode_paged", _lib.ptr(q), _lib.ptr(keys), _lib.ptr(values), _lib.DTYPE_CODE[q.dtype],
         _lib.ptr(tables), _lib.ptr(lens), _lib.ptr(requests), R, Hq, heads, _HEAD_DIM, n_pages, page_size,
-        int(tables.shape[0]), int(tables.shape[1]), float(scale), _lib.ptr(out), _lib.ptr(workspace),
-        workspace.numel() * workspace.element_size()), "sdpa_decode_paged")
+        int(tables.shape[0]), int(tables.shape[1]), float(scale), _lib.ptr(out), *_lib.workspace_args(workspace, dev)), "sdpa_decode_paged")
     return out
 
 
@@ -375,7 +374,7 @@ def sdpa_decode_paged_q8(queries, k_wq, k_scales, k_biases, v_wq, v_scales, v_bi
         dev, "mspr_sdpa_decode_paged_q8", _lib.ptr(q), _lib.DTYPE_CODE[q.dtype], *(_lib.ptr(t) for t in parts),
         _lib.DTYPE_CODE[k_scales.dtype], _lib.ptr(tables), _lib.ptr(lens), _lib.ptr(requests), R, Hq, heads, _HEAD_DIM,
         n_pages, page_size, int(tables.shape[0]), int(tables.shape[1]), float(scale), 64, 8, _lib.ptr(out),
-        _lib.ptr(workspace), workspace.numel() * workspace.element_size()), "sdpa_decode_paged_q8")
+        *_lib.workspace_args(workspace, dev)), "sdpa_decode_paged_q8")
     return out
 
 
@@ -434,7 +433,7 @@ def sdpa_decode_paged_shared(queries, keys, values, prefix_tables, prefix_lens, 
         dev, "mspr_sdpa_decode_paged_shared", _lib.ptr(q), _lib.ptr(keys), _lib.ptr(values), _lib.DTYPE_CODE[q.dtype],
         _lib.ptr(prefix_tables), _lib.ptr(prefix_lens), _lib.ptr(groups), _lib.ptr(tables), _lib.ptr(lens), _lib.ptr(requests), R,
         Hq, heads, _HEAD_DIM, n_pages, page_size, G, width, int(tables.shape[0]), int(tables.shape[1]), float(scale),
-        _lib.ptr(out), _lib.ptr(workspace), workspace.numel() * workspace.element_size()), "sdpa_decode_paged_shared")
+        _lib.ptr(out), *_lib.workspace_args(workspace, dev)), "sdpa_decode_paged_shared")
     return out
 
 
@@ -472,8 +471,7 @@ def sdpa_decode_paged_shared_q8(queries, k_wq, k_scales, k_biases, v_wq, v_scale
         dev, "mspr_sdpa_decode_paged_shared_q8", _lib.ptr(q), _lib.DTYPE_CODE[q.dtype], *(_lib.ptr(t) for t in parts),
         _lib.DTYPE_CODE[k_scales.dtype], _lib.ptr(prefix_tables), _lib.ptr(prefix_lens), _lib.ptr(groups), _lib.ptr(tables),
         _lib.ptr(lens), _lib.ptr(requests), R, Hq, heads, _HEAD_DIM, n_pages, page_size, G, width, int(tables.shape[0]),
-        int(tables.shape[1]), float(scale), 64, 8, _lib.ptr(out), _lib.ptr(workspace),
-        workspace.numel() * workspace.element_size()), "sdpa_decode_paged_shared_q8")
+        int(tables.shape[1]), float(scale), 64, 8, _lib.ptr(out), *_lib.workspace_args(workspace, dev)), "sdpa_decode_paged_shared_q8")
     return out
 
 
@@ -590,8 +588,7 @@ def select_pages(queries, codes, scales, tables, lens, n_selected, *, page_size:
     _lib.check(_lib.launch(
         dev, "mspr_select_pages", _lib.ptr(q), _lib.DTYPE_CODE[q.dtype], _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(tables),
         _lib.ptr(lens), _lib.ptr(requests), R, Hq, heads, _HEAD_DIM, n_pages, page_size, int(tables.shape[0]), int(tables.shape[1]),
-        n_selected, first, recent, _lib.ptr(out_tables), _lib.ptr(out_lens), _lib.ptr(workspace),
-        workspace.numel() * workspace.element_size()), "select_pages")
+        n_selected, first, recent, _lib.ptr(out_tables), _lib.ptr(out_lens), *_lib.workspace_args(workspace, dev)), "select_pages")
     return out_tables, out_lens
 
 
@@ -626,7 +623,7 @@ def sdpa_decode_paged_sparse(queries, keys, values, codes, scales, tables, lens,
         dev, "mspr_sdpa_decode_paged_sparse", _lib.ptr(q), _lib.ptr(keys), _lib.ptr(values), _lib.DTYPE_CODE[q.dtype],
         _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(tables), _lib.ptr(lens), _lib.ptr(requests), R, Hq, heads, _HEAD_DIM, n_pages,
         page_size, int(tables.shape[0]), int(tables.shape[1]), n_selected, first, recent, float(scale), _lib.ptr(out),
-        _lib.ptr(workspace), workspace.numel() * workspace.element_size()), "sdpa_decode_paged_sparse")
+        *_lib.workspace_args(workspace, dev)), "sdpa_decode_paged_sparse")
     return out
 
 
@@ -664,7 +661,7 @@ def sdpa_decode_paged_sparse_q8(queries, k_wq, k_scales, k_biases, v_wq, v_scale
         dev, "mspr_sdpa_decode_paged_sparse_q8", _lib.ptr(q), _lib.DTYPE_CODE[q.dtype], *(_lib.ptr(t) for t in parts),
         _lib.DTYPE_CODE[k_scales.dtype], _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(tables), _lib.ptr(lens), _lib.ptr(requests), R,
         Hq, heads, _HEAD_DIM, n_pages, page_size, int(tables.shape[0]), int(tables.shape[1]), n_selected, first, recent, float(scale),
-        64, 8, _lib.ptr(out), _lib.ptr(workspace), workspace.numel() * workspace.element_size()), "sdpa_decode_paged_sparse_q8")
+        64, 8, _lib.ptr(out), *_lib.workspace_args(workspace, dev)), "sdpa_decode_paged_sparse_q8")
     return out
 
 
