@@ -5,7 +5,7 @@
 // over the rows of a page and KV head. Steps are powers of two because floor(floor(x / 2^a) / 2^b) = floor(x / 2^(a + b)): bounds made
 // of the old codes and the new rows equal those of all rows, so that an append reads its own rows only.
 //
-// Bound by latency (slots, rows, codes one after the other; 16 tokens 3.5 us, 16088 rows of 8 bits, 4.2 MB, 6.9 us): a key row is read once. A
+// Bound by latency (slots, rows, codes one after the other; 16 tokens 3.6 us, 16088 rows of 8 bits, 4.2 MB, 6.7 us): a key row is read once. A
 // workgroup takes the runs of rows (consecutive slots of one page) that end among `span` rows of the step, of one KV head; its
 // four waves take a run's rows in turn, two 16-bit rows or one 8-bit row a load, and meet in LDS. 8-bit rows are code * scale +
 // bias in 64 bits, rounded down for the lower bounds and up for the upper ones: a value next to a whole number of steps must not be
@@ -213,8 +213,8 @@ __global__ __launch_bounds__(64 * kWaves) void page_bounds_kernel(const int32_t*
 }
 
 // Rows of a step from which on a workgroup looks after sixteen of them (fewer: each after one, which may end a run). In us with the
-// copies of a captured call, sixteen and one: 16 rows 29 and 8.7, 1024 11.7 and 9.9, 3200 10.4 and 12.5, 16088 12.2 and 24.3 (64 rows a
-// workgroup 14.3).
+// copies of a captured call, sixteen and one: 16 requests of one row 29.7 and 8.8, 1024 such 34.0 and 16.3, 8 of 400 8-bit rows 10.4 and 12.7
+// (16-bit ones 11.8 and 12.6), 8 of 2011 12.1 and 24.4 (64 rows a workgroup 14.1).
 constexpr int kManyRows = 2048;
 
 template <int FMT, int SDT>

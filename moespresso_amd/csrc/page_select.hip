@@ -13,7 +13,7 @@
 //
 // Two launches: bounds of 16 pages a wave (516 bytes a page and KV head), and the choice, a workgroup a query and KV head. Bound by
 // latency: requests and lengths, table, bounds one after the other (4.7 us for one request of 256 or of 2048 pages), then the choice's
-// barriers (4.2 us for 256 pages, 7.6 for 2048); 48 ragged requests read 49 MB of bounds in 14.2 us, 3.4 TB/s. The pages of a KV head are then
+// barriers (4.3 us for 256 pages, 7.5 for 2048); 48 ragged requests read 49 MB of bounds in 14.3 us, 3.4 TB/s. The pages of a KV head are then
 // pages of a pool of its own (page * n_kv + head, one head a page), over which paged_decode.hip attends.
 #include "page_bounds.h"
 
@@ -24,8 +24,7 @@ typedef __attribute__((ext_vector_type(4))) int i32x4_t;
 constexpr int kTile = 16;          // pages of a matrix instruction
 constexpr int kScoreWaves = 4;
 // Tiles of all tables, as wide as they are, from which on a wave takes two (fewer: one, on as many more compute units). In us, with one
-// and with two: a request of 256 pages 8.7 and 9.9, 16 of up to 2048 20.0 and 18.5, 64 such 38.7 and 34.8 (with four 34.1, but 11.6
-// for the first).
+// and with two: a request of 256 pages 8.5 and 9.6, 16 of up to 2048 18.3 and 17.1, 64 such 36.6 and 33.1.
 constexpr int kManyTiles = 1024;
 constexpr int kMaxTablePages = 32768;  // a workgroup of 1024 threads has 32 a thread
 constexpr int kMaxSelected = 4096;
@@ -494,8 +493,8 @@ int select_launch(const char* what, const SelectArgs& a, int q_dtype, hipStream_
     else score(std::integral_constant<int, 2>{});
     MSPR_CHECK_LAUNCH(what);
   }
-  // (In us: 256 pages by 256 threads 9.9, by 512 12.1, by 1024 16.0; 16 requests of up to 2048 pages by 512 18.2, by 1024 22.2. Rows of bounds
-  // for 16 heads where there are 8: 256 pages 11.1, 2048 20.9.)
+  // (In us: 256 pages by 256 threads 8.5, by 512 10.1, by 1024 14.8; 16 requests of up to 2048 pages by 512 17.0, by 1024 22.2. Rows of bounds
+  // for 16 heads where there are 8: 256 pages 8.8, 2048 13.3 instead of 11.6.)
   auto choose = [&](auto heads) {
     constexpr int kHeads = decltype(heads)::value;
     if (a.width <= 1024) page_choose_kernel<256, 4, kHeads><<<dim3(rows), dim3(256), 0, st>>>(a);

@@ -19,7 +19,7 @@
 // wave has 32 columns of every second tile, of 8-bit ones (paged_prefix_codes_kernel) sixteen of every tile.
 //
 // What bounds it: few queries the chain of accesses (requests, groups, lengths, table, rows) and two launches; long prefixes of few
-// queries HBM (16 queries over 32768 rows: the tiles' loop reads 6.4 TB/s, 10 of the kernel's 25 us; the others are the plan, the first
+// queries HBM (16 queries over 32768 rows: the tiles' loop reads 6.4 TB/s, 10 of the kernel's 27 us; the others are the plan, the first
 // tiles, and 34 MB of partials); many columns the matrix units (256 queries over 8192 rows: 45 us at the rate of a library's product
 // with two terms a weight, 55 to 65 taken); 8-bit rows a wave's own chain of scales, terms and cross-lane moves (60 us for 33 queries over
 // 20001 rows).
@@ -816,8 +816,8 @@ __device__ __forceinline__ int swizzle(int r) { return ((r & 7) << 1) | ((r >> 3
 
 // One piece: `columns` columns (head rows of q in `column_row`) over tiles [tile0, tile1), two at a time: wave w has columns 32 (w % 4)
 // on and every second tile. (Blocks of 256 columns, which read a prefix half as often, a tile at a time: 2048 query heads a KV head over
-// 8192 rows 108.6 us instead of 109.1, over 20000 rows 160 instead of 164, but 256 over 32768 rows 55.7 instead of 52.0, 200 ragged queries
-// 127 instead of 123. One tile at a time for blocks of 128: 42.4 us instead of 42.0 for 16 queries over 32768 rows.)
+// 8192 rows 0.5 % less time, over 20000 rows 2 % less, but 256 over 32768 rows 7 % more, 200 ragged queries 3 % more. One tile at a time for
+// blocks of 128: 1 % more for 16 queries over 32768 rows.)
 template <int FMT, typename F>
 __device__ __forceinline__ void prefix_piece(const SharedRest& a, const int32_t* table, int len, int tile0, int tile1, int n_kv, int kvh,
                                              int slot, int columns, const int* column_row, F&& find_members, unsigned char* lds,
@@ -1133,7 +1133,7 @@ __device__ __forceinline__ void prefix_workgroup(const int32_t* requests, const 
   units *= n_kv;
   // A range's tiles: so many that there are no more pieces than compute units, as a unit has at most one piece that is not full; where
   // there are too many units for that, half as many again. Of few prefixes the least of 64 lengths that does it, tried one a lane (256
-  // queries over 8192 rows of two KV heads: 256 pieces of 32 tiles, not 224 of 37; the kernel 57 us, not 65).
+  // queries over 8192 rows of two KV heads: 256 pieces of 32 tiles, not 224 of 37; 12 % of the kernel's time).
   int share = max(kMinShare, ceil_div(all, max(kGroups - units, kGroups / 2)));
   if (n_prefixes <= 16 && all < (1 << 21)) {
     const int tried = (max(kMinShare, ceil_div(all, kGroups)) + step - 1) / step * step + step * lane;
@@ -1249,8 +1249,8 @@ __device__ __forceinline__ int turn(int r) { return ((r & 3) << 1) | (r >> 2 & 1
 // Eight weights as two float16 terms each: the first cut off instead of rounded (half the instructions), which the second, a rounded
 // rest of at most 2^-10 of the weight, makes up for.
 __device__ __forceinline__ void cut_terms(const float* x, u32x4_t* t) {
-  // (unknown to the compiler, which else makes two conversions and a difference of one mixed multiplication: 75.6 -> 74.6 us for 33
-  // queries over 20001 rows; of 16-bit rows, whose kernel has fewer registers to spare, 55.5 -> 56.3 for 61 ragged ones)
+  // (unknown to the compiler, which else makes two conversions and a difference of one mixed multiplication: 1.3 % of the call for 33
+  // queries over 20001 rows; of 16-bit rows, whose kernel has fewer registers to spare, it cost 1.4 % for 61 ragged ones)
   float minus = -1.0f;
   asm("" : "+s"(minus));
 #pragma unroll
@@ -1418,7 +1418,7 @@ __device__ __forceinline__ void codes_piece(const SharedRest& a, const int32_t* 
   auto unpack = [&](int i) {
     if (idle == 0) {
       unpack_part(i, wave);
-    } else {  // (waves without columns unpack for the others: 33 queries, of which six waves have 88 heads, 84.0 -> 79.7 us)
+    } else {  // (waves without columns unpack for the others: 33 queries, of which six waves have 88 heads, 5 % of the call)
       for (int part = wave - busy; part >= 0 && part < kWideWaves; part += idle) unpack_part(i, part);
     }
   };
@@ -1730,10 +1730,12 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_shared_merge_kernel(co
 
 // Whether prefixes are a kernel's own: from so many columns times rows that their tables hold (the lengths are on the device) on, and of
 // many columns always. A second kernel costs 9 to 11 us; blocks of 32 columns read a prefix again and again, and own rows of many
-// queries are better dealt out by paged_decode.hip. In us, one launch and two, 8 query heads a KV head: 16-bit rows, 8 queries over 32768
-// rows 35.7 and 37.4, 12 over them 44.3 and 39.5; 32 over 4000 29.3 and 36.1, 128 over 1000 44.1 and 49.5, 256 over 1000 75.0 and 67.5; 20 ragged
-// ones behind 5 prefixes of up to 9001 33.4 and 39.1, 40 such 59.3 and 51.6. 8-bit rows: 24 queries over 20000 rows 60.6 and 61.5, 32 over
-// them 79.7 and 68.9, 48 over 4000 49.5 and 49.7, 96 over 1000 34.6 and 49.3, 200 over 1000 52.6 and 54.4.
+// queries are better dealt out by paged_decode.hip. In us a call of a captured graph, one launch and two, two KV heads of 8 query heads: 16-bit
+// rows, 8 queries over 32768 rows 36.1 and 37.2, 12 over them 44.9 and 40.6; 32 over 4000 29.2 and 38.7, 128 over 1000 43.3 and 49.3, 256 over
+// 1000 65.4 either way; 20 ragged ones behind 5 prefixes of up to 9001 33.4 and 38.9, 40 such 59.3 and 51.0. 8-bit rows: 24 queries over 20000
+// rows 59.7 and 61.9, 32 over them 77.3 and 67.6, 48 over 4000 47.6 and 50.0, 96 over 1000 34.0 and 50.1, 200 over 1000 52.0 and 55.6. The number of
+// KV heads is not in the rule, though with more of them two launches are better earlier: eight of 4 query heads, 16 queries over 4096 rows 32.6
+// and 33.1, 32 over them 44.8 and 42.0, 16 over 16384 rows 73.6 and 52.2, 32 over them 127 and 69, where the rule takes one launch.
 constexpr int kManyColumns = 1024;
 bool wide_prefixes(int batch, int rep, int64_t prefix_cap, bool codes) {
   const int64_t columns = (int64_t)batch * rep;
@@ -1801,7 +1803,7 @@ int reserve_lds(K* kernel, int bytes, bool (&done)[64]) {
 }
 
 // Joins the pieces of `heads` query heads: eight waves a head where they are few and have many pieces, else one. (In us, with eight and with
-// one: 256 heads of 129 pieces 42.0 and 54.8 the call, 1024 of 33 83.0 and 83.9, 2048 133 and 129, 4096 120 and 107.)
+// one: 256 heads of 129 pieces 44.4 and 50.1 the call, 1024 of 33 85.4 and 84.1, 2048 137.5 and 135.3, 4096 116.6 and 109.9.)
 template <int QDT, bool PARTS>
 int merge_launch(const SharedArgs& a, const PagedParts& own, hipStream_t st) {
   const SharedRest& r = a.rest;
