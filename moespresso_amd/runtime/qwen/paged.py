@@ -757,7 +757,8 @@ class PagedKVCache:
         self.scales = torch.ones((n_pages, n_kv_heads), dtype=torch.float32, device=device) if bounds else None
 
     def append(self, q, k, v, q_weight, k_weight, positions, inv_freq, slots, *, eps: float = 1e-6, sections=None):
-        """``qk_norm_rope_append`` into these pages, and ``page_bounds`` where they have bounds."""
+        """``qk_norm_rope_append`` into these pages, and ``page_bounds`` where they have bounds (``slots`` in the order of ``page_step``
+        then: the rows of a page one behind the other)."""
         q = qk_norm_rope_append(q, k, v, q_weight, k_weight, positions, inv_freq, slots, self.keys, self.values, eps=eps,
                                 sections=sections)
         if self.codes is not None:

@@ -101,3 +101,26 @@ def test_rows_of_16_bits_far_below_the_step():
             keys[p, 0, :, 20 + c] = x
     _check(keys, [16])
     _check(keys, [2, 7, 7])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_groups_beside_one_that_is_no_number(dtype):
+    """An infinite or missing bias takes the page's step to its largest; the other groups' codes are their own bounds in such steps."""
+    codes, scales, biases = _triplet(3, 1, dtype, 4)
+    scales[:], biases[:] = 1e-20, 3
+    biases[..., 2] = -127 * 2.0 ** 50
+    scales[..., 2], biases[..., 3] = -1.0, 2.0 ** 50
+    for p, bad in enumerate((float("inf"), float("-inf"), float("nan"))):
+        biases[p, 0, 7, 0] = bad
+        if p < 2:
+            scales[p, 0, 9, 0] = bad
+    side = codes.view(torch.int32).view(torch.uint32), scales, biases
+    got, of = torch.zeros(3, 1, 2, 256, dtype=torch.int8, device="cuda"), torch.zeros(3, 1, device="cuda")
+    paged.page_bounds(i32(range(3 * PAGE)), side, got, of)
+    biases[..., 0] = scales[..., 0] = 0
+    keys = _keys(side)
+    for p in range(3):
+        low, high, e = _bounds(keys[p, 0])
+        assert e == 50 and of[p, 0] == 2.0 ** 50
+        assert got[p, 0, 0, 64:].tolist() == low[64:] and got[p, 0, 1, 64:].tolist() == high[64:], p
+        assert (got[p, 0, 0, :64].long() <= got[p, 0, 1, :64].long()).all()
